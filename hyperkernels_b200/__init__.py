@@ -35,4 +35,13 @@ from .attention import (  # noqa: F401
     FLAG_DETERMINISTIC_DQ,
 )
 from .graph_step import GraphedAttentionStep  # noqa: F401
+from .operators import (  # noqa: F401
+    RotaryPlan,
+    qk_norm_rotary_backward,
+    qk_norm_rotary_forward,
+    rotary_backward,
+    rotary_forward,
+    rotary_plan,
+    shared_prefix_attention,
+)
 from .host_step import HostAttentionStep  # noqa: F401

@@ -135,6 +135,7 @@ def lib() -> C.CDLL:
         L.hk_attn_launch_count.restype = C.c_uint64
         L.hk_attn_round_tf32.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
         L.hk_attn_selftest.argtypes = [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+        L.hk_rotary_plan_fill.argtypes = [C.c_void_p, C.c_int, C.POINTER(C.c_int), C.c_double, C.POINTER(C.c_double), C.c_int]
         _lib = L
     return _lib
 

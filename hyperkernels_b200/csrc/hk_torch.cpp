@@ -1,5 +1,5 @@
-// hk_torch.cpp -- attention_forward / attention_backward over torch tensors, from native code: reads the tensors,
-// allocates the outputs that were not given, fills the argument block and calls the library.
+// hk_torch.cpp -- attention_forward / attention_backward and the operators round them over torch tensors, from native code:
+// reads the tensors, allocates the outputs that were not given, fills the argument block and calls the library.
 //
 // The two calls on a small problem are host-bound: filling the ctypes blocks, allocating through torch's Python API and
 // asking for the current stream took longer than the kernels run.  This module does the same work without Python
@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <Python.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <string.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
@@ -22,12 +23,20 @@ typedef int (*BwdFn)(const hk_attn_bwd_params*, void*);
 typedef int (*ZeroFn)(const hk_attn_bwd_params*, void*);
 typedef size_t (*FwdSizeFn)(const hk_attn_fwd_params*);
 typedef size_t (*BwdSizeFn)(const hk_attn_bwd_params*);
+typedef int (*QkFn)(const hk_qk_params*, void*);
+typedef size_t (*QkSizeFn)(const hk_qk_params*);
+typedef int (*PrefixFn)(const hk_shared_prefix_params*, void*);
+typedef size_t (*PrefixSizeFn)(const hk_shared_prefix_params*);
 struct Library {
     FwdFn forward;
     BwdFn backward;
     ZeroFn zero_dq;
     FwdSizeFn fwd_bytes;
     BwdSizeFn bwd_bytes;
+    QkFn qk[4];
+    QkSizeFn qk_bytes;
+    PrefixFn prefix;
+    PrefixSizeFn prefix_bytes;
 } g_lib = {};
 
 // A tensor argument; None, where it may be left out, gives nullptr.  Anything else is refused: a mask or an output buffer
@@ -255,6 +264,230 @@ static PyObject* zero_body(PyObject* const* a, Py_ssize_t n) {
     return PyLong_FromLong(g_lib.zero_dq(&p, stream));
 }
 
+// ---- the operators round the attention: tensors of three types, on one device, checked against each other -------------------
+namespace {
+
+bool refuse(const char* name, const char* what) {
+    PyErr_Format(PyExc_AssertionError, "%s: %s", name, what);
+    return false;
+}
+int dtype_code(const at::Tensor& t) {
+    return t.scalar_type() == at::kFloat ? HK_F32 : t.scalar_type() == at::kBFloat16 ? HK_BF16 : t.scalar_type() == at::kHalf ? HK_F16 : -1;
+}
+at::ScalarType scalar_of(int code) { return code == HK_BF16 ? at::kBFloat16 : code == HK_F16 ? at::kHalf : at::kFloat; }
+
+constexpr int64_t MOST = 1 << 30;  // rows, heads, batches: what the argument blocks' integers hold
+
+// t as [B, n, T, 64] of `type` (-1: of any of the three) into a block's view; the sizes that are -1 are not looked at
+bool view(const at::Tensor& t, const char* name, int64_t B, int64_t n, int64_t T, int type, hk_view* v) {
+    if (t.dim() != 4 || t.size(3) != 64 || t.stride(3) != 1) return refuse(name, "expected [B,H,T,64] with unit last stride");
+    for (int i = 0; i < 3; ++i)
+        if (t.size(i) > MOST) return refuse(name, "too large");
+    if ((B >= 0 && t.size(0) != B) || (n >= 0 && t.size(1) != n) || (T >= 0 && t.size(2) != T)) return refuse(name, "sizes do not fit the other tensors'");
+    if (dtype_code(t) < 0 || (type >= 0 && dtype_code(t) != type))
+        return refuse(name, type < 0 ? "expected float32, bfloat16 or float16" : "element type does not fit the other tensors'");
+    *v = {t.data_ptr(), t.stride(0), t.stride(2), t.stride(1)};
+    return true;
+}
+
+// All of them on one CUDA device; false with AssertionError set.
+bool one_device(std::initializer_list<const at::Tensor*> all) {
+    const at::Tensor* first = nullptr;
+    for (const at::Tensor* t : all) {
+        if (!t) continue;
+        if (!first) first = t;
+        if (!t->is_cuda()) return refuse("tensors", "expected CUDA tensors");
+        if (t->device() != first->device()) return refuse("tensors", "expected all on one device");
+    }
+    return true;
+}
+
+// Makes the tensors' device the current one and the stream asked for (None: that device's current one) the one that
+// results and workspaces are allocated for: they are written there, whatever becomes of them here.
+struct OnStream {
+    c10::cuda::CUDAGuard device;
+    c10::cuda::OptionalCUDAStreamGuard guard;
+    void* stream;
+    OnStream(PyObject* o, const at::Tensor& t) : device(t.device()) {
+        stream = stream_of(o);
+        if (o == Py_None || PyErr_Occurred()) return;
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        // 0 and cudaStreamLegacy are the default stream, which torch does not know by a handle
+        guard.reset_stream(s == nullptr || s == cudaStreamLegacy ? c10::cuda::getDefaultCUDAStream(t.device().index())
+                                                                 : c10::cuda::getStreamFromExternal(s, t.device().index()));
+    }
+};
+
+PyObject* wrap(std::initializer_list<at::Tensor> r) {
+    PyObject* res = PyTuple_New((Py_ssize_t)r.size());
+    if (!res) return nullptr;
+    Py_ssize_t i = 0;
+    for (const at::Tensor& t : r) {
+        PyObject* o = t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None);
+        PyTuple_SET_ITEM(res, i++, o);
+    }
+    return res;
+}
+
+}  // namespace
+
+// qk(which, Q, K, dQ, dK, w_q, w_k, positions, plan, eps, out_dtype, out_q, out_k, stream)
+//   which: 0 rotation, 1 its backward, 2 norm and rotation, 3 its backward; plan: the bytes of an hk_rotary_plan;
+//   out_dtype: of the results of 0, 1, 2 (hk_dtype, -1: the argument's)
+// -> the results, with 3 followed by the weights' gradients, or the negative status of the call
+static PyObject* qk_body(PyObject* const* a, Py_ssize_t n) {
+    if (n != 14) {
+        PyErr_SetString(PyExc_TypeError, "qk: 14 arguments");
+        return nullptr;
+    }
+    const int which = (int)PyLong_AsLong(a[0]);
+    if (PyErr_Occurred()) return nullptr;
+    if (which < 0 || which > 3) {
+        PyErr_SetString(PyExc_ValueError, "qk: which");
+        return nullptr;
+    }
+    const bool norm = which >= 2, back = which & 1, grads = back, rows = which != 1;
+    const at::Tensor *x[2], *g[2], *w[2], *pos, *out[2];
+    if (!tensors({{a[1], "Q", !rows, &x[0]}, {a[2], "K", true, &x[1]}, {a[3], "dQ", !grads, &g[0]}, {a[4], "dK", true, &g[1]},
+                  {a[5], "w_q", true, &w[0]}, {a[6], "w_k", true, &w[1]}, {a[7], "positions", false, &pos},
+                  {a[11], "out_q", true, &out[0]}, {a[12], "out_k", true, &out[1]}}))
+        return nullptr;
+    hk_qk_params p = {};
+    if (!PyBytes_Check(a[8]) || PyBytes_GET_SIZE(a[8]) != (Py_ssize_t)sizeof(p.plan)) {
+        PyErr_SetString(PyExc_TypeError, "plan: expected the bytes of a plan");
+        return nullptr;
+    }
+    memcpy(&p.plan, PyBytes_AS_STRING(a[8]), sizeof(p.plan));
+    p.eps = (float)PyFloat_AsDouble(a[9]);
+    int out_type = (int)PyLong_AsLong(a[10]);
+    if (PyErr_Occurred()) return nullptr;
+
+    const at::Tensor** src = rows ? x : g;  // what decides sizes
+    const char* names[2][2] = {{"Q", "K"}, {"dQ", "dK"}};
+    if (rows && grads && !x[1] != !g[1]) return refuse("dK", "expected together with K"), nullptr;
+    hk_view none = {}, *src_view[2] = {rows ? &p.q : &p.dq_out, rows ? &p.k : &p.dk_out};
+    if (!view(*src[0], names[!rows][0], -1, -1, -1, -1, src_view[0])) return nullptr;
+    const int64_t B = src[0]->size(0), H = src[0]->size(1), T = src[0]->size(2), Hk = src[1] ? src[1]->size(1) : 0;
+    const int type = dtype_code(*src[0]);
+    if (src[1] && !view(*src[1], names[!rows][1], B, -1, T, type, src_view[1])) return nullptr;
+    p.B = (int)B; p.nh = (int)H; p.nh_k = (int)Hk; p.T = T;
+    if (which == 3) {  // the gradients' type stands for out_dtype, the results are of the rows' type
+        if (!view(*g[0], "dQ", B, H, T, -1, &p.dq_out)) return nullptr;
+        p.out_dtype = dtype_code(*g[0]);
+        if (g[1] && !view(*g[1], "dK", B, Hk, T, p.out_dtype, &p.dk_out)) return nullptr;
+        p.dtype = type;
+        out_type = type;
+    } else {
+        if (out_type < 0) out_type = out[0] ? dtype_code(*out[0]) : type;
+        p.dtype = back ? out_type : type;
+        p.out_dtype = back ? type : out_type;
+    }
+    for (int k = 0; k < 2; ++k) {
+        const char* name = k ? "w_k" : "w_q";
+        if (!norm || !w[k]) continue;
+        if (w[k]->dim() != 1 || w[k]->size(0) != 64 || w[k]->stride(0) != 1) return refuse(name, "expected [64], contiguous"), nullptr;
+        if (dtype_code(*w[k]) < 0 || (k && w[0] && dtype_code(*w[0]) != dtype_code(*w[k])))
+            return refuse(name, "element type does not fit the other tensors'"), nullptr;
+        p.weight_dtype = dtype_code(*w[k]);
+    }
+    if (pos->dim() != 3 || pos->size(0) != p.plan.n_axes || pos->size(1) != B || pos->size(2) != T)
+        return refuse("positions", "expected [axes,B,T]"), nullptr;
+    if (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong) return refuse("positions", "expected int32 or int64"), nullptr;
+    hk_view* dst_view[2] = {back ? &p.dq : &p.q_out, back ? &p.dk : &p.k_out};
+    for (int k = 0; k < 2; ++k) {
+        if (!out[k]) continue;
+        if (!src[k]) return refuse("out_k", "there is no K"), nullptr;
+        if (!view(*out[k], k ? "out_k" : "out_q", B, k ? Hk : H, T, out_type, &none)) return nullptr;
+    }
+    if (!one_device({src[0], src[1], x[0], x[1], g[0], g[1], norm ? w[0] : nullptr, norm ? w[1] : nullptr, pos, out[0], out[1]})) return nullptr;
+    OnStream on(a[13], *src[0]);
+    if (PyErr_Occurred()) return nullptr;
+
+    const auto opt = src[0]->options();
+    at::Tensor r[2], dw[2], ws;
+    for (int k = 0; k < 2; ++k) {
+        if (!src[k]) continue;
+        r[k] = out[k] ? *out[k] : at::empty({B, k ? Hk : H, T, 64}, opt.dtype(scalar_of(out_type)));
+        *dst_view[k] = {r[k].data_ptr(), r[k].stride(0), r[k].stride(2), r[k].stride(1)};
+    }
+    p.q_weight = norm && w[0] ? w[0]->data_ptr() : nullptr;
+    p.k_weight = norm && w[1] ? w[1]->data_ptr() : nullptr;
+    if (which == 3) {
+        for (int k = 0; k < 2; ++k)
+            if (w[k] && src[k]) dw[k] = at::empty({64}, opt.dtype(at::kFloat));
+        p.dq_weight = dw[0].defined() ? data(dw[0]) : nullptr;
+        p.dk_weight = dw[1].defined() ? data(dw[1]) : nullptr;
+        p.workspace_bytes = g_lib.qk_bytes(&p);
+        ws = at::empty({(int64_t)p.workspace_bytes}, opt.dtype(at::kByte));
+        p.workspace = ws.data_ptr();
+    }
+    p.positions = pos->data_ptr();
+    p.pos_bits = pos->scalar_type() == at::kLong ? 64 : 32;
+    p.pos_strideA = pos->stride(0); p.pos_strideB = pos->stride(1); p.pos_strideT = pos->stride(2);
+    int rc;
+    {
+        NoGil nogil;
+        rc = g_lib.qk[which](&p, on.stream);
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    return which == 3 ? wrap({r[0], r[1], dw[0], dw[1]}) : wrap({r[0], r[1]});
+}
+
+// prefix(Q, K_prefix, V_prefix, K, V, lengths, scale, causal, workspace, out, lse, stream) -> (O, LSE), or the negative status
+static PyObject* prefix_body(PyObject* const* a, Py_ssize_t n) {
+    if (n != 12) {
+        PyErr_SetString(PyExc_TypeError, "prefix: 12 arguments");
+        return nullptr;
+    }
+    const at::Tensor *Q, *kv[4], *lens, *ws, *out, *lse;
+    if (!tensors({{a[0], "Q", false, &Q}, {a[1], "K_prefix", false, &kv[0]}, {a[2], "V_prefix", false, &kv[1]}, {a[3], "K", false, &kv[2]},
+                  {a[4], "V", false, &kv[3]}, {a[5], "lengths", true, &lens}, {a[8], "workspace", true, &ws}, {a[9], "out", true, &out}, {a[10], "lse", true, &lse}}))
+        return nullptr;
+    hk_shared_prefix_params p = {};
+    if (!view(*Q, "Q", -1, -1, -1, -1, &p.Q)) return nullptr;
+    const int64_t B = Q->size(0), H = Q->size(1), T = Q->size(2);
+    p.dtype = dtype_code(*Q);
+    at::Tensor whole[2];  // [heads, length, 64] as a batch of one
+    for (int k = 0; k < 2; ++k) whole[k] = kv[k]->dim() == 3 ? kv[k]->unsqueeze(0) : *kv[k];
+    if (!view(*kv[2], "K", B, -1, -1, p.dtype, &p.K)) return nullptr;
+    const int64_t Hk = kv[2]->size(1), S = kv[2]->size(2);
+    if (!view(*kv[3], "V", B, Hk, S, p.dtype, &p.V) || !view(whole[0], "K_prefix", 1, Hk, -1, p.dtype, &p.Kp) ||
+        !view(whole[1], "V_prefix", 1, Hk, whole[0].size(2), p.dtype, &p.Vp))
+        return nullptr;
+    if (lens && (lens->dim() != 1 || lens->size(0) != B || (B > 1 && lens->stride(0) != 1) || lens->scalar_type() != at::kInt))
+        return refuse("lengths", "expected [B] of int32, contiguous"), nullptr;
+    if (out && !view(*out, "out", B, H, T, p.dtype, &p.O)) return nullptr;
+    if (lse && (lse->dim() != 3 || lse->size(0) != B || lse->size(1) != H || lse->size(2) != T || (T > 1 && lse->stride(2) != 1) || lse->scalar_type() != at::kFloat))
+        return refuse("lse", "expected [B,H,T] of float32 with unit last stride"), nullptr;
+    p.scale = (float)PyFloat_AsDouble(a[6]);
+    p.is_causal = PyObject_IsTrue(a[7]) != 0;
+    if (PyErr_Occurred()) return nullptr;
+    p.B = (int)B; p.nh = (int)H; p.nh_kv = (int)Hk; p.T = T; p.prefix_len = whole[0].size(2); p.kv_len = S;
+    p.lengths = lens ? static_cast<const int32_t*>(lens->data_ptr()) : nullptr;
+    if (!one_device({Q, kv[0], kv[1], kv[2], kv[3], lens, ws, out, lse})) return nullptr;
+    OnStream on(a[11], *Q);
+    if (PyErr_Occurred()) return nullptr;
+    const auto opt = Q->options();
+    at::Tensor O = out ? *out : at::empty({B, H, T, 64}, opt), L = lse ? *lse : at::empty({B, H, T}, opt.dtype(at::kFloat)), own;
+    p.O = {O.data_ptr(), O.stride(0), O.stride(2), O.stride(1)};
+    p.LSE = data(L); p.lse_strideB = L.stride(0); p.lse_strideH = L.stride(1);
+    const size_t need = g_lib.prefix_bytes(&p);
+    if (!ws && need > 0) {
+        own = at::empty({(int64_t)need + 256}, opt.dtype(at::kByte));
+        ws = &own;
+    }
+    if (ws && !given_workspace(ws, need, &p.workspace, &p.workspace_bytes)) return nullptr;
+    int rc;
+    {
+        NoGil nogil;
+        rc = g_lib.prefix(&p, on.stream);
+    }
+    return rc != 0 ? PyLong_FromLong(rc) : wrap({O, L});
+}
+
+static PyObject* qk(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return qk_body(a, n); }); }
+static PyObject* prefix(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return prefix_body(a, n); }); }
+
 static PyObject* forward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return forward_body(a, n); }); }
 static PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return backward_body(a, n); }); }
 static PyObject* zero(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return zero_body(a, n); }); }
@@ -268,7 +501,13 @@ static PyObject* bind(PyObject*, PyObject* h) {
     g_lib.zero_dq = reinterpret_cast<ZeroFn>(dlsym(so, "hk_attn_zero_dq"));
     g_lib.fwd_bytes = reinterpret_cast<FwdSizeFn>(dlsym(so, "hk_attn_fwd_workspace_bytes"));
     g_lib.bwd_bytes = reinterpret_cast<BwdSizeFn>(dlsym(so, "hk_attn_bwd_workspace_bytes"));
-    if (!g_lib.forward || !g_lib.backward || !g_lib.zero_dq || !g_lib.fwd_bytes || !g_lib.bwd_bytes) {
+    const char* qk_names[4] = {"hk_rotary_forward", "hk_rotary_backward", "hk_qk_norm_rotary_forward", "hk_qk_norm_rotary_backward"};
+    bool all = true;
+    for (int i = 0; i < 4; ++i) all = (g_lib.qk[i] = reinterpret_cast<QkFn>(dlsym(so, qk_names[i]))) && all;
+    g_lib.qk_bytes = reinterpret_cast<QkSizeFn>(dlsym(so, "hk_qk_norm_rotary_workspace_bytes"));
+    g_lib.prefix = reinterpret_cast<PrefixFn>(dlsym(so, "hk_shared_prefix_attention"));
+    g_lib.prefix_bytes = reinterpret_cast<PrefixSizeFn>(dlsym(so, "hk_shared_prefix_workspace_bytes"));
+    if (!all || !g_lib.qk_bytes || !g_lib.prefix || !g_lib.prefix_bytes || !g_lib.forward || !g_lib.backward || !g_lib.zero_dq || !g_lib.fwd_bytes || !g_lib.bwd_bytes) {
         PyErr_SetString(PyExc_ImportError, "libhk_attention.so lacks an entry point");
         return nullptr;
     }
@@ -279,6 +518,8 @@ static PyMethodDef methods[] = {
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(forward)), METH_FASTCALL, nullptr},
     {"backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(backward)), METH_FASTCALL, nullptr},
     {"zero", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(zero)), METH_FASTCALL, nullptr},
+    {"qk", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk)), METH_FASTCALL, nullptr},
+    {"prefix", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefix)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hk_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

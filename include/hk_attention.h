@@ -284,6 +284,90 @@ int hk_attn_kernel_timing_read(int kind, double* total_ms, int* launches);
  * hyperkernels_b200/csrc/umma_selftest.cu. */
 int hk_attn_selftest(int which, const float* A, const float* B, float* out, void* stream);
 
+/* ---- operators round the attention -------------------------------------------
+ * No counterpart in the reference.  They read and write fp32, bf16 or fp16; everything in between is fp32. */
+typedef enum hk_dtype { HK_F32 = 0, HK_BF16 = 1, HK_F16 = 2 } hk_dtype;
+
+/* A [B, heads, T, 64] tensor: pointer and element strides, last stride 1.  The pointer and the bytes of every stride
+ * are multiples of 16; the stride of a dimension of one is not used. */
+typedef struct hk_view {
+    void* ptr;
+    int64_t strideB, strideM, strideH;
+} hk_view;
+
+/* Rotary positions with several axes.  The 64 elements of a row are 32 pairs (p, p + 32), or (2 p, 2 p + 1) with
+ * `interleaved`; pair p turns by positions[axis[p], b, t] * turn[p] / 2^64 of a full turn.  An integer position times an
+ * integer fraction of a turn, modulo one turn, has no error however far the position is; turn[p] itself is rounded to
+ * 2^-64 of a turn.  A pair of axis HK_ROTARY_STILL is left as it is. */
+#define HK_ROTARY_STILL 255
+typedef struct hk_rotary_plan {
+    uint64_t turn[32];
+    uint8_t axis[32];
+    int32_t n_axes;
+    int32_t interleaved;
+} hk_rotary_plan;
+
+/* Fills a plan: the first sections[0] pairs turn with axis 0, the next sections[1] with axis 1, and so on; pairs behind
+ * the last section are left as they are.  `frequency` holds radians per position for each turning pair, or is NULL for
+ * base^(-p / 32), p counted over all axes. */
+int hk_rotary_plan_fill(hk_rotary_plan* plan, int n_axes, const int* sections, double base, const double* frequency,
+                        int interleaved);
+
+typedef struct hk_qk_params {
+    hk_view q, k;           /* what the projection gives, `dtype`; the rotary backward does not read it */
+    hk_view q_out, k_out;   /* forward, written: `out_dtype` */
+    hk_view dq_out, dk_out; /* backward, read: gradients of q_out, k_out, `out_dtype` */
+    hk_view dq, dk;         /* backward, written: gradients of q, k, `dtype` */
+    const void* q_weight;   /* norm: [64] of weight_dtype, or NULL for ones */
+    const void* k_weight;
+    float* dq_weight; /* norm, backward, written: [64], or NULL if not wanted */
+    float* dk_weight;
+    const void* positions; /* [n_axes, B, T] with the element strides below (0 broadcasts), 32- or 64-bit integers */
+    int64_t pos_strideA, pos_strideB, pos_strideT;
+    int B, nh, nh_k; /* nh_k = 0: no keys */
+    int pos_bits;    /* 32 or 64 */
+    int64_t T;
+    int dtype, out_dtype, weight_dtype; /* hk_dtype; the norm's out_dtype is HK_F32 or dtype, and so is weight_dtype;
+                                         * 16-bit types are not mixed with each other */
+    float eps;
+    hk_rotary_plan plan;
+    void* workspace; /* norm, backward: hk_qk_norm_rotary_workspace_bytes, 16-byte aligned */
+    size_t workspace_bytes;
+} hk_qk_params;
+
+/* q_out = the rotation of q, k_out that of k.  The result may be the argument itself (same pointer, strides, type). */
+int hk_rotary_forward(const hk_qk_params* p, void* stream);
+/* dq = the rotation of dq_out by the opposite angles, dk that of dk_out. */
+int hk_rotary_backward(const hk_qk_params* p, void* stream);
+/* The same behind an RMS norm of every row: x -> x / sqrt(mean(x^2) + eps) * weight. */
+int hk_qk_norm_rotary_forward(const hk_qk_params* p, void* stream);
+/* Gradients of q, k and of the weights (sums over all rows, in an order that depends on sizes and device alone: the same
+ * call gives the same bits). */
+int hk_qk_norm_rotary_backward(const hk_qk_params* p, void* stream);
+size_t hk_qk_norm_rotary_workspace_bytes(const hk_qk_params* p);
+
+/* Attention of a batch whose requests share a prefix.  Row (b, i) of a head sees every prefix key and the keys
+ * j < lengths[b] of its request, with is_causal those with j <= lengths[b] - T + i.  Heads in groups of nh / nh_kv
+ * share a head of keys and values.  A row that sees nothing gives O = 0, LSE = -inf. */
+typedef struct hk_shared_prefix_params {
+    hk_view Q;        /* [B, nh, T, 64], `dtype` */
+    hk_view Kp, Vp;   /* [1, nh_kv, prefix_len, 64], once for the whole batch; strideB is not used */
+    hk_view K, V;     /* [B, nh_kv, kv_len, 64] */
+    hk_view O;        /* [B, nh, T, 64], `dtype`, written */
+    float* LSE;       /* [B, nh, T], written */
+    int64_t lse_strideB, lse_strideH;
+    const int32_t* lengths; /* device, [B]: keys each request has, taken into [0, kv_len]; NULL: kv_len.  Rows of K and V
+                             * behind them are not part of any result, whatever they hold. */
+    int B, nh, nh_kv, dtype;
+    int64_t T, prefix_len, kv_len; /* prefix_len or kv_len may be 0 */
+    float scale;
+    bool is_causal;
+    void* workspace; /* hk_shared_prefix_workspace_bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} hk_shared_prefix_params;
+int hk_shared_prefix_attention(const hk_shared_prefix_params* p, void* stream);
+size_t hk_shared_prefix_workspace_bytes(const hk_shared_prefix_params* p);
+
 const char* hk_status_string(int status);
 
 #ifdef __cplusplus

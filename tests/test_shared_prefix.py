@@ -1,0 +1,312 @@
+"""Attention of a batch that shares a prefix, against the definition in 64 bits, request by request.
+
+Error bounds (u = 2^-24).  A score in fp32 is a sum of 64 products: 80 u of the sum of the products' sizes, whatever the order;
+so its exponential is off by that much of itself (D), and O, a weighted mean, by 2 D of the mean of |v| plus the roundings of
+sums over the keys, taken by blocks of at most 128 keys and 64 blocks in a row: 200 u.  The exponential's own error (2 u) and the
+argument's rounding (u times its size, below 64 in log2 units here) are 70 u.  Sixteen-bit types round each weight and the result
+by half a step; their products are exact in fp32."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import hyperkernels_b200 as hk
+
+U = 2.0 ** -24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+SCALE = 0.125
+
+
+def make(seed, B, H, Hk, T, P, S, dtype, layout="bhtd", lengths=None, junk=math.nan, sigma=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = TYPES[dtype]
+
+    def rand(*shape):
+        return (torch.randn(shape, generator=g, device="cuda") * sigma).to(t)
+
+    if layout == "bthd":
+        q = rand(B, T, H, 64).transpose(1, 2)
+        kp, vp = (rand(P, Hk, 64).transpose(0, 1) for _ in range(2))
+        k, v = (rand(B, S, Hk, 64).transpose(1, 2) for _ in range(2))
+    elif layout == "wide":  # rows of a fused cache: keys and values side by side, with room between heads
+        q = rand(B, H, T, 192)[..., 64:128]
+        kp, vp = (lambda x: (x[..., :64], x[..., 64:]))(rand(Hk, P + 3, 128)[:, :P])
+        k, v = (lambda x: (x[..., :64], x[..., 64:]))(rand(B, Hk, S + 5, 128)[:, :, :S])
+    else:
+        q = rand(B, H, T, 64)
+        kp, vp = (rand(Hk, P, 64) for _ in range(2))
+        k, v = (rand(B, Hk, S, 64) for _ in range(2))
+    if lengths is None:
+        lengths = [(7 * b + 3) % (S + 1) for b in range(B)]
+    for b, n in enumerate(lengths):  # what is behind a request's last key must not matter
+        k[b, :, max(0, n):], v[b, :, max(0, n):] = junk, junk
+    return q, kp, vp, k, v, torch.tensor(lengths, device="cuda", dtype=torch.int32)
+
+
+def definition(q, kp, vp, k, v, lens, causal, scale=SCALE):
+    """O, LSE, and for the bounds the mean of |v| under the softmax and the largest sum of products' sizes of a row"""
+    B, H, T, _ = q.shape
+    G, P = H // k.shape[1], kp.shape[-2]
+    O, LSE, mean, size = (torch.zeros((B, H, T, n), device="cuda", dtype=torch.float64) for n in (64, 1, 64, 1))
+    for b in range(B):
+        n = min(max(int(lens[b]), 0), k.shape[2])
+        kk = torch.cat([kp, k[b, :, :n]], 1).double().repeat_interleave(G, 0)
+        vv = torch.cat([vp, v[b, :, :n]], 1).double().repeat_interleave(G, 0)
+        x = q[b].double() @ kk.transpose(1, 2) * scale
+        if causal:
+            own = torch.arange(P + n, device="cuda") - P
+            x = x.masked_fill((own >= 0) & (own > n - T + torch.arange(T, device="cuda")[:, None]), -math.inf)
+        if P + n == 0:
+            LSE[b] = -math.inf
+            continue
+        w = torch.nan_to_num(torch.softmax(x, -1))  # rows that see nothing
+        O[b], mean[b], LSE[b, ..., 0] = w @ vv, w @ vv.abs(), torch.logsumexp(x, -1)
+        size[b] = (q[b].double().abs() @ kk.abs().transpose(1, 2) * abs(scale)).amax(-1, keepdim=True)
+    return O, LSE[..., 0], mean, size[..., 0]
+
+
+def check(got, want, dtype, what=""):
+    (o, lse), (O, LSE, mean, size) = got, want
+    step = torch.finfo(TYPES[dtype]).eps / 2 if dtype != "f32" else 0.0
+    d = (80 * size + 70) * U
+    bound = (2 * d[..., None] + 200 * U + step) * mean + step * O.abs() + (2.0 ** -25 if dtype == "f16" else 1e-30)
+    off = (o.double() - O).abs()
+    assert o.dtype == TYPES[dtype] and lse.dtype == torch.float32
+    assert bool((off <= bound).all()), (what, float((off - bound).max()), float(off.max()))
+    seen = LSE > -math.inf
+    assert torch.equal(lse > -math.inf, seen), what
+    assert bool((o[~seen] == 0).all()), what
+    assert bool(((lse.double() - LSE).abs()[seen] <= (d + 200 * U + 4 * U * LSE.abs())[seen]).all()), what
+    if dtype == "f32" and bool(seen.any()):  # fp32 throughout: roundings that do not add up all one way
+        assert float((o.double() - O).norm() / O.norm()) <= 1e-5, what
+
+
+# (B, H, Hk, T, P, S): one token to long, odd sizes, groups, empty parts, tiles' borders
+SIZES = [
+    (1, 1, 1, 1, 1, 1), (1, 1, 1, 1, 0, 5), (2, 2, 1, 1, 7, 0), (4, 12, 12, 1, 333, 64), (3, 6, 2, 1, 130, 257), (16, 4, 4, 1, 1000, 65),
+    (64, 8, 2, 1, 515, 100), (5, 3, 3, 2, 128, 128), (2, 8, 1, 3, 64, 33), (9, 8, 2, 5, 129, 300), (3, 4, 4, 17, 127, 63), (2, 4, 2, 77, 500, 333),
+    (2, 3, 3, 128, 256, 128), (1, 2, 1, 200, 100, 450), (2, 2, 2, 300, 0, 300), (70, 1, 1, 1, 40, 9), (1, 16, 1, 9, 2000, 0), (1, 1, 1, 130, 5, 131),
+    (33, 5, 5, 4, 65, 20), (1, 32, 8, 1, 5000, 700)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,T,P,S", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("layout", ["bhtd", "bthd", "wide"])
+def test_against_the_definition(B, H, Hk, T, P, S, dtype, causal, layout):
+    x = make(B + P, B, H, Hk, T, P, S, dtype, layout)
+    got = hk.shared_prefix_attention(*x, SCALE, causal)
+    check(got, definition(*x, causal), dtype)
+    assert hk.last_device_status() == 0
+    again = hk.shared_prefix_attention(*x, SCALE, causal)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1, 3, 40, 150])
+@pytest.mark.parametrize("P", [0, 70])
+def test_lengths_at_borders_and_outside(dtype, T, P):
+    """Empty, one, tiles' ends and the rows next to them, full, and lengths that the cache does not have (taken into it)."""
+    lengths = [0, 1, 2, 63, 64, 65, 127, 128, 129, 191, 192, 193, 255, 256, 300, -4, 1000000]
+    x = make(T, len(lengths), 4, 2, T, P, 300, dtype, lengths=lengths)
+    for junk in (math.nan, math.inf, 60000.0):
+        for b, n in enumerate(lengths):
+            x[3][b, :, max(0, n):], x[4][b, :, max(0, n):] = junk, junk
+        for causal in (True, False):
+            check(hk.shared_prefix_attention(*x, SCALE, causal), definition(*x, causal), dtype, (junk, causal))
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1, 6, 130])
+def test_no_lengths_means_all(dtype, T):
+    x = list(make(1, 3, 4, 4, T, 90, 200, dtype, lengths=[200] * 3))
+    full = hk.shared_prefix_attention(*x, SCALE)
+    x[5] = None
+    none = hk.shared_prefix_attention(*x, SCALE)
+    assert torch.equal(full[0], none[0]) and torch.equal(full[1], none[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1, 20, 140])
+def test_large_scores_and_other_scales(dtype, T):
+    """Scores of +-200: one key takes almost everything, the maximum moves late, masked keys would be the largest."""
+    x = make(3, 3, 4, 2, T, 200, 150, dtype, lengths=[100, 150, 0], sigma=1.0)
+    x[1][:, 150:] *= 3.0
+    x[3][:, :, :100] *= 3.0
+    for scale in (1.0, -0.7, 1e-3):
+        O, LSE, mean, size = definition(*x, True, scale)
+        o, lse = hk.shared_prefix_attention(*x, scale, True)
+        d = (80 * size + 3 * size.clamp(min=1) * 1.45 + 70) * U  # the exponent's argument in log2 units is as large as the scores
+        step = torch.finfo(TYPES[dtype]).eps / 2 if dtype != "f32" else 0.0
+        bound = (2 * d[..., None] + 200 * U + step) * mean + step * O.abs() + (2.0 ** -25 if dtype == "f16" else 1e-30)
+        assert bool(((o.double() - O).abs() <= bound).all()), scale
+        assert bool(((lse.double() - LSE).abs() <= d + 200 * U + 4 * U * LSE.abs()).all()), scale
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 5, 150])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_given_tensors_graphs_and_streams(dtype, T):
+    x = make(5, 4, 8, 2, T, 700, 260, dtype, lengths=[260, 200, 151, 160])
+    want = hk.shared_prefix_attention(*x, SCALE)
+    room = torch.full((4, T + 2, 9, 64), 7.0, device="cuda", dtype=TYPES[dtype])
+    out = room[:, 1:T + 1, :8].transpose(1, 2)
+    lse_room = torch.full((4, 8, T + 3), 7.0, device="cuda")
+    got = hk.shared_prefix_attention(*x, SCALE, out=out, lse=lse_room[..., :T])
+    assert got[0].data_ptr() == out.data_ptr() and torch.equal(out, want[0]) and torch.equal(lse_room[..., :T], want[1])
+    room[:, 1:T + 1, :8] = 7.0
+    assert bool((room == 7.0).all()) and bool((lse_room[..., T:] == 7.0).all())
+    # two graphs, each with a workspace of its own, replayed side by side; lengths are read at replay
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            r = hk.shared_prefix_attention(*x, SCALE)
+        graphs.append((g, r, torch.cuda.Stream()))
+    for lens in ([260, 200, 151, 160], [150, 260, 0, 1]):
+        x[5].copy_(torch.tensor(lens, dtype=torch.int32))
+        for b, n in enumerate(lens):
+            x[3][b, :, :n] = torch.nan_to_num(x[3][b, :, :n], 0.25)
+            x[4][b, :, :n] = torch.nan_to_num(x[4][b, :, :n], 0.5)
+        want = hk.shared_prefix_attention(*x, SCALE)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, _, s in graphs:
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for _, r, _ in graphs:
+            assert torch.equal(r[0], want[0]) and torch.equal(r[1], want[1])
+        check(want, definition(*x, True), dtype)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+    r = hk.shared_prefix_attention(*x, SCALE, stream=side)  # its workspace is given back before the kernels have begun
+    others = [torch.full((1 << 22,), 3.0, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(r[0], want[0]) and torch.equal(r[1], want[1]) and all(bool((t == 3.0).all()) for t in others)
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A cache whose last request starts more than 2^32 elements behind the first."""
+    B, Hk, S = 3, 2, 1 << 24
+    cache = torch.empty((B, Hk, S, 64), device="cuda", dtype=torch.bfloat16)  # 12.9 GB
+    x = list(make(6, B, 4, Hk, 1, 100, 500, "bf16"))
+    want = hk.shared_prefix_attention(*x, SCALE)
+    cache[:, :, :500] = x[3]
+    values = x[4]
+    x[3] = cache
+    big = torch.empty((B, Hk, S, 64), device="cuda", dtype=torch.bfloat16)
+    big[:, :, :500] = values
+    x[4] = big
+    got = hk.shared_prefix_attention(*x, SCALE)
+    # the work may be cut otherwise: the sums' order differs, a result by a step of its type
+    assert torch.allclose(got[0].float(), want[0].float(), rtol=2.0 ** -7, atol=2.0 ** -9) and torch.allclose(got[1], want[1], atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_serving_loop(dtype):
+    """A prompt's common part goes into the prefix once; then requests of different lengths take a first chunk and decode: norm and
+    rotation, append, attention.  Every step against the whole computed again in 64 bits."""
+    t, B, H, Hk, P, S = TYPES[dtype], 5, 6, 3, 150, 40
+    g = torch.Generator(device="cuda").manual_seed(9)
+    w = [(1 + 0.2 * torch.randn(64, generator=g, device="cuda")) for _ in range(2)]
+
+    def project(batch, T):
+        return [torch.randn((batch, n, T, 64), generator=g, device="cuda").to(t) for n in (H, Hk, Hk)]
+
+    _, k, v = project(1, P)
+    pos = torch.arange(P, device="cuda", dtype=torch.int32)[None, None]
+    kp, vp = hk.qk_norm_rotary_forward(k, None, w[1], None, pos, (32,))[0][0], v[0]
+    K, V = (torch.full((B, Hk, S, 64), math.nan, device="cuda", dtype=t) for _ in range(2))
+    lens = torch.zeros(B, device="cuda", dtype=torch.int32)
+    for step, new in enumerate([7, 1, 1, 1, 3, 1]):
+        q, k, v = project(B, new)
+        start = lens.clone()
+        if step == 0:
+            start += torch.arange(B, device="cuda", dtype=torch.int32)  # requests that are some tokens in already
+            K[:, :, :B], V[:, :, :B] = 0.5, -0.25
+        lens = start + new
+        pos = (P + start[:, None] + torch.arange(new, device="cuda"))[None].to(torch.int32)
+        q, k = hk.qk_norm_rotary_forward(q, k, *w, pos, (32,))
+        rows = (start[:, None] + torch.arange(new, device="cuda"))[:, None, :, None].expand(B, Hk, new, 64)
+        K.scatter_(2, rows, k)
+        V.scatter_(2, rows, v)
+        got = hk.shared_prefix_attention(q, kp, vp, K, V, lens, SCALE)
+        check(got, definition(q, kp, vp, K, V, lens, True), dtype, step)
+
+
+# ---- what is refused: none of these gets as far as a launch --------------------------------------------------------------------
+def _host():
+    return dict(Q=torch.zeros(2, 4, 3, 64), K_prefix=torch.zeros(2, 9, 64), V_prefix=torch.zeros(2, 9, 64), K=torch.zeros(2, 2, 8, 64),
+                V=torch.zeros(2, 2, 8, 64), lengths=torch.zeros(2, dtype=torch.int32), scale=SCALE)
+
+
+@pytest.mark.parametrize("name,wrong", [
+    ("Q", torch.zeros(2, 4, 3, 32)), ("Q", torch.zeros(2, 4, 3, 64, dtype=torch.float64)), ("K", torch.zeros(3, 2, 8, 64)), ("K", torch.zeros(2, 2, 64, 8).transpose(2, 3)),
+    ("V", torch.zeros(2, 2, 7, 64)), ("V", torch.zeros(2, 2, 8, 64, dtype=torch.bfloat16)), ("K_prefix", torch.zeros(3, 9, 64)), ("K_prefix", torch.zeros(2, 2, 9, 64)),
+    ("K_prefix", torch.zeros(9, 64)), ("V_prefix", torch.zeros(2, 8, 64)), ("lengths", torch.zeros(3, dtype=torch.int32)), ("lengths", torch.zeros(2, dtype=torch.int64)),
+    ("lengths", torch.zeros(4, dtype=torch.int32)[::2]), ("out", torch.zeros(2, 4, 3, 64, dtype=torch.float16)), ("out", torch.zeros(2, 4, 2, 64)),
+    ("lse", torch.zeros(2, 4, 4)), ("lse", torch.zeros(2, 4, 3, dtype=torch.float64))])
+def test_arguments_that_do_not_fit_are_refused(name, wrong):
+    with pytest.raises(AssertionError, match="^" + name):
+        hk.shared_prefix_attention(**{**_host(), name: wrong})
+
+
+@pytest.mark.parametrize("name", ["Q", "K_prefix", "V_prefix", "K", "V", "lengths", "workspace", "out", "lse"])
+@pytest.mark.parametrize("wrong", [[1.0], 4096, False])
+def test_what_is_no_tensor_is_refused(name, wrong):
+    with pytest.raises(TypeError, match=f"^{name}: expected a tensor"):
+        hk.shared_prefix_attention(**{**_host(), name: wrong})
+
+
+def test_host_tensors_are_refused():
+    with pytest.raises(AssertionError, match="CUDA"):
+        hk.shared_prefix_attention(**_host())
+
+
+class _View(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("sB", C.c_int64), ("sM", C.c_int64), ("sH", C.c_int64)]
+
+
+class _Block(C.Structure):
+    _fields_ = [(n, _View) for n in ("Q", "Kp", "Vp", "K", "V", "O")] + [
+        ("LSE", C.c_void_p), ("lse_sB", C.c_int64), ("lse_sH", C.c_int64), ("lengths", C.c_void_p), ("B", C.c_int), ("nh", C.c_int), ("nh_kv", C.c_int),
+        ("dtype", C.c_int), ("T", C.c_int64), ("prefix_len", C.c_int64), ("kv_len", C.c_int64), ("scale", C.c_float), ("is_causal", C.c_bool),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+def _block():
+    b = _Block(LSE=0x1000, lse_sB=12, lse_sH=3, lengths=0x1000, B=2, nh=4, nh_kv=2, T=3, prefix_len=9, kv_len=8, scale=SCALE, workspace=0x1000, workspace_bytes=1 << 30)
+    for n, rows, heads in (("Q", 3, 4), ("Kp", 9, 2), ("Vp", 9, 2), ("K", 8, 2), ("V", 8, 2), ("O", 3, 4)):
+        setattr(b, n, _View(0x1000, heads * rows * 64, 64, rows * 64))
+    return b
+
+
+@pytest.mark.parametrize("path,value,status", [
+    ("Q.ptr", None, -1), ("Kp.ptr", None, -1), ("V.ptr", None, -1), ("O.ptr", None, -1), ("LSE", None, -1), ("B", 0, -2), ("nh", 0, -2), ("nh_kv", 0, -2), ("nh_kv", 3, -2),
+    ("T", 0, -2), ("T", (1 << 30) + 1, -2), ("prefix_len", -1, -2), ("kv_len", -1, -2), ("kv_len", (1 << 30) + 1, -2), ("scale", 0.0, -2), ("scale", math.inf, -2), ("scale", math.nan, -2),
+    ("Q.ptr", 0x1004, -3), ("K.sM", 66, -3), ("Vp.sH", 9 * 64 + 2, -3), ("K.sB", -1024, -3), ("lengths", 0x1002, -3), ("LSE", 0x1002, -3),
+    ("O.sM", 0, -6), ("O.sH", 32, -6), ("dtype", 3, -6), ("dtype", -1, -6)])
+def test_blocks_that_are_refused(path, value, status):
+    b = _block()
+    *head, last = path.split(".")
+    x = b
+    for n in head:
+        x = getattr(x, n)
+    setattr(x, last, value)
+    f = hk.lib().hk_shared_prefix_attention
+    f.argtypes = [C.c_void_p, C.c_void_p]
+    assert f(C.byref(b), None) == status
+    assert f(None, None) == -1
