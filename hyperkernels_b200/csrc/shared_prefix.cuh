@@ -1,0 +1,49 @@
+// shared_prefix.cuh -- what the kernels of the attention over a shared prefix (hk_shared_prefix_attention) have in common.
+#pragma once
+
+#include "operators.cuh"
+
+namespace hk {
+
+// The rows of a key head: row r = (b * T + i) * group + g is token i of request b under query head kvh * group + g, so that a
+// request's rows follow each other; R of them.  What a run of the prefix's keys gives for row kvh * R + r is left in the
+// workspace: the maximum and the sum of its weights (log2 units), and the weighted sum of the values.  The kernel that takes
+// the request's own keys adds the runs up in their order.
+struct PrefixArgs {
+    hk_view Q, Kp, Vp, K, V, O;
+    float* LSE;
+    int64_t lse_sB, lse_sH;
+    const int32_t* lengths;
+    int B, Hk, group, T, P, S;  // batch, key heads, query heads of each, new tokens, prefix keys, rows of the requests' caches
+    int R;
+    float scale_log2e;  // its size; a negative scale turns the queries' signs (flip)
+    uint32_t flip;
+    int causal;
+    int splits_p, per_p, tiles_p;  // over the prefix: runs of keys, keys of a run, row tiles of a key head
+    int splits_o, tiles_o;         // over the requests' own keys
+    float2* ml;                    // [splits_p][Hk * R]
+    float* part;                   // the same, [64]
+};
+
+template <class X>
+__device__ __forceinline__ const X* row_of(const hk_view& v, int64_t b, int64_t h, int64_t m) {
+    return static_cast<const X*>(v.ptr) + b * v.strideB + h * v.strideH + m * v.strideM;
+}
+// keys that request b has
+__device__ __forceinline__ int request_keys(const PrefixArgs& a, int b) { return a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S; }
+// own keys that token t of a request of `len` keys sees
+__device__ __forceinline__ int token_keys(const PrefixArgs& a, int len, int t) { return a.causal ? min(len, max(0, len - a.T + t + 1)) : len; }
+
+inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Launchers.  The kernel over the requests' own keys starts under the tail of the one over the prefix.
+struct FewPlan {
+    int rows;      // rows of a tile: 1, 2 (fp32 arithmetic lane by lane) or 16 (matrix instructions)
+    int step;      // keys that a CTA takes at once
+    int per_sm;    // CTAs that an SM holds
+};
+FewPlan few_plan(int dtype, int rows);
+int launch_prefix_few(const PrefixArgs& a, int dtype, cudaStream_t stream);
+int launch_own_few(const PrefixArgs& a, int dtype, cudaStream_t stream);
+
+}  // namespace hk

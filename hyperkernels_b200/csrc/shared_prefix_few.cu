@@ -1,0 +1,604 @@
+// shared_prefix_few.cu -- attention over a shared prefix where few rows meet a run of keys (decoding): bound by reading keys and
+// values.
+//
+// A warp takes its rows through batches of keys.  Every lane copies (cp.async) the very bytes it will work on into 16-byte slots
+// of its own, FEW_STAGES - 1 batches ahead, and waits for its own copies alone: no barrier until the warps merge what they have.
+// An SM has up to 12 warps x 12 KB on their way, four times what its share of the memory's latency takes.
+//   One or two rows in fp32: a half-warp to a key, four elements a lane (RowsOfOne).
+//   Up to 16 rows: matrix instructions (m16n8k8 on TF32, m16n8k16 on 16-bit types).  A lane's part of an operand is whatever
+// 16-byte pieces it loads, because the order of the contracted index (head dimension, keys) and of the result's columns is free
+// as long as both operands agree on it.  The instructions on tensor memory would need 128 rows to a tile.
+//   The requests' own keys: a cluster of CTAs shares them by the keys there are, adds up the prefix's runs and writes the result.
+#include <cmath>
+#include <mutex>
+#include <type_traits>
+
+#include "shared_prefix.cuh"
+
+namespace hk {
+namespace {
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <class X>
+__device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(X) == 2 && std::is_same<X, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t tf32_high(uint32_t x) { return x & 0xffffe000u; }
+__device__ __forceinline__ uint32_t tf32_low(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf32_high(x))); }
+
+
+constexpr int FEW_WARPS = 4, FEW_STAGES = 4;
+
+// fp32: x = h + l with h the upper 11 bits of the significand; a product is h h' + h l' + l h', added from the small ones on: what
+// is left out is 2^-22 of it.  A batch's weighted values are added to the rest in fp32 adds, since the tensor core's own additions
+// cut off instead of rounding.
+// Lane (g, c) = (lane / 4, lane % 4) of a matrix instruction: rows g and g + 8, columns and contracted elements by c.
+template <class X>
+struct FewMath;
+template <>
+struct FewMath<float> {
+    static constexpr int KEYS = 8;
+    uint4 k[4], v[4];  // k: key g, elements 16 i + 4 c ..; v: keys 2 c, 2 c, 2 c + 1, 2 c + 1, elements 4 g .. and 32 + 4 g ..
+    static __device__ __forceinline__ int key_k(int, int g) { return g; }
+    static __device__ __forceinline__ int at_k(int i, int c) { return 16 * i + 4 * c; }
+    static __device__ __forceinline__ int key_v(int i, int c) { return 2 * c + (i >> 1); }
+    static __device__ __forceinline__ int at_v(int i, int g) { return 32 * (i & 1) + 4 * g; }
+    uint32_t qh[8][4], ql[8][4];
+    __device__ __forceinline__ void load_q(const float* lo, const float* hi, int c, uint32_t flip) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 z = make_uint4(0, 0, 0, 0);
+            const uint4 a = lo ? *reinterpret_cast<const uint4*>(lo + 16 * i + 4 * c) : z, b = hi ? *reinterpret_cast<const uint4*>(hi + 16 * i + 4 * c) : z;
+            const uint32_t q[2][4] = {{a.x ^ flip, b.x ^ flip, a.y ^ flip, b.y ^ flip}, {a.z ^ flip, b.z ^ flip, a.w ^ flip, b.w ^ flip}};
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    qh[2 * i + h][e] = tf32_high(q[h][e]);
+                    ql[2 * i + h][e] = tf32_low(q[h][e]);
+                }
+        }
+    }
+    // s: rows g, g + 8 of keys 2 c, 2 c + 1
+    __device__ __forceinline__ void scores(float (&s)[1][4]) const {
+        uint32_t b[16], bl[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                b[4 * i + e] = tf32_high(w[e]);
+                bl[4 * i + e] = tf32_low(w[e]);
+            }
+        }
+        float lo[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][e] = 0.f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            mma_tf32(s[0], ql[x], b[2 * x], b[2 * x + 1]);
+            mma_tf32(lo, qh[x], bl[2 * x], bl[2 * x + 1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][e] += lo[e];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) mma_tf32(s[0], qh[x], b[2 * x], b[2 * x + 1]);
+    }
+    // o[j] = alpha o[j] + p V: rows g, g + 8 of columns n = 2 c, 2 c + 1, element 4 n + j or 32 + 4 n + j - 4
+    __device__ __forceinline__ void weigh(const float (&p)[1][4], const float (&alpha)[2], bool, float (&o)[8][4]) const {
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t x = __float_as_uint(p[0][(e & 1) * 2 + (e >> 1)]);  // rows g, g + 8 of key 2 c, then of 2 c + 1
+            ph[e] = tf32_high(x);
+            pl[e] = tf32_low(x);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint4 &x = v[j >> 2], &y = v[2 + (j >> 2)];
+            const uint32_t b0 = (j & 3) == 0 ? x.x : (j & 3) == 1 ? x.y : (j & 3) == 2 ? x.z : x.w;
+            const uint32_t b1 = (j & 3) == 0 ? y.x : (j & 3) == 1 ? y.y : (j & 3) == 2 ? y.z : y.w;
+            float t[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_tf32(t, pl, tf32_high(b0), tf32_high(b1));
+            mma_tf32(t, ph, tf32_low(b0), tf32_low(b1));
+            mma_tf32(t, ph, tf32_high(b0), tf32_high(b1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][e] = fmaf(o[j][e], alpha[e >> 1], t[e]);
+        }
+    }
+    static __device__ __forceinline__ int column(int j, int n) { return (j < 4 ? 0 : 28) + 4 * n + j; }
+};
+template <class X>
+struct FewMath {
+    static constexpr int KEYS = 16;
+    uint4 k[4], v[4];  // k: keys g, g, 8 + g, 8 + g, elements 32 (i & 1) + 8 c ..; v: keys 2 c, 2 c + 1, 8 + 2 c, 8 + 2 c + 1, elements 8 g ..
+    static __device__ __forceinline__ int key_k(int i, int g) { return g + 8 * (i >> 1); }
+    static __device__ __forceinline__ int at_k(int i, int c) { return 32 * (i & 1) + 8 * c; }
+    static __device__ __forceinline__ int key_v(int i, int c) { return 2 * c + (i & 1) + 8 * (i >> 1); }
+    static __device__ __forceinline__ int at_v(int, int g) { return 8 * g; }
+    uint32_t q[4][4];
+    __device__ __forceinline__ void load_q(const X* lo, const X* hi, int c, uint32_t flip) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint4 z = make_uint4(0, 0, 0, 0);
+            const uint4 a = lo ? *reinterpret_cast<const uint4*>(lo + 32 * i + 8 * c) : z, b = hi ? *reinterpret_cast<const uint4*>(hi + 32 * i + 8 * c) : z;
+            q[2 * i][0] = a.x; q[2 * i][1] = b.x; q[2 * i][2] = a.y; q[2 * i][3] = b.y;
+            q[2 * i + 1][0] = a.z; q[2 * i + 1][1] = b.z; q[2 * i + 1][2] = a.w; q[2 * i + 1][3] = b.w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[2 * i + (e >> 2)][e & 3] ^= flip;
+        }
+    }
+    // s[t]: rows g, g + 8 of keys 8 t + 2 c, 8 t + 2 c + 1
+    __device__ __forceinline__ void scores(float (&s)[2][4]) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint4 &x = k[2 * t], &y = k[2 * t + 1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+            mma_16<X>(s[t], q[0], x.x, x.y);
+            mma_16<X>(s[t], q[1], x.z, x.w);
+            mma_16<X>(s[t], q[2], y.x, y.y);
+            mma_16<X>(s[t], q[3], y.z, y.w);
+        }
+    }
+    __device__ __forceinline__ void weigh(const float (&p)[2][4], const float (&alpha)[2], bool rescale, float (&o)[8][4]) const {
+        // the weights take the type of the values: half a step of it each
+        const uint32_t a[4] = {pack<X>(p[0][0], p[0][1]), pack<X>(p[0][2], p[0][3]), pack<X>(p[1][0], p[1][1]), pack<X>(p[1][2], p[1][3])};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = j < 2 ? v[i].x : j < 4 ? v[i].y : j < 6 ? v[i].z : v[i].w;
+            if (rescale) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][e] *= alpha[e >> 1];
+            }
+            mma_16<X>(o[j], a, __byte_perm(w[0], w[1], j & 1 ? 0x7632 : 0x5410), __byte_perm(w[2], w[3], j & 1 ? 0x7632 : 0x5410));
+        }
+    }
+    static __device__ __forceinline__ int column(int j, int n) { return 8 * n + j; }
+};
+
+
+// Up to 16 rows of a warp.  Lane (g, c) has rows g and g + 8.
+template <class T>
+struct RowsOf16 {
+    typedef T X;
+    typedef FewMath<X> Math;
+    static constexpr int ROWS = 16, KEYS = Math::KEYS, PARTS = 1, NT = KEYS / 8;
+    static __device__ __forceinline__ int key_k(int i, int lane) { return Math::key_k(i, lane >> 2); }
+    static __device__ __forceinline__ int at_k(int i, int lane) { return Math::at_k(i, lane & 3); }
+    static __device__ __forceinline__ int key_v(int i, int lane) { return Math::key_v(i, lane & 3); }
+    static __device__ __forceinline__ int at_v(int i, int lane) { return Math::at_v(i, lane >> 2); }
+
+    Math f;
+    int limit[2];
+    float o[8][4], m[2], l[2];
+
+    __device__ __forceinline__ void start(const X* const (&q)[2], uint32_t flip, int lane) {
+        f.load_q(q[0], q[1], lane & 3, flip);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) m[e] = -INFINITY, l[e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+    }
+    static __device__ __forceinline__ int row(int i, int lane) { return (lane >> 2) + 8 * i; }
+    template <class F>
+    __device__ __forceinline__ void batch(const uint4 (*from)[32], int lane, int key0, int end, float scale_log2e, F&& copy_next) {
+        const int c = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.k[i] = from[i][lane];
+        float s[NT][4];
+        f.scores(s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.v[i] = from[4 + i][lane];
+        copy_next();
+        if (!__all_sync(0xffffffffu, key0 + KEYS <= min(limit[0], limit[1]))) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (key0 + 8 * t + 2 * c + (e & 1) >= limit[e >> 1]) s[t][e] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)  // copies of the last key: no weight, but the matrix instruction multiplies
+                if (key0 + key_v(i, lane) >= end) f.v[i] = make_uint4(0, 0, 0, 0);
+        }
+        float mx[2] = {-INFINITY, -INFINITY}, alpha[2], ref[2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+        bool raised = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * scale_log2e;
+            const float mn = fmaxf(m[i], mx[i]);
+            raised |= mn > m[i];
+            ref[i] = mn == -INFINITY ? 0.f : mn;
+            alpha[i] = ex2_approx(m[i] - ref[i]);  // 0 while m is -inf
+            m[i] = mn;
+            l[i] *= alpha[i];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[t][e] = ex2_approx(fmaf(s[t][e], scale_log2e, -ref[e >> 1]));
+                l[e >> 1] += s[t][e];
+            }
+        f.weigh(s, alpha, __any_sync(0xffffffffu, raised), o);
+    }
+    // a run of the prefix's keys
+    __device__ __forceinline__ void fold(const float2* ml, const float* part, int rows, int lane) {
+        const int c = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = row(i, lane);
+            if (r >= rows) continue;
+            const float2 x = ml[r];
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const float4*>(part + (int64_t)r * 64 + Math::column((k >> 1) * 4, 2 * c + (k & 1)));
+            const float mn = fmaxf(m[i], x.x), ref = mn == -INFINITY ? 0.f : mn, p = ex2_approx(m[i] - ref), w = ex2_approx(x.x - ref);
+            m[i] = mn;
+            l[i] = l[i] * p + (c == 0 ? x.y * w : 0.f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float y[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float& z = o[(k >> 1) * 4 + e][2 * i + (k & 1)];
+                    z = fmaf(y[e], w, z * p);
+                }
+            }
+        }
+    }
+    template <class P>
+    __device__ __forceinline__ void finish(P* part, float2 (*ml)[ROWS], int warp, int lane) {
+        const int c = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = row(i, lane);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if (c == 0) ml[warp][r] = make_float2(m[i], l[i]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int j = (k >> 1) * 4, e = 2 * i + (k & 1);
+                *reinterpret_cast<float4*>(&part[warp][r][Math::column(j, 2 * c + (k & 1))]) = make_float4(o[j][e], o[j + 1][e], o[j + 2][e], o[j + 3][e]);
+            }
+        }
+    }
+};
+
+// N rows of fp32, in the same half-warp: lane `sub` of 16 has elements 4 sub .. 4 sub + 3 of queries, keys and results.  A batch is
+// four keys of each half-warp; their scores are summed over the lanes with five shuffles a row, after which a lane has the score
+// of one key and takes its exponential alone.
+template <int N>
+struct RowsOfOne {
+    typedef float X;
+    static constexpr int ROWS = N, KEYS = 8, PARTS = 2;
+    static __device__ __forceinline__ int key_k(int i, int lane) { return 2 * i + (lane >> 4); }
+    static __device__ __forceinline__ int at_k(int, int lane) { return 4 * (lane & 15); }
+    static __device__ __forceinline__ int key_v(int i, int lane) { return key_k(i, lane); }
+    static __device__ __forceinline__ int at_v(int, int lane) { return 4 * (lane & 15); }
+
+    float4 q[N], o[N];
+    float m[N], l[N];
+    int limit[N];
+
+    static __device__ __forceinline__ int row(int i, int) { return i; }
+    __device__ __forceinline__ void start(const X* const (&from)[N], uint32_t flip, int lane) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (from[i]) {
+                const uint4 x = *reinterpret_cast<const uint4*>(from[i] + 4 * (lane & 15));
+                q[i] = make_float4(__uint_as_float(x.x ^ flip), __uint_as_float(x.y ^ flip), __uint_as_float(x.z ^ flip), __uint_as_float(x.w ^ flip));
+            }
+            o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+        }
+    }
+    template <class F>
+    __device__ __forceinline__ void batch(const uint4 (*from)[32], int lane, int key0, int end, float scale_log2e, F&& copy_next) {
+        const bool b3 = lane & 8, b2 = lane & 4;
+        float s[N];
+        {
+            float4 k[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) k[i] = reinterpret_cast<const float4&>(from[i][lane]);
+#pragma unroll
+            for (int r = 0; r < N; ++r) {
+                float d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = fmaf(q[r].x, k[i].x, q[r].y * k[i].y) + fmaf(q[r].z, k[i].z, q[r].w * k[i].w);
+                const float u0 = (b3 ? d[2] : d[0]) + __shfl_xor_sync(0xffffffffu, b3 ? d[0] : d[2], 8);
+                const float u1 = (b3 ? d[3] : d[1]) + __shfl_xor_sync(0xffffffffu, b3 ? d[1] : d[3], 8);
+                float u = (b2 ? u1 : u0) + __shfl_xor_sync(0xffffffffu, b2 ? u0 : u1, 4);
+                u += __shfl_xor_sync(0xffffffffu, u, 2);
+                u += __shfl_xor_sync(0xffffffffu, u, 1);
+                s[r] = u;  // of key 2 (2 b3 + b2) + the half
+            }
+        }
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = reinterpret_cast<const float4&>(from[4 + i][lane]);
+        copy_next();
+        const int key = key0 + (b3 ? 4 : 0) + (b2 ? 2 : 0) + (lane >> 4);
+        if (key0 + KEYS > end) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (key0 + key_v(i, lane) >= end) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            if (key >= limit[r]) s[r] = -INFINITY;
+            float mx = fmaxf(s[r], __shfl_xor_sync(0xffffffffu, s[r], 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4)) * scale_log2e;
+            const float mn = fmaxf(m[r], mx), ref = mn == -INFINITY ? 0.f : mn, alpha = ex2_approx(m[r] - ref);
+            const float p = ex2_approx(fmaf(s[r], scale_log2e, -ref));
+            m[r] = mn;
+            l[r] = fmaf(l[r], alpha, p);
+            o[r].x *= alpha; o[r].y *= alpha; o[r].z *= alpha; o[r].w *= alpha;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float w = __shfl_sync(0xffffffffu, p, (i & 2) * 4 + (i & 1) * 4, 16);
+                o[r].x = fmaf(w, v[i].x, o[r].x); o[r].y = fmaf(w, v[i].y, o[r].y); o[r].z = fmaf(w, v[i].z, o[r].z); o[r].w = fmaf(w, v[i].w, o[r].w);
+            }
+        }
+    }
+    __device__ __forceinline__ void fold(const float2* ml, const float* part, int rows, int lane) {
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            if (r >= rows) continue;
+            const float2 x = ml[r];
+            const float4 v = *reinterpret_cast<const float4*>(part + r * 64 + 4 * (lane & 15));
+            const float mn = fmaxf(m[r], x.x), ref = mn == -INFINITY ? 0.f : mn, p = ex2_approx(m[r] - ref), w = ex2_approx(x.x - ref);
+            m[r] = mn;
+            l[r] = l[r] * p + ((lane & 15) == 0 ? x.y * w : 0.f);
+            o[r].x = fmaf(v.x, w, o[r].x * p); o[r].y = fmaf(v.y, w, o[r].y * p); o[r].z = fmaf(v.z, w, o[r].z * p); o[r].w = fmaf(v.w, w, o[r].w * p);
+        }
+    }
+    template <class P>
+    __device__ __forceinline__ void finish(P* part, float2 (*ml)[ROWS], int warp, int lane) {
+        const int at = 2 * warp + (lane >> 4);
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            // every key's weight is in four lanes, a run of the prefix in lane 0 and so in one of the four sums
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 8);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 4);
+            if ((lane & 15) == 0) ml[at][r] = make_float2(m[r], l[r]);
+            *reinterpret_cast<float4*>(&part[at][r][4 * (lane & 15)]) = o[r];
+        }
+    }
+};
+
+template <class Rows>
+struct FewShared {
+    static constexpr int PARTS = FEW_WARPS * Rows::PARTS;
+    union {
+        uint4 ring[FEW_WARPS][FEW_STAGES][8][32];
+        float part[PARTS][Rows::ROWS][64 + 4];
+    };
+    float2 ml[PARTS][Rows::ROWS];
+    float merged[Rows::ROWS][64 + 4];  // of the CTA, for the others of its cluster
+    float2 merged_ml[Rows::ROWS];
+};
+
+__device__ __forceinline__ void copy16(void* smem, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(src) : "memory");
+}
+template <class X>
+__device__ __forceinline__ void store4(X* p, float4 v) {
+    if constexpr (sizeof(X) == 4) *reinterpret_cast<float4*>(p) = v;
+    else *reinterpret_cast<uint2*>(p) = make_uint2(pack<X>(v.x, v.y), pack<X>(v.z, v.w));
+}
+
+// OWN: a cluster takes a request's own keys, adds the runs of the prefix and writes the result.  Otherwise: a CTA takes a run of
+// the prefix and leaves its partial result.
+template <class Rows, bool OWN>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 3) prefix_few_kernel(const __grid_constant__ PrefixArgs a) {
+    typedef typename Rows::X X;
+    constexpr int N = Rows::ROWS, KEYS = Rows::KEYS, STEP = FEW_WARPS * KEYS, MINE = N < 16 ? N : 2;  // rows that a lane works on
+    extern __shared__ __align__(16) uint8_t few_smem[];
+    FewShared<Rows>& sh = *reinterpret_cast<FewShared<Rows>*>(few_smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (!OWN || a.splits_p == 0) {
+        pdl_wait();
+        pdl_trigger();
+    }
+    // the rows
+    const int ns = OWN ? a.splits_o : a.splits_p, item = blockIdx.x / ns, split = blockIdx.x - item * ns;
+    const int tiles = OWN ? a.tiles_o : a.tiles_p, at = item / tiles, tile = item - at * tiles;
+    const int b = OWN ? at / a.Hk : 0, kvh = at - b * a.Hk;
+    const int all = OWN ? a.T * a.group : a.R, row0 = b * a.T * a.group + tile * N, rows = min(N, all - tile * N);
+    // the keys
+    int len = a.P, begin = split * a.per_p, end = min(a.P, begin + a.per_p);
+    if (OWN) {
+        len = request_keys(a, b);
+        const int seen = token_keys(a, len, (tile * N + rows - 1) / a.group), per = ((seen + ns - 1) / ns + KEYS - 1) / KEYS * KEYS;
+        begin = min(seen, split * per);
+        end = min(seen, begin + per);
+    }
+    const int64_t stride_k = OWN ? a.K.strideM : a.Kp.strideM, stride_v = OWN ? a.V.strideM : a.Vp.strideM;
+    const X* K = OWN ? row_of<X>(a.K, b, kvh, 0) : row_of<X>(a.Kp, 0, kvh, 0);
+    const X* V = OWN ? row_of<X>(a.V, b, kvh, 0) : row_of<X>(a.Vp, 0, kvh, 0);
+    int put = 0, put_key = begin + warp * KEYS;
+    auto copy_next = [&] {  // the next batch of this warp, if there is one (behind the end the last key again); a group either way
+        if (put_key < end) {
+            uint4(*to)[32] = sh.ring[warp][put];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) copy16(&to[i][lane], K + min(put_key + Rows::key_k(i, lane), end - 1) * stride_k + Rows::at_k(i, lane));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) copy16(&to[4 + i][lane], V + min(put_key + Rows::key_v(i, lane), end - 1) * stride_v + Rows::at_v(i, lane));
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        put_key += STEP;
+        put = put + 1 == FEW_STAGES ? 0 : put + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < FEW_STAGES - 1; ++i) copy_next();
+    Rows w;
+    {
+        const X* q[MINE];
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int r = Rows::row(i, lane), row = row0 + r, token = row / a.group, bq = OWN ? b : token / a.T, t = token - bq * a.T;
+            q[i] = r < rows ? row_of<X>(a.Q, bq, kvh * a.group + (row - token * a.group), t) : nullptr;
+            w.limit[i] = OWN && r < rows ? min(end, token_keys(a, len, t)) : end;
+        }
+        w.start(q, a.flip, lane);
+    }
+    int get = 0;
+    for (int key0 = begin + warp * KEYS; key0 < end; key0 += STEP) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(FEW_STAGES - 2) : "memory");
+        const uint4(*from)[32] = sh.ring[warp][get];
+        get = get + 1 == FEW_STAGES ? 0 : get + 1;
+        w.batch(from, lane, key0, end, a.scale_log2e, copy_next);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const int64_t slot0 = (int64_t)kvh * a.R + row0, slot_rows = (int64_t)a.Hk * a.R;
+    if (OWN && a.splits_p > 0) {
+        pdl_wait();  // for the kernel over the prefix; what was before it was complete when this one began
+        pdl_trigger();
+        const int part = Rows::PARTS == 2 ? 2 * warp + (lane >> 4) : warp;
+        for (int s = split * FewShared<Rows>::PARTS + part; s < a.splits_p; s += ns * FewShared<Rows>::PARTS)
+            w.fold(a.ml + s * slot_rows + slot0, a.part + (s * slot_rows + slot0) * 64, rows, lane);
+    }
+    __syncthreads();  // the ring is the warps' exchange now
+    w.finish(sh.part, sh.ml, warp, lane);
+    __syncthreads();
+    // PER threads a row, 64 / PER elements each
+    constexpr int PER = N < 16 ? 16 : 8, E = 64 / PER;
+    const int r = threadIdx.x / PER, d = threadIdx.x % PER * E;
+    const bool mine = r < rows;
+    float M = -INFINITY, L = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    if (mine) {
+#pragma unroll
+        for (int p = 0; p < FewShared<Rows>::PARTS; ++p) M = fmaxf(M, sh.ml[p][r].x);
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int p = 0; p < FewShared<Rows>::PARTS; ++p) {
+            const float f = ex2_approx(sh.ml[p][r].x - ref);
+            L += sh.ml[p][r].y * f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(sh.part[p][r][d + e], f, acc[e]);
+        }
+    }
+    if (!OWN) {
+        if (!mine) return;
+        const int64_t to = split * slot_rows + slot0 + r;
+        if (d == 0) a.ml[to] = make_float2(M, L);
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(a.part + to * 64 + d + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+        return;
+    }
+    if (ns > 1) {
+        if (mine) {
+            if (d == 0) sh.merged_ml[r] = make_float2(M, L);
+#pragma unroll
+            for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(&sh.merged[r][d + e]) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (split == 0 && mine)
+            for (int s = 1; s < ns; ++s) {
+                const float ms = ld_cluster_f(mapa(&sh.merged_ml[r].x, s)), ls = ld_cluster_f(mapa(&sh.merged_ml[r].y, s));
+                const float mn = fmaxf(M, ms), ref = mn == -INFINITY ? 0.f : mn, p = ex2_approx(M - ref), f = ex2_approx(ms - ref);
+                M = mn;
+                L = fmaf(ls, f, L * p);
+#pragma unroll
+                for (int e = 0; e < E; e += 4) {
+                    const float4 v = ld_cluster_f4(mapa(&sh.merged[r][d + e], s));
+                    acc[e] = fmaf(v.x, f, acc[e] * p); acc[e + 1] = fmaf(v.y, f, acc[e + 1] * p);
+                    acc[e + 2] = fmaf(v.z, f, acc[e + 2] * p); acc[e + 3] = fmaf(v.w, f, acc[e + 3] * p);
+                }
+            }
+    }
+    if (split == 0 && mine) {
+        const float f = L > 0.f ? 1.f / L : 0.f;
+        const int row = row0 + r, token = row / a.group, t = token - b * a.T, h = kvh * a.group + (row - token * a.group);
+        X* to = const_cast<X*>(row_of<X>(a.O, b, h, t)) + d;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) store4(to + e, make_float4(acc[e] * f, acc[e + 1] * f, acc[e + 2] * f, acc[e + 3] * f));
+        if (d == 0) a.LSE[b * a.lse_sB + h * a.lse_sH + t] = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
+    }
+    if (ns > 1) {  // the others' results have been read
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    }
+}
+
+typedef void (*FewKernel)(PrefixArgs);
+struct FewEntry {
+    FewKernel kernel;
+    size_t smem;
+};
+template <class Rows, bool OWN>
+FewEntry entry() {
+    return {prefix_few_kernel<Rows, OWN>, sizeof(FewShared<Rows>)};
+}
+template <bool OWN>
+FewEntry pick(int dtype, int rows) {
+    if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>, OWN>();
+    if (dtype == HK_F16) return entry<RowsOf16<__half>, OWN>();
+    return rows == 1 ? entry<RowsOfOne<1>, OWN>() : rows == 2 ? entry<RowsOfOne<2>, OWN>() : entry<RowsOf16<float>, OWN>();
+}
+
+int launch(const FewEntry& k, const PrefixArgs& a, int64_t blocks, int cluster, cudaStream_t stream) {
+    // once per device and kernel: more than 48 KB of shared memory
+    static std::mutex mu;
+    static FewKernel known[HK_MAX_DEVICES][16];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        for (FewKernel& x : known[dev]) {
+            if (x == k.kernel) break;
+            if (x) continue;
+            if (cudaFuncSetAttribute(k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.smem) != cudaSuccess) return check_launch();
+            x = k.kernel;
+            break;
+        }
+    }
+    if (blocks > 0x7fffffffLL) return HK_ERR_BAD_SHAPE;
+    LaunchConfig lc((unsigned)blocks, FEW_WARPS * 32, k.smem, stream, cluster, true);
+    if (cudaLaunchKernelEx(&lc.cfg, k.kernel, a) != cudaSuccess) return check_launch();
+    count_launch();
+    return HK_OK;
+}
+
+}  // namespace
+
+FewPlan few_plan(int dtype, int rows) {
+    if (dtype != HK_F32) return {16, FEW_WARPS * 16, 3};
+    return {rows <= 2 ? rows : 16, FEW_WARPS * 8, 3};
+}
+int launch_prefix_few(const PrefixArgs& a, int dtype, cudaStream_t stream) {
+    return launch(pick<false>(dtype, few_plan(dtype, a.R).rows), a, (int64_t)a.Hk * a.tiles_p * a.splits_p, 1, stream);
+}
+int launch_own_few(const PrefixArgs& a, int dtype, cudaStream_t stream) {
+    return launch(pick<true>(dtype, few_plan(dtype, a.T * a.group).rows), a, (int64_t)a.B * a.Hk * a.tiles_o * a.splits_o, a.splits_o, stream);
+}
+
+}  // namespace hk
