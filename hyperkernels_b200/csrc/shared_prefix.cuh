@@ -45,5 +45,12 @@ struct FewPlan {
 FewPlan few_plan(int dtype, int rows);
 int launch_prefix_few(const PrefixArgs& a, int dtype, cudaStream_t stream);
 int launch_own_few(const PrefixArgs& a, int dtype, cudaStream_t stream);
+struct ManyPlan {
+    int rows;  // of a CTA's blocks
+    int keys;  // of a tile
+};
+ManyPlan many_plan(int dtype);
+int launch_prefix_many(const PrefixArgs& a, int dtype, cudaStream_t stream);
+int launch_own_many(const PrefixArgs& a, int dtype, bool prefix, cudaStream_t stream);  // prefix: its keys are taken first
 
 }  // namespace hk

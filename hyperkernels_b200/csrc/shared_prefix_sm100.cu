@@ -1,0 +1,533 @@
+// shared_prefix_sm100.cu -- attention over a shared prefix where many rows meet a run of keys: chunks of new tokens, or the rows of
+// a whole batch against the prefix.
+//
+// A CTA takes blocks of 128 rows of one key head (two of 16-bit types, one of fp32) through tiles of keys: a run of the prefix, the
+// request's own keys, or the prefix and then those.  Rows of a block are whatever rows of the key head follow each other (tokens
+// and query heads of one request, or of several against the prefix), so every key is loaded once for 128 or 256 of them.
+//   Warp 0 loads tiles with TMA, warp 1 issues the products S = Q K^T and, two products behind, O += P V (tcgen05, operands in
+// shared and tensor memory), four warps to a block of rows take S through the softmax, a row to a thread.  Scores are three deep
+// in tensor memory; P takes the place of its S.
+//   fp32: x = h + l with h the upper 11 bits of the significand, which is what the tensor core reads of an fp32 word.  Two warps
+// write the l parts of each tile beside it; a product is l h' + h l' + h h', in this order: what is left out is 2^-22 of it.  P V of
+// a tile comes back into registers and is added there in fp32: the tensor core's additions cut off instead of rounding, and over
+// thousands of keys in one accumulator that would be seen.
+#include <cmath>
+#include <cstring>
+#include <mutex>
+#include <type_traits>
+
+#include "shared_prefix.cuh"
+
+namespace hk {
+namespace {
+
+// tcgen05.mma of 16-bit operands (K = 16), one CTA
+__host__ __device__ constexpr uint32_t make_idesc_16(int M, int N, bool bf16, bool b_mn_major) {
+    const uint32_t fmt = bf16 ? 1u : 0u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void umma_ss_16(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "setp.ne.b32 q, %5, 0;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ts_16(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "setp.ne.b32 q, %5, 0;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
+        : "memory");
+}
+
+template <class X>
+struct Many {
+    static constexpr bool LOW = sizeof(X) == 4;      // products in three parts
+    static constexpr int STREAMS = LOW ? 1 : 2;      // blocks of rows
+    static constexpr int KEYS = LOW ? 64 : 128;      // of a tile
+    static constexpr int THREADS = 128 + 128 * STREAMS;
+    static constexpr int SLOTS = LOW ? 5 : 8;
+    static constexpr int Q_RAW = TILE * 64 * (int)sizeof(X), Q_BYTES = Q_RAW * (LOW ? 2 : 1);
+    static constexpr int KV_RAW = KEYS * 64 * (int)sizeof(X), KV_BYTES = KV_RAW * (LOW ? 2 : 1);
+    static constexpr int KV_BOX = KEYS * 128;        // 128 bytes of each row
+    struct __align__(16) Shared {
+        uint64_t q_full[STREAMS], kv_full[SLOTS], kv_empty[SLOTS], s_full[3], p_full[3], o_full[3];
+        uint64_t kv_ready[LOW ? SLOTS : 1];  // low parts are there
+        uint64_t last_full, last_ready;      // the request's last tile of values, with and without what is behind its last key
+        uint32_t tmem_base;
+        Abort abort;
+    };
+    static constexpr int OFF_KV = STREAMS * Q_BYTES, OFF_SH = OFF_KV + SLOTS * KV_BYTES, SMEM = OFF_SH + (int)sizeof(Shared);
+    static_assert(SMEM <= 232448, "exceeds the 227 KiB a CTA may opt in to");
+};
+constexpr uint32_t COL_O = 384;  // O_j: 64 columns, two of them behind three buffers of 128 for scores and weights
+
+enum ManyWait { W_Q = 301, W_KV, W_READY, W_EMPTY, W_S, W_P, W_O };
+
+struct ManyArgs {
+    PrefixArgs p;
+    DeviceStatus* status;
+    int own;           // the request's own keys are part of it, and the result is final
+    int prefix;        // the prefix is: of a run if not `own`, of all keys otherwise
+    int late;          // started under the tail of the kernel over the prefix, whose runs are added
+    int tiles;         // items of row blocks: of a key head, or of a request's
+};
+
+template <class X>
+__global__ void __launch_bounds__(Many<X>::THREADS, 1)
+prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ManyArgs args) {
+    typedef Many<X> C;
+    constexpr bool LOW = C::LOW, BF16 = std::is_same<X, __nv_bfloat16>::value;
+    constexpr int KEYS = C::KEYS, SLOTS = C::SLOTS;
+    const PrefixArgs& a = args.p;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *sQ = smem, *sKV = smem + C::OFF_KV;
+    typename C::Shared& sh = *reinterpret_cast<typename C::Shared*>(smem + C::OFF_SH);
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int t = 0; t < C::STREAMS; ++t) mbar_init(&sh.q_full[t], 4);
+        for (int s = 0; s < SLOTS; ++s) {
+            mbar_init(&sh.kv_full[s], 1);
+            if (LOW) mbar_init(&sh.kv_ready[s], 2);
+            mbar_init(&sh.kv_empty[s], 1);
+        }
+        for (int b = 0; b < 3; ++b) {
+            mbar_init(&sh.s_full[b], 1);
+            mbar_init(&sh.p_full[b], 4);
+            mbar_init(&sh.o_full[b], 1);
+        }
+        mbar_init(&sh.last_full, 1);
+        mbar_init(&sh.last_ready, 1);
+        sh.abort.id = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&sh.tmem_base, 512);
+        tmem_relinquish();
+        tc_fence_before_sync();
+    }
+    if (!args.late) {
+        pdl_wait();
+        pdl_trigger();
+    }
+    // the item: rows
+    const int ns = args.own ? 1 : a.splits_p, item = blockIdx.x / ns, split = blockIdx.x - item * ns, at = item / args.tiles;
+    const int tile = args.tiles - 1 - (item - at * args.tiles);  // the last rows see the most keys
+    const int b = args.own ? at / a.Hk : 0, kvh = at - b * a.Hk, BLOCK = C::STREAMS * TILE;
+    const int all = args.own ? a.T * a.group : a.R, first = tile * BLOCK, row0 = b * a.T * a.group + first, rows = min(BLOCK, all - first);
+    // and keys: tiles of the prefix, then the request's own
+    const int p_begin = args.own ? 0 : split * a.per_p, p_end = !args.prefix ? 0 : args.own ? a.P : min(a.P, p_begin + a.per_p);
+    const int len = args.own ? request_keys(a, b) : 0, seen = args.own ? token_keys(a, len, (first + rows - 1) / a.group) : 0;
+    const int n_p = (p_end - p_begin + KEYS - 1) / KEYS, n = n_p + (seen + KEYS - 1) / KEYS;
+    const int streams = C::STREAMS == 2 && rows > TILE ? 2 : 1;
+    __syncthreads();
+    tc_fence_after_sync();
+    constexpr uint32_t tmem = 0;  // all columns are this CTA's
+    if (sh.tmem_base != tmem) sh.abort.id = 398;
+    WaitNote wc{&sh.abort};
+    // 16-bit types: the last tile of a request's values goes by a warp that clears it (fp32: every tile does), on barriers of its
+    // own, for that warp sees no other phase of the slots' ones
+    auto by_hand = [&](int i) { return !LOW && i == 2 * n - 1 && n > n_p; };
+    // first key of tile j, in the prefix or of the request's own
+    auto key_of = [&](int j) { return j < n_p ? p_begin + j * KEYS : (j - n_p) * KEYS; };
+
+    if (warp < 4) {
+        if constexpr (C::STREAMS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        if (warp == 0) {
+            // ------------------------------ tiles of keys and values ------------------------------
+            if (lane == 0) {
+                bool ok = true;
+                for (int i = 0; ok && i < 2 * n; ++i) {
+                    const int j = i >> 1, s = i % SLOTS;
+                    if (i >= SLOTS && !(ok = mbar_wait(wc, &sh.kv_empty[s], (i / SLOTS - 1) & 1, W_EMPTY, i))) break;
+                    uint64_t* full = by_hand(i) ? &sh.last_full : &sh.kv_full[s];
+                    mbar_arrive_expect_tx(full, C::KV_RAW);
+                    const CUtensorMap* map = j < n_p ? (i & 1 ? &map_vp : &map_kp) : (i & 1 ? &map_v : &map_k);
+                    tma_load_tile(sKV + s * C::KV_BYTES, map, full, key_of(j), kvh, j < n_p ? 0 : b);
+                }
+                // a CTA that gave up may have copies in flight: they get time to land
+                if (!ok)
+                    for (const unsigned long long t0 = globaltimer_ns(); globaltimer_ns() - t0 < 100000ull;) {}
+            }
+        } else if (warp == 1) {
+            // ------------------------------ products ------------------------------
+            const uint32_t leader = elect_one_sync();
+            const int total = n * streams;
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, uint32_t parity, int id, int aux) { return (bool)__all_sync(0xffffffffu, mbar_wait(wc, bar, parity, id, aux)); };
+            auto wait_tile = [&](int i) {
+                const int s = i % SLOTS;
+                const uint32_t phase = (i / SLOTS) & 1;
+                if constexpr (LOW) return wait(&sh.kv_ready[s], phase, W_READY, i);
+                return by_hand(i) ? wait(&sh.last_ready, 0, W_READY, i) : wait(&sh.kv_full[s], phase, W_KV, i);
+            };
+            const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
+            for (int q = 0; q < total + 2 && ok; ++q) {
+                if (q < total) {  // S
+                    const int j = q >> (streams - 1), t = q & (streams - 1), i = 2 * j;
+                    if (j == 0 && !(ok = wait(&sh.q_full[t], 0, W_Q, t))) break;
+                    if (t == 0 && !(ok = wait_tile(i))) break;
+                    tc_fence_after_sync();
+                    const uint32_t d = tmem + (q % 3) * 128, qa = q_addr + t * C::Q_BYTES, ka = kv_addr + (i % SLOTS) * C::KV_BYTES;
+                    if constexpr (LOW) {
+                        constexpr uint32_t IDESC = make_idesc_tf32(TILE, KEYS, false, false);
+                        const Desc qd = kmajor_desc(qa, 0, BOX_BYTES), kd = kmajor_desc(ka, 0, C::KV_BOX);
+                        auto four = [&](uint32_t x, uint32_t y, uint32_t acc) {
+                            umma_ss4<KMAJOR_STEP, KMAJOR_STEP>(leader, d, qd + x, kd + y, IDESC, acc);
+                            umma_ss4<KMAJOR_STEP, KMAJOR_STEP>(leader, d, qd + (x + BOX_BYTES), kd + (y + C::KV_BOX), IDESC, 1u);
+                        };
+                        four(C::Q_RAW, 0, 0u);
+                        four(0, C::KV_RAW, 1u);
+                        four(0, 0, 1u);
+                    } else {
+                        constexpr uint32_t IDESC = make_idesc_16(TILE, KEYS, BF16, false);
+                        const uint64_t qd = make_smem_desc(qa, 16, 1024, DESC_SW128), kd = make_smem_desc(ka, 16, 1024, DESC_SW128);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) umma_ss_16(leader, d, qd + 2 * k, kd + 2 * k, IDESC, k > 0);
+                    }
+                    umma_commit_lead(leader, &sh.s_full[q % 3]);
+                    if (t == streams - 1) umma_commit_lead(leader, &sh.kv_empty[i % SLOTS]);
+                }
+                if (q >= 2) {  // O_j, two products behind
+                    const int r = q - 2, j = r >> (streams - 1), t = r & (streams - 1), i = 2 * j + 1;
+                    if (t == 0 && !(ok = wait_tile(i))) break;
+                    if (!(ok = wait(&sh.p_full[r % 3], (r / 3) & 1, W_P, r))) break;
+                    tc_fence_after_sync();
+                    const uint32_t p = tmem + (r % 3) * 128, d = tmem + COL_O + (LOW ? j & 1 : t) * 64, va = kv_addr + (i % SLOTS) * C::KV_BYTES;
+                    if constexpr (LOW) {
+                        constexpr uint32_t IDESC = make_idesc_tf32(TILE, HEAD_DIM, false, true);
+                        const Desc vd = mnmajor_desc(va, 0, C::KV_BOX);
+                        auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
+                            umma_ts4<MNMAJOR_STEP>(leader, d, p + x, vd + y, IDESC, acc);
+                            umma_ts4<MNMAJOR_STEP>(leader, d, p + x + 32, vd + (y + 4096), IDESC, 1u);
+                        };
+                        eight(64, 0, 0u);
+                        eight(0, C::KV_RAW, 1u);
+                        eight(0, 0, 1u);
+                    } else {
+                        constexpr uint32_t IDESC = make_idesc_16(TILE, HEAD_DIM, BF16, true);
+                        const uint64_t vd = make_smem_desc(va, 16, 1024, DESC_SW128);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) umma_ts_16(leader, d, p + 8 * k, vd + (2048 >> 4) * k, IDESC, k > 0 || j > 0);
+                    }
+                    umma_commit_lead(leader, &sh.o_full[r % 3]);
+                    if (t == streams - 1) umma_commit_lead(leader, &sh.kv_empty[i % SLOTS]);
+                }
+            }
+        } else if (LOW || warp == 2) {
+            // Rows behind the request's last key may hold anything, and 0 times a NaN is one: they are cleared among the values.
+            // fp32: the tiles' low parts.
+            const int me = LOW ? threadIdx.x - 64 : lane;
+            bool ok = true;
+            for (int i = LOW ? 0 : 2 * n - 1; ok && n > (LOW ? 0 : n_p) && i < 2 * n; ++i) {
+                const int j = i >> 1, s = i % SLOTS;
+                ok = __all_sync(0xffffffffu, LOW ? mbar_wait(wc, &sh.kv_full[s], (i / SLOTS) & 1, W_KV, i) : mbar_wait(wc, &sh.last_full, 0, W_KV, i));
+                if (!ok) break;
+                const int keep = (i & 1) && j >= n_p ? min(KEYS, len - key_of(j)) : KEYS;  // rows that are values
+                uint4* raw = reinterpret_cast<uint4*>(sKV + s * C::KV_BYTES);
+                if constexpr (LOW) {
+                    constexpr int EACH = C::KV_RAW / 16 / 64, AT_ONCE = 8;
+                    auto rest = [](uint32_t v) { return __float_as_uint(__uint_as_float(v) - __uint_as_float(v & 0xffffe000u)); };
+                    uint4 *from = raw + me, *low = from + C::KV_RAW / 16;
+                    if (keep < KEYS) {
+#pragma unroll
+                        for (int k = 0; k < EACH; ++k)
+                            if (((k * 64 + me) & (C::KV_BOX / 16 - 1)) / 8 >= keep) from[k * 64] = make_uint4(0, 0, 0, 0);  // row of the box
+                    }
+#pragma unroll 1
+                    for (int k0 = 0; k0 < EACH; k0 += AT_ONCE, from += AT_ONCE * 64, low += AT_ONCE * 64) {
+                        uint4 x[AT_ONCE];
+#pragma unroll
+                        for (int k = 0; k < AT_ONCE; ++k) x[k] = from[k * 64];
+#pragma unroll
+                        for (int k = 0; k < AT_ONCE; ++k) low[k * 64] = make_uint4(rest(x[k].x), rest(x[k].y), rest(x[k].z), rest(x[k].w));
+                    }
+                } else {
+                    for (int k = keep * 8 + me; k < C::KV_RAW / 16; k += 32) raw[k] = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                mbar_arrive_warp(LOW ? &sh.kv_ready[s] : &sh.last_ready, lane);
+            }
+        }
+    } else {
+        // ------------------------------ softmax ------------------------------
+        if constexpr (C::STREAMS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+        const int t = (warp - 4) >> 2, quarter = warp & 3, in_block = quarter * 32 + lane, r = t * TILE + in_block;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        const bool live = t * TILE + quarter * 32 < rows, valid = r < rows;
+        const int row = row0 + r, token = row / a.group, bq = args.own ? b : token / a.T, tok = token - bq * a.T, h = kvh * a.group + row - token * a.group;
+        const int limit = args.own && valid ? token_keys(a, len, tok) : 0;  // own keys the row sees
+        if (t < streams) {  // the row of Q, in the layout of a K-major operand
+            const uint4* from = reinterpret_cast<const uint4*>(row_of<X>(a.Q, valid ? bq : 0, valid ? h : 0, valid ? tok : 0));
+            uint8_t* to = sQ + t * C::Q_BYTES + in_block * 128;
+            constexpr int CHUNKS = 64 * sizeof(X) / 16;
+            uint4 x[CHUNKS];
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) x[c] = valid ? from[c] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                x[c].x ^= a.flip; x[c].y ^= a.flip; x[c].z ^= a.flip; x[c].w ^= a.flip;
+                uint8_t* slot = to + (c >> 3) * BOX_BYTES + (((c & 7) ^ (in_block & 7)) << 4);
+                *reinterpret_cast<uint4*>(slot) = x[c];
+                if constexpr (LOW) {
+                    auto rest = [](uint32_t v) { return __float_as_uint(__uint_as_float(v) - __uint_as_float(v & 0xffffe000u)); };
+                    *reinterpret_cast<uint4*>(slot + C::Q_RAW) = make_uint4(rest(x[c].x), rest(x[c].y), rest(x[c].z), rest(x[c].w));
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive_warp(&sh.q_full[t], lane);
+        }
+        float o[64], m = -INFINITY, l = 0.f;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, int q, int id, int j) {  // of product q
+            ok = __all_sync(0xffffffffu, mbar_wait(wc, &bar[q % 3], (q / 3) & 1, id, j));
+            if (ok) tc_fence_after_sync();
+            return ok;
+        };
+        const float2 scale2 = make_float2(a.scale_log2e, a.scale_log2e);
+        if constexpr (LOW) {
+            // O_j of every tile comes back and is added here: o = o * before + O_j
+            float before = 0.f, alpha = 0.f;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) o[i] = 0.f;
+            auto add = [&](int j) {
+                if (!wait(sh.o_full, j, W_O, j) || !live) return;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t x[32];
+                    tmem_ld32(lanes + COL_O + (j & 1) * 64 + 32 * half, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float2& y = reinterpret_cast<float2&>(o[32 * half + i]);
+                        y = __ffma2_rn(y, make_float2(before, before), make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+                    }
+                }
+            };
+            for (int j = 0; j < n && wait(sh.s_full, j, W_S, j); ++j) {
+                const uint32_t at_s = lanes + j % 3 * 128;
+                if (live) {
+                    const int lim = (j < n_p ? p_end : limit) - key_of(j);  // columns the row sees
+                    uint32_t x[64];
+                    tmem_ld32p(at_s, x);
+                    tmem_ld32p(at_s + 32, x + 32);
+                    tmem_wait_ld();
+                    if (lim < KEYS) {
+#pragma unroll
+                        for (int i = 0; i < 64; ++i)
+                            if (i >= lim) x[i] = __float_as_uint(-INFINITY);
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                    const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e), ref = mn == -INFINITY ? 0.f : mn;
+                    alpha = ex2_approx(m - ref);  // 0 while m is -inf
+                    m = mn;
+                    const float2 nm = make_float2(-ref, -ref);
+                    float2 sum[2] = {};
+#pragma unroll
+                    for (int c = 0; c < 64; c += 32) {
+                        uint32_t z[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[c + i]), __uint_as_float(x[c + i + 1])), scale2, nm);
+                            const float2 w = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                            sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
+                            x[c + i] = __float_as_uint(w.x);
+                            x[c + i + 1] = __float_as_uint(w.y);
+                            z[i] = __float_as_uint(w.x - __uint_as_float(x[c + i] & 0xffffe000u));
+                            z[i + 1] = __float_as_uint(w.y - __uint_as_float(x[c + i + 1] & 0xffffe000u));
+                        }
+                        tmem_st32p(at_s + c, x + c);
+                        tmem_st32(at_s + 64 + c, z);
+                    }
+                    l = fmaf(l, alpha, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                    tmem_wait_st();
+                }
+                tc_fence_before_sync();
+                mbar_arrive_warp(&sh.p_full[j % 3], lane);
+                if (j > 0) add(j - 1);
+                if (!ok) break;
+                before = alpha;
+            }
+            if (ok && n > 0) add(n - 1);
+        } else if (t < streams) {
+            // O stays in tensor memory and is scaled there when a maximum has risen by more than 2^RISE: a stale one makes weights
+            // larger, which neither fp32 sums nor 16-bit types mind up to there
+            constexpr float RISE = 8.f;
+            const uint32_t at_o = lanes + COL_O + t * 64;
+            uint32_t x[128];
+            for (int j = 0; j < n && wait(sh.s_full, j * streams + t, W_S, j); ++j) {
+                const int q = j * streams + t;
+                const uint32_t at_s = lanes + q % 3 * 128;
+                if (live) {
+                    const int lim = (j < n_p ? p_end : limit) - key_of(j);  // columns the row sees
+#pragma unroll
+                    for (int c = 0; c < 128; c += 32) tmem_ld32p(at_s + c, x + c);
+                    tmem_wait_ld();
+                    if (lim < KEYS) {
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (i >= lim) x[i] = __float_as_uint(-INFINITY);
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e;
+                    const bool raise = m == -INFINITY ? top > -INFINITY : top > m + RISE;
+                    const float mn = raise ? top : m, alpha = raise ? ex2_approx(m - mn) : 1.f;  // 0 from -inf
+                    m = mn;
+                    if (j > 0 && __any_sync(0xffffffffu, raise)) {
+                        if (!wait(sh.o_full, q - streams, W_O, j)) break;
+#pragma unroll 1
+                        for (int c = 0; c < 64; c += 32) {
+                            uint32_t y[32];
+                            tmem_ld32(at_o + c, y);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+                            tmem_st32(at_o + c, y);
+                        }
+                    }
+                    const float ref = mn == -INFINITY ? 0.f : mn;
+                    const float2 nm = make_float2(-ref, -ref);
+                    float2 sum[2] = {};
+#pragma unroll
+                    for (int i = 0; i < 128; i += 2) {
+                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, nm);
+                        const float2 w = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                        sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
+                        x[i / 2] = pack<X>(w.x, w.y);  // the weights take the type of the values: half a step of it each
+                    }
+                    tmem_st32p(at_s, x);
+                    tmem_st32p(at_s + 32, x + 32);
+                    l = fmaf(l, alpha, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                    tmem_wait_st();
+                }
+                tc_fence_before_sync();
+                mbar_arrive_warp(&sh.p_full[q % 3], lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 64; ++i) o[i] = 0.f;
+            if (ok && n > 0 && wait(sh.o_full, (n - 1) * streams + t, W_O, n) && live) {
+                tmem_ld32p(at_o, reinterpret_cast<uint32_t*>(o));
+                tmem_ld32p(at_o + 32, reinterpret_cast<uint32_t*>(o) + 32);
+                tmem_wait_ld();
+            }
+        }
+        if (args.late) {
+            pdl_wait();  // for the kernel over the prefix; what was before it was complete when this one began
+            pdl_trigger();
+        }
+        if (valid && ok) {
+            const int64_t slot = (int64_t)kvh * a.R + row, slot_rows = (int64_t)a.Hk * a.R;
+            if (!args.own) {
+                a.ml[split * slot_rows + slot] = make_float2(m, l);
+                float4* to = reinterpret_cast<float4*>(a.part + (split * slot_rows + slot) * 64);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            } else {
+                for (int s = 0; args.late && s < a.splits_p; ++s) {
+                    const float2 x = a.ml[s * slot_rows + slot];
+                    const float4* from = reinterpret_cast<const float4*>(a.part + (s * slot_rows + slot) * 64);
+                    const float mn = fmaxf(m, x.x), ref = mn == -INFINITY ? 0.f : mn, f = ex2_approx(m - ref), w = ex2_approx(x.x - ref);
+                    m = mn;
+                    l = fmaf(l, f, x.y * w);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float4 v = from[i];
+                        o[4 * i] = fmaf(v.x, w, o[4 * i] * f); o[4 * i + 1] = fmaf(v.y, w, o[4 * i + 1] * f);
+                        o[4 * i + 2] = fmaf(v.z, w, o[4 * i + 2] * f); o[4 * i + 3] = fmaf(v.w, w, o[4 * i + 3] * f);
+                    }
+                }
+                const float f = l > 0.f ? 1.f / l : 0.f;
+                uint4* to = reinterpret_cast<uint4*>(const_cast<X*>(row_of<X>(a.O, b, h, tok)));
+                if constexpr (LOW) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        to[i] = make_uint4(__float_as_uint(o[4 * i] * f), __float_as_uint(o[4 * i + 1] * f), __float_as_uint(o[4 * i + 2] * f), __float_as_uint(o[4 * i + 3] * f));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        to[i] = make_uint4(pack<X>(o[8 * i] * f, o[8 * i + 1] * f), pack<X>(o[8 * i + 2] * f, o[8 * i + 3] * f),
+                                           pack<X>(o[8 * i + 4] * f, o[8 * i + 5] * f), pack<X>(o[8 * i + 6] * f, o[8 * i + 7] * f));
+                }
+                a.LSE[b * a.lse_sB + h * a.lse_sH + tok] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+        if (lane == 0) report_abort(sh.abort, args.status);
+    }
+}
+
+// The tiles of a view of keys or values: rows of 128 bytes (fp32: two pieces of a row).
+int tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, bool values) {
+    if (T == 0) {
+        memset(map, 0, sizeof(*map));  // no tile of it is loaded
+        return HK_OK;
+    }
+    if (dtype == HK_F32) return make_tile_map(map, static_cast<const float*>(v.ptr), HEAD_DIM, (int)B, H, T, v.strideB, T == 1 ? 64 : v.strideM, v.strideH, Many<float>::KEYS, values);
+    EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return HK_ERR_CUDA;
+    const int64_t sM = T == 1 ? 64 : v.strideM, sH = H == 1 ? sM * T : v.strideH, sB = B == 1 ? std::max(sH * H, sM * T) : v.strideB;
+    cuuint64_t dims[5] = {64, (cuuint64_t)T, 1, (cuuint64_t)H, (cuuint64_t)B};
+    cuuint64_t strides[4] = {(cuuint64_t)sM * 2, 128, (cuuint64_t)sH * 2, (cuuint64_t)sB * 2};
+    cuuint32_t box[5] = {64, (cuuint32_t)Many<__half>::KEYS, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+    const CUresult r = enc(map, dtype == HK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, v.ptr, dims, strides, box, ones,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HK_OK : HK_ERR_CUDA;
+}
+
+template <class X>
+int launch(const ManyArgs& args, int dtype, int64_t blocks, cudaStream_t stream) {
+    static std::once_flag once[HK_MAX_DEVICES];
+    static cudaError_t rc[HK_MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
+    std::call_once(once[dev], [dev] { rc[dev] = cudaFuncSetAttribute(prefix_many_kernel<X>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<X>::SMEM); });
+    if (rc[dev] != cudaSuccess) return HK_ERR_CUDA;
+    if (blocks > 0x7fffffffLL) return HK_ERR_BAD_SHAPE;
+    const PrefixArgs& a = args.p;
+    CUtensorMap kp, vp, k, v;
+    int s;
+    if ((s = tile_map(&kp, a.Kp, dtype, 1, a.Hk, args.prefix ? a.P : 0, false)) || (s = tile_map(&vp, a.Vp, dtype, 1, a.Hk, args.prefix ? a.P : 0, true)) ||
+        (s = tile_map(&k, a.K, dtype, a.B, a.Hk, args.own ? a.S : 0, false)) || (s = tile_map(&v, a.V, dtype, a.B, a.Hk, args.own ? a.S : 0, true)))
+        return s;
+    LaunchConfig lc((unsigned)blocks, Many<X>::THREADS, Many<X>::SMEM, stream, 1, true);
+    if (cudaLaunchKernelEx(&lc.cfg, prefix_many_kernel<X>, kp, vp, k, v, args) != cudaSuccess) return check_launch();
+    count_launch();
+    return HK_OK;
+}
+int launch(const ManyArgs& args, int dtype, int64_t blocks, cudaStream_t stream) {
+    return dtype == HK_F32 ? launch<float>(args, dtype, blocks, stream) : dtype == HK_BF16 ? launch<__nv_bfloat16>(args, dtype, blocks, stream) : launch<__half>(args, dtype, blocks, stream);
+}
+
+}  // namespace
+
+ManyPlan many_plan(int dtype) { return dtype == HK_F32 ? ManyPlan{TILE, 64} : ManyPlan{2 * TILE, 128}; }
+int launch_prefix_many(const PrefixArgs& a, int dtype, cudaStream_t stream) {
+    ManyArgs args{a, device_status_ptr(), 0, 1, 0, a.tiles_p};
+    return args.status ? launch(args, dtype, (int64_t)a.Hk * a.tiles_p * a.splits_p, stream) : HK_ERR_CUDA;
+}
+int launch_own_many(const PrefixArgs& a, int dtype, bool prefix, cudaStream_t stream) {
+    ManyArgs args{a, device_status_ptr(), 1, prefix, !prefix && a.splits_p > 0, a.tiles_o};
+    return args.status ? launch(args, dtype, (int64_t)a.B * a.Hk * a.tiles_o, stream) : HK_ERR_CUDA;
+}
+
+}  // namespace hk
