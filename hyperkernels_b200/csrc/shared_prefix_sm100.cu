@@ -4,7 +4,7 @@
 // A CTA takes blocks of 128 rows of one key head (two of 16-bit types, one of fp32) through tiles of keys: a run of the prefix, the
 // request's own keys, or the prefix and then those.  Rows of a block are whatever rows of the key head follow each other (tokens
 // and query heads of one request, or of several against the prefix), so every key is loaded once for 128 or 256 of them.
-//   Warp 0 loads tiles with TMA, warp 1 issues the products S = Q K^T and, two products behind, O += P V (tcgen05, operands in
+//   Warp 0 loads tiles with TMA, warp 1 issues the products S = Q K^T and, a tile or two behind, O += P V (tcgen05, operands in
 // shared and tensor memory), four warps to a block of rows take S through the softmax, a row to a thread.  Scores are three deep
 // in tensor memory; P takes the place of its S.
 //   fp32: x = h + l with h the upper 11 bits of the significand, which is what the tensor core reads of an fp32 word.  Two warps
@@ -56,6 +56,7 @@ struct Many {
     static constexpr int KEYS = LOW ? 64 : 128;      // of a tile
     static constexpr int THREADS = 128 + 128 * STREAMS;
     static constexpr int SLOTS = LOW ? 5 : 8;
+    static constexpr int AHEAD = LOW ? 2 : 1;        // tiles that the scores are ahead of the weighted values
     static constexpr int Q_RAW = TILE * 64 * (int)sizeof(X), Q_BYTES = Q_RAW * (LOW ? 2 : 1);
     static constexpr int KV_RAW = KEYS * 64 * (int)sizeof(X), KV_BYTES = KV_RAW * (LOW ? 2 : 1);
     static constexpr int KV_BOX = KEYS * 128;        // 128 bytes of each row
@@ -139,6 +140,19 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     // 16-bit types: the last tile of a request's values goes by a warp that clears it (fp32: every tile does), on barriers of its
     // own, for that warp sees no other phase of the slots' ones
     auto by_hand = [&](int i) { return !LOW && i == 2 * n - 1 && n > n_p; };
+    // Tiles go through the ring in the order of their use, keys a tile (fp32: two) ahead: K0 .. K(A) V0 K(A+1) V1 ..
+    constexpr int A = C::AHEAD;
+    auto entry_k = [](int j) { return j + max(0, j - A); };
+    auto entry_v = [&](int j) { return j + min(n, A + 1 + j); };
+    struct Entry {
+        int j;
+        bool v;
+    };
+    auto entry = [&](int i) -> Entry {
+        if (i < min(n, A + 1)) return {i, false};
+        const int k = i - (A + 1);
+        return k < 2 * (n - A - 1) ? (k & 1 ? Entry{A + 1 + (k >> 1), false} : Entry{k >> 1, true}) : Entry{i - n, true};
+    };
     // first key of tile j, in the prefix or of the request's own
     auto key_of = [&](int j) { return j < n_p ? p_begin + j * KEYS : (j - n_p) * KEYS; };
 
@@ -149,11 +163,12 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             if (lane == 0) {
                 bool ok = true;
                 for (int i = 0; ok && i < 2 * n; ++i) {
-                    const int j = i >> 1, s = i % SLOTS;
+                    const auto [j, is_v] = entry(i);
+                    const int s = i % SLOTS;
                     if (i >= SLOTS && !(ok = mbar_wait(wc, &sh.kv_empty[s], (i / SLOTS - 1) & 1, W_EMPTY, i))) break;
                     uint64_t* full = by_hand(i) ? &sh.last_full : &sh.kv_full[s];
                     mbar_arrive_expect_tx(full, C::KV_RAW);
-                    const CUtensorMap* map = j < n_p ? (i & 1 ? &map_vp : &map_kp) : (i & 1 ? &map_v : &map_k);
+                    const CUtensorMap* map = j < n_p ? (is_v ? &map_vp : &map_kp) : (is_v ? &map_v : &map_k);
                     tma_load_tile(sKV + s * C::KV_BYTES, map, full, key_of(j), kvh, j < n_p ? 0 : b);
                 }
                 // a CTA that gave up may have copies in flight: they get time to land
@@ -164,6 +179,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             // ------------------------------ products ------------------------------
             const uint32_t leader = elect_one_sync();
             const int total = n * streams;
+            const int ahead = A * streams;  // products that S is ahead of O
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t parity, int id, int aux) { return (bool)__all_sync(0xffffffffu, mbar_wait(wc, bar, parity, id, aux)); };
             auto wait_tile = [&](int i) {
@@ -173,9 +189,9 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                 return by_hand(i) ? wait(&sh.last_ready, 0, W_READY, i) : wait(&sh.kv_full[s], phase, W_KV, i);
             };
             const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
-            for (int q = 0; q < total + 2 && ok; ++q) {
+            for (int q = 0; q < total + ahead && ok; ++q) {
                 if (q < total) {  // S
-                    const int j = q >> (streams - 1), t = q & (streams - 1), i = 2 * j;
+                    const int j = q >> (streams - 1), t = q & (streams - 1), i = entry_k(j);
                     if (j == 0 && !(ok = wait(&sh.q_full[t], 0, W_Q, t))) break;
                     if (t == 0 && !(ok = wait_tile(i))) break;
                     tc_fence_after_sync();
@@ -199,8 +215,8 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                     umma_commit_lead(leader, &sh.s_full[q % 3]);
                     if (t == streams - 1) umma_commit_lead(leader, &sh.kv_empty[i % SLOTS]);
                 }
-                if (q >= 2) {  // O_j, two products behind
-                    const int r = q - 2, j = r >> (streams - 1), t = r & (streams - 1), i = 2 * j + 1;
+                if (q >= ahead) {  // O
+                    const int r = q - ahead, j = r >> (streams - 1), t = r & (streams - 1), i = entry_v(j);
                     if (t == 0 && !(ok = wait_tile(i))) break;
                     if (!(ok = wait(&sh.p_full[r % 3], (r / 3) & 1, W_P, r))) break;
                     tc_fence_after_sync();
@@ -231,10 +247,11 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             const int me = LOW ? threadIdx.x - 64 : lane;
             bool ok = true;
             for (int i = LOW ? 0 : 2 * n - 1; ok && n > (LOW ? 0 : n_p) && i < 2 * n; ++i) {
-                const int j = i >> 1, s = i % SLOTS;
+                const auto [j, is_v] = entry(i);
+                const int s = i % SLOTS;
                 ok = __all_sync(0xffffffffu, LOW ? mbar_wait(wc, &sh.kv_full[s], (i / SLOTS) & 1, W_KV, i) : mbar_wait(wc, &sh.last_full, 0, W_KV, i));
                 if (!ok) break;
-                const int keep = (i & 1) && j >= n_p ? min(KEYS, len - key_of(j)) : KEYS;  // rows that are values
+                const int keep = is_v && j >= n_p ? min(KEYS, len - key_of(j)) : KEYS;  // rows that are values
                 uint4* raw = reinterpret_cast<uint4*>(sKV + s * C::KV_BYTES);
                 if constexpr (LOW) {
                     constexpr int EACH = C::KV_RAW / 16 / 64, AT_ONCE = 8;
