@@ -1,11 +1,53 @@
 // shared_prefix.cu -- attention of a batch whose requests share a prefix (include/hk_attention.h: hk_shared_prefix_attention):
 // checks of arguments and how the work is cut.
 #include <cmath>
+#include <cstring>
 
 #include "shared_prefix.cuh"
 
 namespace hk {
 namespace {
+
+// ---------------------------------------------------------------------------
+// The slots of each row, added up in their order: 16 lanes a row.
+// ---------------------------------------------------------------------------
+template <class X>
+__global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_constant__ PrefixArgs a) {
+    const int sub = threadIdx.x & 15;
+    const int64_t rows = (int64_t)a.Hk * a.R, row = min((int64_t)blockIdx.x * 8 + (threadIdx.x >> 4), rows - 1);  // the last row more than once
+    const int kvh = (int)(row / a.R), r = (int)(row - (int64_t)kvh * a.R), token = r / a.group, b = token / a.T, t = token - b * a.T, h = kvh * a.group + r - token * a.group;
+    pdl_wait();
+    pdl_trigger();
+    float M = -INFINITY, L = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < a.slots; s0 += 16) {
+        const int k = min(16, a.slots - s0);
+        const float* from = a.part + ((int64_t)s0 * rows + row) * 64 + 4 * sub;
+        float4 v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < k) v[i] = *reinterpret_cast<const float4*>(from + i * rows * 64);
+        const float2 x = sub < k ? a.ml[(s0 + sub) * rows + row] : make_float2(-INFINITY, 0.f);  // a lane looks up one slot
+        float mx = x.x;
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        mx = fmaxf(mx, M);
+        const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(M - ref), w = x.y == 0.f ? 0.f : ex2_approx(x.x - ref);
+        M = mx;
+        L *= old;
+        o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (i >= k) break;
+            const float f = __shfl_sync(0xffffffffu, w, i, 16), l = __shfl_sync(0xffffffffu, x.y, i, 16);
+            L = fmaf(l, f, L);
+            o.x = fmaf(v[i].x, f, o.x); o.y = fmaf(v[i].y, f, o.y); o.z = fmaf(v[i].z, f, o.z); o.w = fmaf(v[i].w, f, o.w);
+        }
+    }
+    const float f = L > 0.f ? 1.f / L : 0.f;
+    store4(const_cast<X*>(row_of<X>(a.O, b, h, t)) + 4 * sub, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+    if (sub == 0) a.LSE[b * a.lse_sB + h * a.lse_sH + t] = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
+}
 
 int check_sizes(const hk_shared_prefix_params* p) {
     if (!p) return HK_ERR_NULL_POINTER;
@@ -21,10 +63,13 @@ int check(const hk_shared_prefix_params* p) {
     int rc = check_sizes(p);
     if (rc != HK_OK) return rc;
     if ((rc = check_view(p->Q, p->B, p->nh, p->T, p->dtype, false)) || (rc = check_view(p->O, p->B, p->nh, p->T, p->dtype, true))) return rc;
-    for (const hk_view* v : {&p->Kp, &p->Vp})
-        if (p->prefix_len > 0 && (rc = check_view(*v, 1, p->nh_kv, p->prefix_len, p->dtype, false))) return rc;
-    for (const hk_view* v : {&p->K, &p->V})
-        if (p->kv_len > 0 && (rc = check_view(*v, p->B, p->nh_kv, p->kv_len, p->dtype, false))) return rc;
+    auto keys = [&](const hk_view& v, int B, int64_t T) {
+        const int rc = T > 0 ? check_view(v, B, p->nh_kv, T, p->dtype, false) : HK_OK;
+        // tensor maps do not know a stride of 0
+        const bool spread = T == 0 || ((B == 1 || v.strideB > 0) && (p->nh_kv == 1 || v.strideH > 0) && (T == 1 || v.strideM > 0));
+        return rc != HK_OK ? rc : spread ? HK_OK : (int)HK_ERR_UNSUPPORTED;
+    };
+    if ((rc = keys(p->Kp, 1, p->prefix_len)) || (rc = keys(p->Vp, 1, p->prefix_len)) || (rc = keys(p->K, p->B, p->kv_len)) || (rc = keys(p->V, p->B, p->kv_len))) return rc;
     if (!p->LSE) return HK_ERR_NULL_POINTER;
     if ((reinterpret_cast<uintptr_t>(p->LSE) | reinterpret_cast<uintptr_t>(p->lengths)) & 3u) return HK_ERR_MISALIGNED;
     return HK_OK;
@@ -35,15 +80,12 @@ struct Plan {
     bool prefix_many, own_many;  // which kernels
     bool whole;                  // a block of rows takes the prefix and the request's own keys in one go
 };
-// a view that a tensor map can describe
-bool mappable(const hk_view& v, int64_t B, int64_t H, int64_t T) { return (B == 1 || v.strideB > 0) && (H == 1 || v.strideH > 0) && (T == 1 || v.strideM > 0); }
-
-Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a, bool many) {
+Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
     a.B = p->B; a.Hk = p->nh_kv; a.group = p->nh / p->nh_kv; a.T = (int)p->T; a.P = (int)p->prefix_len; a.S = (int)p->kv_len;
     a.R = p->B * a.T * a.group;
     const int own_rows = a.T * a.group, sms = sm_count();
     const ManyPlan mp = many_plan(p->dtype);
-    Plan plan{many && a.P > 0 && a.R > 32, many && own_rows > 16, false};
+    Plan plan{a.P > 0 && a.R > 32, own_rows > 16, false};
     a.splits_p = a.per_p = a.tiles_p = 0;
     double prefix_time = 0.0;
     if (a.P > 0 && plan.prefix_many) {
@@ -67,7 +109,7 @@ Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a, bool many) {
         a.per_p = cdiv(cdiv(a.P, n), fp.step) * fp.step;
         a.splits_p = cdiv(a.P, a.per_p);
     }
-    a.splits_o = 1;
+    a.splits_o = a.S > 0 || a.P == 0;  // without keys of their own, the prefix alone
     if (plan.own_many) {
         a.tiles_o = cdiv(own_rows, mp.rows);
         const int64_t items = (int64_t)a.B * a.Hk * a.tiles_o;
@@ -76,19 +118,40 @@ Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a, bool many) {
         if (a.P > 0 && plan.prefix_many && whole <= prefix_time + 4) {
             plan.whole = true;
             a.splits_p = a.per_p = a.tiles_p = 0;
+            a.splits_o = 1;
         }
     } else {
         const FewPlan fo = few_plan(p->dtype, own_rows);
         a.tiles_o = cdiv(own_rows, fo.rows);
         const int64_t items = (int64_t)a.B * a.Hk * a.tiles_o, places = sms * fo.per_sm;
-        while (a.splits_o < 8 && items * a.splits_o * 2 <= places && a.splits_o * 2 * 2 * fo.step <= a.S) a.splits_o *= 2;
+        while (a.splits_o > 0 && a.splits_o < 16 && items * a.splits_o * 2 <= places && a.splits_o * 2 * 4 * fo.step <= a.S) a.splits_o *= 2;
     }
+    a.slots = a.splits_p + a.splits_o;
     return plan;
 }
-size_t slots(const PrefixArgs& a) { return (size_t)a.splits_p * a.Hk * a.R; }
+// rows of slots in the workspace
+size_t slot_rows(const PrefixArgs& a) { return a.slots > 1 ? (size_t)a.slots * a.Hk * a.R : 0; }
 constexpr size_t SLOT_BYTES = 64 * sizeof(float) + sizeof(float2);
 
 }  // namespace
+
+int prefix_tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, int rows, bool mn_major) {
+    if (T == 0) {
+        memset(map, 0, sizeof(*map));  // no tile of it is loaded
+        return HK_OK;
+    }
+    const int64_t sM = T == 1 ? HEAD_DIM : v.strideM, sH = H == 1 ? sM * T : v.strideH, sB = B == 1 ? std::max(sH * H, sM * T) : v.strideB;
+    if (dtype == HK_F32) return make_tile_map(map, static_cast<const float*>(v.ptr), HEAD_DIM, (int)B, H, T, sB, sM, sH, rows, mn_major);
+    EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return HK_ERR_CUDA;
+    cuuint64_t dims[5] = {HEAD_DIM, (cuuint64_t)T, 1, (cuuint64_t)H, (cuuint64_t)B};
+    cuuint64_t strides[4] = {(cuuint64_t)sM * 2, 128, (cuuint64_t)sH * 2, (cuuint64_t)sB * 2};
+    cuuint32_t box[5] = {HEAD_DIM, (cuuint32_t)rows, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+    const CUresult r = enc(map, dtype == HK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, v.ptr, dims, strides, box, ones,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HK_OK : HK_ERR_CUDA;
+}
+
 }  // namespace hk
 
 using namespace hk;
@@ -98,12 +161,8 @@ extern "C" {
 size_t hk_shared_prefix_workspace_bytes(const hk_shared_prefix_params* p) {
     if (check_sizes(p) != HK_OK) return 0;
     PrefixArgs a{};
-    size_t n = 0;
-    for (bool many : {false, true}) {  // by sizes alone: whichever the views allow
-        make_plan(p, a, many);
-        n = std::max(n, slots(a));
-    }
-    return n * SLOT_BYTES;
+    make_plan(p, a);
+    return slot_rows(a) * SLOT_BYTES;
 }
 
 int hk_shared_prefix_attention(const hk_shared_prefix_params* p, void* stream_) {
@@ -111,9 +170,8 @@ int hk_shared_prefix_attention(const hk_shared_prefix_params* p, void* stream_) 
     if (rc != HK_OK) return rc;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     PrefixArgs a{};
-    const Plan plan = make_plan(p, a, (p->prefix_len == 0 || (mappable(p->Kp, 1, p->nh_kv, p->prefix_len) && mappable(p->Vp, 1, p->nh_kv, p->prefix_len))) &&
-                                          (p->kv_len == 0 || (mappable(p->K, p->B, p->nh_kv, p->kv_len) && mappable(p->V, p->B, p->nh_kv, p->kv_len))));
-    const size_t n = slots(a);
+    const Plan plan = make_plan(p, a);
+    const size_t n = slot_rows(a);
     if (n > 0 && (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) || p->workspace_bytes < n * SLOT_BYTES)) return HK_ERR_WORKSPACE;
     a.part = static_cast<float*>(p->workspace);
     a.ml = reinterpret_cast<float2*>(a.part + n * 64);
@@ -123,8 +181,17 @@ int hk_shared_prefix_attention(const hk_shared_prefix_params* p, void* stream_) 
     a.scale_log2e = std::fabs(p->scale) * LOG2E;
     a.flip = p->scale > 0.f ? 0u : p->dtype == HK_F32 ? 0x80000000u : 0x80008000u;
     a.causal = p->is_causal;
+    a.status = device_status_ptr();
+    if (!a.status) return HK_ERR_CUDA;
     if (a.splits_p > 0 && (rc = plan.prefix_many ? launch_prefix_many(a, p->dtype, stream) : launch_prefix_few(a, p->dtype, stream))) return rc;
-    return plan.own_many ? launch_own_many(a, p->dtype, plan.whole, stream) : launch_own_few(a, p->dtype, stream);
+    if (a.splits_o > 0 && (rc = plan.own_many ? launch_own_many(a, p->dtype, plan.whole, stream) : launch_own_few(a, p->dtype, stream))) return rc;
+    if (a.slots == 1) return HK_OK;
+    typedef void (*Kernel)(PrefixArgs);
+    static const Kernel combine[] = {prefix_combine_kernel<float>, prefix_combine_kernel<__nv_bfloat16>, prefix_combine_kernel<__half>};
+    LaunchConfig lc((unsigned)cdiv((int64_t)a.Hk * a.R, 8), 128, 0, stream, 1, true);
+    if (cudaLaunchKernelEx(&lc.cfg, combine[p->dtype], a) != cudaSuccess) return check_launch();
+    count_launch();
+    return HK_OK;
 }
 
 }  // extern "C"

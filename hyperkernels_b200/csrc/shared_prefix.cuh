@@ -6,9 +6,9 @@
 namespace hk {
 
 // The rows of a key head: row r = (b * T + i) * group + g is token i of request b under query head kvh * group + g, so that a
-// request's rows follow each other; R of them.  What a run of the prefix's keys gives for row kvh * R + r is left in the
-// workspace: the maximum and the sum of its weights (log2 units), and the weighted sum of the values.  The kernel that takes
-// the request's own keys adds the runs up in their order.
+// request's rows follow each other; R of them.  What a run of keys, of the prefix or of a request's own, gives for row
+// kvh * R + r is left in a slot of the workspace: the maximum and the sum of its weights (log2 units), and the weighted sum of
+// the values.  The last kernel adds the slots of a row in their order.
 struct PrefixArgs {
     hk_view Q, Kp, Vp, K, V, O;
     float* LSE;
@@ -21,8 +21,10 @@ struct PrefixArgs {
     int causal;
     int splits_p, per_p, tiles_p;  // over the prefix: runs of keys, keys of a run, row tiles of a key head
     int splits_o, tiles_o;         // over the requests' own keys
-    float2* ml;                    // [splits_p][Hk * R]
+    int slots;                     // of a row; one: the result is written where it is worked out
+    float2* ml;                    // [slots][Hk * R]
     float* part;                   // the same, [64]
+    DeviceStatus* status;
 };
 
 template <class X>
@@ -34,9 +36,19 @@ __device__ __forceinline__ int request_keys(const PrefixArgs& a, int b) { return
 // own keys that token t of a request of `len` keys sees
 __device__ __forceinline__ int token_keys(const PrefixArgs& a, int len, int t) { return a.causal ? min(len, max(0, len - a.T + t + 1)) : len; }
 
+template <class X>
+__device__ __forceinline__ void store4(X* p, float4 v) {
+    if constexpr (sizeof(X) == 4) *reinterpret_cast<float4*>(p) = v;
+    else *reinterpret_cast<uint2*>(p) = make_uint2(pack<X>(v.x, v.y), pack<X>(v.z, v.w));
+}
+
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Launchers.  The kernel over the requests' own keys starts under the tail of the one over the prefix.
+// Tiles of `rows` rows of a view of keys or values, all heads and batches (tma_load_tile): 128 bytes of each row side by side,
+// swizzled; fp32 rows are two such pieces.  mn_major: the values as an MN-major operand of fp32 products.
+int prefix_tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, int rows, bool mn_major);
+
+// Launchers.  The kernel over the requests' own keys runs beside the one over the prefix, if that is launched just before it.
 struct FewPlan {
     int rows;      // rows of a tile: 1, 2 (fp32 arithmetic lane by lane) or 16 (matrix instructions)
     int step;      // keys that a CTA takes at once

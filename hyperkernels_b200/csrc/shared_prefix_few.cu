@@ -1,14 +1,14 @@
 // shared_prefix_few.cu -- attention over a shared prefix where few rows meet a run of keys (decoding): bound by reading keys and
 // values.
 //
-// A warp takes its rows through batches of keys.  Every lane copies (cp.async) the very bytes it will work on into 16-byte slots
-// of its own, FEW_STAGES - 1 batches ahead, and waits for its own copies alone: no barrier until the warps merge what they have.
-// An SM has up to 12 warps x 12 KB on their way, four times what its share of the memory's latency takes.
+// A warp takes its rows through batches of keys that TMA brings into a ring of its own, two or three batches ahead: no barrier
+// between warps until they merge what they have.  (Copies by the lanes themselves, cp.async, kept the load/store unit busy for 112
+// cycles a batch and warp, which was what the kernel took: 28 us instead of 16 for the own keys of 64 requests, 4 rows, bf16.)
 //   One or two rows in fp32: a half-warp to a key, four elements a lane (RowsOfOne).
 //   Up to 16 rows: matrix instructions (m16n8k8 on TF32, m16n8k16 on 16-bit types).  A lane's part of an operand is whatever
-// 16-byte pieces it loads, because the order of the contracted index (head dimension, keys) and of the result's columns is free
-// as long as both operands agree on it.  The instructions on tensor memory would need 128 rows to a tile.
-//   The requests' own keys: a cluster of CTAs shares them by the keys there are, adds up the prefix's runs and writes the result.
+// 16-byte pieces it reads, because the order of the contracted index (head dimension, keys) and of the result's columns is free
+// as long as both operands agree on it; the order taken makes every read free of bank conflicts in the layout TMA writes (16-byte
+// piece c of row r at c ^ (r % 8)).  The instructions on tensor memory would need 128 rows to a tile.
 #include <cmath>
 #include <mutex>
 #include <type_traits>
@@ -38,22 +38,33 @@ __device__ __forceinline__ uint32_t tf32_high(uint32_t x) { return x & 0xffffe00
 __device__ __forceinline__ uint32_t tf32_low(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf32_high(x))); }
 
 
-constexpr int FEW_WARPS = 4, FEW_STAGES = 4;
+constexpr int FEW_WARPS = 4;
 
 // fp32: x = h + l with h the upper 11 bits of the significand; a product is h h' + h l' + l h', added from the small ones on: what
 // is left out is 2^-22 of it.  A batch's weighted values are added to the rest in fp32 adds, since the tensor core's own additions
 // cut off instead of rounding.
 // Lane (g, c) = (lane / 4, lane % 4) of a matrix instruction: rows g and g + 8, columns and contracted elements by c.
+// Which of eight keys (or pieces of a row) column n stands for: neighbours are four apart, so that the eight lanes that read at once
+// meet all banks.
+__device__ __forceinline__ int order(int n) { return (n >> 1) | ((n & 1) << 2); }
 template <class X>
 struct FewMath;
 template <>
 struct FewMath<float> {
     static constexpr int KEYS = 8;
-    uint4 k[4], v[4];  // k: key g, elements 16 i + 4 c ..; v: keys 2 c, 2 c, 2 c + 1, 2 c + 1, elements 4 g .. and 32 + 4 g ..
-    static __device__ __forceinline__ int key_k(int, int g) { return g; }
-    static __device__ __forceinline__ int at_k(int i, int c) { return 16 * i + 4 * c; }
-    static __device__ __forceinline__ int key_v(int i, int c) { return 2 * c + (i >> 1); }
-    static __device__ __forceinline__ int at_v(int i, int g) { return 32 * (i & 1) + 4 * g; }
+    // Column n of the scores is key order(n); column n of the result has elements 4 order(n) .. and 32 + 4 order(n) ..
+    uint4 k[4], v[4];  // k: key order(g), elements 16 i + 4 c ..; v: keys c, c, c + 4, c + 4
+    __device__ __forceinline__ void read_k(const uint8_t* at, int g, int c) {  // two boxes of 128 bytes of each row
+        const int key = order(g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const uint4*>(at + (i >> 1) * 1024 + key * 128 + ((((i & 1) * 4 + c) ^ key) << 4));
+    }
+    __device__ __forceinline__ void read_v(const uint8_t* at, int g, int c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(at + (i & 1) * 1024 + key_v(i, c) * 128 + ((order(g) ^ key_v(i, c)) << 4));
+    }
+    static __device__ __forceinline__ int key_v(int i, int c) { return c + 4 * (i >> 1); }
+    static __device__ __forceinline__ int key_s(int, int c, int e) { return c + 4 * (e & 1); }  // of a lane's scores
     uint32_t qh[8][4], ql[8][4];
     __device__ __forceinline__ void load_q(const float* lo, const float* hi, int c, uint32_t flip) {
 #pragma unroll
@@ -70,7 +81,7 @@ struct FewMath<float> {
                 }
         }
     }
-    // s: rows g, g + 8 of keys 2 c, 2 c + 1
+    // s: rows g, g + 8 of columns 2 c, 2 c + 1
     __device__ __forceinline__ void scores(float (&s)[1][4]) const {
         uint32_t b[16], bl[16];
 #pragma unroll
@@ -95,12 +106,12 @@ struct FewMath<float> {
 #pragma unroll
         for (int x = 0; x < 8; ++x) mma_tf32(s[0], qh[x], b[2 * x], b[2 * x + 1]);
     }
-    // o[j] = alpha o[j] + p V: rows g, g + 8 of columns n = 2 c, 2 c + 1, element 4 n + j or 32 + 4 n + j - 4
+    // o[j] = alpha o[j] + p V: rows g, g + 8 of columns n = 2 c, 2 c + 1
     __device__ __forceinline__ void weigh(const float (&p)[1][4], const float (&alpha)[2], bool, float (&o)[8][4]) const {
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t x = __float_as_uint(p[0][(e & 1) * 2 + (e >> 1)]);  // rows g, g + 8 of key 2 c, then of 2 c + 1
+            const uint32_t x = __float_as_uint(p[0][(e & 1) * 2 + (e >> 1)]);  // rows g, g + 8 of key c, then of c + 4
             ph[e] = tf32_high(x);
             pl[e] = tf32_low(x);
         }
@@ -117,16 +128,24 @@ struct FewMath<float> {
             for (int e = 0; e < 4; ++e) o[j][e] = fmaf(o[j][e], alpha[e >> 1], t[e]);
         }
     }
-    static __device__ __forceinline__ int column(int j, int n) { return (j < 4 ? 0 : 28) + 4 * n + j; }
+    static __device__ __forceinline__ int column(int j, int n) { return (j < 4 ? 0 : 28) + 4 * order(n) + j; }
 };
 template <class X>
 struct FewMath {
     static constexpr int KEYS = 16;
-    uint4 k[4], v[4];  // k: keys g, g, 8 + g, 8 + g, elements 32 (i & 1) + 8 c ..; v: keys 2 c, 2 c + 1, 8 + 2 c, 8 + 2 c + 1, elements 8 g ..
-    static __device__ __forceinline__ int key_k(int i, int g) { return g + 8 * (i >> 1); }
-    static __device__ __forceinline__ int at_k(int i, int c) { return 32 * (i & 1) + 8 * c; }
-    static __device__ __forceinline__ int key_v(int i, int c) { return 2 * c + (i & 1) + 8 * (i >> 1); }
-    static __device__ __forceinline__ int at_v(int, int g) { return 8 * g; }
+    // Column n of scores t is key 8 t + order(n); column n of the result has elements 8 order(n) ..
+    uint4 k[4], v[4];  // k: keys order(g), order(g), 8 + order(g) twice, elements 32 (i & 1) + 8 c ..; v: keys c, c + 4, 8 + c, 12 + c
+    __device__ __forceinline__ void read_k(const uint8_t* at, int g, int c) {
+        const int key = order(g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const uint4*>(at + ((i >> 1) * 8 + key) * 128 + ((((i & 1) * 4 + c) ^ key) << 4));
+    }
+    __device__ __forceinline__ void read_v(const uint8_t* at, int g, int c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(at + key_v(i, c) * 128 + ((order(g) ^ (key_v(i, c) & 7)) << 4));
+    }
+    static __device__ __forceinline__ int key_v(int i, int c) { return c + 4 * i; }
+    static __device__ __forceinline__ int key_s(int t, int c, int e) { return 8 * t + c + 4 * (e & 1); }
     uint32_t q[4][4];
     __device__ __forceinline__ void load_q(const X* lo, const X* hi, int c, uint32_t flip) {
 #pragma unroll
@@ -139,7 +158,7 @@ struct FewMath {
             for (int e = 0; e < 8; ++e) q[2 * i + (e >> 2)][e & 3] ^= flip;
         }
     }
-    // s[t]: rows g, g + 8 of keys 8 t + 2 c, 8 t + 2 c + 1
+    // s[t]: rows g, g + 8 of columns 2 c, 2 c + 1
     __device__ __forceinline__ void scores(float (&s)[2][4]) const {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -167,7 +186,7 @@ struct FewMath {
             mma_16<X>(o[j], a, __byte_perm(w[0], w[1], j & 1 ? 0x7632 : 0x5410), __byte_perm(w[2], w[3], j & 1 ? 0x7632 : 0x5410));
         }
     }
-    static __device__ __forceinline__ int column(int j, int n) { return 8 * n + j; }
+    static __device__ __forceinline__ int column(int j, int n) { return 8 * order(n) + j; }
 };
 
 
@@ -177,11 +196,7 @@ struct RowsOf16 {
     typedef T X;
     typedef FewMath<X> Math;
     static constexpr int ROWS = 16, KEYS = Math::KEYS, PARTS = 1, NT = KEYS / 8;
-    static __device__ __forceinline__ int key_k(int i, int lane) { return Math::key_k(i, lane >> 2); }
-    static __device__ __forceinline__ int at_k(int i, int lane) { return Math::at_k(i, lane & 3); }
-    static __device__ __forceinline__ int key_v(int i, int lane) { return Math::key_v(i, lane & 3); }
-    static __device__ __forceinline__ int at_v(int i, int lane) { return Math::at_v(i, lane >> 2); }
-
+    static constexpr int STAGES = sizeof(T) == 4 ? 4 : 3, CTAS = sizeof(T) == 4 ? 3 : 4;  // of the ring; CTAs that an SM holds
     Math f;
     int limit[2];
     float o[8][4], m[2], l[2];
@@ -197,24 +212,22 @@ struct RowsOf16 {
     }
     static __device__ __forceinline__ int row(int i, int lane) { return (lane >> 2) + 8 * i; }
     template <class F>
-    __device__ __forceinline__ void batch(const uint4 (*from)[32], int lane, int key0, int end, float scale_log2e, F&& copy_next) {
-        const int c = lane & 3;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f.k[i] = from[i][lane];
+    __device__ __forceinline__ void batch(const uint8_t* from, int lane, int key0, int end, float scale_log2e, F&& copy_next) {
+        const int g = lane >> 2, c = lane & 3;
+        f.read_k(from, g, c);
         float s[NT][4];
         f.scores(s);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f.v[i] = from[4 + i][lane];
+        f.read_v(from + 2048, g, c);
         copy_next();
         if (!__all_sync(0xffffffffu, key0 + KEYS <= min(limit[0], limit[1]))) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (key0 + 8 * t + 2 * c + (e & 1) >= limit[e >> 1]) s[t][e] = -INFINITY;
+                    if (key0 + Math::key_s(t, c, e) >= limit[e >> 1]) s[t][e] = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)  // copies of the last key: no weight, but the matrix instruction multiplies
-                if (key0 + key_v(i, lane) >= end) f.v[i] = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 4; ++i)  // what is behind the last key may be anything: it has no weight, but 0 times a NaN is one
+                if (key0 + Math::key_v(i, c) >= end) f.v[i] = make_uint4(0, 0, 0, 0);
         }
         float mx[2] = {-INFINITY, -INFINITY}, alpha[2], ref[2];
 #pragma unroll
@@ -242,31 +255,6 @@ struct RowsOf16 {
             }
         f.weigh(s, alpha, __any_sync(0xffffffffu, raised), o);
     }
-    // a run of the prefix's keys
-    __device__ __forceinline__ void fold(const float2* ml, const float* part, int rows, int lane) {
-        const int c = lane & 3;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = row(i, lane);
-            if (r >= rows) continue;
-            const float2 x = ml[r];
-            float4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const float4*>(part + (int64_t)r * 64 + Math::column((k >> 1) * 4, 2 * c + (k & 1)));
-            const float mn = fmaxf(m[i], x.x), ref = mn == -INFINITY ? 0.f : mn, p = ex2_approx(m[i] - ref), w = ex2_approx(x.x - ref);
-            m[i] = mn;
-            l[i] = l[i] * p + (c == 0 ? x.y * w : 0.f);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float y[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float& z = o[(k >> 1) * 4 + e][2 * i + (k & 1)];
-                    z = fmaf(y[e], w, z * p);
-                }
-            }
-        }
-    }
     template <class P>
     __device__ __forceinline__ void finish(P* part, float2 (*ml)[ROWS], int warp, int lane) {
         const int c = lane & 3;
@@ -291,11 +279,12 @@ struct RowsOf16 {
 template <int N>
 struct RowsOfOne {
     typedef float X;
-    static constexpr int ROWS = N, KEYS = 8, PARTS = 2;
-    static __device__ __forceinline__ int key_k(int i, int lane) { return 2 * i + (lane >> 4); }
-    static __device__ __forceinline__ int at_k(int, int lane) { return 4 * (lane & 15); }
-    static __device__ __forceinline__ int key_v(int i, int lane) { return key_k(i, lane); }
-    static __device__ __forceinline__ int at_v(int, int lane) { return 4 * (lane & 15); }
+    static constexpr int ROWS = N, KEYS = 8, PARTS = 2, STAGES = 3, CTAS = 4;
+    // a lane's piece of key i of its half-warp
+    static __device__ __forceinline__ float4 piece(const uint8_t* at, int i, int lane) {
+        const int key = 2 * i + (lane >> 4);
+        return *reinterpret_cast<const float4*>(at + ((lane >> 3) & 1) * 1024 + key * 128 + (((lane & 7) ^ key) << 4));
+    }
 
     float4 q[N], o[N];
     float m[N], l[N];
@@ -316,13 +305,13 @@ struct RowsOfOne {
         }
     }
     template <class F>
-    __device__ __forceinline__ void batch(const uint4 (*from)[32], int lane, int key0, int end, float scale_log2e, F&& copy_next) {
+    __device__ __forceinline__ void batch(const uint8_t* from, int lane, int key0, int end, float scale_log2e, F&& copy_next) {
         const bool b3 = lane & 8, b2 = lane & 4;
         float s[N];
         {
             float4 k[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) k[i] = reinterpret_cast<const float4&>(from[i][lane]);
+            for (int i = 0; i < 4; ++i) k[i] = piece(from, i, lane);
 #pragma unroll
             for (int r = 0; r < N; ++r) {
                 float d[4];
@@ -338,13 +327,13 @@ struct RowsOfOne {
         }
         float4 v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = reinterpret_cast<const float4&>(from[4 + i][lane]);
+        for (int i = 0; i < 4; ++i) v[i] = piece(from + 2048, i, lane);
         copy_next();
         const int key = key0 + (b3 ? 4 : 0) + (b2 ? 2 : 0) + (lane >> 4);
         if (key0 + KEYS > end) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (key0 + key_v(i, lane) >= end) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (key0 + 2 * i + (lane >> 4) >= end) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
         for (int r = 0; r < N; ++r) {
@@ -363,24 +352,11 @@ struct RowsOfOne {
             }
         }
     }
-    __device__ __forceinline__ void fold(const float2* ml, const float* part, int rows, int lane) {
-#pragma unroll
-        for (int r = 0; r < N; ++r) {
-            if (r >= rows) continue;
-            const float2 x = ml[r];
-            const float4 v = *reinterpret_cast<const float4*>(part + r * 64 + 4 * (lane & 15));
-            const float mn = fmaxf(m[r], x.x), ref = mn == -INFINITY ? 0.f : mn, p = ex2_approx(m[r] - ref), w = ex2_approx(x.x - ref);
-            m[r] = mn;
-            l[r] = l[r] * p + ((lane & 15) == 0 ? x.y * w : 0.f);
-            o[r].x = fmaf(v.x, w, o[r].x * p); o[r].y = fmaf(v.y, w, o[r].y * p); o[r].z = fmaf(v.z, w, o[r].z * p); o[r].w = fmaf(v.w, w, o[r].w * p);
-        }
-    }
     template <class P>
     __device__ __forceinline__ void finish(P* part, float2 (*ml)[ROWS], int warp, int lane) {
         const int at = 2 * warp + (lane >> 4);
 #pragma unroll
         for (int r = 0; r < N; ++r) {
-            // every key's weight is in four lanes, a run of the prefix in lane 0 and so in one of the four sums
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 8);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 4);
             if ((lane & 15) == 0) ml[at][r] = make_float2(m[r], l[r]);
@@ -393,95 +369,91 @@ template <class Rows>
 struct FewShared {
     static constexpr int PARTS = FEW_WARPS * Rows::PARTS;
     union {
-        uint4 ring[FEW_WARPS][FEW_STAGES][8][32];
+        uint8_t ring[FEW_WARPS][Rows::STAGES][4096];  // a batch's keys and values
         float part[PARTS][Rows::ROWS][64 + 4];
     };
     float2 ml[PARTS][Rows::ROWS];
-    float merged[Rows::ROWS][64 + 4];  // of the CTA, for the others of its cluster
-    float2 merged_ml[Rows::ROWS];
+    uint64_t full[FEW_WARPS][Rows::STAGES];
+    Abort abort;
 };
 
-__device__ __forceinline__ void copy16(void* smem, const void* src) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(src) : "memory");
-}
-template <class X>
-__device__ __forceinline__ void store4(X* p, float4 v) {
-    if constexpr (sizeof(X) == 4) *reinterpret_cast<float4*>(p) = v;
-    else *reinterpret_cast<uint2*>(p) = make_uint2(pack<X>(v.x, v.y), pack<X>(v.z, v.w));
-}
+// A CTA takes a run of the prefix's keys or (OWN) of a request's own, by the keys there are.
+constexpr int W_FEW = 401;
 
-// OWN: a cluster takes a request's own keys, adds the runs of the prefix and writes the result.  Otherwise: a CTA takes a run of
-// the prefix and leaves its partial result.
 template <class Rows, bool OWN>
-__global__ void __launch_bounds__(FEW_WARPS * 32, 3) prefix_few_kernel(const __grid_constant__ PrefixArgs a) {
+__global__ void __launch_bounds__(FEW_WARPS * 32, Rows::CTAS) prefix_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefixArgs a) {
     typedef typename Rows::X X;
     constexpr int N = Rows::ROWS, KEYS = Rows::KEYS, STEP = FEW_WARPS * KEYS, MINE = N < 16 ? N : 2;  // rows that a lane works on
-    extern __shared__ __align__(16) uint8_t few_smem[];
+    extern __shared__ __align__(1024) uint8_t few_smem[];
     FewShared<Rows>& sh = *reinterpret_cast<FewShared<Rows>*>(few_smem);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (!OWN || a.splits_p == 0) {
-        pdl_wait();
-        pdl_trigger();
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (lane == 0) {
+        for (int s = 0; s < Rows::STAGES; ++s) mbar_init(&sh.full[warp][s], 1);
+        if (warp == 0) sh.abort.id = 0;
+        fence_mbar_init();
     }
+    // Over the requests' own keys: starts under the tail of the kernel over the prefix.  What was before that is complete then.
+    const bool late = OWN && a.splits_p > 0;
+    if (!late) pdl_wait();
+    pdl_trigger();
+    const int32_t all_keys = OWN && a.lengths ? __ldg(a.lengths + blockIdx.x / a.splits_o / a.tiles_o / a.Hk) : a.S;
     // the rows
     const int ns = OWN ? a.splits_o : a.splits_p, item = blockIdx.x / ns, split = blockIdx.x - item * ns;
     const int tiles = OWN ? a.tiles_o : a.tiles_p, at = item / tiles, tile = item - at * tiles;
     const int b = OWN ? at / a.Hk : 0, kvh = at - b * a.Hk;
     const int all = OWN ? a.T * a.group : a.R, row0 = b * a.T * a.group + tile * N, rows = min(N, all - tile * N);
-    // the keys
-    int len = a.P, begin = split * a.per_p, end = min(a.P, begin + a.per_p);
-    if (OWN) {
-        len = request_keys(a, b);
-        const int seen = token_keys(a, len, (tile * N + rows - 1) / a.group), per = ((seen + ns - 1) / ns + KEYS - 1) / KEYS * KEYS;
-        begin = min(seen, split * per);
-        end = min(seen, begin + per);
-    }
-    const int64_t stride_k = OWN ? a.K.strideM : a.Kp.strideM, stride_v = OWN ? a.V.strideM : a.Vp.strideM;
-    const X* K = OWN ? row_of<X>(a.K, b, kvh, 0) : row_of<X>(a.Kp, 0, kvh, 0);
-    const X* V = OWN ? row_of<X>(a.V, b, kvh, 0) : row_of<X>(a.Vp, 0, kvh, 0);
-    int put = 0, put_key = begin + warp * KEYS;
-    auto copy_next = [&] {  // the next batch of this warp, if there is one (behind the end the last key again); a group either way
-        if (put_key < end) {
-            uint4(*to)[32] = sh.ring[warp][put];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) copy16(&to[i][lane], K + min(put_key + Rows::key_k(i, lane), end - 1) * stride_k + Rows::at_k(i, lane));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) copy16(&to[4 + i][lane], V + min(put_key + Rows::key_v(i, lane), end - 1) * stride_v + Rows::at_v(i, lane));
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        put_key += STEP;
-        put = put + 1 == FEW_STAGES ? 0 : put + 1;
-    };
-#pragma unroll
-    for (int i = 0; i < FEW_STAGES - 1; ++i) copy_next();
     Rows w;
+    int token_of[MINE];
     {
         const X* q[MINE];
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
-            const int r = Rows::row(i, lane), row = row0 + r, token = row / a.group, bq = OWN ? b : token / a.T, t = token - bq * a.T;
-            q[i] = r < rows ? row_of<X>(a.Q, bq, kvh * a.group + (row - token * a.group), t) : nullptr;
-            w.limit[i] = OWN && r < rows ? min(end, token_keys(a, len, t)) : end;
+            const int r = Rows::row(i, lane), row = row0 + r, token = row / a.group, bq = OWN ? b : token / a.T;
+            token_of[i] = r < rows ? token - bq * a.T : a.T;
+            q[i] = r < rows ? row_of<X>(a.Q, bq, kvh * a.group + (row - token * a.group), token_of[i]) : nullptr;
         }
         w.start(q, a.flip, lane);
     }
+    // the keys
+    int len = a.P, begin = split * a.per_p, end = min(a.P, begin + a.per_p);
+    if (OWN) {
+        len = min(max(all_keys, 0), a.S);
+        const int seen = token_keys(a, len, (tile * N + rows - 1) / a.group), per = ((seen + ns - 1) / ns + KEYS - 1) / KEYS * KEYS;
+        begin = min(seen, split * per);
+        end = min(seen, begin + per);
+    }
+    int put = 0, put_key = begin + warp * KEYS;
+    auto copy_next = [&] {  // the next batch of this warp, if there is one, into the slot that its lanes have read
+        __syncwarp();
+        if (put_key < end && lane == 0) {
+            uint64_t* full = &sh.full[warp][put];
+            uint8_t* to = sh.ring[warp][put];
+            mbar_arrive_expect_tx(full, 4096);
+            tma_load_tile(to, &map_k, full, put_key, kvh, b);
+            tma_load_tile(to + 2048, &map_v, full, put_key, kvh, b);
+        }
+        put_key += STEP;
+        put = put + 1 == Rows::STAGES ? 0 : put + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < Rows::STAGES - 1; ++i) copy_next();
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) w.limit[i] = OWN && token_of[i] < a.T ? min(end, token_keys(a, len, token_of[i])) : end;
+    __syncthreads();  // the record of waits that gave up
+    WaitNote wc{&sh.abort};
     int get = 0;
+    uint32_t phase = 0;
     for (int key0 = begin + warp * KEYS; key0 < end; key0 += STEP) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(FEW_STAGES - 2) : "memory");
-        const uint4(*from)[32] = sh.ring[warp][get];
-        get = get + 1 == FEW_STAGES ? 0 : get + 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.full[warp][get], phase, W_FEW, key0))) {
+            for (const unsigned long long t0 = globaltimer_ns(); globaltimer_ns() - t0 < 100000ull;) {}  // copies in flight land
+            break;
+        }
+        const uint8_t* from = sh.ring[warp][get];
+        if (++get == Rows::STAGES) get = 0, phase ^= 1u;
         w.batch(from, lane, key0, end, a.scale_log2e, copy_next);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     const int64_t slot0 = (int64_t)kvh * a.R + row0, slot_rows = (int64_t)a.Hk * a.R;
-    if (OWN && a.splits_p > 0) {
-        pdl_wait();  // for the kernel over the prefix; what was before it was complete when this one began
-        pdl_trigger();
-        const int part = Rows::PARTS == 2 ? 2 * warp + (lane >> 4) : warp;
-        for (int s = split * FewShared<Rows>::PARTS + part; s < a.splits_p; s += ns * FewShared<Rows>::PARTS)
-            w.fold(a.ml + s * slot_rows + slot0, a.part + (s * slot_rows + slot0) * 64, rows, lane);
-    }
-    __syncthreads();  // the ring is the warps' exchange now
+    __syncthreads();  // the ring is the warps' exchange now: every copy has been waited for
     w.finish(sh.part, sh.ml, warp, lane);
     __syncthreads();
     // PER threads a row, 64 / PER elements each
@@ -503,53 +475,24 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 3) prefix_few_kernel(const __g
             for (int e = 0; e < E; ++e) acc[e] = fmaf(sh.part[p][r][d + e], f, acc[e]);
         }
     }
-    if (!OWN) {
-        if (!mine) return;
-        const int64_t to = split * slot_rows + slot0 + r;
+    if (threadIdx.x == 0) report_abort(sh.abort, a.status);
+    if (mine && a.slots > 1) {
+        const int64_t to = (OWN ? a.splits_p + split : split) * slot_rows + slot0 + r;
         if (d == 0) a.ml[to] = make_float2(M, L);
 #pragma unroll
         for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(a.part + to * 64 + d + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-        return;
-    }
-    if (ns > 1) {
-        if (mine) {
-            if (d == 0) sh.merged_ml[r] = make_float2(M, L);
-#pragma unroll
-            for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(&sh.merged[r][d + e]) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-        }
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-        if (split == 0 && mine)
-            for (int s = 1; s < ns; ++s) {
-                const float ms = ld_cluster_f(mapa(&sh.merged_ml[r].x, s)), ls = ld_cluster_f(mapa(&sh.merged_ml[r].y, s));
-                const float mn = fmaxf(M, ms), ref = mn == -INFINITY ? 0.f : mn, p = ex2_approx(M - ref), f = ex2_approx(ms - ref);
-                M = mn;
-                L = fmaf(ls, f, L * p);
-#pragma unroll
-                for (int e = 0; e < E; e += 4) {
-                    const float4 v = ld_cluster_f4(mapa(&sh.merged[r][d + e], s));
-                    acc[e] = fmaf(v.x, f, acc[e] * p); acc[e + 1] = fmaf(v.y, f, acc[e + 1] * p);
-                    acc[e + 2] = fmaf(v.z, f, acc[e + 2] * p); acc[e + 3] = fmaf(v.w, f, acc[e + 3] * p);
-                }
-            }
-    }
-    if (split == 0 && mine) {
+    } else if (mine) {
         const float f = L > 0.f ? 1.f / L : 0.f;
-        const int row = row0 + r, token = row / a.group, t = token - b * a.T, h = kvh * a.group + (row - token * a.group);
-        X* to = const_cast<X*>(row_of<X>(a.O, b, h, t)) + d;
+        const int row = row0 + r, token = row / a.group, bq = OWN ? b : token / a.T, t = token - bq * a.T, h = kvh * a.group + (row - token * a.group);
+        X* to = const_cast<X*>(row_of<X>(a.O, bq, h, t)) + d;
 #pragma unroll
         for (int e = 0; e < E; e += 4) store4(to + e, make_float4(acc[e] * f, acc[e + 1] * f, acc[e + 2] * f, acc[e + 3] * f));
-        if (d == 0) a.LSE[b * a.lse_sB + h * a.lse_sH + t] = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
+        if (d == 0) a.LSE[bq * a.lse_sB + h * a.lse_sH + t] = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
     }
-    if (ns > 1) {  // the others' results have been read
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-    }
+    if (late && blockIdx.x == gridDim.x - 1) pdl_wait();  // this kernel is complete when the one over the prefix is
 }
 
-typedef void (*FewKernel)(PrefixArgs);
+typedef void (*FewKernel)(CUtensorMap, CUtensorMap, PrefixArgs);
 struct FewEntry {
     FewKernel kernel;
     size_t smem;
@@ -565,7 +508,7 @@ FewEntry pick(int dtype, int rows) {
     return rows == 1 ? entry<RowsOfOne<1>, OWN>() : rows == 2 ? entry<RowsOfOne<2>, OWN>() : entry<RowsOf16<float>, OWN>();
 }
 
-int launch(const FewEntry& k, const PrefixArgs& a, int64_t blocks, int cluster, cudaStream_t stream) {
+int launch(const FewEntry& k, const PrefixArgs& a, int dtype, bool own, int64_t blocks, cudaStream_t stream) {
     // once per device and kernel: more than 48 KB of shared memory
     static std::mutex mu;
     static FewKernel known[HK_MAX_DEVICES][16];
@@ -582,8 +525,14 @@ int launch(const FewEntry& k, const PrefixArgs& a, int64_t blocks, int cluster, 
         }
     }
     if (blocks > 0x7fffffffLL) return HK_ERR_BAD_SHAPE;
-    LaunchConfig lc((unsigned)blocks, FEW_WARPS * 32, k.smem, stream, cluster, true);
-    if (cudaLaunchKernelEx(&lc.cfg, k.kernel, a) != cudaSuccess) return check_launch();
+    LaunchConfig lc((unsigned)blocks, FEW_WARPS * 32, k.smem, stream, 1, true);
+    CUtensorMap mk, mv;
+    const int rows = few_plan(dtype, 16).step / FEW_WARPS;
+    int rc;
+    if ((rc = own ? prefix_tile_map(&mk, a.K, dtype, a.B, a.Hk, a.S, rows, false) : prefix_tile_map(&mk, a.Kp, dtype, 1, a.Hk, a.P, rows, false)) ||
+        (rc = own ? prefix_tile_map(&mv, a.V, dtype, a.B, a.Hk, a.S, rows, false) : prefix_tile_map(&mv, a.Vp, dtype, 1, a.Hk, a.P, rows, false)))
+        return rc;
+    if (cudaLaunchKernelEx(&lc.cfg, k.kernel, mk, mv, a) != cudaSuccess) return check_launch();
     count_launch();
     return HK_OK;
 }
@@ -591,14 +540,14 @@ int launch(const FewEntry& k, const PrefixArgs& a, int64_t blocks, int cluster, 
 }  // namespace
 
 FewPlan few_plan(int dtype, int rows) {
-    if (dtype != HK_F32) return {16, FEW_WARPS * 16, 3};
-    return {rows <= 2 ? rows : 16, FEW_WARPS * 8, 3};
+    if (dtype != HK_F32) return {16, FEW_WARPS * 16, RowsOf16<__half>::CTAS};
+    return {rows <= 2 ? rows : 16, FEW_WARPS * 8, rows <= 2 ? RowsOfOne<1>::CTAS : RowsOf16<float>::CTAS};
 }
 int launch_prefix_few(const PrefixArgs& a, int dtype, cudaStream_t stream) {
-    return launch(pick<false>(dtype, few_plan(dtype, a.R).rows), a, (int64_t)a.Hk * a.tiles_p * a.splits_p, 1, stream);
+    return launch(pick<false>(dtype, few_plan(dtype, a.R).rows), a, dtype, false, (int64_t)a.Hk * a.tiles_p * a.splits_p, stream);
 }
 int launch_own_few(const PrefixArgs& a, int dtype, cudaStream_t stream) {
-    return launch(pick<true>(dtype, few_plan(dtype, a.T * a.group).rows), a, (int64_t)a.B * a.Hk * a.tiles_o * a.splits_o, a.splits_o, stream);
+    return launch(pick<true>(dtype, few_plan(dtype, a.T * a.group).rows), a, dtype, true, (int64_t)a.B * a.Hk * a.tiles_o * a.splits_o, stream);
 }
 
 }  // namespace hk

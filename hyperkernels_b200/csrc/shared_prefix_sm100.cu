@@ -12,7 +12,6 @@
 // a tile comes back into registers and is added there in fp32: the tensor core's additions cut off instead of rounding, and over
 // thousands of keys in one accumulator that would be seen.
 #include <cmath>
-#include <cstring>
 #include <mutex>
 #include <type_traits>
 
@@ -76,10 +75,9 @@ enum ManyWait { W_Q = 301, W_KV, W_READY, W_EMPTY, W_S, W_P, W_O };
 
 struct ManyArgs {
     PrefixArgs p;
-    DeviceStatus* status;
-    int own;           // the request's own keys are part of it, and the result is final
-    int prefix;        // the prefix is: of a run if not `own`, of all keys otherwise
-    int late;          // started under the tail of the kernel over the prefix, whose runs are added
+    int own;           // the request's own keys are part of it
+    int prefix;        // the prefix is: a run of it if not `own`, all of it otherwise
+    int late;          // runs beside the kernel over the prefix; what was before that is complete when this one begins
     int tiles;         // items of row blocks: of a key head, or of a request's
 };
 
@@ -118,10 +116,8 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
         tmem_relinquish();
         tc_fence_before_sync();
     }
-    if (!args.late) {
-        pdl_wait();
-        pdl_trigger();
-    }
+    if (!args.late) pdl_wait();
+    pdl_trigger();
     // the item: rows
     const int ns = args.own ? 1 : a.splits_p, item = blockIdx.x / ns, split = blockIdx.x - item * ns, at = item / args.tiles;
     const int tile = args.tiles - 1 - (item - at * args.tiles);  // the last rows see the most keys
@@ -443,33 +439,17 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                 tmem_wait_ld();
             }
         }
-        if (args.late) {
-            pdl_wait();  // for the kernel over the prefix; what was before it was complete when this one began
-            pdl_trigger();
-        }
         if (valid && ok) {
             const int64_t slot = (int64_t)kvh * a.R + row, slot_rows = (int64_t)a.Hk * a.R;
-            if (!args.own) {
-                a.ml[split * slot_rows + slot] = make_float2(m, l);
-                float4* to = reinterpret_cast<float4*>(a.part + (split * slot_rows + slot) * 64);
+            if (a.slots > 1) {
+                const int64_t at_slot = (args.own ? a.splits_p : split) * slot_rows + slot;
+                a.ml[at_slot] = make_float2(m, l);
+                float4* to = reinterpret_cast<float4*>(a.part + at_slot * 64);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             } else {
-                for (int s = 0; args.late && s < a.splits_p; ++s) {
-                    const float2 x = a.ml[s * slot_rows + slot];
-                    const float4* from = reinterpret_cast<const float4*>(a.part + (s * slot_rows + slot) * 64);
-                    const float mn = fmaxf(m, x.x), ref = mn == -INFINITY ? 0.f : mn, f = ex2_approx(m - ref), w = ex2_approx(x.x - ref);
-                    m = mn;
-                    l = fmaf(l, f, x.y * w);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float4 v = from[i];
-                        o[4 * i] = fmaf(v.x, w, o[4 * i] * f); o[4 * i + 1] = fmaf(v.y, w, o[4 * i + 1] * f);
-                        o[4 * i + 2] = fmaf(v.z, w, o[4 * i + 2] * f); o[4 * i + 3] = fmaf(v.w, w, o[4 * i + 3] * f);
-                    }
-                }
                 const float f = l > 0.f ? 1.f / l : 0.f;
-                uint4* to = reinterpret_cast<uint4*>(const_cast<X*>(row_of<X>(a.O, b, h, tok)));
+                uint4* to = reinterpret_cast<uint4*>(const_cast<X*>(row_of<X>(a.O, bq, h, tok)));
                 if constexpr (LOW) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
@@ -480,7 +460,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                         to[i] = make_uint4(pack<X>(o[8 * i] * f, o[8 * i + 1] * f), pack<X>(o[8 * i + 2] * f, o[8 * i + 3] * f),
                                            pack<X>(o[8 * i + 4] * f, o[8 * i + 5] * f), pack<X>(o[8 * i + 6] * f, o[8 * i + 7] * f));
                 }
-                a.LSE[b * a.lse_sB + h * a.lse_sH + tok] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+                a.LSE[bq * a.lse_sB + h * a.lse_sH + tok] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
             }
         }
     }
@@ -489,30 +469,14 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     if (warp == 1) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
-        if (lane == 0) report_abort(sh.abort, args.status);
+        if (lane == 0) report_abort(sh.abort, a.status);
     }
-}
-
-// The tiles of a view of keys or values: rows of 128 bytes (fp32: two pieces of a row).
-int tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, bool values) {
-    if (T == 0) {
-        memset(map, 0, sizeof(*map));  // no tile of it is loaded
-        return HK_OK;
-    }
-    if (dtype == HK_F32) return make_tile_map(map, static_cast<const float*>(v.ptr), HEAD_DIM, (int)B, H, T, v.strideB, T == 1 ? 64 : v.strideM, v.strideH, Many<float>::KEYS, values);
-    EncodeTiledFn enc = get_encode_tiled();
-    if (!enc) return HK_ERR_CUDA;
-    const int64_t sM = T == 1 ? 64 : v.strideM, sH = H == 1 ? sM * T : v.strideH, sB = B == 1 ? std::max(sH * H, sM * T) : v.strideB;
-    cuuint64_t dims[5] = {64, (cuuint64_t)T, 1, (cuuint64_t)H, (cuuint64_t)B};
-    cuuint64_t strides[4] = {(cuuint64_t)sM * 2, 128, (cuuint64_t)sH * 2, (cuuint64_t)sB * 2};
-    cuuint32_t box[5] = {64, (cuuint32_t)Many<__half>::KEYS, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
-    const CUresult r = enc(map, dtype == HK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, v.ptr, dims, strides, box, ones,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? HK_OK : HK_ERR_CUDA;
+    if (args.late && blockIdx.x == gridDim.x - 1) pdl_wait();  // this kernel is complete when the one over the prefix is
 }
 
 template <class X>
 int launch(const ManyArgs& args, int dtype, int64_t blocks, cudaStream_t stream) {
+    typedef Many<X> C;
     static std::once_flag once[HK_MAX_DEVICES];
     static cudaError_t rc[HK_MAX_DEVICES];
     int dev = 0;
@@ -523,8 +487,8 @@ int launch(const ManyArgs& args, int dtype, int64_t blocks, cudaStream_t stream)
     const PrefixArgs& a = args.p;
     CUtensorMap kp, vp, k, v;
     int s;
-    if ((s = tile_map(&kp, a.Kp, dtype, 1, a.Hk, args.prefix ? a.P : 0, false)) || (s = tile_map(&vp, a.Vp, dtype, 1, a.Hk, args.prefix ? a.P : 0, true)) ||
-        (s = tile_map(&k, a.K, dtype, a.B, a.Hk, args.own ? a.S : 0, false)) || (s = tile_map(&v, a.V, dtype, a.B, a.Hk, args.own ? a.S : 0, true)))
+    if ((s = prefix_tile_map(&kp, a.Kp, dtype, 1, a.Hk, args.prefix ? a.P : 0, C::KEYS, false)) || (s = prefix_tile_map(&vp, a.Vp, dtype, 1, a.Hk, args.prefix ? a.P : 0, C::KEYS, true)) ||
+        (s = prefix_tile_map(&k, a.K, dtype, a.B, a.Hk, args.own ? a.S : 0, C::KEYS, false)) || (s = prefix_tile_map(&v, a.V, dtype, a.B, a.Hk, args.own ? a.S : 0, C::KEYS, true)))
         return s;
     LaunchConfig lc((unsigned)blocks, Many<X>::THREADS, Many<X>::SMEM, stream, 1, true);
     if (cudaLaunchKernelEx(&lc.cfg, prefix_many_kernel<X>, kp, vp, k, v, args) != cudaSuccess) return check_launch();
@@ -539,12 +503,10 @@ int launch(const ManyArgs& args, int dtype, int64_t blocks, cudaStream_t stream)
 
 ManyPlan many_plan(int dtype) { return dtype == HK_F32 ? ManyPlan{TILE, 64} : ManyPlan{2 * TILE, 128}; }
 int launch_prefix_many(const PrefixArgs& a, int dtype, cudaStream_t stream) {
-    ManyArgs args{a, device_status_ptr(), 0, 1, 0, a.tiles_p};
-    return args.status ? launch(args, dtype, (int64_t)a.Hk * a.tiles_p * a.splits_p, stream) : HK_ERR_CUDA;
+    return launch(ManyArgs{a, 0, 1, 0, a.tiles_p}, dtype, (int64_t)a.Hk * a.tiles_p * a.splits_p, stream);
 }
 int launch_own_many(const PrefixArgs& a, int dtype, bool prefix, cudaStream_t stream) {
-    ManyArgs args{a, device_status_ptr(), 1, prefix, !prefix && a.splits_p > 0, a.tiles_o};
-    return args.status ? launch(args, dtype, (int64_t)a.B * a.Hk * a.tiles_o, stream) : HK_ERR_CUDA;
+    return launch(ManyArgs{a, 1, prefix, !prefix && a.splits_p > 0, a.tiles_o}, dtype, (int64_t)a.B * a.Hk * a.tiles_o, stream);
 }
 
 }  // namespace hk
