@@ -3,10 +3,11 @@
 // formulas.
 //
 // Every call is bound by HBM: each row is read and written once, and the arithmetic of a row (about 10 operations an element
-// backward) is a fraction of what an SM can do meanwhile.  A warp takes a token and goes through its heads: the 32 lanes
-// compute the 32 pairs' sines and cosines once, and all heads use them.  Eight lanes share a row, each with elements
-// 4 s .. 4 s + 3 and 32 + 4 s .. 32 + 4 s + 3, so both halves of a pair are in one lane whether pairs are neighbours or half a
-// row apart, and a load instruction of a warp takes whole 128-byte lines of four rows.
+// backward) is a fraction of what an SM can do meanwhile.  A warp takes a token and goes through the heads of its queries, or of its
+// keys: the 32 lanes compute the 32 pairs' sines and cosines once, and all heads use them.  Eight lanes share a row, each with
+// elements 4 s .. 4 s + 3 and 32 + 4 s .. 32 + 4 s + 3, so both halves of a pair are in one lane whether pairs are neighbours or half a
+// row apart, and a load instruction of a warp takes whole 128-byte lines of four rows.  The rows of the next step are on their way
+// while a step is worked on.
 #include <cmath>
 
 #include "operators.cuh"
@@ -16,7 +17,7 @@ namespace {
 
 enum QkMode { QK_ROTATE = 0, QK_NORM = 1, QK_NORM_BACK = 2 };
 constexpr int QK_WARPS = 8;
-constexpr int QK_BACK_CTAS = 4;  // per SM at most: room in the workspace
+constexpr int QK_CTAS = 2;  // that an SM holds
 
 struct RowView {
     char* ptr;
@@ -29,64 +30,66 @@ struct QkArgs {
     const void* positions;
     int64_t pA, pB, pT;
     float* partial;
-    int nh, rows;  // query heads, heads of both
-    uint32_t T, units;
-    int per_unit, units_per_token;  // heads a warp takes with one set of angles
+    int heads[2];
+    uint32_t T, tokens, blocks_q;  // CTAs that take queries; the others take keys
+    int split;                     // a warp takes one step of a token's heads, not all of them
     int pos64, w_dtype, back;
     float eps;
     hk_rotary_plan plan;
 };
 
-__device__ __forceinline__ float4 load4(const float* p) { return __ldcs(reinterpret_cast<const float4*>(p)); }
+// A lane's part of a row as it is in memory, and as numbers: elements 4 s .. 4 s + 3, then 32 + 4 s ..
 template <class T>
-__device__ __forceinline__ float4 load4(const T* p) {
-    const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
-    const float2 a = unpack<T>(v.x), b = unpack<T>(v.y);
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
-template <class T>
-__device__ __forceinline__ void store4(T* p, float4 v) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack<T>(v.x, v.y), pack<T>(v.z, v.w));
-}
-
+struct Raw {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void load(const char* p, int sub) {
+        if constexpr (sizeof(T) == 4) {
+            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p) + sub), b = __ldcs(reinterpret_cast<const uint4*>(p + 128) + sub);
+            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+        } else {
+            const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p) + sub), b = __ldcs(reinterpret_cast<const uint2*>(p + 64) + sub);
+            w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
+        }
+    }
+};
 struct Row8 {
-    float v[8];  // elements 4 s .. 4 s + 3, then 32 + 4 s ..
+    float v[8];
 };
 template <class T>
-__device__ __forceinline__ Row8 load_row(const char* p, int sub) {
-    const float4 a = load4(reinterpret_cast<const T*>(p) + 4 * sub), b = load4(reinterpret_cast<const T*>(p) + 32 + 4 * sub);
-    return Row8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-}
-// The same row as 16-bit words, kept for the elements that do not change: their way through fp32 gives a NaN other bits.
-struct Words {
-    uint32_t w[4];
-};
-template <class T>
-__device__ __forceinline__ Row8 load_row(const char* p, int sub, Words& raw) {
-    const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p) + sub), b = __ldcs(reinterpret_cast<const uint2*>(p + 64) + sub);
-    raw = {{a.x, a.y, b.x, b.y}};
+__device__ __forceinline__ Row8 numbers(const Raw<T>& x) {
     Row8 r;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack<T>(raw.w[i]);
-        r.v[2 * i] = f.x;
-        r.v[2 * i + 1] = f.y;
+        for (int i = 0; i < 8; ++i) r.v[i] = __uint_as_float(x.w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack<T>(x.w[i]);
+            r.v[2 * i] = f.x;
+            r.v[2 * i + 1] = f.y;
+        }
     }
     return r;
 }
-template <class T>
-__device__ __forceinline__ void store_row(char* p, int sub, const Row8& r, const Words& raw, const Words& keep) {
-    uint32_t o[4];
+// keep: which bits of 16-bit words are those of `raw`; their way through fp32 would give a NaN other ones
+struct Keep {
+    uint32_t w[4];
+};
+template <class T, bool KEEPS>
+__device__ __forceinline__ void store_row(char* p, int sub, const Row8& r, const uint32_t* raw, const Keep& keep) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(p)[sub] = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
+        reinterpret_cast<float4*>(p + 128)[sub] = make_float4(r.v[4], r.v[5], r.v[6], r.v[7]);
+    } else {
+        uint32_t o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = (pack<T>(r.v[2 * i], r.v[2 * i + 1]) & ~keep.w[i]) | (raw.w[i] & keep.w[i]);
-    reinterpret_cast<uint2*>(p)[sub] = make_uint2(o[0], o[1]);
-    reinterpret_cast<uint2*>(p + 64)[sub] = make_uint2(o[2], o[3]);
-}
-template <class T>
-__device__ __forceinline__ void store_row(char* p, int sub, const Row8& r) {
-    store4(reinterpret_cast<T*>(p) + 4 * sub, make_float4(r.v[0], r.v[1], r.v[2], r.v[3]));
-    store4(reinterpret_cast<T*>(p) + 32 + 4 * sub, make_float4(r.v[4], r.v[5], r.v[6], r.v[7]));
+        for (int i = 0; i < 4; ++i) {
+            o[i] = pack<T>(r.v[2 * i], r.v[2 * i + 1]);
+            if (KEEPS) o[i] = (o[i] & ~keep.w[i]) | (raw[i] & keep.w[i]);
+        }
+        reinterpret_cast<uint2*>(p)[sub] = make_uint2(o[0], o[1]);
+        reinterpret_cast<uint2*>(p + 64)[sub] = make_uint2(o[2], o[3]);
+    }
 }
 __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
     return !w ? 1.f
@@ -124,40 +127,93 @@ __device__ __forceinline__ float rms_inverse(const Row8& x, float eps) {
     return rsqrtf(fmaf(sum8(ss), 1.f / 64.f, eps));
 }
 
-// U rows of each of the warp's four groups of lanes are loaded before the first is used.
+// U rows of each of the warp's four groups of lanes are a step.
 template <class X, class Y, int MODE, int U>
-__global__ void __launch_bounds__(QK_WARPS * 32) qk_rotary_kernel(const __grid_constant__ QkArgs a) {
-    constexpr bool KEEPS = MODE == QK_ROTATE && sizeof(X) == 2 && sizeof(Y) == 2;
+__global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const __grid_constant__ QkArgs a) {
+    constexpr bool KEEPS = MODE == QK_ROTATE && sizeof(X) == 2 && sizeof(Y) == 2, BACK = MODE == QK_NORM_BACK;
+    constexpr int STEP = 4 * U;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane >> 3, sub = lane & 7;
+    const int k = blockIdx.x >= a.blocks_q;
+    const uint32_t block = blockIdx.x - (k ? a.blocks_q : 0u), blocks = k ? gridDim.x - a.blocks_q : a.blocks_q;
+    const int heads = a.heads[k];
+    const RowView vx = a.x[k], vy = a.y[k], vd = a.dx[k];
     const uint64_t my_turn = a.plan.turn[lane];
     const int my_axis = a.plan.axis[lane];
     const bool interleaved = a.plan.interleaved != 0;
+    // strips: all heads of a token, or one step of them
+    const uint32_t per_token = a.split ? (heads + STEP - 1) / STEP : 1, strips = a.tokens * per_token, hop = blocks * QK_WARPS;
+    struct Place {
+        uint32_t strip;
+        int64_t x, y, d;  // offsets of the token's first row
+        int64_t pos;
+        int head, end;    // first of the step, end of the strip
+    };
+    auto place = [&](uint32_t strip) {
+        Place p;
+        p.strip = strip;
+        const uint32_t token = strip / per_token, b = token / a.T, t = token - b * a.T;
+        p.x = b * vx.sB + t * vx.sM;
+        p.y = b * vy.sB + t * vy.sM;
+        p.d = BACK ? b * vd.sB + t * vd.sM : 0;
+        p.pos = my_axis * a.pA + b * a.pB + t * a.pT;
+        p.head = (int)(strip - token * per_token) * STEP;
+        p.end = a.split ? min(p.head + STEP, heads) : heads;
+        return p;
+    };
+    Raw<X> next_x[U];
+    Raw<Y> next_g[BACK ? U : 1];
+    auto load = [&](const Place& p) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int h = p.head + 4 * i + grp;
+            if (h < p.end) {
+                next_x[i].load(vx.ptr + p.x + h * vx.sH, sub);
+                if constexpr (BACK) next_g[i].load(vy.ptr + p.y + h * vy.sH, sub);
+            }
+        }
+    };
+    auto position = [&](const Place& p) {
+        if (my_axis == HK_ROTARY_STILL) return (int64_t)0;
+        return a.pos64 ? static_cast<const int64_t*>(a.positions)[p.pos] : (int64_t)static_cast<const int32_t*>(a.positions)[p.pos];
+    };
+    Place at = place(block * QK_WARPS + warp);
     pdl_wait();
     pdl_trigger();
-    float w[2][MODE == QK_ROTATE ? 1 : 8], dw[2][MODE == QK_NORM_BACK ? 8 : 1];
+    int64_t next_pos = 0;
+    if (at.strip < strips) {
+        load(at);
+        next_pos = position(at);
+    }
+    float w[MODE == QK_ROTATE ? 1 : 8], dw[BACK ? 8 : 1];
     if (MODE != QK_ROTATE)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int i = 0; i < 8; ++i) w[i] = weight_at(a.w[k], a.w_dtype, (i < 4 ? 0 : 28) + 4 * sub + i);
+    if (BACK)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[k][i] = weight_at(a.w[k], a.w_dtype, (i < 4 ? 0 : 28) + 4 * sub + i);
-    if (MODE == QK_NORM_BACK)
+        for (int i = 0; i < 8; ++i) dw[i] = 0.f;
+    float c[4], s[4];
+    Keep keep;
+    bool fresh = true;  // the angles are another token's
+    while (at.strip < strips) {
+        Raw<X> x[U];
+        Raw<Y> g[BACK ? U : 1];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dw[k][i] = 0.f;
-
-    for (uint32_t u = blockIdx.x * QK_WARPS + warp; u < a.units; u += gridDim.x * QK_WARPS) {
-        const uint32_t token = u / a.units_per_token, b = token / a.T, t = token - b * a.T;
-        const int first = (int)(u - token * a.units_per_token) * a.per_unit, end = min(first + a.per_unit, a.rows);
-        float c[4], s[4];
-        {
-            uint64_t angle = 0;
-            if (my_axis != HK_ROTARY_STILL) {
-                const int64_t at = my_axis * a.pA + b * a.pB + t * a.pT;
-                angle = my_turn * (uint64_t)(a.pos64 ? static_cast<const int64_t*>(a.positions)[at] : (int64_t)static_cast<const int32_t*>(a.positions)[at]);
-            }
+        for (int i = 0; i < U; ++i) {
+            x[i] = next_x[i];
+            if (BACK) g[i] = next_g[i];
+        }
+        const int64_t pos = next_pos;
+        Place next = at;
+        next.head += STEP;
+        const bool on = next.head >= at.end;  // to another strip
+        if (on) next = place(at.strip + hop < at.strip ? 0xffffffffu : at.strip + hop);
+        if (next.strip < strips) {
+            load(next);
+            if (on) next_pos = position(next);
+        }
+        if (fresh) {
             float mc, ms;
-            sincospif((float)(int32_t)(angle >> 32) * 0x1p-31f, &ms, &mc);
+            sincospif((float)(int32_t)((my_turn * (uint64_t)pos) >> 32) * 0x1p-31f, &ms, &mc);
             if (a.back) ms = -ms;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -165,100 +221,85 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_rotary_kernel(const __grid_c
                 c[i] = __shfl_sync(0xffffffffu, mc, pair);
                 s[i] = __shfl_sync(0xffffffffu, ms, pair);
             }
-        }
-        Words keep;  // which of a row's 16-bit elements stay as they are
-        if (KEEPS) {
+            if (KEEPS) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int lo = (2 * i) & 3, hi = lo + 1;
-                keep.w[i] = interleaved ? (is_still(c[i], s[i]) ? 0xffffffffu : 0u)
-                                        : (is_still(c[lo], s[lo]) ? 0xffffu : 0u) | (is_still(c[hi], s[hi]) ? 0xffff0000u : 0u);
-            }
-        }
-        auto row = [&](const RowView* v, int r) {
-            const int k = r >= a.nh;
-            return v[k].ptr + b * v[k].sB + t * v[k].sM + (r - (k ? a.nh : 0)) * v[k].sH;
-        };
-        for (int r0 = first; r0 < end; r0 += 4 * U) {
-            Row8 x[U], g[MODE == QK_NORM_BACK ? U : 1];
-            Words raw[KEEPS ? U : 1];
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int r = min(r0 + 4 * i + grp, end - 1);  // behind the end: computed and not used
-                if constexpr (KEEPS) x[i] = load_row<X>(row(a.x, r), sub, raw[i]);
-                else x[i] = load_row<X>(row(a.x, r), sub);
-                if (MODE == QK_NORM_BACK) g[i] = load_row<Y>(row(a.y, r), sub);
-            }
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int r = r0 + 4 * i + grp;
-                const bool k = r >= a.nh, valid = r < end;
-                if (MODE == QK_ROTATE) {
-                    rotate(x[i], c, s, interleaved);
-                    if constexpr (KEEPS) {
-                        if (valid) store_row<Y>(row(a.y, r), sub, x[i], raw[i], keep);
-                    } else if (valid) {
-                        store_row<Y>(row(a.y, r), sub, x[i]);
-                    }
-                } else if (MODE == QK_NORM) {
-                    const float inv = rms_inverse(x[i], a.eps);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[i].v[e] *= inv * (k ? w[1][e] : w[0][e]);
-                    rotate(x[i], c, s, interleaved);
-                    if (valid) store_row<Y>(row(a.y, r), sub, x[i]);
-                } else {
-                    const float inv = rms_inverse(x[i], a.eps);
-                    rotate(g[i], c, s, interleaved);
-                    float dot = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[i].v[e] *= inv;
-                        const float gx = g[i].v[e] * x[i].v[e];
-                        dw[0][e] += valid && !k ? gx : 0.f;
-                        dw[1][e] += valid && k ? gx : 0.f;
-                        g[i].v[e] *= k ? w[1][e] : w[0][e];
-                        dot = fmaf(g[i].v[e], x[i].v[e], dot);
-                    }
-                    dot = sum8(dot) * (1.f / 64.f);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) g[i].v[e] = inv * fmaf(-x[i].v[e], dot, g[i].v[e]);
-                    if (valid) store_row<X>(row(a.dx, r), sub, g[i]);
+                for (int i = 0; i < 4; ++i) {
+                    const int lo = (2 * i) & 3, hi = lo + 1;
+                    keep.w[i] = interleaved ? (is_still(c[i], s[i]) ? 0xffffffffu : 0u)
+                                            : (is_still(c[lo], s[lo]) ? 0xffffu : 0u) | (is_still(c[hi], s[hi]) ? 0xffff0000u : 0u);
                 }
             }
         }
+        fresh = on;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int h = at.head + 4 * i + grp;
+            const bool valid = h < at.end;
+            if (!__any_sync(0xffffffffu, valid)) break;
+            Row8 r = numbers(x[i]);
+            if (MODE != QK_ROTATE && !valid) r = Row8{};
+            if (!BACK) {
+                if (MODE == QK_NORM) {
+                    const float inv = rms_inverse(r, a.eps);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) r.v[e] *= inv * w[e];
+                }
+                rotate(r, c, s, interleaved);
+                if (valid) store_row<Y, KEEPS>(vy.ptr + at.y + h * vy.sH, sub, r, x[i].w, keep);
+            } else {
+                Row8 z = numbers(g[BACK ? i : 0]);
+                if (!valid) z = Row8{};
+                const float inv = rms_inverse(r, a.eps);
+                rotate(z, c, s, interleaved);
+                float dot = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    r.v[e] *= inv;
+                    if (valid) dw[e] = fmaf(z.v[e], r.v[e], dw[e]);
+                    z.v[e] *= w[e];
+                    dot = fmaf(z.v[e], r.v[e], dot);
+                }
+                dot = sum8(dot) * (1.f / 64.f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z.v[e] = inv * fmaf(-r.v[e], dot, z.v[e]);
+                if (valid) store_row<X, false>(vd.ptr + at.d + h * vd.sH, sub, z, nullptr, keep);
+            }
+        }
+        at = next;
     }
-    if (MODE == QK_NORM_BACK) {  // sums of the CTA's rows: [queries, keys][64]
-        __shared__ float sums[QK_WARPS * 4][2][64];
+    if (BACK) {  // sums of the CTA's rows
+        __shared__ float sums[QK_WARPS * 4][64];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sums[threadIdx.x >> 3][k][(e < 4 ? 0 : 28) + 4 * sub + e] = dw[k][e];
+        for (int e = 0; e < 8; ++e) sums[threadIdx.x >> 3][(e < 4 ? 0 : 28) + 4 * sub + e] = dw[e];
         __syncthreads();
-        if (threadIdx.x < 128) {
+        if (threadIdx.x < 64) {
             float x = 0.f;
 #pragma unroll
-            for (int i = 0; i < QK_WARPS * 4; ++i) x += sums[i][threadIdx.x >> 6][threadIdx.x & 63];
-            a.partial[blockIdx.x * 128 + threadIdx.x] = x;
+            for (int i = 0; i < QK_WARPS * 4; ++i) x += sums[i][threadIdx.x];
+            a.partial[blockIdx.x * 64 + threadIdx.x] = x;
         }
     }
 }
 
-// The CTAs' sums, 16 columns a CTA, 16 threads a column; always in the same order.
-__global__ void __launch_bounds__(256) qk_weight_sum_kernel(const float* partial, int n, float* dq, float* dk) {
+// The sums of the CTAs that took queries, and of those that took keys: 16 columns a CTA, 16 threads a column, always in the same
+// order.
+__global__ void __launch_bounds__(256) qk_weight_sum_kernel(const float* partial, int n_q, int n, float* dq, float* dk) {
     __shared__ float sums[16][17];
-    const int col = threadIdx.x & 15, part = threadIdx.x >> 4, at = blockIdx.x * 16 + col;
+    const int col = threadIdx.x & 15, part = threadIdx.x >> 4, at = (blockIdx.x & 3) * 16 + col;
+    const bool keys = blockIdx.x >= 4;
     pdl_wait();
     pdl_trigger();
     float x = 0.f;
+    const int end = keys ? n : n_q;
 #pragma unroll 4
-    for (int i = part; i < n; i += 16) x += partial[i * 128 + at];
+    for (int i = (keys ? n_q : 0) + part; i < end; i += 16) x += partial[i * 64 + at];
     sums[part][col] = x;
     __syncthreads();
     if (part == 0) {
 #pragma unroll
         for (int i = 1; i < 16; ++i) x += sums[i][col];
-        float* to = at < 64 ? dq : dk;
-        if (to) to[at & 63] = x;
+        float* to = keys ? dk : dq;
+        if (to) to[at] = x;
     }
 }
 
@@ -267,20 +308,26 @@ RowView row_view(const hk_view& v, int dtype) {
     return {static_cast<char*>(v.ptr), v.strideB * e, v.strideM * e, v.strideH * e};
 }
 
-template <int MODE, int U>
-using QkKernel = void (*)(QkArgs);
-
-template <int MODE, int U>
-QkKernel<MODE, U> pick(int x, int y) {
+typedef void (*QkKernel)(QkArgs);
+// Groups of four rows in a step: what fits the registers twice.
+template <class X, int MODE>
+constexpr int rows_of() { return MODE == QK_NORM_BACK ? 2 : 4; }
+template <class X, class Y, int MODE>
+QkKernel kernel_of(int& step) {
+    step = 4 * rows_of<X, MODE>();
+    return qk_rotary_kernel<X, Y, MODE, rows_of<X, MODE>()>;
+}
+template <int MODE>
+QkKernel pick(int x, int y, int& step) {
     typedef __nv_bfloat16 bf16;
-    if (x == HK_F32 && y == HK_F32) return qk_rotary_kernel<float, float, MODE, U>;
-    if (x == HK_BF16 && y == HK_BF16) return qk_rotary_kernel<bf16, bf16, MODE, U>;
-    if (x == HK_F16 && y == HK_F16) return qk_rotary_kernel<__half, __half, MODE, U>;
-    if (x == HK_BF16 && y == HK_F32) return qk_rotary_kernel<bf16, float, MODE, U>;
-    if (x == HK_F16 && y == HK_F32) return qk_rotary_kernel<__half, float, MODE, U>;
+    if (x == HK_F32 && y == HK_F32) return kernel_of<float, float, MODE>(step);
+    if (x == HK_BF16 && y == HK_BF16) return kernel_of<bf16, bf16, MODE>(step);
+    if (x == HK_F16 && y == HK_F16) return kernel_of<__half, __half, MODE>(step);
+    if (x == HK_BF16 && y == HK_F32) return kernel_of<bf16, float, MODE>(step);
+    if (x == HK_F16 && y == HK_F32) return kernel_of<__half, float, MODE>(step);
     if constexpr (MODE == QK_ROTATE) {  // gradients from the attention back to the projection's type
-        if (x == HK_F32 && y == HK_BF16) return qk_rotary_kernel<float, bf16, MODE, U>;
-        if (x == HK_F32 && y == HK_F16) return qk_rotary_kernel<float, __half, MODE, U>;
+        if (x == HK_F32 && y == HK_BF16) return kernel_of<float, bf16, MODE>(step);
+        if (x == HK_F32 && y == HK_F16) return kernel_of<float, __half, MODE>(step);
     }
     return nullptr;
 }
@@ -337,38 +384,46 @@ int qk_run(const hk_qk_params* p, int mode, bool back, cudaStream_t stream) {
     }
     a.positions = p->positions;
     a.pA = p->pos_strideA; a.pB = p->pos_strideB; a.pT = p->pos_strideT;
-    a.nh = p->nh; a.rows = p->nh + p->nh_k;
+    a.heads[0] = p->nh; a.heads[1] = p->nh_k;
     a.T = (uint32_t)p->T;
+    a.tokens = (uint32_t)(p->B * p->T);
     a.pos64 = p->pos_bits == 64;
     a.w_dtype = p->weight_dtype;
     a.back = back;
     a.eps = p->eps;
     a.plan = p->plan;
 
-    constexpr int U_FWD = 4, U_BACK = 2;
-    const int step = 4 * (mode == QK_NORM_BACK ? U_BACK : U_FWD);
-    const uint32_t tokens = (uint32_t)(p->B * p->T);
-    // Few tokens: a warp takes as few heads as keep its loads in flight, so that more SMs take part.
-    a.per_unit = a.rows;
-    if (tokens < (uint32_t)sm_count() * 16) a.per_unit = tokens * ((a.rows + step - 1) / step) < (uint32_t)sm_count() * QK_WARPS ? 4 : step;
-    a.units_per_token = (a.rows + a.per_unit - 1) / a.per_unit;
-    a.units = tokens * a.units_per_token;
-    uint32_t blocks = (a.units + QK_WARPS - 1) / QK_WARPS;
-    QkKernel<0, 0> kernel = mode == QK_ROTATE ? pick<QK_ROTATE, U_FWD>(src_t, dst_t)
-                            : mode == QK_NORM ? pick<QK_NORM, U_FWD>(src_t, dst_t)
-                                              : pick<QK_NORM_BACK, U_BACK>(src_t, p->out_dtype);
+    int step = 0;
+    const QkKernel kernel = mode == QK_ROTATE ? pick<QK_ROTATE>(src_t, dst_t, step)
+                            : mode == QK_NORM ? pick<QK_NORM>(src_t, dst_t, step)
+                                              : pick<QK_NORM_BACK>(src_t, p->out_dtype, step);
     if (!kernel) return HK_ERR_UNSUPPORTED;
-    if (mode == QK_NORM_BACK) blocks = std::min(blocks, (uint32_t)sm_count() * 2);
+    // Warps enough for all that an SM holds; where there are fewer tokens, a warp takes one step of a token's heads.
+    const int64_t most = (int64_t)sm_count() * QK_CTAS;
+    a.split = (int64_t)a.tokens < most * QK_WARPS;
+    auto strips = [&](int heads) { return (int64_t)a.tokens * (a.split ? (heads + step - 1) / step : 1); };
+    // CTAs by the steps there are
+    int64_t n_q = (strips(p->nh) + QK_WARPS - 1) / QK_WARPS, n_k = (strips(p->nh_k) + QK_WARPS - 1) / QK_WARPS;
+    if (p->nh_k == 0) n_k = 0;
+    if (n_q + n_k > most) {
+        const int64_t s_q = (p->nh + step - 1) / step, s_k = (p->nh_k + step - 1) / step;
+        const int64_t for_q = std::max<int64_t>(1, std::min<int64_t>(most - (n_k > 0), (most * s_q + (s_q + s_k) / 2) / (s_q + s_k)));
+        n_q = std::min(n_q, for_q);
+        n_k = std::min(n_k, most - n_q);
+    }
+    if (strips(p->nh) > 0xffffffffLL || strips(p->nh_k) > 0xffffffffLL) return HK_ERR_BAD_SHAPE;
+    a.blocks_q = (uint32_t)n_q;
+    const int blocks = (int)(n_q + n_k);
     LaunchConfig lc(blocks, QK_WARPS * 32, 0, stream, 1, true);
     if (cudaLaunchKernelEx(&lc.cfg, kernel, a) != cudaSuccess) return check_launch();
     count_launch();
     if (mode == QK_NORM_BACK && (p->dq_weight || p->dk_weight)) {
         LaunchConfig sum(8, 256, 0, stream, 1, true);
-        if (cudaLaunchKernelEx(&sum.cfg, qk_weight_sum_kernel, (const float*)a.partial, (int)blocks, p->dq_weight, p->dk_weight) != cudaSuccess)
+        if (cudaLaunchKernelEx(&sum.cfg, qk_weight_sum_kernel, (const float*)a.partial, (int)n_q, blocks, p->dq_weight, p->dk_weight) != cudaSuccess)
             return check_launch();
         count_launch();
     }
-    return check_launch();
+    return HK_OK;
 }
 
 }  // namespace
@@ -408,6 +463,6 @@ int hk_rotary_backward(const hk_qk_params* p, void* stream) { return qk_run(p, Q
 int hk_qk_norm_rotary_forward(const hk_qk_params* p, void* stream) { return qk_run(p, QK_NORM, false, static_cast<cudaStream_t>(stream)); }
 int hk_qk_norm_rotary_backward(const hk_qk_params* p, void* stream) { return qk_run(p, QK_NORM_BACK, true, static_cast<cudaStream_t>(stream)); }
 
-size_t hk_qk_norm_rotary_workspace_bytes(const hk_qk_params*) { return (size_t)sm_count() * QK_BACK_CTAS * 128 * sizeof(float); }
+size_t hk_qk_norm_rotary_workspace_bytes(const hk_qk_params*) { return (size_t)sm_count() * QK_CTAS * 64 * sizeof(float); }
 
 }  // extern "C"
