@@ -7,8 +7,8 @@
 //   Warp 0 loads tiles with TMA, warp 1 issues the products S = Q K^T and, a tile or two behind, O += P V (tcgen05, operands in
 // shared and tensor memory), four warps to a block of rows take S through the softmax, a row to a thread.  Scores are three deep
 // in tensor memory; P takes the place of its S.
-//   fp32: x = h + l with h the upper 11 bits of the significand, which is what the tensor core reads of an fp32 word.  Two warps
-// write the l parts of each tile beside it; a product is l h' + h l' + h h', in this order: what is left out is 2^-22 of it.  P V of
+//   fp32: x = h + l with h the upper 11 bits of the significand, which is what the tensor core reads of an fp32 word.  Q lies in tensor memory
+// with its l parts, four warps write those of each tile beside it; a product is l h' + h l' + h h', in this order: what is left out is 2^-22 of it.  P V of
 // a tile comes back into registers and is added there in fp32: the tensor core's additions cut off instead of rounding, and over
 // thousands of keys in one accumulator that would be seen.
 #include <cmath>
@@ -53,10 +53,9 @@ struct Many {
     static constexpr bool LOW = sizeof(X) == 4;      // products in three parts
     static constexpr int STREAMS = LOW ? 1 : 2;      // blocks of rows
     static constexpr int KEYS = LOW ? 64 : 128;      // of a tile
-    static constexpr int THREADS = 128 + 128 * STREAMS;
-    static constexpr int SLOTS = LOW ? 5 : 8;
+    static constexpr int SLOTS = LOW ? 7 : 8;
     static constexpr int AHEAD = LOW ? 2 : 1;        // tiles that the scores are ahead of the weighted values
-    static constexpr int Q_RAW = TILE * 64 * (int)sizeof(X), Q_BYTES = Q_RAW * (LOW ? 2 : 1);
+    static constexpr int Q_BYTES = LOW ? 0 : TILE * 64 * (int)sizeof(X);  // fp32: in tensor memory
     static constexpr int KV_RAW = KEYS * 64 * (int)sizeof(X), KV_BYTES = KV_RAW * (LOW ? 2 : 1);
     static constexpr int KV_BOX = KEYS * 128;        // 128 bytes of each row
     struct __align__(16) Shared {
@@ -69,7 +68,10 @@ struct Many {
     static constexpr int OFF_KV = STREAMS * Q_BYTES, OFF_SH = OFF_KV + SLOTS * KV_BYTES, SMEM = OFF_SH + (int)sizeof(Shared);
     static_assert(SMEM <= 232448, "exceeds the 227 KiB a CTA may opt in to");
 };
-constexpr uint32_t COL_O = 384;  // O_j: 64 columns, two of them behind three buffers of 128 for scores and weights
+constexpr int MANY_THREADS = 384;
+// Tensor memory.  16-bit types: three buffers of 128 columns for scores and weights, O of two blocks of rows.  fp32: three buffers of
+// 64 for scores and weights, two for the weights' low parts, O of a tile, Q and its low parts.
+constexpr uint32_t COL_O = 384, LOW_COL_LOW = 192, LOW_COL_O = 320, LOW_COL_Q = 384;
 
 enum ManyWait { W_Q = 301, W_KV, W_READY, W_EMPTY, W_S, W_P, W_O };
 
@@ -82,7 +84,7 @@ struct ManyArgs {
 };
 
 template <class X>
-__global__ void __launch_bounds__(Many<X>::THREADS, 1)
+__global__ void __launch_bounds__(MANY_THREADS, 1)
 prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ManyArgs args) {
     typedef Many<X> C;
@@ -123,9 +125,21 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     const int tile = args.tiles - 1 - (item - at * args.tiles);  // the last rows see the most keys
     const int b = args.own ? at / a.Hk : 0, kvh = at - b * a.Hk, BLOCK = C::STREAMS * TILE;
     const int all = args.own ? a.T * a.group : a.R, first = tile * BLOCK, row0 = b * a.T * a.group + first, rows = min(BLOCK, all - first);
+    const int len = args.own ? request_keys(a, b) : 0;
+    // a row of Q to a softmax thread
+    const int t = (warp - 4) >> 2, quarter = warp & 3, in_block = quarter * 32 + lane, r = t * TILE + in_block;
+    const bool valid = warp >= 4 && r < rows;
+    const int row = row0 + r, token = row / a.group, bq = args.own ? b : token / a.T, tok = token - bq * a.T, h = kvh * a.group + row - token * a.group;
+    constexpr int CHUNKS = 64 * sizeof(X) / 16;
+    uint4 x_q[CHUNKS];
+    if (warp >= 4) {
+        const uint4* from = reinterpret_cast<const uint4*>(row_of<X>(a.Q, valid ? bq : 0, valid ? h : 0, valid ? tok : 0));
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) x_q[c] = valid ? from[c] : make_uint4(0, 0, 0, 0);
+    }
     // and keys: tiles of the prefix, then the request's own
     const int p_begin = args.own ? 0 : split * a.per_p, p_end = !args.prefix ? 0 : args.own ? a.P : min(a.P, p_begin + a.per_p);
-    const int len = args.own ? request_keys(a, b) : 0, seen = args.own ? token_keys(a, len, (first + rows - 1) / a.group) : 0;
+    const int seen = args.own ? token_keys(a, len, (first + rows - 1) / a.group) : 0;
     const int n_p = (p_end - p_begin + KEYS - 1) / KEYS, n = n_p + (seen + KEYS - 1) / KEYS;
     const int streams = C::STREAMS == 2 && rows > TILE ? 2 : 1;
     __syncthreads();
@@ -152,8 +166,40 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     // first key of tile j, in the prefix or of the request's own
     auto key_of = [&](int j) { return j < n_p ? p_begin + j * KEYS : (j - n_p) * KEYS; };
 
+    // What the tiles need beside the loads.  Rows behind the request's last key may hold anything, and 0 times a NaN is one: they are
+    // cleared among the values.  fp32: the tiles' low parts, by two pairs of warps, every other tile each.
+    auto tend = [&](int me, int first_entry) {
+        bool ok = true;
+        for (int i = first_entry; ok && n > (LOW ? 0 : n_p) && i < 2 * n; i += 2) {
+            const auto [j, is_v] = entry(i);
+            const int s = i % SLOTS;
+            ok = __all_sync(0xffffffffu, LOW ? mbar_wait(wc, &sh.kv_full[s], (i / SLOTS) & 1, W_KV, i) : mbar_wait(wc, &sh.last_full, 0, W_KV, i));
+            if (!ok) break;
+            const int keep = is_v && j >= n_p ? min(KEYS, len - key_of(j)) : KEYS;  // rows that are values
+            uint4* raw = reinterpret_cast<uint4*>(sKV + s * C::KV_BYTES);
+            if constexpr (LOW) {
+                constexpr int EACH = C::KV_RAW / 16 / 64;
+                auto rest = [](uint32_t v) { return __float_as_uint(__uint_as_float(v) - __uint_as_float(v & 0xffffe000u)); };
+                uint4 *from = raw + me, *low = from + C::KV_RAW / 16, x[EACH];
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) x[k] = from[k * 64];
+                if (keep < KEYS) {
+#pragma unroll
+                    for (int k = 0; k < EACH; ++k)
+                        if (((k * 64 + me) & (C::KV_BOX / 16 - 1)) / 8 >= keep) from[k * 64] = x[k] = make_uint4(0, 0, 0, 0);  // row of the box
+                }
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) low[k * 64] = make_uint4(rest(x[k].x), rest(x[k].y), rest(x[k].z), rest(x[k].w));
+            } else {
+                for (int k = keep * 8 + me; k < C::KV_RAW / 16; k += 32) raw[k] = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            mbar_arrive_warp(LOW ? &sh.kv_ready[s] : &sh.last_ready, lane);
+        }
+    };
+
     if (warp < 4) {
-        if constexpr (C::STREAMS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         if (warp == 0) {
             // ------------------------------ tiles of keys and values ------------------------------
             if (lane == 0) {
@@ -177,128 +223,133 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             const int total = n * streams;
             const int ahead = A * streams;  // products that S is ahead of O
             bool ok = true;
-            auto wait = [&](uint64_t* bar, uint32_t parity, int id, int aux) { return (bool)__all_sync(0xffffffffu, mbar_wait(wc, bar, parity, id, aux)); };
-            auto wait_tile = [&](int i) {
-                const int s = i % SLOTS;
-                const uint32_t phase = (i / SLOTS) & 1;
-                if constexpr (LOW) return wait(&sh.kv_ready[s], phase, W_READY, i);
-                return by_hand(i) ? wait(&sh.last_ready, 0, W_READY, i) : wait(&sh.kv_full[s], phase, W_KV, i);
+            // The tensor pipe queues next to nothing, and a wait takes some 100 cycles even when its barrier is long complete: each
+            // is looked at while the products before it are still being issued, and waited for if that look came too early.
+            struct Barrier {
+                uint64_t* bar;
+                uint32_t parity;
             };
+            auto seen = [&](const Barrier& x) { return mbar_test_wait(x.bar, x.parity); };
+            auto wait = [&](bool was_seen, const Barrier& x, int id, int aux) {
+                return __all_sync(0xffffffffu, was_seen) || (bool)__all_sync(0xffffffffu, mbar_wait(wc, x.bar, x.parity, id, aux));
+            };
+            auto tile_barrier = [&](int i) -> Barrier {
+                const int s = i % SLOTS;
+                if constexpr (LOW) return {&sh.kv_ready[s], (uint32_t)(i / SLOTS) & 1u};
+                return by_hand(i) ? Barrier{&sh.last_ready, 0u} : Barrier{&sh.kv_full[s], (uint32_t)(i / SLOTS) & 1u};
+            };
+            bool seen_k = false, seen_v = false, seen_p = false;
             const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
             for (int q = 0; q < total + ahead && ok; ++q) {
                 if (q < total) {  // S
                     const int j = q >> (streams - 1), t = q & (streams - 1), i = entry_k(j);
-                    if (j == 0 && !(ok = wait(&sh.q_full[t], 0, W_Q, t))) break;
-                    if (t == 0 && !(ok = wait_tile(i))) break;
+                    if (j == 0 && !(ok = wait(false, {&sh.q_full[t], 0u}, W_Q, t))) break;
+                    if (t == 0 && !(ok = wait(seen_k, tile_barrier(i), W_READY, i))) break;
                     tc_fence_after_sync();
-                    const uint32_t d = tmem + (q % 3) * 128, qa = q_addr + t * C::Q_BYTES, ka = kv_addr + (i % SLOTS) * C::KV_BYTES;
+                    // what O needs next
+                    const int r = max(q - ahead, 0);
+                    const Barrier v_next = tile_barrier(entry_v(r >> (streams - 1))), p_next = {&sh.p_full[r % 3], (uint32_t)(r / 3) & 1u};
+                    const uint32_t ka = kv_addr + (i % SLOTS) * C::KV_BYTES;
                     if constexpr (LOW) {
                         constexpr uint32_t IDESC = make_idesc_tf32(TILE, KEYS, false, false);
-                        const Desc qd = kmajor_desc(qa, 0, BOX_BYTES), kd = kmajor_desc(ka, 0, C::KV_BOX);
-                        auto four = [&](uint32_t x, uint32_t y, uint32_t acc) {
-                            umma_ss4<KMAJOR_STEP, KMAJOR_STEP>(leader, d, qd + x, kd + y, IDESC, acc);
-                            umma_ss4<KMAJOR_STEP, KMAJOR_STEP>(leader, d, qd + (x + BOX_BYTES), kd + (y + C::KV_BOX), IDESC, 1u);
+                        const uint32_t d = tmem + (q % 3) * 64;
+                        const Desc kd = kmajor_desc(ka, 0, C::KV_BOX);
+                        auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
+                            umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x, kd + y, IDESC, acc);
+                            umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x + 32, kd + (y + C::KV_BOX), IDESC, 1u);
                         };
-                        four(C::Q_RAW, 0, 0u);
-                        four(0, C::KV_RAW, 1u);
-                        four(0, 0, 1u);
+                        eight(64, 0, 0u);
+                        eight(0, C::KV_RAW, 1u);
+                        seen_v = seen(v_next);
+                        seen_p = seen(p_next);
+                        eight(0, 0, 1u);
                     } else {
                         constexpr uint32_t IDESC = make_idesc_16(TILE, KEYS, BF16, false);
-                        const uint64_t qd = make_smem_desc(qa, 16, 1024, DESC_SW128), kd = make_smem_desc(ka, 16, 1024, DESC_SW128);
+                        const uint32_t d = tmem + (q % 3) * 128;
+                        const uint64_t qd = make_smem_desc(q_addr + t * C::Q_BYTES, 16, 1024, DESC_SW128), kd = make_smem_desc(ka, 16, 1024, DESC_SW128);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) umma_ss_16(leader, d, qd + 2 * k, kd + 2 * k, IDESC, k > 0);
+                        for (int k = 0; k < 4; ++k) {
+                            if (k == 2) {
+                                seen_v = seen(v_next);
+                                seen_p = seen(p_next);
+                            }
+                            umma_ss_16(leader, d, qd + 2 * k, kd + 2 * k, IDESC, k > 0);
+                        }
                     }
                     umma_commit_lead(leader, &sh.s_full[q % 3]);
                     if (t == streams - 1) umma_commit_lead(leader, &sh.kv_empty[i % SLOTS]);
                 }
                 if (q >= ahead) {  // O
                     const int r = q - ahead, j = r >> (streams - 1), t = r & (streams - 1), i = entry_v(j);
-                    if (t == 0 && !(ok = wait_tile(i))) break;
-                    if (!(ok = wait(&sh.p_full[r % 3], (r / 3) & 1, W_P, r))) break;
+                    if (t == 0 && !(ok = wait(seen_v, tile_barrier(i), W_READY, i))) break;
+                    if (!(ok = wait(seen_p, {&sh.p_full[r % 3], (uint32_t)(r / 3) & 1u}, W_P, r))) break;
                     tc_fence_after_sync();
-                    const uint32_t p = tmem + (r % 3) * 128, d = tmem + COL_O + (LOW ? j & 1 : t) * 64, va = kv_addr + (i % SLOTS) * C::KV_BYTES;
+                    seen_v = seen_p = false;
+                    const Barrier k_next = tile_barrier(entry_k(min((q + 1) >> (streams - 1), n - 1)));
+                    const uint32_t va = kv_addr + (i % SLOTS) * C::KV_BYTES;
                     if constexpr (LOW) {
                         constexpr uint32_t IDESC = make_idesc_tf32(TILE, HEAD_DIM, false, true);
+                        const uint32_t high = tmem + (r % 3) * 64, low = tmem + LOW_COL_LOW + (r & 1) * 64, d = tmem + LOW_COL_O;
                         const Desc vd = mnmajor_desc(va, 0, C::KV_BOX);
                         auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
-                            umma_ts4<MNMAJOR_STEP>(leader, d, p + x, vd + y, IDESC, acc);
-                            umma_ts4<MNMAJOR_STEP>(leader, d, p + x + 32, vd + (y + 4096), IDESC, 1u);
+                            umma_ts4<MNMAJOR_STEP>(leader, d, x, vd + y, IDESC, acc);
+                            umma_ts4<MNMAJOR_STEP>(leader, d, x + 32, vd + (y + 4096), IDESC, 1u);
                         };
-                        eight(64, 0, 0u);
-                        eight(0, C::KV_RAW, 1u);
-                        eight(0, 0, 1u);
+                        eight(low, 0, 0u);
+                        eight(high, C::KV_RAW, 1u);
+                        seen_k = seen(k_next);
+                        eight(high, 0, 1u);
                     } else {
                         constexpr uint32_t IDESC = make_idesc_16(TILE, HEAD_DIM, BF16, true);
+                        const uint32_t p = tmem + (r % 3) * 128, d = tmem + COL_O + t * 64;
                         const uint64_t vd = make_smem_desc(va, 16, 1024, DESC_SW128);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) umma_ts_16(leader, d, p + 8 * k, vd + (2048 >> 4) * k, IDESC, k > 0 || j > 0);
+                        for (int k = 0; k < 8; ++k) {
+                            if (k == 4) seen_k = seen(k_next);
+                            umma_ts_16(leader, d, p + 8 * k, vd + (2048 >> 4) * k, IDESC, k > 0 || j > 0);
+                        }
                     }
                     umma_commit_lead(leader, &sh.o_full[r % 3]);
                     if (t == streams - 1) umma_commit_lead(leader, &sh.kv_empty[i % SLOTS]);
                 }
             }
-        } else if (LOW || warp == 2) {
-            // Rows behind the request's last key may hold anything, and 0 times a NaN is one: they are cleared among the values.
-            // fp32: the tiles' low parts.
-            const int me = LOW ? threadIdx.x - 64 : lane;
-            bool ok = true;
-            for (int i = LOW ? 0 : 2 * n - 1; ok && n > (LOW ? 0 : n_p) && i < 2 * n; ++i) {
-                const auto [j, is_v] = entry(i);
-                const int s = i % SLOTS;
-                ok = __all_sync(0xffffffffu, LOW ? mbar_wait(wc, &sh.kv_full[s], (i / SLOTS) & 1, W_KV, i) : mbar_wait(wc, &sh.last_full, 0, W_KV, i));
-                if (!ok) break;
-                const int keep = is_v && j >= n_p ? min(KEYS, len - key_of(j)) : KEYS;  // rows that are values
-                uint4* raw = reinterpret_cast<uint4*>(sKV + s * C::KV_BYTES);
-                if constexpr (LOW) {
-                    constexpr int EACH = C::KV_RAW / 16 / 64, AT_ONCE = 8;
-                    auto rest = [](uint32_t v) { return __float_as_uint(__uint_as_float(v) - __uint_as_float(v & 0xffffe000u)); };
-                    uint4 *from = raw + me, *low = from + C::KV_RAW / 16;
-                    if (keep < KEYS) {
-#pragma unroll
-                        for (int k = 0; k < EACH; ++k)
-                            if (((k * 64 + me) & (C::KV_BOX / 16 - 1)) / 8 >= keep) from[k * 64] = make_uint4(0, 0, 0, 0);  // row of the box
-                    }
-#pragma unroll 1
-                    for (int k0 = 0; k0 < EACH; k0 += AT_ONCE, from += AT_ONCE * 64, low += AT_ONCE * 64) {
-                        uint4 x[AT_ONCE];
-#pragma unroll
-                        for (int k = 0; k < AT_ONCE; ++k) x[k] = from[k * 64];
-#pragma unroll
-                        for (int k = 0; k < AT_ONCE; ++k) low[k * 64] = make_uint4(rest(x[k].x), rest(x[k].y), rest(x[k].z), rest(x[k].w));
-                    }
-                } else {
-                    for (int k = keep * 8 + me; k < C::KV_RAW / 16; k += 32) raw[k] = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async_smem();
-                mbar_arrive_warp(LOW ? &sh.kv_ready[s] : &sh.last_ready, lane);
-            }
+        } else if (!LOW && warp == 2) {
+            tend(lane, 2 * n - 1);
         }
+    } else if (LOW && warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 128;\n");
+        tend(threadIdx.x & 63, (warp >> 1) & 1);
     } else {
         // ------------------------------ softmax ------------------------------
-        if constexpr (C::STREAMS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
-        const int t = (warp - 4) >> 2, quarter = warp & 3, in_block = quarter * 32 + lane, r = t * TILE + in_block;
+        if constexpr (LOW) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        const bool live = t * TILE + quarter * 32 < rows, valid = r < rows;
-        const int row = row0 + r, token = row / a.group, bq = args.own ? b : token / a.T, tok = token - bq * a.T, h = kvh * a.group + row - token * a.group;
+        const bool live = t * TILE + quarter * 32 < rows;
         const int limit = args.own && valid ? token_keys(a, len, tok) : 0;  // own keys the row sees
-        if (t < streams) {  // the row of Q, in the layout of a K-major operand
-            const uint4* from = reinterpret_cast<const uint4*>(row_of<X>(a.Q, valid ? bq : 0, valid ? h : 0, valid ? tok : 0));
-            uint8_t* to = sQ + t * C::Q_BYTES + in_block * 128;
-            constexpr int CHUNKS = 64 * sizeof(X) / 16;
-            uint4 x[CHUNKS];
+        if (t < streams) {  // the row of Q
+            if constexpr (LOW) {
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) x[c] = valid ? from[c] : make_uint4(0, 0, 0, 0);
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t y[32], z[32];
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                x[c].x ^= a.flip; x[c].y ^= a.flip; x[c].z ^= a.flip; x[c].w ^= a.flip;
-                uint8_t* slot = to + (c >> 3) * BOX_BYTES + (((c & 7) ^ (in_block & 7)) << 4);
-                *reinterpret_cast<uint4*>(slot) = x[c];
-                if constexpr (LOW) {
-                    auto rest = [](uint32_t v) { return __float_as_uint(__uint_as_float(v) - __uint_as_float(v & 0xffffe000u)); };
-                    *reinterpret_cast<uint4*>(slot + C::Q_RAW) = make_uint4(rest(x[c].x), rest(x[c].y), rest(x[c].z), rest(x[c].w));
+                    for (int c = 0; c < 8; ++c) {
+                        const uint4& v = x_q[8 * half + c];
+                        y[4 * c] = v.x ^ a.flip; y[4 * c + 1] = v.y ^ a.flip; y[4 * c + 2] = v.z ^ a.flip; y[4 * c + 3] = v.w ^ a.flip;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) z[i] = __float_as_uint(__uint_as_float(y[i]) - __uint_as_float(y[i] & 0xffffe000u));
+                    tmem_st32(lanes + LOW_COL_Q + 32 * half, y);
+                    tmem_st32(lanes + LOW_COL_Q + 64 + 32 * half, z);
                 }
+                tmem_wait_st();
+                tc_fence_before_sync();
+            } else {
+                uint8_t* to = sQ + t * C::Q_BYTES + in_block * 128;  // in the layout of a K-major operand
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c)
+                    *reinterpret_cast<uint4*>(to + ((c ^ (in_block & 7)) << 4)) = make_uint4(x_q[c].x ^ a.flip, x_q[c].y ^ a.flip, x_q[c].z ^ a.flip, x_q[c].w ^ a.flip);
+                fence_proxy_async_smem();
             }
-            fence_proxy_async_smem();
             mbar_arrive_warp(&sh.q_full[t], lane);
         }
         float o[64], m = -INFINITY, l = 0.f;
@@ -319,7 +370,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t x[32];
-                    tmem_ld32(lanes + COL_O + (j & 1) * 64 + 32 * half, x);
+                    tmem_ld32(lanes + LOW_COL_O + 32 * half, x);
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
@@ -329,7 +380,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                 }
             };
             for (int j = 0; j < n && wait(sh.s_full, j, W_S, j); ++j) {
-                const uint32_t at_s = lanes + j % 3 * 128;
+                const uint32_t at_s = lanes + j % 3 * 64, at_low = lanes + LOW_COL_LOW + (j & 1) * 64;
                 if (live) {
                     const int lim = (j < n_p ? p_end : limit) - key_of(j);  // columns the row sees
                     uint32_t x[64];
@@ -363,15 +414,15 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                             z[i + 1] = __float_as_uint(w.y - __uint_as_float(x[c + i + 1] & 0xffffe000u));
                         }
                         tmem_st32p(at_s + c, x + c);
-                        tmem_st32(at_s + 64 + c, z);
+                        tmem_st32(at_low + c, z);
                     }
                     l = fmaf(l, alpha, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
                     tmem_wait_st();
                 }
+                if (j > 0) add(j - 1);  // before O_j may come to the same place
+                if (!ok) break;
                 tc_fence_before_sync();
                 mbar_arrive_warp(&sh.p_full[j % 3], lane);
-                if (j > 0) add(j - 1);
-                if (!ok) break;
                 before = alpha;
             }
             if (ok && n > 0) add(n - 1);
@@ -490,7 +541,7 @@ int launch(const ManyArgs& args, int dtype, int64_t blocks, cudaStream_t stream)
     if ((s = prefix_tile_map(&kp, a.Kp, dtype, 1, a.Hk, args.prefix ? a.P : 0, C::KEYS, false)) || (s = prefix_tile_map(&vp, a.Vp, dtype, 1, a.Hk, args.prefix ? a.P : 0, C::KEYS, true)) ||
         (s = prefix_tile_map(&k, a.K, dtype, a.B, a.Hk, args.own ? a.S : 0, C::KEYS, false)) || (s = prefix_tile_map(&v, a.V, dtype, a.B, a.Hk, args.own ? a.S : 0, C::KEYS, true)))
         return s;
-    LaunchConfig lc((unsigned)blocks, Many<X>::THREADS, Many<X>::SMEM, stream, 1, true);
+    LaunchConfig lc((unsigned)blocks, MANY_THREADS, Many<X>::SMEM, stream, 1, true);
     if (cudaLaunchKernelEx(&lc.cfg, prefix_many_kernel<X>, kp, vp, k, v, args) != cudaSuccess) return check_launch();
     count_launch();
     return HK_OK;
