@@ -83,6 +83,20 @@ struct ManyArgs {
     int tiles;         // items of row blocks: of a key head, or of a request's
 };
 
+// 2^x of two numbers, for x >= -126, without the special function unit, which is what the softmax of 16-bit types is bound by: x is
+// split into the nearest whole number, which goes to the exponent, and the rest, of whose power a polynomial (least relative error on
+// [-1/2, 1/2], found by reweighted least squares) is 2.7e-6 off.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    const float2 big = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);  // 1.5 * 2^23
+    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+    const float2 t = __fadd2_rn(x, big), n = __fadd2_rn(t, minus), f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 p = __ffma2_rn(f, make_float2(9.5701022e-3f, 9.5701022e-3f), make_float2(5.5917859e-2f, 5.5917859e-2f));
+    p = __ffma2_rn(p, f, make_float2(0.24024744f, 0.24024744f));
+    p = __ffma2_rn(p, f, make_float2(0.69312179f, 0.69312179f));
+    p = __ffma2_rn(p, f, make_float2(0.99999928f, 0.99999928f));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 template <class X>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
 prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_k,
@@ -152,8 +166,6 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     auto by_hand = [&](int i) { return !LOW && i == 2 * n - 1 && n > n_p; };
     // Tiles go through the ring in the order of their use, keys a tile (fp32: two) ahead: K0 .. K(A) V0 K(A+1) V1 ..
     constexpr int A = C::AHEAD;
-    auto entry_k = [](int j) { return j + max(0, j - A); };
-    auto entry_v = [&](int j) { return j + min(n, A + 1 + j); };
     struct Entry {
         int j;
         bool v;
@@ -220,11 +232,11 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
         } else if (warp == 1) {
             // ------------------------------ products ------------------------------
             const uint32_t leader = elect_one_sync();
-            const int total = n * streams;
-            const int ahead = A * streams;  // products that S is ahead of O
+            const int total = n * streams, ahead = A * streams;  // products, and those that S is ahead of O
             bool ok = true;
             // The tensor pipe queues next to nothing, and a wait takes some 100 cycles even when its barrier is long complete: each
-            // is looked at while the products before it are still being issued, and waited for if that look came too early.
+            // is looked at while the products before it are still being issued, and waited for if that look came too early.  For
+            // the same reason nothing is divided here: the tiles come in the order of the ring.
             struct Barrier {
                 uint64_t* bar;
                 uint32_t parity;
@@ -233,84 +245,104 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             auto wait = [&](bool was_seen, const Barrier& x, int id, int aux) {
                 return __all_sync(0xffffffffu, was_seen) || (bool)__all_sync(0xffffffffu, mbar_wait(wc, x.bar, x.parity, id, aux));
             };
-            auto tile_barrier = [&](int i) -> Barrier {
-                const int s = i % SLOTS;
-                if constexpr (LOW) return {&sh.kv_ready[s], (uint32_t)(i / SLOTS) & 1u};
-                return by_hand(i) ? Barrier{&sh.last_ready, 0u} : Barrier{&sh.kv_full[s], (uint32_t)(i / SLOTS) & 1u};
+            struct Cursor {
+                int at;
+                uint32_t phase;
+                __device__ __forceinline__ void next(int n) {
+                    if (++at == n) {
+                        at = 0;
+                        phase ^= 1u;
+                    }
+                }
+            };
+            Cursor tile{0, 0u}, p{0, 0u};  // the next tile in the ring, the next weights
+            int s_buf = 0, k_slot = 0, v_slot = 0;
+            int t_s = 0, t_o = 0, v_left = n;  // block of rows of the next S and O; tiles of values that have not been taken
+            auto tile_barrier = [&](bool v) -> Barrier {
+                if (LOW) return {&sh.kv_ready[tile.at], tile.phase};
+                return v && v_left == 1 && n > n_p ? Barrier{&sh.last_ready, 0u} : Barrier{&sh.kv_full[tile.at], tile.phase};
             };
             bool seen_k = false, seen_v = false, seen_p = false;
-            const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
-            for (int q = 0; q < total + ahead && ok; ++q) {
+            const uint32_t kv_addr = smem_u32(sKV);
+            const Desc q_desc = make_smem_desc(smem_u32(sQ), 16, 1024, DESC_SW128), k_desc = make_smem_desc(kv_addr, 16, 1024, DESC_SW128),
+                       v_desc = LOW ? mnmajor_desc(kv_addr, 0, C::KV_BOX) : make_smem_desc(kv_addr, 16, 1024, DESC_SW128);
+            auto look = [&] {  // for what O needs
+                seen_v = t_o == 0 && seen(tile_barrier(true));
+                seen_p = seen({&sh.p_full[p.at], p.phase});
+            };
+#pragma unroll 1
+            for (int q = 0; q < total + ahead; ++q) {
                 if (q < total) {  // S
-                    const int j = q >> (streams - 1), t = q & (streams - 1), i = entry_k(j);
-                    if (j == 0 && !(ok = wait(false, {&sh.q_full[t], 0u}, W_Q, t))) break;
-                    if (t == 0 && !(ok = wait(seen_k, tile_barrier(i), W_READY, i))) break;
+                    if (q < streams && !(ok = wait(false, {&sh.q_full[t_s], 0u}, W_Q, t_s))) break;
+                    if (t_s == 0) {
+                        if (!(ok = wait(seen_k, tile_barrier(false), W_READY, q))) break;
+                        k_slot = tile.at;
+                        tile.next(SLOTS);
+                    }
                     tc_fence_after_sync();
-                    // what O needs next
-                    const int r = max(q - ahead, 0);
-                    const Barrier v_next = tile_barrier(entry_v(r >> (streams - 1))), p_next = {&sh.p_full[r % 3], (uint32_t)(r / 3) & 1u};
-                    const uint32_t ka = kv_addr + (i % SLOTS) * C::KV_BYTES;
+                    const Desc kd = k_desc + k_slot * C::KV_BYTES;
                     if constexpr (LOW) {
                         constexpr uint32_t IDESC = make_idesc_tf32(TILE, KEYS, false, false);
-                        const uint32_t d = tmem + (q % 3) * 64;
-                        const Desc kd = kmajor_desc(ka, 0, C::KV_BOX);
+                        const uint32_t d = tmem + s_buf * 64;
                         auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
                             umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x, kd + y, IDESC, acc);
                             umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x + 32, kd + (y + C::KV_BOX), IDESC, 1u);
                         };
                         eight(64, 0, 0u);
                         eight(0, C::KV_RAW, 1u);
-                        seen_v = seen(v_next);
-                        seen_p = seen(p_next);
+                        if (q >= ahead) look();
                         eight(0, 0, 1u);
                     } else {
                         constexpr uint32_t IDESC = make_idesc_16(TILE, KEYS, BF16, false);
-                        const uint32_t d = tmem + (q % 3) * 128;
-                        const uint64_t qd = make_smem_desc(q_addr + t * C::Q_BYTES, 16, 1024, DESC_SW128), kd = make_smem_desc(ka, 16, 1024, DESC_SW128);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if (k == 2) {
-                                seen_v = seen(v_next);
-                                seen_p = seen(p_next);
-                            }
-                            umma_ss_16(leader, d, qd + 2 * k, kd + 2 * k, IDESC, k > 0);
-                        }
+                        const uint32_t d = tmem + s_buf * 128;
+                        const Desc qd = q_desc + t_s * C::Q_BYTES;
+                        umma_ss_16(leader, d, qd.d, kd.d, IDESC, 0u);
+                        umma_ss_16(leader, d, qd.d + 2, kd.d + 2, IDESC, 1u);
+                        if (q >= ahead) look();
+                        umma_ss_16(leader, d, qd.d + 4, kd.d + 4, IDESC, 1u);
+                        umma_ss_16(leader, d, qd.d + 6, kd.d + 6, IDESC, 1u);
                     }
-                    umma_commit_lead(leader, &sh.s_full[q % 3]);
-                    if (t == streams - 1) umma_commit_lead(leader, &sh.kv_empty[i % SLOTS]);
+                    umma_commit_lead(leader, &sh.s_full[s_buf]);
+                    if (t_s == streams - 1) umma_commit_lead(leader, &sh.kv_empty[k_slot]);
+                    s_buf = s_buf == 2 ? 0 : s_buf + 1;
+                    t_s ^= streams - 1;
                 }
                 if (q >= ahead) {  // O
-                    const int r = q - ahead, j = r >> (streams - 1), t = r & (streams - 1), i = entry_v(j);
-                    if (t == 0 && !(ok = wait(seen_v, tile_barrier(i), W_READY, i))) break;
-                    if (!(ok = wait(seen_p, {&sh.p_full[r % 3], (uint32_t)(r / 3) & 1u}, W_P, r))) break;
+                    if (t_o == 0) {
+                        if (!(ok = wait(seen_v, tile_barrier(true), W_READY, q))) break;
+                        v_slot = tile.at;
+                        tile.next(SLOTS);
+                        --v_left;
+                    }
+                    if (!(ok = wait(seen_p, {&sh.p_full[p.at], p.phase}, W_P, q))) break;
                     tc_fence_after_sync();
                     seen_v = seen_p = false;
-                    const Barrier k_next = tile_barrier(entry_k(min((q + 1) >> (streams - 1), n - 1)));
-                    const uint32_t va = kv_addr + (i % SLOTS) * C::KV_BYTES;
+                    const bool look_k = t_s == 0 && q + 1 < total;
+                    const Desc vd = v_desc + v_slot * C::KV_BYTES;
                     if constexpr (LOW) {
                         constexpr uint32_t IDESC = make_idesc_tf32(TILE, HEAD_DIM, false, true);
-                        const uint32_t high = tmem + (r % 3) * 64, low = tmem + LOW_COL_LOW + (r & 1) * 64, d = tmem + LOW_COL_O;
-                        const Desc vd = mnmajor_desc(va, 0, C::KV_BOX);
+                        const uint32_t high = tmem + p.at * 64, low = tmem + LOW_COL_LOW + ((q - ahead) & 1) * 64, d = tmem + LOW_COL_O;
                         auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
                             umma_ts4<MNMAJOR_STEP>(leader, d, x, vd + y, IDESC, acc);
                             umma_ts4<MNMAJOR_STEP>(leader, d, x + 32, vd + (y + 4096), IDESC, 1u);
                         };
                         eight(low, 0, 0u);
                         eight(high, C::KV_RAW, 1u);
-                        seen_k = seen(k_next);
+                        seen_k = look_k && seen(tile_barrier(false));
                         eight(high, 0, 1u);
                     } else {
                         constexpr uint32_t IDESC = make_idesc_16(TILE, HEAD_DIM, BF16, true);
-                        const uint32_t p = tmem + (r % 3) * 128, d = tmem + COL_O + t * 64;
-                        const uint64_t vd = make_smem_desc(va, 16, 1024, DESC_SW128);
+                        const uint32_t w = tmem + p.at * 128, d = tmem + COL_O + t_o * 64, acc = q >= ahead + streams;
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            if (k == 4) seen_k = seen(k_next);
-                            umma_ts_16(leader, d, p + 8 * k, vd + (2048 >> 4) * k, IDESC, k > 0 || j > 0);
+                            if (k == 4) seen_k = look_k && seen(tile_barrier(false));
+                            umma_ts_16(leader, d, w + 8 * k, vd.d + (2048 >> 4) * k, IDESC, k > 0 ? 1u : acc);
                         }
                     }
-                    umma_commit_lead(leader, &sh.o_full[r % 3]);
-                    if (t == streams - 1) umma_commit_lead(leader, &sh.kv_empty[i % SLOTS]);
+                    umma_commit_lead(leader, &sh.o_full[p.at]);
+                    if (t_o == streams - 1) umma_commit_lead(leader, &sh.kv_empty[v_slot]);
+                    p.next(3);
+                    t_o ^= streams - 1;
                 }
             }
         } else if (!LOW && warp == 2) {
@@ -430,6 +462,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             // O stays in tensor memory and is scaled there when a maximum has risen by more than 2^RISE: a stale one makes weights
             // larger, which neither fp32 sums nor 16-bit types mind up to there
             constexpr float RISE = 8.f;
+            constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial
             const uint32_t at_o = lanes + COL_O + t * 64;
             uint32_t x[128];
             for (int j = 0; j < n && wait(sh.s_full, j * streams + t, W_S, j); ++j) {
@@ -467,13 +500,19 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                     const float ref = mn == -INFINITY ? 0.f : mn;
                     const float2 nm = make_float2(-ref, -ref);
                     float2 sum[2] = {};
+                    // the weights take the type of the values: half a step of it each
+                    auto weights = [&](auto poly) {
 #pragma unroll
-                    for (int i = 0; i < 128; i += 2) {
-                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, nm);
-                        const float2 w = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-                        sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
-                        x[i / 2] = pack<X>(w.x, w.y);  // the weights take the type of the values: half a step of it each
-                    }
+                        for (int i = 0; i < 128; i += 2) {
+                            const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, nm);
+                            const float2 w = decltype(poly)::value && (i >> 1) % POLY_OF == POLY_OF - 1 ? ex2_poly(e) : make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                            sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
+                            x[i / 2] = pack<X>(w.x, w.y);
+                        }
+                    };
+                    // a masked score is -inf and has no weight at all: not by the polynomial
+                    if (__all_sync(0xffffffffu, lim >= KEYS)) weights(std::true_type{});
+                    else weights(std::false_type{});
                     tmem_st32p(at_s, x);
                     tmem_st32p(at_s + 32, x + 32);
                     l = fmaf(l, alpha, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
