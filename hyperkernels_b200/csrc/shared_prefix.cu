@@ -14,8 +14,22 @@ namespace {
 template <class X>
 __global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_constant__ PrefixArgs a) {
     const int sub = threadIdx.x & 15;
-    const int64_t rows = (int64_t)a.Hk * a.R, row = min((int64_t)blockIdx.x * 8 + (threadIdx.x >> 4), rows - 1);  // the last row more than once
-    const int kvh = (int)(row / a.R), r = (int)(row - (int64_t)kvh * a.R), token = r / a.group, b = token / a.T, t = token - b * a.T, h = kvh * a.group + r - token * a.group;
+    const int64_t rows = a.slot_rows, row = min((int64_t)blockIdx.x * 8 + (threadIdx.x >> 4), rows - 1);  // the last row more than once
+    int kvh, b, r;  // the row among those of its key head and request
+    bool valid = true;
+    if (a.whole) {
+        const int item = a.first_split + (int)(row / a.block_rows), at = item / a.tiles_o;
+        b = at / a.Hk;
+        kvh = at - b * a.Hk;
+        r = (a.tiles_o - 1 - (item - at * a.tiles_o)) * a.block_rows + (int)(row % a.block_rows);
+        valid = r < a.T * a.group;  // the last block of a request is not full
+    } else {
+        kvh = (int)(row / a.R);
+        r = (int)(row - (int64_t)kvh * a.R);
+        b = r / (a.T * a.group);
+        r -= b * a.T * a.group;
+    }
+    const int t = r / a.group, h = kvh * a.group + r - t * a.group;
     pdl_wait();
     pdl_trigger();
     float M = -INFINITY, L = 0.f;
@@ -44,6 +58,7 @@ __global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_consta
             o.x = fmaf(v[i].x, f, o.x); o.y = fmaf(v[i].y, f, o.y); o.z = fmaf(v[i].z, f, o.z); o.w = fmaf(v[i].w, f, o.w);
         }
     }
+    if (!valid) return;
     const float f = L > 0.f ? 1.f / L : 0.f;
     store4(const_cast<X*>(row_of<X>(a.O, b, h, t)) + 4 * sub, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
     if (sub == 0) a.LSE[b * a.lse_sB + h * a.lse_sH + t] = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
@@ -75,62 +90,85 @@ int check(const hk_shared_prefix_params* p) {
     return HK_OK;
 }
 
-// How the work is cut.  The runs of keys depend on sizes, lengths and the number of SMs alone: the same call gives the same bits.
+// How the work is cut.  It depends on sizes, lengths and the number of SMs alone: the same call gives the same bits.
 struct Plan {
     bool prefix_many, own_many;  // which kernels
-    bool whole;                  // a block of rows takes the prefix and the request's own keys in one go
 };
+
+// CTAs of `items` blocks of rows, `tiles` tiles each and four to start and end, on `sms` SMs: the last ones, which do not fill the
+// SMs, in `parts` by their keys (at least four tiles).  In tiles.
+double whole_time(int64_t items, double tiles, int sms, int& parts) {
+    const int64_t full = items / sms, tail = items % sms;
+    double best = 0.0;
+    parts = 1;
+    for (int k = 1; tail > 0 && k <= 8 && (k == 1 || tiles >= 4.0 * k); ++k) {
+        const double time = cdiv(tail * k, sms) * (tiles / k + 4.0) + (k > 1 ? 3.0 : 0.0);
+        if (k > 1 && time >= best) continue;
+        best = time;
+        parts = k;
+    }
+    return full * (tiles + 4.0) + best;
+}
+
 Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
     a.B = p->B; a.Hk = p->nh_kv; a.group = p->nh / p->nh_kv; a.T = (int)p->T; a.P = (int)p->prefix_len; a.S = (int)p->kv_len;
     a.R = p->B * a.T * a.group;
     const int own_rows = a.T * a.group, sms = sm_count();
     const ManyPlan mp = many_plan(p->dtype);
-    Plan plan{a.P > 0 && a.R > 32, own_rows > 16, false};
-    a.splits_p = a.per_p = a.tiles_p = 0;
-    double prefix_time = 0.0;
-    if (a.P > 0 && plan.prefix_many) {
-        // as many runs as make the waves of CTAs shortest, four tiles to start and end one
+    // Many rows: the tensor cores' 128 at a time.  Fewer than 16 (33 against the prefix) are taken faster by the other kernel.
+    Plan plan{a.P > 0 && a.R > 32, own_rows > 16};
+    const FewPlan fp = few_plan(p->dtype, a.R), fo = few_plan(p->dtype, own_rows);
+    a.tiles_o = cdiv(own_rows, plan.own_many ? mp.rows : fo.rows);
+    a.splits_o = a.S > 0 || a.P == 0;  // without keys of their own, the prefix alone
+    const int64_t items_o = (int64_t)a.B * a.Hk * a.tiles_o;
+    // SM time for the requests' own keys, half of their caches, in tiles: of 1.3 us, the other kernel reads at 7 TB/s
+    const double tiles_own = 0.5 * a.S / mp.keys;
+    const double own_time = plan.own_many ? items_o * (tiles_own + 4.0)
+                                          : sms * (2.0 + (double)a.B * a.Hk * a.S * HEAD_DIM * esize(p->dtype) / 7e12 / 1.3e-6);
+    a.whole = a.splits_p = a.per_p = a.tiles_p = 0;
+    double time = 0.0;
+    if (plan.prefix_many) {
+        // as many runs as make the longer of: the waves of CTAs over the prefix; all of the work spread over the SMs
         a.tiles_p = cdiv(a.R, mp.rows);
         const int64_t items = (int64_t)a.Hk * a.tiles_p;
         const int most = std::min(64, std::max(1, cdiv(a.P, 2 * mp.keys)));
         for (int n = 1; n <= most; ++n) {
             const int tiles = cdiv(cdiv(a.P, n), mp.keys);
-            const double time = (double)cdiv(items * n, sms) * (tiles + 4) + 0.25 * n;
-            if (n > 1 && time >= prefix_time) continue;
-            prefix_time = time;
+            const double t = std::max((double)cdiv(items * n, sms) * (tiles + 4), (items * n * (tiles + 4) + own_time) / sms) + 0.25 * n;
+            if (n > 1 && t >= time) continue;
+            time = t;
             a.per_p = tiles * mp.keys;
         }
         a.splits_p = cdiv(a.P, a.per_p);
     } else if (a.P > 0) {
-        const FewPlan fp = few_plan(p->dtype, a.R);
         a.tiles_p = cdiv(a.R, fp.rows);
         const int64_t items = (int64_t)a.Hk * a.tiles_p, places = sms * fp.per_sm;
         const int n = (int)std::max<int64_t>(1, std::min<int64_t>({64, places / items, cdiv(a.P, 4 * fp.step)}));
         a.per_p = cdiv(cdiv(a.P, n), fp.step) * fp.step;
         a.splits_p = cdiv(a.P, a.per_p);
     }
-    a.splits_o = a.S > 0 || a.P == 0;  // without keys of their own, the prefix alone
-    if (plan.own_many) {
-        a.tiles_o = cdiv(own_rows, mp.rows);
-        const int64_t items = (int64_t)a.B * a.Hk * a.tiles_o;
-        // the prefix again for every request, or once and its results through memory: in tiles, as above
-        const double whole = (double)cdiv(items, sms) * cdiv(a.P, mp.keys);
-        if (a.P > 0 && plan.prefix_many && whole <= prefix_time + 4) {
-            plan.whole = true;
-            a.splits_p = a.per_p = a.tiles_p = 0;
-            a.splits_o = 1;
-        }
-    } else {
-        const FewPlan fo = few_plan(p->dtype, own_rows);
-        a.tiles_o = cdiv(own_rows, fo.rows);
-        const int64_t items = (int64_t)a.B * a.Hk * a.tiles_o, places = sms * fo.per_sm;
-        while (a.splits_o > 0 && a.splits_o < 16 && items * a.splits_o * 2 <= places && a.splits_o * 2 * 4 * fo.step <= a.S) a.splits_o *= 2;
+    int parts = 1;
+    if (plan.own_many && plan.prefix_many && whole_time(items_o, (double)a.P / mp.keys + tiles_own, sms, parts) <= time + 3.0) {
+        // every block of rows takes the prefix: no more often than once for 128 or 256 rows, and nothing goes through memory
+        a.whole = 1;
+        a.splits_p = a.per_p = a.tiles_p = 0;
+        a.splits_o = 1;
+        a.slots = parts;
+        a.first_split = (int)(parts > 1 ? items_o / sms * sms : items_o);
+        a.block_rows = mp.rows;
+        a.slot_rows = (items_o - a.first_split) * mp.rows;
+        return plan;
+    }
+    if (!plan.own_many) {
+        const int64_t places = sms * fo.per_sm;
+        while (a.splits_o > 0 && a.splits_o < 16 && items_o * a.splits_o * 2 <= places && a.splits_o * 2 * 4 * fo.step <= a.S) a.splits_o *= 2;
     }
     a.slots = a.splits_p + a.splits_o;
+    a.slot_rows = (int64_t)a.Hk * a.R;
     return plan;
 }
-// rows of slots in the workspace
-size_t slot_rows(const PrefixArgs& a) { return a.slots > 1 ? (size_t)a.slots * a.Hk * a.R : 0; }
+// rows of all slots in the workspace
+size_t slot_rows(const PrefixArgs& a) { return a.slots > 1 ? (size_t)a.slots * a.slot_rows : 0; }
 constexpr size_t SLOT_BYTES = 64 * sizeof(float) + sizeof(float2);
 
 }  // namespace
@@ -184,11 +222,11 @@ int hk_shared_prefix_attention(const hk_shared_prefix_params* p, void* stream_) 
     a.status = device_status_ptr();
     if (!a.status) return HK_ERR_CUDA;
     if (a.splits_p > 0 && (rc = plan.prefix_many ? launch_prefix_many(a, p->dtype, stream) : launch_prefix_few(a, p->dtype, stream))) return rc;
-    if (a.splits_o > 0 && (rc = plan.own_many ? launch_own_many(a, p->dtype, plan.whole, stream) : launch_own_few(a, p->dtype, stream))) return rc;
+    if (a.splits_o > 0 && (rc = plan.own_many ? launch_own_many(a, p->dtype, stream) : launch_own_few(a, p->dtype, stream))) return rc;
     if (a.slots == 1) return HK_OK;
     typedef void (*Kernel)(PrefixArgs);
     static const Kernel combine[] = {prefix_combine_kernel<float>, prefix_combine_kernel<__nv_bfloat16>, prefix_combine_kernel<__half>};
-    LaunchConfig lc((unsigned)cdiv((int64_t)a.Hk * a.R, 8), 128, 0, stream, 1, true);
+    LaunchConfig lc((unsigned)cdiv(a.slot_rows, 8), 128, 0, stream, 1, true);
     if (cudaLaunchKernelEx(&lc.cfg, combine[p->dtype], a) != cudaSuccess) return check_launch();
     count_launch();
     return HK_OK;

@@ -22,7 +22,11 @@ struct PrefixArgs {
     int splits_p, per_p, tiles_p;  // over the prefix: runs of keys, keys of a run, row tiles of a key head
     int splits_o, tiles_o;         // over the requests' own keys
     int slots;                     // of a row; one: the result is written where it is worked out
-    float2* ml;                    // [slots][Hk * R]
+    // Blocks of rows that take the prefix and the request's own keys in one go (`whole`): the last ones, which would not fill the
+    // SMs, in parts of their keys, as many as there are slots.  Only they have slots then, block by block.
+    int whole, first_split, block_rows;
+    int64_t slot_rows;             // rows that have slots
+    float2* ml;                    // [slots][slot_rows]
     float* part;                   // the same, [64]
     DeviceStatus* status;
 };
@@ -63,6 +67,6 @@ struct ManyPlan {
 };
 ManyPlan many_plan(int dtype);
 int launch_prefix_many(const PrefixArgs& a, int dtype, cudaStream_t stream);
-int launch_own_many(const PrefixArgs& a, int dtype, bool prefix, cudaStream_t stream);  // prefix: its keys are taken first
+int launch_own_many(const PrefixArgs& a, int dtype, cudaStream_t stream);  // and the prefix's before them, if `whole`
 
 }  // namespace hk

@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Rows::CTAS) prefix_few_kernel(
         if (++get == Rows::STAGES) get = 0, phase ^= 1u;
         w.batch(from, lane, key0, end, a.scale_log2e, copy_next);
     }
-    const int64_t slot0 = (int64_t)kvh * a.R + row0, slot_rows = (int64_t)a.Hk * a.R;
+    const int64_t slot0 = (int64_t)kvh * a.R + row0, slot_rows = a.slot_rows;
     __syncthreads();  // the ring is the warps' exchange now: every copy has been waited for
     w.finish(sh.part, sh.ml, warp, lane);
     __syncthreads();

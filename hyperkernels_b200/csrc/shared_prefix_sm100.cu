@@ -54,6 +54,7 @@ struct Many {
     static constexpr int STREAMS = LOW ? 1 : 2;      // blocks of rows
     static constexpr int KEYS = LOW ? 64 : 128;      // of a tile
     static constexpr int SLOTS = LOW ? 7 : 8;
+    static constexpr int THREADS = LOW ? 320 : 384;
     static constexpr int AHEAD = LOW ? 2 : 1;        // tiles that the scores are ahead of the weighted values
     static constexpr int Q_BYTES = LOW ? 0 : TILE * 64 * (int)sizeof(X);  // fp32: in tensor memory
     static constexpr int KV_RAW = KEYS * 64 * (int)sizeof(X), KV_BYTES = KV_RAW * (LOW ? 2 : 1);
@@ -68,7 +69,6 @@ struct Many {
     static constexpr int OFF_KV = STREAMS * Q_BYTES, OFF_SH = OFF_KV + SLOTS * KV_BYTES, SMEM = OFF_SH + (int)sizeof(Shared);
     static_assert(SMEM <= 232448, "exceeds the 227 KiB a CTA may opt in to");
 };
-constexpr int MANY_THREADS = 384;
 // Tensor memory.  16-bit types: three buffers of 128 columns for scores and weights, O of two blocks of rows.  fp32: three buffers of
 // 64 for scores and weights, two for the weights' low parts, O of a tile, Q and its low parts.
 constexpr uint32_t COL_O = 384, LOW_COL_LOW = 192, LOW_COL_O = 320, LOW_COL_Q = 384;
@@ -98,7 +98,7 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
 }
 
 template <class X>
-__global__ void __launch_bounds__(MANY_THREADS, 1)
+__global__ void __launch_bounds__(Many<X>::THREADS, 1)
 prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ManyArgs args) {
     typedef Many<X> C;
@@ -135,7 +135,16 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     if (!args.late) pdl_wait();
     pdl_trigger();
     // the item: rows
-    const int ns = args.own ? 1 : a.splits_p, item = blockIdx.x / ns, split = blockIdx.x - item * ns, at = item / args.tiles;
+    int item = blockIdx.x, split = 0, parts = 1;
+    if (!args.own) {
+        item = blockIdx.x / a.splits_p;
+        split = blockIdx.x - item * a.splits_p;
+    } else if (a.whole && item >= a.first_split) {
+        parts = a.slots;
+        item = a.first_split + (blockIdx.x - a.first_split) / parts;
+        split = (blockIdx.x - a.first_split) % parts;
+    }
+    const int at = item / args.tiles;
     const int tile = args.tiles - 1 - (item - at * args.tiles);  // the last rows see the most keys
     const int b = args.own ? at / a.Hk : 0, kvh = at - b * a.Hk, BLOCK = C::STREAMS * TILE;
     const int all = args.own ? a.T * a.group : a.R, first = tile * BLOCK, row0 = b * a.T * a.group + first, rows = min(BLOCK, all - first);
@@ -143,18 +152,33 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     // a row of Q to a softmax thread
     const int t = (warp - 4) >> 2, quarter = warp & 3, in_block = quarter * 32 + lane, r = t * TILE + in_block;
     const bool valid = warp >= 4 && r < rows;
-    const int row = row0 + r, token = row / a.group, bq = args.own ? b : token / a.T, tok = token - bq * a.T, h = kvh * a.group + row - token * a.group;
+    struct Where {
+        int b, h, t;
+    };
+    auto where = [&](int row) -> Where {  // row of the key head
+        const int token = row / a.group, bq = args.own ? b : token / a.T;
+        return {bq, kvh * a.group + row - token * a.group, token - bq * a.T};
+    };
     constexpr int CHUNKS = 64 * sizeof(X) / 16;
     uint4 x_q[CHUNKS];
     if (warp >= 4) {
-        const uint4* from = reinterpret_cast<const uint4*>(row_of<X>(a.Q, valid ? bq : 0, valid ? h : 0, valid ? tok : 0));
+        const Where at_q = valid ? where(row0 + r) : Where{0, 0, 0};
+        const uint4* from = reinterpret_cast<const uint4*>(row_of<X>(a.Q, at_q.b, at_q.h, at_q.t));
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) x_q[c] = valid ? from[c] : make_uint4(0, 0, 0, 0);
     }
     // and keys: tiles of the prefix, then the request's own
-    const int p_begin = args.own ? 0 : split * a.per_p, p_end = !args.prefix ? 0 : args.own ? a.P : min(a.P, p_begin + a.per_p);
+    int p_begin = args.own ? 0 : split * a.per_p, own_begin = 0;
+    const int p_end = !args.prefix ? 0 : args.own ? a.P : min(a.P, p_begin + a.per_p);
     const int seen = args.own ? token_keys(a, len, (first + rows - 1) / a.group) : 0;
-    const int n_p = (p_end - p_begin + KEYS - 1) / KEYS, n = n_p + (seen + KEYS - 1) / KEYS;
+    int n_p = (p_end - p_begin + KEYS - 1) / KEYS, n = n_p + (seen + KEYS - 1) / KEYS;
+    if (parts > 1) {  // a run of the block's tiles
+        const int per = (n + parts - 1) / parts, from = min(n, split * per);
+        own_begin = max(0, from - n_p) * KEYS;
+        p_begin = from * KEYS;
+        n = min(per, n - from);
+        n_p = min(n, max(0, n_p - from));
+    }
     const int streams = C::STREAMS == 2 && rows > TILE ? 2 : 1;
     __syncthreads();
     tc_fence_after_sync();
@@ -176,7 +200,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
         return k < 2 * (n - A - 1) ? (k & 1 ? Entry{A + 1 + (k >> 1), false} : Entry{k >> 1, true}) : Entry{i - n, true};
     };
     // first key of tile j, in the prefix or of the request's own
-    auto key_of = [&](int j) { return j < n_p ? p_begin + j * KEYS : (j - n_p) * KEYS; };
+    auto key_of = [&](int j) { return j < n_p ? p_begin + j * KEYS : own_begin + (j - n_p) * KEYS; };
 
     // What the tiles need beside the loads.  Rows behind the request's last key may hold anything, and 0 times a NaN is one: they are
     // cleared among the values.  fp32: the tiles' low parts, by two pairs of warps, every other tile each.
@@ -211,7 +235,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     };
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        if constexpr (!LOW) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         if (warp == 0) {
             // ------------------------------ tiles of keys and values ------------------------------
             if (lane == 0) {
@@ -345,19 +369,19 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                     t_o ^= streams - 1;
                 }
             }
-        } else if (!LOW && warp == 2) {
+        } else if (LOW) {
+            tend(threadIdx.x & 63, 0);
+        } else if (warp == 2) {
             tend(lane, 2 * n - 1);
         }
     } else if (LOW && warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 128;\n");
-        tend(threadIdx.x & 63, (warp >> 1) & 1);
+        tend(threadIdx.x & 63, 1);
     } else {
         // ------------------------------ softmax ------------------------------
-        if constexpr (LOW) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n");
-        else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+        if constexpr (!LOW) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const bool live = t * TILE + quarter * 32 < rows;
-        const int limit = args.own && valid ? token_keys(a, len, tok) : 0;  // own keys the row sees
+        const int limit = args.own && valid ? token_keys(a, len, (first + r) / a.group) : 0;  // own keys the row sees
         if (t < streams) {  // the row of Q
             if constexpr (LOW) {
 #pragma unroll
@@ -530,16 +554,19 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             }
         }
         if (valid && ok) {
-            const int64_t slot = (int64_t)kvh * a.R + row, slot_rows = (int64_t)a.Hk * a.R;
-            if (a.slots > 1) {
-                const int64_t at_slot = (args.own ? a.splits_p : split) * slot_rows + slot;
+            int row = row0 + r;
+            asm volatile("" : "+r"(row));  // worked out again, not kept in registers all the while
+            if (a.whole ? parts > 1 : a.slots > 1) {
+                const int64_t at_slot = a.whole ? split * a.slot_rows + (int64_t)(item - a.first_split) * BLOCK + r
+                                                : (args.own ? a.splits_p : split) * a.slot_rows + (int64_t)kvh * a.R + row;
                 a.ml[at_slot] = make_float2(m, l);
                 float4* to = reinterpret_cast<float4*>(a.part + at_slot * 64);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             } else {
                 const float f = l > 0.f ? 1.f / l : 0.f;
-                uint4* to = reinterpret_cast<uint4*>(const_cast<X*>(row_of<X>(a.O, bq, h, tok)));
+                const Where to_row = where(row);
+                uint4* to = reinterpret_cast<uint4*>(const_cast<X*>(row_of<X>(a.O, to_row.b, to_row.h, to_row.t)));
                 if constexpr (LOW) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
@@ -550,7 +577,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                         to[i] = make_uint4(pack<X>(o[8 * i] * f, o[8 * i + 1] * f), pack<X>(o[8 * i + 2] * f, o[8 * i + 3] * f),
                                            pack<X>(o[8 * i + 4] * f, o[8 * i + 5] * f), pack<X>(o[8 * i + 6] * f, o[8 * i + 7] * f));
                 }
-                a.LSE[bq * a.lse_sB + h * a.lse_sH + tok] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+                a.LSE[to_row.b * a.lse_sB + to_row.h * a.lse_sH + to_row.t] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
             }
         }
     }
@@ -580,7 +607,7 @@ int launch(const ManyArgs& args, int dtype, int64_t blocks, cudaStream_t stream)
     if ((s = prefix_tile_map(&kp, a.Kp, dtype, 1, a.Hk, args.prefix ? a.P : 0, C::KEYS, false)) || (s = prefix_tile_map(&vp, a.Vp, dtype, 1, a.Hk, args.prefix ? a.P : 0, C::KEYS, true)) ||
         (s = prefix_tile_map(&k, a.K, dtype, a.B, a.Hk, args.own ? a.S : 0, C::KEYS, false)) || (s = prefix_tile_map(&v, a.V, dtype, a.B, a.Hk, args.own ? a.S : 0, C::KEYS, true)))
         return s;
-    LaunchConfig lc((unsigned)blocks, MANY_THREADS, Many<X>::SMEM, stream, 1, true);
+    LaunchConfig lc((unsigned)blocks, Many<X>::THREADS, Many<X>::SMEM, stream, 1, true);
     if (cudaLaunchKernelEx(&lc.cfg, prefix_many_kernel<X>, kp, vp, k, v, args) != cudaSuccess) return check_launch();
     count_launch();
     return HK_OK;
@@ -595,8 +622,9 @@ ManyPlan many_plan(int dtype) { return dtype == HK_F32 ? ManyPlan{TILE, 64} : Ma
 int launch_prefix_many(const PrefixArgs& a, int dtype, cudaStream_t stream) {
     return launch(ManyArgs{a, 0, 1, 0, a.tiles_p}, dtype, (int64_t)a.Hk * a.tiles_p * a.splits_p, stream);
 }
-int launch_own_many(const PrefixArgs& a, int dtype, bool prefix, cudaStream_t stream) {
-    return launch(ManyArgs{a, 1, prefix, !prefix && a.splits_p > 0, a.tiles_o}, dtype, (int64_t)a.B * a.Hk * a.tiles_o, stream);
+int launch_own_many(const PrefixArgs& a, int dtype, cudaStream_t stream) {
+    const int64_t items = (int64_t)a.B * a.Hk * a.tiles_o;
+    return launch(ManyArgs{a, 1, a.whole, !a.whole && a.splits_p > 0, a.tiles_o}, dtype, a.whole ? a.first_split + (items - a.first_split) * a.slots : items, stream);
 }
 
 }  // namespace hk
