@@ -147,6 +147,14 @@ Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
         a.per_p = cdiv(cdiv(a.P, n), fp.step) * fp.step;
         a.splits_p = cdiv(a.P, a.per_p);
     }
+    // Small calls: up to six batches a warp take less than two more launches do (B4 H12, 333 + 64 keys: TIMES us).
+    if (!plan.own_many && a.P > 0 && items_o <= sms && a.P + a.S <= 6 * (own_rows <= 2 && p->dtype == HK_F32 ? 4 : 2) * fo.step) {
+        a.whole = 1;
+        a.splits_p = a.per_p = a.tiles_p = 0;
+        a.splits_o = a.slots = 1;
+        plan.prefix_many = false;
+        return plan;
+    }
     int parts = 1;
     if (plan.own_many && plan.prefix_many && whole_time(items_o, (double)a.P / mp.keys + tiles_own, sms, parts) <= time + 3.0) {
         // every block of rows takes the prefix: no more often than once for 128 or 256 rows, and nothing goes through memory

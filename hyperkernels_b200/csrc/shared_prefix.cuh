@@ -22,8 +22,8 @@ struct PrefixArgs {
     int splits_p, per_p, tiles_p;  // over the prefix: runs of keys, keys of a run, row tiles of a key head
     int splits_o, tiles_o;         // over the requests' own keys
     int slots;                     // of a row; one: the result is written where it is worked out
-    // Blocks of rows that take the prefix and the request's own keys in one go (`whole`): the last ones, which would not fill the
-    // SMs, in parts of their keys, as many as there are slots.  Only they have slots then, block by block.
+    // Blocks of rows that take the prefix and the request's own keys in one go (`whole`): of many rows the last ones, which would not
+    // fill the SMs, in parts of their keys, as many as there are slots.  Only they have slots then, block by block.
     int whole, first_split, block_rows;
     int64_t slot_rows;             // rows that have slots
     float2* ml;                    // [slots][slot_rows]
@@ -60,7 +60,7 @@ struct FewPlan {
 };
 FewPlan few_plan(int dtype, int rows);
 int launch_prefix_few(const PrefixArgs& a, int dtype, cudaStream_t stream);
-int launch_own_few(const PrefixArgs& a, int dtype, cudaStream_t stream);
+int launch_own_few(const PrefixArgs& a, int dtype, cudaStream_t stream);   // and the prefix's before them, if `whole`
 struct ManyPlan {
     int rows;  // of a CTA's blocks
     int keys;  // of a tile

@@ -66,11 +66,12 @@ struct FewMath<float> {
     static __device__ __forceinline__ int key_v(int i, int c) { return c + 4 * (i >> 1); }
     static __device__ __forceinline__ int key_s(int, int c, int e) { return c + 4 * (e & 1); }  // of a lane's scores
     uint32_t qh[8][4], ql[8][4];
-    __device__ __forceinline__ void load_q(const float* lo, const float* hi, int c, uint32_t flip) {
+    static constexpr int Q_WORDS = 4;
+    static __device__ __forceinline__ int at_q(int i, int c) { return 16 * i + 4 * c; }
+    __device__ __forceinline__ void set_q(const uint4 (&lo)[4], const uint4 (&hi)[4], uint32_t flip) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint4 z = make_uint4(0, 0, 0, 0);
-            const uint4 a = lo ? *reinterpret_cast<const uint4*>(lo + 16 * i + 4 * c) : z, b = hi ? *reinterpret_cast<const uint4*>(hi + 16 * i + 4 * c) : z;
+            const uint4 &a = lo[i], &b = hi[i];
             const uint32_t q[2][4] = {{a.x ^ flip, b.x ^ flip, a.y ^ flip, b.y ^ flip}, {a.z ^ flip, b.z ^ flip, a.w ^ flip, b.w ^ flip}};
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -147,11 +148,12 @@ struct FewMath {
     static __device__ __forceinline__ int key_v(int i, int c) { return c + 4 * i; }
     static __device__ __forceinline__ int key_s(int t, int c, int e) { return 8 * t + c + 4 * (e & 1); }
     uint32_t q[4][4];
-    __device__ __forceinline__ void load_q(const X* lo, const X* hi, int c, uint32_t flip) {
+    static constexpr int Q_WORDS = 2;
+    static __device__ __forceinline__ int at_q(int i, int c) { return 32 * i + 8 * c; }
+    __device__ __forceinline__ void set_q(const uint4 (&lo)[2], const uint4 (&hi)[2], uint32_t flip) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint4 z = make_uint4(0, 0, 0, 0);
-            const uint4 a = lo ? *reinterpret_cast<const uint4*>(lo + 32 * i + 8 * c) : z, b = hi ? *reinterpret_cast<const uint4*>(hi + 32 * i + 8 * c) : z;
+            const uint4 &a = lo[i], &b = hi[i];
             q[2 * i][0] = a.x; q[2 * i][1] = b.x; q[2 * i][2] = a.y; q[2 * i][3] = b.y;
             q[2 * i + 1][0] = a.z; q[2 * i + 1][1] = b.z; q[2 * i + 1][2] = a.w; q[2 * i + 1][3] = b.w;
 #pragma unroll
@@ -201,8 +203,16 @@ struct RowsOf16 {
     int limit[2];
     float o[8][4], m[2], l[2];
 
-    __device__ __forceinline__ void start(const X* const (&q)[2], uint32_t flip, int lane) {
-        f.load_q(q[0], q[1], lane & 3, flip);
+    // a lane's pieces of its rows of Q
+    struct Query {
+        uint4 row[2][Math::Q_WORDS];
+        __device__ __forceinline__ void load(int i, const X* from, int lane) {
+#pragma unroll
+            for (int k = 0; k < Math::Q_WORDS; ++k) row[i][k] = from ? *reinterpret_cast<const uint4*>(from + Math::at_q(k, lane & 3)) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    __device__ __forceinline__ void start(const Query& q, uint32_t flip) {
+        f.set_q(q.row[0], q.row[1], flip);
 #pragma unroll
         for (int e = 0; e < 2; ++e) m[e] = -INFINITY, l[e] = 0.f;
 #pragma unroll
@@ -212,19 +222,20 @@ struct RowsOf16 {
     }
     static __device__ __forceinline__ int row(int i, int lane) { return (lane >> 2) + 8 * i; }
     template <class F>
-    __device__ __forceinline__ void batch(const uint8_t* from, int lane, int key0, int end, float scale_log2e, F&& copy_next) {
+    __device__ __forceinline__ void batch(const uint8_t* from, int lane, int key0, int end, bool own, float scale_log2e, F&& copy_next) {
         const int g = lane >> 2, c = lane & 3;
         f.read_k(from, g, c);
         float s[NT][4];
         f.scores(s);
         f.read_v(from + 2048, g, c);
         copy_next();
-        if (!__all_sync(0xffffffffu, key0 + KEYS <= min(limit[0], limit[1]))) {
+        const int last[2] = {own ? limit[0] : end, own ? limit[1] : end};
+        if (!__all_sync(0xffffffffu, key0 + KEYS <= min(last[0], last[1]))) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (key0 + Math::key_s(t, c, e) >= limit[e >> 1]) s[t][e] = -INFINITY;
+                    if (key0 + Math::key_s(t, c, e) >= last[e >> 1]) s[t][e] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; ++i)  // what is behind the last key may be anything: it has no weight, but 0 times a NaN is one
                 if (key0 + Math::key_v(i, c) >= end) f.v[i] = make_uint4(0, 0, 0, 0);
@@ -291,21 +302,24 @@ struct RowsOfOne {
     int limit[N];
 
     static __device__ __forceinline__ int row(int i, int) { return i; }
-    __device__ __forceinline__ void start(const X* const (&from)[N], uint32_t flip, int lane) {
+    struct Query {
+        uint4 row[N];
+        __device__ __forceinline__ void load(int i, const X* from, int lane) {
+            row[i] = from ? *reinterpret_cast<const uint4*>(from + 4 * (lane & 15)) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    __device__ __forceinline__ void start(const Query& from, uint32_t flip) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (from[i]) {
-                const uint4 x = *reinterpret_cast<const uint4*>(from[i] + 4 * (lane & 15));
-                q[i] = make_float4(__uint_as_float(x.x ^ flip), __uint_as_float(x.y ^ flip), __uint_as_float(x.z ^ flip), __uint_as_float(x.w ^ flip));
-            }
+            const uint4& x = from.row[i];
+            q[i] = make_float4(__uint_as_float(x.x ^ flip), __uint_as_float(x.y ^ flip), __uint_as_float(x.z ^ flip), __uint_as_float(x.w ^ flip));
             o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             m[i] = -INFINITY;
             l[i] = 0.f;
         }
     }
     template <class F>
-    __device__ __forceinline__ void batch(const uint8_t* from, int lane, int key0, int end, float scale_log2e, F&& copy_next) {
+    __device__ __forceinline__ void batch(const uint8_t* from, int lane, int key0, int end, bool own, float scale_log2e, F&& copy_next) {
         const bool b3 = lane & 8, b2 = lane & 4;
         float s[N];
         {
@@ -337,7 +351,7 @@ struct RowsOfOne {
         }
 #pragma unroll
         for (int r = 0; r < N; ++r) {
-            if (key >= limit[r]) s[r] = -INFINITY;
+            if (key >= (own ? limit[r] : end)) s[r] = -INFINITY;
             float mx = fmaxf(s[r], __shfl_xor_sync(0xffffffffu, s[r], 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4)) * scale_log2e;
             const float mn = fmaxf(m[r], mx), ref = mn == -INFINITY ? 0.f : mn, alpha = ex2_approx(m[r] - ref);
@@ -365,27 +379,33 @@ struct RowsOfOne {
     }
 };
 
-template <class Rows>
+// What a CTA takes: a run of the prefix's keys; a run of a request's own, by the keys there are; or the whole prefix and all of the
+// request's own, with more warps (small calls, where a second and a third launch would take longer).
+enum FewJob { FEW_PREFIX = 0, FEW_OWN = 1, FEW_WHOLE = 2 };
+template <class Rows, int JOB>
 struct FewShared {
-    static constexpr int PARTS = FEW_WARPS * Rows::PARTS;
+    static constexpr int WARPS = JOB != FEW_WHOLE ? FEW_WARPS : Rows::ROWS < 16 ? 16 : 8, PARTS = WARPS * Rows::PARTS;
     union {
-        uint8_t ring[FEW_WARPS][Rows::STAGES][4096];  // a batch's keys and values
+        uint8_t ring[WARPS][Rows::STAGES][4096];  // a batch's keys and values
         float part[PARTS][Rows::ROWS][64 + 4];
     };
     float2 ml[PARTS][Rows::ROWS];
-    uint64_t full[FEW_WARPS][Rows::STAGES];
+    uint64_t full[WARPS][Rows::STAGES];
     Abort abort;
 };
 
-// A CTA takes a run of the prefix's keys or (OWN) of a request's own, by the keys there are.
 constexpr int W_FEW = 401;
 
-template <class Rows, bool OWN>
-__global__ void __launch_bounds__(FEW_WARPS * 32, Rows::CTAS) prefix_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefixArgs a) {
+template <class Rows, int JOB>
+__global__ void __launch_bounds__(FewShared<Rows, JOB>::WARPS * 32, JOB == FEW_WHOLE ? 1 : Rows::CTAS)
+prefix_few_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefixArgs a) {
     typedef typename Rows::X X;
-    constexpr int N = Rows::ROWS, KEYS = Rows::KEYS, STEP = FEW_WARPS * KEYS, MINE = N < 16 ? N : 2;  // rows that a lane works on
+    typedef FewShared<Rows, JOB> Shared;
+    constexpr bool OWN = JOB != FEW_PREFIX;
+    constexpr int N = Rows::ROWS, KEYS = Rows::KEYS, WARPS = Shared::WARPS, MINE = N < 16 ? N : 2;  // rows that a lane works on
     extern __shared__ __align__(1024) uint8_t few_smem[];
-    FewShared<Rows>& sh = *reinterpret_cast<FewShared<Rows>*>(few_smem);
+    Shared& sh = *reinterpret_cast<Shared*>(few_smem);
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (lane == 0) {
         for (int s = 0; s < Rows::STAGES; ++s) mbar_init(&sh.full[warp][s], 1);
@@ -393,64 +413,70 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Rows::CTAS) prefix_few_kernel(
         fence_mbar_init();
     }
     // Over the requests' own keys: starts under the tail of the kernel over the prefix.  What was before that is complete then.
-    const bool late = OWN && a.splits_p > 0;
+    const bool late = JOB == FEW_OWN && a.splits_p > 0;
     if (!late) pdl_wait();
     pdl_trigger();
-    const int32_t all_keys = OWN && a.lengths ? __ldg(a.lengths + blockIdx.x / a.splits_o / a.tiles_o / a.Hk) : a.S;
     // the rows
-    const int ns = OWN ? a.splits_o : a.splits_p, item = blockIdx.x / ns, split = blockIdx.x - item * ns;
+    const int ns = JOB == FEW_PREFIX ? a.splits_p : JOB == FEW_OWN ? a.splits_o : 1, item = blockIdx.x / ns, split = blockIdx.x - item * ns;
     const int tiles = OWN ? a.tiles_o : a.tiles_p, at = item / tiles, tile = item - at * tiles;
     const int b = OWN ? at / a.Hk : 0, kvh = at - b * a.Hk;
+    const int32_t all_keys = OWN && a.lengths ? __ldg(a.lengths + b) : a.S;
     const int all = OWN ? a.T * a.group : a.R, row0 = b * a.T * a.group + tile * N, rows = min(N, all - tile * N);
-    Rows w;
+    typename Rows::Query query;
     int token_of[MINE];
-    {
-        const X* q[MINE];
 #pragma unroll
-        for (int i = 0; i < MINE; ++i) {
-            const int r = Rows::row(i, lane), row = row0 + r, token = row / a.group, bq = OWN ? b : token / a.T;
-            token_of[i] = r < rows ? token - bq * a.T : a.T;
-            q[i] = r < rows ? row_of<X>(a.Q, bq, kvh * a.group + (row - token * a.group), token_of[i]) : nullptr;
-        }
-        w.start(q, a.flip, lane);
+    for (int i = 0; i < MINE; ++i) {
+        const int r = Rows::row(i, lane), row = row0 + r, token = row / a.group, bq = OWN ? b : token / a.T;
+        token_of[i] = r < rows ? token - bq * a.T : a.T;
+        query.load(i, r < rows ? row_of<X>(a.Q, bq, kvh * a.group + (row - token * a.group), token_of[i]) : nullptr, lane);
     }
-    // the keys
-    int len = a.P, begin = split * a.per_p, end = min(a.P, begin + a.per_p);
-    if (OWN) {
+    // the keys: batches of the prefix, then of the request's own
+    int p_begin = 0, p_end = 0, o_begin = 0, o_end = 0, len = 0;
+    if (JOB == FEW_PREFIX) {
+        p_begin = split * a.per_p;
+        p_end = min(a.P, p_begin + a.per_p);
+    } else {
         len = min(max(all_keys, 0), a.S);
         const int seen = token_keys(a, len, (tile * N + rows - 1) / a.group), per = ((seen + ns - 1) / ns + KEYS - 1) / KEYS * KEYS;
-        begin = min(seen, split * per);
-        end = min(seen, begin + per);
+        o_begin = min(seen, split * per);
+        o_end = min(seen, o_begin + per);
+        if (JOB == FEW_WHOLE) p_end = a.P;
     }
-    int put = 0, put_key = begin + warp * KEYS;
+    const int n_p = (p_end - p_begin + KEYS - 1) / KEYS, n = n_p + (o_end - o_begin + KEYS - 1) / KEYS;
+    auto key_of = [&](int i) { return i < n_p ? p_begin + i * KEYS : o_begin + (i - n_p) * KEYS; };
+    int put = 0, put_at = warp;
     auto copy_next = [&] {  // the next batch of this warp, if there is one, into the slot that its lanes have read
         __syncwarp();
-        if (put_key < end && lane == 0) {
+        if (put_at < n && lane == 0) {
+            const bool own = JOB == FEW_OWN || (JOB == FEW_WHOLE && put_at >= n_p);
             uint64_t* full = &sh.full[warp][put];
             uint8_t* to = sh.ring[warp][put];
             mbar_arrive_expect_tx(full, 4096);
-            tma_load_tile(to, &map_k, full, put_key, kvh, b);
-            tma_load_tile(to + 2048, &map_v, full, put_key, kvh, b);
+            tma_load_tile(to, own ? &map_k : &map_kp, full, key_of(put_at), kvh, own ? b : 0);
+            tma_load_tile(to + 2048, own ? &map_v : &map_vp, full, key_of(put_at), kvh, own ? b : 0);
         }
-        put_key += STEP;
+        put_at += WARPS;
         put = put + 1 == Rows::STAGES ? 0 : put + 1;
     };
 #pragma unroll
     for (int i = 0; i < Rows::STAGES - 1; ++i) copy_next();
+    Rows w;
+    w.start(query, a.flip);
 #pragma unroll
-    for (int i = 0; i < MINE; ++i) w.limit[i] = OWN && token_of[i] < a.T ? min(end, token_keys(a, len, token_of[i])) : end;
+    for (int i = 0; i < MINE; ++i) w.limit[i] = OWN && token_of[i] < a.T ? min(o_end, token_keys(a, len, token_of[i])) : o_end;
     __syncthreads();  // the record of waits that gave up
     WaitNote wc{&sh.abort};
     int get = 0;
     uint32_t phase = 0;
-    for (int key0 = begin + warp * KEYS; key0 < end; key0 += STEP) {
-        if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.full[warp][get], phase, W_FEW, key0))) {
+    for (int i = warp; i < n; i += WARPS) {
+        if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.full[warp][get], phase, W_FEW, i))) {
             for (const unsigned long long t0 = globaltimer_ns(); globaltimer_ns() - t0 < 100000ull;) {}  // copies in flight land
             break;
         }
         const uint8_t* from = sh.ring[warp][get];
         if (++get == Rows::STAGES) get = 0, phase ^= 1u;
-        w.batch(from, lane, key0, end, a.scale_log2e, copy_next);
+        const bool own = JOB == FEW_OWN || (JOB == FEW_WHOLE && i >= n_p);
+        w.batch(from, lane, key_of(i), own ? o_end : p_end, own, a.scale_log2e, copy_next);
     }
     const int64_t slot0 = (int64_t)kvh * a.R + row0, slot_rows = a.slot_rows;
     __syncthreads();  // the ring is the warps' exchange now: every copy has been waited for
@@ -465,10 +491,10 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Rows::CTAS) prefix_few_kernel(
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
     if (mine) {
 #pragma unroll
-        for (int p = 0; p < FewShared<Rows>::PARTS; ++p) M = fmaxf(M, sh.ml[p][r].x);
+        for (int p = 0; p < Shared::PARTS; ++p) M = fmaxf(M, sh.ml[p][r].x);
         const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
-        for (int p = 0; p < FewShared<Rows>::PARTS; ++p) {
+        for (int p = 0; p < Shared::PARTS; ++p) {
             const float f = ex2_approx(sh.ml[p][r].x - ref);
             L += sh.ml[p][r].y * f;
 #pragma unroll
@@ -476,7 +502,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Rows::CTAS) prefix_few_kernel(
         }
     }
     if (threadIdx.x == 0) report_abort(sh.abort, a.status);
-    if (mine && a.slots > 1) {
+    if (mine && JOB != FEW_WHOLE && a.slots > 1) {
         const int64_t to = (OWN ? a.splits_p + split : split) * slot_rows + slot0 + r;
         if (d == 0) a.ml[to] = make_float2(M, L);
 #pragma unroll
@@ -492,26 +518,27 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, Rows::CTAS) prefix_few_kernel(
     if (late && blockIdx.x == gridDim.x - 1) pdl_wait();  // this kernel is complete when the one over the prefix is
 }
 
-typedef void (*FewKernel)(CUtensorMap, CUtensorMap, PrefixArgs);
+typedef void (*FewKernel)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PrefixArgs);
 struct FewEntry {
     FewKernel kernel;
     size_t smem;
+    int threads;
 };
-template <class Rows, bool OWN>
+template <class Rows, int JOB>
 FewEntry entry() {
-    return {prefix_few_kernel<Rows, OWN>, sizeof(FewShared<Rows>)};
+    return {prefix_few_kernel<Rows, JOB>, sizeof(FewShared<Rows, JOB>), FewShared<Rows, JOB>::WARPS * 32};
 }
-template <bool OWN>
+template <int JOB>
 FewEntry pick(int dtype, int rows) {
-    if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>, OWN>();
-    if (dtype == HK_F16) return entry<RowsOf16<__half>, OWN>();
-    return rows == 1 ? entry<RowsOfOne<1>, OWN>() : rows == 2 ? entry<RowsOfOne<2>, OWN>() : entry<RowsOf16<float>, OWN>();
+    if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>, JOB>();
+    if (dtype == HK_F16) return entry<RowsOf16<__half>, JOB>();
+    return rows == 1 ? entry<RowsOfOne<1>, JOB>() : rows == 2 ? entry<RowsOfOne<2>, JOB>() : entry<RowsOf16<float>, JOB>();
 }
 
-int launch(const FewEntry& k, const PrefixArgs& a, int dtype, bool own, int64_t blocks, cudaStream_t stream) {
+int launch(const FewEntry& k, const PrefixArgs& a, int dtype, bool prefix, bool own, int64_t blocks, cudaStream_t stream) {
     // once per device and kernel: more than 48 KB of shared memory
     static std::mutex mu;
-    static FewKernel known[HK_MAX_DEVICES][16];
+    static FewKernel known[HK_MAX_DEVICES][32];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
     {
@@ -525,14 +552,14 @@ int launch(const FewEntry& k, const PrefixArgs& a, int dtype, bool own, int64_t 
         }
     }
     if (blocks > 0x7fffffffLL) return HK_ERR_BAD_SHAPE;
-    LaunchConfig lc((unsigned)blocks, FEW_WARPS * 32, k.smem, stream, 1, true);
-    CUtensorMap mk, mv;
+    LaunchConfig lc((unsigned)blocks, k.threads, k.smem, stream, 1, true);
+    CUtensorMap kp, vp, mk, mv;
     const int rows = few_plan(dtype, 16).step / FEW_WARPS;
     int rc;
-    if ((rc = own ? prefix_tile_map(&mk, a.K, dtype, a.B, a.Hk, a.S, rows, false) : prefix_tile_map(&mk, a.Kp, dtype, 1, a.Hk, a.P, rows, false)) ||
-        (rc = own ? prefix_tile_map(&mv, a.V, dtype, a.B, a.Hk, a.S, rows, false) : prefix_tile_map(&mv, a.Vp, dtype, 1, a.Hk, a.P, rows, false)))
+    if ((rc = prefix_tile_map(&kp, a.Kp, dtype, 1, a.Hk, prefix ? a.P : 0, rows, false)) || (rc = prefix_tile_map(&vp, a.Vp, dtype, 1, a.Hk, prefix ? a.P : 0, rows, false)) ||
+        (rc = prefix_tile_map(&mk, a.K, dtype, a.B, a.Hk, own ? a.S : 0, rows, false)) || (rc = prefix_tile_map(&mv, a.V, dtype, a.B, a.Hk, own ? a.S : 0, rows, false)))
         return rc;
-    if (cudaLaunchKernelEx(&lc.cfg, k.kernel, mk, mv, a) != cudaSuccess) return check_launch();
+    if (cudaLaunchKernelEx(&lc.cfg, k.kernel, kp, vp, mk, mv, a) != cudaSuccess) return check_launch();
     count_launch();
     return HK_OK;
 }
@@ -544,10 +571,12 @@ FewPlan few_plan(int dtype, int rows) {
     return {rows <= 2 ? rows : 16, FEW_WARPS * 8, rows <= 2 ? RowsOfOne<1>::CTAS : RowsOf16<float>::CTAS};
 }
 int launch_prefix_few(const PrefixArgs& a, int dtype, cudaStream_t stream) {
-    return launch(pick<false>(dtype, few_plan(dtype, a.R).rows), a, dtype, false, (int64_t)a.Hk * a.tiles_p * a.splits_p, stream);
+    return launch(pick<FEW_PREFIX>(dtype, few_plan(dtype, a.R).rows), a, dtype, true, false, (int64_t)a.Hk * a.tiles_p * a.splits_p, stream);
 }
 int launch_own_few(const PrefixArgs& a, int dtype, cudaStream_t stream) {
-    return launch(pick<true>(dtype, few_plan(dtype, a.T * a.group).rows), a, dtype, true, (int64_t)a.B * a.Hk * a.tiles_o * a.splits_o, stream);
+    const int rows = few_plan(dtype, a.T * a.group).rows;
+    if (a.whole) return launch(pick<FEW_WHOLE>(dtype, rows), a, dtype, true, true, (int64_t)a.B * a.Hk * a.tiles_o, stream);
+    return launch(pick<FEW_OWN>(dtype, rows), a, dtype, false, true, (int64_t)a.B * a.Hk * a.tiles_o * a.splits_o, stream);
 }
 
 }  // namespace hk
