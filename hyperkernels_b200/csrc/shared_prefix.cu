@@ -9,12 +9,17 @@ namespace hk {
 namespace {
 
 // ---------------------------------------------------------------------------
-// The slots of each row, added up in their order: 16 lanes a row.
+// The slots of each row, added up in an order of their own: 16 lanes a row, four elements a lane, or a warp, a half of it to every
+// other slot.  What bounds it is the latency of one round of loads and of the launch: up to 16 slots are loaded at once by 16 lanes, 32
+// by a warp (B16 H12, 18 slots of 192 rows: 0.8 us less than 16 lanes take; 3 slots of 7 392 rows: 2 us more).
 // ---------------------------------------------------------------------------
-template <class X>
+template <class X, int HALVES>
 __global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_constant__ PrefixArgs a) {
-    const int sub = threadIdx.x & 15;
-    const int64_t rows = a.slot_rows, row = min((int64_t)blockIdx.x * 8 + (threadIdx.x >> 4), rows - 1);  // the last row more than once
+    constexpr int LANES = 16 * HALVES;
+    const int lane = threadIdx.x & (LANES - 1), half = lane >> 4, sub = lane & 15;
+    const uint32_t together = HALVES == 2 ? 0xffffffffu : threadIdx.x & 16 ? 0xffff0000u : 0xffffu;
+    const int64_t rows = a.slot_rows, row = (int64_t)blockIdx.x * (128 / LANES) + threadIdx.x / LANES;
+    if (row >= rows) return;
     int kvh, b, r;  // the row among those of its key head and request
     bool valid = true;
     if (a.whole) {
@@ -29,39 +34,45 @@ __global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_consta
         b = r / (a.T * a.group);
         r -= b * a.T * a.group;
     }
+    if (!valid) return;
     const int t = r / a.group, h = kvh * a.group + r - t * a.group;
+    X* const O = const_cast<X*>(row_of<X>(a.O, b, h, t)) + 4 * sub;
+    float* const LSE = a.LSE + b * a.lse_sB + h * a.lse_sH + t;
     pdl_wait();
     pdl_trigger();
     float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < a.slots; s0 += 16) {
-        const int k = min(16, a.slots - s0);
-        const float* from = a.part + ((int64_t)s0 * rows + row) * 64 + 4 * sub;
+    for (int s0 = 0; s0 < a.slots; s0 += LANES) {
+        const float2 x = s0 + lane < a.slots ? a.ml[(s0 + lane) * rows + row] : make_float2(-INFINITY, 0.f);  // a lane looks up one slot
+        const float* from = a.part + ((int64_t)(s0 + half) * rows + row) * 64 + 4 * sub;
         float4 v[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            if (i < k) v[i] = *reinterpret_cast<const float4*>(from + i * rows * 64);
-        const float2 x = sub < k ? a.ml[(s0 + sub) * rows + row] : make_float2(-INFINITY, 0.f);  // a lane looks up one slot
+            v[i] = s0 + HALVES * i + half < a.slots ? *reinterpret_cast<const float4*>(from + HALVES * i * rows * 64) : make_float4(0.f, 0.f, 0.f, 0.f);
         float mx = x.x;
 #pragma unroll
-        for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        for (int off = LANES / 2; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(together, mx, off));
         mx = fmaxf(mx, M);
         const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(M - ref), w = x.y == 0.f ? 0.f : ex2_approx(x.x - ref);
         M = mx;
-        L *= old;
+        L = L * old + x.y * w;
         o.x *= old; o.y *= old; o.z *= old; o.w *= old;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            if (i >= k) break;
-            const float f = __shfl_sync(0xffffffffu, w, i, 16), l = __shfl_sync(0xffffffffu, x.y, i, 16);
-            L = fmaf(l, f, L);
+            if (s0 + HALVES * i >= a.slots) break;
+            const float f = __shfl_sync(together, w, HALVES * i + half, LANES);
             o.x = fmaf(v[i].x, f, o.x); o.y = fmaf(v[i].y, f, o.y); o.z = fmaf(v[i].z, f, o.z); o.w = fmaf(v[i].w, f, o.w);
         }
     }
-    if (!valid) return;
+#pragma unroll
+    for (int off = LANES / 2; off > 0; off >>= 1) L += __shfl_xor_sync(together, L, off);
+    if (HALVES == 2) {
+        o.x += __shfl_xor_sync(together, o.x, 16); o.y += __shfl_xor_sync(together, o.y, 16);
+        o.z += __shfl_xor_sync(together, o.z, 16); o.w += __shfl_xor_sync(together, o.w, 16);
+    }
     const float f = L > 0.f ? 1.f / L : 0.f;
-    store4(const_cast<X*>(row_of<X>(a.O, b, h, t)) + 4 * sub, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-    if (sub == 0) a.LSE[b * a.lse_sB + h * a.lse_sH + t] = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
+    if (half == 0) store4(O, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+    if (lane == 0) *LSE = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
 }
 
 int check_sizes(const hk_shared_prefix_params* p) {
@@ -229,13 +240,20 @@ int hk_shared_prefix_attention(const hk_shared_prefix_params* p, void* stream_) 
     a.causal = p->is_causal;
     a.status = device_status_ptr();
     if (!a.status) return HK_ERR_CUDA;
-    if (a.splits_p > 0 && (rc = plan.prefix_many ? launch_prefix_many(a, p->dtype, stream) : launch_prefix_few(a, p->dtype, stream))) return rc;
-    if (a.splits_o > 0 && (rc = plan.own_many ? launch_own_many(a, p->dtype, stream) : launch_own_few(a, p->dtype, stream))) return rc;
+    if (a.splits_p > 0 && a.splits_o > 0 && !plan.prefix_many && !plan.own_many) {
+        rc = launch_both_few(a, p->dtype, stream);
+    } else {
+        if (a.splits_p > 0) rc = plan.prefix_many ? launch_prefix_many(a, p->dtype, stream) : launch_prefix_few(a, p->dtype, stream);
+        if (rc == HK_OK && a.splits_o > 0) rc = plan.own_many ? launch_own_many(a, p->dtype, stream) : launch_own_few(a, p->dtype, stream);
+    }
+    if (rc != HK_OK) return rc;
     if (a.slots == 1) return HK_OK;
     typedef void (*Kernel)(PrefixArgs);
-    static const Kernel combine[] = {prefix_combine_kernel<float>, prefix_combine_kernel<__nv_bfloat16>, prefix_combine_kernel<__half>};
-    LaunchConfig lc((unsigned)cdiv(a.slot_rows, 8), 128, 0, stream, 1, true);
-    if (cudaLaunchKernelEx(&lc.cfg, combine[p->dtype], a) != cudaSuccess) return check_launch();
+    static const Kernel combine[2][3] = {{prefix_combine_kernel<float, 1>, prefix_combine_kernel<__nv_bfloat16, 1>, prefix_combine_kernel<__half, 1>},
+                                         {prefix_combine_kernel<float, 2>, prefix_combine_kernel<__nv_bfloat16, 2>, prefix_combine_kernel<__half, 2>}};
+    const int wide = a.slots > 16;
+    LaunchConfig lc((unsigned)cdiv(a.slot_rows, wide ? 4 : 8), 128, 0, stream, 1, true);
+    if (cudaLaunchKernelEx(&lc.cfg, combine[wide][p->dtype], a) != cudaSuccess) return check_launch();
     count_launch();
     return HK_OK;
 }

@@ -61,6 +61,7 @@ struct FewPlan {
 FewPlan few_plan(int dtype, int rows);
 int launch_prefix_few(const PrefixArgs& a, int dtype, cudaStream_t stream);
 int launch_own_few(const PrefixArgs& a, int dtype, cudaStream_t stream);   // and the prefix's before them, if `whole`
+int launch_both_few(const PrefixArgs& a, int dtype, cudaStream_t stream);  // the two in one launch
 struct ManyPlan {
     int rows;  // of a CTA's blocks
     int keys;  // of a tile

@@ -9,6 +9,7 @@
 // 16-byte pieces it reads, because the order of the contracted index (head dimension, keys) and of the result's columns is free
 // as long as both operands agree on it; the order taken makes every read free of bank conflicts in the layout TMA writes (16-byte
 // piece c of row r at c ^ (r % 8)).  The instructions on tensor memory would need 128 rows to a tile.
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 #include <type_traits>
@@ -40,7 +41,7 @@ __device__ __forceinline__ uint32_t tf32_low(uint32_t x) { return __float_as_uin
 
 constexpr int FEW_WARPS = 4;
 
-// fp32: x = h + l with h the upper 11 bits of the significand; a product is h h' + h l' + l h', added from the small ones on: what
+// fp32: x = h + l with h the upper 11 bits of the significand; a product is h h' + (h l' + l h'): what
 // is left out is 2^-22 of it.  A batch's weighted values are added to the rest in fp32 adds, since the tensor core's own additions
 // cut off instead of rounding.
 // Lane (g, c) = (lane / 4, lane % 4) of a matrix instruction: rows g and g + 8, columns and contracted elements by c.
@@ -94,18 +95,18 @@ struct FewMath<float> {
                 bl[4 * i + e] = tf32_low(w[e]);
             }
         }
-        float lo[4] = {0.f, 0.f, 0.f, 0.f};
+        // three chains of eight instead of one of 24: the instruction's latency is what a batch waits for
+        float lh[4] = {0.f, 0.f, 0.f, 0.f}, hl[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[0][e] = 0.f;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            mma_tf32(s[0], ql[x], b[2 * x], b[2 * x + 1]);
-            mma_tf32(lo, qh[x], bl[2 * x], bl[2 * x + 1]);
+            mma_tf32(s[0], qh[x], b[2 * x], b[2 * x + 1]);
+            mma_tf32(lh, ql[x], b[2 * x], b[2 * x + 1]);
+            mma_tf32(hl, qh[x], bl[2 * x], bl[2 * x + 1]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] += lo[e];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) mma_tf32(s[0], qh[x], b[2 * x], b[2 * x + 1]);
+        for (int e = 0; e < 4; ++e) s[0][e] += lh[e] + hl[e];
     }
     // o[j] = alpha o[j] + p V: rows g, g + 8 of columns n = 2 c, 2 c + 1
     __device__ __forceinline__ void weigh(const float (&p)[1][4], const float (&alpha)[2], bool, float (&o)[8][4]) const {
@@ -397,9 +398,8 @@ struct FewShared {
 constexpr int W_FEW = 401;
 
 template <class Rows, int JOB>
-__global__ void __launch_bounds__(FewShared<Rows, JOB>::WARPS * 32, JOB == FEW_WHOLE ? 1 : Rows::CTAS)
-prefix_few_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_k,
-                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefixArgs a) {
+__device__ __forceinline__ void few_job(const CUtensorMap& map_kp, const CUtensorMap& map_vp, const CUtensorMap& map_k, const CUtensorMap& map_v, const PrefixArgs& a,
+                                        const int block, const bool late) {
     typedef typename Rows::X X;
     typedef FewShared<Rows, JOB> Shared;
     constexpr bool OWN = JOB != FEW_PREFIX;
@@ -412,12 +412,10 @@ prefix_few_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_const
         if (warp == 0) sh.abort.id = 0;
         fence_mbar_init();
     }
-    // Over the requests' own keys: starts under the tail of the kernel over the prefix.  What was before that is complete then.
-    const bool late = JOB == FEW_OWN && a.splits_p > 0;
     if (!late) pdl_wait();
     pdl_trigger();
     // the rows
-    const int ns = JOB == FEW_PREFIX ? a.splits_p : JOB == FEW_OWN ? a.splits_o : 1, item = blockIdx.x / ns, split = blockIdx.x - item * ns;
+    const int ns = JOB == FEW_PREFIX ? a.splits_p : JOB == FEW_OWN ? a.splits_o : 1, item = block / ns, split = block - item * ns;
     const int tiles = OWN ? a.tiles_o : a.tiles_p, at = item / tiles, tile = item - at * tiles;
     const int b = OWN ? at / a.Hk : 0, kvh = at - b * a.Hk;
     const int32_t all_keys = OWN && a.lengths ? __ldg(a.lengths + b) : a.S;
@@ -515,7 +513,25 @@ prefix_few_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_const
         for (int e = 0; e < E; e += 4) store4(to + e, make_float4(acc[e] * f, acc[e + 1] * f, acc[e + 2] * f, acc[e + 3] * f));
         if (d == 0) a.LSE[bq * a.lse_sB + h * a.lse_sH + t] = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
     }
-    if (late && blockIdx.x == gridDim.x - 1) pdl_wait();  // this kernel is complete when the one over the prefix is
+}
+
+// late: runs beside the kernel over the prefix.  What was before that is complete when this one begins, and this one when that is.
+template <class Rows, int JOB>
+__global__ void __launch_bounds__(FewShared<Rows, JOB>::WARPS * 32, JOB == FEW_WHOLE ? 1 : Rows::CTAS)
+prefix_few_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefixArgs a) {
+    const bool late = JOB == FEW_OWN && a.splits_p > 0;
+    few_job<Rows, JOB>(map_kp, map_vp, map_k, map_v, a, blockIdx.x, late);
+    if (late && blockIdx.x == gridDim.x - 1) pdl_wait();
+}
+// The runs of the prefix and those of the requests' own keys in one launch.
+template <class Prefix, class Own>
+__global__ void __launch_bounds__(FEW_WARPS * 32, Prefix::CTAS < Own::CTAS ? Prefix::CTAS : Own::CTAS)
+prefix_few_both_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefixArgs a) {
+    const int n = a.Hk * a.tiles_p * a.splits_p;
+    if ((int)blockIdx.x < n) few_job<Prefix, FEW_PREFIX>(map_kp, map_vp, map_k, map_v, a, blockIdx.x, false);
+    else few_job<Own, FEW_OWN>(map_kp, map_vp, map_k, map_v, a, blockIdx.x - n, false);
 }
 
 typedef void (*FewKernel)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PrefixArgs);
@@ -533,6 +549,18 @@ FewEntry pick(int dtype, int rows) {
     if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>, JOB>();
     if (dtype == HK_F16) return entry<RowsOf16<__half>, JOB>();
     return rows == 1 ? entry<RowsOfOne<1>, JOB>() : rows == 2 ? entry<RowsOfOne<2>, JOB>() : entry<RowsOf16<float>, JOB>();
+}
+
+template <class Prefix, class Own>
+FewEntry both() {
+    return {prefix_few_both_kernel<Prefix, Own>, std::max(sizeof(FewShared<Prefix, FEW_PREFIX>), sizeof(FewShared<Own, FEW_OWN>)), FEW_WARPS * 32};
+}
+FewEntry pick_both(int dtype, int prefix, int own) {  // rows of a tile: own <= prefix
+    if (dtype == HK_BF16) return both<RowsOf16<__nv_bfloat16>, RowsOf16<__nv_bfloat16>>();
+    if (dtype == HK_F16) return both<RowsOf16<__half>, RowsOf16<__half>>();
+    if (prefix == 1) return both<RowsOfOne<1>, RowsOfOne<1>>();
+    if (prefix == 2) return own == 1 ? both<RowsOfOne<2>, RowsOfOne<1>>() : both<RowsOfOne<2>, RowsOfOne<2>>();
+    return own == 1 ? both<RowsOf16<float>, RowsOfOne<1>>() : own == 2 ? both<RowsOf16<float>, RowsOfOne<2>>() : both<RowsOf16<float>, RowsOf16<float>>();
 }
 
 int launch(const FewEntry& k, const PrefixArgs& a, int dtype, bool prefix, bool own, int64_t blocks, cudaStream_t stream) {
@@ -577,6 +605,10 @@ int launch_own_few(const PrefixArgs& a, int dtype, cudaStream_t stream) {
     const int rows = few_plan(dtype, a.T * a.group).rows;
     if (a.whole) return launch(pick<FEW_WHOLE>(dtype, rows), a, dtype, true, true, (int64_t)a.B * a.Hk * a.tiles_o, stream);
     return launch(pick<FEW_OWN>(dtype, rows), a, dtype, false, true, (int64_t)a.B * a.Hk * a.tiles_o * a.splits_o, stream);
+}
+int launch_both_few(const PrefixArgs& a, int dtype, cudaStream_t stream) {
+    return launch(pick_both(dtype, few_plan(dtype, a.R).rows, few_plan(dtype, a.T * a.group).rows), a, dtype, true, true,
+                  (int64_t)a.Hk * a.tiles_p * a.splits_p + (int64_t)a.B * a.Hk * a.tiles_o * a.splits_o, stream);
 }
 
 }  // namespace hk
