@@ -145,7 +145,7 @@ Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
         const int most = std::min(64, std::max(1, cdiv(a.P, 2 * mp.keys)));
         for (int n = 1; n <= most; ++n) {
             const int tiles = cdiv(cdiv(a.P, n), mp.keys);
-            const double t = std::max((double)cdiv(items * n, sms) * (tiles + 4), (items * n * (tiles + 4) + own_time) / sms) + 0.25 * n;
+            const double t = std::max((double)cdiv(items * n, sms) * (tiles + 4), (items * n * (tiles + 4) + own_time) / sms) + 0.05 * n;
             if (n > 1 && t >= time) continue;
             time = t;
             a.per_p = tiles * mp.keys;
