@@ -36,7 +36,8 @@ __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], ui
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t tf32_high(uint32_t x) { return x & 0xffffe000u; }
-__device__ __forceinline__ uint32_t tf32_low(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf32_high(x))); }
+// rounded to nearest where the tensor core cuts off: cut off, with the sign of x, every product would be a little too small
+__device__ __forceinline__ uint32_t tf32_low(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf32_high(x))) + 0x1000u; }
 
 
 constexpr int FEW_WARPS = 4;
@@ -95,18 +96,17 @@ struct FewMath<float> {
                 bl[4 * i + e] = tf32_low(w[e]);
             }
         }
-        // three chains of eight instead of one of 24: the instruction's latency is what a batch waits for
-        float lh[4] = {0.f, 0.f, 0.f, 0.f}, hl[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] = 0.f;
+        // Chains of two and of four, not one of 24: the instruction's latency is what a batch waits for, and an accumulator of scores
+        // (they come to 30 and more before they are scaled) loses up to 2^-23 of itself with every addition.
+        float h[4][4] = {}, m[4][4] = {};
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            mma_tf32(s[0], qh[x], b[2 * x], b[2 * x + 1]);
-            mma_tf32(lh, ql[x], b[2 * x], b[2 * x + 1]);
-            mma_tf32(hl, qh[x], bl[2 * x], bl[2 * x + 1]);
+            mma_tf32(h[x & 3], qh[x], b[2 * x], b[2 * x + 1]);
+            mma_tf32(m[x & 1], ql[x], b[2 * x], b[2 * x + 1]);
+            mma_tf32(m[2 + (x & 1)], qh[x], bl[2 * x], bl[2 * x + 1]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] += lh[e] + hl[e];
+        for (int e = 0; e < 4; ++e) s[0][e] = ((h[0][e] + h[1][e]) + (h[2][e] + h[3][e])) + ((m[0][e] + m[1][e]) + (m[2][e] + m[3][e]));
     }
     // o[j] = alpha o[j] + p V: rows g, g + 8 of columns n = 2 c, 2 c + 1
     __device__ __forceinline__ void weigh(const float (&p)[1][4], const float (&alpha)[2], bool, float (&o)[8][4]) const {

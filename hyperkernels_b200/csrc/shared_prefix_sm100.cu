@@ -48,6 +48,10 @@ __device__ __forceinline__ void umma_ts_16(uint32_t leader, uint32_t d, uint32_t
         : "memory");
 }
 
+// What the tensor core leaves of an fp32 word when it cuts it off to TF32, rounded to nearest, since it is cut off too: always
+// towards zero, every product would be a little too small.
+__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u)) + 0x1000u; }
+
 template <class X>
 struct Many {
     static constexpr bool LOW = sizeof(X) == 4;      // products in three parts
@@ -215,7 +219,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             uint4* raw = reinterpret_cast<uint4*>(sKV + s * C::KV_BYTES);
             if constexpr (LOW) {
                 constexpr int EACH = C::KV_RAW / 16 / 64;
-                auto rest = [](uint32_t v) { return __float_as_uint(__uint_as_float(v) - __uint_as_float(v & 0xffffe000u)); };
+                
                 uint4 *from = raw + me, *low = from + C::KV_RAW / 16, x[EACH];
 #pragma unroll
                 for (int k = 0; k < EACH; ++k) x[k] = from[k * 64];
@@ -225,7 +229,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                         if (((k * 64 + me) & (C::KV_BOX / 16 - 1)) / 8 >= keep) from[k * 64] = x[k] = make_uint4(0, 0, 0, 0);  // row of the box
                 }
 #pragma unroll
-                for (int k = 0; k < EACH; ++k) low[k * 64] = make_uint4(rest(x[k].x), rest(x[k].y), rest(x[k].z), rest(x[k].w));
+                for (int k = 0; k < EACH; ++k) low[k * 64] = make_uint4(tf32_rest(x[k].x), tf32_rest(x[k].y), tf32_rest(x[k].z), tf32_rest(x[k].w));
             } else {
                 for (int k = keep * 8 + me; k < C::KV_RAW / 16; k += 32) raw[k] = make_uint4(0, 0, 0, 0);
             }
@@ -393,7 +397,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                         y[4 * c] = v.x ^ a.flip; y[4 * c + 1] = v.y ^ a.flip; y[4 * c + 2] = v.z ^ a.flip; y[4 * c + 3] = v.w ^ a.flip;
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) z[i] = __float_as_uint(__uint_as_float(y[i]) - __uint_as_float(y[i] & 0xffffe000u));
+                    for (int i = 0; i < 32; ++i) z[i] = tf32_rest(y[i]);
                     tmem_st32(lanes + LOW_COL_Q + 32 * half, y);
                     tmem_st32(lanes + LOW_COL_Q + 64 + 32 * half, z);
                 }
@@ -466,8 +470,8 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                             sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
                             x[c + i] = __float_as_uint(w.x);
                             x[c + i + 1] = __float_as_uint(w.y);
-                            z[i] = __float_as_uint(w.x - __uint_as_float(x[c + i] & 0xffffe000u));
-                            z[i + 1] = __float_as_uint(w.y - __uint_as_float(x[c + i + 1] & 0xffffe000u));
+                            z[i] = tf32_rest(x[c + i]);
+                            z[i + 1] = tf32_rest(x[c + i + 1]);
                         }
                         tmem_st32p(at_s + c, x + c);
                         tmem_st32(at_low + c, z);
