@@ -127,37 +127,44 @@ __device__ __forceinline__ float rms_inverse(const Row8& x, float eps) {
     return rsqrtf(fmaf(sum8(ss), 1.f / 64.f, eps));
 }
 
-// U rows of each of the warp's four groups of lanes are a step.
-template <class X, class Y, int MODE, int U>
+// U rows of each of the warp's four groups of lanes are a step.  TOKENS: the groups take four tokens that follow each other, and each
+// U heads; otherwise all take the same token, and four heads after each other.  Whichever dimension's rows are next to each other in
+// memory: rows of 16 bits, head by head in memory, run at 70 % of the copy rate when a load takes four of them out of four heads.
+template <class X, class Y, int MODE, int U, bool TOKENS>
 __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const __grid_constant__ QkArgs a) {
     constexpr bool KEEPS = MODE == QK_ROTATE && sizeof(X) == 2 && sizeof(Y) == 2, BACK = MODE == QK_NORM_BACK;
-    constexpr int STEP = 4 * U;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane >> 3, sub = lane & 7;
+    constexpr int STEP = TOKENS ? U : 4 * U, HOP = TOKENS ? 1 : 4;  // heads of a step, and from a lane's to its next
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane >> 3, sub = lane & 7, first_head = TOKENS ? 0 : grp;
     const int k = blockIdx.x >= a.blocks_q;
     const uint32_t block = blockIdx.x - (k ? a.blocks_q : 0u), blocks = k ? gridDim.x - a.blocks_q : a.blocks_q;
     const int heads = a.heads[k];
     const RowView vx = a.x[k], vy = a.y[k], vd = a.dx[k];
-    const uint64_t my_turn = a.plan.turn[lane];
-    const int my_axis = a.plan.axis[lane];
     const bool interleaved = a.plan.interleaved != 0;
-    // strips: all heads of a token, or one step of them
-    const uint32_t per_token = a.split ? (heads + STEP - 1) / STEP : 1, strips = a.tokens * per_token, hop = blocks * QK_WARPS;
+    // a lane's pairs: with TOKENS the four that it turns; otherwise one of the token's 32, which the lanes hand to each other
+    constexpr int PAIRS = TOKENS ? 4 : 1;
+    auto turned_by = [&](int i) { return interleaved ? (i < 2 ? 2 * sub + i : 16 + 2 * sub + i - 2) : 4 * sub + i; };
+    const uint64_t turn_of_lane = a.plan.turn[lane];
+    const int axis_of_lane = a.plan.axis[lane];
+    auto my_turn = [&](int i) { return TOKENS ? a.plan.turn[turned_by(i)] : turn_of_lane; };
+    auto my_axis = [&](int i) { return TOKENS ? (int)a.plan.axis[turned_by(i)] : axis_of_lane; };
+    // strips: all heads of a token (of four), or one step of them
+    const uint32_t per_token = a.split ? (heads + STEP - 1) / STEP : 1, strips = TOKENS ? (a.tokens + 3) / 4 : a.tokens * per_token, hop = blocks * QK_WARPS;
     struct Place {
         uint32_t strip;
         int64_t x, y, d;  // offsets of the token's first row
         int64_t pos;
-        int head, end;    // first of the step, end of the strip
+        int head, end;    // first of the step, end of the strip (0: no token for this lane)
     };
     auto place = [&](uint32_t strip) {
         Place p;
         p.strip = strip;
-        const uint32_t token = strip / per_token, b = token / a.T, t = token - b * a.T;
+        const uint32_t token = TOKENS ? min(4 * strip + grp, a.tokens - 1) : strip / per_token, b = token / a.T, t = token - b * a.T;
         p.x = b * vx.sB + t * vx.sM;
         p.y = b * vy.sB + t * vy.sM;
         p.d = BACK ? b * vd.sB + t * vd.sM : 0;
-        p.pos = my_axis * a.pA + b * a.pB + t * a.pT;
-        p.head = (int)(strip - token * per_token) * STEP;
-        p.end = a.split ? min(p.head + STEP, heads) : heads;
+        p.pos = b * a.pB + t * a.pT;
+        p.head = TOKENS ? 0 : (int)(strip - token * per_token) * STEP;
+        p.end = TOKENS ? (4 * strip + grp < a.tokens ? heads : 0) : a.split ? min(p.head + STEP, heads) : heads;
         return p;
     };
     Raw<X> next_x[U];
@@ -165,24 +172,34 @@ __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const
     auto load = [&](const Place& p) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int h = p.head + 4 * i + grp;
+            const int h = p.head + HOP * i + first_head;
             if (h < p.end) {
                 next_x[i].load(vx.ptr + p.x + h * vx.sH, sub);
                 if constexpr (BACK) next_g[i].load(vy.ptr + p.y + h * vy.sH, sub);
             }
         }
     };
+    // Fractions of a turn (2^-32).  With TOKENS worked out at once, in half the registers: they come once for all heads.
+    int64_t next_pos[PAIRS];
+    uint32_t next_angle[PAIRS];
+    auto angle_of = [&](int i, int64_t pos) { return (uint32_t)((my_turn(i) * (uint64_t)pos) >> 32); };
     auto position = [&](const Place& p) {
-        if (my_axis == HK_ROTARY_STILL) return (int64_t)0;
-        return a.pos64 ? static_cast<const int64_t*>(a.positions)[p.pos] : (int64_t)static_cast<const int32_t*>(a.positions)[p.pos];
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+            const int64_t at = p.pos + my_axis(i) * a.pA;
+            const int64_t pos = my_axis(i) == HK_ROTARY_STILL ? 0
+                                : a.pos64                     ? static_cast<const int64_t*>(a.positions)[at]
+                                                              : (int64_t)static_cast<const int32_t*>(a.positions)[at];
+            if (TOKENS) next_angle[i] = angle_of(i, pos);
+            else next_pos[i] = pos;
+        }
     };
     Place at = place(block * QK_WARPS + warp);
     pdl_wait();
     pdl_trigger();
-    int64_t next_pos = 0;
     if (at.strip < strips) {
         load(at);
-        next_pos = position(at);
+        position(at);
     }
     float w[MODE == QK_ROTATE ? 1 : 8], dw[BACK ? 8 : 1];
     if (MODE != QK_ROTATE)
@@ -202,24 +219,32 @@ __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const
             x[i] = next_x[i];
             if (BACK) g[i] = next_g[i];
         }
-        const int64_t pos = next_pos;
+        int64_t pos[PAIRS];
+        uint32_t angle[PAIRS];
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+            pos[i] = next_pos[i];
+            angle[i] = next_angle[i];
+        }
         Place next = at;
         next.head += STEP;
-        const bool on = next.head >= at.end;  // to another strip
+        const bool on = next.head >= (TOKENS ? heads : at.end);  // to another strip
         if (on) next = place(at.strip + hop < at.strip ? 0xffffffffu : at.strip + hop);
         if (next.strip < strips) {
             load(next);
-            if (on) next_pos = position(next);
+            if (on) position(next);
         }
         if (fresh) {
-            float mc, ms;
-            sincospif((float)(int32_t)((my_turn * (uint64_t)pos) >> 32) * 0x1p-31f, &ms, &mc);
-            if (a.back) ms = -ms;
+            float mc[PAIRS], ms[PAIRS];
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+                sincospif((float)(int32_t)(TOKENS ? angle[i] : angle_of(i, pos[i])) * 0x1p-31f, &ms[i], &mc[i]);
+                if (a.back) ms[i] = -ms[i];
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int pair = interleaved ? (i < 2 ? 2 * sub + i : 16 + 2 * sub + i - 2) : 4 * sub + i;
-                c[i] = __shfl_sync(0xffffffffu, mc, pair);
-                s[i] = __shfl_sync(0xffffffffu, ms, pair);
+                c[i] = TOKENS ? mc[i % PAIRS] : __shfl_sync(0xffffffffu, mc[0], turned_by(i));
+                s[i] = TOKENS ? ms[i % PAIRS] : __shfl_sync(0xffffffffu, ms[0], turned_by(i));
             }
             if (KEEPS) {
 #pragma unroll
@@ -233,7 +258,7 @@ __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const
         fresh = on;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int h = at.head + 4 * i + grp;
+            const int h = at.head + HOP * i + first_head;
             const bool valid = h < at.end;
             if (!__any_sync(0xffffffffu, valid)) break;
             Row8 r = numbers(x[i]);
@@ -281,10 +306,10 @@ __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const
     }
 }
 
-// The sums of the CTAs that took queries, and of those that took keys: 16 columns a CTA, 16 threads a column, always in the same
+// The sums of the CTAs that took queries, and of those that took keys: 16 columns a CTA, 64 threads a column, always in the same
 // order.
-__global__ void __launch_bounds__(256) qk_weight_sum_kernel(const float* partial, int n_q, int n, float* dq, float* dk) {
-    __shared__ float sums[16][17];
+__global__ void __launch_bounds__(1024) qk_weight_sum_kernel(const float* partial, int n_q, int n, float* dq, float* dk) {
+    __shared__ float sums[64][17];
     const int col = threadIdx.x & 15, part = threadIdx.x >> 4, at = (blockIdx.x & 3) * 16 + col;
     const bool keys = blockIdx.x >= 4;
     pdl_wait();
@@ -292,12 +317,20 @@ __global__ void __launch_bounds__(256) qk_weight_sum_kernel(const float* partial
     float x = 0.f;
     const int end = keys ? n : n_q;
 #pragma unroll 4
-    for (int i = (keys ? n_q : 0) + part; i < end; i += 16) x += partial[i * 64 + at];
+    for (int i = (keys ? n_q : 0) + part; i < end; i += 64) x += partial[i * 64 + at];
     sums[part][col] = x;
+    __syncthreads();
+    if (part < 8) {
+        x = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x += sums[8 * part + i][col];
+    }
+    __syncthreads();
+    if (part < 8) sums[part][col] = x;
     __syncthreads();
     if (part == 0) {
 #pragma unroll
-        for (int i = 1; i < 16; ++i) x += sums[i][col];
+        for (int i = 1; i < 8; ++i) x += sums[i][col];
         float* to = keys ? dk : dq;
         if (to) to[at] = x;
     }
@@ -313,21 +346,21 @@ typedef void (*QkKernel)(QkArgs);
 template <class X, int MODE>
 constexpr int rows_of() { return MODE == QK_NORM_BACK ? 2 : 4; }
 template <class X, class Y, int MODE>
-QkKernel kernel_of(int& step) {
-    step = 4 * rows_of<X, MODE>();
-    return qk_rotary_kernel<X, Y, MODE, rows_of<X, MODE>()>;
+QkKernel kernel_of(int& step, bool tokens) {
+    step = rows_of<X, MODE>() * (tokens ? 1 : 4);
+    return tokens ? qk_rotary_kernel<X, Y, MODE, rows_of<X, MODE>(), true> : qk_rotary_kernel<X, Y, MODE, rows_of<X, MODE>(), false>;
 }
 template <int MODE>
-QkKernel pick(int x, int y, int& step) {
+QkKernel pick(int x, int y, int& step, bool tokens) {
     typedef __nv_bfloat16 bf16;
-    if (x == HK_F32 && y == HK_F32) return kernel_of<float, float, MODE>(step);
-    if (x == HK_BF16 && y == HK_BF16) return kernel_of<bf16, bf16, MODE>(step);
-    if (x == HK_F16 && y == HK_F16) return kernel_of<__half, __half, MODE>(step);
-    if (x == HK_BF16 && y == HK_F32) return kernel_of<bf16, float, MODE>(step);
-    if (x == HK_F16 && y == HK_F32) return kernel_of<__half, float, MODE>(step);
+    if (x == HK_F32 && y == HK_F32) return kernel_of<float, float, MODE>(step, tokens);
+    if (x == HK_BF16 && y == HK_BF16) return kernel_of<bf16, bf16, MODE>(step, tokens);
+    if (x == HK_F16 && y == HK_F16) return kernel_of<__half, __half, MODE>(step, tokens);
+    if (x == HK_BF16 && y == HK_F32) return kernel_of<bf16, float, MODE>(step, tokens);
+    if (x == HK_F16 && y == HK_F32) return kernel_of<__half, float, MODE>(step, tokens);
     if constexpr (MODE == QK_ROTATE) {  // gradients from the attention back to the projection's type
-        if (x == HK_F32 && y == HK_BF16) return kernel_of<float, bf16, MODE>(step);
-        if (x == HK_F32 && y == HK_F16) return kernel_of<float, __half, MODE>(step);
+        if (x == HK_F32 && y == HK_BF16) return kernel_of<float, bf16, MODE>(step, tokens);
+        if (x == HK_F32 && y == HK_F16) return kernel_of<float, __half, MODE>(step, tokens);
     }
     return nullptr;
 }
@@ -393,15 +426,27 @@ int qk_run(const hk_qk_params* p, int mode, bool back, cudaStream_t stream) {
     a.eps = p->eps;
     a.plan = p->plan;
 
-    int step = 0;
-    const QkKernel kernel = mode == QK_ROTATE ? pick<QK_ROTATE>(src_t, dst_t, step)
-                            : mode == QK_NORM ? pick<QK_NORM>(src_t, dst_t, step)
-                                              : pick<QK_NORM_BACK>(src_t, p->out_dtype, step);
-    if (!kernel) return HK_ERR_UNSUPPORTED;
     // Warps enough for all that an SM holds; where there are fewer tokens, a warp takes one step of a token's heads.
     const int64_t most = (int64_t)sm_count() * QK_CTAS;
     a.split = (int64_t)a.tokens < most * QK_WARPS;
-    auto strips = [&](int heads) { return (int64_t)a.tokens * (a.split ? (heads + step - 1) / step : 1); };
+    // Groups of lanes by tokens where most of the 16-bit tensors lie head by head (B1, 32 and 8 heads, T 32768, bf16 in and out:
+    // 65 us instead of 74, fp32 gradients into bf16 86 instead of 95; fp32 alone gains 1 % and its backward pass has no registers for it)
+    int by_head = 0, of_16 = 0;
+    auto count = [&](const hk_view& v, int dtype) {
+        if (dtype == HK_F32) return;
+        ++of_16;
+        if (v.strideM < v.strideH && p->nh > 1) ++by_head;
+    };
+    count(*src[0], src_t);
+    count(*dst[0], dst_t);
+    if (mode == QK_NORM_BACK) count(*grad[0], p->out_dtype);
+    const bool tokens = !a.split && 2 * by_head > of_16;
+    int step = 0;
+    const QkKernel kernel = mode == QK_ROTATE ? pick<QK_ROTATE>(src_t, dst_t, step, tokens)
+                            : mode == QK_NORM ? pick<QK_NORM>(src_t, dst_t, step, tokens)
+                                              : pick<QK_NORM_BACK>(src_t, p->out_dtype, step, tokens);
+    if (!kernel) return HK_ERR_UNSUPPORTED;
+    auto strips = [&](int heads) { return tokens ? ((int64_t)a.tokens + 3) / 4 : (int64_t)a.tokens * (a.split ? (heads + step - 1) / step : 1); };
     // CTAs by the steps there are
     int64_t n_q = (strips(p->nh) + QK_WARPS - 1) / QK_WARPS, n_k = (strips(p->nh_k) + QK_WARPS - 1) / QK_WARPS;
     if (p->nh_k == 0) n_k = 0;
@@ -418,7 +463,7 @@ int qk_run(const hk_qk_params* p, int mode, bool back, cudaStream_t stream) {
     if (cudaLaunchKernelEx(&lc.cfg, kernel, a) != cudaSuccess) return check_launch();
     count_launch();
     if (mode == QK_NORM_BACK && (p->dq_weight || p->dk_weight)) {
-        LaunchConfig sum(8, 256, 0, stream, 1, true);
+        LaunchConfig sum(8, 1024, 0, stream, 1, true);
         if (cudaLaunchKernelEx(&sum.cfg, qk_weight_sum_kernel, (const float*)a.partial, (int)n_q, blocks, p->dq_weight, p->dk_weight) != cudaSuccess)
             return check_launch();
         count_launch();
