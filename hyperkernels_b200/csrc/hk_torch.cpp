@@ -6,6 +6,8 @@
 // objects in between.  The library is the one attention.py loads (dlsym on its handle), so an instrumented build given
 // by HK_ATTENTION_LIB is used here too.
 #include <ATen/ATen.h>
+#include <ATen/Context.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <Python.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <string.h>
@@ -302,6 +304,14 @@ bool one_device(std::initializer_list<const at::Tensor*> all) {
     return true;
 }
 
+// A tensor that a kernel is about to fill, without the way through the dispatcher, which takes as long again as the allocation;
+// torch's own switch that fills such tensors is heard.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
+    if (at::globalContext().deterministicAlgorithms() && at::globalContext().deterministicFillUninitializedMemory())
+        return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
+    return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
+}
+
 // Makes the tensors' device the current one and the stream asked for (None: that device's current one) the one that
 // results and workspaces are allocated for: they are written there, whatever becomes of them here.
 struct OnStream {
@@ -403,22 +413,22 @@ static PyObject* qk_body(PyObject* const* a, Py_ssize_t n) {
     OnStream on(a[13], *src[0]);
     if (PyErr_Occurred()) return nullptr;
 
-    const auto opt = src[0]->options();
+    const at::Device device = src[0]->device();
     at::Tensor r[2], dw[2], ws;
     for (int k = 0; k < 2; ++k) {
         if (!src[k]) continue;
-        r[k] = out[k] ? *out[k] : at::empty({B, k ? Hk : H, T, 64}, opt.dtype(scalar_of(out_type)));
+        r[k] = out[k] ? *out[k] : fresh({B, k ? Hk : H, T, 64}, scalar_of(out_type), device);
         *dst_view[k] = {r[k].data_ptr(), r[k].stride(0), r[k].stride(2), r[k].stride(1)};
     }
     p.q_weight = norm && w[0] ? w[0]->data_ptr() : nullptr;
     p.k_weight = norm && w[1] ? w[1]->data_ptr() : nullptr;
     if (which == 3) {
         for (int k = 0; k < 2; ++k)
-            if (w[k] && src[k]) dw[k] = at::empty({64}, opt.dtype(at::kFloat));
+            if (w[k] && src[k]) dw[k] = fresh({64}, at::kFloat, device);
         p.dq_weight = dw[0].defined() ? data(dw[0]) : nullptr;
         p.dk_weight = dw[1].defined() ? data(dw[1]) : nullptr;
         p.workspace_bytes = g_lib.qk_bytes(&p);
-        ws = at::empty({(int64_t)p.workspace_bytes}, opt.dtype(at::kByte));
+        ws = fresh({(int64_t)p.workspace_bytes}, at::kByte, device);
         p.workspace = ws.data_ptr();
     }
     p.positions = pos->data_ptr();
@@ -467,13 +477,13 @@ static PyObject* prefix_body(PyObject* const* a, Py_ssize_t n) {
     if (!one_device({Q, kv[0], kv[1], kv[2], kv[3], lens, ws, out, lse})) return nullptr;
     OnStream on(a[11], *Q);
     if (PyErr_Occurred()) return nullptr;
-    const auto opt = Q->options();
-    at::Tensor O = out ? *out : at::empty({B, H, T, 64}, opt), L = lse ? *lse : at::empty({B, H, T}, opt.dtype(at::kFloat)), own;
+    const at::Device device = Q->device();
+    at::Tensor O = out ? *out : fresh({B, H, T, 64}, scalar_of(p.dtype), device), L = lse ? *lse : fresh({B, H, T}, at::kFloat, device), own;
     p.O = {O.data_ptr(), O.stride(0), O.stride(2), O.stride(1)};
     p.LSE = data(L); p.lse_strideB = L.stride(0); p.lse_strideH = L.stride(1);
     const size_t need = g_lib.prefix_bytes(&p);
     if (!ws && need > 0) {
-        own = at::empty({(int64_t)need + 256}, opt.dtype(at::kByte));
+        own = fresh({(int64_t)need + 256}, at::kByte, device);
         ws = &own;
     }
     if (ws && !given_workspace(ws, need, &p.workspace, &p.workspace_bytes)) return nullptr;
