@@ -106,85 +106,109 @@ struct Plan {
     bool prefix_many, own_many;  // which kernels
 };
 
-// CTAs of `items` blocks of rows, `tiles` tiles each and four to start and end, on `sms` SMs: the last ones, which do not fill the
-// SMs, in `parts` by their keys (at least four tiles).  In tiles.
+// Estimates, in microseconds, from calls taken apart with the clock of one B200; the choice they make was then compared with its
+// neighbours (runs of the prefix 1 to 32, requests' own keys in 1 to 8 runs) at a dozen sizes.
+constexpr double TILE_US = 1.3, BLOCK_US = 5.2;   // many rows: a tile of keys; to start and end a CTA
+constexpr double FEW_US = 2.2, COMBINE_US = 3.0;  // few rows: to start and end a CTA; the last kernel
+double batch_us(int dtype, int rows) { return dtype != HK_F32 ? 0.45 : rows <= 2 ? 0.4 : 0.65; }  // few rows: a batch of every warp
+
+// One kind of work: CTAs, microseconds of each, how many an SM holds.
+struct Work {
+    double ctas, us, per_sm;
+    double rounds(int sms) const { return std::ceil(ctas / (sms * per_sm)) * us; }
+    double sm_time() const { return ctas * us / per_sm; }
+};
+// Two kinds side by side.  They do not fit each other without gaps: a part of all the work on top.
+double together(const Work& x, const Work& y, int sms) {
+    const double all = (x.sm_time() + y.sm_time()) / sms;
+    return std::max({x.rounds(sms), y.rounds(sms), all}) + 0.15 * all;
+}
+// CTAs of few rows through `keys` keys each: by the batches of a warp, or by what the memory gives to all that run at once
+Work few_work(double ctas, double keys, const FewPlan& f, int dtype, int sms) {
+    return {ctas, FEW_US + std::max(std::ceil(keys / f.step) * batch_us(dtype, f.rows), keys * 2 * HEAD_DIM * esize(dtype) * std::min(ctas, (double)sms * f.per_sm) / 6e6),
+            (double)f.per_sm};
+}
+
+// `items` blocks of many rows, `tiles` tiles each: the last ones, which do not fill the SMs, in `parts` by their keys.
 double whole_time(int64_t items, double tiles, int sms, int& parts) {
     const int64_t full = items / sms, tail = items % sms;
     double best = 0.0;
     parts = 1;
-    for (int k = 1; tail > 0 && k <= 8 && (k == 1 || tiles >= 4.0 * k); ++k) {
-        const double time = cdiv(tail * k, sms) * (tiles / k + 4.0) + (k > 1 ? 3.0 : 0.0);
+    for (int k = 1; tail > 0 && k <= 16 && (k == 1 || tiles >= 1.5 * k); ++k) {
+        const double time = cdiv(tail * k, sms) * (tiles / k * TILE_US + BLOCK_US) + (k > 1 ? COMBINE_US : 0.0);
         if (k > 1 && time >= best) continue;
         best = time;
         parts = k;
     }
-    return full * (tiles + 4.0) + best;
+    return full * (tiles * TILE_US + BLOCK_US) + best;
 }
 
 Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
     a.B = p->B; a.Hk = p->nh_kv; a.group = p->nh / p->nh_kv; a.T = (int)p->T; a.P = (int)p->prefix_len; a.S = (int)p->kv_len;
     a.R = p->B * a.T * a.group;
-    const int own_rows = a.T * a.group, sms = sm_count();
-    const ManyPlan mp = many_plan(p->dtype);
-    // Many rows: the tensor cores' 128 at a time.  Fewer than 16 (33 against the prefix) are taken faster by the other kernel.
-    Plan plan{a.P > 0 && a.R > 32, own_rows > 16};
-    const FewPlan fp = few_plan(p->dtype, a.R), fo = few_plan(p->dtype, own_rows);
-    a.tiles_o = cdiv(own_rows, plan.own_many ? mp.rows : fo.rows);
-    a.splits_o = a.S > 0 || a.P == 0;  // without keys of their own, the prefix alone
-    const int64_t items_o = (int64_t)a.B * a.Hk * a.tiles_o;
-    // SM time for the requests' own keys, half of their caches, in tiles: of 1.3 us, the other kernel reads at 7 TB/s
-    const double tiles_own = 0.5 * a.S / mp.keys;
-    const double own_time = plan.own_many ? items_o * (tiles_own + 4.0)
-                                          : sms * (2.0 + (double)a.B * a.Hk * a.S * HEAD_DIM * esize(p->dtype) / 7e12 / 1.3e-6);
-    a.whole = a.splits_p = a.per_p = a.tiles_p = 0;
-    double time = 0.0;
-    if (plan.prefix_many) {
-        // as many runs as make the longer of: the waves of CTAs over the prefix; all of the work spread over the SMs
-        a.tiles_p = cdiv(a.R, mp.rows);
-        const int64_t items = (int64_t)a.Hk * a.tiles_p;
-        const int most = std::min(64, std::max(1, cdiv(a.P, 2 * mp.keys)));
-        for (int n = 1; n <= most; ++n) {
-            const int tiles = cdiv(cdiv(a.P, n), mp.keys);
-            const double t = std::max((double)cdiv(items * n, sms) * (tiles + 4), (items * n * (tiles + 4) + own_time) / sms) + 0.05 * n;
-            if (n > 1 && t >= time) continue;
-            time = t;
-            a.per_p = tiles * mp.keys;
-        }
-        a.splits_p = cdiv(a.P, a.per_p);
-    } else if (a.P > 0) {
-        a.tiles_p = cdiv(a.R, fp.rows);
-        const int64_t items = (int64_t)a.Hk * a.tiles_p, places = sms * fp.per_sm;
-        const int n = (int)std::max<int64_t>(1, std::min<int64_t>({64, places / items, cdiv(a.P, 4 * fp.step)}));
-        a.per_p = cdiv(cdiv(a.P, n), fp.step) * fp.step;
-        a.splits_p = cdiv(a.P, a.per_p);
-    }
-    // Small calls: up to six batches a warp take less than two more launches do (B4 H12, 333 + 64 keys: TIMES us).
-    if (!plan.own_many && a.P > 0 && items_o <= sms && a.P + a.S <= 6 * (own_rows <= 2 && p->dtype == HK_F32 ? 4 : 2) * fo.step) {
-        a.whole = 1;
-        a.splits_p = a.per_p = a.tiles_p = 0;
-        a.splits_o = a.slots = 1;
-        plan.prefix_many = false;
-        return plan;
-    }
+    const int own_rows = a.T * a.group, sms = sm_count(), dtype = p->dtype;
+    const ManyPlan mp = many_plan(dtype);
+    const FewPlan fp = few_plan(dtype, a.R), fo = few_plan(dtype, own_rows);
+    const int64_t requests = (int64_t)a.B * a.Hk;
+    const double mean_own = 0.5 * a.S;  // the caches are taken to be half full
+    const bool own = a.S > 0 || a.P == 0;  // without keys of their own, the prefix alone
+
+    // the requests' own keys, by few or by many rows: CTAs and runs
+    const int few_tiles = cdiv(own_rows, fo.rows), many_tiles = cdiv(own_rows, mp.rows);
+    int few_splits = 1;
+    while (few_splits < 16 && requests * few_tiles * few_splits * 2 <= sms * fo.per_sm && few_splits * 2 * 4 * fo.step <= a.S) few_splits *= 2;
+    const Work own_few = few_work((double)requests * few_tiles * few_splits, mean_own / few_splits, fo, dtype, sms);
+    const Work own_many{(double)requests * many_tiles, BLOCK_US + std::ceil(mean_own / mp.keys) * TILE_US, 1.0}, nothing{0.0, 0.0, 1.0};
+
+    struct Choice {
+        double us;
+        Plan plan;
+        int whole, per_p;
+    } best{1e30, {false, false}, 0, 0};
+    auto consider = [&](const Choice& c) {
+        if (c.us < best.us) best = c;
+    };
     int parts = 1;
-    if (plan.own_many && plan.prefix_many && whole_time(items_o, (double)a.P / mp.keys + tiles_own, sms, parts) <= time + 3.0) {
-        // every block of rows takes the prefix: no more often than once for 128 or 256 rows, and nothing goes through memory
-        a.whole = 1;
-        a.splits_p = a.per_p = a.tiles_p = 0;
+    // every block of rows takes the prefix and then its request's keys: nothing goes through memory, in one launch
+    if (own) {
+        const int warps = fo.rows < 16 ? 16 : 8, keys = fo.step / 4 * warps;
+        consider({std::ceil((double)requests * few_tiles / sms) * (FEW_US + 1.0 + std::ceil((a.P + mean_own) / keys) * 1.3 * batch_us(dtype, fo.rows)), {false, false}, 1, 0});
+        if (own_rows > 16) consider({whole_time(requests * many_tiles, ((double)a.P + mean_own) / mp.keys, sms, parts), {false, true}, 1, 0});
+    }
+    // the prefix once for all rows, in runs: as many as make the longer of its waves of CTAs and all of the work spread over the SMs
+    // shortest
+    for (int k = 0; a.P > 0 && k < 2; ++k) {
+        if (k == 1 && a.R <= 32) break;
+        const int64_t items = (int64_t)a.Hk * cdiv(a.R, k ? mp.rows : fp.rows);
+        const int step = k ? mp.keys : fp.step, most = std::min(64, std::max(1, cdiv(a.P, (k ? 2 : 4) * step)));
+        if (!k && items > 16 * sms) continue;  // far from few rows
+        for (int n = 1; n <= most; ++n) {
+            const int per = cdiv(a.P, (int64_t)n * step) * step;
+            const Work w = k ? Work{(double)items * n, BLOCK_US + per / step * TILE_US, 1.0}
+                             : few_work((double)items * n, per, fp, dtype, sms);
+            const double last = COMBINE_US + 0.07 * n;
+            consider({together(w, own ? own_few : nothing, sms) + last + (k && own ? 1.0 : 0.0), {k == 1, false}, 0, per});
+            if (own && own_rows > 16) consider({together(w, own_many, sms) + last + 1.0, {k == 1, true}, 0, per});
+        }
+    }
+    a.tiles_o = best.plan.own_many ? many_tiles : few_tiles;
+    a.whole = best.whole;
+    a.per_p = best.per_p;
+    a.splits_p = a.per_p ? cdiv(a.P, a.per_p) : 0;
+    a.tiles_p = a.per_p ? cdiv(a.R, best.plan.prefix_many ? mp.rows : fp.rows) : 0;
+    if (a.whole) {
+        const int64_t items = requests * a.tiles_o;
         a.splits_o = 1;
-        a.slots = parts;
-        a.first_split = (int)(parts > 1 ? items_o / sms * sms : items_o);
+        a.slots = best.plan.own_many ? parts : 1;
+        a.first_split = (int)(a.slots > 1 ? items / sms * sms : items);
         a.block_rows = mp.rows;
-        a.slot_rows = (items_o - a.first_split) * mp.rows;
-        return plan;
+        a.slot_rows = (items - a.first_split) * mp.rows;
+    } else {
+        a.splits_o = !own ? 0 : best.plan.own_many ? 1 : few_splits;
+        a.slots = a.splits_p + a.splits_o;
+        a.slot_rows = (int64_t)a.Hk * a.R;
     }
-    if (!plan.own_many) {
-        const int64_t places = sms * fo.per_sm;
-        while (a.splits_o > 0 && a.splits_o < 16 && items_o * a.splits_o * 2 <= places && a.splits_o * 2 * 4 * fo.step <= a.S) a.splits_o *= 2;
-    }
-    a.slots = a.splits_p + a.splits_o;
-    a.slot_rows = (int64_t)a.Hk * a.R;
-    return plan;
+    return best.plan;
 }
 // rows of all slots in the workspace
 size_t slot_rows(const PrefixArgs& a) { return a.slots > 1 ? (size_t)a.slots * a.slot_rows : 0; }

@@ -470,8 +470,8 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                             sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
                             x[c + i] = __float_as_uint(w.x);
                             x[c + i + 1] = __float_as_uint(w.y);
-                            z[i] = tf32_rest(x[c + i]);
-                            z[i + 1] = tf32_rest(x[c + i + 1]);
+                            z[i] = __float_as_uint(w.x - __uint_as_float(x[c + i] & 0xffffe000u));
+                            z[i + 1] = __float_as_uint(w.y - __uint_as_float(x[c + i + 1] & 0xffffe000u));
                         }
                         tmem_st32p(at_s + c, x + c);
                         tmem_st32(at_low + c, z);
