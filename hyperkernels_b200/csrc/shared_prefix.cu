@@ -172,7 +172,11 @@ Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
     // every block of rows takes the prefix and then its request's keys: nothing goes through memory, in one launch
     if (own) {
         const int warps = fo.rows < 16 ? 16 : 8, keys = fo.step / 4 * warps;
-        consider({std::ceil((double)requests * few_tiles / sms) * (FEW_US + 1.0 + std::ceil((a.P + mean_own) / keys) * 1.3 * batch_us(dtype, fo.rows)), {false, false}, 1, 0});
+        const double items = (double)requests * few_tiles, all_keys = a.P + mean_own, bytes = all_keys * 2 * HEAD_DIM * esize(dtype);
+        // a batch of every warp takes longer beside more warps; an SM reads 80 GB/s, all of them 6 TB/s
+        const double us = FEW_US + 1.0 + std::max({std::ceil(all_keys / keys) * 1.3 * batch_us(dtype, fo.rows), bytes / 80e3, bytes * std::min(items, (double)sms) / 6e6});
+        consider({std::ceil(items / sms) * us, {false, false}, 1, 0});
+        if (a.P == 0) consider({together(own_few, nothing, sms) + (few_splits > 1 ? COMBINE_US : 0.0), {false, false}, 0, 0});
         if (own_rows > 16) consider({whole_time(requests * many_tiles, ((double)a.P + mean_own) / mp.keys, sms, parts), {false, true}, 1, 0});
     }
     // the prefix once for all rows, in runs: as many as make the longer of its waves of CTAs and all of the work spread over the SMs

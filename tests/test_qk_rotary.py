@@ -176,6 +176,43 @@ def test_norm_and_rotation(B, H, Hk, T, xt, yt, wt, sections, interleaved, layou
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,T", [(3, 4, 2, 1027), (1, 9, 1, 6001), (2600, 3, 3, 1), (5, 32, 8, 700)])
+@pytest.mark.parametrize("xt,yt", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("layout,grads", [("bhtd", "bhtd"), ("packed", "bhtd"), ("bhtd", "packed"), ("wide", "wide")])
+def test_many_tokens(B, H, Hk, T, xt, yt, layout, grads):
+    """Enough tokens for warps that go from one to the next, by heads and by tokens."""
+    sections, eps = (8, 12, 12), 1e-6
+    q, k = inputs(B + T, B, H, Hk, T, TYPES[xt], layout, 1.2)
+    dq, dk = inputs(B * T + 1, B, H, Hk, T, TYPES[yt], grads, 0.7)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = [1 + 0.3 * torch.randn(64, generator=g, device="cuda") for _ in range(2)]
+    pos = torch.randint(0, 3000, (3, B, T), generator=g, device="cuda")
+    angle = angles(pos, sections)
+    turn = hk.rotary_forward(q, k, pos, sections, out_dtype=TYPES[yt])
+    back = hk.rotary_backward(dq, dk, pos, sections, out_dtype=TYPES[xt])
+    norm = hk.qk_norm_rotary_forward(q, k, *w, pos, sections, eps=eps, out_dtype=TYPES[yt])
+    grad = hk.qk_norm_rotary_backward(q, k, dq, dk, *w, pos, sections, eps=eps)
+    for i, (x, dy) in enumerate(((q, dq), (k, dk))):
+        want = turned(x.double(), angle, False)
+        close(turn[i], want, size_of_pairs(x.double(), False) * 8.01 * U + half_step(TYPES[yt], want) * (yt != "f32"), "turn")
+        want = turned(dy.double(), -angle, False)
+        zs = size_of_pairs(dy.double(), False)
+        close(back[i], want, zs * 8.01 * U + half_step(TYPES[xt], want) * (xt != "f32"), "back")
+        n, one = normed(x, w[i], eps), w[i].double()
+        want = turned(n, angle, False)
+        close(norm[i], want, size_of_pairs(n, False) * 20 * U + half_step(TYPES[yt], want) * (yt != "f32"), "norm")
+        z = turned(dy.double(), -angle, False)
+        inv = 1 / (x.double().square().mean(-1, keepdim=True) + eps).sqrt()
+        n = x.double() * inv
+        want = inv * (one * z - n * (one * z * n).mean(-1, keepdim=True))
+        bound = inv * (zs * one.abs() * 22 * U + n.abs() * (zs * one.abs() * n.abs()).mean(-1, keepdim=True) * 55 * U)
+        close(grad[i], want, bound + half_step(TYPES[xt], want) * (xt != "f32"), "norm back")
+        # a lane's rows: those of its warp, eight lanes a row; then 32 lanes of a CTA, three CTAs, 64 threads
+        rows = B * T * x.shape[1] / (148 * 8 * 4) * 3 + 8
+        close(grad[2 + i], (z * n).sum((0, 1, 2)), (zs * n.abs()).sum((0, 1, 2)) * (20 + rows + 32 + 3 + 64) * U, "weight")
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences():
     """Directional derivatives of the definition in 64 bits (central differences, step 1e-5: error of the order 1e-10)."""
     sections = (8, 12, 12)

@@ -104,10 +104,37 @@ def test_against_the_definition(B, H, Hk, T, P, S, dtype, causal, layout):
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
 
 
+# sizes for each way of cutting the work, with the launches it takes on a B200: few rows and many, the prefix in runs and in one go
+# with the requests' own keys, blocks of rows in parts of their keys
+WAYS = [
+    (4, 12, 12, 1, 333, 64, "f32", 1), (64, 8, 2, 1, 515, 100, "f16", 1), (5, 6, 6, 2, 130, 70, "f32", 1), (3, 4, 4, 9, 90, 61, "f32", 1),  # few rows, in one go
+    (1, 2, 1, 1, 9000, 500, "f32", 2), (2, 1, 1, 1, 9001, 500, "f32", 2), (1, 4, 4, 2, 9000, 513, "f32", 2), (16, 4, 4, 1, 4000, 300, "f32", 2),
+    (8, 4, 2, 1, 4000, 700, "f32", 2), (4, 12, 4, 1, 3000, 400, "f32", 2), (20, 8, 2, 1, 3001, 400, "bf16", 2), (1, 2, 2, 24, 20000, 100, "f16", 2),  # few rows, in runs
+    (4, 4, 4, 1, 3000, 0, "bf16", 2), (40, 8, 2, 1, 3000, 0, "f32", 2), (9, 4, 4, 1, 0, 4000, "f32", 2), (300, 4, 2, 1, 0, 400, "f16", 1),  # only one kind of keys
+    (64, 32, 8, 1, 8192, 1000, "bf16", 3), (64, 32, 8, 1, 4100, 1000, "f32", 3), (16, 8, 2, 20, 2500, 300, "bf16", 3),  # many rows against the prefix, few against the own keys
+    (16, 4, 4, 40, 2500, 300, "f32", 3), (16, 4, 4, 77, 4097, 333, "f16", 3), (700, 8, 1, 1, 3000, 0, "bf16", None),  # many rows against both, or the prefix alone
+    (40, 4, 4, 260, 300, 300, "bf16", 1), (37, 4, 2, 129, 301, 300, "f16", None), (3, 4, 4, 300, 900, 400, "f32", 2), (3, 8, 2, 301, 901, 403, "bf16", 2),
+    (40, 4, 4, 130, 300, 140, "f32", 2), (2, 4, 4, 700, 0, 700, "bf16", None), (2, 4, 4, 700, 0, 701, "f32", None), (5, 8, 2, 512, 3001, 700, "f16", None)]  # many rows, in one go
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,T,P,S,dtype,launches", WAYS)
+@pytest.mark.parametrize("causal,layout", [(True, "bhtd"), (True, "wide"), (False, "bthd")])
+def test_every_way_of_cutting_the_work(B, H, Hk, T, P, S, dtype, launches, causal, layout):
+    x = make(B + T, B, H, Hk, T, P, S, dtype, layout, junk=math.nan if layout == "bhtd" else math.inf)
+    before = hk.launch_count()
+    got = hk.shared_prefix_attention(*x, SCALE, causal)
+    assert launches is None or hk.launch_count() - before == launches
+    check(got, definition(*x, causal), dtype)
+    again = hk.shared_prefix_attention(*x, SCALE, causal)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    assert hk.last_device_status() == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T", [1, 3, 40, 150])
-@pytest.mark.parametrize("P", [0, 70])
+@pytest.mark.parametrize("T", [1, 3, 40, 150, 400])
+@pytest.mark.parametrize("P", [0, 70, 2600])
 def test_lengths_at_borders_and_outside(dtype, T, P):
     """Empty, one, tiles' ends and the rows next to them, full, and lengths that the cache does not have (taken into it)."""
     lengths = [0, 1, 2, 63, 64, 65, 127, 128, 129, 191, 192, 193, 255, 256, 300, -4, 1000000]
@@ -215,6 +242,54 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.gpu
+def test_views_that_a_tensor_map_cannot_describe_are_refused():
+    """A stride of 0 over heads or requests, as attention_forward refuses it; queries may be broadcast."""
+    x = list(make(7, 3, 4, 2, 1, 60, 50, "f32"))
+    want = hk.shared_prefix_attention(*x, SCALE)
+    one = x[0][:, :1].expand(3, 4, 1, 64)
+    same = hk.shared_prefix_attention(one, *x[1:], SCALE)
+    copy = hk.shared_prefix_attention(one.contiguous(), *x[1:], SCALE)
+    assert torch.equal(same[0], copy[0])
+    for i in (1, 2):
+        y = list(x)
+        y[i] = y[i][:1].expand(2, 60, 64)
+        with pytest.raises(hk.HKError, match="unsupported"):
+            hk.shared_prefix_attention(*y, SCALE)
+    for i in (3, 4):
+        y = list(x)
+        y[i] = y[i][:1].expand(3, 2, 50, 64)
+        with pytest.raises(hk.HKError, match="unsupported"):
+            hk.shared_prefix_attention(*y, SCALE)
+    assert torch.equal(hk.shared_prefix_attention(*x, SCALE)[0], want[0])
+
+
+@pytest.mark.gpu
+def test_two_threads_on_streams_of_their_own():
+    import threading
+
+    cases = [make(i, 16, 8, 2, T, 3000, 300, "bf16") for i, T in enumerate((1, 20))]
+    want = [hk.shared_prefix_attention(*x, SCALE) for x in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(50):
+                got = hk.shared_prefix_attention(*cases[i], SCALE)
+                s.synchronize()
+                if not (torch.equal(got[0], want[i][0]) and torch.equal(got[1], want[i][1])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_serving_loop(dtype):
     """A prompt's common part goes into the prefix once; then requests of different lengths take a first chunk and decode: norm and
@@ -298,7 +373,7 @@ def _block():
     ("Q.ptr", None, -1), ("Kp.ptr", None, -1), ("V.ptr", None, -1), ("O.ptr", None, -1), ("LSE", None, -1), ("B", 0, -2), ("nh", 0, -2), ("nh_kv", 0, -2), ("nh_kv", 3, -2),
     ("T", 0, -2), ("T", (1 << 30) + 1, -2), ("prefix_len", -1, -2), ("kv_len", -1, -2), ("kv_len", (1 << 30) + 1, -2), ("scale", 0.0, -2), ("scale", math.inf, -2), ("scale", math.nan, -2),
     ("Q.ptr", 0x1004, -3), ("K.sM", 66, -3), ("Vp.sH", 9 * 64 + 2, -3), ("K.sB", -1024, -3), ("lengths", 0x1002, -3), ("LSE", 0x1002, -3),
-    ("O.sM", 0, -6), ("O.sH", 32, -6), ("dtype", 3, -6), ("dtype", -1, -6)])
+    ("O.sM", 0, -6), ("O.sH", 32, -6), ("Kp.sH", 0, -6), ("K.sB", 0, -6), ("V.sM", 0, -6), ("dtype", 3, -6), ("dtype", -1, -6)])
 def test_blocks_that_are_refused(path, value, status):
     b = _block()
     *head, last = path.split(".")
