@@ -108,8 +108,9 @@ struct Plan {
 
 // Estimates, in microseconds, from calls taken apart with the clock of one B200; the choice they make was then compared with its
 // neighbours (runs of the prefix 1 to 32, requests' own keys in 1 to 8 runs) at a dozen sizes.
-constexpr double TILE_US = 1.3, BLOCK_US = 5.2;   // many rows: a tile of keys; to start and end a CTA
+constexpr double BLOCK_US = 4.4;                   // many rows: to start and end a CTA
 constexpr double FEW_US = 2.2, COMBINE_US = 3.0;  // few rows: to start and end a CTA; the last kernel
+double tile_us(int dtype, bool own) { return dtype == HK_F32 ? (own ? 1.3 : 1.15) : own ? 1.85 : 1.4; }  // many rows: a tile; own keys are masked
 double batch_us(int dtype, int rows) { return dtype != HK_F32 ? 0.45 : rows <= 2 ? 0.4 : 0.65; }  // few rows: a batch of every warp
 
 // One kind of work: CTAs, microseconds of each, how many an SM holds.
@@ -129,18 +130,19 @@ Work few_work(double ctas, double keys, const FewPlan& f, int dtype, int sms) {
             (double)f.per_sm};
 }
 
-// `items` blocks of many rows, `tiles` tiles each: the last ones, which do not fill the SMs, in `parts` by their keys.
-double whole_time(int64_t items, double tiles, int sms, int& parts) {
+// `items` blocks of many rows through all of their keys: of `mean` microseconds, the longest of `longest` and `tiles` tiles.  The last
+// ones, which do not fill the SMs, in `parts` by their keys.
+double whole_time(int64_t items, double mean, double longest, double tiles, int sms, int& parts) {
     const int64_t full = items / sms, tail = items % sms;
     double best = 0.0;
     parts = 1;
     for (int k = 1; tail > 0 && k <= 16 && (k == 1 || tiles >= 1.5 * k); ++k) {
-        const double time = cdiv(tail * k, sms) * (tiles / k * TILE_US + BLOCK_US) + (k > 1 ? COMBINE_US : 0.0);
+        const double time = cdiv(tail * k, sms) * (longest / k + BLOCK_US) + (k > 1 ? COMBINE_US : 0.0);
         if (k > 1 && time >= best) continue;
         best = time;
         parts = k;
     }
-    return full * (tiles * TILE_US + BLOCK_US) + best;
+    return full * (mean + BLOCK_US) + best;
 }
 
 Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
@@ -158,7 +160,7 @@ Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
     int few_splits = 1;
     while (few_splits < 16 && requests * few_tiles * few_splits * 2 <= sms * fo.per_sm && few_splits * 2 * 4 * fo.step <= a.S) few_splits *= 2;
     const Work own_few = few_work((double)requests * few_tiles * few_splits, mean_own / few_splits, fo, dtype, sms);
-    const Work own_many{(double)requests * many_tiles, BLOCK_US + std::ceil(mean_own / mp.keys) * TILE_US, 1.0}, nothing{0.0, 0.0, 1.0};
+    const Work own_many{(double)requests * many_tiles, BLOCK_US + std::ceil(mean_own / mp.keys) * tile_us(dtype, true), 1.0}, nothing{0.0, 0.0, 1.0};
 
     struct Choice {
         double us;
@@ -177,7 +179,10 @@ Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
         const double us = FEW_US + 1.0 + std::max({std::ceil(all_keys / keys) * 1.3 * batch_us(dtype, fo.rows), bytes / 80e3, bytes * std::min(items, (double)sms) / 6e6});
         consider({std::ceil(items / sms) * us, {false, false}, 1, 0});
         if (a.P == 0) consider({together(own_few, nothing, sms) + (few_splits > 1 ? COMBINE_US : 0.0), {false, false}, 0, 0});
-        if (own_rows > 16) consider({whole_time(requests * many_tiles, ((double)a.P + mean_own) / mp.keys, sms, parts), {false, true}, 1, 0});
+        if (own_rows > 16) {
+            const double prefix = std::ceil((double)a.P / mp.keys), most = std::ceil((double)a.S / mp.keys), us = prefix * tile_us(dtype, false), own_us = most * tile_us(dtype, true);
+            consider({whole_time(requests * many_tiles, us + 0.5 * own_us, us + own_us, prefix + most, sms, parts), {false, true}, 1, 0});
+        }
     }
     // the prefix once for all rows, in runs: as many as make the longer of its waves of CTAs and all of the work spread over the SMs
     // shortest
@@ -188,7 +193,7 @@ Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
         if (!k && items > 16 * sms) continue;  // far from few rows
         for (int n = 1; n <= most; ++n) {
             const int per = cdiv(a.P, (int64_t)n * step) * step;
-            const Work w = k ? Work{(double)items * n, BLOCK_US + per / step * TILE_US, 1.0}
+            const Work w = k ? Work{(double)items * n, BLOCK_US + per / step * tile_us(dtype, false), 1.0}
                              : few_work((double)items * n, per, fp, dtype, sms);
             const double last = COMBINE_US + 0.07 * n;
             consider({together(w, own ? own_few : nothing, sms) + last + (k && own ? 1.0 : 0.0), {k == 1, false}, 0, per});
@@ -248,6 +253,18 @@ size_t hk_shared_prefix_workspace_bytes(const hk_shared_prefix_params* p) {
     PrefixArgs a{};
     make_plan(p, a);
     return slot_rows(a) * SLOT_BYTES;
+}
+
+// For tests: which kernels take the call's blocks of rows (many rows against the prefix, against the own keys; both in one go), the runs
+// of the prefix and of the own keys, and the slots of a row.
+int hk_shared_prefix_plan(const hk_shared_prefix_params* p, int* plan) {
+    const int rc = check_sizes(p);
+    if (rc != HK_OK) return rc;
+    PrefixArgs a{};
+    const Plan x = make_plan(p, a);
+    const int out[] = {x.prefix_many, x.own_many, a.whole, a.splits_p, a.splits_o, a.slots};
+    std::copy(out, out + 6, plan);
+    return HK_OK;
 }
 
 int hk_shared_prefix_attention(const hk_shared_prefix_params* p, void* stream_) {
