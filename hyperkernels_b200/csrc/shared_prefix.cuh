@@ -1,6 +1,8 @@
 // shared_prefix.cuh -- what the kernels of the attention over a shared prefix (hk_shared_prefix_attention) have in common.
 #pragma once
 
+#include <type_traits>
+
 #include "operators.cuh"
 
 namespace hk {
@@ -39,6 +41,12 @@ __device__ __forceinline__ const X* row_of(const hk_view& v, int64_t b, int64_t 
 __device__ __forceinline__ int request_keys(const PrefixArgs& a, int b) { return a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S; }
 // own keys that token t of a request of `len` keys sees
 __device__ __forceinline__ int token_keys(const PrefixArgs& a, int len, int t) { return a.causal ? min(len, max(0, len - a.T + t + 1)) : len; }
+
+// The 2^ of what a softmax's reference lies below the row's largest score.  A weight takes the type of the values, and fp16 has none below
+// 2^-24: with the largest at 2^7 (2^15 where a stale maximum may lie 2^8 lower), those down to 2^-31 of it are kept, where many of
+// them would be lost beside one that is large.  The sums and the LSE take it back by themselves.
+template <class X>
+__host__ __device__ constexpr float lift() { return std::is_same<X, __half>::value ? 7.f : 0.f; }
 
 template <class X>
 __device__ __forceinline__ void store4(X* p, float4 v) {

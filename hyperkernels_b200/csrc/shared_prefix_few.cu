@@ -250,7 +250,7 @@ struct RowsOf16 {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * scale_log2e;
+            mx[i] = fmaf(fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)), scale_log2e, -lift<X>());
             const float mn = fmaxf(m[i], mx[i]);
             raised |= mn > m[i];
             ref[i] = mn == -INFINITY ? 0.f : mn;

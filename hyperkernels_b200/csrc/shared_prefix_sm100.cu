@@ -219,7 +219,6 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             uint4* raw = reinterpret_cast<uint4*>(sKV + s * C::KV_BYTES);
             if constexpr (LOW) {
                 constexpr int EACH = C::KV_RAW / 16 / 64;
-                
                 uint4 *from = raw + me, *low = from + C::KV_RAW / 16, x[EACH];
 #pragma unroll
                 for (int k = 0; k < EACH; ++k) x[k] = from[k * 64];
@@ -525,8 +524,8 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                             tmem_st32(at_o + c, y);
                         }
                     }
-                    const float ref = mn == -INFINITY ? 0.f : mn;
-                    const float2 nm = make_float2(-ref, -ref);
+                    const float up = mn == -INFINITY ? 0.f : lift<X>() - mn;
+                    const float2 nm = make_float2(up, up);
                     float2 sum[2] = {};
                     // the weights take the type of the values: half a step of it each
                     auto weights = [&](auto poly) {
@@ -549,6 +548,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                 tc_fence_before_sync();
                 mbar_arrive_warp(&sh.p_full[q % 3], lane);
             }
+            m -= lift<X>();  // what the weights were taken by
 #pragma unroll
             for (int i = 0; i < 64; ++i) o[i] = 0.f;
             if (ok && n > 0 && wait(sh.o_full, (n - 1) * streams + t, W_O, n) && live) {

@@ -179,6 +179,32 @@ def test_no_lengths_means_all(dtype, T):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,P,S", [(1, 4000, 60), (3, 4000, 0), (150, 4000, 200), (700, 2000, 700), (140, 0, 300)])
+def test_many_small_weights_beside_a_large_one(dtype, T, P, S):
+    """The first key takes nearly all, and its value is 0: the result is what the others give, each 2^-26 of the first.
+
+    A weight of 2^-26.1 or more (26 ln 2 rounds to within 0.1), lifted by seven binary places in fp16, is rounded there to a multiple of
+    2^-24: by 2^-25 in 2^-19.1 at most; in the other types by half a step.  The score of the first key is 26 ln 2 more than that of the others, which is 0; a score's error of
+    d = 80 u * 26 + 70 u moves all weights by less than 2 d, and a rounding of the result to fp16 is 2^-25 at most below 2^-14."""
+    t = TYPES[dtype]
+    q = torch.zeros((2, 2, T, 64), device="cuda", dtype=t)
+    q[..., 0] = 26.0 * math.log(2.0)
+    kp, vp = (torch.full((2, P, 64), x, device="cuda", dtype=t) for x in (0.0, 1.0))
+    k, v = (torch.full((2, 2, S, 64), x, device="cuda", dtype=t) for x in (0.0, 1.0))
+    first = (kp[:, 0], vp[:, 0]) if P else (k[:, :, 0], v[:, :, 0])
+    first[0][..., 0], first[1][:] = 1.0, 0.0
+    lens = torch.full((2,), S, device="cuda", dtype=torch.int32)
+    o, lse = hk.shared_prefix_attention(q, kp, vp, k, v, lens, 1.0, True)
+    O, LSE, _, _ = definition(q, kp, vp, k, v, lens, True, 1.0)
+    d = (80 * 26 + 70) * U
+    step = torch.finfo(t).eps / 2 if dtype != "f32" else 0.0
+    weight = 2.0 ** -5.9 if dtype == "f16" else step
+    assert bool(((o.double() - O).abs() <= (2 * d + 200 * U + weight + step) * O + (2.0 ** -25 if dtype == "f16" else 0.0)).all())
+    assert bool(((lse.double() - LSE).abs() <= d + 200 * U + 4 * U * LSE.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T", [1, 20, 140])
 def test_large_scores_and_other_scales(dtype, T):
     """Scores of +-200: one key takes almost everything, the maximum moves late, masked keys would be the largest."""
