@@ -97,6 +97,7 @@ int check(const hk_shared_prefix_params* p) {
     };
     if ((rc = keys(p->Kp, 1, p->prefix_len)) || (rc = keys(p->Vp, 1, p->prefix_len)) || (rc = keys(p->K, p->B, p->kv_len)) || (rc = keys(p->V, p->B, p->kv_len))) return rc;
     if (!p->LSE) return HK_ERR_NULL_POINTER;
+    if ((p->B > 1 && p->lse_strideB < p->T) || (p->nh > 1 && p->lse_strideH < p->T)) return HK_ERR_UNSUPPORTED;  // rows on top of each other
     if ((reinterpret_cast<uintptr_t>(p->LSE) | reinterpret_cast<uintptr_t>(p->lengths)) & 3u) return HK_ERR_MISALIGNED;
     return HK_OK;
 }
@@ -190,7 +191,7 @@ Plan make_plan(const hk_shared_prefix_params* p, PrefixArgs& a) {
         if (k == 1 && a.R <= 32) break;
         const int64_t items = (int64_t)a.Hk * cdiv(a.R, k ? mp.rows : fp.rows);
         const int step = k ? mp.keys : fp.step, most = std::min(64, std::max(1, cdiv(a.P, (k ? 2 : 4) * step)));
-        if (!k && items > 16 * sms) continue;  // far from few rows
+        if (!k && a.R > 32 && items > 16 * sms) continue;  // far from few rows
         for (int n = 1; n <= most; ++n) {
             const int per = cdiv(a.P, (int64_t)n * step) * step;
             const Work w = k ? Work{(double)items * n, BLOCK_US + per / step * tile_us(dtype, false), 1.0}

@@ -112,6 +112,8 @@ def shared_prefix_attention(Q, K_prefix, V_prefix, K, V, lengths, scale: float, 
     those of the new tokens among them.  Rows behind them may hold anything.  H is a multiple of Hkv; query head h reads head
     ``h // (H // Hkv)``.  Every new token sees the whole prefix and its request's own keys, with ``causal`` those up to its
     own: token i of T sees j <= lengths[b] - T + i.  A row that sees no key gives O = 0, LSE = -inf.  P and S may be 0.
+    A key that only ``causal`` hides from a row takes part in it with weight 0, so its values have to be finite.  Keys and values
+    may not be expanded (a stride of 0).  The same call gives the same bits.
     All of one type, which O has too; LSE is float32.  Softmax and sums are fp32."""
     r = (_att._native or _att._torch_calls()).prefix(Q, K_prefix, V_prefix, K, V, lengths, scale, causal, workspace, out, lse,
                                                      stream if stream is None else _stream_handle(stream))

@@ -348,7 +348,11 @@ size_t hk_qk_norm_rotary_workspace_bytes(const hk_qk_params* p);
 
 /* Attention of a batch whose requests share a prefix.  Row (b, i) of a head sees every prefix key and the keys
  * j < lengths[b] of its request, with is_causal those with j <= lengths[b] - T + i.  Heads in groups of nh / nh_kv
- * share a head of keys and values.  A row that sees nothing gives O = 0, LSE = -inf. */
+ * share a head of keys and values.  A row that sees nothing gives O = 0, LSE = -inf.  A key that is_causal alone hides from
+ * a row takes part in it with weight 0, so its values have to be finite.
+ * Keys and values are read by TMA: a stride of 0 over a dimension larger than 1 is refused (HK_ERR_UNSUPPORTED), and so are
+ * results whose rows lie on top of each other.  The same call gives the same bits; how a row's keys are shared out depends on
+ * all sizes of the call, not on `lengths`. */
 typedef struct hk_shared_prefix_params {
     hk_view Q;        /* [B, nh, T, 64], `dtype` */
     hk_view Kp, Vp;   /* [1, nh_kv, prefix_len, 64], once for the whole batch; strideB is not used */

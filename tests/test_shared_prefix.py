@@ -115,7 +115,8 @@ WAYS = [
     (16, 4, 4, 40, 2500, 300, "f32"), (16, 4, 4, 77, 4097, 333, "f16"), (700, 8, 1, 1, 3000, 0, "bf16"), (700, 8, 1, 1, 3001, 0, "f32"),
     (40, 4, 4, 260, 300, 300, "bf16"), (37, 4, 2, 129, 301, 300, "f16"), (3, 4, 4, 300, 900, 400, "f32"), (3, 8, 2, 301, 901, 403, "bf16"),
     (40, 4, 4, 130, 300, 140, "f32"), (2, 4, 4, 700, 0, 700, "bf16"), (2, 4, 4, 700, 0, 701, "f32"), (5, 8, 2, 512, 3001, 700, "f16"),
-    (37, 4, 4, 100, 1, 129, "bf16"), (37, 4, 4, 100, 64, 65, "f32")]
+    (37, 4, 4, 100, 1, 129, "bf16"), (37, 4, 4, 100, 64, 65, "f32"), (1, 3000, 3000, 1, 70, 0, "f32"), (3, 2400, 2400, 1, 33, 0, "bf16"),
+    (1, 5000, 2500, 3, 40, 9, "f16")]
 
 
 def test_the_sizes_take_every_way():
@@ -418,7 +419,7 @@ def _block():
     ("Q.ptr", None, -1), ("Kp.ptr", None, -1), ("V.ptr", None, -1), ("O.ptr", None, -1), ("LSE", None, -1), ("B", 0, -2), ("nh", 0, -2), ("nh_kv", 0, -2), ("nh_kv", 3, -2),
     ("T", 0, -2), ("T", (1 << 30) + 1, -2), ("prefix_len", -1, -2), ("kv_len", -1, -2), ("kv_len", (1 << 30) + 1, -2), ("scale", 0.0, -2), ("scale", math.inf, -2), ("scale", math.nan, -2),
     ("Q.ptr", 0x1004, -3), ("K.sM", 66, -3), ("Vp.sH", 9 * 64 + 2, -3), ("K.sB", -1024, -3), ("lengths", 0x1002, -3), ("LSE", 0x1002, -3),
-    ("O.sM", 0, -6), ("O.sH", 32, -6), ("Kp.sH", 0, -6), ("K.sB", 0, -6), ("V.sM", 0, -6), ("dtype", 3, -6), ("dtype", -1, -6)])
+    ("lse_sB", 2, -6), ("lse_sH", 0, -6), ("O.sM", 0, -6), ("O.sH", 32, -6), ("Kp.sH", 0, -6), ("K.sB", 0, -6), ("V.sM", 0, -6), ("dtype", 3, -6), ("dtype", -1, -6)])
 def test_blocks_that_are_refused(path, value, status):
     b = _block()
     *head, last = path.split(".")
