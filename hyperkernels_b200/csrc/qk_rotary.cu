@@ -8,6 +8,11 @@
 // elements 4 s .. 4 s + 3 and 32 + 4 s .. 32 + 4 s + 3, so both halves of a pair are in one lane whether pairs are neighbours or half a
 // row apart, and a load instruction of a warp takes whole 128-byte lines of four rows.  The rows of the next step are on their way
 // while a step is worked on.
+//
+// Measured (a plain copy runs at 6.54 TB/s): B8, 12 and 12 heads, T 1024, fp32, rotation 18.7 us (82 % of that rate), norm 20.1 (77 %), its
+// backward pass 30.9 (75 %, of which the weights' sums about 2); T 32768, 32 and 32 heads, bf16 rows and fp32 gradients 194 us
+// (85 %); T 32767, 32 and 8 heads, fp32 gradients into bf16 90 us (86 %).  One token of 16 or 64 requests 2.8 to 3.3 us.  Three CTAs to an SM
+// would leave 80 registers a thread, and what is on its way would not fit them (spills: 37.7 us instead of 20.1, 223 instead of 90).
 #include <cmath>
 
 #include "operators.cuh"
