@@ -214,10 +214,13 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     auto key_of = [&](int j) { return j < n_p ? p_begin + j * KEYS : own_begin + (j - n_p) * KEYS; };
 
     // What the tiles need beside the loads.  Rows behind the request's last key may hold anything, and 0 times a NaN is one: they are
-    // cleared among the values.  fp32: the tiles' low parts, by two pairs of warps, every other tile each.
+    // cleared among the values.  fp32: the tiles' low parts, by two pairs of warps.  A pair has every other slot of the ring, not every
+    // other tile: a barrier is waited for by the parity of its phase, and who does not see all phases of a slot can take the one before the
+    // last for its own.
     auto tend = [&](int me, int first_entry) {
+        auto following = [&](int i) { return i % SLOTS + 2 < SLOTS ? i + 2 : (i / SLOTS + 1) * SLOTS + first_entry; };
         bool ok = true;
-        for (int i = first_entry; ok && n > (LOW ? 0 : n_p) && i < 2 * n; i += 2) {
+        for (int i = first_entry; ok && n > (LOW ? 0 : n_p) && i < 2 * n; i = LOW ? following(i) : 2 * n) {
             const auto [j, is_v] = entry(i);
             const int s = i % SLOTS;
             ok = __all_sync(0xffffffffu, LOW ? mbar_wait(wc, &sh.kv_full[s], (i / SLOTS) & 1, W_KV, i) : mbar_wait(wc, &sh.last_full, 0, W_KV, i));
@@ -420,6 +423,8 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
         }
         float o[64], m = -INFINITY, l = 0.f;
         bool ok = true;
+        // 16-bit types: a block of rows waits for every other use of a buffer's barrier.  The use in between, of the other block, is
+        // complete: it was issued before products that this thread has waited for already.
         auto wait = [&](uint64_t* bar, int q, int id, int j) {  // of product q
             ok = __all_sync(0xffffffffu, mbar_wait(wc, &bar[q % 3], (q / 3) & 1, id, j));
             if (ok) tc_fence_after_sync();

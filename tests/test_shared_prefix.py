@@ -152,6 +152,25 @@ def test_every_way_of_cutting_the_work(B, H, Hk, T, P, S, dtype, causal, layout)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,T,P,S,dtype", [
+    (64, 32, 8, 1, 4100, 1000, "f32"), (3, 4, 4, 300, 900, 400, "f32"), (8, 12, 12, 77, 4096, 333, "f32"), (64, 32, 8, 1, 8192, 1000, "bf16"),
+    (5, 8, 2, 512, 3001, 700, "f16"), (16, 12, 12, 1, 2047, 512, "f32")])
+def test_the_same_bits_however_late_the_keys_come(B, H, Hk, T, P, S, dtype):
+    """Every other call finds its keys in the L2, the others in memory: tiles land in other orders and at other times."""
+    x = make(B + T, B, H, Hk, T, P, S, dtype, "bthd")
+    want = hk.shared_prefix_attention(*x, SCALE)
+    check(want, definition(*x, True), dtype)
+    room = torch.empty(1 << 28, device="cuda", dtype=torch.uint8)
+    different = torch.zeros((), device="cuda", dtype=torch.int64)
+    for i in range(400):
+        if i % 2:
+            room.fill_(i & 255)
+        o, lse = hk.shared_prefix_attention(*x, SCALE)
+        different += (o != want[0]).any() | (lse != want[1]).any()
+    assert int(different) == 0 and hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T", [1, 3, 40, 150, 400])
 @pytest.mark.parametrize("P", [0, 70, 2600])
