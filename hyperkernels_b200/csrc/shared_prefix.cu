@@ -70,9 +70,9 @@ __global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_consta
         o.x += __shfl_xor_sync(together, o.x, 16); o.y += __shfl_xor_sync(together, o.y, 16);
         o.z += __shfl_xor_sync(together, o.z, 16); o.w += __shfl_xor_sync(together, o.w, 16);
     }
-    const float f = L > 0.f ? 1.f / L : 0.f;
+    const float f = L != 0.f ? 1.f / L : 0.f;
     if (half == 0) store4(O, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-    if (lane == 0) *LSE = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
+    if (lane == 0) *LSE = L != 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
 }
 
 int check_sizes(const hk_shared_prefix_params* p) {

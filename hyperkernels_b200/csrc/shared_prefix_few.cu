@@ -509,12 +509,12 @@ __device__ __forceinline__ void few_job(const CUtensorMap& map_kp, const CUtenso
 #pragma unroll
         for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(a.part + to * 64 + d + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
     } else if (mine) {
-        const float f = L > 0.f ? 1.f / L : 0.f;
+        const float f = L != 0.f ? 1.f / L : 0.f;
         const int row = row0 + r, token = row / a.group, bq = OWN ? b : token / a.T, t = token - bq * a.T, h = kvh * a.group + (row - token * a.group);
         X* to = const_cast<X*>(row_of<X>(a.O, bq, h, t)) + d;
 #pragma unroll
         for (int e = 0; e < E; e += 4) store4(to + e, make_float4(acc[e] * f, acc[e + 1] * f, acc[e + 2] * f, acc[e + 3] * f));
-        if (d == 0) a.LSE[bq * a.lse_sB + h * a.lse_sH + t] = L > 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
+        if (d == 0) a.LSE[bq * a.lse_sB + h * a.lse_sH + t] = L != 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
     }
 }
 

@@ -108,6 +108,13 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
     return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
+// The largest of three, or NaN if one is: then the polynomial, which would make a number of it, is not taken.
+__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 template <class X>
 __global__ void __launch_bounds__(Many<X>::THREADS, 1)
 prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_k,
@@ -519,8 +526,8 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                     }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e;
+                    for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = max3_or_nan(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                    const float top = max3_or_nan(mx[0], mx[1], max3_or_nan(mx[2], mx[3], mx[3])) * a.scale_log2e;
                     const bool raise = m == -INFINITY ? top > -INFINITY : top > m + RISE;
                     const float mn = raise ? top : m, alpha = raise ? ex2_approx(m - mn) : 1.f;  // 0 from -inf
                     m = mn;
@@ -549,8 +556,8 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                             x[i / 2] = pack<X>(w.x, w.y);
                         }
                     };
-                    // a masked score is -inf and has no weight at all: not by the polynomial
-                    if (__all_sync(0xffffffffu, lim >= KEYS)) weights(std::true_type{});
+                    // a masked score is -inf and has no weight at all, one that is NaN has to stay so: not by the polynomial
+                    if (__all_sync(0xffffffffu, lim >= KEYS && top == top)) weights(std::true_type{});
                     else weights(std::false_type{});
                     tmem_st32p(at_s, x);
                     tmem_st32p(at_s + 32, x + 32);
@@ -580,7 +587,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
 #pragma unroll
                 for (int i = 0; i < 16; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             } else {
-                const float f = l > 0.f ? 1.f / l : 0.f;
+                const float f = l != 0.f ? 1.f / l : 0.f;
                 const Where to_row = where(row);
                 uint4* to = reinterpret_cast<uint4*>(const_cast<X*>(row_of<X>(a.O, to_row.b, to_row.h, to_row.t)));
                 if constexpr (LOW) {
@@ -593,7 +600,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                         to[i] = make_uint4(pack<X>(o[8 * i] * f, o[8 * i + 1] * f), pack<X>(o[8 * i + 2] * f, o[8 * i + 3] * f),
                                            pack<X>(o[8 * i + 4] * f, o[8 * i + 5] * f), pack<X>(o[8 * i + 6] * f, o[8 * i + 7] * f));
                 }
-                a.LSE[to_row.b * a.lse_sB + to_row.h * a.lse_sH + to_row.t] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+                a.LSE[to_row.b * a.lse_sB + to_row.h * a.lse_sH + to_row.t] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
             }
         }
     }

@@ -350,6 +350,7 @@ size_t hk_qk_norm_rotary_workspace_bytes(const hk_qk_params* p);
  * j < lengths[b] of its request, with is_causal those with j <= lengths[b] - T + i.  Heads in groups of nh / nh_kv
  * share a head of keys and values.  A row that sees nothing gives O = 0, LSE = -inf.  A key that is_causal alone hides from
  * a row takes part in it with weight 0, so its values have to be finite.
+ * A NaN among a row's scores makes O and LSE of the row NaN; so may an infinite score.
  * Keys and values are read by TMA: a stride of 0 over a dimension larger than 1 is refused (HK_ERR_UNSUPPORTED), and so are
  * results whose rows lie on top of each other.  The same call gives the same bits; how a row's keys are shared out depends on
  * all sizes of the call, not on `lengths`. */

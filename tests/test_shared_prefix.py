@@ -225,6 +225,33 @@ def test_many_small_weights_beside_a_large_one(dtype, T, P, S):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,T,P,S", [(2, 1, 300, 40), (2, 3, 0, 200), (2, 140, 300, 300), (2, 300, 1000, 300), (8, 40, 1500, 100), (2, 140, 0, 300)])
+def test_scores_that_are_no_numbers(H, T, P, S, dtype):
+    """Scores that are NaN, in any column of a tile, make NaN of the rows that see them; the others stay as they were."""
+    x = make(5, 2, H, 2, T, P, S, dtype, lengths=[S, S - 3])
+    want = definition(*x, True)
+    plain = hk.shared_prefix_attention(*x, SCALE)
+    check(plain, want, dtype)
+    first = (S - 3) - T  # keys that all rows of request 1 see, with one more for each row
+    for at in list(range(3)) + list(range(60, 70)) + [127, 128, 129, 255]:
+        for bad in (math.nan, math.inf):
+            for where in ("prefix", "own"):
+                if at >= (P if where == "prefix" else first):
+                    continue
+                k, rows = (x[1][0], slice(None)) if where == "prefix" else (x[3][1, 0], slice(1, 2))
+                keep = k[at].clone()
+                k[at] = bad  # infinities of both signs meet in a score
+                o, lse = hk.shared_prefix_attention(*x, SCALE)
+                k[at] = keep
+                hit, G = torch.zeros_like(lse, dtype=torch.bool), H // 2
+                hit[rows, :G] = True
+                assert bool(o[hit].isnan().all()) and bool(lse[hit].isnan().all()), (at, bad, where)
+                assert torch.equal(o[~hit], plain[0][~hit]) and torch.equal(lse[~hit], plain[1][~hit]), (at, bad, where)
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T", [1, 20, 140])
 def test_large_scores_and_other_scales(dtype, T):
     """Scores of +-200: one key takes almost everything, the maximum moves late, masked keys would be the largest."""
