@@ -108,7 +108,7 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
     return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
-// The largest of three, or NaN if one is: then the polynomial, which would make a number of it, is not taken.
+// The largest of three, or NaN if one is.
 __device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -524,10 +524,14 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                         for (int i = 0; i < 128; ++i)
                             if (i >= lim) x[i] = __float_as_uint(-INFINITY);
                     }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    // Of the columns that the polynomial would take, which makes a number of a NaN, the largest is NaN if one is.
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, poly_mx = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = max3_or_nan(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                    const float top = max3_or_nan(mx[0], mx[1], max3_or_nan(mx[2], mx[3], mx[3])) * a.scale_log2e;
+                    for (int i = 0; i < 128; i += 2) {
+                        if ((i >> 1) % POLY_OF == POLY_OF - 1) poly_mx = max3_or_nan(poly_mx, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                        else mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                    }
+                    const float top = fmax3(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]), poly_mx) * a.scale_log2e;
                     const bool raise = m == -INFINITY ? top > -INFINITY : top > m + RISE;
                     const float mn = raise ? top : m, alpha = raise ? ex2_approx(m - mn) : 1.f;  // 0 from -inf
                     m = mn;
@@ -557,7 +561,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                         }
                     };
                     // a masked score is -inf and has no weight at all, one that is NaN has to stay so: not by the polynomial
-                    if (__all_sync(0xffffffffu, lim >= KEYS && top == top)) weights(std::true_type{});
+                    if (__all_sync(0xffffffffu, lim >= KEYS && poly_mx == poly_mx)) weights(std::true_type{});
                     else weights(std::false_type{});
                     tmem_st32p(at_s, x);
                     tmem_st32p(at_s + 32, x + 32);
