@@ -9,9 +9,9 @@
 // row apart, and a load instruction of a warp takes whole 128-byte lines of four rows.  The rows of the next step are on their way
 // while a step is worked on.
 //
-// Measured (a plain copy runs at 6.54 TB/s): B8, 12 and 12 heads, T 1024, fp32, rotation 18.7 us (82 % of that rate), norm 20.1 (77 %), its
-// backward pass 30.9 (75 %, of which the weights' sums about 2); T 32768, 32 and 32 heads, bf16 rows and fp32 gradients 194 us
-// (85 %); T 32767, 32 and 8 heads, fp32 gradients into bf16 90 us (86 %).  One token of 16 or 64 requests 2.8 to 3.3 us.  Three CTAs to an SM
+// Measured (a plain copy runs at 6.54 TB/s): B8, 12 and 12 heads, T 1024, fp32, rotation 18.2 us (85 % of that rate), norm 20.3 (76 %), its
+// backward pass 31.0 (75 %, of which the weights' sums about 2); T 32768, 32 and 32 heads, bf16 rows and fp32 gradients 190 us
+// (86 %); T 32767, 32 and 8 heads, fp32 gradients into bf16 85 us (91 %).  One token of 16 or 64 requests 2.8 to 3.3 us.  Three CTAs to an SM
 // would leave 80 registers a thread, and what is on its way would not fit them (spills: 37.7 us instead of 20.1, 223 instead of 90).
 #include <cmath>
 
@@ -23,6 +23,7 @@ namespace {
 enum QkMode { QK_ROTATE = 0, QK_NORM = 1, QK_NORM_BACK = 2 };
 constexpr int QK_WARPS = 8;
 constexpr int QK_CTAS = 2;  // that an SM holds
+constexpr int64_t L2_BYTES = 126 << 20;
 
 struct RowView {
     char* ptr;
@@ -38,6 +39,7 @@ struct QkArgs {
     int heads[2];
     uint32_t T, tokens, blocks_q;  // CTAs that take queries; the others take keys
     int split;                     // a warp takes one step of a token's heads, not all of them
+    int past;                      // results are more than the L2 keeps
     int pos64, w_dtype, back;
     float eps;
     hk_rotary_plan plan;
@@ -80,11 +82,18 @@ __device__ __forceinline__ Row8 numbers(const Raw<T>& x) {
 struct Keep {
     uint32_t w[4];
 };
+// With the policy of the results' way through the L2 (two stores to choose from took norm of B8 T1024 from 20.1 to 20.8 us).
+__device__ __forceinline__ void store(float4* p, float4 x, uint64_t policy) {
+    asm volatile("st.global.L2::cache_hint.v4.f32 [%0], {%1,%2,%3,%4}, %5;" ::"l"(p), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void store(uint2* p, uint2 x, uint64_t policy) {
+    asm volatile("st.global.L2::cache_hint.v2.b32 [%0], {%1,%2}, %3;" ::"l"(p), "r"(x.x), "r"(x.y), "l"(policy) : "memory");
+}
 template <class T, bool KEEPS>
-__device__ __forceinline__ void store_row(char* p, int sub, const Row8& r, const uint32_t* raw, const Keep& keep) {
+__device__ __forceinline__ void store_row(char* p, int sub, const Row8& r, const uint32_t* raw, const Keep& keep, uint64_t policy) {
     if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(p)[sub] = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
-        reinterpret_cast<float4*>(p + 128)[sub] = make_float4(r.v[4], r.v[5], r.v[6], r.v[7]);
+        store(reinterpret_cast<float4*>(p) + sub, make_float4(r.v[0], r.v[1], r.v[2], r.v[3]), policy);
+        store(reinterpret_cast<float4*>(p + 128) + sub, make_float4(r.v[4], r.v[5], r.v[6], r.v[7]), policy);
     } else {
         uint32_t o[4];
 #pragma unroll
@@ -92,8 +101,8 @@ __device__ __forceinline__ void store_row(char* p, int sub, const Row8& r, const
             o[i] = pack<T>(r.v[2 * i], r.v[2 * i + 1]);
             if (KEEPS) o[i] = (o[i] & ~keep.w[i]) | (raw[i] & keep.w[i]);
         }
-        reinterpret_cast<uint2*>(p)[sub] = make_uint2(o[0], o[1]);
-        reinterpret_cast<uint2*>(p + 64)[sub] = make_uint2(o[2], o[3]);
+        store(reinterpret_cast<uint2*>(p) + sub, make_uint2(o[0], o[1]), policy);
+        store(reinterpret_cast<uint2*>(p + 64) + sub, make_uint2(o[2], o[3]), policy);
     }
 }
 __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
@@ -199,6 +208,9 @@ __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const
             else next_pos[i] = pos;
         }
     };
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+    if (a.past) asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
     Place at = place(block * QK_WARPS + warp);
     pdl_wait();
     pdl_trigger();
@@ -275,7 +287,7 @@ __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const
                     for (int e = 0; e < 8; ++e) r.v[e] *= inv * w[e];
                 }
                 rotate(r, c, s, interleaved);
-                if (valid) store_row<Y, KEEPS>(vy.ptr + at.y + h * vy.sH, sub, r, x[i].w, keep);
+                if (valid) store_row<Y, KEEPS>(vy.ptr + at.y + h * vy.sH, sub, r, x[i].w, keep, policy);
             } else {
                 Row8 z = numbers(g[BACK ? i : 0]);
                 if (!valid) z = Row8{};
@@ -292,7 +304,7 @@ __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const
                 dot = sum8(dot) * (1.f / 64.f);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) z.v[e] = inv * fmaf(-r.v[e], dot, z.v[e]);
-                if (valid) store_row<X, false>(vd.ptr + at.d + h * vd.sH, sub, z, nullptr, keep);
+                if (valid) store_row<X, false>(vd.ptr + at.d + h * vd.sH, sub, z, nullptr, keep, policy);
             }
         }
         at = next;
@@ -434,6 +446,10 @@ int qk_run(const hk_qk_params* p, int mode, bool back, cudaStream_t stream) {
     // Warps enough for all that an SM holds; where there are fewer tokens, a warp takes one step of a token's heads.
     const int64_t most = (int64_t)sm_count() * QK_CTAS;
     a.split = (int64_t)a.tokens < most * QK_WARPS;
+    // What is next reads the results, out of the L2 if they fit it: there they are stored to stay (norm and attention, 12 heads, T 1024, fp32:
+    // B8 59.4 us and B16 104.4, 61.4 and 108.5 with stores that do not ask to).  Results that do not fit would only push each other out
+    // (T 32767, 32 and 8 heads, into bf16: 89.3 us, and 84.7 with such stores; norm backward, T 32768, 32 and 32 heads, bf16 193 and 190).
+    a.past = (int64_t)a.tokens * (p->nh + p->nh_k) * HEAD_DIM * esize(dst_t) > L2_BYTES;
     // Groups of lanes by tokens where most of the 16-bit tensors lie head by head (B1, 32 and 8 heads, T 32768, bf16 in and out:
     // 65 us instead of 74, fp32 gradients into bf16 86 instead of 95; fp32 alone gains 1 % and its backward pass has no registers for it)
     int by_head = 0, of_16 = 0;
