@@ -442,3 +442,31 @@ def test_mixed_types_are_refused():
         f = getattr(hk.lib(), "hk_" + call)
         f.argtypes = [C.c_void_p, C.c_void_p]
         assert f(C.byref(b), None) == -6, (call, x, y, w)
+
+
+@pytest.mark.gpu
+def test_small_results_are_tensors_of_their_own():
+    """They may share an allocation, but no element, and what is done to one, or its end, leaves the others alone."""
+    q, k = inputs(8, 3, 4, 2, 5, BF16, "packed")
+    pos = torch.arange(5, device="cuda").expand(1, 3, 5)
+    w = torch.ones(64, device="cuda", dtype=BF16)
+    first = hk.qk_norm_rotary_backward(q, k, q, k, w, w, pos, (32,))
+    want = [x.clone() for x in first]
+    assert all(x.is_contiguous() and x.data_ptr() % 256 == 0 for x in first)
+    spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in first)
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+    kept = first[3]
+    for x in first[:3]:
+        x.fill_(7.0)
+    assert torch.equal(kept, want[3]) and kept._version == 0 and kept._base is None
+    del first, x
+    others = [hk.qk_norm_rotary_backward(q, k, q, k, w, w, pos, (32,)) for _ in range(20)]
+    assert torch.equal(kept, want[3]) and all(torch.equal(a, b) for o in others for a, b in zip(o, want))
+    with torch.inference_mode():
+        assert torch.equal(hk.rotary_forward(q, None, pos, (32,))[0], hk.rotary_forward(q, None, pos, (32,))[0])
+    leaf = hk.rotary_forward(q, None, pos, (32,), out_dtype=F32)[0].requires_grad_()  # as any tensor: autograd takes it for a leaf
+    (leaf * 2.0).sum().backward()
+    assert bool((leaf.grad == 2.0).all())
+    huge = torch.zeros((1, 1, 1, 64), device="cuda").expand(1 << 20, 1 << 10, 1 << 20, 64)  # 2^58 bytes
+    with pytest.raises((hk.HKError, RuntimeError)):
+        hk.rotary_forward(huge, None, pos[:, :1, :1].expand(1, 1 << 20, 1 << 20), (32,))
