@@ -11,7 +11,7 @@
 //
 // Measured (a plain copy runs at 6.54 TB/s): B8, 12 and 12 heads, T 1024, fp32, rotation 18.2 us (85 % of that rate), norm 20.3 (76 %), its
 // backward pass 31.0 (75 %, of which the weights' sums about 2); T 32768, 32 and 32 heads, bf16 rows and fp32 gradients 190 us
-// (86 %); T 32767, 32 and 8 heads, fp32 gradients into bf16 85 us (91 %).  One token of 16 or 64 requests 2.8 to 3.3 us.  Three CTAs to an SM
+// (86 %); T 32767, 32 and 8 heads, fp32 gradients into bf16 85 us (91 %).  One token of 16 or 64 requests 2.2 to 2.9 us.  Three CTAs to an SM
 // would leave 80 registers a thread, and what is on its way would not fit them (spills: 37.7 us instead of 20.1, 223 instead of 90).
 #include <cmath>
 

@@ -14,9 +14,9 @@
 //
 // 16-bit types are bound by the exponentials: 256 rows x 128 keys are 2 070 cycles of the special function units if they take four of
 // five, and a tile takes 2 500 to 2 750 (1.4 us; masked 1.8).  fp32 is bound by the tensor core: 1 680 cycles of a tile's 2 030 (1.1 us).  A
-// CTA takes about 5 us beside its tiles.  8 requests of 512 tokens, 32 heads on 8, 8 192 and up to 1 024 keys, bf16: 345 us alone, 384
+// CTA takes about 5 us beside its tiles.  8 requests of 512 tokens, 32 heads on 8, 8 192 and up to 1 024 keys, bf16: 348 us alone, 385
 // under load (760 TFLOP/s; 245 us for the exponentials at 16 a clock and SM, 175 for the products).  8 requests of 77 tokens, 12 heads,
-// 4 096 and up to 333 keys, fp32: 46.5 us (52 from Python, 29 for the products).
+// 4 096 and up to 333 keys, fp32: 47 us (52 from Python, 29 for the products).
 // A row of Q and of O to a thread: with eight lanes to a row, through shared memory, the two took 351 and 48.6 instead of 346 and 47.0.
 #include <cmath>
 #include <mutex>
