@@ -12,9 +12,10 @@
 // a tile comes back into registers and is added there in fp32: the tensor core's additions cut off instead of rounding, and over
 // thousands of keys in one accumulator that would be seen.
 //
-// 16-bit types are bound by the exponentials: 256 rows x 128 keys are 2 070 cycles of the special function units if they take four of
-// five, and a tile takes 2 500 to 2 750 (1.4 us; masked 1.8).  fp32 is bound by the tensor core: 1 680 cycles of a tile's 2 030 (1.1 us).  A
-// CTA takes about 5 us beside its tiles.  8 requests of 512 tokens, 32 heads on 8, 8 192 and up to 1 024 keys, bf16: 348 us alone, 385
+// 16-bit types are bound by the softmax: scaling, exponentials, sums and rounding of 256 rows x 128 keys take 1 930 to 2 120 cycles by
+// themselves, whether none or a third of the exponentials goes by a polynomial (the special functions alone need 2 048 or less, packed
+// arithmetic takes two issue slots), and a tile takes 2 500 to 2 600 (masked 0.4 us more).  fp32 is bound by the tensor core: 1 680 cycles of a tile's 2 030 (1.1 us).  A
+// CTA takes about 5 us beside its tiles.  8 requests of 512 tokens, 32 heads on 8, 8 192 and up to 1 024 keys, bf16: 342 us alone, 380
 // under load (760 TFLOP/s; 245 us for the exponentials at 16 a clock and SM, 175 for the products).  8 requests of 77 tokens, 12 heads,
 // 4 096 and up to 333 keys, fp32: 47 us (52 from Python, 29 for the products).
 // A row of Q and of O to a thread: with eight lanes to a row, through shared memory, the two took 351 and 48.6 instead of 346 and 47.0.
@@ -508,7 +509,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             // O stays in tensor memory and is scaled there when a maximum has risen by more than 2^RISE: a stale one makes weights
             // larger, which neither fp32 sums nor 16-bit types mind up to there
             constexpr float RISE = 8.f;
-            constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial (2, 4, 5, 6, 8, none: 437, 388, 376, 375, 404, 407 us, prefill)
+            constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial (4, 5, 6: 352, 342, 346 us, prefill)
             const uint32_t at_o = lanes + COL_O + t * 64;
             uint32_t x[128];
             for (int j = 0; j < n && wait(sh.s_full, j * streams + t, W_S, j); ++j) {
@@ -551,13 +552,25 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                     const float2 nm = make_float2(up, up);
                     float2 sum[2] = {};
                     // the weights take the type of the values: half a step of it each
+                    // A run of them is summed and packed while the next one's exponentials are under way (prefill, runs of 8, 16, 32, 64: 351,
+                    // 342, 346, 347 us; each pair at once: 348).
                     auto weights = [&](auto poly) {
+                        constexpr int RUN = 16;
 #pragma unroll
-                        for (int i = 0; i < 128; i += 2) {
-                            const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, nm);
-                            const float2 w = decltype(poly)::value && (i >> 1) % POLY_OF == POLY_OF - 1 ? ex2_poly(e) : make_float2(ex2_approx(e.x), ex2_approx(e.y));
-                            sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
-                            x[i / 2] = pack<X>(w.x, w.y);
+                        for (int c = 0; c < 128 + RUN; c += RUN) {
+#pragma unroll
+                            for (int i = c; i < c + RUN && i < 128; i += 2) {
+                                const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, nm);
+                                const float2 w = decltype(poly)::value && (i >> 1) % POLY_OF == POLY_OF - 1 ? ex2_poly(e) : make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                                x[i] = __float_as_uint(w.x);
+                                x[i + 1] = __float_as_uint(w.y);
+                            }
+#pragma unroll
+                            for (int i = c - RUN; i >= 0 && i < c; i += 2) {
+                                const float2 w = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                                sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
+                                x[i / 2] = pack<X>(w.x, w.y);
+                            }
                         }
                     };
                     // a masked score is -inf and has no weight at all, one that is NaN has to stay so: not by the polynomial
