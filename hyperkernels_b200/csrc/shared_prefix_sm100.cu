@@ -509,7 +509,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             // O stays in tensor memory and is scaled there when a maximum has risen by more than 2^RISE: a stale one makes weights
             // larger, which neither fp32 sums nor 16-bit types mind up to there
             constexpr float RISE = 8.f;
-            constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial (4, 5, 6: 352, 342, 346 us, prefill)
+            constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial (3 to 8: 356, 352, 342, 346, 350, 354 us, prefill)
             const uint32_t at_o = lanes + COL_O + t * 64;
             uint32_t x[128];
             for (int j = 0; j < n && wait(sh.s_full, j * streams + t, W_S, j); ++j) {
