@@ -506,9 +506,9 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             }
             if (ok && n > 0) add(n - 1);
         } else if (t < streams) {
-            // O stays in tensor memory and is scaled there when a maximum has risen by more than 2^RISE: a stale one makes weights
-            // larger, which neither fp32 sums nor 16-bit types mind up to there
-            constexpr float RISE = 8.f;
+            // O stays in tensor memory and is scaled there when a tile's weights come to more than MOST: a stale maximum makes them larger,
+            // which neither fp32 sums nor 16-bit types mind up to there
+            constexpr float MOST = lift<X>() > 0.f ? 32768.f : 256.f;  // 2^8 of the reference's own weight
             constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial (3 to 8: 356, 352, 342, 346, 350, 354 us, prefill)
             const uint32_t at_o = lanes + COL_O + t * 64;
             uint32_t x[128];
@@ -517,45 +517,19 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                 const uint32_t at_s = lanes + q % 3 * 128;
                 if (live) {
                     const int lim = (j < n_p ? p_end : limit) - key_of(j);  // columns the row sees
+                    auto load = [&] {
 #pragma unroll
-                    for (int c = 0; c < 128; c += 32) tmem_ld32p(at_s + c, x + c);
-                    tmem_wait_ld();
-                    if (lim < KEYS) {
-#pragma unroll
-                        for (int i = 0; i < 128; ++i)
-                            if (i >= lim) x[i] = __float_as_uint(-INFINITY);
-                    }
-                    // Of the columns that the polynomial would take, which makes a number of a NaN, the largest is NaN if one is.
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, poly_mx = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 128; i += 2) {
-                        if ((i >> 1) % POLY_OF == POLY_OF - 1) poly_mx = max3_or_nan(poly_mx, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                        else mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                    }
-                    const float top = fmax3(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]), poly_mx) * a.scale_log2e;
-                    const bool raise = m == -INFINITY ? top > -INFINITY : top > m + RISE;
-                    const float mn = raise ? top : m, alpha = raise ? ex2_approx(m - mn) : 1.f;  // 0 from -inf
-                    m = mn;
-                    if (j > 0 && __any_sync(0xffffffffu, raise)) {
-                        if (!wait(sh.o_full, q - streams, W_O, j)) break;
-#pragma unroll 1
-                        for (int c = 0; c < 64; c += 32) {
-                            uint32_t y[32];
-                            tmem_ld32(at_o + c, y);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
-                            tmem_st32(at_o + c, y);
-                        }
-                    }
-                    const float up = mn == -INFINITY ? 0.f : lift<X>() - mn;
-                    const float2 nm = make_float2(up, up);
-                    float2 sum[2] = {};
-                    // the weights take the type of the values: half a step of it each
-                    // A run of them is summed and packed while the next one's exponentials are under way (prefill, runs of 8, 16, 32, 64: 351,
-                    // 342, 346, 347 us; each pair at once: 348).
+                        for (int c = 0; c < 128; c += 32) tmem_ld32p(at_s + c, x + c);
+                        tmem_wait_ld();
+                    };
+                    float2 sum[2];
+                    // The weights take the type of the values: half a step of it each.  A run of them is summed and packed while the next
+                    // one's exponentials are under way (runs of 16 for 8, 32, 64: prefill 342 us, 351, 346, 347; each pair at once: 348).
                     auto weights = [&](auto poly) {
                         constexpr int RUN = 16;
+                        const float up = m == -INFINITY ? 0.f : lift<X>() - m;
+                        const float2 nm = make_float2(up, up);
+                        sum[0] = sum[1] = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int c = 0; c < 128 + RUN; c += RUN) {
 #pragma unroll
@@ -572,13 +546,54 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                                 x[i / 2] = pack<X>(w.x, w.y);
                             }
                         }
+                        return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     };
-                    // a masked score is -inf and has no weight at all, one that is NaN has to stay so: not by the polynomial
-                    if (__all_sync(0xffffffffu, lim >= KEYS && poly_mx == poly_mx)) weights(std::true_type{});
-                    else weights(std::false_type{});
+                    load();
+                    // Most tiles raise no maximum by much: their weights are taken by the one there is, and their sum tells if it was too
+                    // low.  Then, and where keys are masked, the maximum is sought first.  (Always to seek it took 342 us instead of 327,
+                    // to seek it beside the weights 354.)  The polynomial would make small numbers of a large argument and of a NaN.
+                    float alpha = 1.f, add = 0.f;
+                    bool done = false;
+                    if (__all_sync(0xffffffffu, lim >= KEYS && m > -INFINITY)) {
+                        float poly_top = -INFINITY;
+#pragma unroll
+                        for (int i = 2 * (POLY_OF - 1); i < 128; i += 2 * POLY_OF) poly_top = max3_or_nan(poly_top, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                        add = weights(std::true_type{});
+                        done = __all_sync(0xffffffffu, add <= MOST && fmaf(poly_top, a.scale_log2e, -m) <= 8.f);
+                        if (!done) load();
+                    }
+                    if (!done) {
+                        if (lim < KEYS) {
+#pragma unroll
+                            for (int i = 0; i < 128; ++i)
+                                if (i >= lim) x[i] = __float_as_uint(-INFINITY);
+                        }
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e;
+                        const bool raise = top > m;
+                        if (raise) {
+                            alpha = ex2_approx(m - top);  // 0 from -inf
+                            m = top;
+                        }
+                        if (j > 0 && __any_sync(0xffffffffu, raise)) {
+                            if (!wait(sh.o_full, q - streams, W_O, j)) break;
+#pragma unroll 1
+                            for (int c = 0; c < 64; c += 32) {
+                                uint32_t y[32];
+                                tmem_ld32(at_o + c, y);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+                                tmem_st32(at_o + c, y);
+                            }
+                        }
+                        add = weights(std::false_type{});
+                    }
                     tmem_st32p(at_s, x);
                     tmem_st32p(at_s + 32, x + 32);
-                    l = fmaf(l, alpha, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                    l = fmaf(l, alpha, add);
                     tmem_wait_st();
                 }
                 tc_fence_before_sync();

@@ -225,6 +225,30 @@ def test_many_small_weights_beside_a_large_one(dtype, T, P, S):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,P,S", [(140, 390, 0), (300, 0, 300), (3, 390, 5)])
+@pytest.mark.parametrize("height", [4.0, 30.0, 90.0, 1000.0, 40000.0])
+def test_one_late_key_that_takes_all(height, T, P, S, dtype):
+    """Scores of about 1, and in each column of the second and third tile, in turn, one key of `height` (16-bit types hold all five)."""
+    t = TYPES[dtype]
+    x = list(make(9, 1, 1, 1, T, P, S, dtype, lengths=[S], sigma=0.3))
+    x[0][..., 0] = 1.0
+    keys, values, n = (x[1], x[2], P) if P else (x[3][:, 0], x[4][:, 0], S)
+    keys[..., 0] = 0.0
+    step = torch.finfo(t).eps / 2 if dtype != "f32" else 0.0
+    for at in range(128, min(n, 384), 1 if height == 90.0 else 7):
+        keys[0, at, 0] = height
+        O, LSE, mean, size = definition(*x, P > 0, 1.0)
+        o, lse = hk.shared_prefix_attention(*x, 1.0, P > 0)
+        keys[0, at, 0] = 0.0
+        d = (80 * size + 3 * size.clamp(min=1) * 1.45 + 70) * U
+        bound = (2 * d[..., None] + 200 * U + step) * mean + step * O.abs() + (2.0 ** -25 if dtype == "f16" else 1e-30)
+        assert bool(((o.double() - O).abs() <= bound).all()), at
+        assert bool(((lse.double() - LSE).abs() <= d + 200 * U + 4 * U * LSE.abs()).all()), at
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("H,T,P,S", [(2, 1, 300, 40), (2, 3, 0, 200), (2, 140, 300, 300), (2, 300, 1000, 300), (8, 40, 1500, 100), (2, 140, 0, 300)])
 def test_scores_that_are_no_numbers(H, T, P, S, dtype):
     """Scores that are NaN, in any column of a tile, make NaN of the rows that see them; the others stay as they were."""
@@ -233,7 +257,7 @@ def test_scores_that_are_no_numbers(H, T, P, S, dtype):
     plain = hk.shared_prefix_attention(*x, SCALE)
     check(plain, want, dtype)
     first = (S - 3) - T  # keys that all rows of request 1 see, with one more for each row
-    for at in list(range(3)) + list(range(60, 70)) + [127, 128, 129, 255]:
+    for at in list(range(3)) + list(range(60, 70)) + [127, 128, 129] + list(range(134, 140)) + [188, 255]:
         for bad in (math.nan, math.inf):
             for where in ("prefix", "own"):
                 if at >= (P if where == "prefix" else first):
