@@ -14,9 +14,9 @@
 //
 // 16-bit types are bound by the softmax: scaling, exponentials, sums and rounding of 256 rows x 128 keys take 1 930 to 2 120 cycles by
 // themselves, whether none or a third of the exponentials goes by a polynomial (the special functions alone need 2 048 or less, packed
-// arithmetic takes two issue slots), and a tile takes 2 500 to 2 600 (masked 0.4 us more).  fp32 is bound by the tensor core: 1 680 cycles of a tile's 2 030 (1.1 us).  A
-// CTA takes about 5 us beside its tiles.  8 requests of 512 tokens, 32 heads on 8, 8 192 and up to 1 024 keys, bf16: 342 us alone, 380
-// under load (760 TFLOP/s; 245 us for the exponentials at 16 a clock and SM, 175 for the products).  8 requests of 77 tokens, 12 heads,
+// arithmetic takes two issue slots), and a tile takes 2 400 to 2 500 (masked 0.4 us more).  fp32 is bound by the tensor core: 1 680 cycles of a tile's 2 030 (1.1 us).  A
+// CTA takes about 5 us beside its tiles.  8 requests of 512 tokens, 32 heads on 8, 8 192 and up to 1 024 keys, bf16: 326 us alone, 365
+// under load (800 TFLOP/s; 245 us for the exponentials at 16 a clock and SM, 175 for the products).  8 requests of 77 tokens, 12 heads,
 // 4 096 and up to 333 keys, fp32: 47 us (52 from Python, 29 for the products).
 // A row of Q and of O to a thread: with eight lanes to a row, through shared memory, the two took 351 and 48.6 instead of 346 and 47.0.
 #include <cmath>
@@ -509,7 +509,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
             // O stays in tensor memory and is scaled there when a tile's weights come to more than MOST: a stale maximum makes them larger,
             // which neither fp32 sums nor 16-bit types mind up to there
             constexpr float MOST = lift<X>() > 0.f ? 32768.f : 256.f;  // 2^8 of the reference's own weight
-            constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial (3 to 8: 356, 352, 342, 346, 350, 354 us, prefill)
+            constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial (3, 4, 5, 6, 8: 336, 324, 326, 329, 332 us, prefill; under load 4 takes 369, 5 365)
             const uint32_t at_o = lanes + COL_O + t * 64;
             uint32_t x[128];
             for (int j = 0; j < n && wait(sh.s_full, j * streams + t, W_S, j); ++j) {
@@ -524,7 +524,7 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
                     };
                     float2 sum[2];
                     // The weights take the type of the values: half a step of it each.  A run of them is summed and packed while the next
-                    // one's exponentials are under way (runs of 16 for 8, 32, 64: prefill 342 us, 351, 346, 347; each pair at once: 348).
+                    // one's exponentials are under way (runs of 16: prefill 342 us, each pair at once 348).
                     auto weights = [&](auto poly) {
                         constexpr int RUN = 16;
                         const float up = m == -INFINITY ? 0.f : lift<X>() - m;
