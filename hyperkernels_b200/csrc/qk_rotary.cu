@@ -9,9 +9,9 @@
 // row apart, and a load instruction of a warp takes whole 128-byte lines of four rows.  The rows of the next step are on their way
 // while a step is worked on.
 //
-// Measured (a plain copy runs at 6.54 TB/s): B8, 12 and 12 heads, T 1024, fp32, rotation 18.2 us (85 % of that rate), norm 20.3 (76 %), its
-// backward pass 31.0 (75 %, of which the weights' sums about 2); T 32768, 32 and 32 heads, bf16 rows and fp32 gradients 190 us
-// (86 %); T 32767, 32 and 8 heads, fp32 gradients into bf16 85 us (91 %).  One token of 16 or 64 requests 2.2 to 2.9 us.  Three CTAs to an SM
+// Measured (a plain copy runs at 6.54 TB/s): B8, 12 and 12 heads, T 1024, fp32, rotation 17.9 us (86 % of that rate), norm 19.5 (79 %), its
+// backward pass 31.1 (74 %, of which the weights' sums about 2); T 32768, 32 and 32 heads, bf16 rows and fp32 gradients 188 us
+// (87 %); T 32767, 32 and 8 heads, fp32 gradients into bf16 84 us (92 %).  One token of 16 or 64 requests 2.2 to 2.9 us.  Three CTAs to an SM
 // would leave 80 registers a thread, and what is on its way would not fit them (spills: 37.7 us instead of 20.1, 223 instead of 90).
 #include <cmath>
 
@@ -129,16 +129,27 @@ __device__ __forceinline__ void rotate(Row8& r, const float (&c)[4], const float
         for (int i = 0; i < 4; ++i) turn(r.v[i], r.v[i + 4], c[i], s[i]);
     }
 }
-__device__ __forceinline__ float sum8(float x) {  // over the eight lanes of a row
+// Sums over the eight lanes of a row, of several rows side by side: one after the other, they would be a chain of
+// shuffles (norm of B8 T1024 20.3 us instead of 19.5).
+template <int U>
+__device__ __forceinline__ void sum8(float (&x)[U]) {
 #pragma unroll
-    for (int off = 4; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-    return x;
+    for (int off = 4; off > 0; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < U; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], off);
 }
-__device__ __forceinline__ float rms_inverse(const Row8& x, float eps) {
-    float ss = 0.f;
+template <class T, int U>
+__device__ __forceinline__ void rms_inverse(const Raw<T> (&x)[U], float eps, float (&inv)[U]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x.v[i], x.v[i], ss);
-    return rsqrtf(fmaf(sum8(ss), 1.f / 64.f, eps));
+    for (int i = 0; i < U; ++i) {
+        const Row8 r = numbers(x[i]);
+        inv[i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) inv[i] = fmaf(r.v[e], r.v[e], inv[i]);
+    }
+    sum8(inv);
+#pragma unroll
+    for (int i = 0; i < U; ++i) inv[i] = rsqrtf(fmaf(inv[i], 1.f / 64.f, eps));
 }
 
 // U rows of each of the warp's four groups of lanes are a step.  TOKENS: the groups take four tokens that follow each other, and each
@@ -181,8 +192,8 @@ __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const
         p.end = TOKENS ? (4 * strip + grp < a.tokens ? heads : 0) : a.split ? min(p.head + STEP, heads) : heads;
         return p;
     };
-    Raw<X> next_x[U];
-    Raw<Y> next_g[BACK ? U : 1];
+    Raw<X> next_x[U] = {};
+    Raw<Y> next_g[BACK ? U : 1] = {};
     auto load = [&](const Place& p) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
@@ -273,38 +284,48 @@ __global__ void __launch_bounds__(QK_WARPS * 32, QK_CTAS) qk_rotary_kernel(const
             }
         }
         fresh = on;
+        float inv[U];  // of rows that are none: anything
+        if (MODE != QK_ROTATE) rms_inverse(x, a.eps, inv);
+        if (!BACK) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int h = at.head + HOP * i + first_head;
-            const bool valid = h < at.end;
-            if (!__any_sync(0xffffffffu, valid)) break;
-            Row8 r = numbers(x[i]);
-            if (MODE != QK_ROTATE && !valid) r = Row8{};
-            if (!BACK) {
+            for (int i = 0; i < U; ++i) {
+                const int h = at.head + HOP * i + first_head;
+                if (h >= at.end) break;
+                Row8 r = numbers(x[i]);
                 if (MODE == QK_NORM) {
-                    const float inv = rms_inverse(r, a.eps);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) r.v[e] *= inv * w[e];
+                    for (int e = 0; e < 8; ++e) r.v[e] *= inv[i] * w[e];
                 }
                 rotate(r, c, s, interleaved);
-                if (valid) store_row<Y, KEEPS>(vy.ptr + at.y + h * vy.sH, sub, r, x[i].w, keep, policy);
-            } else {
-                Row8 z = numbers(g[BACK ? i : 0]);
-                if (!valid) z = Row8{};
-                const float inv = rms_inverse(r, a.eps);
-                rotate(z, c, s, interleaved);
-                float dot = 0.f;
+                store_row<Y, KEEPS>(vy.ptr + at.y + h * vy.sH, sub, r, x[i].w, keep, policy);
+            }
+        } else {
+            Row8 z[U];
+            float dot[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const bool valid = at.head + HOP * i + first_head < at.end;
+                const Row8 r = numbers(x[i]);
+                z[i] = numbers(g[BACK ? i : 0]);
+                rotate(z[i], c, s, interleaved);
+                dot[i] = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    r.v[e] *= inv;
-                    if (valid) dw[e] = fmaf(z.v[e], r.v[e], dw[e]);
-                    z.v[e] *= w[e];
-                    dot = fmaf(z.v[e], r.v[e], dot);
+                    const float n = r.v[e] * inv[i];
+                    if (valid) dw[e] = fmaf(z[i].v[e], n, dw[e]);
+                    z[i].v[e] *= w[e];
+                    dot[i] = fmaf(z[i].v[e], n, dot[i]);
                 }
-                dot = sum8(dot) * (1.f / 64.f);
+            }
+            sum8(dot);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) z.v[e] = inv * fmaf(-r.v[e], dot, z.v[e]);
-                if (valid) store_row<X, false>(vd.ptr + at.d + h * vd.sH, sub, z, nullptr, keep, policy);
+            for (int i = 0; i < U; ++i) {
+                const int h = at.head + HOP * i + first_head;
+                if (h >= at.end) break;
+                const Row8 r = numbers(x[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[i].v[e] = inv[i] * fmaf(-(r.v[e] * inv[i]), dot[i] * (1.f / 64.f), z[i].v[e]);
+                store_row<X, false>(vd.ptr + at.d + h * vd.sH, sub, z[i], nullptr, keep, policy);
             }
         }
         at = next;
@@ -365,7 +386,9 @@ constexpr int rows_of() { return MODE == QK_NORM_BACK ? 2 : 4; }
 template <class X, class Y, int MODE>
 QkKernel kernel_of(int& step, bool tokens) {
     step = rows_of<X, MODE>() * (tokens ? 1 : 4);
-    return tokens ? qk_rotary_kernel<X, Y, MODE, rows_of<X, MODE>(), true> : qk_rotary_kernel<X, Y, MODE, rows_of<X, MODE>(), false>;
+    if constexpr (sizeof(X) == 2 || sizeof(Y) == 2)
+        if (tokens) return qk_rotary_kernel<X, Y, MODE, rows_of<X, MODE>(), true>;
+    return qk_rotary_kernel<X, Y, MODE, rows_of<X, MODE>(), false>;
 }
 template <int MODE>
 QkKernel pick(int x, int y, int& step, bool tokens) {
