@@ -111,7 +111,7 @@ struct Plan {
 // neighbours (runs of the prefix 1 to 32, requests' own keys in 1 to 8 runs) at a dozen sizes.
 constexpr double BLOCK_US = 4.4;                   // many rows: to start and end a CTA
 constexpr double FEW_US = 2.2, COMBINE_US = 3.0;  // few rows: to start and end a CTA; the last kernel
-double tile_us(int dtype, bool own) { return dtype == HK_F32 ? (own ? 1.3 : 1.15) : own ? 1.85 : 1.4; }  // many rows: a tile; own keys are masked
+double tile_us(int dtype, bool own) { return dtype == HK_F32 ? (own ? 1.3 : 1.15) : own ? 1.7 : 1.28; }  // many rows: a tile; own keys are masked
 double batch_us(int dtype, int rows) { return dtype != HK_F32 ? 0.45 : rows <= 2 ? 0.4 : 0.65; }  // few rows: a batch of every warp
 
 // One kind of work: CTAs, microseconds of each, how many an SM holds.
