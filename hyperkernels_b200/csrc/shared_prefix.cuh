@@ -37,8 +37,13 @@ template <class X>
 __device__ __forceinline__ const X* row_of(const hk_view& v, int64_t b, int64_t h, int64_t m) {
     return static_cast<const X*>(v.ptr) + b * v.strideB + h * v.strideH + m * v.strideM;
 }
+// Lengths and queries are what the launch before this call wrote a moment ago: they are read behind pdl_wait, in program order.  The kernel
+// over the own keys next to the prefix's (late) begins when that one's wait is over and has none of its own; nothing says that its SM's
+// L1 has no older line of them, so it does not take them from there.  Few rows read past the L1, many have a fence in front (a row to a
+// thread comes in pieces of lines that the L1 keeps meanwhile): chunk 51.6 us with the fence, 52.5 with the other; decoding of 64 26.1
+// and 25.3.
 // keys that request b has
-__device__ __forceinline__ int request_keys(const PrefixArgs& a, int b) { return a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S; }
+__device__ __forceinline__ int request_keys(const PrefixArgs& a, int b) { return a.lengths ? min(max(__ldcg(a.lengths + b), 0), a.S) : a.S; }
 // own keys that token t of a request of `len` keys sees
 __device__ __forceinline__ int token_keys(const PrefixArgs& a, int len, int t) { return a.causal ? min(len, max(0, len - a.T + t + 1)) : len; }
 

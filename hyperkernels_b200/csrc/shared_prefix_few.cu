@@ -45,6 +45,10 @@ __device__ __forceinline__ uint32_t tf32_low(uint32_t x) { return __float_as_uin
 
 constexpr int FEW_WARPS = 4;
 
+__device__ __forceinline__ uint4 query_piece(const void* p, bool late) {
+    return late ? __ldcg(static_cast<const uint4*>(p)) : *static_cast<const uint4*>(p);
+}
+
 // fp32: x = h + l with h the upper 11 bits of the significand; a product is h h' + (h l' + l h'): what
 // is left out is 2^-22 of it.  A batch's weighted values are added to the rest in fp32 adds, since the tensor core's own additions
 // cut off instead of rounding.
@@ -210,9 +214,9 @@ struct RowsOf16 {
     // a lane's pieces of its rows of Q
     struct Query {
         uint4 row[2][Math::Q_WORDS];
-        __device__ __forceinline__ void load(int i, const X* from, int lane) {
+        __device__ __forceinline__ void load(int i, const X* from, int lane, bool late) {
 #pragma unroll
-            for (int k = 0; k < Math::Q_WORDS; ++k) row[i][k] = from ? *reinterpret_cast<const uint4*>(from + Math::at_q(k, lane & 3)) : make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < Math::Q_WORDS; ++k) row[i][k] = from ? query_piece(from + Math::at_q(k, lane & 3), late) : make_uint4(0, 0, 0, 0);
         }
     };
     __device__ __forceinline__ void start(const Query& q, uint32_t flip) {
@@ -308,8 +312,8 @@ struct RowsOfOne {
     static __device__ __forceinline__ int row(int i, int) { return i; }
     struct Query {
         uint4 row[N];
-        __device__ __forceinline__ void load(int i, const X* from, int lane) {
-            row[i] = from ? *reinterpret_cast<const uint4*>(from + 4 * (lane & 15)) : make_uint4(0, 0, 0, 0);
+        __device__ __forceinline__ void load(int i, const X* from, int lane, bool late) {
+            row[i] = from ? query_piece(from + 4 * (lane & 15), late) : make_uint4(0, 0, 0, 0);
         }
     };
     __device__ __forceinline__ void start(const Query& from, uint32_t flip) {
@@ -421,7 +425,7 @@ __device__ __forceinline__ void few_job(const CUtensorMap& map_kp, const CUtenso
     const int ns = JOB == FEW_PREFIX ? a.splits_p : JOB == FEW_OWN ? a.splits_o : 1, item = block / ns, split = block - item * ns;
     const int tiles = OWN ? a.tiles_o : a.tiles_p, at = item / tiles, tile = item - at * tiles;
     const int b = OWN ? at / a.Hk : 0, kvh = at - b * a.Hk;
-    const int32_t all_keys = OWN && a.lengths ? __ldg(a.lengths + b) : a.S;
+    const int len = OWN ? request_keys(a, b) : 0;
     const int all = OWN ? a.T * a.group : a.R, row0 = b * a.T * a.group + tile * N, rows = min(N, all - tile * N);
     typename Rows::Query query;
     int token_of[MINE];
@@ -429,15 +433,14 @@ __device__ __forceinline__ void few_job(const CUtensorMap& map_kp, const CUtenso
     for (int i = 0; i < MINE; ++i) {
         const int r = Rows::row(i, lane), row = row0 + r, token = row / a.group, bq = OWN ? b : token / a.T;
         token_of[i] = r < rows ? token - bq * a.T : a.T;
-        query.load(i, r < rows ? row_of<X>(a.Q, bq, kvh * a.group + (row - token * a.group), token_of[i]) : nullptr, lane);
+        query.load(i, r < rows ? row_of<X>(a.Q, bq, kvh * a.group + (row - token * a.group), token_of[i]) : nullptr, lane, late);
     }
     // the keys: batches of the prefix, then of the request's own
-    int p_begin = 0, p_end = 0, o_begin = 0, o_end = 0, len = 0;
+    int p_begin = 0, p_end = 0, o_begin = 0, o_end = 0;
     if (JOB == FEW_PREFIX) {
         p_begin = split * a.per_p;
         p_end = min(a.P, p_begin + a.per_p);
     } else {
-        len = min(max(all_keys, 0), a.S);
         const int seen = token_keys(a, len, (tile * N + rows - 1) / a.group), per = ((seen + ns - 1) / ns + KEYS - 1) / KEYS * KEYS;
         o_begin = min(seen, split * per);
         o_end = min(seen, o_begin + per);

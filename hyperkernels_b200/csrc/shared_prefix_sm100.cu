@@ -151,7 +151,8 @@ prefix_many_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
         tmem_relinquish();
         tc_fence_before_sync();
     }
-    if (!args.late) pdl_wait();
+    if (args.late) __threadfence();
+    else pdl_wait();
     pdl_trigger();
     // the item: rows
     int item = blockIdx.x, split = 0, parts = 1;

@@ -467,6 +467,8 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
 // ended): its set-up then runs beside the predecessor's last CTAs.  pdl_wait returns when the predecessor is complete and
 // its writes are visible; nothing the predecessor may have written is read, and nothing at all written, before it.  A
 // kernel triggers only after its own pdl_wait, so that what precedes IT is complete too when its successor starts.
+// What a predecessor may have written is never read with __ldg: for the compiler that memory does not change while the kernel
+// runs, and it may move the load in front of the wait.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

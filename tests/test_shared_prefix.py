@@ -501,3 +501,39 @@ def test_blocks_that_are_refused(path, value, status):
     f.argtypes = [C.c_void_p, C.c_void_p]
     assert f(C.byref(b), None) == status
     assert f(None, None) == -1
+
+
+# ---- calls behind other launches -----------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,T,P,S,dtype", [
+    (4, 12, 12, 1, 333, 64, "f32"), (16, 12, 12, 1, 2047, 512, "f32"), (2, 1, 1, 1, 9001, 500, "f32"), (4, 12, 4, 1, 3000, 400, "f32"), (64, 32, 8, 1, 8192, 1000, "bf16"),
+    (64, 8, 2, 1, 515, 100, "f16"), (300, 4, 2, 1, 0, 400, "f16"), (16, 8, 2, 20, 2500, 300, "bf16"), (16, 4, 4, 77, 4097, 333, "f32"), (37, 4, 4, 100, 1, 160, "bf16")])
+@pytest.mark.parametrize("last", ["lengths", "queries"])
+def test_lengths_and_queries_written_by_the_launch_before(B, H, Hk, T, P, S, dtype, last):
+    """A decoding loop without a synchronisation: each step's queries and lengths come from the launches right before the call, in the
+    memory that the step before used.  Every step has the bits of the same call on inputs that were there long before."""
+    steps, t = 24, TYPES[dtype]
+    _, kp, vp, k, v, _ = make(B + T, B, H, Hk, T, P, S, dtype, lengths=[S] * B)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    rows = torch.randn((steps, B, H, T, 64), generator=g, device="cuda").to(t)
+    pos = torch.randint(0, 9000, (1, B, T), generator=g, device="cuda", dtype=torch.int32)
+    first = (torch.arange(B, device="cuda") % (S - T - steps) + T).to(torch.int32)
+    q, lens, got = torch.zeros((B, H, T, 64), device="cuda", dtype=t), first.clone(), []
+    torch.cuda.synchronize()
+    torch.cuda._sleep(20_000_000)  # all steps are in the queue before the first one runs
+    for i in range(steps):
+        if last == "queries":
+            lens.add_(1)
+        hk.rotary_forward(rows[i], None, pos, (32,), out_q=q)
+        if last == "lengths":
+            lens.add_(1)
+        got.append(hk.shared_prefix_attention(q, kp, vp, k, v, lens, SCALE))
+    torch.cuda.synchronize()
+    for i, (o, lse) in enumerate(got):
+        q, lens = hk.rotary_forward(rows[i], None, pos, (32,))[0], first + (i + 1)
+        torch.cuda.synchronize()
+        O, LSE = hk.shared_prefix_attention(q, kp, vp, k, v, lens, SCALE)
+        torch.cuda.synchronize()
+        assert torch.equal(o, O) and torch.equal(lse, LSE), i
+    check((O, LSE), definition(q, kp, vp, k, v, lens, True), dtype)
+    assert hk.last_device_status() == 0
