@@ -551,8 +551,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
 #pragma unroll
                 for (int u = 0; u < TILE / 32; ++u) {
                     const int q = (s.x.it0 + it) * TILE + 32 * u + lane;
-                    l[u] = q < a.Tq ? __ldg(lse_bh + q) : -INFINITY;
-                    d[u] = q < a.Tq ? __ldg(d_bh + q) : 0.f;
+                    l[u] = q < a.Tq ? lse_bh[q] : -INFINITY;
+                    d[u] = q < a.Tq ? d_bh[q] : 0.f;
                 }
             };
             pdl_wait();  // D
@@ -678,7 +678,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
 #pragma unroll 4
                         for (int i = 0; i < 32; ++i) {
                             const int q = q0 + c0 + i;
-                            if (q < a.Tq && __ldg(a.mask + ((size_t)bh * a.Tq + q) * (size_t)a.Tk + kvrow) != 0.f)
+                            if (q < a.Tq && a.mask[((size_t)bh * a.Tq + q) * (size_t)a.Tk + kvrow] != 0.f)
                                 keep |= 1u << i;
                         }
                     }

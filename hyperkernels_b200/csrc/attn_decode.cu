@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(WARPS * 32, (NQ == 1 ? 24 : 16) / WARPS) attn_
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
         const int row = min(i, a.Tq - 1);
-        q[i] = __ldg(reinterpret_cast<const float4*>(a.Q.ptr + (int64_t)b * a.Q.sB + (int64_t)h * a.Q.sH + row * a.Q.sM) + sub);
+        q[i] = reinterpret_cast<const float4*>(a.Q.ptr + (int64_t)b * a.Q.sB + (int64_t)h * a.Q.sH + row * a.Q.sM)[sub];
         q[i].x *= a.scale_log2e; q[i].y *= a.scale_log2e; q[i].z *= a.scale_log2e; q[i].w *= a.scale_log2e;
         o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         m[i] = -INFINITY;

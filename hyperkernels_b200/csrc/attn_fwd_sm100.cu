@@ -718,7 +718,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
                         for (int i = 0; i < 128; ++i) {
                             float p = ex2_approx(fmaf(__uint_as_float(r[i]), cs, neg_m));
                             if (scaled) s2 += (i <= lim_local) ? p : 0.f;
-                            p = (i <= lim_local) ? p * __ldg(mrow + i) : 0.f;
+                            p = (i <= lim_local) ? p * mrow[i] : 0.f;
                             s0 += p;
                             r[i] = tf32_round_bits_mma(__float_as_uint(p));
                         }

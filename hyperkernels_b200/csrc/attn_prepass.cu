@@ -70,8 +70,8 @@ __global__ void __launch_bounds__(256) precompute_D_kernel(const DJob j, uint32_
     for (int u = 0; u < 4; ++u) {
         const uint32_t row = min(row0 + 16 * u, nrows - 1);  // rows past the end are computed and not stored
         p[u] = row_pos(row, j.T, j.H);
-        g[u] = __ldg(reinterpret_cast<const float4*>(j.dO.ptr + row_off(p[u], j.dO.sB, j.dO.sM, j.dO.sH)) + sub);
-        o[u] = __ldg(reinterpret_cast<const float4*>(j.O.ptr + row_off(p[u], j.O.sB, j.O.sM, j.O.sH)) + sub);
+        g[u] = reinterpret_cast<const float4*>(j.dO.ptr + row_off(p[u], j.dO.sB, j.dO.sM, j.dO.sH))[sub];
+        o[u] = reinterpret_cast<const float4*>(j.O.ptr + row_off(p[u], j.O.sB, j.O.sM, j.O.sH))[sub];
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {

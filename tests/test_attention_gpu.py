@@ -915,3 +915,55 @@ def test_query_splits_of_few_key_tiles(BH, Tq, Tk, causal):
         hk.attention_backward(*args, k_pos0=kp, dK=dK2, dV=dV2, accum_dkdv=True, **kw)
         ok_status()
         assert torch.equal(dK2, dK + dK) and torch.equal(dV2, dV + dV)
+
+
+# ---- calls behind other launches ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("Tq,Tk,what", [(1, 2047, "Q"), (2, 700, "Q"), (1, 2047, "rotated Q"), (200, 200, "dO"), (300, 170, "dO"), (200, 200, "mask"), (130, 260, "LSE"),
+                                        (700, 700, "D"), (200, 200, "Q")])
+def test_rows_written_by_the_launch_before(Tq, Tk, what):
+    """Calls without a synchronisation, each behind the launch that writes one of its inputs into the memory the step before
+    used: the bits of the same call on inputs that were there long before."""
+    steps, B, H, causal = 16, 4, 6, Tq == Tk
+    g = torch.Generator(device="cuda").manual_seed(Tq + Tk)
+    rand = lambda *shape: torch.randn(shape, generator=g, device="cuda")  # noqa: E731
+    Q, dO, K, V = rand(B, H, Tq, 64), rand(B, H, Tq, 64), rand(B, H, Tk, 64), rand(B, H, Tk, 64)
+    O, LSE = hk.attention_forward(Q, K, V, SCALE, causal)
+    x = {"Q": Q, "rotated Q": Q, "dO": dO, "LSE": LSE, "D": (dO * O).sum(-1), "mask": torch.ones(B * H, Tq, Tk, device="cuda")}
+    given = x[what]
+    new = rand(steps, *given.shape)
+    if what == "mask":
+        new = (new > -1.0).float()
+    elif what in ("LSE", "D"):
+        new = given + 0.3 * new
+    pos = torch.arange(Tq, device="cuda", dtype=torch.int32).expand(1, B, Tq)
+
+    def write(i):
+        if what == "rotated Q":
+            hk.rotary_forward(new[i], None, pos, (32,), out_q=Q)
+        else:
+            given.copy_(new[i])
+
+    def call():
+        drop = dict(dropout_p=0.1, dropout_mask=given) if what == "mask" else {}
+        r = []
+        if what in ("Q", "rotated Q", "mask"):
+            r += hk.attention_forward(Q, K, V, SCALE, causal, **drop)
+        if what not in ("Q", "rotated Q"):
+            d = dict(D=given, d_precomputed=True) if what == "D" else {}
+            r += hk.attention_backward(Q, K, V, O, dO, LSE, SCALE, causal, deterministic_dq=True, **d, **drop)[:3]
+        return r
+
+    torch.cuda.synchronize()
+    torch.cuda._sleep(20_000_000)  # all steps are in the queue before the first one runs
+    got = []
+    for i in range(steps):
+        write(i)
+        got.append(call())
+    torch.cuda.synchronize()
+    for i in range(steps):
+        write(i)
+        torch.cuda.synchronize()
+        want = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want)), i
+    assert hk.last_device_status() == 0
