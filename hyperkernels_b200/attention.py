@@ -233,6 +233,8 @@ def attention_forward(Q, K, V, scale: float, causal: bool, *, dropout_p: float =
                       round_in_hbm: bool = False, workspace=None, out=None, lse=None, stream=None):
     """O, LSE = fused attention forward of [B,H,Tq,64] Q against [B,H,Tk,64] K, V (fp32 CUDA tensors).
 
+    A tensor of another type, or one that is smaller than Q and K say, is refused (AssertionError).  Every head of Q has its
+    own of K and V: heads that a group shares are repeated first.
     With Tk <= 4096 and Tk < 2 Tq a (batch, head) slice gives the same bits in any batch; otherwise (long sequences,
     chunks against a cache, decoding) they may change with B * H, by the rounding of sums in another order."""
     flags = 0
@@ -261,7 +263,7 @@ def attention_backward(Q, K, V, O, dO, LSE, scale: float, causal: bool, *, dropo
                        accum_dq: bool = False, reuse_fwd_rounded: bool = False, dropout_scaled: bool = False,
                        round_in_hbm: bool = False, deterministic_dq: bool = False, workspace=None, dQ=None, dK=None, dV=None,
                        stream=None):
-    """dQ, dK, dV, D = fused attention backward (fp32 CUDA tensors, [B,H,T,64]).
+    """dQ, dK, dV, D = fused attention backward (fp32 CUDA tensors, [B,H,T,64]; others are refused as in attention_forward).
 
     With Tq < 2 Tk a (batch, head) slice gives the same dK and dV in any batch (dQ: deterministic_dq); otherwise they may
     change with B * H, by the rounding of sums in another order."""

@@ -63,6 +63,29 @@ bool tensors(std::initializer_list<TensorArg> args) {
     return true;
 }
 
+bool refuse(const char* name, const char* what) {
+    PyErr_Format(PyExc_AssertionError, "%s: %s", name, what);
+    return false;
+}
+
+// Whether the attention kernels, which take every tensor for fp32 of the sizes that Q and K give, stay inside this one: of that type,
+// and no smaller.  rows: [B, H, T, 64], whose strides have been looked at; otherwise [B, H, T], a number to a row.
+// False with AssertionError set.
+bool holds(const at::Tensor& t, const char* name, int64_t B, int64_t H, int64_t T, bool rows = true) {
+    if (t.scalar_type() != at::kFloat) return refuse(name, "expected float32");
+    const at::IntArrayRef size = t.sizes();
+    if (!rows && (size.size() < 3 || (T > 1 && t.stride(2) != 1))) return refuse(name, "expected [B,H,T] with unit last stride");
+    if (size[0] < B || size[1] < H || size[2] < T) return refuse(name, "smaller than the other tensors");
+    return true;
+}
+// The same for a dense dropout mask, which is read as [B * H, Tq, Tk] without gaps where the call drops anything by it.
+bool mask_holds(const at::Tensor* mask, float p, uint32_t flags, int64_t B, int64_t H, int64_t Tq, int64_t Tk) {
+    if (!mask || !(p > 0.f) || (flags & HK_FLAG_PHILOX_DROPOUT)) return true;
+    if (mask->scalar_type() != at::kFloat || !mask->is_contiguous()) return refuse("dropout_mask", "expected float32, contiguous");
+    if ((double)mask->numel() < (double)B * H * Tq * Tk) return refuse("dropout_mask", "smaller than the other tensors");
+    return true;
+}
+
 // strides of a [B, H, T, 64] view into the block's (B, M, H) triple; false with AssertionError set
 bool strides(const at::Tensor& t, int64_t* sB, int64_t* sM, int64_t* sH) {
     if (t.dim() != 4 || t.size(3) != 64 || t.stride(3) != 1) {
@@ -156,6 +179,9 @@ static PyObject* forward_body(PyObject* const* a, Py_ssize_t n) {
     p.flags = (uint32_t)PyLong_AsUnsignedLongLongMask(a[12]);
     void* stream = stream_of(a[16]);
     if (PyErr_Occurred()) return nullptr;
+    if (!holds(*Q, "Q", B, H, Tq) || !holds(*K, "K", B, H, Tk) || !holds(*V, "V", B, H, Tk) || !holds(O, "out", B, H, Tq) ||
+        !holds(L, "lse", B, H, Tq, false) || !mask_holds(mask, p.dropout_p, p.flags, B, H, Tq, Tk))
+        return nullptr;
     if (ws && !given_workspace(ws, g_lib.fwd_bytes(&p), &p.workspace, &p.workspace_bytes)) return nullptr;
     int rc;
     {
@@ -237,6 +263,10 @@ static PyObject* backward_body(PyObject* const* a, Py_ssize_t n) {
     p.k_pos0 = PyLong_AsLongLong(a[13]);
     p.bh_pos0 = (uint32_t)PyLong_AsUnsignedLongLongMask(a[14]);
     if (PyErr_Occurred()) return nullptr;
+    if (!holds(*Q, "Q", B, H, Tq) || !holds(*K, "K", B, H, Tk) || !holds(*V, "V", B, H, Tk) || (O && !holds(*O, "O", B, H, Tq)) ||
+        !holds(*dO, "dO", B, H, Tq) || !holds(*LSE, "LSE", B, H, Tq, false) || !holds(r[0], "dQ", B, H, Tq) || !holds(r[1], "dK", B, H, Tk) ||
+        !holds(r[2], "dV", B, H, Tk) || !holds(r[3], "D", B, H, Tq, false) || !mask_holds(mask, p.dropout_p, p.flags, B, H, Tq, Tk))
+        return nullptr;
     int rc;
     {
         NoGil nogil;
@@ -263,16 +293,13 @@ static PyObject* zero_body(PyObject* const* a, Py_ssize_t n) {
     p.dQ = data(*x);
     void* stream = stream_of(a[1]);
     if (PyErr_Occurred()) return nullptr;
+    if (!holds(*x, "dQ", 0, 0, 0)) return nullptr;
     return PyLong_FromLong(g_lib.zero_dq(&p, stream));
 }
 
 // ---- the operators round the attention: tensors of three types, on one device, checked against each other -------------------
 namespace {
 
-bool refuse(const char* name, const char* what) {
-    PyErr_Format(PyExc_AssertionError, "%s: %s", name, what);
-    return false;
-}
 int dtype_code(const at::Tensor& t) {
     return t.scalar_type() == at::kFloat ? HK_F32 : t.scalar_type() == at::kBFloat16 ? HK_BF16 : t.scalar_type() == at::kHalf ? HK_F16 : -1;
 }

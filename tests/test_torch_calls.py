@@ -158,3 +158,50 @@ def test_slabs_under_the_streams_that_have_no_object(handle):
     torch.cuda.synchronize()
     assert hk.last_device_status() == 0
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- what the kernels would read or write past its end -------------------------------------------------------------------
+def _attention_arguments(call):
+    x, kv, l = torch.zeros(2, 3, 5, 64), torch.zeros(2, 3, 9, 64), torch.zeros(2, 3, 5)
+    args = dict(Q=x, K=kv, V=kv, scale=0.125, causal=True, dropout_p=0.1, dropout_mask=torch.ones(6, 5, 9), stream=0)
+    return dict(args, out=x, lse=l) if call == "attention_forward" else dict(args, O=x, dO=x, LSE=l, D=l, dQ=x, dK=kv, dV=kv)
+
+
+_LIKE_Q, _LIKE_K, _LIKE_L = ("Q", "out", "O", "dO", "dQ"), ("K", "V", "dK", "dV"), ("lse", "LSE", "D")
+_WRONG = [(n, torch.zeros(2, 3, t, 64, dtype=d)) for names, t in ((_LIKE_Q, 5), (_LIKE_K, 9)) for n in names for d in (torch.bfloat16, torch.float16, torch.float64)]
+_WRONG += [(n, torch.zeros(*s, 64)) for n in _LIKE_Q[1:] for s in ((1, 3, 5), (2, 1, 5), (2, 2, 5), (2, 3, 4))]
+_WRONG += [(n, torch.zeros(*s, 64)) for n in _LIKE_K for s in ((1, 3, 9), (2, 1, 9), (2, 2, 9))]  # a group's shared heads among them
+_WRONG += [(n, torch.zeros(2, 3, 8, 64)) for n in _LIKE_K[1:]]
+_WRONG += [(n, x) for n in _LIKE_L for x in (torch.zeros(2, 3, 5, dtype=torch.bfloat16), torch.zeros(1, 3, 5), torch.zeros(2, 2, 5), torch.zeros(2, 3, 4), torch.zeros(6, 5),
+                                             torch.zeros(2, 3, 10)[..., ::2])]
+_WRONG += [("dropout_mask", x) for x in (torch.ones(6, 5, 9, dtype=torch.bool), torch.ones(6, 5, 8), torch.ones(6, 9, 5).transpose(1, 2), torch.ones(1, 5, 9).expand(6, 5, 9))]
+
+
+@pytest.mark.parametrize("call,name,wrong", [(c, n, x) for c in ("attention_forward", "attention_backward") for n, x in _WRONG if n in _attention_arguments(c)])
+def test_tensors_that_the_kernels_would_leave_are_refused(call, name, wrong):
+    """Half-precision rows or shared key heads, as the operators round the attention give them, read as fp32 of Q's heads."""
+    import hyperkernels_b200 as hk
+
+    with pytest.raises(AssertionError, match=f"^{name}: "):
+        getattr(hk, call)(**{**_attention_arguments(call), name: wrong})
+
+
+def test_zero_dq_refuses_what_is_not_fp32():
+    import hyperkernels_b200.attention as att
+
+    with pytest.raises(AssertionError, match="^dQ: expected float32"):
+        att.zero_dq(torch.zeros(1, 2, 5, 64, dtype=torch.bfloat16), 0)
+
+
+def test_larger_tensors_and_masks_without_use_are_taken():
+    """Room behind the rows, as before; a mask is looked at where the call drops anything by it.  (dropout_p = 1 and a mask beside a seed are
+    refused by the library, behind these checks and in front of any launch.)"""
+    import hyperkernels_b200 as hk
+
+    room, rows = torch.zeros(3, 4, 9, 64), torch.zeros(3, 4, 9, 1)
+    for call, more in (("attention_forward", dict(out=room, lse=rows[..., 0])), ("attention_backward", dict(O=room, dO=room, LSE=rows, D=rows, dQ=room, dK=room, dV=room))):
+        args = {**_attention_arguments(call), **more, "V": torch.zeros(3, 3, 12, 64), "dropout_p": 1.0}
+        with pytest.raises(hk.HKError, match="dropout"):
+            getattr(hk, call)(**args)
+        with pytest.raises(hk.HKError, match="dropout"):
+            getattr(hk, call)(**{**args, "dropout_p": 0.5, "philox_seed": 3, "dropout_mask": torch.ones(1)})
