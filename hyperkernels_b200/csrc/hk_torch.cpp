@@ -128,7 +128,8 @@ bool given_workspace(const at::Tensor* t, size_t need, void** ptr, size_t* bytes
     if (!t) return true;
     uint8_t* base = static_cast<uint8_t*>(t->data_ptr());
     const size_t off = (256 - (reinterpret_cast<uintptr_t>(base) & 255u)) & 255u;
-    const size_t have = (size_t)t->numel();
+    const size_t have = t->nbytes();  // of its elements, whatever type they have
+    if (need > 0 && !t->is_contiguous()) return refuse("workspace", "expected contiguous memory");  // an expanded one has less than that
     if (need > 0 && have < off + need) {
         PyErr_SetString(PyExc_AssertionError, "workspace too small");
         return false;

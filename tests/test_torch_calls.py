@@ -205,3 +205,22 @@ def test_larger_tensors_and_masks_without_use_are_taken():
             getattr(hk, call)(**args)
         with pytest.raises(hk.HKError, match="dropout"):
             getattr(hk, call)(**{**args, "dropout_p": 0.5, "philox_seed": 3, "dropout_mask": torch.ones(1)})
+
+
+@pytest.mark.parametrize("call", ["attention_forward", "attention_backward"])
+def test_a_workspace_is_as_large_as_its_memory(call):
+    """An expanded tensor has less memory than elements, one of a wider type more bytes than elements.  Those that are large enough get as
+    far as the library, which refuses dropout_p = 1 in front of any launch."""
+    import hyperkernels_b200 as hk
+
+    x, l = torch.zeros(1, 2, 64, 64), torch.zeros(1, 2, 64)
+    args = dict(Q=x, K=x, V=x, scale=0.125, causal=True, round_in_hbm=True, dropout_p=1.0, stream=0)
+    args.update({} if call == "attention_forward" else dict(O=x, dO=x, LSE=l))
+    need = 6 * 64 * 256 if call == "attention_forward" else 8 * 64 * 256
+    for wrong, why in ((torch.zeros(1, dtype=torch.uint8).expand(1 << 20), "contiguous"), (torch.zeros(1 << 20, 2, dtype=torch.uint8)[:, 0], "contiguous"),
+                       (torch.zeros(need - 1, dtype=torch.uint8), "too small"), (torch.zeros(need // 4 - 1), "too small"), (torch.zeros(0), "too small")):
+        with pytest.raises(AssertionError, match=why):
+            getattr(hk, call)(**args, workspace=wrong)
+    for enough in (torch.zeros(need + 256, dtype=torch.uint8), torch.zeros(need // 4 + 64), torch.zeros(need // 512 + 1, 64, dtype=torch.float64)):
+        with pytest.raises(hk.HKError, match="dropout"):
+            getattr(hk, call)(**args, workspace=enough)
