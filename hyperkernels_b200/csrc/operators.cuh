@@ -37,17 +37,32 @@ __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
 
 inline int esize(int dtype) { return dtype == HK_F32 ? 4 : 2; }
 
+// Whether stretches of `row` elements at all places of these dimensions lie apart: from the smallest stride on, each step goes past
+// all that the dimensions before it reach.  (Dimensions that interleave without meeting are not recognised; no slice or transposition
+// of a tensor has such.)
+struct Dim {
+    int64_t n, stride;
+};
+template <int N>
+bool lie_apart(Dim (&d)[N], int64_t row) {
+    std::sort(d, d + N, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+    __int128 reach = row;
+    for (const Dim& x : d) {
+        if (x.n <= 1) continue;
+        if (x.stride < reach) return false;
+        reach += (__int128)(x.n - 1) * x.stride;
+    }
+    return true;
+}
+
 // A view of `n` heads whose rows the kernels read or write in pieces of up to 16 bytes.
 inline int check_view(const hk_view& v, int64_t B, int64_t n, int64_t T, int dtype, bool written) {
     if (!v.ptr) return HK_ERR_NULL_POINTER;
     if (reinterpret_cast<uintptr_t>(v.ptr) & 15u) return HK_ERR_MISALIGNED;
-    const int64_t s[] = {v.strideB, v.strideM, v.strideH}, d[] = {B, T, n};
-    for (int i = 0; i < 3; ++i) {
-        if (d[i] <= 1) continue;
-        if (s[i] < 0 || (s[i] * esize(dtype)) % 16) return HK_ERR_MISALIGNED;
-        if (written && s[i] < HEAD_DIM) return HK_ERR_UNSUPPORTED;  // rows on top of each other
-    }
-    return HK_OK;
+    Dim d[] = {{B, v.strideB}, {T, v.strideM}, {n, v.strideH}};
+    for (const Dim& x : d)
+        if (x.n > 1 && (x.stride < 0 || x.stride % (16 / esize(dtype)))) return HK_ERR_MISALIGNED;
+    return written && !lie_apart(d, HEAD_DIM) ? HK_ERR_UNSUPPORTED : HK_OK;  // rows on top of each other
 }
 
 }  // namespace hk

@@ -455,6 +455,7 @@ int qk_run(const hk_qk_params* p, int mode, bool back, cudaStream_t stream) {
         if ((reinterpret_cast<uintptr_t>(p->dq_weight) | reinterpret_cast<uintptr_t>(p->dk_weight)) & 3u) return HK_ERR_MISALIGNED;
         a.partial = static_cast<float*>(p->workspace);
     }
+    if (p->nh_k > 0 && dst[0]->ptr == dst[1]->ptr) return HK_ERR_UNSUPPORTED;  // queries' and keys' results in the same place
     a.positions = p->positions;
     a.pA = p->pos_strideA; a.pB = p->pos_strideB; a.pT = p->pos_strideT;
     a.heads[0] = p->nh; a.heads[1] = p->nh_k;

@@ -97,7 +97,8 @@ int check(const hk_shared_prefix_params* p) {
     };
     if ((rc = keys(p->Kp, 1, p->prefix_len)) || (rc = keys(p->Vp, 1, p->prefix_len)) || (rc = keys(p->K, p->B, p->kv_len)) || (rc = keys(p->V, p->B, p->kv_len))) return rc;
     if (!p->LSE) return HK_ERR_NULL_POINTER;
-    if ((p->B > 1 && p->lse_strideB < p->T) || (p->nh > 1 && p->lse_strideH < p->T)) return HK_ERR_UNSUPPORTED;  // rows on top of each other
+    Dim lse[] = {{p->B, p->lse_strideB}, {p->nh, p->lse_strideH}};
+    if (!lie_apart(lse, p->T)) return HK_ERR_UNSUPPORTED;  // rows on top of each other
     if ((reinterpret_cast<uintptr_t>(p->LSE) | reinterpret_cast<uintptr_t>(p->lengths)) & 3u) return HK_ERR_MISALIGNED;
     return HK_OK;
 }

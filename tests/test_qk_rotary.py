@@ -470,3 +470,32 @@ def test_small_results_are_tensors_of_their_own():
     huge = torch.zeros((1, 1, 1, 64), device="cuda").expand(1 << 20, 1 << 10, 1 << 20, 64)  # 2^58 bytes
     with pytest.raises((hk.HKError, RuntimeError)):
         hk.rotary_forward(huge, None, pos[:, :1, :1].expand(1, 1 << 20, 1 << 20), (32,))
+
+
+# ---- results that lie on top of each other: B = 2, 3 heads of queries, 1 of keys, 5 tokens -------------------------------------------
+@pytest.mark.parametrize("call,view", [("rotary_forward", "q_out"), ("rotary_backward", "dq"), ("qk_norm_rotary_forward", "q_out"), ("qk_norm_rotary_backward", "dq")])
+@pytest.mark.parametrize("strides", [(64, 64, 64), (320, 320, 320), (960, 64, 64), (960, 128, 64), (640, 64, 256), (256, 64, 640), (64, 64, 1 << 40)])
+def test_results_on_top_of_each_other_are_refused(call, view, strides):
+    b = _block()
+    v = getattr(b, view)
+    v.sB, v.sM, v.sH = strides
+    b.k_out.ptr = b.dk.ptr = 0x100000
+    f = getattr(hk.lib(), "hk_" + call)
+    f.argtypes = [C.c_void_p, C.c_void_p]
+    assert f(C.byref(b), None) == -6
+
+
+def test_results_that_lie_apart_get_past_that():
+    f = hk.lib().hk_qk_norm_rotary_backward
+    f.argtypes = [C.c_void_p, C.c_void_p]
+    for strides in ((960, 64, 320), (960, 192, 64), (64, 384, 128), (320, 64, 640), (1 << 60, 1 << 40, 1 << 50)):
+        b = _block()
+        b.dq.sB, b.dq.sM, b.dq.sH = strides
+        b.dk.ptr, b.workspace = 0x100000, None
+        assert f(C.byref(b), None) == -5, strides
+    for call, q, k in (("rotary_forward", "q_out", "k_out"), ("rotary_backward", "dq", "dk"), ("qk_norm_rotary_forward", "q_out", "k_out"), ("qk_norm_rotary_backward", "dq", "dk")):
+        b = _block()  # the same memory for both
+        assert getattr(b, q).ptr == getattr(b, k).ptr
+        f = getattr(hk.lib(), "hk_" + call)
+        f.argtypes = [C.c_void_p, C.c_void_p]
+        assert f(C.byref(b), None) == -6

@@ -537,3 +537,41 @@ def test_lengths_and_queries_written_by_the_launch_before(B, H, Hk, T, P, S, dty
         assert torch.equal(o, O) and torch.equal(lse, LSE), i
     check((O, LSE), definition(q, kp, vp, k, v, lens, True), dtype)
     assert hk.last_device_status() == 0
+
+
+# ---- results that lie on top of each other: B = 2, 4 heads, 3 tokens ----------------------------------------------------------------
+@pytest.mark.parametrize("o", [(64, 64, 64), (64, 256, 64), (192, 192, 384), (256, 64, 128), (768, 64, 128), (384, 64, 192), (512, 256, 64), (128, 256, 64), (192, 768, 384), (64, 64, 1 << 40)])
+def test_rows_of_o_on_top_of_each_other_are_refused(o):
+    b = _block()
+    b.O.sB, b.O.sM, b.O.sH = o
+    f = hk.lib().hk_shared_prefix_attention
+    f.argtypes = [C.c_void_p, C.c_void_p]
+    assert f(C.byref(b), None) == -6
+
+
+@pytest.mark.parametrize("sB,sH", [(3, 3), (3, 5), (4, 4), (100, 100), (11, 3), (4, 6), (1 << 40, 2)])
+def test_rows_of_lse_on_top_of_each_other_are_refused(sB, sH):
+    b = _block()
+    b.lse_sB, b.lse_sH = sB, sH
+    f = hk.lib().hk_shared_prefix_attention
+    f.argtypes = [C.c_void_p, C.c_void_p]
+    assert f(C.byref(b), None) == -6
+
+
+def test_results_that_lie_apart_get_past_that():
+    """In any order of dimensions, with room between, however far: what is refused is the check behind it."""
+    f = hk.lib().hk_shared_prefix_attention
+    f.argtypes = [C.c_void_p, C.c_void_p]
+    for o in ((768, 64, 192), (768, 256, 64), (192, 384 * 4, 384), (64, 512, 128), (64, 128, 384), (880, 72, 224), (1 << 50, 1 << 40, 1 << 30), (1 << 62, 1 << 60, 1 << 58)):
+        b = _block()
+        b.O.sB, b.O.sM, b.O.sH = o
+        b.LSE = None
+        assert f(C.byref(b), None) == -1, o
+    for sB, sH in ((12, 3), (3, 6), (4, 7), (3, 11), (1 << 60, 1 << 50)):
+        b = _block()
+        b.lse_sB, b.lse_sH, b.LSE = sB, sH, 0x1002
+        assert f(C.byref(b), None) == -3, (sB, sH)
+    b = _block()  # strides of dimensions of one are not used
+    b.B, b.nh, b.nh_kv, b.T, b.lse_sB, b.lse_sH, b.LSE = 1, 1, 1, 1, 0, 0, 0x1002
+    b.O.sB = b.O.sM = b.O.sH = 0
+    assert f(C.byref(b), None) == -3
