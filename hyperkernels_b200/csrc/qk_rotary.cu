@@ -531,10 +531,12 @@ int hk_rotary_plan_fill(hk_rotary_plan* plan, int n_axes, const int* sections, d
     for (int a = 0; a < n_axes; ++a) {
         if (sections[a] < 0 || sections[a] > 32 - n) return HK_ERR_BAD_SHAPE;
         for (int i = 0; i < sections[a]; ++i, ++n) {
-            const double f = frequency ? frequency[n] : std::pow(base, -n / 32.0);
+            // 64 bits of significand up to the rounding of the fraction: the 53 of a power in double would be 2^-57 of a turn off, and the
+            // position multiplies that
+            const long double f = frequency ? (long double)frequency[n] : std::pow((long double)base, -n / 32.0L);
             if (!std::isfinite(f)) return HK_ERR_BAD_SHAPE;
             // turns per position without whole ones, which an integer position turns into whole turns again
-            const long double turns = (long double)f / 6.283185307179586476925286766559005768L;
+            const long double turns = f / 6.283185307179586476925286766559005768L;
             const long double part = turns - std::floor(turns);
             const long double scaled = std::nearbyint(std::ldexp(part, 64));
             r.turn[n] = scaled >= 18446744073709551616.0L ? 0u : (uint64_t)scaled;

@@ -71,7 +71,7 @@ def rotary_forward(Q, K, positions, sections, *, base: float = 10000.0, frequenc
     ``positions``: [axes, B, T] of int32 or int64, any strides (expanded ones too).  ``sections``: how many of a row's 32 pairs
     turn with each axis, in order; pairs behind the last section are left as they are.  Pair p of all is elements (p, p + 32), or
     (2 p, 2 p + 1) with ``interleaved``, and turns by ``base ** (-p / 32)`` radians per position, or by ``frequencies[p]``.  The
-    angle of an integer position has no rounding error that grows with the position.
+    turns per position are rounded once, to 2^-64 of a turn; their product with an integer position is exact, modulo a turn.
     ``K`` may be None.  Results are new tensors of ``out_dtype`` (default: Q's type), or ``out_q`` / ``out_k``, which may be Q
     and K themselves.  A 16-bit type becomes float32 (what ``attention_forward`` reads) or stays; float32 becomes any."""
     return _qk(0, "hk_rotary_forward", Q, K, None, None, None, None, positions, sections, base, frequencies, interleaved, 0.0,

@@ -499,3 +499,21 @@ def test_results_that_lie_apart_get_past_that():
         f = getattr(hk.lib(), "hk_" + call)
         f.argtypes = [C.c_void_p, C.c_void_p]
         assert f(C.byref(b), None) == -6
+
+
+@pytest.mark.parametrize("base", [1.0, 100.0, 10000.0, 500000.0, 2.5e6, 1e30, 0.5, 1e-3])
+@pytest.mark.parametrize("given", [False, True])
+def test_fractions_of_a_turn_to_the_last_bits(base, given):
+    """Against 50 decimal digits.  Numbers of 64 bits: the power is a step off (2^-63 of itself), 2 pi and the quotient half of one each, and
+    the fraction is rounded to 2^-64: half a unit of that and four for every turn per position."""
+    import decimal
+
+    with decimal.localcontext() as c:
+        c.prec = 50
+        two_pi = 2 * decimal.Decimal("3.14159265358979323846264338327950288419716939937511")
+        exact = [(decimal.Decimal(base).ln() * -p / 32).exp() for p in range(32)]
+        plan = hk.rotary_plan((32,), frequencies=[float(x) for x in exact]) if given else hk.rotary_plan((32,), base=base)
+        for p in range(32):
+            turns = (decimal.Decimal(float(exact[p])) if given else exact[p]) / two_pi
+            off = abs(plan.turn[p] - turns * 2 ** 64) % 2 ** 64
+            assert min(off, 2 ** 64 - off) <= decimal.Decimal(0.5) + 4 * turns, p
