@@ -336,42 +336,13 @@ bool one_device(std::initializer_list<const at::Tensor*> all) {
 }
 
 // A tensor that a kernel is about to fill, without the way through the dispatcher, which takes as long again as the allocation;
-// torch's own switch that fills such tensors is heard.
+// torch's own switch that fills such tensors is heard.  Each result has memory of its own: two in one allocation would take 0.4 us
+// less, but who keeps or writes out one of them would have both.
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
     if (at::globalContext().deterministicAlgorithms() && at::globalContext().deterministicFillUninitializedMemory())
         return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
     return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
-
-// The results of a call.  Those of up to 256 KB lie in one allocation, as tensors of their own: two results of one token of 16 requests
-// take 1.2 us instead of 1.6, of 5.2 that the call takes from Python.  Larger ones are worth their own, so that one that is kept does
-// not keep the others' memory.
-struct Results {
-    static constexpr int64_t SMALL = 256 << 10, ALIGN = 512;
-    const at::Device device;
-    at::Tensor all;
-    int64_t at = 0;
-    static int64_t bytes_of(at::IntArrayRef sizes, int64_t each) {  // of views with strides of 0 there may be more than a number holds
-        int64_t n = each;
-        for (int64_t s : sizes) n = s > 0 && n > SMALL / s ? SMALL + 1 : n * s;
-        return n;
-    }
-    static int64_t room(int64_t bytes) { return bytes <= SMALL ? (bytes + ALIGN - 1) / ALIGN * ALIGN : 0; }
-    Results(const at::Device& device, std::initializer_list<int64_t> bytes) : device(device) {
-        int64_t sum = 0;
-        for (int64_t b : bytes) sum += room(b);
-        if (sum > 0) all = fresh({sum}, at::kByte, device);
-    }
-    at::Tensor take(at::IntArrayRef sizes, at::ScalarType type) {
-        const int64_t each = (int64_t)at::elementSize(type), bytes = bytes_of(sizes, each);
-        if (room(bytes) == 0) return fresh(sizes, type, device);
-        at::Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
-        r.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-        r.unsafeGetTensorImpl()->set_storage_offset(at / each);
-        at += room(bytes);
-        return r;
-    }
-};
 
 // Makes the tensors' device the current one and the stream asked for (None: that device's current one) the one that
 // results and workspaces are allocated for: they are written there, whatever becomes of them here.
@@ -476,19 +447,16 @@ static PyObject* qk_body(PyObject* const* a, Py_ssize_t n) {
 
     const at::Device device = src[0]->device();
     at::Tensor r[2], dw[2], ws;
-    auto rows_of = [&](int64_t heads) { return Results::bytes_of({B, heads, T, 64}, out_type == HK_F32 ? 4 : 2); };
-    auto weights = [&](int k) { return which == 3 && w[k] && src[k]; };
-    Results results(device, {out[0] ? 0 : rows_of(H), out[1] || !src[1] ? 0 : rows_of(Hk), weights(0) ? 256 : 0, weights(1) ? 256 : 0});
     for (int k = 0; k < 2; ++k) {
         if (!src[k]) continue;
-        r[k] = out[k] ? *out[k] : results.take({B, k ? Hk : H, T, 64}, scalar_of(out_type));
+        r[k] = out[k] ? *out[k] : fresh({B, k ? Hk : H, T, 64}, scalar_of(out_type), device);
         *dst_view[k] = {r[k].data_ptr(), r[k].stride(0), r[k].stride(2), r[k].stride(1)};
     }
     p.q_weight = norm && w[0] ? w[0]->data_ptr() : nullptr;
     p.k_weight = norm && w[1] ? w[1]->data_ptr() : nullptr;
     if (which == 3) {
         for (int k = 0; k < 2; ++k)
-            if (weights(k)) dw[k] = results.take({64}, at::kFloat);
+            if (w[k] && src[k]) dw[k] = fresh({64}, at::kFloat, device);
         p.dq_weight = dw[0].defined() ? data(dw[0]) : nullptr;
         p.dk_weight = dw[1].defined() ? data(dw[1]) : nullptr;
         p.workspace_bytes = g_lib.qk_bytes(&p);
@@ -540,8 +508,7 @@ static PyObject* prefix_body(PyObject* const* a, Py_ssize_t n) {
     OnStream on(a[11], *Q);
     if (PyErr_Occurred()) return nullptr;
     const at::Device device = Q->device();
-    Results results(device, {out ? 0 : Results::bytes_of({B, H, T, 64}, p.dtype == HK_F32 ? 4 : 2), lse ? 0 : Results::bytes_of({B, H, T}, 4)});
-    at::Tensor O = out ? *out : results.take({B, H, T, 64}, scalar_of(p.dtype)), L = lse ? *lse : results.take({B, H, T}, at::kFloat), own;
+    at::Tensor O = out ? *out : fresh({B, H, T, 64}, scalar_of(p.dtype), device), L = lse ? *lse : fresh({B, H, T}, at::kFloat, device), own;
     p.O = {O.data_ptr(), O.stride(0), O.stride(2), O.stride(1)};
     p.LSE = data(L); p.lse_strideB = L.stride(0); p.lse_strideH = L.stride(1);
     const size_t need = g_lib.prefix_bytes(&p);

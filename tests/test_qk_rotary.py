@@ -517,3 +517,21 @@ def test_fractions_of_a_turn_to_the_last_bits(base, given):
             turns = (decimal.Decimal(float(exact[p])) if given else exact[p]) / two_pi
             off = abs(plan.turn[p] - turns * 2 ** 64) % 2 ** 64
             assert min(off, 2 ** 64 - off) <= decimal.Decimal(0.5) + 4 * turns, p
+
+
+@pytest.mark.gpu
+def test_each_result_has_memory_of_its_own():
+    """What keeps, shares or writes out one of them has nothing of the others."""
+    import io
+
+    q, k = inputs(8, 3, 4, 2, 5, BF16, "packed")
+    pos, w = torch.arange(5, device="cuda").expand(1, 3, 5), torch.ones(64, device="cuda", dtype=BF16)
+    lens = torch.full((3,), 5, device="cuda", dtype=torch.int32)
+    for results in (hk.rotary_forward(q, k, pos, (32,)), hk.rotary_backward(q, k, pos, (32,)), hk.qk_norm_rotary_forward(q, k, w, w, pos, (32,)),
+                    hk.qk_norm_rotary_backward(q, k, q, k, w, w, pos, (32,)), hk.shared_prefix_attention(q, k[0], k[0], k, k, lens, 0.125)):
+        assert len({x.untyped_storage().data_ptr() for x in results}) == len(results)
+        for x in results:
+            assert x.storage_offset() == 0 and x.untyped_storage().nbytes() == x.numel() * x.element_size()
+            file = io.BytesIO()
+            torch.save(x, file)
+            assert file.tell() < x.numel() * x.element_size() + 4096
