@@ -43,5 +43,6 @@ from .operators import (  # noqa: F401
     rotary_forward,
     rotary_plan,
     shared_prefix_attention,
+    shared_prefix_workspace_bytes,
 )
 from .host_step import HostAttentionStep  # noqa: F401

@@ -475,6 +475,33 @@ static PyObject* qk_body(PyObject* const* a, Py_ssize_t n) {
     return which == 3 ? wrap({r[0], r[1], dw[0], dw[1]}) : wrap({r[0], r[1]});
 }
 
+// What of a shared prefix's call its workspace depends on; false with AssertionError set.
+static bool prefix_sizes(const at::Tensor& Q, const at::Tensor& K_prefix, const at::Tensor& K, hk_shared_prefix_params* p) {
+    if (!view(Q, "Q", -1, -1, -1, -1, &p->Q)) return false;
+    p->dtype = dtype_code(Q);
+    if (!view(K, "K", Q.size(0), -1, -1, p->dtype, &p->K) || !view(K_prefix, "K_prefix", 1, K.size(1), -1, p->dtype, &p->Kp, true)) return false;
+    p->B = (int)Q.size(0); p->nh = (int)Q.size(1); p->nh_kv = (int)K.size(1);
+    p->T = Q.size(2); p->prefix_len = K_prefix.size(-2); p->kv_len = K.size(2);
+    return true;
+}
+
+// prefix_workspace(Q, K_prefix, K) -> bytes that are enough for the workspace of the call, wherever they start
+static PyObject* prefix_workspace_body(PyObject* const* a, Py_ssize_t n) {
+    if (n != 3) {
+        PyErr_SetString(PyExc_TypeError, "prefix_workspace: 3 arguments");
+        return nullptr;
+    }
+    const at::Tensor *Q, *K_prefix, *K;
+    if (!tensors({{a[0], "Q", false, &Q}, {a[1], "K_prefix", false, &K_prefix}, {a[2], "K", false, &K}})) return nullptr;
+    hk_shared_prefix_params p = {};
+    if (!prefix_sizes(*Q, *K_prefix, *K, &p)) return nullptr;
+    p.scale = 1.f;
+    c10::cuda::OptionalCUDAGuard device;  // the plan goes by its SMs
+    if (Q->is_cuda()) device.set_device(Q->device());
+    const size_t need = g_lib.prefix_bytes(&p);
+    return PyLong_FromSize_t(need > 0 ? need + 256 : 0);
+}
+
 // prefix(Q, K_prefix, V_prefix, K, V, lengths, scale, causal, workspace, out, lse, stream) -> (O, LSE), or the negative status
 static PyObject* prefix_body(PyObject* const* a, Py_ssize_t n) {
     if (n != 12) {
@@ -486,14 +513,9 @@ static PyObject* prefix_body(PyObject* const* a, Py_ssize_t n) {
                   {a[4], "V", false, &kv[3]}, {a[5], "lengths", true, &lens}, {a[8], "workspace", true, &ws}, {a[9], "out", true, &out}, {a[10], "lse", true, &lse}}))
         return nullptr;
     hk_shared_prefix_params p = {};
-    if (!view(*Q, "Q", -1, -1, -1, -1, &p.Q)) return nullptr;
-    const int64_t B = Q->size(0), H = Q->size(1), T = Q->size(2);
-    p.dtype = dtype_code(*Q);
-    if (!view(*kv[2], "K", B, -1, -1, p.dtype, &p.K)) return nullptr;
-    const int64_t Hk = kv[2]->size(1), S = kv[2]->size(2);
-    if (!view(*kv[3], "V", B, Hk, S, p.dtype, &p.V) || !view(*kv[0], "K_prefix", 1, Hk, -1, p.dtype, &p.Kp, true) ||
-        !view(*kv[1], "V_prefix", 1, Hk, kv[0]->size(-2), p.dtype, &p.Vp, true))
-        return nullptr;
+    if (!prefix_sizes(*Q, *kv[0], *kv[2], &p)) return nullptr;
+    const int64_t B = Q->size(0), H = Q->size(1), T = Q->size(2), Hk = kv[2]->size(1);
+    if (!view(*kv[3], "V", B, Hk, p.kv_len, p.dtype, &p.V) || !view(*kv[1], "V_prefix", 1, Hk, p.prefix_len, p.dtype, &p.Vp, true)) return nullptr;
     if (lens && (lens->dim() != 1 || lens->size(0) != B || (B > 1 && lens->stride(0) != 1) || lens->scalar_type() != at::kInt))
         return refuse("lengths", "expected [B] of int32, contiguous"), nullptr;
     if (out && !view(*out, "out", B, H, T, p.dtype, &p.O)) return nullptr;
@@ -502,7 +524,6 @@ static PyObject* prefix_body(PyObject* const* a, Py_ssize_t n) {
     p.scale = (float)PyFloat_AsDouble(a[6]);
     p.is_causal = PyObject_IsTrue(a[7]) != 0;
     if (PyErr_Occurred()) return nullptr;
-    p.B = (int)B; p.nh = (int)H; p.nh_kv = (int)Hk; p.T = T; p.prefix_len = kv[0]->size(-2); p.kv_len = S;
     p.lengths = lens ? static_cast<const int32_t*>(lens->data_ptr()) : nullptr;
     if (!one_device({Q, kv[0], kv[1], kv[2], kv[3], lens, ws, out, lse})) return nullptr;
     OnStream on(a[11], *Q);
@@ -527,6 +548,7 @@ static PyObject* prefix_body(PyObject* const* a, Py_ssize_t n) {
 
 static PyObject* qk(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return qk_body(a, n); }); }
 static PyObject* prefix(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return prefix_body(a, n); }); }
+static PyObject* prefix_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return prefix_workspace_body(a, n); }); }
 
 static PyObject* forward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return forward_body(a, n); }); }
 static PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return backward_body(a, n); }); }
@@ -560,6 +582,7 @@ static PyMethodDef methods[] = {
     {"zero", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(zero)), METH_FASTCALL, nullptr},
     {"qk", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk)), METH_FASTCALL, nullptr},
     {"prefix", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefix)), METH_FASTCALL, nullptr},
+    {"prefix_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefix_workspace)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hk_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

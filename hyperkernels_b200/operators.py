@@ -103,6 +103,13 @@ def qk_norm_rotary_backward(Q, K, dQ, dK, w_q, w_k, positions, sections, *, eps:
                None, out_q, out_k, stream)
 
 
+def shared_prefix_workspace_bytes(Q, K_prefix, K) -> int:
+    """Bytes that a ``workspace`` of ``shared_prefix_attention`` needs for these tensors' sizes and type, on Q's device; 0: none.
+
+    It goes by how the work is cut: other sizes, even smaller ones, may need more."""
+    return (_att._native or _att._torch_calls()).prefix_workspace(Q, K_prefix, K)
+
+
 def shared_prefix_attention(Q, K_prefix, V_prefix, K, V, lengths, scale: float, causal: bool = True, *, workspace=None, out=None,
                             lse=None, stream=None):
     """O, LSE of the new tokens Q [B, H, T, 64] of B requests that share a prefix: forward only, for serving (T = 1: decoding).
@@ -114,6 +121,8 @@ def shared_prefix_attention(Q, K_prefix, V_prefix, K, V, lengths, scale: float, 
     own: token i of T sees j <= lengths[b] - T + i.  A row that sees no key gives O = 0, LSE = -inf.  P and S may be 0.
     A key that only ``causal`` hides from a row takes part in it with weight 0, so its values have to be finite.  Keys and values
     may not be expanded (a stride of 0).  The same call gives the same bits.
+    ``workspace``: contiguous memory of ``shared_prefix_workspace_bytes`` on the device, of any type, for this call alone until it
+    is done (None: allocated).  It needs no contents and keeps none; each captured call needs its own.
     All of one type, which O has too; LSE is float32.  Softmax and sums are fp32."""
     r = (_att._native or _att._torch_calls()).prefix(Q, K_prefix, V_prefix, K, V, lengths, scale, causal, workspace, out, lse,
                                                      stream if stream is None else _stream_handle(stream))

@@ -575,3 +575,55 @@ def test_results_that_lie_apart_get_past_that():
     b.B, b.nh, b.nh_kv, b.T, b.lse_sB, b.lse_sH, b.LSE = 1, 1, 1, 1, 0, 0, 0x1002
     b.O.sB = b.O.sM = b.O.sH = 0
     assert f(C.byref(b), None) == -3
+
+
+# ---- workspaces that the caller brings -------------------------------------------------------------------------------------------------
+def _tensors_of(B, H, Hk, T, P, S, dtype):
+    one = torch.zeros(1, 1, 1, 64, dtype=TYPES[dtype])
+    return one.expand(B, H, T, 64), one[0].expand(Hk, P, 64), one.expand(B, Hk, S, 64)
+
+
+def test_the_size_of_a_workspace():
+    """On the 148 SMs that the library takes where there is no device."""
+    f = hk.lib().hk_shared_prefix_workspace_bytes
+    f.restype, f.argtypes = C.c_size_t, [C.c_void_p]
+    seen = set()
+    for B, H, Hk, T, P, S, dtype in WAYS:
+        b = _block()
+        b.B, b.nh, b.nh_kv, b.T, b.prefix_len, b.kv_len, b.dtype = B, H, Hk, T, P, S, list(TYPES).index(dtype)
+        need, got = f(C.byref(b)), hk.shared_prefix_workspace_bytes(*_tensors_of(B, H, Hk, T, P, S, dtype))
+        assert got == (need + 256 if need else 0)
+        seen.add(need > 0)
+    assert seen == {False, True}
+    q, kp, k = _tensors_of(2, 4, 2, 3, 9, 8, "f32")
+    for name, args in (("Q", (q[0], kp, k)), ("K_prefix", (q, kp[:1], k)), ("K", (q, kp, k[:1])), ("K", (q, kp, k.half()))):
+        with pytest.raises(AssertionError, match="^" + name):
+            hk.shared_prefix_workspace_bytes(*args)
+    with pytest.raises(TypeError, match="^K_prefix: expected a tensor"):
+        hk.shared_prefix_workspace_bytes(q, None, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,T,P,S,dtype", [(16, 12, 12, 1, 2047, 512, "f32"), (64, 32, 8, 1, 8192, 1000, "bf16"), (16, 4, 4, 77, 4097, 333, "f16"), (3, 4, 4, 300, 900, 400, "f32"),
+                                                (4, 12, 12, 1, 333, 64, "f32")])
+def test_a_workspace_of_ones_own(B, H, Hk, T, P, S, dtype):
+    """Whatever it holds and wherever it starts, the call has the bits of one that allocates it, and stays inside."""
+    x = make(B + T, B, H, Hk, T, P, S, dtype)
+    want = hk.shared_prefix_attention(*x, SCALE)
+    need = hk.shared_prefix_workspace_bytes(x[0], x[1], x[3])
+    room = torch.full((need + 1024,), 0xFF, device="cuda", dtype=torch.uint8)
+    for at in (0, 1, 255):
+        room.fill_(0xFF)
+        got = hk.shared_prefix_attention(*x, SCALE, workspace=room[at:at + need])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert bool((room[:at] == 0xFF).all()) and bool((room[at + need:] == 0xFF).all())
+    wide = torch.full((need // 4 + 1,), float("nan"), device="cuda")
+    for _ in range(3):  # one after the other in the same memory
+        got = hk.shared_prefix_attention(*x, SCALE, workspace=wide)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    if need:
+        with pytest.raises(AssertionError, match="too small"):
+            hk.shared_prefix_attention(*x, SCALE, workspace=room[:need - 256 - 1])
+        with pytest.raises(AssertionError, match="contiguous"):
+            hk.shared_prefix_attention(*x, SCALE, workspace=room[:1].expand(need))
+    assert hk.last_device_status() == 0
