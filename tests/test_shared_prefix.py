@@ -627,3 +627,56 @@ def test_a_workspace_of_ones_own(B, H, Hk, T, P, S, dtype):
         with pytest.raises(AssertionError, match="contiguous"):
             hk.shared_prefix_attention(*x, SCALE, workspace=room[:1].expand(need))
     assert hk.last_device_status() == 0
+
+
+# ---- both kinds of keys in one go --------------------------------------------------------------------------------------------------------
+def _plan_of(B, H, Hk, T, P, S, dtype):
+    f = hk.lib().hk_shared_prefix_plan
+    f.argtypes = [C.c_void_p, C.POINTER(C.c_int)]
+    b, plan = _block(), (C.c_int * 6)()
+    b.B, b.nh, b.nh_kv, b.T, b.prefix_len, b.kv_len, b.dtype = B, H, Hk, T, P, S, list(TYPES).index(dtype)
+    assert f(C.byref(b), plan) == 0
+    return tuple(plan)
+
+
+def test_parts_of_blocks_in_one_go():
+    """No runs of the prefix beside it, one of the own keys; few rows in one part, many in up to 16 of their last blocks, never in more than
+    two thirds of their tiles; a workspace for exactly those blocks."""
+    import random
+
+    g, parts = random.Random(5), set()
+    for _ in range(4000):
+        Hk = g.choice([1, 2, 4, 8])
+        case = (g.randint(1, 48), Hk * g.choice([1, 2, 4]), Hk, g.choice([1, 3, 17, 80, 300, 700]), g.choice([0, 1, 70, 500, 2000]), g.choice([0, 9, 130, 700, 1500]), g.choice(["f32", "bf16"]))
+        B, H, _, T, P, S, dtype = case
+        prefix_many, own_many, whole, runs, own_runs, slots = _plan_of(*case)
+        if not whole:
+            assert slots == runs + own_runs, case
+            continue
+        assert not prefix_many and runs == 0 and own_runs == 1 and 1 <= slots <= 16, case
+        assert own_many or slots == 1, case
+        rows, keys = (128, 64) if dtype == "f32" else (256, 128)
+        blocks = B * Hk * -(-T * (H // Hk) // rows)
+        if slots > 1:
+            assert blocks % 148 and 1.5 * slots <= -(-P // keys) + -(-S // keys), case
+        need = hk.shared_prefix_workspace_bytes(*_tensors_of(*case))
+        assert need == (slots * (blocks % 148) * rows * (64 + 2) * 4 + 256 if slots > 1 else 0), case
+        parts.add(slots)
+    assert {1, 2, 3, 4} <= parts and max(parts) >= 10, parts
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,T,P,S,dtype", [(2, 4, 4, 700, 0, 1500, "f32"), (2, 4, 4, 700, 0, 1500, "bf16"), (5, 4, 2, 300, 0, 1500, "f16"), (3, 4, 4, 300, 70, 1500, "f32"),
+                                                (3, 8, 2, 301, 1, 1500, "bf16")])
+@pytest.mark.parametrize("causal", [True, False])
+def test_parts_without_keys(B, H, Hk, T, P, S, dtype, causal):
+    """Requests with fewer tiles of keys than their blocks have parts: parts without a tile, rows without a key, next to full ones."""
+    slots = _plan_of(B, H, Hk, T, P, S, dtype)
+    assert slots[1] and slots[2] and slots[5] > 2, slots
+    tile = 64 if dtype == "f32" else 128
+    for lengths in ([0] * B, [1] * B, [0, 1, tile, tile + 1, S][-B:], [S, 1, 0, tile, 2 * tile + 1][:B], [2] + [0] * (B - 1)):
+        x = make(B + T, B, H, Hk, T, P, S, dtype, lengths=lengths)
+        room = torch.full((hk.shared_prefix_workspace_bytes(x[0], x[1], x[3]),), 0xFF, device="cuda", dtype=torch.uint8)  # NaN in every slot
+        got = hk.shared_prefix_attention(*x, SCALE, causal, workspace=room)
+        check(got, definition(*x, causal), dtype, lengths)
+    assert hk.last_device_status() == 0
