@@ -925,8 +925,8 @@ FwdPlan plan_attn_fwd(int BH, int Tq, int Tk, int causal, int q_pos0, int k_pos0
     const int n_kvtiles = (Tk + TILE - 1) / TILE;
     // CTAs take over further items where the grid is larger than the device and items are short: what overlaps at their ends is
     // then more than the bookkeeping costs per step (about 2 %, of which some may be registers: the kernels that take over spill
-    // 76 to 160 bytes per thread, those for one item none).  (With a dense mask the latter spill 172 bytes and are the faster for it:
-    // in another schedule of the same code with 88, H36 T512 took 87.1 instead of 62.5 us, H8 T4096 815 instead of 548.)
+    // 76 to 120 bytes per thread, those for one item none).  (With a dense mask the latter spill 148 bytes, and how the compiler orders
+    // the mask's loads decides: H36 T512 54.2 us, with __ldg 63.1 and in another schedule of that 87.1, H8 T4096 466, 550 and 815.)
     // Steps per item on average, one item per CTA -> taken over: 1.5 (H384 T256) 26.9 -> 23.9 us, 5 (H96 T1024) 41.3 -> 39.8, 9 (H96 T2048) 128 -> 124.5, 16 (the same
     // without a mask) 224 -> 225, 17 (H48 T4096) 206 -> 208, 33 (H32 T8192) 494 -> 505.
     // Every block sees a key then (q_pos0 >= k_pos0 under the mask): the hand-over between the streams, the issuing and the

@@ -9,9 +9,9 @@
 // row apart, and a load instruction of a warp takes whole 128-byte lines of four rows.  The rows of the next step are on their way
 // while a step is worked on.
 //
-// Measured (a plain copy runs at 6.54 TB/s): B8, 12 and 12 heads, T 1024, fp32, rotation 17.9 us (86 % of that rate), norm 19.5 (79 %), its
+// Measured (a plain copy runs at 6.54 TB/s): B8, 12 and 12 heads, T 1024, fp32, rotation 17.9 us (86 % of that rate), norm 19.6 (79 %), its
 // backward pass 31.1 (74 %, of which the weights' sums about 2); T 32768, 32 and 32 heads, bf16 rows and fp32 gradients 188 us
-// (87 %); T 32767, 32 and 8 heads, fp32 gradients into bf16 84 us (92 %).  One token of 16 or 64 requests 2.2 to 2.9 us.  Three CTAs to an SM
+// (87 %); T 32767, 32 and 8 heads, fp32 gradients into bf16 84 us (92 %).  One token of 16 or 64 requests 1.9 to 2.3 us.  Three CTAs to an SM
 // would leave 80 registers a thread, and what is on its way would not fit them (spills: 37.7 us instead of 20.1, 223 instead of 90).
 #include <cmath>
 

@@ -103,7 +103,8 @@ int check(const hk_shared_prefix_params* p) {
     return HK_OK;
 }
 
-// How the work is cut.  It depends on sizes, lengths and the number of SMs alone: the same call gives the same bits.
+// How the work is cut: kernels and numbers of runs depend on sizes and the number of SMs alone (lengths are on the device), the borders of
+// the runs of a request's own keys on its length too.  The same call gives the same bits.
 struct Plan {
     bool prefix_many, own_many;  // which kernels
 };

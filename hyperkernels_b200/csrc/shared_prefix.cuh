@@ -65,7 +65,8 @@ inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // swizzled; fp32 rows are two such pieces.  mn_major: the values as an MN-major operand of fp32 products.
 int prefix_tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, int rows, bool mn_major);
 
-// Launchers.  The kernel over the requests' own keys runs beside the one over the prefix, if that is launched just before it.
+// Launchers.  The kernel over the requests' own keys runs beside the one over the prefix, if that is launched just before it; it does
+// not wait for it, so a launch that does has to follow (there are slots to add up then).
 struct FewPlan {
     int rows;      // rows of a tile: 1, 2 (fp32 arithmetic lane by lane) or 16 (matrix instructions)
     int step;      // keys that a CTA takes at once

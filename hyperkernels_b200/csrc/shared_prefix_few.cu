@@ -5,8 +5,8 @@
 // barrier between warps until they merge what they have.  (Copies by the lanes themselves, cp.async, kept the load/store unit busy for
 // 112 cycles a batch and warp: 64 requests, 32 heads on 8, 8 192 and up to 1 000 keys, bf16, took 37.7 us instead of 30.5, launches
 // behind each other.)  A batch of all warps of an SM takes 0.45 us for 16-bit types, 0.65 for 16 rows of fp32, 0.4 for one or two, and
-// a CTA 2.2 us beside its batches.  Sixteen requests of 12 heads on 2 047 and up to 512 keys, fp32: 12.2 us with the launch that adds
-// up the slots, for 37.8 MB (47 % of the copy rate); four on 333 and up to 64, in one launch: 5.2 us, of which the keys take one.
+// a CTA 2.2 us beside its batches.  Sixteen requests of 12 heads on 2 047 and up to 512 keys, fp32: 12.0 us with the launch that adds
+// up the slots, for 37.8 MB (48 % of the copy rate); four on 333 and up to 64, in one launch: 5.0 us, of which the keys take one.
 //   One or two rows in fp32: a half-warp to a key, four elements a lane (RowsOfOne).
 //   Up to 16 rows: matrix instructions (m16n8k8 on TF32, m16n8k16 on 16-bit types).  A lane's part of an operand is whatever
 // 16-byte pieces it reads, because the order of the contracted index (head dimension, keys) and of the result's columns is free

@@ -15,9 +15,9 @@
 // 16-bit types are bound by the softmax: scaling, exponentials, sums and rounding of 256 rows x 128 keys take 1 930 to 2 120 cycles by
 // themselves, whether none or a third of the exponentials goes by a polynomial (the special functions alone need 2 048 or less, packed
 // arithmetic takes two issue slots), and a tile takes 2 400 to 2 500 (masked 0.4 us more).  fp32 is bound by the tensor core: 1 680 cycles of a tile's 2 030 (1.1 us).  A
-// CTA takes about 5 us beside its tiles.  8 requests of 512 tokens, 32 heads on 8, 8 192 and up to 1 024 keys, bf16: 326 us alone, 365
-// under load (800 TFLOP/s; 245 us for the exponentials at 16 a clock and SM, 175 for the products).  8 requests of 77 tokens, 12 heads,
-// 4 096 and up to 333 keys, fp32: 47 us (52 from Python, 29 for the products).
+// CTA takes about 5 us beside its tiles.  8 requests of 512 tokens, 32 heads on 8, 8 192 and up to 1 024 keys, bf16: 326 us alone, 363
+// under load (800 TFLOP/s; 175 us for the products, 196 for four fifths of the exponentials at 16 a clock and SM).  8 requests of 77 tokens, 12 heads,
+// 4 096 and up to 333 keys, fp32: 45.4 us (51.7 from Python, 29 for the products); that kernel spills 36 bytes a thread.
 // A row of Q and of O to a thread: with eight lanes to a row, through shared memory, the two took 351 and 48.6 instead of 346 and 47.0.
 #include <cmath>
 #include <mutex>

@@ -467,6 +467,9 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
 // ended): its set-up then runs beside the predecessor's last CTAs.  pdl_wait returns when the predecessor is complete and
 // its writes are visible; nothing the predecessor may have written is read, and nothing at all written, before it.  A
 // kernel triggers only after its own pdl_wait, so that what precedes IT is complete too when its successor starts.
+// A kernel that runs beside its predecessor (that over the own keys next to the prefix's, shared_prefix.cuh) triggers without a
+// wait.  That is sound because the predecessor triggered behind its own wait, the last CTA waits before it ends, so that the
+// kernel is not complete before its predecessor, and the launch behind it is one that waits (the sum of the slots).
 // What a predecessor may have written is never read with __ldg: for the compiler that memory does not change while the kernel
 // runs, and it may move the load in front of the wait.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

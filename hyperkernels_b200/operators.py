@@ -2,7 +2,8 @@
 the rotation in the same pass, both with their backward passes, and the attention of a batch that shares a prefix.
 
 They have no counterpart in the reference.  Tensors are ``[B, heads, T, 64]`` views with any strides whose last is 1 (rows on
-16 bytes), of float32, bfloat16 or float16; arithmetic is fp32.  A call runs on the tensors' device, on that device's current
+16 bytes), of float32, bfloat16 or float16; arithmetic is fp32 (shared prefixes of 16-bit types: but for the
+weights that multiply values, see there).  A call runs on the tensors' device, on that device's current
 stream or the one given; results and workspaces that were not given are allocated for that stream.
 """
 from __future__ import annotations
@@ -73,7 +74,7 @@ def rotary_forward(Q, K, positions, sections, *, base: float = 10000.0, frequenc
     (2 p, 2 p + 1) with ``interleaved``, and turns by ``base ** (-p / 32)`` radians per position, or by ``frequencies[p]``.  The
     turns per position are rounded once, to 2^-64 of a turn; their product with an integer position is exact, modulo a turn.
     ``K`` may be None.  Results are new tensors of ``out_dtype`` (default: Q's type), or ``out_q`` / ``out_k``, which may be Q
-    and K themselves.  A 16-bit type becomes float32 (what ``attention_forward`` reads) or stays; float32 becomes any."""
+    and K themselves and must not lie on top of each other.  A 16-bit type becomes float32 (what ``attention_forward`` reads) or stays; float32 becomes any."""
     return _qk(0, "hk_rotary_forward", Q, K, None, None, None, None, positions, sections, base, frequencies, interleaved, 0.0,
                out_dtype, out_q, out_k, stream)
 
@@ -123,7 +124,8 @@ def shared_prefix_attention(Q, K_prefix, V_prefix, K, V, lengths, scale: float, 
     may not be expanded (a stride of 0).  The same call gives the same bits.
     ``workspace``: contiguous memory of ``shared_prefix_workspace_bytes`` on the device, of any type, for this call alone until it
     is done (None: allocated).  It needs no contents and keeps none; each captured call needs its own.
-    All of one type, which O has too; LSE is float32.  Softmax and sums are fp32."""
+    All of one type, which O has too; LSE is float32.  Scores, exponentials and sums are fp32; with 16-bit types the weights that
+    multiply the values are rounded to that type, half a step each, as O is."""
     r = (_att._native or _att._torch_calls()).prefix(Q, K_prefix, V_prefix, K, V, lengths, scale, causal, workspace, out, lse,
                                                      stream if stream is None else _stream_handle(stream))
     if type(r) is int:

@@ -285,7 +285,10 @@ int hk_attn_kernel_timing_read(int kind, double* total_ms, int* launches);
 int hk_attn_selftest(int which, const float* A, const float* B, float* out, void* stream);
 
 /* ---- operators round the attention -------------------------------------------
- * No counterpart in the reference.  They read and write fp32, bf16 or fp16; everything in between is fp32. */
+ * No counterpart in the reference.  They read and write fp32, bf16 or fp16.  What is in between is fp32, but for the products
+ * of the shared prefix: 16-bit types multiply values by weights that are rounded to their type too (half a step each; the sums
+ * that divide, and LSE, are of the weights before that), fp32 tensors may go through the tensor core in two parts, which leaves
+ * out 2^-22 of a product.  A fifth of the 16-bit types' exponentials may come from a polynomial that is 2.7e-6 of them off. */
 typedef enum hk_dtype { HK_F32 = 0, HK_BF16 = 1, HK_F16 = 2 } hk_dtype;
 
 /* A [B, heads, T, 64] tensor: pointer and element strides, last stride 1.  The pointer and the bytes of every stride
@@ -350,10 +353,11 @@ size_t hk_qk_norm_rotary_workspace_bytes(const hk_qk_params* p);
  * j < lengths[b] of its request, with is_causal those with j <= lengths[b] - T + i.  Heads in groups of nh / nh_kv
  * share a head of keys and values.  A row that sees nothing gives O = 0, LSE = -inf.  A key that is_causal alone hides from
  * a row takes part in it with weight 0, so its values have to be finite.
- * A NaN among a row's scores makes O and LSE of the row NaN; so may an infinite score.
+ * A NaN among a row's scores makes O and LSE of the row NaN; so may an infinite score.  An infinite value that a row sees makes
+ * its element of O infinite or NaN.
  * Keys and values are read by TMA: a stride of 0 over a dimension larger than 1 is refused (HK_ERR_UNSUPPORTED), and so are
- * results whose rows lie on top of each other.  The same call gives the same bits; how a row's keys are shared out depends on
- * all sizes of the call, not on `lengths`. */
+ * results whose rows lie on top of each other.  The same call gives the same bits: the kernels and how many runs they cut the keys
+ * into depend on the sizes of the call and the device's SMs alone, where the runs of a request's own keys begin on its length too. */
 typedef struct hk_shared_prefix_params {
     hk_view Q;        /* [B, nh, T, 64], `dtype` */
     hk_view Kp, Vp;   /* [1, nh_kv, prefix_len, 64], once for the whole batch; strideB is not used */
