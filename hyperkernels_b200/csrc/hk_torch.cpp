@@ -264,7 +264,7 @@ static PyObject* backward_body(PyObject* const* a, Py_ssize_t n) {
     p.k_pos0 = PyLong_AsLongLong(a[13]);
     p.bh_pos0 = (uint32_t)PyLong_AsUnsignedLongLongMask(a[14]);
     if (PyErr_Occurred()) return nullptr;
-    if (!holds(*Q, "Q", B, H, Tq) || !holds(*K, "K", B, H, Tk) || !holds(*V, "V", B, H, Tk) || (O && !holds(*O, "O", B, H, Tq)) ||
+    if (!holds(*Q, "Q", B, H, Tq) || !holds(*K, "K", B, H, Tk) || !holds(*V, "V", B, H, Tk) || (O && !(p.flags & HK_FLAG_D_PRECOMPUTED) && !holds(*O, "O", B, H, Tq)) ||
         !holds(*dO, "dO", B, H, Tq) || !holds(*LSE, "LSE", B, H, Tq, false) || !holds(r[0], "dQ", B, H, Tq) || !holds(r[1], "dK", B, H, Tk) ||
         !holds(r[2], "dV", B, H, Tk) || !holds(r[3], "D", B, H, Tq, false) || !mask_holds(mask, p.dropout_p, p.flags, B, H, Tq, Tk))
         return nullptr;

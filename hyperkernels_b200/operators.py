@@ -74,7 +74,8 @@ def rotary_forward(Q, K, positions, sections, *, base: float = 10000.0, frequenc
     (2 p, 2 p + 1) with ``interleaved``, and turns by ``base ** (-p / 32)`` radians per position, or by ``frequencies[p]``.  The
     turns per position are rounded once, to 2^-64 of a turn; their product with an integer position is exact, modulo a turn.
     ``K`` may be None.  Results are new tensors of ``out_dtype`` (default: Q's type), or ``out_q`` / ``out_k``, which may be Q
-    and K themselves and must not lie on top of each other.  A 16-bit type becomes float32 (what ``attention_forward`` reads) or stays; float32 becomes any."""
+    and K themselves and must not lie on top of each other.  A 16-bit type becomes float32 (what ``attention_forward`` reads) or
+    stays; float32 becomes any."""
     return _qk(0, "hk_rotary_forward", Q, K, None, None, None, None, positions, sections, base, frequencies, interleaved, 0.0,
                out_dtype, out_q, out_k, stream)
 

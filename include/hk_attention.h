@@ -301,7 +301,8 @@ typedef struct hk_view {
 /* Rotary positions with several axes.  The 64 elements of a row are 32 pairs (p, p + 32), or (2 p, 2 p + 1) with
  * `interleaved`; pair p turns by positions[axis[p], b, t] * turn[p] / 2^64 of a full turn.  An integer position times an
  * integer fraction of a turn, modulo one turn, has no error however far the position is.  turn[p] itself is rounded: half
- * of 2^-64 of a turn and, from hk_rotary_plan_fill, 2^-62 of the turns per position, which the position multiplies.  A pair of axis HK_ROTARY_STILL is left as it is. */
+ * of 2^-64 of a turn and, from hk_rotary_plan_fill, 2^-62 of the turns per position, which the position multiplies.  A pair of axis
+ * HK_ROTARY_STILL is left as it is. */
 #define HK_ROTARY_STILL 255
 typedef struct hk_rotary_plan {
     uint64_t turn[32];

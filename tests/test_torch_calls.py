@@ -205,6 +205,9 @@ def test_larger_tensors_and_masks_without_use_are_taken():
             getattr(hk, call)(**args)
         with pytest.raises(hk.HKError, match="dropout"):
             getattr(hk, call)(**{**args, "dropout_p": 0.5, "philox_seed": 3, "dropout_mask": torch.ones(1)})
+        if call == "attention_backward":  # with D there, O is not read
+            with pytest.raises(hk.HKError, match="dropout"):
+                getattr(hk, call)(**{**args, "d_precomputed": True, "O": torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16)})
 
 
 @pytest.mark.parametrize("call", ["attention_forward", "attention_backward"])
