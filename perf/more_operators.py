@@ -8,8 +8,8 @@ A case is a dict of plain values; ``op`` picks the entry point.
   ``keys`` keys of each in pages of ``page`` tokens.
 * ``append``   ``cache_append``: keys and values of new tokens into the pages: of packed prompts, or of those of ``T`` drafts
   that were accepted.
-* ``fork``     ``cache_fork``: one step of a batch: requests go on, end, or are continued several times (``beams``), with pages
-  for the ``room`` tokens to come, in the pools of ``L`` layers.
+* ``fork``     ``cache_fork``: one step of a batch: requests go on, end, are continued several times (``beams``) or start, with pages for
+  the tokens to come (``room``, or a prompt), in the pools of ``L`` layers.
 * ``compact``  ``cache_compact``: the pages in use to the front of the pools.
 
 ``layout`` is how a page lies in memory: head by head ("hpd") or token by token ("phd").  ``lens`` says how the requests' lengths
@@ -107,7 +107,7 @@ def draw(rng):
         elif op == "fork":
             beams = rng.choice([1, 2, 4, 5])
             c = _fork(None, beams * _log(rng, 1, 32), beams, rng.choice([1, 2, 12]), Hk, _log(rng, 1, 2048), page, rng.choice([1, 1, _log(rng, 1, 100)]), dtype, layout)
-            if c["B"] * c["L"] * Hk * (c["keys"] + 2 * page + c["room"]) * 256 * BYTES[dtype] <= 6e9:
+            if c["B"] * c["L"] * Hk * (1.1 * c["keys"] + 2 * page + c["room"]) * 256 * BYTES[dtype] <= 6e9:
                 return c
         else:
             c = _compact(None, _log(rng, 1, 64), rng.choice([1, 2, 4]), _log(rng, 8, 4000), Hk, page, rng.uniform(0.05, 0.95), dtype, layout)
@@ -153,6 +153,12 @@ def _sources(c):
     if W == 1:
         return [-1 if b % 9 == 4 else b for b in range(B)]
     return [b - b % W + (b * b // W + b % W * (b // W % 2)) % W for b in range(B)]
+
+
+def _rooms(c):
+    """Tokens that each request of the new batch needs pages for: those that go on some, of the places of those that have ended
+    every other one is a new prompt's."""
+    return [c["room"] if s >= 0 else c["keys"] // 2 * (b % 2) for b, s in enumerate(_sources(c))]
 
 
 def work(c):
@@ -208,7 +214,7 @@ def _pool(c):
     else:
         need = sum(_cdiv(n, c["page"]) for n in _lengths(c))
     if c["op"] == "fork":
-        need += c["B"] * (_cdiv(c["room"], c["page"]) + 2)
+        need += sum(_cdiv(r, c["page"]) + 2 for r in _rooms(c))
     return need + need // 8 + 3
 
 
@@ -308,7 +314,7 @@ def prepare(case, seed):
     if c["beams"] > 1:
         source = group * c["beams"] + (source + shift) % c["beams"]
     return dict(s, P=P, k_all=_pages(c, g, P, c["L"]), v_all=_pages(c, g, P, c["L"]), pages=pages, lens=on_device, users=users[:P].clone(),
-                source=source.to(torch.int32))
+                source=source.to(torch.int32), rooms=torch.tensor(_rooms(c), device="cuda", dtype=torch.int32))
 
 
 # ---- the operators' plain forms ------------------------------------------------------------------------------------------
@@ -388,7 +394,7 @@ def _plain_fork(s):
     first = torch.full((B,), B, device="cuda", dtype=torch.int32).scatter_reduce_(0, src, torch.where(live, i, B), "amin")
     full, begun = lens // page, lens % page
     shared = (j < full[:, None]) | ((j == full[:, None]) & (begun > 0)[:, None] & (first[src] == i)[:, None])
-    needed = j < ((lens + s["room"] + page - 1) // page * live)[:, None]
+    needed = j < ((lens + s["rooms"] + page - 1) // page)[:, None]
     kept = torch.where(shared, s["pages"][src], -1)
     users = _count(kept, P, 1, _count(s["pages"], P, -1, s["users"]))
     order = (users != 0).to(torch.int8).argsort(stable=True)
@@ -452,7 +458,7 @@ def run(s):
             return {"k": k_pages, "v": v_pages}
         k_pages, v_pages = s["k_all"][:, :P], s["v_all"][:, :P]
         if s["op"] == "fork":
-            pages, lens, users, missing = hk.cache_fork(k_pages, v_pages, s["pages"], s["lens"], s["users"], s["source"], s["room"])
+            pages, lens, users, missing = hk.cache_fork(k_pages, v_pages, s["pages"], s["lens"], s["users"], s["source"], s["rooms"])
             return {"pages": pages, "lens": lens, "users": users, "missing": missing, "k": k_pages, "v": v_pages}
         pages, users, where = hk.cache_compact(k_pages, v_pages, s["pages"], s["users"])
         return {"pages": pages, "users": users, "where": where, "k": k_pages, "v": v_pages}
@@ -538,8 +544,8 @@ def _exact_fork(s):
         new.append(row)
         new_lens.append(n)
     free = [p for p in range(P) if users[p] == 0]
-    for i, b in enumerate(s["source"].tolist()):
-        while b >= 0 and len(new[i]) < _cdiv(new_lens[i] + s["room"], page):
+    for i, room in enumerate(s["rooms"].tolist()):
+        while len(new[i]) < _cdiv(new_lens[i] + room, page):
             p = free.pop(0) if free else -1
             missing += p < 0
             if p >= 0:
