@@ -45,4 +45,13 @@ from .operators import (  # noqa: F401
     shared_prefix_attention,
     shared_prefix_workspace_bytes,
 )
+from .serving import (  # noqa: F401
+    cache_append,
+    cache_compact,
+    cache_fork,
+    prompt_attention,
+    prompt_workspace_bytes,
+    tree_attention,
+    tree_workspace_bytes,
+)
 from .host_step import HostAttentionStep  # noqa: F401

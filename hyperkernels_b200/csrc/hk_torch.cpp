@@ -29,6 +29,15 @@ typedef int (*QkFn)(const hk_qk_params*, void*);
 typedef size_t (*QkSizeFn)(const hk_qk_params*);
 typedef int (*PrefixFn)(const hk_shared_prefix_params*, void*);
 typedef size_t (*PrefixSizeFn)(const hk_shared_prefix_params*);
+typedef int (*PromptFn)(const hk_prompt_params*, void*);
+typedef size_t (*PromptSizeFn)(const hk_prompt_params*);
+typedef int (*TreeFn)(const hk_tree_params*, void*);
+typedef size_t (*TreeSizeFn)(const hk_tree_params*);
+typedef int (*AppendFn)(const hk_append_params*, void*);
+typedef int (*ForkFn)(const hk_fork_params*, void*);
+typedef size_t (*ForkSizeFn)(const hk_fork_params*);
+typedef int (*CompactFn)(const hk_compact_params*, void*);
+typedef size_t (*CompactSizeFn)(const hk_compact_params*);
 struct Library {
     FwdFn forward;
     BwdFn backward;
@@ -39,6 +48,15 @@ struct Library {
     QkSizeFn qk_bytes;
     PrefixFn prefix;
     PrefixSizeFn prefix_bytes;
+    PromptFn prompt;
+    PromptSizeFn prompt_bytes;
+    TreeFn tree;
+    TreeSizeFn tree_bytes;
+    AppendFn append;
+    ForkFn fork;
+    ForkSizeFn fork_bytes;
+    CompactFn compact;
+    CompactSizeFn compact_bytes;
 } g_lib = {};
 
 // A tensor argument; None, where it may be left out, gives nullptr.  Anything else is refused: a mask or an output buffer
@@ -546,6 +564,301 @@ static PyObject* prefix_body(PyObject* const* a, Py_ssize_t n) {
     return rc != 0 ? PyLong_FromLong(rc) : wrap({O, L});
 }
 
+// ---- serving from a cache of pages -----------------------------------------------------------------------------------------
+namespace {
+
+// t as packed rows [N, n, 64] of `type` (-1: of any) into a block's view
+bool packed(const at::Tensor& t, const char* name, int64_t N, int64_t n, int type, hk_view* v) {
+    if (t.dim() != 3 || t.size(2) != 64 || t.stride(2) != 1) return refuse(name, "expected [N,H,64] with unit last stride");
+    if (t.size(0) > MOST || t.size(1) > MOST) return refuse(name, "too large");
+    if ((N >= 0 && t.size(0) != N) || (n >= 0 && t.size(1) != n)) return refuse(name, "sizes do not fit the other tensors'");
+    if (dtype_code(t) < 0 || (type >= 0 && dtype_code(t) != type))
+        return refuse(name, type < 0 ? "expected float32, bfloat16 or float16" : "element type does not fit the other tensors'");
+    *v = {t.data_ptr(), 0, t.stride(0), t.stride(1)};
+    return true;
+}
+
+// t, if there is one, as [n] of int32, contiguous
+bool ints(const at::Tensor* t, const char* name, int64_t n, const int32_t** ptr) {
+    if (!t) return true;
+    if (t->dim() != 1 || t->size(0) != n || (n > 1 && t->stride(0) != 1) || t->scalar_type() != at::kInt) {
+        PyErr_Format(PyExc_AssertionError, "%s: expected [%lld] of int32, contiguous", name, (long long)n);
+        return false;
+    }
+    *ptr = static_cast<const int32_t*>(t->data_ptr());
+    return true;
+}
+
+// K_pages and V_pages, [P, Hk, page, 64] or [layers, P, Hk, page, 64], and the table, [B, width]; -1: whatever they are.
+// With `layers` the last three are where pools of several layers may be given.
+bool pool(const at::Tensor& K, const at::Tensor& V, const at::Tensor& pages, int64_t B, int64_t Hk, int type, hk_pool* p, int64_t* layers = nullptr,
+          int64_t* kL = nullptr, int64_t* vL = nullptr) {
+    const at::Tensor* x[2] = {&K, &V};
+    const char* names[2] = {"K_pages", "V_pages"};
+    for (int i = 0; i < 2; ++i) {
+        const at::Tensor& t = *x[i];
+        const int lead = layers && t.dim() == 5 ? 1 : 0;
+        const at::IntArrayRef size = t.sizes(), stride = t.strides();
+        if (t.dim() != lead + 4 || size[lead + 3] != 64 || stride[lead + 3] != 1)
+            return refuse(names[i], layers ? "expected [pages,H,page,64] or [layers,pages,H,page,64] with unit last stride" : "expected [pages,H,page,64] with unit last stride");
+        for (int d = 0; d < lead + 3; ++d)
+            if (size[d] > MOST) return refuse(names[i], "too large");
+        if ((Hk >= 0 && size[lead + 1] != Hk) || (i && t.sizes() != K.sizes())) return refuse(names[i], "sizes do not fit the other tensors'");
+        const int code = dtype_code(t);
+        if (code < 0 || (type >= 0 && code != type) || (i && code != dtype_code(K)))
+            return refuse(names[i], code < 0 ? "expected float32, bfloat16 or float16" : "element type does not fit the other tensors'");
+        *(i ? &p->V : &p->K) = {t.data_ptr(), stride[lead], stride[lead + 2], stride[lead + 1]};
+        if (layers) {
+            *layers = lead ? size[0] : 1;
+            *(i ? vL : kL) = lead ? stride[0] : 0;
+        }
+        p->n_pages = (int)size[lead];
+        p->page = (int)size[lead + 2];
+    }
+    if (pages.dim() != 2 || (B >= 0 && pages.size(0) != B) || (pages.size(1) > 1 && pages.stride(1) != 1) || pages.scalar_type() != at::kInt)
+        return refuse("pages", "expected [B,width] of int32 with unit last stride");
+    if (pages.size(0) > MOST || pages.size(1) > MOST) return refuse("pages", "too large");
+    p->pages = static_cast<const int32_t*>(pages.data_ptr());
+    p->pages_stride = pages.stride(0);
+    p->width = (int)pages.size(1);
+    return true;
+}
+
+// The workspace that a caller brought, or one of the call's stream's.
+bool space(const at::Tensor* given, size_t need, const at::Device& device, at::Tensor* own, void** ptr, size_t* bytes) {
+    if (!given && need > 0) {
+        *own = fresh({(int64_t)need + 256}, at::kByte, device);
+        given = own;
+    }
+    return !given || given_workspace(given, need, ptr, bytes);
+}
+
+bool prompt_sizes(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& starts, hk_prompt_params* p) {
+    if (!packed(Q, "Q", -1, -1, -1, &p->Q)) return false;
+    p->dtype = dtype_code(Q);
+    if (!packed(K, "K", Q.size(0), -1, p->dtype, &p->K)) return false;
+    if (starts.dim() != 1 || starts.size(0) < 2 || starts.size(0) > MOST || starts.stride(0) != 1 || starts.scalar_type() != at::kInt)
+        return refuse("starts", "expected [B+1] of int32, contiguous");
+    p->starts = static_cast<const int32_t*>(starts.data_ptr());
+    p->B = (int)starts.size(0) - 1; p->nh = (int)Q.size(1); p->nh_kv = (int)K.size(1); p->N = Q.size(0);
+    return true;
+}
+
+bool tree_sizes(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& K_pages, const at::Tensor& V_pages, const at::Tensor& pages, hk_tree_params* p) {
+    if (!view(Q, "Q", -1, -1, -1, -1, &p->Q)) return false;
+    p->dtype = dtype_code(Q);
+    if (!view(K, "K", Q.size(0), -1, Q.size(2), p->dtype, &p->K) || !pool(K_pages, V_pages, pages, Q.size(0), K.size(1), p->dtype, &p->pool)) return false;
+    p->B = (int)Q.size(0); p->nh = (int)Q.size(1); p->nh_kv = (int)K.size(1); p->T = Q.size(2);
+    return true;
+}
+
+}  // namespace
+
+// prompt(Q, K, V, starts, scale, causal, workspace, out, lse, stream) -> (O, LSE), or the negative status
+static PyObject* prompt_body(PyObject* const* a, Py_ssize_t n) {
+    if (n != 10) {
+        PyErr_SetString(PyExc_TypeError, "prompt: 10 arguments");
+        return nullptr;
+    }
+    const at::Tensor *Q, *K, *V, *starts, *ws, *out, *lse;
+    if (!tensors({{a[0], "Q", false, &Q}, {a[1], "K", false, &K}, {a[2], "V", false, &V}, {a[3], "starts", false, &starts}, {a[6], "workspace", true, &ws},
+                  {a[7], "out", true, &out}, {a[8], "lse", true, &lse}}))
+        return nullptr;
+    hk_prompt_params p = {};
+    if (!prompt_sizes(*Q, *K, *starts, &p)) return nullptr;
+    const int64_t N = Q->size(0), H = Q->size(1);
+    if (!packed(*V, "V", N, K->size(1), p.dtype, &p.V) || (out && !packed(*out, "out", N, H, p.dtype, &p.O))) return nullptr;
+    if (lse && (lse->dim() != 2 || lse->size(0) != H || lse->size(1) != N || (N > 1 && lse->stride(1) != 1) || lse->scalar_type() != at::kFloat))
+        return refuse("lse", "expected [H,N] of float32 with unit last stride"), nullptr;
+    p.scale = (float)PyFloat_AsDouble(a[4]);
+    p.is_causal = PyObject_IsTrue(a[5]) != 0;
+    if (PyErr_Occurred()) return nullptr;
+    if (!one_device({Q, K, V, starts, ws, out, lse})) return nullptr;
+    OnStream on(a[9], *Q);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Device device = Q->device();
+    at::Tensor O = out ? *out : fresh({N, H, 64}, scalar_of(p.dtype), device), L = lse ? *lse : fresh({H, N}, at::kFloat, device), own;
+    p.O = {O.data_ptr(), 0, O.stride(0), O.stride(1)};
+    p.LSE = data(L); p.lse_strideH = L.stride(0);
+    if (!space(ws, g_lib.prompt_bytes(&p), device, &own, &p.workspace, &p.workspace_bytes)) return nullptr;
+    int rc;
+    {
+        NoGil nogil;
+        rc = g_lib.prompt(&p, on.stream);
+    }
+    return rc != 0 ? PyLong_FromLong(rc) : wrap({O, L});
+}
+
+// tree(Q, K, V, K_pages, V_pages, pages, lengths, scale, tree, workspace, out, lse, stream) -> (O, LSE), or the negative status
+static PyObject* tree_body(PyObject* const* a, Py_ssize_t n) {
+    if (n != 13) {
+        PyErr_SetString(PyExc_TypeError, "tree: 13 arguments");
+        return nullptr;
+    }
+    const at::Tensor *Q, *K, *V, *Kp, *Vp, *pages, *lens, *bits, *ws, *out, *lse;
+    if (!tensors({{a[0], "Q", false, &Q}, {a[1], "K", false, &K}, {a[2], "V", false, &V}, {a[3], "K_pages", false, &Kp}, {a[4], "V_pages", false, &Vp},
+                  {a[5], "pages", false, &pages}, {a[6], "lengths", false, &lens}, {a[8], "tree", true, &bits}, {a[9], "workspace", true, &ws}, {a[10], "out", true, &out},
+                  {a[11], "lse", true, &lse}}))
+        return nullptr;
+    hk_tree_params p = {};
+    if (!tree_sizes(*Q, *K, *Kp, *Vp, *pages, &p)) return nullptr;
+    const int64_t B = Q->size(0), H = Q->size(1), T = Q->size(2);
+    if (!view(*V, "V", B, K->size(1), T, p.dtype, &p.V) || !ints(lens, "lengths", B, &p.lengths) || (out && !view(*out, "out", B, H, T, p.dtype, &p.O))) return nullptr;
+    if (bits && (bits->dim() != 2 || bits->size(0) != B || bits->size(1) != T || (T > 1 && bits->stride(1) != 1) || bits->scalar_type() != at::kLong))
+        return refuse("tree", "expected [B,T] of int64 with unit last stride"), nullptr;
+    if (lse && (lse->dim() != 3 || lse->size(0) != B || lse->size(1) != H || lse->size(2) != T || (T > 1 && lse->stride(2) != 1) || lse->scalar_type() != at::kFloat))
+        return refuse("lse", "expected [B,H,T] of float32 with unit last stride"), nullptr;
+    p.scale = (float)PyFloat_AsDouble(a[7]);
+    if (PyErr_Occurred()) return nullptr;
+    p.tree = bits ? static_cast<const int64_t*>(bits->data_ptr()) : nullptr;
+    p.tree_stride = bits ? bits->stride(0) : 0;
+    if (!one_device({Q, K, V, Kp, Vp, pages, lens, bits, ws, out, lse})) return nullptr;
+    OnStream on(a[12], *Q);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Device device = Q->device();
+    at::Tensor O = out ? *out : fresh({B, H, T, 64}, scalar_of(p.dtype), device), L = lse ? *lse : fresh({B, H, T}, at::kFloat, device), own;
+    p.O = {O.data_ptr(), O.stride(0), O.stride(2), O.stride(1)};
+    p.LSE = data(L); p.lse_strideB = L.stride(0); p.lse_strideH = L.stride(1);
+    if (!space(ws, g_lib.tree_bytes(&p), device, &own, &p.workspace, &p.workspace_bytes)) return nullptr;
+    int rc;
+    {
+        NoGil nogil;
+        rc = g_lib.tree(&p, on.stream);
+    }
+    return rc != 0 ? PyLong_FromLong(rc) : wrap({O, L});
+}
+
+// prompt_workspace(Q, K, starts), tree_workspace(Q, K, K_pages, V_pages, pages) -> bytes that are enough for the workspace of the call,
+// wherever they start
+static PyObject* serving_workspace_body(PyObject* const* a, Py_ssize_t n, bool tree) {
+    if (n != (tree ? 5 : 3)) {
+        PyErr_SetString(PyExc_TypeError, tree ? "tree_workspace: 5 arguments" : "prompt_workspace: 3 arguments");
+        return nullptr;
+    }
+    const at::Tensor *Q, *K, *x, *V_pages = nullptr, *pages = nullptr;
+    if (!tensors({{a[0], "Q", false, &Q}, {a[1], "K", false, &K}, {a[2], tree ? "K_pages" : "starts", false, &x}})) return nullptr;
+    if (tree && !tensors({{a[3], "V_pages", false, &V_pages}, {a[4], "pages", false, &pages}})) return nullptr;
+    hk_prompt_params p = {};
+    hk_tree_params t = {};
+    if (tree ? !tree_sizes(*Q, *K, *x, *V_pages, *pages, &t) : !prompt_sizes(*Q, *K, *x, &p)) return nullptr;
+    p.scale = t.scale = 1.f;
+    c10::cuda::OptionalCUDAGuard device;  // it goes by its SMs
+    if (Q->is_cuda()) device.set_device(Q->device());
+    const size_t need = tree ? g_lib.tree_bytes(&t) : g_lib.prompt_bytes(&p);
+    return PyLong_FromSize_t(need > 0 ? need + 256 : 0);
+}
+
+// append(K, V, K_pages, V_pages, pages, lengths, starts, picks, counts, stream) -> the status
+static PyObject* append_body(PyObject* const* a, Py_ssize_t n) {
+    if (n != 10) {
+        PyErr_SetString(PyExc_TypeError, "append: 10 arguments");
+        return nullptr;
+    }
+    const at::Tensor *K, *V, *Kp, *Vp, *pages, *lens, *starts, *picks, *counts;
+    if (!tensors({{a[0], "K", false, &K}, {a[1], "V", false, &V}, {a[2], "K_pages", false, &Kp}, {a[3], "V_pages", false, &Vp}, {a[4], "pages", false, &pages},
+                  {a[5], "lengths", false, &lens}, {a[6], "starts", true, &starts}, {a[7], "picks", true, &picks}, {a[8], "counts", true, &counts}}))
+        return nullptr;
+    hk_append_params p = {};
+    const int64_t B = pages->dim() > 0 ? pages->size(0) : 0;
+    if (starts) {
+        if (picks || counts) return refuse("starts", "not together with picks or counts"), nullptr;
+        if (!packed(*K, "K", -1, -1, -1, &p.K) || !packed(*V, "V", K->size(0), K->size(1), dtype_code(*K), &p.V)) return nullptr;
+        p.T = K->size(0); p.nh_kv = (int)K->size(1);
+    } else {
+        if (!view(*K, "K", B, -1, -1, -1, &p.K) || !view(*V, "V", B, K->size(1), K->size(2), dtype_code(*K), &p.V)) return nullptr;
+        p.T = K->size(2); p.nh_kv = (int)K->size(1);
+    }
+    p.dtype = dtype_code(*K); p.B = (int)B;
+    if (!pool(*Kp, *Vp, *pages, -1, p.nh_kv, p.dtype, &p.pool) || !ints(lens, "lengths", B, &p.lengths) || !ints(starts, "starts", B + 1, &p.starts) || !ints(counts, "counts", B, &p.counts))
+        return nullptr;
+    if (picks && (picks->dim() != 2 || picks->size(0) != B || picks->size(1) != p.T || !picks->is_contiguous() || picks->scalar_type() != at::kInt))
+        return refuse("picks", "expected [B,T] of int32, contiguous"), nullptr;
+    p.picks = picks ? static_cast<const int32_t*>(picks->data_ptr()) : nullptr;
+    if (!one_device({K, V, Kp, Vp, pages, lens, starts, picks, counts})) return nullptr;
+    OnStream on(a[9], *K);
+    if (PyErr_Occurred()) return nullptr;
+    int rc;
+    {
+        NoGil nogil;
+        rc = g_lib.append(&p, on.stream);
+    }
+    return PyLong_FromLong(rc);
+}
+
+// fork(K_pages, V_pages, pages, lengths, users, source, room, stream) -> (pages, lengths, users, missing), or the negative status
+static PyObject* fork_body(PyObject* const* a, Py_ssize_t n) {
+    if (n != 8) {
+        PyErr_SetString(PyExc_TypeError, "fork: 8 arguments");
+        return nullptr;
+    }
+    const at::Tensor *Kp, *Vp, *pages, *lens, *users, *source, *room = nullptr;
+    if (!tensors({{a[0], "K_pages", false, &Kp}, {a[1], "V_pages", false, &Vp}, {a[2], "pages", false, &pages}, {a[3], "lengths", false, &lens}, {a[4], "users", false, &users},
+                  {a[5], "source", false, &source}}))
+        return nullptr;
+    if (THPVariable_Check(a[6]) && !tensors({{a[6], "room", false, &room}})) return nullptr;
+    hk_fork_params p = {};
+    int64_t layers;
+    if (!pool(*Kp, *Vp, *pages, -1, -1, -1, &p.pool, &layers, &p.k_strideL, &p.v_strideL)) return nullptr;
+    const int64_t B = pages->size(0), B_out = source->dim() > 0 ? source->size(0) : 0;
+    if (B_out > MOST) return refuse("source", "too large"), nullptr;
+    if (!ints(lens, "lengths", B, &p.lengths) || !ints(users, "users", p.pool.n_pages, &p.users) || !ints(source, "source", B_out, &p.source)) return nullptr;
+    p.B = (int)B; p.B_out = (int)B_out; p.layers = (int)layers; p.nh_kv = (int)Kp->size(-3); p.dtype = dtype_code(*Kp);
+    if (!ints(room, "room", B_out, &p.room)) return nullptr;
+    p.room_all = room ? 0 : PyLong_AsLongLong(a[6]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!one_device({Kp, Vp, pages, lens, users, source, room})) return nullptr;
+    OnStream on(a[7], *Kp);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Device device = Kp->device();
+    at::Tensor table = fresh({B_out, (int64_t)p.pool.width}, at::kInt, device), l = fresh({B_out}, at::kInt, device), u = fresh({(int64_t)p.pool.n_pages}, at::kInt, device),
+               missing = fresh({1}, at::kInt, device), own;
+    p.pages_out = static_cast<int32_t*>(table.data_ptr()); p.lengths_out = static_cast<int32_t*>(l.data_ptr());
+    p.users_out = static_cast<int32_t*>(u.data_ptr()); p.missing = static_cast<int32_t*>(missing.data_ptr());
+    if (!space(nullptr, g_lib.fork_bytes(&p), device, &own, &p.workspace, &p.workspace_bytes)) return nullptr;
+    int rc;
+    {
+        NoGil nogil;
+        rc = g_lib.fork(&p, on.stream);
+    }
+    return rc != 0 ? PyLong_FromLong(rc) : wrap({table, l, u, missing});
+}
+
+// compact(K_pages, V_pages, pages, users, stream) -> (pages, users, where), or the negative status
+static PyObject* compact_body(PyObject* const* a, Py_ssize_t n) {
+    if (n != 5) {
+        PyErr_SetString(PyExc_TypeError, "compact: 5 arguments");
+        return nullptr;
+    }
+    const at::Tensor *Kp, *Vp, *pages, *users;
+    if (!tensors({{a[0], "K_pages", false, &Kp}, {a[1], "V_pages", false, &Vp}, {a[2], "pages", false, &pages}, {a[3], "users", false, &users}})) return nullptr;
+    hk_compact_params p = {};
+    int64_t layers;
+    if (!pool(*Kp, *Vp, *pages, -1, -1, -1, &p.pool, &layers, &p.k_strideL, &p.v_strideL) || !ints(users, "users", p.pool.n_pages, &p.users)) return nullptr;
+    const int64_t B = pages->size(0);
+    p.B = (int)B; p.layers = (int)layers; p.nh_kv = (int)Kp->size(-3); p.dtype = dtype_code(*Kp);
+    if (!one_device({Kp, Vp, pages, users})) return nullptr;
+    OnStream on(a[4], *Kp);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Device device = Kp->device();
+    at::Tensor table = fresh({B, (int64_t)p.pool.width}, at::kInt, device), u = fresh({(int64_t)p.pool.n_pages}, at::kInt, device), where = fresh({(int64_t)p.pool.n_pages}, at::kInt, device), own;
+    p.pages_out = static_cast<int32_t*>(table.data_ptr()); p.users_out = static_cast<int32_t*>(u.data_ptr()); p.where = static_cast<int32_t*>(where.data_ptr());
+    if (!space(nullptr, g_lib.compact_bytes(&p), device, &own, &p.workspace, &p.workspace_bytes)) return nullptr;
+    int rc;
+    {
+        NoGil nogil;
+        rc = g_lib.compact(&p, on.stream);
+    }
+    return rc != 0 ? PyLong_FromLong(rc) : wrap({table, u, where});
+}
+
+static PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return prompt_body(a, n); }); }
+static PyObject* prompt_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return serving_workspace_body(a, n, false); }); }
+static PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return tree_body(a, n); }); }
+static PyObject* tree_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return serving_workspace_body(a, n, true); }); }
+static PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return append_body(a, n); }); }
+static PyObject* fork_pages(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return fork_body(a, n); }); }
+static PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return compact_body(a, n); }); }
+
 static PyObject* qk(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return qk_body(a, n); }); }
 static PyObject* prefix(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return prefix_body(a, n); }); }
 static PyObject* prefix_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return prefix_workspace_body(a, n); }); }
@@ -569,6 +882,16 @@ static PyObject* bind(PyObject*, PyObject* h) {
     g_lib.qk_bytes = reinterpret_cast<QkSizeFn>(dlsym(so, "hk_qk_norm_rotary_workspace_bytes"));
     g_lib.prefix = reinterpret_cast<PrefixFn>(dlsym(so, "hk_shared_prefix_attention"));
     g_lib.prefix_bytes = reinterpret_cast<PrefixSizeFn>(dlsym(so, "hk_shared_prefix_workspace_bytes"));
+    const auto find = [&](auto& f, const char* name) { all = (f = reinterpret_cast<std::decay_t<decltype(f)>>(dlsym(so, name))) && all; };
+    find(g_lib.prompt, "hk_prompt_attention");
+    find(g_lib.prompt_bytes, "hk_prompt_workspace_bytes");
+    find(g_lib.tree, "hk_tree_attention");
+    find(g_lib.tree_bytes, "hk_tree_workspace_bytes");
+    find(g_lib.append, "hk_cache_append");
+    find(g_lib.fork, "hk_cache_fork");
+    find(g_lib.fork_bytes, "hk_cache_fork_workspace_bytes");
+    find(g_lib.compact, "hk_cache_compact");
+    find(g_lib.compact_bytes, "hk_cache_compact_workspace_bytes");
     if (!all || !g_lib.qk_bytes || !g_lib.prefix || !g_lib.prefix_bytes || !g_lib.forward || !g_lib.backward || !g_lib.zero_dq || !g_lib.fwd_bytes || !g_lib.bwd_bytes) {
         PyErr_SetString(PyExc_ImportError, "libhk_attention.so lacks an entry point");
         return nullptr;
@@ -583,6 +906,13 @@ static PyMethodDef methods[] = {
     {"qk", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk)), METH_FASTCALL, nullptr},
     {"prefix", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefix)), METH_FASTCALL, nullptr},
     {"prefix_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefix_workspace)), METH_FASTCALL, nullptr},
+    {"prompt", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prompt)), METH_FASTCALL, nullptr},
+    {"prompt_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prompt_workspace)), METH_FASTCALL, nullptr},
+    {"tree", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tree)), METH_FASTCALL, nullptr},
+    {"tree_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tree_workspace)), METH_FASTCALL, nullptr},
+    {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
+    {"fork", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fork_pages)), METH_FASTCALL, nullptr},
+    {"compact", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(compact)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hk_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

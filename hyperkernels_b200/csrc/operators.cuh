@@ -1,5 +1,5 @@
-// operators.cuh -- what the operators round the attention (qk_rotary.cu, shared_prefix.cu) share: element types and the checks of
-// their views.
+// operators.cuh -- what the operators round the attention (qk_rotary.cu, shared_prefix.cu, serving_attention.cu, cache_pages.cu) share:
+// element types and the checks of their views.
 #pragma once
 
 #include <algorithm>
@@ -35,7 +35,13 @@ __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
     return reinterpret_cast<const uint32_t&>(v);
 }
 
+inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 inline int esize(int dtype) { return dtype == HK_F32 ? 4 : 2; }
+
+template <class X>
+__device__ __forceinline__ const X* row_of(const hk_view& v, int64_t b, int64_t h, int64_t m) {
+    return static_cast<const X*>(v.ptr) + b * v.strideB + h * v.strideH + m * v.strideM;
+}
 
 // Whether stretches of `row` elements at all places of these dimensions lie apart: from the smallest stride on, each step goes past
 // all that the dimensions before it reach.  (Dimensions that interleave without meeting are not recognised; no slice or transposition

@@ -33,10 +33,6 @@ struct PrefixArgs {
     DeviceStatus* status;
 };
 
-template <class X>
-__device__ __forceinline__ const X* row_of(const hk_view& v, int64_t b, int64_t h, int64_t m) {
-    return static_cast<const X*>(v.ptr) + b * v.strideB + h * v.strideH + m * v.strideM;
-}
 // Lengths and queries are what the launch before this call wrote a moment ago: they are read behind pdl_wait, in program order.  The kernel
 // over the own keys next to the prefix's (late) begins when that one's wait is over and has none of its own; nothing says that its SM's
 // L1 has no older line of them, so it does not take them from there.  Few rows read past the L1, many have a fence in front (a row to a
@@ -58,8 +54,6 @@ __device__ __forceinline__ void store4(X* p, float4 v) {
     if constexpr (sizeof(X) == 4) *reinterpret_cast<float4*>(p) = v;
     else *reinterpret_cast<uint2*>(p) = make_uint2(pack<X>(v.x, v.y), pack<X>(v.z, v.w));
 }
-
-inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Tiles of `rows` rows of a view of keys or values, all heads and batches (tma_load_tile): 128 bytes of each row side by side,
 // swizzled; fp32 rows are two such pieces.  mn_major: the values as an MN-major operand of fp32 products.

@@ -378,6 +378,127 @@ typedef struct hk_shared_prefix_params {
 int hk_shared_prefix_attention(const hk_shared_prefix_params* p, void* stream);
 size_t hk_shared_prefix_workspace_bytes(const hk_shared_prefix_params* p);
 
+/* ---- serving from a cache of pages ----------------------------------------------
+ * No counterpart in the reference.  Prompts of different lengths behind each other, new tokens (drafted ones, or one) of each request against
+ * keys and values that lie in pages, and what happens to the pages in between.
+ *
+ * A pool holds n_pages pages of `page` tokens (a multiple of 16) of every key head, [n_pages, nh_kv, page, 64], as a view whose strideB
+ * leads from page to page: pages stored token by token are one with strideM > strideH.  Request b's token i is row i % page of the page
+ * pages[b * pages_stride + i / page].  An entry outside [0, n_pages) stands for no page: nothing is written there, and as keys and values
+ * it counts as rows of zeros.  The tables are read by the kernels: a captured call follows what they hold when it is replayed. */
+typedef struct hk_pool {
+    hk_view K, V;
+    const int32_t* pages; /* device, [B, width] */
+    int64_t pages_stride;
+    int width;
+    int n_pages, page;
+} hk_pool;
+
+/* Attention within whole prompts, packed: sequence b is rows starts[b] <= i < starts[b + 1] of Q, K, V and O; the starts are taken into
+ * [0, N] and have to ascend.  Row i sees the keys j of its sequence, with is_causal those with j <= i.  Rows in no sequence are left as
+ * they are, in O and LSE.  Heads in groups of nh / nh_kv share a head of keys and values.  NaN, infinities and bits: as in
+ * hk_shared_prefix_attention; a key that is_causal alone hides from a row has to have finite values, other sequences' may hold
+ * anything. */
+typedef struct hk_prompt_params {
+    hk_view Q, K, V;  /* [1, nh or nh_kv, N, 64], `dtype`; strideB is not used */
+    hk_view O;        /* the same, written */
+    float* LSE;       /* [nh, N], written */
+    int64_t lse_strideH;
+    const int32_t* starts; /* device, [B + 1] */
+    int B, nh, nh_kv, dtype;
+    int64_t N;
+    float scale;
+    bool is_causal;
+    void* workspace; /* hk_prompt_workspace_bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} hk_prompt_params;
+int hk_prompt_attention(const hk_prompt_params* p, void* stream);
+size_t hk_prompt_workspace_bytes(const hk_prompt_params* p);
+
+/* Attention of T <= 64 new tokens of each request.  Token i of request b sees the lengths[b] keys that lie in its pages (taken into [0,
+ * width * page]) and of the new tokens those j with bit j of tree[b * tree_stride + i]: its ancestors in a tree of drafts, and itself.
+ * Without `tree` it sees j <= i.  T = 1 is plain decoding.  A row that sees nothing gives O = 0, LSE = -inf.  Rows of pages behind a
+ * request's last key may hold anything; a new token that the tree hides from a row takes part with weight 0, so its values have to be finite. */
+#define HK_TREE_TOKENS 64
+typedef struct hk_tree_params {
+    hk_view Q;        /* [B, nh, T, 64], `dtype` */
+    hk_view K, V;     /* [B, nh_kv, T, 64], the new tokens' */
+    hk_view O;        /* [B, nh, T, 64], written */
+    float* LSE;       /* [B, nh, T], written */
+    int64_t lse_strideB, lse_strideH;
+    hk_pool pool;
+    const int32_t* lengths; /* device, [B] */
+    const int64_t* tree;    /* device, [B, T], or NULL */
+    int64_t tree_stride;
+    int B, nh, nh_kv, dtype;
+    int64_t T;
+    float scale;
+    void* workspace; /* hk_tree_workspace_bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} hk_tree_params;
+int hk_tree_attention(const hk_tree_params* p, void* stream);
+size_t hk_tree_workspace_bytes(const hk_tree_params* p);
+
+/* Brings keys and values of new tokens into the pages, behind the lengths[b] that are there: new token k of request b becomes token
+ * lengths[b] + k.  Which rows these are: with `starts` rows starts[b] <= i < starts[b + 1] of a packed [1, nh_kv, T, 64] (k = i -
+ * starts[b]); otherwise of [B, nh_kv, T, 64] the rows picks[b * T + k] (NULL: k), k < counts[b] (NULL: T).  A pick outside [0, T) is
+ * left out, and so is a token that has no page.  No two tokens may come to the same place. */
+typedef struct hk_append_params {
+    hk_view K, V;
+    hk_pool pool;           /* written */
+    const int32_t* lengths; /* device, [B] */
+    const int32_t* starts;  /* device, [B + 1], or NULL */
+    const int32_t* picks;   /* device, [B, T], or NULL */
+    const int32_t* counts;  /* device, [B], or NULL */
+    int B, nh_kv, dtype;
+    int64_t T;
+} hk_append_params;
+int hk_cache_append(const hk_append_params* p, void* stream);
+
+/* The next batch of B_out requests out of one of B: request i of it goes on where source[i] is (an entry outside [0, B): it starts
+ * anew, with a length of 0).  users[p] counts who holds page p: the entries of the tables, and whoever else keeps pages (it counts on).  Pages
+ * that are full of a request's tokens are shared by all that go on with it.  One that is begun stays with the first of these; the others
+ * get a page of their own with its rows copied, in every layer.  Then each request gets pages until it has room for room[i] tokens more,
+ * out of those that nobody holds any longer: the lowest first, to the requests in their order.  What does not fit, because the pool is
+ * empty or a row of the table at its end, is -1 in the table and counted in `missing`.
+ * Pages of requests that do not go on are free at once, and may be the ones that are given.  The old table and the new one, the old
+ * users and the new ones may not overlap. */
+typedef struct hk_fork_params {
+    hk_pool pool;             /* of the first layer, with the old table; rows of pages are written */
+    int64_t k_strideL, v_strideL; /* from layer to layer */
+    const int32_t* lengths;   /* device, [B] */
+    const int32_t* users;     /* device, [n_pages] */
+    const int32_t* source;    /* device, [B_out] */
+    const int32_t* room;      /* device, [B_out], or NULL: room_all for each */
+    int32_t* pages_out;       /* device, [B_out, width], contiguous, written */
+    int32_t* lengths_out;     /* device, [B_out], written */
+    int32_t* users_out;       /* device, [n_pages], written */
+    int32_t* missing;         /* device, [1], written */
+    int B, B_out, layers, nh_kv, dtype;
+    int64_t room_all;
+    void* workspace; /* hk_cache_fork_workspace_bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} hk_fork_params;
+int hk_cache_fork(const hk_fork_params* p, void* stream);
+size_t hk_cache_fork_workspace_bytes(const hk_fork_params* p);
+
+/* Brings the n pages that somebody holds (users > 0) to the front of the pools, in every layer: those at n and behind it are copied, in
+ * their order, to the free ones before it, in theirs.  where[p] is page p's new place, -1 if it is free; pages_out and users_out are the table
+ * and the users as they are then.  The same restrictions as above; the rows of pages that are free then are left as they are. */
+typedef struct hk_compact_params {
+    hk_pool pool;
+    int64_t k_strideL, v_strideL;
+    const int32_t* users;
+    int32_t* pages_out; /* device, [B, width], contiguous, written */
+    int32_t* users_out; /* device, [n_pages], written */
+    int32_t* where;     /* device, [n_pages], written */
+    int B, layers, nh_kv, dtype;
+    void* workspace; /* hk_cache_compact_workspace_bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} hk_compact_params;
+int hk_cache_compact(const hk_compact_params* p, void* stream);
+size_t hk_cache_compact_workspace_bytes(const hk_compact_params* p);
+
 const char* hk_status_string(int status);
 
 #ifdef __cplusplus
