@@ -35,6 +35,12 @@ __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
     return reinterpret_cast<const uint32_t&>(v);
 }
 
+template <class X>
+__device__ __forceinline__ void store4(X* p, float4 v) {
+    if constexpr (sizeof(X) == 4) *reinterpret_cast<float4*>(p) = v;
+    else *reinterpret_cast<uint2*>(p) = make_uint2(pack<X>(v.x, v.y), pack<X>(v.z, v.w));
+}
+
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 inline int esize(int dtype) { return dtype == HK_F32 ? 4 : 2; }
 

@@ -123,6 +123,30 @@ int check_sizes(const hk_tree_params* p) {
     return p->T > HK_TREE_TOKENS ? HK_ERR_UNSUPPORTED : HK_OK;
 }
 
+// What the kernel of many rows leaves of blocks that fell to several CTAs; nothing where no block can: `keys` are the most that there are.
+size_t parts_bytes(int dtype, int64_t keys, bool more) {
+    const RowsPlan plan = rows_plan(dtype);
+    if ((keys + plan.keys - 1) / plan.keys + more < 2 * plan.least) return 0;
+    return (size_t)sm_count() * (2 * plan.rows * (64 * sizeof(float) + sizeof(float2)) + sizeof(PartRecord));
+}
+int set_parts(ServingArgs& a, int dtype, size_t need, void* workspace, size_t bytes) {
+    if (need == 0) return HK_OK;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || bytes < need) return HK_ERR_WORKSPACE;
+    const size_t rows = (size_t)sm_count() * 2 * rows_plan(dtype).rows;
+    a.part = static_cast<float*>(workspace);
+    a.ml = reinterpret_cast<float2*>(a.part + rows * 64);
+    a.parts = reinterpret_cast<PartRecord*>(a.ml + rows);
+    return HK_OK;
+}
+int set_scale(ServingArgs& a, int dtype, float scale) {
+    a.scale = scale;
+    a.scale_log2e = std::fabs(scale) * LOG2E;
+    a.flip = scale > 0.f ? 0u : dtype == HK_F32 ? 0x80000000u : 0x80008000u;
+    a.status = device_status_ptr();
+    return a.status ? HK_OK : HK_ERR_CUDA;
+}
+bool few_rows(const hk_tree_params* p) { return p->T * (p->nh / p->nh_kv) <= 16; }
+
 }  // namespace
 }  // namespace hk
 
@@ -130,7 +154,7 @@ using namespace hk;
 
 extern "C" {
 
-size_t hk_prompt_workspace_bytes(const hk_prompt_params* p) { return 0; }
+size_t hk_prompt_workspace_bytes(const hk_prompt_params* p) { return check_sizes(p) == HK_OK ? parts_bytes(p->dtype, p->N, false) : 0; }
 
 int hk_prompt_attention(const hk_prompt_params* p, void* stream) {
     int rc = check_sizes(p);
@@ -146,12 +170,14 @@ int hk_prompt_attention(const hk_prompt_params* p, void* stream) {
     a.LSE = p->LSE; a.lse_sH = p->lse_strideH;
     a.starts = p->starts;
     a.B = p->B; a.Hk = p->nh_kv; a.group = p->nh / p->nh_kv; a.N = (int)p->N;
-    a.scale = p->scale;
     a.causal = p->is_causal;
-    return launch_rows<false>(a, p->dtype, a.N, static_cast<cudaStream_t>(stream));
+    if ((rc = set_parts(a, p->dtype, hk_prompt_workspace_bytes(p), p->workspace, p->workspace_bytes)) || (rc = set_scale(a, p->dtype, p->scale))) return rc;
+    return launch_prompt_rows(a, p->dtype, static_cast<cudaStream_t>(stream));
 }
 
-size_t hk_tree_workspace_bytes(const hk_tree_params* p) { return 0; }
+size_t hk_tree_workspace_bytes(const hk_tree_params* p) {
+    return check_sizes(p) == HK_OK && !few_rows(p) ? parts_bytes(p->dtype, (int64_t)p->pool.width * p->pool.page, true) : 0;
+}
 
 int hk_tree_attention(const hk_tree_params* p, void* stream) {
     int rc = check_sizes(p);
@@ -171,7 +197,8 @@ int hk_tree_attention(const hk_tree_params* p, void* stream) {
     a.LSE = p->LSE; a.lse_sB = p->lse_strideB; a.lse_sH = p->lse_strideH;
     a.lengths = p->lengths; a.tree = p->tree; a.tree_stride = p->tree_stride;
     a.B = p->B; a.Hk = p->nh_kv; a.group = p->nh / p->nh_kv; a.T = (int)p->T;
-    a.scale = p->scale;
+    if ((rc = set_parts(a, p->dtype, hk_tree_workspace_bytes(p), p->workspace, p->workspace_bytes)) || (rc = set_scale(a, p->dtype, p->scale))) return rc;
+    if (!few_rows(p)) return launch_tree_rows(a, p->dtype, static_cast<cudaStream_t>(stream));
     return launch_rows<true>(a, p->dtype, (int64_t)a.B * a.T, static_cast<cudaStream_t>(stream));
 }
 

@@ -1,0 +1,1087 @@
+// serving_sm100.cu -- attention within packed prompts, and of many new tokens against a cache of pages: blocks of 128 rows (fp32) or 256
+// (16-bit types: two streams of 128) against tiles of keys, on tcgen05.
+//
+// A row is a token under one of the query heads that share a key head; rows of a block follow each other (token by token, its heads
+// side by side), so a key is loaded once for all of them.  Lengths are on the device, so the work is cut there: block by block, head by
+// head, request by request the tiles of keys make one line, of which every CTA takes an equal stretch.  A block of rows whose tiles fall to
+// several CTAs leaves its parts (maximum, sum, weighted values) in slots of the workspace, a pair to a CTA, and a second kernel adds
+// them up in their order.
+//   Warp 0 cuts the stretch into items (a block of rows, a run of its tiles), makes them known to the other warps in a ring and loads
+// their tiles by TMA, warp 1 issues the products S = Q K^T and, two products behind, O += P V (tcgen05, operands in shared and tensor memory),
+// four warps to a stream take S through the softmax, a row to a thread.  All of them go from one item to the next without a barrier: the
+// queries and the first tiles of the next are there, and its first scores under way, when the last weights of this one are worked out.
+// Scores are three deep in tensor memory; P takes the place of its S.
+//   fp32: x = h + l with h the upper 11 bits of the significand, which is what the tensor core reads of an fp32 word.  Q lies in tensor memory
+// with its l parts, four warps write those of each tile beside it; a product is l h' + h l' + h h', in this order: what is left out is 2^-22 of it.  P V of
+// a tile comes back into registers and is added there in fp32: the tensor core's additions cut off instead of rounding.
+#include <cmath>
+#include <mutex>
+#include <numeric>
+
+#include "serving_attention.cuh"
+
+namespace hk {
+namespace {
+
+template <class X>
+struct Rows {
+    static constexpr bool LOW = sizeof(X) == 4;  // products in three parts
+    static constexpr int STREAMS = LOW ? 1 : 2;  // blocks of 128 rows
+    static constexpr int BLOCK = STREAMS * TILE;
+    static constexpr int KEYS = LOW ? 64 : 128;  // of a tile
+    static constexpr int SLOTS = LOW ? 6 : 8;    // of the ring of tiles; even: each of two pairs of warps has every other one
+    static constexpr int THREADS = 384;
+    static constexpr int SOFTMAX_WARPS = LOW ? 4 : 8;
+    static constexpr int LEAST = LOW ? 4 : 2;    // tiles of a part of a block
+    static constexpr int KV_RAW = KEYS * 64 * (int)sizeof(X), KV_BYTES = KV_RAW * (LOW ? 2 : 1);
+    static constexpr int KV_BOX = KEYS * 128;    // 128 bytes of each row
+    // queries: 16-bit types as K-major operands, two items deep; fp32 on their way to tensor memory, rows apart for the banks
+    static constexpr int Q_ROW = LOW ? 272 : 128, Q_BYTES = TILE * Q_ROW, Q_BUFFERS = LOW ? 1 : 2;
+    static constexpr int ITEMS = 8;
+};
+
+struct Item {
+    int b, kvh, row0, rows;  // request, key head, the block's first row among the request's and how many there are; 0: the end
+    int begin, len;          // of the packed rows; keys of the sequence, or in pages
+    int key0;                // of the first tile
+    int tiles, n0, n1;       // tiles of the item, and of each of its streams
+    int slot;                // of the workspace, -1: the result
+    int new_tile;            // number of the tile that is the new tokens'
+};
+
+template <class X>
+struct __align__(16) RowsShared {
+    typedef Rows<X> C;
+    uint64_t q_full[C::Q_BUFFERS], q_empty[C::Q_BUFFERS], q_ready, kv_full[C::SLOTS], kv_empty[C::SLOTS], p_full[3];
+    uint64_t s_full[C::STREAMS][3], o_full[C::STREAMS][3];  // of a stream's own products: it does not see the other's
+    uint64_t item_full[C::ITEMS], item_empty[C::ITEMS];
+    uint64_t kv_ready[C::SLOTS];  // tended: low parts are there, what is behind a last key is cleared
+    Item items[C::ITEMS];
+    int keep[C::SLOTS];  // rows of the tile that are values, LAST: none follows
+    uint32_t tmem_base;
+    Abort abort;
+};
+constexpr int LAST = -1;
+
+template <class X>
+struct RowsSpace {
+    typedef Rows<X> C;
+    static constexpr int OFF_Q = C::SLOTS * C::KV_BYTES, OFF_SH = OFF_Q + C::STREAMS * C::Q_BUFFERS * C::Q_BYTES, SMEM = OFF_SH + (int)sizeof(RowsShared<X>);
+    static_assert(SMEM <= 232448, "exceeds the 227 KiB a CTA may opt in to");
+};
+// Tensor memory.  16-bit types: three buffers of 128 columns for scores and weights, O of two streams.  fp32: three buffers of
+// 64 for scores and weights, two for the weights' low parts, O of a tile, Q and its low parts.
+constexpr uint32_t COL_O = 384, LOW_COL_LOW = 192, LOW_COL_O = 320, LOW_COL_Q = 384;
+
+enum RowsWait { W_Q = 501, W_Q_EMPTY, W_KV, W_READY, W_EMPTY, W_S, W_P, W_O, W_ITEM, W_ITEM_EMPTY };
+
+// ---------------------------------------------------------------------------
+// How the work is cut.  Block i of a request's rows meets n(i) tiles of keys, and counts as n(i) + 1.
+// ---------------------------------------------------------------------------
+// The scores of block i (rows i * BLOCK .., tokens of `group` rows) end, under the causal mask, in tile ceil(2 (i + 1) / group): both
+// types' blocks have twice as many rows as their tiles have keys.
+struct Request {
+    int begin, len, rows, blocks;
+    int64_t units;  // of all of its blocks, under one key head
+};
+template <class X, bool TREE>
+struct Work {
+    typedef Rows<X> C;
+    static_assert(C::BLOCK == 2 * C::KEYS, "tiles up to the diagonal");
+    const ServingArgs& a;
+    __device__ __forceinline__ int tiles(const Request& r, int i) const {
+        if (TREE) return (r.len + C::KEYS - 1) / C::KEYS + 1;
+        return !a.causal || i == r.blocks - 1 ? (r.len + C::KEYS - 1) / C::KEYS : (2 * (i + 1) + a.group - 1) / a.group;
+    }
+    // units in front of block i
+    __device__ __forceinline__ int64_t before(const Request& r, int i) const {
+        if (TREE || !a.causal) return (int64_t)i * (tiles(r, 0) + 1);
+        // the sum of ceil(2 k / group) for k = 1 .. i: every `group` of them come to `turn`, and each time 2 more apiece
+        const int q = i / a.group, rest = i - q * a.group, half = a.group / 2, turn = 2 * a.group - half;
+        return (int64_t)q * turn + (int64_t)a.group * q * (q - 1) + (int64_t)rest * 2 * q + rest + max(0, rest - half) + i;
+    }
+    __device__ __forceinline__ Request request(int b) const {
+        Request r;
+        if (TREE) {
+            r.begin = 0;
+            r.len = cache_keys(a, b);
+            r.rows = a.T * a.group;
+        } else {
+            r.begin = min(max(a.starts[b], 0), a.N);
+            r.len = max(0, min(max(a.starts[b + 1], 0), a.N) - r.begin);
+            r.rows = r.len * a.group;
+        }
+        r.blocks = (r.rows + C::BLOCK - 1) / C::BLOCK;
+        r.units = r.blocks ? before(r, r.blocks - 1) + tiles(r, r.blocks - 1) + 1 : 0;
+        return r;
+    }
+};
+// A place in the line of tiles: tile j of block i (j = the block's tiles: behind it)
+struct Place {
+    int b, kvh, i, j;
+    __device__ __forceinline__ bool operator==(const Place& x) const { return b == x.b && kvh == x.kvh && i == x.i; }
+};
+
+__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+    }
+    return x;
+}
+
+// The stretch of this CTA, [from, to), by one warp; false: there is none.  A border inside a block is moved to its beginning or end
+// where a part of less than LEAST tiles would be left.
+template <class X, bool TREE>
+__device__ bool find_stretch(const ServingArgs& a, int lane, Place& from, Place& to) {
+    typedef Rows<X> C;
+    const Work<X, TREE> work{a};
+    constexpr int EACH = 4;  // requests of a lane
+    int64_t all = 0, blocks = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
+        int64_t units = 0, n = 0;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            const int b = b0 + lane * EACH + k;
+            if (b >= a.B) break;
+            const Request r = work.request(b);
+            units += r.units;
+            n += r.blocks;
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            units += __shfl_xor_sync(0xffffffffu, units, off);
+            n += __shfl_xor_sync(0xffffffffu, n, off);
+        }
+        all += units;
+        blocks += n;
+    }
+    all *= a.Hk;
+    blocks *= a.Hk;
+    // A CTA to a block, more if the blocks are long, as many as there are
+    const int64_t ctas = min((int64_t)gridDim.x, max(blocks, all / (3 * C::LEAST)));
+    const int64_t me = blockIdx.x;
+    if (me >= ctas) return false;
+    const int64_t at[2] = {me * all / ctas, (me + 1) * all / ctas};
+    Place place[2];
+    bool found[2] = {false, false};
+    int64_t run = 0;
+    for (int b0 = 0; b0 < a.B && !(found[0] && found[1]); b0 += 32 * EACH) {
+        int64_t units[EACH], sum = 0;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            const int b = b0 + lane * EACH + k;
+            units[k] = b < a.B ? work.request(b).units * a.Hk : 0;
+            sum += units[k];
+        }
+        const int64_t upto = run + warp_scan(sum, lane);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const unsigned here = __ballot_sync(0xffffffffu, at[x] < upto);
+            if (found[x] || !here) continue;
+            const int l = __ffs(here) - 1;
+            int64_t left = at[x] - (upto - sum);
+            int k = 0;
+#pragma unroll
+            for (int m = 0; m < EACH - 1; ++m)
+                if (k == m && left >= units[m]) left -= units[m], ++k;
+            left = __shfl_sync(0xffffffffu, left, l);
+            const int b = b0 + l * EACH + __shfl_sync(0xffffffffu, k, l);
+            const Request r = work.request(b);
+            Place& p = place[x];
+            p.b = b;
+            p.kvh = (int)(left / r.units);
+            left -= p.kvh * r.units;
+            int lo = 0, len = r.blocks;  // the last block that begins at or before it
+            while (len > 1) {
+                const int step = (len + 31) / 32;
+                const int c = __popc(__ballot_sync(0xffffffffu, lane * step < len && work.before(r, lo + lane * step) <= left));
+                lo += (c - 1) * step;
+                len = min(step, len - (c - 1) * step);
+            }
+            p.i = lo;
+            const int n = work.tiles(r, lo), j = (int)(left - work.before(r, lo));
+            p.j = j < C::LEAST ? 0 : n - j < C::LEAST ? n : j;
+            found[x] = true;
+        }
+        run = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    from = place[0];
+    to = place[1];
+    if (!found[1]) to = {a.B, 0, 0, 0};
+    return true;
+}
+
+// A product's place in the CTA's items, in the order they are issued in: tile by tile, stream by stream
+struct Cursor {
+    int j, t, n0, n1;
+    __device__ __forceinline__ void start(int streams0, int streams1) {
+        j = 0;
+        n0 = streams0;
+        n1 = streams1;
+        t = n0 > 0 ? 0 : 1;
+    }
+    __device__ __forceinline__ bool first() const { return t == 0 || j >= n0; }  // of the tile's streams
+    __device__ __forceinline__ bool last() const { return t == 1 || j >= n1; }
+    __device__ __forceinline__ bool next() {  // false: the item is over
+        if (t == 0 && j < n1) {
+            t = 1;
+            return true;
+        }
+        ++j;
+        t = j < n0 ? 0 : 1;
+        return j < max(n0, n1);
+    }
+};
+struct Turn {  // a ring's place
+    int at;
+    uint32_t phase;
+    __device__ __forceinline__ void next(int n) {
+        if (++at == n) {
+            at = 0;
+            phase ^= 1u;
+        }
+    }
+};
+constexpr int BEHIND = 2;  // products that O is behind S
+// Whether S may be issued when it is so many items in front of O.  fp32: the queries of an item come to tensor memory when the softmax is
+// through with the item before the last, which waits for all of O of that.
+template <bool LOW>
+__device__ __forceinline__ bool may_go(int between) { return !LOW || between < 2; }
+
+// 256 bytes of a row, on their way without a tensor map
+__device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void copy16(void* to, const void* from, bool some) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(some ? 16 : 0) : "memory");
+}
+
+template <class X, bool TREE>
+__global__ void __launch_bounds__(Rows<X>::THREADS, 1)
+serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
+                    const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ ServingArgs a) {
+    typedef Rows<X> C;
+    typedef RowsSpace<X> Space;
+    constexpr bool LOW = C::LOW, BF16 = std::is_same<X, __nv_bfloat16>::value;
+    constexpr int KEYS = C::KEYS, SLOTS = C::SLOTS, ITEMS = C::ITEMS;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *sKV = smem, *sQ = smem + Space::OFF_Q;
+    RowsShared<X>& sh = *reinterpret_cast<RowsShared<X>*>(smem + Space::OFF_SH);
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::Q_BUFFERS; ++i) {
+            mbar_init(&sh.q_full[i], 1);
+            mbar_init(&sh.q_empty[i], LOW ? 4 : 1);
+        }
+        mbar_init(&sh.q_ready, 4);
+        for (int s = 0; s < SLOTS; ++s) {
+            mbar_init(&sh.kv_full[s], 1);
+            mbar_init(&sh.kv_empty[s], LOW ? 1 : 2);
+            mbar_init(&sh.kv_ready[s], LOW ? 2 : 1);
+        }
+        for (int b = 0; b < 3; ++b) {
+            mbar_init(&sh.p_full[b], 4);
+            for (int t = 0; t < C::STREAMS; ++t) {
+                mbar_init(&sh.s_full[t][b], 1);
+                mbar_init(&sh.o_full[t][b], 1);
+            }
+        }
+        for (int i = 0; i < ITEMS; ++i) {
+            mbar_init(&sh.item_full[i], 1);
+            mbar_init(&sh.item_empty[i], 1 + (LOW ? 0 : 1) + C::SOFTMAX_WARPS);
+        }
+        sh.abort.id = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&sh.tmem_base, 512);
+        tmem_relinquish();
+        tc_fence_before_sync();
+    }
+    pdl_wait();
+    pdl_trigger();
+    __syncthreads();
+    tc_fence_after_sync();
+    constexpr uint32_t tmem = 0;  // all columns are this CTA's
+    if (sh.tmem_base != tmem) sh.abort.id = 598;
+    WaitNote wc{&sh.abort};
+
+    // What the tiles need beside the loads, entry by entry of the ring.  Rows behind the request's last key may hold anything, and 0 times
+    // a NaN is one: they are cleared among the values.  fp32: the tiles' low parts, by two pairs of warps, each of which has every other
+    // slot of the ring for its own: a barrier is waited for by the parity of its phase, and is to be looked at in every one.
+    auto tend = [&](int me, int first) {
+        constexpr int EVERY = LOW ? 2 : 1;
+        Turn at{first, 0u};
+        while (true) {
+            if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.kv_full[at.at], at.phase, W_KV, at.at))) return;
+            const int keep = sh.keep[at.at];
+            if (keep == LAST) return;
+            uint4* raw = reinterpret_cast<uint4*>(sKV + at.at * C::KV_BYTES);
+            if constexpr (LOW) {
+                constexpr int EACH = C::KV_RAW / 16 / 64;
+                uint4 *from = raw + me, *low = from + C::KV_RAW / 16, x[EACH];
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) x[k] = from[k * 64];
+                if (keep < KEYS) {
+#pragma unroll
+                    for (int k = 0; k < EACH; ++k)
+                        if (((k * 64 + me) & (C::KV_BOX / 16 - 1)) / 8 >= keep) from[k * 64] = x[k] = make_uint4(0, 0, 0, 0);  // row of the box
+                }
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) low[k * 64] = make_uint4(tf32_rest(x[k].x), tf32_rest(x[k].y), tf32_rest(x[k].z), tf32_rest(x[k].w));
+                fence_proxy_async_smem();
+                mbar_arrive_warp(&sh.kv_ready[at.at], lane);
+            } else {
+                for (int k = keep * 8 + me; k < C::KV_RAW / 16; k += 32) raw[k] = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                mbar_arrive_warp(&sh.kv_ready[at.at], lane);
+                if (lane == 0) mbar_arrive(&sh.kv_empty[at.at]);  // a slot is filled again when this warp has seen what it held
+            }
+            for (int k = 0; k < EVERY; ++k) at.next(SLOTS);
+        }
+    };
+
+    // three groups of warps, 168 registers a thread at the launch
+    if (warp < 4) {
+        if constexpr (LOW) asm volatile("setmaxnreg.dec.sync.aligned.u32 120;\n");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        if (warp == 0) {
+            // ------------------------------ items, tiles of keys and values ------------------------------
+            const Work<X, TREE> work{a};
+            Place at, end;
+            bool more = find_stretch<X, TREE>(a, lane, at, end), ok = true;
+            Request req = {};
+            if (more && at.b < a.B) req = work.request(at.b);
+            PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
+            Turn put{0, 0u};
+            // The next item into the ring; one without rows at the end of the stretch
+            auto publish = [&](Item& it) {
+                it.rows = 0;
+                while (more) {
+                    if (at.b >= a.B) {
+                        more = false;
+                        break;
+                    }
+                    if (at.i >= req.blocks) {
+                        at.i = at.j = 0;
+                        if (req.blocks == 0 || ++at.kvh == a.Hk) {
+                            at.kvh = 0;
+                            if (++at.b < a.B) req = work.request(at.b);
+                        }
+                        if (at.b >= a.B) more = false;
+                        if (!more || req.blocks == 0) continue;
+                    }
+                    const bool ends = at == end;
+                    const int n = work.tiles(req, at.i), to = ends ? min(end.j, n) : n, j0 = at.j;
+                    const int i = at.i;
+                    at.i++;
+                    at.j = 0;
+                    more = !ends;
+                    if (to <= j0) continue;
+                    const int row0 = i * C::BLOCK, rows = min(C::BLOCK, req.rows - row0), count = to - j0;
+                    it.b = at.b; it.kvh = at.kvh; it.row0 = row0; it.rows = rows;
+                    it.begin = req.begin; it.len = req.len; it.key0 = j0 * KEYS; it.tiles = count;
+                    it.new_tile = TREE ? n - 1 - j0 : -1;
+                    it.n0 = count;
+                    it.n1 = 0;
+                    if (!LOW && rows > TILE) {
+                        it.n1 = count;
+                        if (!TREE && a.causal) it.n0 = max(0, min((((row0 + TILE - 1) / a.group) / KEYS) + 1 - j0, count));
+                    }
+                    it.slot = -1;
+                    if (j0 > 0) {
+                        it.slot = 2 * blockIdx.x;
+                        record.head = to < n ? PART_GOES_ON : PART_LAST;
+                    } else {
+                        if (record.head == PART_EMPTY) record.head = PART_NONE;
+                        if (to < n) {
+                            it.slot = 2 * blockIdx.x + 1;
+                            record.b = TREE ? it.b : 0; record.kvh = it.kvh; record.begin = it.begin; record.row0 = row0; record.rows = rows;
+                        }
+                    }
+                    break;
+                }
+            };
+            int made = 0;
+            auto emit = [&](Item& it) -> bool {  // false: gave up
+                publish(it);
+                if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.item_empty[put.at], put.phase ^ 1u, W_ITEM_EMPTY, made))) return false;
+                if (lane == 0) {
+                    sh.items[put.at] = it;
+                    mbar_arrive(&sh.item_full[put.at]);
+                }
+                if constexpr (LOW) {
+                    if (it.rows > 0) {  // its queries, once those before are in tensor memory
+                        if (made > 0 && !__all_sync(0xffffffffu, mbar_wait(wc, &sh.q_empty[0], (made - 1) & 1, W_Q_EMPTY, made))) return false;
+                        if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[0], it.rows * 256);
+                        __syncwarp();
+                        for (int r = lane; r < it.rows; r += 32) {
+                            const int row = it.row0 + r, token = row / a.group;
+                            bulk_load(sQ + r * C::Q_ROW, row_of<X>(a.Q, TREE ? it.b : 0, it.kvh * a.group + row - token * a.group, it.begin + token), 256, &sh.q_full[0]);
+                        }
+                    }
+                }
+                put.next(ITEMS);
+                ++made;
+                return true;
+            };
+            Turn ring{0, 0u};
+            int filled = 0;
+            auto load = [&](const Item& it, int j, bool v) -> bool {
+                if (filled >= SLOTS && !__all_sync(0xffffffffu, mbar_wait(wc, &sh.kv_empty[ring.at], ring.phase ^ 1u, W_EMPTY, filled))) return false;
+                const int key = it.key0 + j * KEYS, s = ring.at;
+                const bool fresh = TREE && j == it.new_tile;
+                uint8_t* to = sKV + s * C::KV_BYTES;
+                if (lane == 0) {
+                    sh.keep[s] = v && !fresh ? min(KEYS, it.len - key) : KEYS;
+                    mbar_arrive_expect_tx(&sh.kv_full[s], C::KV_RAW);
+                    if (!TREE) tma_load_tile(to, v ? &map_v : &map_k, &sh.kv_full[s], it.begin + key, it.kvh, 0);
+                    else if (fresh) tma_load_tile(to, v ? &map_v : &map_k, &sh.kv_full[s], 0, it.kvh, it.b);
+                }
+                if constexpr (TREE) {
+                    if (!fresh) {
+                        __syncwarp();
+                        // a box of a page to a lane; pages that are none, and those behind the last, read as zeros
+                        const int boxes = KEYS / a.box;
+                        if (lane < boxes) {
+                            const int k = key + lane * a.box, at_page = k / a.pool.page;
+                            const int page = k < it.len ? a.pool.pages[it.b * a.pool.pages_stride + at_page] : -1;
+                            const CUtensorMap* map = v ? &map_vp : &map_kp;
+#pragma unroll
+                            for (int half = 0; half < (LOW ? 2 : 1); ++half)
+                                tma_load_box(to + half * C::KV_BOX + lane * a.box * 128, map, &sh.kv_full[s], k - at_page * a.pool.page, half, it.kvh, page);
+                        }
+                    }
+                }
+                ring.next(SLOTS);
+                ++filled;
+                return true;
+            };
+            Item next, old;  // of S and of O
+            Cursor s, o;
+            int ahead = 0;  // products that S is in front of O
+            Turn got{0, 0u};
+            ok = emit(next);
+            bool s_on = ok && next.rows > 0;
+            int between = 0;  // items that S is in front of O
+            if (s_on) {
+                s.start(next.n0, next.n1);
+                old = next;
+                o.start(old.n0, old.n1);
+                got.next(ITEMS);
+            }
+            while (ok && (s_on || ahead > 0)) {  // in step with the products
+                const bool go = s_on && may_go<LOW>(between);
+                if (go) {
+                    if (s.first() && !(ok = load(next, s.j, false))) break;
+                    ++ahead;
+                    if (!s.next()) {
+                        if (!(ok = emit(next))) break;
+                        s_on = next.rows > 0;
+                        if (s_on) s.start(next.n0, next.n1);
+                        ++between;
+                    }
+                }
+                if (ahead > BEHIND || !s_on || !go) {
+                    if (o.first() && !(ok = load(old, o.j, true))) break;
+                    --ahead;
+                    if (!o.next() && (ahead > 0 || s_on)) {
+                        __syncwarp();
+                        old = sh.items[got.at];
+                        o.start(old.n0, old.n1);
+                        got.next(ITEMS);
+                        --between;
+                    }
+                }
+            }
+            for (int k = 0; ok && k < (LOW ? 2 : 1); ++k) {  // to those who tend the tiles: no more
+                if (filled >= SLOTS && !(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.kv_empty[ring.at], ring.phase ^ 1u, W_EMPTY, filled)))) break;
+                if (lane == 0) {
+                    sh.keep[ring.at] = LAST;
+                    mbar_arrive(&sh.kv_full[ring.at]);
+                }
+                ring.next(SLOTS);
+                ++filled;
+            }
+            if (a.parts && lane == 0) a.parts[blockIdx.x] = record;
+            // a CTA that gave up may have copies in flight: they get time to land
+            if (!ok)
+                for (const unsigned long long t0 = globaltimer_ns(); globaltimer_ns() - t0 < 100000ull;) {}
+        } else if (warp == 1) {
+            // ------------------------------ products ------------------------------
+            const uint32_t leader = elect_one_sync();
+            struct Barrier {
+                uint64_t* bar;
+                uint32_t parity;
+            };
+            // each barrier is looked at while the products before it are still being issued, and waited for if that look came too early
+            auto seen = [&](const Barrier& x) { return mbar_test_wait(x.bar, x.parity); };
+            auto wait = [&](bool was_seen, const Barrier& x, int id, int aux) {
+                return __all_sync(0xffffffffu, was_seen) || (bool)__all_sync(0xffffffffu, mbar_wait(wc, x.bar, x.parity, id, aux));
+            };
+            const uint32_t kv_addr = smem_u32(sKV);
+            const Desc q_desc = make_smem_desc(smem_u32(sQ), 16, 1024, DESC_SW128), k_desc = make_smem_desc(kv_addr, 16, 1024, DESC_SW128),
+                       v_desc = LOW ? mnmajor_desc(kv_addr, 0, C::KV_BOX) : make_smem_desc(kv_addr, 16, 1024, DESC_SW128);
+            const uint32_t negate = a.flip ? IDESC_NEGATE_A : 0u;
+            Turn tile{0, 0u}, p{0, 0u}, s_item{0, 0u}, o_item{0, 0u};
+            Cursor s, o;
+            int ahead = 0, k_slot = 0, v_slot = 0, s_buf = 0, items = 0, low_buf = 0;
+            int s_own[2] = {0, 0}, o_own[2] = {0, 0};  // the next barriers of a stream's own
+            auto after = [&](int (&own)[2], int t) {
+                const int x = t ? own[1] : own[0], y = x == 2 ? 0 : x + 1;
+                if (t) own[1] = y;
+                else own[0] = y;
+                return t * 3 + x;
+            };
+            bool ok = true, s_on = false;
+            int between = 0;
+            auto look_at = [&](const Turn& x, bool v) -> Barrier { return LOW || v ? Barrier{&sh.kv_ready[x.at], x.phase} : Barrier{&sh.kv_full[x.at], x.phase}; };
+            auto next_item = [&](Turn& turn, Cursor& c) -> bool {  // false: the end, or gave up
+                if (!(ok = wait(false, {&sh.item_full[turn.at], turn.phase}, W_ITEM, items))) return false;
+                const Item& it = sh.items[turn.at];
+                if ((int)uniform(it.rows) == 0) return false;
+                c.start((int)uniform(it.n0), (int)uniform(it.n1));
+                return true;
+            };
+            s_on = next_item(s_item, s);
+            if (s_on) next_item(o_item, o);
+            bool new_queries = true, seen_k = false, seen_v = false, seen_p = false;
+#pragma unroll 1
+            while (ok && (s_on || ahead > 0)) {
+                const bool go = s_on && may_go<LOW>(between);
+                if (go) {
+                    if (new_queries) {
+                        if (!(ok = wait(false, LOW ? Barrier{&sh.q_ready, (uint32_t)items & 1u} : Barrier{&sh.q_full[items & 1 & (C::Q_BUFFERS - 1)], (uint32_t)(items >> 1) & 1u}, W_Q, items))) break;
+                        new_queries = false;
+                    }
+                    if (s.first()) {
+                        if (!(ok = wait(seen_k, look_at(tile, false), W_READY, items))) break;
+                        k_slot = tile.at;
+                        tile.next(SLOTS);
+                    }
+                    seen_k = false;
+                    tc_fence_after_sync();
+                    const Desc kd = k_desc + k_slot * C::KV_BYTES;
+                    const bool both = ahead >= BEHIND;  // O follows
+                    auto look = [&] {
+                        seen_v = o.first() && seen(look_at(tile, true));
+                        seen_p = seen({&sh.p_full[p.at], p.phase});
+                    };
+                    if constexpr (LOW) {
+                        constexpr uint32_t IDESC = make_idesc_tf32(TILE, KEYS, false, false);
+                        const uint32_t d = tmem + s_buf * 64;
+                        auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
+                            umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x, kd + y, IDESC, acc);
+                            umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x + 32, kd + (y + C::KV_BOX), IDESC, 1u);
+                        };
+                        eight(64, 0, 0u);
+                        eight(0, C::KV_RAW, 1u);
+                        if (both) look();
+                        eight(0, 0, 1u);
+                    } else {
+                        const uint32_t IDESC = make_idesc_16(TILE, KEYS, BF16, false) | negate;
+                        const uint32_t d = tmem + s_buf * 128;
+                        const Desc qd = q_desc + ((items & 1) * C::STREAMS + s.t) * C::Q_BYTES;
+                        umma_ss_16(leader, d, qd.d, kd.d, IDESC, 0u);
+                        umma_ss_16(leader, d, qd.d + 2, kd.d + 2, IDESC, 1u);
+                        if (both) look();
+                        umma_ss_16(leader, d, qd.d + 4, kd.d + 4, IDESC, 1u);
+                        umma_ss_16(leader, d, qd.d + 6, kd.d + 6, IDESC, 1u);
+                    }
+                    umma_commit_lead(leader, &sh.s_full[0][0] + after(s_own, s.t));
+                    if (s.last()) umma_commit_lead(leader, &sh.kv_empty[k_slot]);
+                    s_buf = s_buf == 2 ? 0 : s_buf + 1;
+                    ++ahead;
+                    if (!s.next()) {
+                        if (!LOW) umma_commit_lead(leader, &sh.q_empty[items & (C::Q_BUFFERS - 1)]);
+                        ++items;
+                        s_item.next(ITEMS);
+                        s_on = next_item(s_item, s);
+                        if (!ok) break;
+                        new_queries = true;
+                        ++between;
+                    }
+                }
+                if (ahead > BEHIND || !s_on || !go) {  // O
+                    if (o.first()) {
+                        if (!(ok = wait(seen_v, look_at(tile, true), W_READY, items))) break;
+                        v_slot = tile.at;
+                        tile.next(SLOTS);
+                    }
+                    if (!(ok = wait(seen_p, {&sh.p_full[p.at], p.phase}, W_P, items))) break;
+                    tc_fence_after_sync();
+                    seen_v = seen_p = false;
+                    const Desc vd = v_desc + v_slot * C::KV_BYTES;
+                    const uint32_t acc = o.j > 0;
+                    const bool look_k = s_on && s.first() && o.last();
+                    if constexpr (LOW) {
+                        constexpr uint32_t IDESC = make_idesc_tf32(TILE, HEAD_DIM, false, true);
+                        const uint32_t high = tmem + p.at * 64, low = tmem + LOW_COL_LOW + low_buf * 64, d = tmem + LOW_COL_O;
+                        auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
+                            umma_ts4<MNMAJOR_STEP>(leader, d, x, vd + y, IDESC, acc);
+                            umma_ts4<MNMAJOR_STEP>(leader, d, x + 32, vd + (y + 4096), IDESC, 1u);
+                        };
+                        eight(low, 0, 0u);
+                        eight(high, C::KV_RAW, 1u);
+                        seen_k = look_k && seen(look_at(tile, false));
+                        eight(high, 0, 1u);
+                        low_buf ^= 1;
+                    } else {
+                        constexpr uint32_t IDESC = make_idesc_16(TILE, HEAD_DIM, BF16, true);
+                        const uint32_t w = tmem + p.at * 128, d = tmem + COL_O + o.t * 64;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            if (k == 4) seen_k = look_k && seen(look_at(tile, false));
+                            umma_ts_16(leader, d, w + 8 * k, vd.d + (2048 >> 4) * k, IDESC, k > 0 ? 1u : acc);
+                        }
+                    }
+                    umma_commit_lead(leader, &sh.o_full[0][0] + after(o_own, o.t));
+                    if (o.last()) umma_commit_lead(leader, &sh.kv_empty[v_slot]);
+                    p.next(3);
+                    --ahead;
+                    if (!o.next()) {
+                        if (lane == 0) mbar_arrive(&sh.item_empty[o_item.at]);
+                        o_item.next(ITEMS);
+                        --between;
+                        if (ahead > 0 || s_on) next_item(o_item, o);
+                        if (!ok) break;
+                    }
+                }
+            }
+        } else if (LOW) {
+            tend(threadIdx.x & 63, 0);
+        } else if (warp == 2) {
+            tend(lane, 0);
+        } else {
+            // ------------------------------ queries of 16-bit types ------------------------------
+            Turn get{0, 0u};
+            for (int n = 0;; ++n) {
+                if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.item_full[get.at], get.phase, W_ITEM, n))) break;
+                const Item& it = sh.items[get.at];
+                const int rows = it.rows, row0 = it.row0, b = TREE ? it.b : 0, h0 = it.kvh * a.group, begin = it.begin;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.item_empty[get.at]);
+                get.next(ITEMS);
+                if (rows == 0) break;
+                const int buf = n & 1;
+                if (n >= 2 && !__all_sync(0xffffffffu, mbar_wait(wc, &sh.q_empty[buf], (n / 2 - 1) & 1, W_Q_EMPTY, n))) break;
+                uint8_t* to = sQ + buf * C::STREAMS * C::Q_BYTES;
+                const int c = lane & 7;
+                for (int r = lane >> 3; r < (rows > TILE ? 2 * TILE : TILE); r += 4) {  // in the layout of a K-major operand
+                    const int row = row0 + min(r, rows - 1), token = row / a.group;
+                    copy16(to + r * 128 + ((c ^ (r & 7)) << 4), row_of<X>(a.Q, b, h0 + row - token * a.group, begin + token) + 8 * c, r < rows);
+                }
+                asm volatile("cp.async.wait_all;\n" ::: "memory");
+                fence_proxy_async_smem();
+                mbar_arrive_warp(&sh.q_full[buf], lane);
+            }
+        }
+    } else if (LOW && warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;\n");
+        if (warp < 10) tend(threadIdx.x & 63, 1);
+    } else {
+        // ------------------------------ softmax ------------------------------
+        if constexpr (LOW) asm volatile("setmaxnreg.inc.sync.aligned.u32 240;\n");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+        const int t = (warp - 4) >> 2, quarter = warp & 3, r = t * TILE + quarter * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        const float2 scale2 = make_float2(a.scale_log2e, a.scale_log2e);
+        bool ok = true;
+        int q0 = 0, own = 0;  // products of the items before; the stream's own ones so far
+        auto wait = [&](uint64_t (&bar)[3], int c, int id) {  // of the stream's product c
+            ok = __all_sync(0xffffffffu, mbar_wait(wc, &bar[c % 3], (c / 3) & 1, id, c));
+            if (ok) tc_fence_after_sync();
+            return ok;
+        };
+        // fp32: the queries of item n to tensor memory, from where those before are read no longer
+        int fetched = 0;
+        Turn fetch{0, 0u};
+        auto fetch_queries = [&] {
+            if constexpr (LOW) {
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.item_full[fetch.at], fetch.phase, W_ITEM, fetched)))) return;
+                const int rows = sh.items[fetch.at].rows;
+                fetch.next(ITEMS);
+                if (rows == 0) return;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.q_full[0], fetched & 1, W_Q, fetched)))) return;
+                ++fetched;
+                const uint4* from = reinterpret_cast<const uint4*>(sQ + r * C::Q_ROW);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t y[32], z[32];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const uint4 v = r < rows ? from[8 * half + c] : make_uint4(0, 0, 0, 0);
+                        y[4 * c] = v.x ^ a.flip; y[4 * c + 1] = v.y ^ a.flip; y[4 * c + 2] = v.z ^ a.flip; y[4 * c + 3] = v.w ^ a.flip;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) z[i] = tf32_rest(y[i]);
+                    tmem_st32(lanes + LOW_COL_Q + 32 * half, y);
+                    tmem_st32(lanes + LOW_COL_Q + 64 + 32 * half, z);
+                }
+                tmem_wait_st();
+                tc_fence_before_sync();
+                mbar_arrive_warp(&sh.q_ready, lane);
+                mbar_arrive_warp(&sh.q_empty[0], lane);
+            }
+        };
+        fetch_queries();
+        Turn get{0, 0u};
+        while (ok) {
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.item_full[get.at], get.phase, W_ITEM, q0)))) break;
+            const Item& it = sh.items[get.at];
+            const int rows = it.rows, row0 = it.row0, n0 = it.n0, n1 = it.n1, slot = it.slot, begin = it.begin, b = TREE ? it.b : 0, h0 = it.kvh * a.group, key0 = it.key0, len = it.len;
+            const int new_tile = it.new_tile;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.item_empty[get.at]);
+            get.next(ITEMS);
+            if (rows == 0) break;
+            const bool valid = r < rows, live = t * TILE + quarter * 32 < rows;
+            const int token = (row0 + r) / a.group;
+            const int limit = !valid ? 0 : !TREE && a.causal ? token + 1 : len;  // keys the row sees
+            const uint64_t bits = TREE && valid ? tree_bits(a, b, token) : 0ull;
+            const int n = t == 0 ? n0 : n1;
+            auto product = [&](int j) { return q0 + min(j, n0) + min(j, n1) + (t == 1 && j < n0); };
+            float o[64], m = -INFINITY, l = 0.f;
+            if constexpr (LOW) {
+                // O_j of every tile comes back and is added here: o = o * before + O_j
+                float before = 0.f, alpha = 0.f;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) o[i] = 0.f;
+                auto add = [&](int j) {
+                    if (!wait(sh.o_full[0], q0 + j, W_O) || !live) return;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t x[32];
+                        tmem_ld32(lanes + LOW_COL_O + 32 * half, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float2& y = reinterpret_cast<float2&>(o[32 * half + i]);
+                            y = __ffma2_rn(y, make_float2(before, before), make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+                        }
+                    }
+                };
+                for (int j = 0; j < n && wait(sh.s_full[0], q0 + j, W_S); ++j) {
+                    if (j == n - 1) {  // all scores of this item are there
+                        fetch_queries();
+                        if (!ok) break;
+                    }
+                    const int q = q0 + j;
+                    const uint32_t at_s = lanes + q % 3 * 64, at_low = lanes + LOW_COL_LOW + (q & 1) * 64;
+                    if (live) {
+                        const int lim = TREE && j == new_tile ? KEYS : limit - key0 - j * KEYS;  // columns the row sees
+                        uint32_t x[64];
+                        tmem_ld32p(at_s, x);
+                        tmem_ld32p(at_s + 32, x + 32);
+                        tmem_wait_ld();
+                        if (TREE && j == new_tile) {
+#pragma unroll
+                            for (int i = 0; i < 64; ++i)
+                                if (!(bits >> i & 1)) x[i] = __float_as_uint(-INFINITY);
+                        } else if (lim < KEYS) {
+#pragma unroll
+                            for (int i = 0; i < 64; ++i)
+                                if (i >= lim) x[i] = __float_as_uint(-INFINITY);
+                        }
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int i = 0; i < 64; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                        const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e), ref = mn == -INFINITY ? 0.f : mn;
+                        alpha = ex2_approx(m - ref);  // 0 while m is -inf
+                        m = mn;
+                        const float2 nm = make_float2(-ref, -ref);
+                        float2 sum[2] = {};
+#pragma unroll
+                        for (int c = 0; c < 64; c += 32) {
+                            uint32_t z[32];
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[c + i]), __uint_as_float(x[c + i + 1])), scale2, nm);
+                                const float2 w = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                                sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
+                                x[c + i] = __float_as_uint(w.x);
+                                x[c + i + 1] = __float_as_uint(w.y);
+                                z[i] = __float_as_uint(w.x - __uint_as_float(x[c + i] & 0xffffe000u));
+                                z[i + 1] = __float_as_uint(w.y - __uint_as_float(x[c + i + 1] & 0xffffe000u));
+                            }
+                            tmem_st32p(at_s + c, x + c);
+                            tmem_st32(at_low + c, z);
+                        }
+                        l = fmaf(l, alpha, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                        tmem_wait_st();
+                    }
+                    if (j > 0) add(j - 1);  // before O_j may come to the same place
+                    if (!ok) break;
+                    tc_fence_before_sync();
+                    mbar_arrive_warp(&sh.p_full[q % 3], lane);
+                    before = alpha;
+                }
+                if (ok) add(n - 1);
+            } else {
+                // O stays in tensor memory and is scaled there when a tile's weights come to more than MOST: a stale maximum makes them larger,
+                // which neither fp32 sums nor 16-bit types mind up to there
+                constexpr float MOST = lift<X>() > 0.f ? 32768.f : 256.f;  // 2^8 of the reference's own weight
+                constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial
+                const uint32_t at_o = lanes + COL_O + t * 64;
+                uint32_t x[128];
+                for (int j = 0; j < n && wait(sh.s_full[t], own, W_S); ++j, ++own) {
+                    const int q = product(j);
+                    const uint32_t at_s = lanes + q % 3 * 128;
+                    if (live) {
+                        const bool fresh = TREE && j == new_tile;
+                        const int lim = fresh ? 0 : limit - key0 - j * KEYS;  // columns the row sees
+                        auto load = [&] {
+#pragma unroll
+                            for (int c = 0; c < 128; c += 32) tmem_ld32p(at_s + c, x + c);
+                            tmem_wait_ld();
+                        };
+                        float2 sum[2];
+                        // The weights take the type of the values: half a step of it each.  A run of them is summed and packed while the next
+                        // one's exponentials are under way.
+                        auto weights = [&](auto poly) {
+                            constexpr int RUN = 16;
+                            const float up = m == -INFINITY ? 0.f : lift<X>() - m;
+                            const float2 nm = make_float2(up, up);
+                            sum[0] = sum[1] = make_float2(0.f, 0.f);
+#pragma unroll
+                            for (int c = 0; c < 128 + RUN; c += RUN) {
+#pragma unroll
+                                for (int i = c; i < c + RUN && i < 128; i += 2) {
+                                    const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, nm);
+                                    const float2 w = decltype(poly)::value && (i >> 1) % POLY_OF == POLY_OF - 1 ? ex2_poly(e) : make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                                    x[i] = __float_as_uint(w.x);
+                                    x[i + 1] = __float_as_uint(w.y);
+                                }
+#pragma unroll
+                                for (int i = c - RUN; i >= 0 && i < c; i += 2) {
+                                    const float2 w = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                                    sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
+                                    x[i / 2] = pack<X>(w.x, w.y);
+                                }
+                            }
+                            return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                        };
+                        load();
+                        // Most tiles raise no maximum by much: their weights are taken by the one there is, and their sum tells if it was too
+                        // low.  Then, and where keys are masked, the maximum is sought first.  The polynomial would make small numbers of a large
+                        // argument and of a NaN.
+                        float alpha = 1.f, add = 0.f;
+                        bool done = false;
+                        if (__all_sync(0xffffffffu, lim >= KEYS && m > -INFINITY)) {
+                            float poly_top = -INFINITY;
+#pragma unroll
+                            for (int i = 2 * (POLY_OF - 1); i < 128; i += 2 * POLY_OF) poly_top = max3_or_nan(poly_top, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                            add = weights(std::true_type{});
+                            done = __all_sync(0xffffffffu, add <= MOST && fmaf(poly_top, a.scale_log2e, -m) <= 8.f);
+                            if (!done) load();
+                        }
+                        if (!done) {
+                            if (fresh) {
+#pragma unroll
+                                for (int i = 0; i < 128; ++i)
+                                    if (i >= 64 || !(bits >> (i & 63) & 1)) x[i] = __float_as_uint(-INFINITY);
+                            } else if (lim < KEYS) {
+#pragma unroll
+                                for (int i = 0; i < 128; ++i)
+                                    if (i >= lim) x[i] = __float_as_uint(-INFINITY);
+                            }
+                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                            for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e;
+                            const bool raise = top > m;
+                            if (raise) {
+                                alpha = ex2_approx(m - top);  // 0 from -inf
+                                m = top;
+                            }
+                            if (j > 0 && __any_sync(0xffffffffu, raise)) {
+                                if (!wait(sh.o_full[t], own - 1, W_O)) break;
+#pragma unroll 1
+                                for (int c = 0; c < 64; c += 32) {
+                                    uint32_t y[32];
+                                    tmem_ld32(at_o + c, y);
+                                    tmem_wait_ld();
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+                                    tmem_st32(at_o + c, y);
+                                }
+                            }
+                            add = weights(std::false_type{});
+                        }
+                        tmem_st32p(at_s, x);
+                        tmem_st32p(at_s + 32, x + 32);
+                        l = fmaf(l, alpha, add);
+                        tmem_wait_st();
+                    }
+                    tc_fence_before_sync();
+                    mbar_arrive_warp(&sh.p_full[q % 3], lane);
+                }
+                m -= lift<X>();  // what the weights were taken by
+#pragma unroll
+                for (int i = 0; i < 64; ++i) o[i] = 0.f;
+                if (ok && n > 0 && wait(sh.o_full[t], own - 1, W_O) && live) {
+                    tmem_ld32p(at_o, reinterpret_cast<uint32_t*>(o));
+                    tmem_ld32p(at_o + 32, reinterpret_cast<uint32_t*>(o) + 32);
+                    tmem_wait_ld();
+                    tc_fence_before_sync();
+                }
+            }
+            q0 += n0 + n1;
+            if (!ok) break;
+            if (valid) {
+                if (slot >= 0) {
+                    const int64_t at_slot = (int64_t)slot * C::BLOCK + r;
+                    a.ml[at_slot] = make_float2(m, l);
+                    float4* to = reinterpret_cast<float4*>(a.part + at_slot * 64);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                } else {
+                    const float f = l != 0.f ? 1.f / l : 0.f;
+                    const int h = h0 + row0 + r - token * a.group, row = begin + token;
+                    uint4* to = reinterpret_cast<uint4*>(const_cast<X*>(row_of<X>(a.O, b, h, row)));
+                    if constexpr (LOW) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            to[i] = make_uint4(__float_as_uint(o[4 * i] * f), __float_as_uint(o[4 * i + 1] * f), __float_as_uint(o[4 * i + 2] * f), __float_as_uint(o[4 * i + 3] * f));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            to[i] = make_uint4(pack<X>(o[8 * i] * f, o[8 * i + 1] * f), pack<X>(o[8 * i + 2] * f, o[8 * i + 3] * f),
+                                               pack<X>(o[8 * i + 4] * f, o[8 * i + 5] * f), pack<X>(o[8 * i + 6] * f, o[8 * i + 7] * f));
+                    }
+                    a.LSE[b * a.lse_sB + h * a.lse_sH + row] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+                }
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+        if (lane == 0) report_abort(sh.abort, a.status);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The parts of each block that fell to several CTAs, added up in their order: 16 lanes a row, four elements a lane.  The block begins in the
+// second slot of one CTA and goes on in the first ones of those behind it.
+// ---------------------------------------------------------------------------
+template <class X, int BLOCK>
+__global__ void __launch_bounds__(256) serving_combine_kernel(const __grid_constant__ ServingArgs a, const int ctas) {
+    pdl_wait();
+    pdl_trigger();
+    const PartRecord rec = a.parts[blockIdx.x];
+    const int sub = threadIdx.x & 15, r0 = blockIdx.y * 64;
+    if (r0 >= rec.rows) return;
+    int last = blockIdx.x;  // the CTA that has the last part
+    while (++last < ctas - 1) {
+        const int head = a.parts[last].head;
+        if (head != PART_GOES_ON && head != PART_EMPTY) break;
+    }
+    const int n = last - (int)blockIdx.x + 1;
+    const uint32_t together = threadIdx.x & 16 ? 0xffff0000u : 0xffffu;
+    for (int r = r0 + (int)threadIdx.x / 16; r < min(rec.rows, r0 + 64); r += 16) {
+        float M = -INFINITY, L = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p0 = 0; p0 < n; p0 += 16) {
+            // a lane looks up one part
+            const int cta = blockIdx.x + p0 + sub;
+            const bool there = p0 + sub < n && (p0 + sub == 0 || a.parts[cta].head == PART_GOES_ON || a.parts[cta].head == PART_LAST);
+            const int slot = 2 * cta + (p0 + sub == 0);
+            const float2 x = there ? a.ml[(int64_t)slot * BLOCK + r] : make_float2(-INFINITY, 0.f);
+            float mx = x.x;
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(together, mx, off));
+            mx = fmaxf(mx, M);
+            const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(M - ref), w = there && x.y != 0.f ? ex2_approx(x.x - ref) : 0.f;
+            M = mx;
+            float sum = x.y * w;
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(together, sum, off);
+            L = L * old + sum;
+            o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+            for (int i = 0; i < min(16, n - p0); i += 4) {
+                float4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int from = __shfl_sync(together, slot, i + k, 16), is = __shfl_sync(together, (int)there, i + k, 16);
+                    v[k] = is ? *reinterpret_cast<const float4*>(a.part + ((int64_t)from * BLOCK + r) * 64 + 4 * sub) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float f = __shfl_sync(together, w, i + k, 16);
+                    o.x = fmaf(v[k].x, f, o.x); o.y = fmaf(v[k].y, f, o.y); o.z = fmaf(v[k].z, f, o.z); o.w = fmaf(v[k].w, f, o.w);
+                }
+            }
+        }
+        const float f = L != 0.f ? 1.f / L : 0.f;
+        const int token = (rec.row0 + r) / a.group, h = rec.kvh * a.group + rec.row0 + r - token * a.group, row = rec.begin + token;
+        store4(const_cast<X*>(row_of<X>(a.O, rec.b, h, row)) + 4 * sub, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+        if (sub == 0) a.LSE[rec.b * a.lse_sB + h * a.lse_sH + row] = L != 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
+    }
+}
+
+// Boxes of `rows` rows of a page, 128 bytes of each
+int page_map(CUtensorMap* map, const hk_view& v, int dtype, int n_pages, int H, int page, int rows, bool mn_major) {
+    EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return HK_ERR_CUDA;
+    const int e = esize(dtype), inner = 128 / e;
+    const int64_t sM = v.strideM, sH = H == 1 ? sM * page : v.strideH, sB = n_pages == 1 ? std::max(sH * H, sM * page) : v.strideB;
+    cuuint64_t dims[5] = {(cuuint64_t)inner, (cuuint64_t)page, (cuuint64_t)(64 / inner), (cuuint64_t)H, (cuuint64_t)n_pages};
+    cuuint64_t strides[4] = {(cuuint64_t)sM * e, 128, (cuuint64_t)sH * e, (cuuint64_t)sB * e};
+    cuuint32_t box[5] = {(cuuint32_t)inner, (cuuint32_t)rows, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+    const CUtensorMapDataType type = dtype == HK_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == HK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult r = enc(map, type, 5, v.ptr, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, mn_major ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HK_OK : HK_ERR_CUDA;
+}
+
+template <class X, bool TREE>
+int launch(ServingArgs a, int dtype, cudaStream_t stream) {
+    typedef Rows<X> C;
+    static std::once_flag once[HK_MAX_DEVICES];
+    static cudaError_t rc[HK_MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
+    std::call_once(once[dev], [dev] { rc[dev] = cudaFuncSetAttribute(serving_rows_kernel<X, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSpace<X>::SMEM); });
+    if (rc[dev] != cudaSuccess) return HK_ERR_CUDA;
+    CUtensorMap k, v, kp, vp;
+    const int B = TREE ? a.B : 1;
+    const int64_t T = TREE ? a.T : a.N;
+    int s;
+    if ((s = prefix_tile_map(&k, a.K, dtype, B, a.Hk, T, C::KEYS, false)) || (s = prefix_tile_map(&v, a.V, dtype, B, a.Hk, T, C::KEYS, true))) return s;
+    kp = k;
+    vp = v;
+    if (TREE) {
+        a.box = std::gcd(a.pool.page, C::KEYS);
+        if ((s = page_map(&kp, a.pool.K, dtype, a.pool.n_pages, a.Hk, a.pool.page, a.box, false)) ||
+            (s = page_map(&vp, a.pool.V, dtype, a.pool.n_pages, a.Hk, a.pool.page, a.box, C::LOW)))
+            return s;
+    }
+    const int ctas = sm_count();
+    LaunchConfig lc(ctas, C::THREADS, RowsSpace<X>::SMEM, stream, 1, true);
+    if (cudaLaunchKernelEx(&lc.cfg, serving_rows_kernel<X, TREE>, k, v, kp, vp, a) != cudaSuccess) return check_launch();
+    count_launch();
+    if (!a.parts) return HK_OK;
+    LaunchConfig sum(ctas, 256, 0, stream, 1, true);
+    sum.cfg.gridDim.y = C::BLOCK / 64;
+    if (cudaLaunchKernelEx(&sum.cfg, serving_combine_kernel<X, C::BLOCK>, a, ctas) != cudaSuccess) return check_launch();
+    count_launch();
+    return HK_OK;
+}
+template <bool TREE>
+int launch(const ServingArgs& a, int dtype, cudaStream_t stream) {
+    return dtype == HK_F32 ? launch<float, TREE>(a, dtype, stream) : dtype == HK_BF16 ? launch<__nv_bfloat16, TREE>(a, dtype, stream) : launch<__half, TREE>(a, dtype, stream);
+}
+
+}  // namespace
+
+RowsPlan rows_plan(int dtype) { return dtype == HK_F32 ? RowsPlan{Rows<float>::BLOCK, Rows<float>::KEYS, Rows<float>::LEAST} : RowsPlan{Rows<__half>::BLOCK, Rows<__half>::KEYS, Rows<__half>::LEAST}; }
+int launch_prompt_rows(const ServingArgs& a, int dtype, cudaStream_t stream) { return launch<false>(a, dtype, stream); }
+int launch_tree_rows(const ServingArgs& a, int dtype, cudaStream_t stream) { return launch<true>(a, dtype, stream); }
+
+}  // namespace hk

@@ -3,7 +3,7 @@
 
 #include <type_traits>
 
-#include "operators.cuh"
+#include "tile_math.cuh"
 
 namespace hk {
 
@@ -42,22 +42,6 @@ struct PrefixArgs {
 __device__ __forceinline__ int request_keys(const PrefixArgs& a, int b) { return a.lengths ? min(max(__ldcg(a.lengths + b), 0), a.S) : a.S; }
 // own keys that token t of a request of `len` keys sees
 __device__ __forceinline__ int token_keys(const PrefixArgs& a, int len, int t) { return a.causal ? min(len, max(0, len - a.T + t + 1)) : len; }
-
-// The 2^ of what a softmax's reference lies below the row's largest score.  A weight takes the type of the values, and fp16 has none below
-// 2^-24: with the largest at 2^7 (2^15 where a stale maximum may lie 2^8 lower), those down to 2^-31 of it are kept, where many of
-// them would be lost beside one that is large.  The sums and the LSE take it back by themselves.
-template <class X>
-__host__ __device__ constexpr float lift() { return std::is_same<X, __half>::value ? 7.f : 0.f; }
-
-template <class X>
-__device__ __forceinline__ void store4(X* p, float4 v) {
-    if constexpr (sizeof(X) == 4) *reinterpret_cast<float4*>(p) = v;
-    else *reinterpret_cast<uint2*>(p) = make_uint2(pack<X>(v.x, v.y), pack<X>(v.z, v.w));
-}
-
-// Tiles of `rows` rows of a view of keys or values, all heads and batches (tma_load_tile): 128 bytes of each row side by side,
-// swizzled; fp32 rows are two such pieces.  mn_major: the values as an MN-major operand of fp32 products.
-int prefix_tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, int rows, bool mn_major);
 
 // Launchers.  The kernel over the requests' own keys runs beside the one over the prefix, if that is launched just before it; it does
 // not wait for it, so a launch that does has to follow (there are slots to add up then).

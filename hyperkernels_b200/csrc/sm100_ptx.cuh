@@ -188,6 +188,15 @@ __device__ __forceinline__ void tma_load_tile(void* smem_dst, const CUtensorMap*
         : "memory");
 }
 
+// Boxes of 128 bytes x box_rows of slice (b, h): piece `x` of each row's 128-byte pieces.
+__device__ __forceinline__ void tma_load_box(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int row, int x, int h, int b) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(x), "r"(h), "r"(b)
+        : "memory");
+}
+
 // Tile reduction, shared -> global: global[tile] += shared tile (fp32 add performed by the
 // memory system).  Rows of the box that lie outside the tensor are skipped.  Completion is tracked
 // by the issuing thread's bulk async-group.  The shared-memory tile must have been written, and
