@@ -101,8 +101,8 @@ int check_heads(int64_t B, int nh, int nh_kv, int dtype, float scale) {
     if (!std::isfinite(scale) || scale == 0.f) return HK_ERR_BAD_SHAPE;
     return HK_OK;
 }
-// Keys and values: tensor maps do not know a stride of 0
-int check_keys(const hk_view& v, int64_t B, int H, int64_t T, int dtype) {
+// What is read by TMA: tensor maps do not know a stride of 0
+int check_read(const hk_view& v, int64_t B, int H, int64_t T, int dtype) {
     const int rc = check_view(v, B, H, T, dtype, false);
     if (rc != HK_OK) return rc;
     return (B == 1 || v.strideB > 0) && (H == 1 || v.strideH > 0) && (T == 1 || v.strideM > 0) ? HK_OK : HK_ERR_UNSUPPORTED;
@@ -159,8 +159,8 @@ size_t hk_prompt_workspace_bytes(const hk_prompt_params* p) { return check_sizes
 int hk_prompt_attention(const hk_prompt_params* p, void* stream) {
     int rc = check_sizes(p);
     if (rc != HK_OK) return rc;
-    if ((rc = check_view(p->Q, 1, p->nh, p->N, p->dtype, false)) || (rc = check_keys(p->K, 1, p->nh_kv, p->N, p->dtype)) ||
-        (rc = check_keys(p->V, 1, p->nh_kv, p->N, p->dtype)) || (rc = check_view(p->O, 1, p->nh, p->N, p->dtype, true)))
+    if ((rc = check_read(p->Q, 1, p->nh, p->N, p->dtype)) || (rc = check_read(p->K, 1, p->nh_kv, p->N, p->dtype)) ||
+        (rc = check_read(p->V, 1, p->nh_kv, p->N, p->dtype)) || (rc = check_view(p->O, 1, p->nh, p->N, p->dtype, true)))
         return rc;
     if (!p->LSE || !p->starts) return HK_ERR_NULL_POINTER;
     if (odd(p->LSE, 4) || odd(p->starts, 4)) return HK_ERR_MISALIGNED;
@@ -182,10 +182,10 @@ size_t hk_tree_workspace_bytes(const hk_tree_params* p) {
 int hk_tree_attention(const hk_tree_params* p, void* stream) {
     int rc = check_sizes(p);
     if (rc != HK_OK) return rc;
-    if ((rc = check_view(p->Q, p->B, p->nh, p->T, p->dtype, false)) || (rc = check_keys(p->K, p->B, p->nh_kv, p->T, p->dtype)) ||
-        (rc = check_keys(p->V, p->B, p->nh_kv, p->T, p->dtype)) || (rc = check_view(p->O, p->B, p->nh, p->T, p->dtype, true)) ||
-        (rc = check_pool(p->pool, p->B, p->nh_kv, p->dtype, false)) || (rc = check_keys(p->pool.K, p->pool.n_pages, p->nh_kv, p->pool.page, p->dtype)) ||
-        (rc = check_keys(p->pool.V, p->pool.n_pages, p->nh_kv, p->pool.page, p->dtype)))
+    if ((rc = check_read(p->Q, p->B, p->nh, p->T, p->dtype)) || (rc = check_read(p->K, p->B, p->nh_kv, p->T, p->dtype)) ||
+        (rc = check_read(p->V, p->B, p->nh_kv, p->T, p->dtype)) || (rc = check_view(p->O, p->B, p->nh, p->T, p->dtype, true)) ||
+        (rc = check_pool(p->pool, p->B, p->nh_kv, p->dtype, false)) || (rc = check_read(p->pool.K, p->pool.n_pages, p->nh_kv, p->pool.page, p->dtype)) ||
+        (rc = check_read(p->pool.V, p->pool.n_pages, p->nh_kv, p->pool.page, p->dtype)))
         return rc;
     if (!p->LSE || !p->lengths) return HK_ERR_NULL_POINTER;
     if (odd(p->LSE, 4) || odd(p->lengths, 4) || odd(p->tree, 8)) return HK_ERR_MISALIGNED;

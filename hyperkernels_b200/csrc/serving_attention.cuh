@@ -7,11 +7,11 @@
 namespace hk {
 
 // What a CTA of the kernel of many rows has of blocks that fell to several: how the first one goes on that it has not begun itself, and the
-// one that it has begun and not ended (rows 0: none).
+// one that it has begun and not ended (no tokens: none).
 enum PartHead { PART_NONE, PART_LAST, PART_GOES_ON, PART_EMPTY /* nothing of any block */ };
 struct PartRecord {
     int head;
-    int b, kvh, begin, row0, rows;
+    int b, head0, heads, token0, tokens;
 };
 
 struct ServingArgs {
@@ -28,6 +28,11 @@ struct ServingArgs {
     float scale_log2e;  // its size; a negative scale turns the queries' signs (flip)
     uint32_t flip;
     int causal;
+    // kernel of many rows: tokens of a stream and of a block, 128s of query heads, bytes of a stream's queries; x / block_tokens is x *
+    // block_mul >> block_shift for x below 2^31
+    int stream_tokens, block_tokens, chunks, q_bytes;
+    uint32_t block_mul;
+    int block_shift;
     int box;            // rows of a page that are loaded at once
     // slots of the workspace, and who has what in them; no parts: blocks are not cut
     float2* ml;         // [slots][rows]

@@ -1,8 +1,9 @@
 // serving_sm100.cu -- attention within packed prompts, and of many new tokens against a cache of pages: blocks of 128 rows (fp32) or 256
 // (16-bit types: two streams of 128) against tiles of keys, on tcgen05.
 //
-// A row is a token under one of the query heads that share a key head; rows of a block follow each other (token by token, its heads
-// side by side), so a key is loaded once for all of them.  Lengths are on the device, so the work is cut there: block by block, head by
+// A row is a token under one of the query heads that share a key head; 128 rows of a block are as many whole tokens as fit, their heads
+// side by side (of more than 128 heads, each 128 are blocks of their own), so TMA brings the queries of a stream in one copy and a key is
+// loaded once for all of them.  Lengths are on the device, so the work is cut there: block by block, head by
 // head, request by request the tiles of keys make one line, of which every CTA takes an equal stretch.  A block of rows whose tiles fall to
 // several CTAs leaves its parts (maximum, sum, weighted values) in slots of the workspace, a pair to a CTA, and a second kernel adds
 // them up in their order.
@@ -14,6 +15,7 @@
 //   fp32: x = h + l with h the upper 11 bits of the significand, which is what the tensor core reads of an fp32 word.  Q lies in tensor memory
 // with its l parts, four warps write those of each tile beside it; a product is l h' + h l' + h h', in this order: what is left out is 2^-22 of it.  P V of
 // a tile comes back into registers and is added there in fp32: the tensor core's additions cut off instead of rounding.
+#include <climits>
 #include <cmath>
 #include <mutex>
 #include <numeric>
@@ -35,18 +37,18 @@ struct Rows {
     static constexpr int LEAST = LOW ? 4 : 2;    // tiles of a part of a block
     static constexpr int KV_RAW = KEYS * 64 * (int)sizeof(X), KV_BYTES = KV_RAW * (LOW ? 2 : 1);
     static constexpr int KV_BOX = KEYS * 128;    // 128 bytes of each row
-    // queries: 16-bit types as K-major operands, two items deep; fp32 on their way to tensor memory, rows apart for the banks
-    static constexpr int Q_ROW = LOW ? 272 : 128, Q_BYTES = TILE * Q_ROW, Q_BUFFERS = LOW ? 1 : 2;
+    static constexpr int Q_BYTES = TILE * 64 * (int)sizeof(X), Q_BUFFERS = LOW ? 1 : 2;  // of a stream: K-major operands two items deep; fp32: on their way to tensor memory
     static constexpr int ITEMS = 8;
 };
 
 struct Item {
-    int b, kvh, row0, rows;  // request, key head, the block's first row among the request's and how many there are; 0: the end
-    int begin, len;          // of the packed rows; keys of the sequence, or in pages
-    int key0;                // of the first tile
-    int tiles, n0, n1;       // tiles of the item, and of each of its streams
-    int slot;                // of the workspace, -1: the result
-    int new_tile;            // number of the tile that is the new tokens'
+    int b, kvh, chunk;   // request, key head, which 128 of its query heads
+    int token0, tokens;  // of the request; no tokens: the end
+    int begin, len;      // of the packed rows; keys of the sequence, or in pages
+    int key0;            // of the first tile
+    int n0, n1;          // tiles of each stream
+    int slot;            // of the workspace, -1: the result
+    int new_tile;        // number of the tile that is the new tokens'
 };
 
 template <class X>
@@ -76,52 +78,42 @@ constexpr uint32_t COL_O = 384, LOW_COL_LOW = 192, LOW_COL_O = 320, LOW_COL_Q = 
 enum RowsWait { W_Q = 501, W_Q_EMPTY, W_KV, W_READY, W_EMPTY, W_S, W_P, W_O, W_ITEM, W_ITEM_EMPTY };
 
 // ---------------------------------------------------------------------------
-// How the work is cut.  Block i of a request's rows meets n(i) tiles of keys, and counts as n(i) + 1.
+// How the work is cut: a block counts as the keys that it meets and EXTRA for its beginning and end.
 // ---------------------------------------------------------------------------
-// The scores of block i (rows i * BLOCK .., tokens of `group` rows) end, under the causal mask, in tile ceil(2 (i + 1) / group): both
-// types' blocks have twice as many rows as their tiles have keys.
 struct Request {
-    int begin, len, rows, blocks;
-    int64_t units;  // of all of its blocks, under one key head
+    int begin, len, tokens, blocks;  // blocks: of tokens
+    int64_t units;                   // of all of its blocks, under one key head
 };
 template <class X, bool TREE>
 struct Work {
     typedef Rows<X> C;
-    static_assert(C::BLOCK == 2 * C::KEYS, "tiles up to the diagonal");
+    static constexpr int EXTRA = C::KEYS * 3 / 2;  // half a tile is masked
     const ServingArgs& a;
+    __device__ __forceinline__ int all_tiles(const Request& r) const { return (r.len + C::KEYS - 1) / C::KEYS + TREE; }
     __device__ __forceinline__ int tiles(const Request& r, int i) const {
-        if (TREE) return (r.len + C::KEYS - 1) / C::KEYS + 1;
-        return !a.causal || i == r.blocks - 1 ? (r.len + C::KEYS - 1) / C::KEYS : (2 * (i + 1) + a.group - 1) / a.group;
+        return TREE || !a.causal ? all_tiles(r) : (min((i + 1) * a.block_tokens, r.len) + C::KEYS - 1) / C::KEYS;
     }
-    // units in front of block i
+    __device__ __forceinline__ int64_t units(const Request& r, int i) const { return (TREE || !a.causal ? all_tiles(r) * C::KEYS : (i + 1) * a.block_tokens) + EXTRA; }
+    // units in front of block i, of one chunk of heads
     __device__ __forceinline__ int64_t before(const Request& r, int i) const {
-        if (TREE || !a.causal) return (int64_t)i * (tiles(r, 0) + 1);
-        // the sum of ceil(2 k / group) for k = 1 .. i: every `group` of them come to `turn`, and each time 2 more apiece
-        const int q = i / a.group, rest = i - q * a.group, half = a.group / 2, turn = 2 * a.group - half;
-        return (int64_t)q * turn + (int64_t)a.group * q * (q - 1) + (int64_t)rest * 2 * q + rest + max(0, rest - half) + i;
+        if (TREE || !a.causal) return i * units(r, 0);
+        return (int64_t)i * (i + 1) / 2 * a.block_tokens + (int64_t)i * EXTRA;
     }
     __device__ __forceinline__ Request request(int b) const {
         Request r;
         if (TREE) {
             r.begin = 0;
             r.len = cache_keys(a, b);
-            r.rows = a.T * a.group;
+            r.tokens = a.T;
         } else {
             r.begin = min(max(a.starts[b], 0), a.N);
-            r.len = max(0, min(max(a.starts[b + 1], 0), a.N) - r.begin);
-            r.rows = r.len * a.group;
+            r.len = r.tokens = max(0, min(max(a.starts[b + 1], 0), a.N) - r.begin);
         }
-        r.blocks = (r.rows + C::BLOCK - 1) / C::BLOCK;
-        r.units = r.blocks ? before(r, r.blocks - 1) + tiles(r, r.blocks - 1) + 1 : 0;
+        r.blocks = (int)(((uint64_t)(uint32_t)(r.tokens + a.block_tokens - 1) * a.block_mul) >> a.block_shift);
+        r.units = before(r, r.blocks) * a.chunks;
         return r;
     }
 };
-// A place in the line of tiles: tile j of block i (j = the block's tiles: behind it)
-struct Place {
-    int b, kvh, i, j;
-    __device__ __forceinline__ bool operator==(const Place& x) const { return b == x.b && kvh == x.kvh && i == x.i; }
-};
-
 __device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -131,86 +123,88 @@ __device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
     return x;
 }
 
-// The stretch of this CTA, [from, to), by one warp; false: there is none.  A border inside a block is moved to its beginning or end
-// where a part of less than LEAST tiles would be left.
+// Where this CTA's stretch of the line begins: in block i of request b under key head kvh (blocks of the first chunk of heads, of the
+// second, ..), `done` units behind the block's beginning; and how many units it has from there.
+struct Stretch {
+    Request r;
+    int b, kvh, chunk, i;
+    int64_t done, units;
+};
+// By one warp; no units: there is nothing for this CTA.
 template <class X, bool TREE>
-__device__ bool find_stretch(const ServingArgs& a, int lane, Place& from, Place& to) {
+__device__ __forceinline__ Stretch find_stretch(const ServingArgs& a, int lane) {
     typedef Rows<X> C;
     const Work<X, TREE> work{a};
-    constexpr int EACH = 4;  // requests of a lane
-    int64_t all = 0, blocks = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
-        int64_t units = 0, n = 0;
+    constexpr int EACH = 2;  // requests of a lane
+    Stretch s = {};
+    int64_t units[EACH], sum = 0, all = 0;
+    int blocks = 0;
+    auto take = [&](int b0) {
+        sum = 0;
 #pragma unroll
         for (int k = 0; k < EACH; ++k) {
             const int b = b0 + lane * EACH + k;
-            if (b >= a.B) break;
-            const Request r = work.request(b);
-            units += r.units;
-            n += r.blocks;
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) {
-            units += __shfl_xor_sync(0xffffffffu, units, off);
-            n += __shfl_xor_sync(0xffffffffu, n, off);
-        }
-        all += units;
-        blocks += n;
-    }
-    all *= a.Hk;
-    blocks *= a.Hk;
-    // A CTA to a block, more if the blocks are long, as many as there are
-    const int64_t ctas = min((int64_t)gridDim.x, max(blocks, all / (3 * C::LEAST)));
-    const int64_t me = blockIdx.x;
-    if (me >= ctas) return false;
-    const int64_t at[2] = {me * all / ctas, (me + 1) * all / ctas};
-    Place place[2];
-    bool found[2] = {false, false};
-    int64_t run = 0;
-    for (int b0 = 0; b0 < a.B && !(found[0] && found[1]); b0 += 32 * EACH) {
-        int64_t units[EACH], sum = 0;
-#pragma unroll
-        for (int k = 0; k < EACH; ++k) {
-            const int b = b0 + lane * EACH + k;
-            units[k] = b < a.B ? work.request(b).units * a.Hk : 0;
+            units[k] = 0;
+            if (b < a.B) {
+                const Request r = work.request(b);
+                units[k] = r.units;
+                blocks += r.blocks * a.chunks;
+            }
             sum += units[k];
         }
-        const int64_t upto = run + warp_scan(sum, lane);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const unsigned here = __ballot_sync(0xffffffffu, at[x] < upto);
-            if (found[x] || !here) continue;
-            const int l = __ffs(here) - 1;
-            int64_t left = at[x] - (upto - sum);
-            int k = 0;
-#pragma unroll
-            for (int m = 0; m < EACH - 1; ++m)
-                if (k == m && left >= units[m]) left -= units[m], ++k;
-            left = __shfl_sync(0xffffffffu, left, l);
-            const int b = b0 + l * EACH + __shfl_sync(0xffffffffu, k, l);
-            const Request r = work.request(b);
-            Place& p = place[x];
-            p.b = b;
-            p.kvh = (int)(left / r.units);
-            left -= p.kvh * r.units;
-            int lo = 0, len = r.blocks;  // the last block that begins at or before it
-            while (len > 1) {
-                const int step = (len + 31) / 32;
-                const int c = __popc(__ballot_sync(0xffffffffu, lane * step < len && work.before(r, lo + lane * step) <= left));
-                lo += (c - 1) * step;
-                len = min(step, len - (c - 1) * step);
-            }
-            p.i = lo;
-            const int n = work.tiles(r, lo), j = (int)(left - work.before(r, lo));
-            p.j = j < C::LEAST ? 0 : n - j < C::LEAST ? n : j;
-            found[x] = true;
-        }
-        run = __shfl_sync(0xffffffffu, upto, 31);
+        return warp_scan(sum, lane);
+    };
+    int64_t upto = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
+        upto = take(b0);
+        all += __shfl_sync(0xffffffffu, upto, 31);
     }
-    from = place[0];
-    to = place[1];
-    if (!found[1]) to = {a.B, 0, 0, 0};
-    return true;
+    all *= a.Hk;
+    // A CTA to a block, more if the blocks are long, as many as there are
+    const int64_t n_blocks = (int64_t)__reduce_add_sync(0xffffffffu, blocks) * a.Hk;
+    const int ctas = (int)min((int64_t)gridDim.x, max(n_blocks, all / (3 * C::LEAST * C::KEYS)));
+    const int me = blockIdx.x;
+    if (me >= ctas) return s;
+    const int64_t share = all / ctas;
+    const int more = (int)(all - share * ctas);
+    int64_t left = me * share + min(me, more);
+    s.units = share + (me < more);
+    for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
+        if (a.B > 32 * EACH) upto = take(b0);  // otherwise they are here still
+        const unsigned here = __ballot_sync(0xffffffffu, left < upto * a.Hk);
+        if (!here) {
+            left -= __shfl_sync(0xffffffffu, upto, 31) * a.Hk;
+            continue;
+        }
+        const int l = __ffs(here) - 1;
+        left -= (upto - sum) * a.Hk;
+        int k = 0;
+#pragma unroll
+        for (int m = 0; m < EACH - 1; ++m)
+            if (k == m && left >= units[m] * a.Hk) left -= units[m] * a.Hk, ++k;
+        left = __shfl_sync(0xffffffffu, left, l);
+        s.b = b0 + l * EACH + __shfl_sync(0xffffffffu, k, l);
+        break;
+    }
+    s.r = work.request(s.b);
+    s.kvh = (int)((uint64_t)left / (uint64_t)s.r.units);
+    left -= s.kvh * s.r.units;
+    s.chunk = 0;
+    if (a.chunks > 1) {
+        const int64_t one = s.r.units / a.chunks;
+        s.chunk = (int)(left / one);
+        left -= s.chunk * one;
+    }
+    int lo = 0, len = s.r.blocks;  // the last block that begins at or before it
+    while (len > 1) {
+        const int step = (len + 31) / 32;
+        const int c = __popc(__ballot_sync(0xffffffffu, lane * step < len && work.before(s.r, lo + lane * step) <= left));
+        lo += (c - 1) * step;
+        len = min(step, len - (c - 1) * step);
+    }
+    s.i = lo;
+    s.done = left - work.before(s.r, lo);
+    return s;
 }
 
 // A product's place in the CTA's items, in the order they are issued in: tile by tile, stream by stream
@@ -250,17 +244,17 @@ constexpr int BEHIND = 2;  // products that O is behind S
 template <bool LOW>
 __device__ __forceinline__ bool may_go(int between) { return !LOW || between < 2; }
 
-// 256 bytes of a row, on their way without a tensor map
-__device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void copy16(void* to, const void* from, bool some) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(some ? 16 : 0) : "memory");
+// The queries of `stream_tokens` tokens from `token` on under the heads from `head` on, 128 bytes of each (piece `x`)
+__device__ __forceinline__ void tma_load_queries(void* to, const CUtensorMap* map, uint64_t* bar, int head, int token, int x, int b) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(smem_u32(to)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(head), "r"(token), "r"(x), "r"(b)
+        : "memory");
 }
 
 template <class X, bool TREE>
 __global__ void __launch_bounds__(Rows<X>::THREADS, 1)
-serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
+serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
                     const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ ServingArgs a) {
     typedef Rows<X> C;
     typedef RowsSpace<X> Space;
@@ -291,11 +285,15 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         for (int i = 0; i < ITEMS; ++i) {
             mbar_init(&sh.item_full[i], 1);
-            mbar_init(&sh.item_empty[i], 1 + (LOW ? 0 : 1) + C::SOFTMAX_WARPS);
+            mbar_init(&sh.item_empty[i], 1 + C::SOFTMAX_WARPS);
         }
         sh.abort.id = 0;
         fence_mbar_init();
     }
+    // rows that no query comes to stay zero
+    if (!LOW)
+        for (int i = threadIdx.x; i < C::STREAMS * C::Q_BUFFERS * C::Q_BYTES / 16; i += C::THREADS) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
     if (warp == 1) {
         tmem_alloc(&sh.tmem_base, 512);
         tmem_relinquish();
@@ -303,6 +301,8 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     pdl_wait();
     pdl_trigger();
+    Stretch line = {};
+    if (warp == 0) line = find_stretch<X, TREE>(a, lane);
     __syncthreads();
     tc_fence_after_sync();
     constexpr uint32_t tmem = 0;  // all columns are this CTA's
@@ -351,45 +351,46 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (warp == 0) {
             // ------------------------------ items, tiles of keys and values ------------------------------
             const Work<X, TREE> work{a};
-            Place at, end;
-            bool more = find_stretch<X, TREE>(a, lane, at, end), ok = true;
-            Request req = {};
-            if (more && at.b < a.B) req = work.request(at.b);
+            bool ok = true;
             PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
-            Turn put{0, 0u};
-            // The next item into the ring; one without rows at the end of the stretch
+            // A border inside a block is moved to its beginning or end where a part of less than LEAST tiles would be left.
+            auto border = [&](int64_t units, int n) {
+                const int j = units >= (int64_t)n * KEYS ? n : (int)units / KEYS;
+                return j == n ? n : j < C::LEAST ? 0 : n - j < C::LEAST ? n : j;
+            };
+            // The next item into the ring; one without tokens at the end of the stretch
             auto publish = [&](Item& it) {
-                it.rows = 0;
-                while (more) {
-                    if (at.b >= a.B) {
-                        more = false;
-                        break;
-                    }
-                    if (at.i >= req.blocks) {
-                        at.i = at.j = 0;
-                        if (req.blocks == 0 || ++at.kvh == a.Hk) {
-                            at.kvh = 0;
-                            if (++at.b < a.B) req = work.request(at.b);
+                it.tokens = 0;
+                while (line.units > 0) {
+                    if (line.i >= line.r.blocks) {
+                        line.i = 0;
+                        if (line.r.blocks == 0 || ++line.chunk == a.chunks) {
+                            line.chunk = 0;
+                            if (line.r.blocks == 0 || ++line.kvh == a.Hk) {
+                                line.kvh = 0;
+                                if (++line.b >= a.B) break;
+                                line.r = work.request(line.b);
+                            }
                         }
-                        if (at.b >= a.B) more = false;
-                        if (!more || req.blocks == 0) continue;
+                        continue;
                     }
-                    const bool ends = at == end;
-                    const int n = work.tiles(req, at.i), to = ends ? min(end.j, n) : n, j0 = at.j;
-                    const int i = at.i;
-                    at.i++;
-                    at.j = 0;
-                    more = !ends;
+                    const int i = line.i, n = work.tiles(line.r, i);
+                    const int j0 = border(line.done, n), to = border(line.done + line.units, n);
+                    line.units -= work.units(line.r, i) - line.done;
+                    line.done = 0;
+                    ++line.i;
                     if (to <= j0) continue;
-                    const int row0 = i * C::BLOCK, rows = min(C::BLOCK, req.rows - row0), count = to - j0;
-                    it.b = at.b; it.kvh = at.kvh; it.row0 = row0; it.rows = rows;
-                    it.begin = req.begin; it.len = req.len; it.key0 = j0 * KEYS; it.tiles = count;
+                    const int count = to - j0;
+                    it.b = line.b; it.kvh = line.kvh; it.chunk = line.chunk;
+                    it.token0 = i * a.block_tokens;
+                    it.tokens = min(a.block_tokens, line.r.tokens - it.token0);
+                    it.begin = line.r.begin; it.len = line.r.len; it.key0 = j0 * KEYS;
                     it.new_tile = TREE ? n - 1 - j0 : -1;
                     it.n0 = count;
                     it.n1 = 0;
-                    if (!LOW && rows > TILE) {
+                    if (!LOW && it.tokens > a.stream_tokens) {
                         it.n1 = count;
-                        if (!TREE && a.causal) it.n0 = max(0, min((((row0 + TILE - 1) / a.group) / KEYS) + 1 - j0, count));
+                        if (!TREE && a.causal) it.n0 = max(0, min((it.token0 + a.stream_tokens + KEYS - 1) / KEYS - j0, count));
                     }
                     it.slot = -1;
                     if (j0 > 0) {
@@ -399,12 +400,14 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         if (record.head == PART_EMPTY) record.head = PART_NONE;
                         if (to < n) {
                             it.slot = 2 * blockIdx.x + 1;
-                            record.b = TREE ? it.b : 0; record.kvh = it.kvh; record.begin = it.begin; record.row0 = row0; record.rows = rows;
+                            record.b = TREE ? it.b : 0; record.head0 = it.kvh * a.group + it.chunk * TILE; record.heads = min(TILE, a.group - it.chunk * TILE);
+                            record.token0 = it.begin + it.token0; record.tokens = it.tokens;
                         }
                     }
                     break;
                 }
             };
+            Turn put{0, 0u};
             int made = 0;
             auto emit = [&](Item& it) -> bool {  // false: gave up
                 publish(it);
@@ -413,14 +416,16 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     sh.items[put.at] = it;
                     mbar_arrive(&sh.item_full[put.at]);
                 }
-                if constexpr (LOW) {
-                    if (it.rows > 0) {  // its queries, once those before are in tensor memory
-                        if (made > 0 && !__all_sync(0xffffffffu, mbar_wait(wc, &sh.q_empty[0], (made - 1) & 1, W_Q_EMPTY, made))) return false;
-                        if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[0], it.rows * 256);
-                        __syncwarp();
-                        for (int r = lane; r < it.rows; r += 32) {
-                            const int row = it.row0 + r, token = row / a.group;
-                            bulk_load(sQ + r * C::Q_ROW, row_of<X>(a.Q, TREE ? it.b : 0, it.kvh * a.group + row - token * a.group, it.begin + token), 256, &sh.q_full[0]);
+                if (it.tokens > 0) {  // its queries, in the place of those of the item before, or before that
+                    const int buf = made & (C::Q_BUFFERS - 1), use = made / C::Q_BUFFERS;
+                    if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(wc, &sh.q_empty[buf], (use - 1) & 1, W_Q_EMPTY, made))) return false;
+                    if (lane == 0) {
+                        const int streams = it.n1 > 0 ? 2 : 1, head = it.kvh * a.group + it.chunk * TILE;
+                        mbar_arrive_expect_tx(&sh.q_full[buf], streams * a.q_bytes);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {  // streams, or halves of the rows
+                            if (LOW || x < streams)
+                                tma_load_queries(sQ + (buf * 2 + x) * (TILE * 128), &map_q, &sh.q_full[buf], head, it.begin + it.token0 + (LOW ? 0 : x * a.stream_tokens), LOW ? x : 0, TREE ? it.b : 0);
                         }
                     }
                 }
@@ -465,7 +470,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             int ahead = 0;  // products that S is in front of O
             Turn got{0, 0u};
             ok = emit(next);
-            bool s_on = ok && next.rows > 0;
+            bool s_on = ok && next.tokens > 0;
             int between = 0;  // items that S is in front of O
             if (s_on) {
                 s.start(next.n0, next.n1);
@@ -480,7 +485,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     ++ahead;
                     if (!s.next()) {
                         if (!(ok = emit(next))) break;
-                        s_on = next.rows > 0;
+                        s_on = next.tokens > 0;
                         if (s_on) s.start(next.n0, next.n1);
                         ++between;
                     }
@@ -542,7 +547,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             auto next_item = [&](Turn& turn, Cursor& c) -> bool {  // false: the end, or gave up
                 if (!(ok = wait(false, {&sh.item_full[turn.at], turn.phase}, W_ITEM, items))) return false;
                 const Item& it = sh.items[turn.at];
-                if ((int)uniform(it.rows) == 0) return false;
+                if ((int)uniform(it.tokens) == 0) return false;
                 c.start((int)uniform(it.n0), (int)uniform(it.n1));
                 return true;
             };
@@ -655,29 +660,6 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             tend(threadIdx.x & 63, 0);
         } else if (warp == 2) {
             tend(lane, 0);
-        } else {
-            // ------------------------------ queries of 16-bit types ------------------------------
-            Turn get{0, 0u};
-            for (int n = 0;; ++n) {
-                if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.item_full[get.at], get.phase, W_ITEM, n))) break;
-                const Item& it = sh.items[get.at];
-                const int rows = it.rows, row0 = it.row0, b = TREE ? it.b : 0, h0 = it.kvh * a.group, begin = it.begin;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.item_empty[get.at]);
-                get.next(ITEMS);
-                if (rows == 0) break;
-                const int buf = n & 1;
-                if (n >= 2 && !__all_sync(0xffffffffu, mbar_wait(wc, &sh.q_empty[buf], (n / 2 - 1) & 1, W_Q_EMPTY, n))) break;
-                uint8_t* to = sQ + buf * C::STREAMS * C::Q_BYTES;
-                const int c = lane & 7;
-                for (int r = lane >> 3; r < (rows > TILE ? 2 * TILE : TILE); r += 4) {  // in the layout of a K-major operand
-                    const int row = row0 + min(r, rows - 1), token = row / a.group;
-                    copy16(to + r * 128 + ((c ^ (r & 7)) << 4), row_of<X>(a.Q, b, h0 + row - token * a.group, begin + token) + 8 * c, r < rows);
-                }
-                asm volatile("cp.async.wait_all;\n" ::: "memory");
-                fence_proxy_async_smem();
-                mbar_arrive_warp(&sh.q_full[buf], lane);
-            }
         }
     } else if (LOW && warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 120;\n");
@@ -686,7 +668,10 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         // ------------------------------ softmax ------------------------------
         if constexpr (LOW) asm volatile("setmaxnreg.inc.sync.aligned.u32 240;\n");
         else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
-        const int t = (warp - 4) >> 2, quarter = warp & 3, r = t * TILE + quarter * 32 + lane;
+        // The row of this thread: of the item's tokens the `my_token`-th, of the heads the `my_head`-th
+        const int t = (warp - 4) >> 2, quarter = warp & 3, in_stream = quarter * 32 + lane, r = t * TILE + in_stream;
+        const int box_heads = min(a.group, TILE), my_token_in = in_stream / box_heads, my_head = in_stream - my_token_in * box_heads;
+        const int my_token = my_token_in < a.stream_tokens ? t * a.stream_tokens + my_token_in : INT_MAX;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const float2 scale2 = make_float2(a.scale_log2e, a.scale_log2e);
         bool ok = true;
@@ -702,18 +687,18 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         auto fetch_queries = [&] {
             if constexpr (LOW) {
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.item_full[fetch.at], fetch.phase, W_ITEM, fetched)))) return;
-                const int rows = sh.items[fetch.at].rows;
+                const int tokens = sh.items[fetch.at].tokens;
                 fetch.next(ITEMS);
-                if (rows == 0) return;
+                if (tokens == 0) return;
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.q_full[0], fetched & 1, W_Q, fetched)))) return;
                 ++fetched;
-                const uint4* from = reinterpret_cast<const uint4*>(sQ + r * C::Q_ROW);
+                const bool mine = my_token < tokens;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t y[32], z[32];
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
-                        const uint4 v = r < rows ? from[8 * half + c] : make_uint4(0, 0, 0, 0);
+                        const uint4 v = mine ? *reinterpret_cast<const uint4*>(sQ + (half * TILE + in_stream) * 128 + ((c ^ (in_stream & 7)) << 4)) : make_uint4(0, 0, 0, 0);
                         y[4 * c] = v.x ^ a.flip; y[4 * c + 1] = v.y ^ a.flip; y[4 * c + 2] = v.z ^ a.flip; y[4 * c + 3] = v.w ^ a.flip;
                     }
 #pragma unroll
@@ -732,15 +717,16 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         while (ok) {
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.item_full[get.at], get.phase, W_ITEM, q0)))) break;
             const Item& it = sh.items[get.at];
-            const int rows = it.rows, row0 = it.row0, n0 = it.n0, n1 = it.n1, slot = it.slot, begin = it.begin, b = TREE ? it.b : 0, h0 = it.kvh * a.group, key0 = it.key0, len = it.len;
+            const int tokens = it.tokens, token0 = it.token0, n0 = it.n0, n1 = it.n1, slot = it.slot, begin = it.begin, b = TREE ? it.b : 0, key0 = it.key0, len = it.len;
+            const int head0 = it.chunk * TILE, h = it.kvh * a.group + head0 + my_head;
             const int new_tile = it.new_tile;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.item_empty[get.at]);
             get.next(ITEMS);
-            if (rows == 0) break;
-            const bool valid = r < rows, live = t * TILE + quarter * 32 < rows;
-            const int token = (row0 + r) / a.group;
-            const int limit = !valid ? 0 : !TREE && a.causal ? token + 1 : len;  // keys the row sees
+            if (tokens == 0) break;
+            const bool valid = my_token < tokens && my_head < a.group - head0, live = __any_sync(0xffffffffu, valid);
+            const int token = token0 + (valid ? my_token : 0);
+            const int limit = !valid ? INT_MAX / 2 : !TREE && a.causal ? token + 1 : len;  // keys the row sees
             const uint64_t bits = TREE && valid ? tree_bits(a, b, token) : 0ull;
             const int n = t == 0 ? n0 : n1;
             auto product = [&](int j) { return q0 + min(j, n0) + min(j, n1) + (t == 1 && j < n0); };
@@ -870,12 +856,12 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         // argument and of a NaN.
                         float alpha = 1.f, add = 0.f;
                         bool done = false;
-                        if (__all_sync(0xffffffffu, lim >= KEYS && m > -INFINITY)) {
+                        if (__all_sync(0xffffffffu, lim >= KEYS && (m > -INFINITY || !valid))) {
                             float poly_top = -INFINITY;
 #pragma unroll
                             for (int i = 2 * (POLY_OF - 1); i < 128; i += 2 * POLY_OF) poly_top = max3_or_nan(poly_top, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
                             add = weights(std::true_type{});
-                            done = __all_sync(0xffffffffu, add <= MOST && fmaf(poly_top, a.scale_log2e, -m) <= 8.f);
+                            done = __all_sync(0xffffffffu, !valid || (add <= MOST && fmaf(poly_top, a.scale_log2e, -m) <= 8.f));
                             if (!done) load();
                         }
                         if (!done) {
@@ -940,7 +926,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     for (int i = 0; i < 16; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 } else {
                     const float f = l != 0.f ? 1.f / l : 0.f;
-                    const int h = h0 + row0 + r - token * a.group, row = begin + token;
+                    const int row = begin + token;
                     uint4* to = reinterpret_cast<uint4*>(const_cast<X*>(row_of<X>(a.O, b, h, row)));
                     if constexpr (LOW) {
 #pragma unroll
@@ -976,7 +962,7 @@ __global__ void __launch_bounds__(256) serving_combine_kernel(const __grid_const
     pdl_trigger();
     const PartRecord rec = a.parts[blockIdx.x];
     const int sub = threadIdx.x & 15, r0 = blockIdx.y * 64;
-    if (r0 >= rec.rows) return;
+    if (rec.tokens == 0) return;
     int last = blockIdx.x;  // the CTA that has the last part
     while (++last < ctas - 1) {
         const int head = a.parts[last].head;
@@ -984,7 +970,10 @@ __global__ void __launch_bounds__(256) serving_combine_kernel(const __grid_const
     }
     const int n = last - (int)blockIdx.x + 1;
     const uint32_t together = threadIdx.x & 16 ? 0xffff0000u : 0xffffu;
-    for (int r = r0 + (int)threadIdx.x / 16; r < min(rec.rows, r0 + 64); r += 16) {
+    for (int r = r0 + (int)threadIdx.x / 16; r < r0 + 64; r += 16) {
+        const int t = r / TILE, box_heads = min(a.group, TILE), in_stream = r - t * TILE, token_in = in_stream / box_heads, head = in_stream - token_in * box_heads;
+        const int token = t * a.stream_tokens + token_in;
+        if (token_in >= a.stream_tokens || token >= rec.tokens || head >= rec.heads) continue;
         float M = -INFINITY, L = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int p0 = 0; p0 < n; p0 += 16) {
@@ -1019,7 +1008,7 @@ __global__ void __launch_bounds__(256) serving_combine_kernel(const __grid_const
             }
         }
         const float f = L != 0.f ? 1.f / L : 0.f;
-        const int token = (rec.row0 + r) / a.group, h = rec.kvh * a.group + rec.row0 + r - token * a.group, row = rec.begin + token;
+        const int h = rec.head0 + head, row = rec.token0 + token;
         store4(const_cast<X*>(row_of<X>(a.O, rec.b, h, row)) + 4 * sub, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
         if (sub == 0) a.LSE[rec.b * a.lse_sB + h * a.lse_sH + row] = L != 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
     }
@@ -1040,6 +1029,21 @@ int page_map(CUtensorMap* map, const hk_view& v, int dtype, int n_pages, int H, 
     return r == CUDA_SUCCESS ? HK_OK : HK_ERR_CUDA;
 }
 
+// `tokens` tokens under `heads` heads, 128 bytes of each
+int query_map(CUtensorMap* map, const hk_view& v, int dtype, int B, int H, int64_t T, int heads, int tokens) {
+    EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return HK_ERR_CUDA;
+    const int e = esize(dtype), inner = 128 / e;
+    const int64_t sM = T == 1 ? HEAD_DIM : v.strideM, sH = H == 1 ? HEAD_DIM : v.strideH, sB = B == 1 ? HEAD_DIM : v.strideB;
+    cuuint64_t dims[5] = {(cuuint64_t)inner, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)(64 / inner), (cuuint64_t)B};
+    cuuint64_t strides[4] = {(cuuint64_t)sH * e, (cuuint64_t)sM * e, 128, (cuuint64_t)sB * e};
+    cuuint32_t box[5] = {(cuuint32_t)inner, (cuuint32_t)heads, (cuuint32_t)tokens, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+    const CUtensorMapDataType type = dtype == HK_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == HK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult r = enc(map, type, 5, v.ptr, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HK_OK : HK_ERR_CUDA;
+}
+
 template <class X, bool TREE>
 int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     typedef Rows<X> C;
@@ -1049,6 +1053,12 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
     std::call_once(once[dev], [dev] { rc[dev] = cudaFuncSetAttribute(serving_rows_kernel<X, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSpace<X>::SMEM); });
     if (rc[dev] != cudaSuccess) return HK_ERR_CUDA;
+    a.stream_tokens = std::max(1, TILE / a.group);
+    a.block_tokens = C::STREAMS * a.stream_tokens;
+    a.chunks = cdiv(a.group, TILE);
+    a.block_shift = 31;
+    while ((1LL << (a.block_shift - 31)) < a.block_tokens) ++a.block_shift;
+    a.block_mul = (uint32_t)(((1ULL << a.block_shift) + a.block_tokens - 1) / a.block_tokens);
     CUtensorMap k, v, kp, vp;
     const int B = TREE ? a.B : 1;
     const int64_t T = TREE ? a.T : a.N;
@@ -1062,9 +1072,12 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
             (s = page_map(&vp, a.pool.V, dtype, a.pool.n_pages, a.Hk, a.pool.page, a.box, C::LOW)))
             return s;
     }
+    CUtensorMap q;
+    if ((s = query_map(&q, a.Q, dtype, B, a.Hk * a.group, T, std::min(a.group, TILE), a.stream_tokens)) != HK_OK) return s;
+    a.q_bytes = std::min(a.group, TILE) * a.stream_tokens * 64 * (int)sizeof(X);
     const int ctas = sm_count();
     LaunchConfig lc(ctas, C::THREADS, RowsSpace<X>::SMEM, stream, 1, true);
-    if (cudaLaunchKernelEx(&lc.cfg, serving_rows_kernel<X, TREE>, k, v, kp, vp, a) != cudaSuccess) return check_launch();
+    if (cudaLaunchKernelEx(&lc.cfg, serving_rows_kernel<X, TREE>, q, k, v, kp, vp, a) != cudaSuccess) return check_launch();
     count_launch();
     if (!a.parts) return HK_OK;
     LaunchConfig sum(ctas, 256, 0, stream, 1, true);
