@@ -32,7 +32,7 @@ struct ServingArgs {
     // block_mul >> block_shift for x below 2^31
     int stream_tokens, block_tokens, chunks, q_bytes;
     uint32_t block_mul;
-    int block_shift;
+    int block_shift, unit_shift;
     int box;            // rows of a page that are loaded at once
     // slots of the workspace, and who has what in them; no parts: blocks are not cut
     float2* ml;         // [slots][rows]

@@ -41,7 +41,7 @@ struct Rows {
     static constexpr int ITEMS = 8;
 };
 
-struct Item {
+struct __align__(16) Item {
     int b, kvh, chunk;   // request, key head, which 128 of its query heads
     int token0, tokens;  // of the request; no tokens: the end
     int begin, len;      // of the packed rows; keys of the sequence, or in pages
@@ -68,7 +68,7 @@ constexpr int LAST = -1;
 template <class X>
 struct RowsSpace {
     typedef Rows<X> C;
-    static constexpr int OFF_Q = C::SLOTS * C::KV_BYTES, OFF_SH = OFF_Q + C::STREAMS * C::Q_BUFFERS * C::Q_BYTES, SMEM = OFF_SH + (int)sizeof(RowsShared<X>);
+    static constexpr int OFF_Q = C::SLOTS * C::KV_BYTES, OFF_O = OFF_Q + C::STREAMS * C::Q_BUFFERS * C::Q_BYTES, OFF_SH = OFF_O + (C::LOW ? 0 : C::SOFTMAX_WARPS * 4096), SMEM = OFF_SH + (int)sizeof(RowsShared<X>);
     static_assert(SMEM <= 232448, "exceeds the 227 KiB a CTA may opt in to");
 };
 // Tensor memory.  16-bit types: three buffers of 128 columns for scores and weights, O of two streams.  fp32: three buffers of
@@ -80,9 +80,10 @@ enum RowsWait { W_Q = 501, W_Q_EMPTY, W_KV, W_READY, W_EMPTY, W_S, W_P, W_O, W_I
 // ---------------------------------------------------------------------------
 // How the work is cut: a block counts as the keys that it meets and EXTRA for its beginning and end.
 // ---------------------------------------------------------------------------
+// (Units of 2^unit_shift keys, so that all of them fit 32 bits: a division of 64-bit numbers takes a warp some 300 cycles.)
 struct Request {
     int begin, len, tokens, blocks;  // blocks: of tokens
-    int64_t units;                   // of all of its blocks, under one key head
+    int units;                       // of all of its blocks, under one key head
 };
 template <class X, bool TREE>
 struct Work {
@@ -93,11 +94,10 @@ struct Work {
     __device__ __forceinline__ int tiles(const Request& r, int i) const {
         return TREE || !a.causal ? all_tiles(r) : (min((i + 1) * a.block_tokens, r.len) + C::KEYS - 1) / C::KEYS;
     }
-    __device__ __forceinline__ int64_t units(const Request& r, int i) const { return (TREE || !a.causal ? all_tiles(r) * C::KEYS : (i + 1) * a.block_tokens) + EXTRA; }
     // units in front of block i, of one chunk of heads
-    __device__ __forceinline__ int64_t before(const Request& r, int i) const {
-        if (TREE || !a.causal) return i * units(r, 0);
-        return (int64_t)i * (i + 1) / 2 * a.block_tokens + (int64_t)i * EXTRA;
+    __device__ __forceinline__ int before(const Request& r, int i) const {
+        const int64_t keys = TREE || !a.causal ? (int64_t)i * (all_tiles(r) * C::KEYS + EXTRA) : (int64_t)i * (i + 1) / 2 * a.block_tokens + (int64_t)i * EXTRA;
+        return (int)(keys >> a.unit_shift);
     }
     __device__ __forceinline__ Request request(int b) const {
         Request r;
@@ -114,10 +114,10 @@ struct Work {
         return r;
     }
 };
-__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
+__device__ __forceinline__ int warp_scan(int x, int lane) {
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, off);
+        const int y = __shfl_up_sync(0xffffffffu, x, off);
         if (lane >= off) x += y;
     }
     return x;
@@ -128,7 +128,7 @@ __device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
 struct Stretch {
     Request r;
     int b, kvh, chunk, i;
-    int64_t done, units;
+    int done, units;
 };
 // By one warp; no units: there is nothing for this CTA.
 template <class X, bool TREE>
@@ -137,8 +137,7 @@ __device__ __forceinline__ Stretch find_stretch(const ServingArgs& a, int lane) 
     const Work<X, TREE> work{a};
     constexpr int EACH = 2;  // requests of a lane
     Stretch s = {};
-    int64_t units[EACH], sum = 0, all = 0;
-    int blocks = 0;
+    int units[EACH], sum = 0, all = 0, blocks = 0;
     auto take = [&](int b0) {
         sum = 0;
 #pragma unroll
@@ -154,20 +153,19 @@ __device__ __forceinline__ Stretch find_stretch(const ServingArgs& a, int lane) 
         }
         return warp_scan(sum, lane);
     };
-    int64_t upto = 0;
+    int upto = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
         upto = take(b0);
         all += __shfl_sync(0xffffffffu, upto, 31);
     }
     all *= a.Hk;
     // A CTA to a block, more if the blocks are long, as many as there are
-    const int64_t n_blocks = (int64_t)__reduce_add_sync(0xffffffffu, blocks) * a.Hk;
-    const int ctas = (int)min((int64_t)gridDim.x, max(n_blocks, all / (3 * C::LEAST * C::KEYS)));
+    const int n_blocks = (int)min((int64_t)gridDim.x, (int64_t)__reduce_add_sync(0xffffffffu, min(blocks, 1 << 20)) * a.Hk);
+    const int ctas = min((int)gridDim.x, max(n_blocks, all / max(1, 3 * C::LEAST * C::KEYS >> a.unit_shift)));
     const int me = blockIdx.x;
     if (me >= ctas) return s;
-    const int64_t share = all / ctas;
-    const int more = (int)(all - share * ctas);
-    int64_t left = me * share + min(me, more);
+    const int share = (unsigned)all / (unsigned)ctas, more = all - share * ctas;
+    int left = me * share + min(me, more);
     s.units = share + (me < more);
     for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
         if (a.B > 32 * EACH) upto = take(b0);  // otherwise they are here still
@@ -187,12 +185,12 @@ __device__ __forceinline__ Stretch find_stretch(const ServingArgs& a, int lane) 
         break;
     }
     s.r = work.request(s.b);
-    s.kvh = (int)((uint64_t)left / (uint64_t)s.r.units);
+    s.kvh = (unsigned)left / (unsigned)s.r.units;
     left -= s.kvh * s.r.units;
     s.chunk = 0;
     if (a.chunks > 1) {
-        const int64_t one = s.r.units / a.chunks;
-        s.chunk = (int)(left / one);
+        const int one = s.r.units / a.chunks;
+        s.chunk = left / one;
         left -= s.chunk * one;
     }
     int lo = 0, len = s.r.blocks;  // the last block that begins at or before it
@@ -265,6 +263,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     RowsShared<X>& sh = *reinterpret_cast<RowsShared<X>*>(smem + Space::OFF_SH);
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
+    if (warp == 2 && lane < (TREE ? 5 : 3)) tma_prefetch_desc(lane == 0 ? &map_q : lane == 1 ? &map_k : lane == 2 ? &map_v : lane == 3 ? &map_kp : &map_vp);
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::Q_BUFFERS; ++i) {
             mbar_init(&sh.q_full[i], 1);
@@ -309,41 +308,6 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (sh.tmem_base != tmem) sh.abort.id = 598;
     WaitNote wc{&sh.abort};
 
-    // What the tiles need beside the loads, entry by entry of the ring.  Rows behind the request's last key may hold anything, and 0 times
-    // a NaN is one: they are cleared among the values.  fp32: the tiles' low parts, by two pairs of warps, each of which has every other
-    // slot of the ring for its own: a barrier is waited for by the parity of its phase, and is to be looked at in every one.
-    auto tend = [&](int me, int first) {
-        constexpr int EVERY = LOW ? 2 : 1;
-        Turn at{first, 0u};
-        while (true) {
-            if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.kv_full[at.at], at.phase, W_KV, at.at))) return;
-            const int keep = sh.keep[at.at];
-            if (keep == LAST) return;
-            uint4* raw = reinterpret_cast<uint4*>(sKV + at.at * C::KV_BYTES);
-            if constexpr (LOW) {
-                constexpr int EACH = C::KV_RAW / 16 / 64;
-                uint4 *from = raw + me, *low = from + C::KV_RAW / 16, x[EACH];
-#pragma unroll
-                for (int k = 0; k < EACH; ++k) x[k] = from[k * 64];
-                if (keep < KEYS) {
-#pragma unroll
-                    for (int k = 0; k < EACH; ++k)
-                        if (((k * 64 + me) & (C::KV_BOX / 16 - 1)) / 8 >= keep) from[k * 64] = x[k] = make_uint4(0, 0, 0, 0);  // row of the box
-                }
-#pragma unroll
-                for (int k = 0; k < EACH; ++k) low[k * 64] = make_uint4(tf32_rest(x[k].x), tf32_rest(x[k].y), tf32_rest(x[k].z), tf32_rest(x[k].w));
-                fence_proxy_async_smem();
-                mbar_arrive_warp(&sh.kv_ready[at.at], lane);
-            } else {
-                for (int k = keep * 8 + me; k < C::KV_RAW / 16; k += 32) raw[k] = make_uint4(0, 0, 0, 0);
-                fence_proxy_async_smem();
-                mbar_arrive_warp(&sh.kv_ready[at.at], lane);
-                if (lane == 0) mbar_arrive(&sh.kv_empty[at.at]);  // a slot is filled again when this warp has seen what it held
-            }
-            for (int k = 0; k < EVERY; ++k) at.next(SLOTS);
-        }
-    };
-
     // three groups of warps, 168 registers a thread at the launch
     if (warp < 4) {
         if constexpr (LOW) asm volatile("setmaxnreg.dec.sync.aligned.u32 120;\n");
@@ -354,8 +318,8 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             bool ok = true;
             PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
             // A border inside a block is moved to its beginning or end where a part of less than LEAST tiles would be left.
-            auto border = [&](int64_t units, int n) {
-                const int j = units >= (int64_t)n * KEYS ? n : (int)units / KEYS;
+            auto border = [&](int units, int n) {
+                const int j = (int)min((int64_t)n, ((int64_t)units << a.unit_shift) / KEYS);
                 return j == n ? n : j < C::LEAST ? 0 : n - j < C::LEAST ? n : j;
             };
             // The next item into the ring; one without tokens at the end of the stretch
@@ -376,7 +340,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     const int i = line.i, n = work.tiles(line.r, i);
                     const int j0 = border(line.done, n), to = border(line.done + line.units, n);
-                    line.units -= work.units(line.r, i) - line.done;
+                    line.units -= work.before(line.r, i + 1) - work.before(line.r, i) - line.done;
                     line.done = 0;
                     ++line.i;
                     if (to <= j0) continue;
@@ -408,9 +372,13 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
             };
             Turn put{0, 0u};
-            int made = 0;
-            auto emit = [&](Item& it) -> bool {  // false: gave up
+            int made = 0, s_at = 0, o_at = 0;  // items; the places of those of S and of O
+            bool on = true;
+            Cursor s, o;
+            auto emit = [&]() -> bool {  // false: gave up
+                Item it;
                 publish(it);
+                on = it.tokens > 0;
                 if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.item_empty[put.at], put.phase ^ 1u, W_ITEM_EMPTY, made))) return false;
                 if (lane == 0) {
                     sh.items[put.at] = it;
@@ -429,6 +397,8 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         }
                     }
                 }
+                if (on) s.start(it.n0, it.n1);
+                s_at = put.at;
                 put.next(ITEMS);
                 ++made;
                 return true;
@@ -465,42 +435,39 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 ++filled;
                 return true;
             };
-            Item next, old;  // of S and of O
-            Cursor s, o;
-            int ahead = 0;  // products that S is in front of O
-            Turn got{0, 0u};
-            ok = emit(next);
-            bool s_on = ok && next.tokens > 0;
-            int between = 0;  // items that S is in front of O
-            if (s_on) {
-                s.start(next.n0, next.n1);
-                old = next;
-                o.start(old.n0, old.n1);
-                got.next(ITEMS);
-            }
-            while (ok && (s_on || ahead > 0)) {  // in step with the products
-                const bool go = s_on && may_go<LOW>(between);
-                if (go) {
-                    if (s.first() && !(ok = load(next, s.j, false))) break;
-                    ++ahead;
-                    if (!s.next()) {
-                        if (!(ok = emit(next))) break;
-                        s_on = next.tokens > 0;
-                        if (s_on) s.start(next.n0, next.n1);
-                        ++between;
+            // In step with the products: S, then O so many products behind it.  (One place of each call: this code has to stay small, see the top.)
+            int ahead = 0, between = -1;  // products and items that S is in front of O
+            bool s_new = true, o_new = true;
+            while (true) {
+                if (s_new) {
+                    if (!(ok = emit())) break;
+                    s_new = false;
+                    ++between;
+                }
+                if (!on && ahead == 0) break;
+                const bool go = on && may_go<LOW>(between);
+                if (o_new) {
+                    __syncwarp();
+                    o.start(sh.items[o_at].n0, sh.items[o_at].n1);
+                    o_new = false;
+                }
+#pragma unroll 1
+                for (int v = 0; v < 2 && ok; ++v) {
+                    if (v ? ahead <= BEHIND && go : !go) continue;
+                    if (v ? o.first() : s.first()) ok = load(sh.items[v ? o_at : s_at], v ? o.j : s.j, v);
+                    if (v) {
+                        --ahead;
+                        if (!o.next()) {
+                            o_new = true;
+                            o_at = o_at == ITEMS - 1 ? 0 : o_at + 1;
+                            --between;
+                        }
+                    } else {
+                        ++ahead;
+                        s_new = !s.next();
                     }
                 }
-                if (ahead > BEHIND || !s_on || !go) {
-                    if (o.first() && !(ok = load(old, o.j, true))) break;
-                    --ahead;
-                    if (!o.next() && (ahead > 0 || s_on)) {
-                        __syncwarp();
-                        old = sh.items[got.at];
-                        o.start(old.n0, old.n1);
-                        got.next(ITEMS);
-                        --between;
-                    }
-                }
+                if (!ok) break;
             }
             for (int k = 0; ok && k < (LOW ? 2 : 1); ++k) {  // to those who tend the tiles: no more
                 if (filled >= SLOTS && !(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.kv_empty[ring.at], ring.phase ^ 1u, W_EMPTY, filled)))) break;
@@ -541,8 +508,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 else own[0] = y;
                 return t * 3 + x;
             };
-            bool ok = true, s_on = false;
-            int between = 0;
+            bool ok = true, s_on = false, new_queries = false;
             auto look_at = [&](const Turn& x, bool v) -> Barrier { return LOW || v ? Barrier{&sh.kv_ready[x.at], x.phase} : Barrier{&sh.kv_full[x.at], x.phase}; };
             auto next_item = [&](Turn& turn, Cursor& c) -> bool {  // false: the end, or gave up
                 if (!(ok = wait(false, {&sh.item_full[turn.at], turn.phase}, W_ITEM, items))) return false;
@@ -551,12 +517,24 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 c.start((int)uniform(it.n0), (int)uniform(it.n1));
                 return true;
             };
-            s_on = next_item(s_item, s);
-            if (s_on) next_item(o_item, o);
-            bool new_queries = true, seen_k = false, seen_v = false, seen_p = false;
+            bool s_new = true, o_new = true, seen_k = false, seen_v = false, seen_p = false;
+            int between = -1;
 #pragma unroll 1
-            while (ok && (s_on || ahead > 0)) {
+            while (ok) {
+                const bool fresh = s_new;
+                if (s_new) {
+                    s_on = next_item(s_item, s);
+                    if (!ok) break;
+                    s_new = false;
+                    ++between;
+                }
+                if (!s_on && ahead == 0) break;
+                if (o_new) {
+                    if (!next_item(o_item, o)) break;
+                    o_new = false;
+                }
                 const bool go = s_on && may_go<LOW>(between);
+                new_queries |= fresh;
                 if (go) {
                     if (new_queries) {
                         if (!(ok = wait(false, LOW ? Barrier{&sh.q_ready, (uint32_t)items & 1u} : Barrier{&sh.q_full[items & 1 & (C::Q_BUFFERS - 1)], (uint32_t)(items >> 1) & 1u}, W_Q, items))) break;
@@ -604,13 +582,10 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         if (!LOW) umma_commit_lead(leader, &sh.q_empty[items & (C::Q_BUFFERS - 1)]);
                         ++items;
                         s_item.next(ITEMS);
-                        s_on = next_item(s_item, s);
-                        if (!ok) break;
-                        new_queries = true;
-                        ++between;
+                        s_new = true;
                     }
                 }
-                if (ahead > BEHIND || !s_on || !go) {  // O
+                if (ahead > BEHIND || !go) {  // O
                     if (o.first()) {
                         if (!(ok = wait(seen_v, look_at(tile, true), W_READY, items))) break;
                         v_slot = tile.at;
@@ -621,7 +596,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     seen_v = seen_p = false;
                     const Desc vd = v_desc + v_slot * C::KV_BYTES;
                     const uint32_t acc = o.j > 0;
-                    const bool look_k = s_on && s.first() && o.last();
+                    const bool look_k = s_on && !s_new && s.first() && o.last();
                     if constexpr (LOW) {
                         constexpr uint32_t IDESC = make_idesc_tf32(TILE, HEAD_DIM, false, true);
                         const uint32_t high = tmem + p.at * 64, low = tmem + LOW_COL_LOW + low_buf * 64, d = tmem + LOW_COL_O;
@@ -651,19 +626,13 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         if (lane == 0) mbar_arrive(&sh.item_empty[o_item.at]);
                         o_item.next(ITEMS);
                         --between;
-                        if (ahead > 0 || s_on) next_item(o_item, o);
-                        if (!ok) break;
+                        o_new = true;
                     }
                 }
             }
-        } else if (LOW) {
-            tend(threadIdx.x & 63, 0);
-        } else if (warp == 2) {
-            tend(lane, 0);
         }
     } else if (LOW && warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 120;\n");
-        if (warp < 10) tend(threadIdx.x & 63, 1);
     } else {
         // ------------------------------ softmax ------------------------------
         if constexpr (LOW) asm volatile("setmaxnreg.inc.sync.aligned.u32 240;\n");
@@ -712,24 +681,20 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 mbar_arrive_warp(&sh.q_empty[0], lane);
             }
         };
-        fetch_queries();
         Turn get{0, 0u};
         while (ok) {
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.item_full[get.at], get.phase, W_ITEM, q0)))) break;
             const Item& it = sh.items[get.at];
-            const int tokens = it.tokens, token0 = it.token0, n0 = it.n0, n1 = it.n1, slot = it.slot, begin = it.begin, b = TREE ? it.b : 0, key0 = it.key0, len = it.len;
-            const int head0 = it.chunk * TILE, h = it.kvh * a.group + head0 + my_head;
-            const int new_tile = it.new_tile;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.item_empty[get.at]);
-            get.next(ITEMS);
+            const int tokens = it.tokens;
             if (tokens == 0) break;
-            const bool valid = my_token < tokens && my_head < a.group - head0, live = __any_sync(0xffffffffu, valid);
-            const int token = token0 + (valid ? my_token : 0);
-            const int limit = !valid ? INT_MAX / 2 : !TREE && a.causal ? token + 1 : len;  // keys the row sees
-            const uint64_t bits = TREE && valid ? tree_bits(a, b, token) : 0ull;
-            const int n = t == 0 ? n0 : n1;
-            auto product = [&](int j) { return q0 + min(j, n0) + min(j, n1) + (t == 1 && j < n0); };
+            const bool valid = my_token < tokens && my_head < a.group - it.chunk * TILE, live = __any_sync(0xffffffffu, valid);
+            const int token = it.token0 + (valid ? my_token : 0);
+            const int new_tile = it.new_tile, n = t == 0 ? it.n0 : it.n1;
+            const int limit = (!valid ? INT_MAX / 2 : !TREE && a.causal ? token + 1 : it.len) - it.key0;  // keys that the row sees, from the first tile's on
+            const uint64_t bits = TREE && valid ? tree_bits(a, it.b, token) : 0ull;
+            // the item's product of tile j: the other stream's come in between
+            const int between = t == 1 ? it.n0 : it.n1 > 0 ? INT_MAX : 0;
+            auto product = [&](int j) { return q0 + j + min(j + t, between); };
             float o[64], m = -INFINITY, l = 0.f;
             if constexpr (LOW) {
                 // O_j of every tile comes back and is added here: o = o * before + O_j
@@ -750,27 +715,26 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         }
                     }
                 };
-                for (int j = 0; j < n && wait(sh.s_full[0], q0 + j, W_S); ++j) {
-                    if (j == n - 1) {  // all scores of this item are there
+                for (int j = fetched == 0 ? -1 : 0; j <= n; ++j) {  // a step behind the last tile, for its O; one in front of the first item's, for its queries
+                    if (j >= 0 && j < n && !wait(sh.s_full[0], q0 + j, W_S)) break;
+                    if (j < 0 || j == n - 1) {  // the next item's: all scores of this one are there
                         fetch_queries();
                         if (!ok) break;
+                        if (j < 0) continue;
                     }
                     const int q = q0 + j;
                     const uint32_t at_s = lanes + q % 3 * 64, at_low = lanes + LOW_COL_LOW + (q & 1) * 64;
-                    if (live) {
-                        const int lim = TREE && j == new_tile ? KEYS : limit - key0 - j * KEYS;  // columns the row sees
+                    if (live && j < n) {
+                        const bool fresh = TREE && j == new_tile;
+                        const int lim = fresh ? 0 : limit - j * KEYS;  // columns the row sees
                         uint32_t x[64];
                         tmem_ld32p(at_s, x);
                         tmem_ld32p(at_s + 32, x + 32);
                         tmem_wait_ld();
-                        if (TREE && j == new_tile) {
+                        if (lim < KEYS) {
 #pragma unroll
                             for (int i = 0; i < 64; ++i)
-                                if (!(bits >> i & 1)) x[i] = __float_as_uint(-INFINITY);
-                        } else if (lim < KEYS) {
-#pragma unroll
-                            for (int i = 0; i < 64; ++i)
-                                if (i >= lim) x[i] = __float_as_uint(-INFINITY);
+                                if (fresh ? !(bits >> i & 1) : i >= lim) x[i] = __float_as_uint(-INFINITY);
                         }
                         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -800,12 +764,11 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         tmem_wait_st();
                     }
                     if (j > 0) add(j - 1);  // before O_j may come to the same place
-                    if (!ok) break;
+                    if (!ok || j == n) break;
                     tc_fence_before_sync();
                     mbar_arrive_warp(&sh.p_full[q % 3], lane);
                     before = alpha;
                 }
-                if (ok) add(n - 1);
             } else {
                 // O stays in tensor memory and is scaled there when a tile's weights come to more than MOST: a stale maximum makes them larger,
                 // which neither fp32 sums nor 16-bit types mind up to there
@@ -818,7 +781,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     const uint32_t at_s = lanes + q % 3 * 128;
                     if (live) {
                         const bool fresh = TREE && j == new_tile;
-                        const int lim = fresh ? 0 : limit - key0 - j * KEYS;  // columns the row sees
+                        const int lim = fresh ? 0 : limit - j * KEYS;  // columns the row sees
                         auto load = [&] {
 #pragma unroll
                             for (int c = 0; c < 128; c += 32) tmem_ld32p(at_s + c, x + c);
@@ -827,17 +790,16 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         float2 sum[2];
                         // The weights take the type of the values: half a step of it each.  A run of them is summed and packed while the next
                         // one's exponentials are under way.
-                        auto weights = [&](auto poly) {
+                        auto weights = [&] {
                             constexpr int RUN = 16;
-                            const float up = m == -INFINITY ? 0.f : lift<X>() - m;
-                            const float2 nm = make_float2(up, up);
+                            const float2 nm = make_float2(lift<X>() - m, lift<X>() - m);
                             sum[0] = sum[1] = make_float2(0.f, 0.f);
 #pragma unroll
                             for (int c = 0; c < 128 + RUN; c += RUN) {
 #pragma unroll
                                 for (int i = c; i < c + RUN && i < 128; i += 2) {
                                     const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, nm);
-                                    const float2 w = decltype(poly)::value && (i >> 1) % POLY_OF == POLY_OF - 1 ? ex2_poly(e) : make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                                    const float2 w = (i >> 1) % POLY_OF == POLY_OF - 1 ? ex2_poly(e) : make_float2(ex2_approx(e.x), ex2_approx(e.y));
                                     x[i] = __float_as_uint(w.x);
                                     x[i + 1] = __float_as_uint(w.y);
                                 }
@@ -850,34 +812,55 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             }
                             return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                         };
-                        load();
-                        // Most tiles raise no maximum by much: their weights are taken by the one there is, and their sum tells if it was too
-                        // low.  Then, and where keys are masked, the maximum is sought first.  The polynomial would make small numbers of a large
-                        // argument and of a NaN.
+                        // Most tiles raise no maximum by much: their weights are taken by the one there is (of the first tile: by its own), and
+                        // their sum tells if it was too low.  The polynomial would make small numbers of a large argument and of a NaN.
                         float alpha = 1.f, add = 0.f;
                         bool done = false;
-                        if (__all_sync(0xffffffffu, lim >= KEYS && (m > -INFINITY || !valid))) {
+                        if (__all_sync(0xffffffffu, lim >= KEYS)) {
+                            load();
+                            if (j == 0) {
+                                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                                for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                                m = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2e;
+                            }
                             float poly_top = -INFINITY;
 #pragma unroll
                             for (int i = 2 * (POLY_OF - 1); i < 128; i += 2 * POLY_OF) poly_top = max3_or_nan(poly_top, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                            add = weights(std::true_type{});
+                            add = weights();
                             done = __all_sync(0xffffffffu, !valid || (add <= MOST && fmaf(poly_top, a.scale_log2e, -m) <= 8.f));
-                            if (!done) load();
+                            if (done) {
+                                tmem_st32p(at_s, x);
+                                tmem_st32p(at_s + 32, x + 32);
+                            } else if (j == 0) {
+                                m = -INFINITY;
+                            }
                         }
                         if (!done) {
-                            if (fresh) {
+                            // The others, masked ones among them, 32 columns at a time: the maximum, then the weights.  Columns that no row of the
+                            // warp sees are not worked on.
+                            const int all_see = fresh ? 0 : __reduce_min_sync(0xffffffffu, lim), some_see = fresh ? a.T : __reduce_max_sync(0xffffffffu, valid ? lim : 0);
+                            auto scores = [&](int c) {
+                                tmem_ld32p(at_s + c, x);
+                                tmem_wait_ld();
+                                if (c + 32 > all_see) {
+                                    const int left = lim - c;
+                                    const uint32_t own_bits = (uint32_t)(bits >> (c & 63));
 #pragma unroll
-                                for (int i = 0; i < 128; ++i)
-                                    if (i >= 64 || !(bits >> (i & 63) & 1)) x[i] = __float_as_uint(-INFINITY);
-                            } else if (lim < KEYS) {
+                                    for (int i = 0; i < 32; ++i)
+                                        if (fresh ? !(own_bits >> i & 1) : i >= left) x[i] = __float_as_uint(-INFINITY);
+                                }
+                            };
+                            float top = -INFINITY;
+#pragma unroll 1
+                            for (int c = 0; c < 128 && c < some_see; c += 32) {
+                                scores(c);
+                                float mx[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                                for (int i = 0; i < 128; ++i)
-                                    if (i >= lim) x[i] = __float_as_uint(-INFINITY);
+                                for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                                top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
                             }
-                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                            for (int i = 0; i < 128; i += 2) mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2e;
+                            top *= a.scale_log2e;
                             const bool raise = top > m;
                             if (raise) {
                                 alpha = ex2_approx(m - top);  // 0 from -inf
@@ -895,10 +878,29 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                                     tmem_st32(at_o + c, y);
                                 }
                             }
-                            add = weights(std::false_type{});
+                            const float up = m == -INFINITY ? 0.f : lift<X>() - m;
+                            const float2 nm = make_float2(up, up);
+                            sum[0] = sum[1] = make_float2(0.f, 0.f);
+#pragma unroll 1
+                            for (int c = 0; c < 128; c += 32) {  // 16 columns of weights take the place of scores that are done with
+                                uint32_t w16[16];
+                                if (c < some_see) {
+                                    scores(c);
+#pragma unroll
+                                    for (int i = 0; i < 32; i += 2) {
+                                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, nm);
+                                        const float2 w = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                                        sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], w);
+                                        w16[i / 2] = pack<X>(w.x, w.y);
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) w16[i] = 0u;
+                                }
+                                tmem_st16(at_s + c / 2, w16);
+                            }
+                            add = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                         }
-                        tmem_st32p(at_s, x);
-                        tmem_st32p(at_s + 32, x + 32);
                         l = fmaf(l, alpha, add);
                         tmem_wait_st();
                     }
@@ -915,32 +917,87 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     tc_fence_before_sync();
                 }
             }
-            q0 += n0 + n1;
+            q0 += it.n0 + it.n1;
             if (!ok) break;
-            if (valid) {
-                if (slot >= 0) {
+            // Where it goes is looked up again, not kept in registers all the while
+            asm volatile("" ::: "memory");
+            const int slot = it.slot;
+            if (slot >= 0) {
+                if (valid) {
                     const int64_t at_slot = (int64_t)slot * C::BLOCK + r;
                     a.ml[at_slot] = make_float2(m, l);
                     float4* to = reinterpret_cast<float4*>(a.part + at_slot * 64);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                } else {
-                    const float f = l != 0.f ? 1.f / l : 0.f;
-                    const int row = begin + token;
-                    uint4* to = reinterpret_cast<uint4*>(const_cast<X*>(row_of<X>(a.O, b, h, row)));
-                    if constexpr (LOW) {
+                }
+            } else {
+                const float f = l != 0.f ? 1.f / l : 0.f;
+                const int b = TREE ? it.b : 0, row = it.begin + it.token0 + (valid ? my_token : 0), h = it.kvh * a.group + it.chunk * TILE + my_head;
+                X* const to = const_cast<X*>(row_of<X>(a.O, b, h, row));
+                if constexpr (LOW) {
+                    if (valid) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            to[i] = make_uint4(__float_as_uint(o[4 * i] * f), __float_as_uint(o[4 * i + 1] * f), __float_as_uint(o[4 * i + 2] * f), __float_as_uint(o[4 * i + 3] * f));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            to[i] = make_uint4(pack<X>(o[8 * i] * f, o[8 * i + 1] * f), pack<X>(o[8 * i + 2] * f, o[8 * i + 3] * f),
-                                               pack<X>(o[8 * i + 4] * f, o[8 * i + 5] * f), pack<X>(o[8 * i + 6] * f, o[8 * i + 7] * f));
+                            reinterpret_cast<uint4*>(to)[i] = make_uint4(__float_as_uint(o[4 * i] * f), __float_as_uint(o[4 * i + 1] * f), __float_as_uint(o[4 * i + 2] * f), __float_as_uint(o[4 * i + 3] * f));
                     }
-                    a.LSE[b * a.lse_sB + h * a.lse_sH + row] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+                } else {
+                    // Through shared memory, so that eight lanes store a row: a row to a lane is 32 lines an instruction, and all warps' stores of
+                    // an item took 1 700 cycles.
+                    uint4* const mine = reinterpret_cast<uint4*>(smem + Space::OFF_O + (warp - 4) * 4096);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        mine[lane * 8 + (i ^ (lane & 7))] = make_uint4(pack<X>(o[8 * i] * f, o[8 * i + 1] * f), pack<X>(o[8 * i + 2] * f, o[8 * i + 3] * f),
+                                                                       pack<X>(o[8 * i + 4] * f, o[8 * i + 5] * f), pack<X>(o[8 * i + 6] * f, o[8 * i + 7] * f));
+                    __syncwarp();
+                    const uint64_t place = valid ? reinterpret_cast<uint64_t>(to) : 0ull;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int from = 4 * i + (lane >> 3);
+                        const uint64_t at = __shfl_sync(0xffffffffu, place, from);
+                        const uint4 v = mine[from * 8 + ((lane ^ from) & 7)];
+                        if (at) reinterpret_cast<uint4*>(at)[lane & 7] = v;
+                    }
+                    __syncwarp();
                 }
+                if (valid) a.LSE[b * a.lse_sB + h * a.lse_sH + row] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
             }
+            mbar_arrive_warp(&sh.item_empty[get.at], lane);
+            get.next(ITEMS);
+        }
+    }
+    // What the tiles need beside the loads, entry by entry of the ring.  Rows behind the request's last key may hold anything, and 0 times
+    // a NaN is one: they are cleared among the values.  fp32: the tiles' low parts, by two pairs of warps, each of which has every other
+    // slot of the ring for its own: a barrier is waited for by the parity of its phase, and is to be looked at in every one.
+    if (LOW ? warp == 2 || warp == 3 || warp == 8 || warp == 9 : warp == 2) {
+        const int me = LOW ? threadIdx.x & 63 : lane, first = LOW && warp >= 8;
+        constexpr int EVERY = LOW ? 2 : 1;
+        Turn at{first, 0u};
+        while (true) {
+            if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.kv_full[at.at], at.phase, W_KV, at.at))) break;
+            const int keep = sh.keep[at.at];
+            if (keep == LAST) break;
+            uint4* raw = reinterpret_cast<uint4*>(sKV + at.at * C::KV_BYTES);
+            if constexpr (LOW) {
+                constexpr int EACH = C::KV_RAW / 16 / 64;
+                uint4 *from = raw + me, *low = from + C::KV_RAW / 16, x[EACH];
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) x[k] = from[k * 64];
+                if (keep < KEYS) {
+#pragma unroll
+                    for (int k = 0; k < EACH; ++k)
+                        if (((k * 64 + me) & (C::KV_BOX / 16 - 1)) / 8 >= keep) from[k * 64] = x[k] = make_uint4(0, 0, 0, 0);  // row of the box
+                }
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) low[k * 64] = make_uint4(tf32_rest(x[k].x), tf32_rest(x[k].y), tf32_rest(x[k].z), tf32_rest(x[k].w));
+                fence_proxy_async_smem();
+                mbar_arrive_warp(&sh.kv_ready[at.at], lane);
+            } else {
+                for (int k = keep * 8 + me; k < C::KV_RAW / 16; k += 32) raw[k] = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                mbar_arrive_warp(&sh.kv_ready[at.at], lane);
+                if (lane == 0) mbar_arrive(&sh.kv_empty[at.at]);  // a slot is filled again when this warp has seen what it held
+            }
+            for (int k = 0; k < EVERY; ++k) at.next(SLOTS);
         }
     }
     tc_fence_before_sync();
@@ -1053,6 +1110,11 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
     std::call_once(once[dev], [dev] { rc[dev] = cudaFuncSetAttribute(serving_rows_kernel<X, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSpace<X>::SMEM); });
     if (rc[dev] != cudaSuccess) return HK_ERR_CUDA;
+    {  // what all requests can come to, in keys
+        const double tokens = TREE ? (double)a.B * a.T : a.N, keys = TREE ? (double)a.pool.width * a.pool.page + 2 * C::KEYS : a.N + 2.0 * C::BLOCK, rows = std::max(1, TILE / a.group) * C::STREAMS;
+        double all = (tokens / rows + a.B) * (keys + 2 * C::KEYS) * a.Hk * cdiv(a.group, TILE);
+        for (a.unit_shift = 0; all >= 2e9; all /= 2) ++a.unit_shift;
+    }
     a.stream_tokens = std::max(1, TILE / a.group);
     a.block_tokens = C::STREAMS * a.stream_tokens;
     a.chunks = cdiv(a.group, TILE);
