@@ -236,6 +236,13 @@ struct Turn {  // a ring's place
         }
     }
 };
+// of numbers from 1 on
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 constexpr int BEHIND = 2;  // products that O is behind S
 // Whether S may be issued when it is so many items in front of O.  fp32: the queries of an item come to tensor memory when the softmax is
 // through with the item before the last, which waits for all of O of that.
@@ -695,7 +702,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             // the item's product of tile j: the other stream's come in between
             const int between = t == 1 ? it.n0 : it.n1 > 0 ? INT_MAX : 0;
             auto product = [&](int j) { return q0 + j + min(j + t, between); };
-            float o[64], m = -INFINITY, l = 0.f;
+            float o[LOW ? 64 : 1], m = -INFINITY, l = 0.f;
             if constexpr (LOW) {
                 // O_j of every tile comes back and is added here: o = o * before + O_j
                 float before = 0.f, alpha = 0.f;
@@ -908,49 +915,55 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     mbar_arrive_warp(&sh.p_full[q % 3], lane);
                 }
                 m -= lift<X>();  // what the weights were taken by
-#pragma unroll
-                for (int i = 0; i < 64; ++i) o[i] = 0.f;
-                if (ok && n > 0 && wait(sh.o_full[t], own - 1, W_O) && live) {
-                    tmem_ld32p(at_o, reinterpret_cast<uint32_t*>(o));
-                    tmem_ld32p(at_o + 32, reinterpret_cast<uint32_t*>(o) + 32);
-                    tmem_wait_ld();
-                    tc_fence_before_sync();
-                }
+                if (ok && n > 0) wait(sh.o_full[t], own - 1, W_O);
             }
             q0 += it.n0 + it.n1;
             if (!ok) break;
             // Where it goes is looked up again, not kept in registers all the while
             asm volatile("" ::: "memory");
+            // 32 columns of O at a time, in loops: this runs once an item, and what bounds it is how fast its instructions come.
             const int slot = it.slot;
-            if (slot >= 0) {
-                if (valid) {
-                    const int64_t at_slot = (int64_t)slot * C::BLOCK + r;
-                    a.ml[at_slot] = make_float2(m, l);
-                    float4* to = reinterpret_cast<float4*>(a.part + at_slot * 64);
+            const float f = slot >= 0 ? 1.f : l != 0.f ? rcp_approx(l) : 0.f;
+            const int b = TREE ? it.b : 0, row = it.begin + it.token0 + (valid ? my_token : 0), h = it.kvh * a.group + it.chunk * TILE + my_head;
+            X* const to = const_cast<X*>(row_of<X>(a.O, b, h, row));
+            const int64_t at_slot = (int64_t)slot * C::BLOCK + r;
+            if (LOW || slot >= 0) {
+                uint4* const whole = reinterpret_cast<uint4*>(slot >= 0 ? a.part + at_slot * 64 : reinterpret_cast<float*>(to));
+#pragma unroll(LOW ? 2 : 1)
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t y[32];
+                    if constexpr (LOW) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                }
-            } else {
-                const float f = l != 0.f ? 1.f / l : 0.f;
-                const int b = TREE ? it.b : 0, row = it.begin + it.token0 + (valid ? my_token : 0), h = it.kvh * a.group + it.chunk * TILE + my_head;
-                X* const to = const_cast<X*>(row_of<X>(a.O, b, h, row));
-                if constexpr (LOW) {
+                        for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(o[32 * half + i] * f);
+                    } else if (n > 0) {
+                        tmem_ld32(lanes + COL_O + t * 64 + 32 * half, y);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] = 0u;
+                    }
                     if (valid) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            reinterpret_cast<uint4*>(to)[i] = make_uint4(__float_as_uint(o[4 * i] * f), __float_as_uint(o[4 * i + 1] * f), __float_as_uint(o[4 * i + 2] * f), __float_as_uint(o[4 * i + 3] * f));
+                        for (int i = 0; i < 8; ++i) whole[8 * half + i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
                     }
-                } else {
-                    // Through shared memory, so that eight lanes store a row: a row to a lane is 32 lines an instruction, and all warps' stores of
-                    // an item took 1 700 cycles.
+                }
+            } else if (live) {
+                if constexpr (!LOW) {
+                    // Through shared memory, so that eight lanes store a row: a row to a lane is 32 lines an instruction.
                     uint4* const mine = reinterpret_cast<uint4*>(smem + Space::OFF_O + (warp - 4) * 4096);
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t y[32];
+                        tmem_ld32(lanes + COL_O + t * 64 + 32 * half, y);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        mine[lane * 8 + (i ^ (lane & 7))] = make_uint4(pack<X>(o[8 * i] * f, o[8 * i + 1] * f), pack<X>(o[8 * i + 2] * f, o[8 * i + 3] * f),
-                                                                       pack<X>(o[8 * i + 4] * f, o[8 * i + 5] * f), pack<X>(o[8 * i + 6] * f, o[8 * i + 7] * f));
+                        for (int i = 0; i < 16; ++i) y[i] = pack<X>(__uint_as_float(y[2 * i]) * f, __uint_as_float(y[2 * i + 1]) * f);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mine[lane * 8 + ((4 * half + i) ^ (lane & 7))] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                    }
                     __syncwarp();
                     const uint64_t place = valid ? reinterpret_cast<uint64_t>(to) : 0ull;
-#pragma unroll
+#pragma unroll 4
                     for (int i = 0; i < 8; ++i) {
                         const int from = 4 * i + (lane >> 3);
                         const uint64_t at = __shfl_sync(0xffffffffu, place, from);
@@ -959,7 +972,11 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     __syncwarp();
                 }
-                if (valid) a.LSE[b * a.lse_sB + h * a.lse_sH + row] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+            }
+            if (!LOW) tc_fence_before_sync();
+            if (valid) {
+                if (slot >= 0) a.ml[at_slot] = make_float2(m, l);
+                else a.LSE[b * a.lse_sB + h * a.lse_sH + row] = l != 0.f ? (m + __log2f(l)) * LN2 : -INFINITY;
             }
             mbar_arrive_warp(&sh.item_empty[get.at], lane);
             get.next(ITEMS);
