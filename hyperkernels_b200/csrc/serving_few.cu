@@ -1,0 +1,388 @@
+// serving_few.cu -- attention of few new tokens against a cache of pages (decoding, small trees): bound by reading keys and values.
+//
+// Every warp is a worker of its own: it has an equal stretch of all requests' keys (serving_attention.cuh), which TMA brings into a ring
+// of its own in batches of 8 (fp32) or 16 keys, two or three ahead, over the borders of requests.  A batch lies in one page.  Lengths and tables
+// are read where the batches are asked for, 32 entries of a table at a time, so no product waits for them.  A request whose keys fall to
+// several warps leaves its parts in slots; a second kernel adds them up in their order, with as many lanes to a row as its rows leave.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+
+#include "few_rows.cuh"
+#include "serving_attention.cuh"
+
+namespace hk {
+namespace {
+
+constexpr int WARPS = 4, ROWS_MOST = 16;
+
+template <int KEYS>
+using FewWork = Work<KEYS, 128 / KEYS, 128 / KEYS, 2 * KEYS, true>;
+
+struct Segment {  // a run as the products need it
+    int b, kvh, row0, rows, from, to, old, len, slot;
+};
+template <class Rows>
+struct FewShared {
+    uint8_t ring[WARPS][Rows::STAGES][4096];  // a batch's keys and values
+    Segment segments[WARPS][8];               // as many as can be on their way, and more
+    uint64_t full[WARPS][Rows::STAGES];
+    PartRecord record[WARPS];
+    Abort abort;
+};
+static_assert(sizeof(Segment) == 36, "");
+constexpr int W_FEW = 601;
+
+// The weighted sum of a row's values from registers to memory, scaled: fp32 in slots, or the result.
+template <class T, class P>
+__device__ __forceinline__ void store_rows(const RowsOf16<T>& w, int lane, int rows, float f0, float f1, P&& place) {
+    typedef typename RowsOf16<T>::Math Math;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = RowsOf16<T>::row(i, lane);
+        if (r >= rows) continue;
+        auto* const to = place(i);
+        const float f = i ? f1 : f0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int j = (k >> 1) * 4, e = 2 * i + (k & 1);
+            store4(to + Math::column(j, 2 * (lane & 3) + (k & 1)), make_float4(w.o[j][e] * f, w.o[j + 1][e] * f, w.o[j + 2][e] * f, w.o[j + 3][e] * f));
+        }
+    }
+}
+template <int N, class P>
+__device__ __forceinline__ void store_rows(const RowsOfOne<N>& w, int lane, int rows, float f0, float f1, P&& place) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i >= rows || lane >= 16) continue;
+        auto* const to = place(i);
+        const float f = i ? f1 : f0;
+        store4(to + 4 * lane, make_float4(w.o[i].x * f, w.o[i].y * f, w.o[i].z * f, w.o[i].w * f));
+    }
+}
+// Sums of the lanes that share a row; then every lane of a row has its maximum and sum.
+template <class T>
+__device__ __forceinline__ void join(RowsOf16<T>& w) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        w.l[i] += __shfl_xor_sync(0xffffffffu, w.l[i], 1);
+        w.l[i] += __shfl_xor_sync(0xffffffffu, w.l[i], 2);
+    }
+}
+template <int N>
+__device__ __forceinline__ void join(RowsOfOne<N>& w) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        w.l[i] += __shfl_xor_sync(0xffffffffu, w.l[i], 8);
+        w.l[i] += __shfl_xor_sync(0xffffffffu, w.l[i], 4);
+        const float other = __shfl_xor_sync(0xffffffffu, w.m[i], 16), m = fmaxf(w.m[i], other), ref = m == -INFINITY ? 0.f : m;
+        const float mine = ex2_approx(w.m[i] - ref), its = ex2_approx(other - ref);
+        w.l[i] = w.l[i] * mine + __shfl_xor_sync(0xffffffffu, w.l[i], 16) * its;
+        w.m[i] = m;
+        float* o = &w.o[i].x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = o[e] * mine + __shfl_xor_sync(0xffffffffu, o[e], 16) * its;
+    }
+}
+
+template <class Rows>
+__global__ void __launch_bounds__(WARPS * 32, Rows::CTAS)
+tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
+                const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ ServingArgs a) {
+    typedef typename Rows::X X;
+    typedef FewWork<Rows::KEYS> W;
+    constexpr int KEYS = Rows::KEYS, STAGES = Rows::STAGES, MINE = Rows::ROWS < 16 ? Rows::ROWS : 2;  // rows that a lane works on
+    extern __shared__ __align__(1024) uint8_t few_smem[];
+    FewShared<Rows>& sh = *reinterpret_cast<FewShared<Rows>*>(few_smem);
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, workers = gridDim.x * WARPS, me = warp * gridDim.x + blockIdx.x;
+    if (lane < (warp == 0 ? 4 : 0)) tma_prefetch_desc(lane == 0 ? &map_kp : lane == 1 ? &map_vp : lane == 2 ? &map_k : &map_v);
+    if (lane == 0) {
+        for (int s = 0; s < STAGES; ++s) mbar_init(&sh.full[warp][s], 1);
+        if (warp == 0) sh.abort.id = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();  // the record of waits that gave up
+    pdl_wait();
+    pdl_trigger();
+    const W work{a};
+    Line<W> line;
+    line.find(work, lane, me, workers);
+    WaitNote wc{&sh.abort};
+    PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
+
+    // Batches on their way: the run that they come from, the next one's number, 32 entries of the table from page `ids_at` on
+    Segment put = {};
+    int put_j = 0, put_slot = 0, put_segment = 0, ids = 0, ids_at = 0;
+    bool more = true;
+    auto copy_next = [&] {
+        __syncwarp();
+        if (!more) return;
+        if (put_j == put.to) {
+            Run run;
+            more = line.next(work, run);
+            if (more) {
+                put = {run.b, run.kvh, run.i * a.block_tokens, min(a.block_tokens, run.r.tokens - run.i * a.block_tokens), run.from, run.to, run.n - a.new_tiles, run.r.len, run.slot(me)};
+                put_j = run.from;
+                ids_at = INT_MAX;
+                if (run.from > 0) {
+                    record.head = run.to < run.n ? PART_GOES_ON : PART_LAST;
+                } else {
+                    if (record.head == PART_EMPTY) record.head = PART_NONE;
+                    if (run.to < run.n) record.b = put.b, record.head0 = put.kvh, record.token0 = put.row0, record.tokens = put.rows;
+                }
+            } else {
+                put.rows = 0;
+            }
+            if (lane == 0) sh.segments[warp][put_segment] = put;
+            put_segment = (put_segment + 1) & 7;
+            if (!more) return;
+        }
+        uint64_t* full = &sh.full[warp][put_slot];
+        uint8_t* to = sh.ring[warp][put_slot];
+        const int key = put_j * KEYS;
+        const bool old = put_j < put.old;
+        int row, b = put.b;
+        if (old) {
+            const int page = (int)(((uint64_t)(uint32_t)key * a.page_mul) >> a.page_shift);
+            row = key - page * a.pool.page;
+            if ((unsigned)(page - ids_at) >= 32u) {
+                ids_at = page;
+                ids = page + lane < a.pool.width ? __ldcg(a.pool.pages + b * a.pool.pages_stride + page + lane) : -1;
+            }
+            b = __shfl_sync(0xffffffffu, ids, page - ids_at);
+        } else {
+            row = key - put.old * KEYS;
+        }
+        if (lane == 0) {
+            mbar_arrive_expect_tx(full, 4096);
+            tma_load_tile(to, old ? &map_kp : &map_k, full, row, put.kvh, b);
+            tma_load_tile(to + 2048, old ? &map_vp : &map_v, full, row, put.kvh, b);
+        }
+        ++put_j;
+        put_slot = put_slot + 1 == STAGES ? 0 : put_slot + 1;
+    };
+
+    int get_slot = 0, get_segment = 0, j = 0;
+    uint32_t phase = 0;
+    Segment get = {};
+    bool ok = true;
+    Rows w;
+    uint64_t bits[MINE];
+    int token_of[MINE], head_of[MINE];
+    for (int i = 1 - STAGES;; ++i) {
+        copy_next();
+        if (i < 0) continue;
+        if (j == get.to) {  // the next run; between them the result of the one before
+            __syncwarp();
+            get = sh.segments[warp][get_segment];
+            get_segment = (get_segment + 1) & 7;
+            if (get.rows == 0) break;
+            j = get.from;
+            typename Rows::Query query;
+#pragma unroll
+            for (int k = 0; k < MINE; ++k) {
+                const int r = Rows::row(k, lane), row = get.row0 + r;
+                token_of[k] = (int)(((uint64_t)(uint32_t)row * a.group_mul) >> a.group_shift);
+                head_of[k] = get.kvh * a.group + row - token_of[k] * a.group;
+                const bool there = r < get.rows;
+                query.load(k, there ? row_of<X>(a.Q, get.b, head_of[k], token_of[k]) : nullptr, lane, true);
+                bits[k] = there && get.to > get.old ? tree_bits(a, get.b, token_of[k]) : 0ull;
+            }
+            w.start(query, a.flip);
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.full[warp][get_slot], phase, W_FEW, i))) {
+            for (const unsigned long long t0 = globaltimer_ns(); globaltimer_ns() - t0 < 100000ull;) {}  // copies in flight land
+            ok = false;
+            break;
+        }
+        {
+            const bool old = j < get.old;
+            const int key0 = (old ? j : j - get.old) * KEYS, end = old ? get.len : a.T;
+            w.batch(sh.ring[warp][get_slot], lane, key0, end, old && key0 + KEYS <= end, [&](int k, int key) { return old ? key < end : key < a.T && (bits[k] >> key & 1); }, a.scale_log2e,
+                    [] {});
+        }
+        if (++get_slot == STAGES) get_slot = 0, phase ^= 1u;
+        if (++j == get.to) {
+            join(w);
+            float f[2] = {1.f, 1.f};
+            if (get.slot >= 0) {
+                const int64_t at = (int64_t)get.slot * ROWS_MOST;
+                store_rows(w, lane, get.rows, 1.f, 1.f, [&](int k) { return a.part + (at + Rows::row(k, lane)) * 64; });
+#pragma unroll
+                for (int k = 0; k < MINE; ++k)
+                    if (Rows::row(k, lane) < get.rows && (Rows::ROWS < 16 ? lane == 0 : (lane & 3) == 0)) a.ml[at + Rows::row(k, lane)] = make_float2(w.m[k], w.l[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < MINE; ++k) f[k] = w.l[k] != 0.f ? 1.f / w.l[k] : 0.f;
+                store_rows(w, lane, get.rows, f[0], f[1], [&](int k) { return const_cast<X*>(row_of<X>(a.O, get.b, head_of[k], token_of[k])); });
+#pragma unroll
+                for (int k = 0; k < MINE; ++k)
+                    if (Rows::row(k, lane) < get.rows && (Rows::ROWS < 16 ? lane == 0 : (lane & 3) == 0))
+                        a.LSE[get.b * a.lse_sB + head_of[k] * a.lse_sH + token_of[k]] = w.l[k] != 0.f ? (w.m[k] + log2f(w.l[k])) * LN2 : -INFINITY;
+            }
+        }
+    }
+    (void)ok;
+    if (a.parts && lane == 0) a.parts[me] = record;
+    __syncthreads();
+    if (threadIdx.x == 0) report_abort(sh.abort, a.status);
+}
+
+// The parts of each block that fell to several warps, added up in an order of their own: 16 lanes to a part of a row, and as many parts
+// at once as there are lanes left.
+constexpr int GROUPS = 8;
+template <class X>
+__global__ void __launch_bounds__(GROUPS * 16) few_combine_kernel(const __grid_constant__ ServingArgs a, const int workers) {
+    __shared__ float4 sums[GROUPS][16];
+    __shared__ float2 mls[GROUPS];
+    pdl_wait();
+    pdl_trigger();
+    const int first = blockIdx.x;
+    const PartRecord rec = a.parts[first];
+    if (rec.tokens == 0) return;
+    const int last = last_part(a, first, workers), n = last - first + 1;
+    const int sub = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const uint32_t together = threadIdx.x & 16 ? 0xffff0000u : 0xffffu;
+    int side = 1;  // groups to a row
+    while (side * 2 * rec.tokens <= GROUPS && side < n) side *= 2;
+    const int rows_at_once = GROUPS / side;
+    for (int r0 = 0; r0 < rec.tokens; r0 += rows_at_once) {
+        const int r = r0 + g / side, p_first = g % side;
+        float M = -INFINITY, L = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rec.tokens) {
+            for (int p0 = p_first; p0 < n; p0 += 16 * side) {
+                // a lane looks up one part
+                const int p = p0 + sub * side, worker = first + p;
+                int head = PART_EMPTY;
+                if (p < n) head = p == 0 ? PART_GOES_ON : a.parts[worker].head;
+                const bool there = head == PART_GOES_ON || head == PART_LAST;
+                const int slot = 2 * worker + (p == 0);
+                const float2 x = there ? a.ml[(int64_t)slot * ROWS_MOST + r] : make_float2(-INFINITY, 0.f);
+                float mx = x.x;
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(together, mx, off));
+                mx = fmaxf(mx, M);
+                const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(M - ref), w = there && x.y != 0.f ? ex2_approx(x.x - ref) : 0.f;
+                M = mx;
+                float sum = x.y * w;
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(together, sum, off);
+                L = L * old + sum;
+                o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+                const int parts = min(16, (n - p0 + side - 1) / side);
+                for (int i = 0; i < parts; i += 4) {
+                    float4 v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int from = __shfl_sync(together, slot, i + k, 16), is = __shfl_sync(together, (int)there, i + k, 16);
+                        v[k] = is ? *reinterpret_cast<const float4*>(a.part + ((int64_t)from * ROWS_MOST + r) * 64 + 4 * sub) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float f = __shfl_sync(together, w, i + k, 16);
+                        o.x = fmaf(v[k].x, f, o.x); o.y = fmaf(v[k].y, f, o.y); o.z = fmaf(v[k].z, f, o.z); o.w = fmaf(v[k].w, f, o.w);
+                    }
+                }
+            }
+        }
+        if (side > 1) {
+            __syncthreads();
+            sums[g][sub] = o;
+            if (sub == 0) mls[g] = make_float2(M, L);
+            __syncthreads();
+            if (p_first == 0) {
+                for (int k = 1; k < side; ++k) M = fmaxf(M, mls[g + k].x);
+                const float ref = M == -INFINITY ? 0.f : M;
+                L = 0.f;
+                o = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < side; ++k) {
+                    const float2 x = mls[g + k];
+                    const float f = ex2_approx(x.x - ref);
+                    const float4 v = sums[g + k][sub];
+                    L = fmaf(x.y, f, L);
+                    o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+                }
+            }
+        }
+        if (r < rec.tokens && p_first == 0) {
+            const float f = L != 0.f ? 1.f / L : 0.f;
+            const int row = rec.token0 + r, token = (int)(((uint64_t)(uint32_t)row * a.group_mul) >> a.group_shift), h = rec.head0 * a.group + row - token * a.group;
+            store4(const_cast<X*>(row_of<X>(a.O, rec.b, h, token)) + 4 * sub, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+            if (sub == 0) a.LSE[rec.b * a.lse_sB + h * a.lse_sH + token] = L != 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
+        }
+    }
+}
+
+typedef void (*Kernel)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, ServingArgs);
+struct Entry {
+    Kernel kernel;
+    size_t smem;
+    int per_sm, keys, rows;
+};
+template <class Rows>
+Entry entry() {
+    return {tree_few_kernel<Rows>, sizeof(FewShared<Rows>), Rows::CTAS, Rows::KEYS, Rows::ROWS};
+}
+Entry pick(int dtype, int rows) {
+    if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>>();
+    if (dtype == HK_F16) return entry<RowsOf16<__half>>();
+    return rows == 1 ? entry<RowsOfOne<1>>() : rows == 2 ? entry<RowsOfOne<2>>() : entry<RowsOf16<float>>();
+}
+void divide_by(int d, uint32_t& mul, int& shift) {
+    shift = 31;
+    while ((1LL << (shift - 31)) < d) ++shift;
+    mul = (uint32_t)(((1ULL << shift) + d - 1) / d);
+}
+
+}  // namespace
+
+TreeFewPlan tree_few_plan(int dtype, int rows) {
+    const Entry e = pick(dtype, rows);
+    return {ROWS_MOST, e.keys, 128 / e.keys, sm_count() * e.per_sm * WARPS};
+}
+
+int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
+    a.rows = a.T * a.group;
+    const Entry e = pick(dtype, a.rows);
+    // once per device and kernel: more than 48 KB of shared memory
+    static std::mutex mu;
+    static Kernel known[HK_MAX_DEVICES][8];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        for (Kernel& x : known[dev]) {
+            if (x == e.kernel) break;
+            if (x) continue;
+            if (cudaFuncSetAttribute(e.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)e.smem) != cudaSuccess) return check_launch();
+            x = e.kernel;
+            break;
+        }
+    }
+    a.block_tokens = std::min(a.rows, e.rows);
+    a.chunks = 1;
+    a.new_tiles = cdiv(a.T, e.keys);
+    set_line(a, true, e.keys);
+    divide_by(a.group, a.group_mul, a.group_shift);
+    divide_by(a.pool.page, a.page_mul, a.page_shift);
+    CUtensorMap k, v, kp, vp;
+    int s;
+    if ((s = prefix_tile_map(&k, a.K, dtype, a.B, a.Hk, a.T, e.keys, false)) || (s = prefix_tile_map(&v, a.V, dtype, a.B, a.Hk, a.T, e.keys, false)) ||
+        (s = prefix_tile_map(&kp, a.pool.K, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false)) ||
+        (s = prefix_tile_map(&vp, a.pool.V, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false)))
+        return s;
+    const int ctas = sm_count() * e.per_sm;
+    LaunchConfig lc(ctas, WARPS * 32, e.smem, stream, 1, true);
+    if (cudaLaunchKernelEx(&lc.cfg, e.kernel, k, v, kp, vp, a) != cudaSuccess) return check_launch();
+    count_launch();
+    if (!a.parts) return HK_OK;
+    typedef void (*Combine)(ServingArgs, int);
+    static const Combine combine[] = {few_combine_kernel<float>, few_combine_kernel<__nv_bfloat16>, few_combine_kernel<__half>};
+    LaunchConfig sum(ctas * WARPS, GROUPS * 16, 0, stream, 1, true);
+    if (cudaLaunchKernelEx(&sum.cfg, combine[dtype], a, ctas * WARPS) != cudaSuccess) return check_launch();
+    count_launch();
+    return HK_OK;
+}
+
+}  // namespace hk

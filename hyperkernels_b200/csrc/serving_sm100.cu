@@ -41,6 +41,10 @@ struct Rows {
     static constexpr int ITEMS = 8;
 };
 
+// half a tile is masked, and a block's beginning and end take as long as a tile
+template <class X, bool TREE>
+using RowsWork = Work<Rows<X>::KEYS, Rows<X>::LEAST, 3 * Rows<X>::LEAST, Rows<X>::KEYS * 3 / 2, TREE>;
+
 struct __align__(16) Item {
     int b, kvh, chunk;   // request, key head, which 128 of its query heads
     int token0, tokens;  // of the request; no tokens: the end
@@ -76,134 +80,6 @@ struct RowsSpace {
 constexpr uint32_t COL_O = 384, LOW_COL_LOW = 192, LOW_COL_O = 320, LOW_COL_Q = 384;
 
 enum RowsWait { W_Q = 501, W_Q_EMPTY, W_KV, W_READY, W_EMPTY, W_S, W_P, W_O, W_ITEM, W_ITEM_EMPTY };
-
-// ---------------------------------------------------------------------------
-// How the work is cut: a block counts as the keys that it meets and EXTRA for its beginning and end.
-// ---------------------------------------------------------------------------
-// (Units of 2^unit_shift keys, so that all of them fit 32 bits: a division of 64-bit numbers takes a warp some 300 cycles.)
-struct Request {
-    int begin, len, tokens, blocks;  // blocks: of tokens
-    int units;                       // of all of its blocks, under one key head
-};
-template <class X, bool TREE>
-struct Work {
-    typedef Rows<X> C;
-    static constexpr int EXTRA = C::KEYS * 3 / 2;  // half a tile is masked
-    const ServingArgs& a;
-    __device__ __forceinline__ int all_tiles(const Request& r) const { return (r.len + C::KEYS - 1) / C::KEYS + TREE; }
-    __device__ __forceinline__ int tiles(const Request& r, int i) const {
-        return TREE || !a.causal ? all_tiles(r) : (min((i + 1) * a.block_tokens, r.len) + C::KEYS - 1) / C::KEYS;
-    }
-    // units in front of block i, of one chunk of heads
-    __device__ __forceinline__ int before(const Request& r, int i) const {
-        const int64_t keys = TREE || !a.causal ? (int64_t)i * (all_tiles(r) * C::KEYS + EXTRA) : (int64_t)i * (i + 1) / 2 * a.block_tokens + (int64_t)i * EXTRA;
-        return (int)(keys >> a.unit_shift);
-    }
-    __device__ __forceinline__ Request request(int b) const {
-        Request r;
-        if (TREE) {
-            r.begin = 0;
-            r.len = cache_keys(a, b);
-            r.tokens = a.T;
-        } else {
-            r.begin = min(max(a.starts[b], 0), a.N);
-            r.len = r.tokens = max(0, min(max(a.starts[b + 1], 0), a.N) - r.begin);
-        }
-        r.blocks = (int)(((uint64_t)(uint32_t)(r.tokens + a.block_tokens - 1) * a.block_mul) >> a.block_shift);
-        r.units = before(r, r.blocks) * a.chunks;
-        return r;
-    }
-};
-__device__ __forceinline__ int warp_scan(int x, int lane) {
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, off);
-        if (lane >= off) x += y;
-    }
-    return x;
-}
-
-// Where this CTA's stretch of the line begins: in block i of request b under key head kvh (blocks of the first chunk of heads, of the
-// second, ..), `done` units behind the block's beginning; and how many units it has from there.
-struct Stretch {
-    Request r;
-    int b, kvh, chunk, i;
-    int done, units;
-};
-// By one warp; no units: there is nothing for this CTA.
-template <class X, bool TREE>
-__device__ __forceinline__ Stretch find_stretch(const ServingArgs& a, int lane) {
-    typedef Rows<X> C;
-    const Work<X, TREE> work{a};
-    constexpr int EACH = 2;  // requests of a lane
-    Stretch s = {};
-    int units[EACH], sum = 0, all = 0, blocks = 0;
-    auto take = [&](int b0) {
-        sum = 0;
-#pragma unroll
-        for (int k = 0; k < EACH; ++k) {
-            const int b = b0 + lane * EACH + k;
-            units[k] = 0;
-            if (b < a.B) {
-                const Request r = work.request(b);
-                units[k] = r.units;
-                blocks += r.blocks * a.chunks;
-            }
-            sum += units[k];
-        }
-        return warp_scan(sum, lane);
-    };
-    int upto = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
-        upto = take(b0);
-        all += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    all *= a.Hk;
-    // A CTA to a block, more if the blocks are long, as many as there are
-    const int n_blocks = (int)min((int64_t)gridDim.x, (int64_t)__reduce_add_sync(0xffffffffu, min(blocks, 1 << 20)) * a.Hk);
-    const int ctas = min((int)gridDim.x, max(n_blocks, all / max(1, 3 * C::LEAST * C::KEYS >> a.unit_shift)));
-    const int me = blockIdx.x;
-    if (me >= ctas) return s;
-    const int share = (unsigned)all / (unsigned)ctas, more = all - share * ctas;
-    int left = me * share + min(me, more);
-    s.units = share + (me < more);
-    for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
-        if (a.B > 32 * EACH) upto = take(b0);  // otherwise they are here still
-        const unsigned here = __ballot_sync(0xffffffffu, left < upto * a.Hk);
-        if (!here) {
-            left -= __shfl_sync(0xffffffffu, upto, 31) * a.Hk;
-            continue;
-        }
-        const int l = __ffs(here) - 1;
-        left -= (upto - sum) * a.Hk;
-        int k = 0;
-#pragma unroll
-        for (int m = 0; m < EACH - 1; ++m)
-            if (k == m && left >= units[m] * a.Hk) left -= units[m] * a.Hk, ++k;
-        left = __shfl_sync(0xffffffffu, left, l);
-        s.b = b0 + l * EACH + __shfl_sync(0xffffffffu, k, l);
-        break;
-    }
-    s.r = work.request(s.b);
-    s.kvh = (unsigned)left / (unsigned)s.r.units;
-    left -= s.kvh * s.r.units;
-    s.chunk = 0;
-    if (a.chunks > 1) {
-        const int one = s.r.units / a.chunks;
-        s.chunk = left / one;
-        left -= s.chunk * one;
-    }
-    int lo = 0, len = s.r.blocks;  // the last block that begins at or before it
-    while (len > 1) {
-        const int step = (len + 31) / 32;
-        const int c = __popc(__ballot_sync(0xffffffffu, lane * step < len && work.before(s.r, lo + lane * step) <= left));
-        lo += (c - 1) * step;
-        len = min(step, len - (c - 1) * step);
-    }
-    s.i = lo;
-    s.done = left - work.before(s.r, lo);
-    return s;
-}
 
 // A product's place in the CTA's items, in the order they are issued in: tile by tile, stream by stream
 struct Cursor {
@@ -307,8 +183,8 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
     pdl_wait();
     pdl_trigger();
-    Stretch line = {};
-    if (warp == 0) line = find_stretch<X, TREE>(a, lane);
+    Line<RowsWork<X, TREE>> line = {};
+    if (warp == 0) line.find(RowsWork<X, TREE>{a}, lane, blockIdx.x, gridDim.x);
     __syncthreads();
     tc_fence_after_sync();
     constexpr uint32_t tmem = 0;  // all columns are this CTA's
@@ -321,61 +197,35 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         if (warp == 0) {
             // ------------------------------ items, tiles of keys and values ------------------------------
-            const Work<X, TREE> work{a};
+            const RowsWork<X, TREE> work{a};
             bool ok = true;
             PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
-            // A border inside a block is moved to its beginning or end where a part of less than LEAST tiles would be left.
-            auto border = [&](int units, int n) {
-                const int j = (int)min((int64_t)n, ((int64_t)units << a.unit_shift) / KEYS);
-                return j == n ? n : j < C::LEAST ? 0 : n - j < C::LEAST ? n : j;
-            };
             // The next item into the ring; one without tokens at the end of the stretch
             auto publish = [&](Item& it) {
+                Run run;
                 it.tokens = 0;
-                while (line.units > 0) {
-                    if (line.i >= line.r.blocks) {
-                        line.i = 0;
-                        if (line.r.blocks == 0 || ++line.chunk == a.chunks) {
-                            line.chunk = 0;
-                            if (line.r.blocks == 0 || ++line.kvh == a.Hk) {
-                                line.kvh = 0;
-                                if (++line.b >= a.B) break;
-                                line.r = work.request(line.b);
-                            }
-                        }
-                        continue;
+                if (!line.next(work, run)) return;
+                const int count = run.to - run.from;
+                it.b = run.b; it.kvh = run.kvh; it.chunk = run.chunk;
+                it.token0 = run.i * a.block_tokens;
+                it.tokens = min(a.block_tokens, run.r.tokens - it.token0);
+                it.begin = run.r.begin; it.len = run.r.len; it.key0 = run.from * KEYS;
+                it.new_tile = TREE ? run.n - 1 - run.from : -1;
+                it.n0 = count;
+                it.n1 = 0;
+                if (!LOW && it.tokens > a.stream_tokens) {
+                    it.n1 = count;
+                    if (!TREE && a.causal) it.n0 = max(0, min((it.token0 + a.stream_tokens + KEYS - 1) / KEYS - run.from, count));
+                }
+                it.slot = run.slot(blockIdx.x);
+                if (run.from > 0) {
+                    record.head = run.to < run.n ? PART_GOES_ON : PART_LAST;
+                } else {
+                    if (record.head == PART_EMPTY) record.head = PART_NONE;
+                    if (run.to < run.n) {
+                        record.b = TREE ? it.b : 0; record.head0 = it.kvh * a.group + it.chunk * TILE; record.heads = min(TILE, a.group - it.chunk * TILE);
+                        record.token0 = it.begin + it.token0; record.tokens = it.tokens;
                     }
-                    const int i = line.i, n = work.tiles(line.r, i);
-                    const int j0 = border(line.done, n), to = border(line.done + line.units, n);
-                    line.units -= work.before(line.r, i + 1) - work.before(line.r, i) - line.done;
-                    line.done = 0;
-                    ++line.i;
-                    if (to <= j0) continue;
-                    const int count = to - j0;
-                    it.b = line.b; it.kvh = line.kvh; it.chunk = line.chunk;
-                    it.token0 = i * a.block_tokens;
-                    it.tokens = min(a.block_tokens, line.r.tokens - it.token0);
-                    it.begin = line.r.begin; it.len = line.r.len; it.key0 = j0 * KEYS;
-                    it.new_tile = TREE ? n - 1 - j0 : -1;
-                    it.n0 = count;
-                    it.n1 = 0;
-                    if (!LOW && it.tokens > a.stream_tokens) {
-                        it.n1 = count;
-                        if (!TREE && a.causal) it.n0 = max(0, min((it.token0 + a.stream_tokens + KEYS - 1) / KEYS - j0, count));
-                    }
-                    it.slot = -1;
-                    if (j0 > 0) {
-                        it.slot = 2 * blockIdx.x;
-                        record.head = to < n ? PART_GOES_ON : PART_LAST;
-                    } else {
-                        if (record.head == PART_EMPTY) record.head = PART_NONE;
-                        if (to < n) {
-                            it.slot = 2 * blockIdx.x + 1;
-                            record.b = TREE ? it.b : 0; record.head0 = it.kvh * a.group + it.chunk * TILE; record.heads = min(TILE, a.group - it.chunk * TILE);
-                            record.token0 = it.begin + it.token0; record.tokens = it.tokens;
-                        }
-                    }
-                    break;
                 }
             };
             Turn put{0, 0u};
@@ -1037,11 +887,7 @@ __global__ void __launch_bounds__(256) serving_combine_kernel(const __grid_const
     const PartRecord rec = a.parts[blockIdx.x];
     const int sub = threadIdx.x & 15, r0 = blockIdx.y * 64;
     if (rec.tokens == 0) return;
-    int last = blockIdx.x;  // the CTA that has the last part
-    while (++last < ctas - 1) {
-        const int head = a.parts[last].head;
-        if (head != PART_GOES_ON && head != PART_EMPTY) break;
-    }
+    const int last = last_part(a, blockIdx.x, ctas);
     const int n = last - (int)blockIdx.x + 1;
     const uint32_t together = threadIdx.x & 16 ? 0xffff0000u : 0xffffu;
     for (int r = r0 + (int)threadIdx.x / 16; r < r0 + 64; r += 16) {
@@ -1127,17 +973,11 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
     std::call_once(once[dev], [dev] { rc[dev] = cudaFuncSetAttribute(serving_rows_kernel<X, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSpace<X>::SMEM); });
     if (rc[dev] != cudaSuccess) return HK_ERR_CUDA;
-    {  // what all requests can come to, in keys
-        const double tokens = TREE ? (double)a.B * a.T : a.N, keys = TREE ? (double)a.pool.width * a.pool.page + 2 * C::KEYS : a.N + 2.0 * C::BLOCK, rows = std::max(1, TILE / a.group) * C::STREAMS;
-        double all = (tokens / rows + a.B) * (keys + 2 * C::KEYS) * a.Hk * cdiv(a.group, TILE);
-        for (a.unit_shift = 0; all >= 2e9; all /= 2) ++a.unit_shift;
-    }
     a.stream_tokens = std::max(1, TILE / a.group);
     a.block_tokens = C::STREAMS * a.stream_tokens;
     a.chunks = cdiv(a.group, TILE);
-    a.block_shift = 31;
-    while ((1LL << (a.block_shift - 31)) < a.block_tokens) ++a.block_shift;
-    a.block_mul = (uint32_t)(((1ULL << a.block_shift) + a.block_tokens - 1) / a.block_tokens);
+    a.new_tiles = 1;
+    set_line(a, TREE, C::KEYS);
     CUtensorMap k, v, kp, vp;
     const int B = TREE ? a.B : 1;
     const int64_t T = TREE ? a.T : a.N;
