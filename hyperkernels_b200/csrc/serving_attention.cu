@@ -7,6 +7,111 @@
 namespace hk {
 namespace {
 
+// ---------------------------------------------------------------------------
+// The parts of each block that fell to several workers, added up in an order of their own: 16 lanes to a part of a row, and as many parts
+// of a row at once as there are lanes left.  The block begins in the second slot of a worker and goes on in the first ones of those behind it.
+// Latency bounds it: what is looked up is asked for at once, whether there turns out to be such a part or not.
+// ---------------------------------------------------------------------------
+constexpr int GROUPS = 16;
+
+template <class X>
+__global__ void __launch_bounds__(GROUPS * 16) combine_kernel(const __grid_constant__ ServingArgs a, const int workers) {
+    __shared__ float4 sums[GROUPS][16];
+    __shared__ float2 mls[GROUPS];
+    pdl_wait();
+    pdl_trigger();
+    const int first = blockIdx.x;
+    const PartRecord rec = a.parts[first];
+    int n = 0;  // parts: up to the first worker behind that has the last one
+    for (int w0 = first + 1; n == 0; w0 += 32) {
+        const int w = min(w0 + (int)(threadIdx.x & 31), workers - 1), head = a.parts[w].head;
+        if (rec.tokens == 0) return;
+        const unsigned stops = __ballot_sync(0xffffffffu, w == workers - 1 || (head != PART_GOES_ON && head != PART_EMPTY));
+        if (stops) n = min(w0 + __ffs(stops) - 1, workers - 1) - first + 1;
+    }
+    const int sub = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const uint32_t together = threadIdx.x & 16 ? 0xffff0000u : 0xffffu;
+    const int rows = a.rows ? rec.tokens : a.slot_rows, per = (rows + gridDim.y - 1) / gridDim.y, r_end = min(rows, (int)(blockIdx.y + 1) * per);
+    int side = 1;  // groups to a row
+    while (side * 2 * per <= GROUPS && side < n) side *= 2;
+    for (int r0 = blockIdx.y * per; r0 < r_end; r0 += GROUPS / side) {
+        const int r = r0 + g / side, p_first = g % side;
+        // the token and the head that row r is
+        int token, h;
+        bool valid = r < r_end;
+        if (a.rows) {
+            const int row = rec.token0 + r;
+            token = row / a.group;
+            h = rec.head0 * a.group + row - token * a.group;
+        } else {
+            const int t = r / TILE, box_heads = min(a.group, TILE), in_stream = r - t * TILE, token_in = in_stream / box_heads, head = in_stream - token_in * box_heads;
+            token = t * a.stream_tokens + token_in;
+            valid = valid && token_in < a.stream_tokens && token < rec.tokens && head < rec.heads;
+            token += rec.token0;
+            h = rec.head0 + head;
+        }
+        float M = -INFINITY, L = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (valid) {
+            for (int p0 = p_first; p0 < n; p0 += 8 * side) {
+                // eight parts; a lane looks up one
+                const int p = p0 + (sub & 7) * side, worker = min(first + p, workers - 1), slot = 2 * worker + (p == 0);
+                const int head = p == 0 ? PART_GOES_ON : a.parts[worker].head;
+                const float2 ml = a.ml[(int64_t)slot * a.slot_rows + r];
+                float4 v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int q = p0 + k * side, from = 2 * min(first + q, workers - 1) + (q == 0);
+                    v[k] = q < n ? *reinterpret_cast<const float4*>(a.part + ((int64_t)from * a.slot_rows + r) * 64 + 4 * sub) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                const bool there = p < n && (head == PART_GOES_ON || head == PART_LAST);
+                const float2 x = there ? ml : make_float2(-INFINITY, 0.f);
+                float mx = x.x;
+#pragma unroll
+                for (int off = 4; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(together, mx, off));
+                mx = fmaxf(mx, M);
+                const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(M - ref), w = there && x.y != 0.f ? ex2_approx(x.x - ref) : 0.f;
+                M = mx;
+                float sum = x.y * w;
+#pragma unroll
+                for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(together, sum, off);
+                L = L * old + sum;
+                o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float f = __shfl_sync(together, w, k, 16);
+                    if (!__shfl_sync(together, (int)there, k, 16)) continue;  // what nobody wrote may be anything
+                    o.x = fmaf(v[k].x, f, o.x); o.y = fmaf(v[k].y, f, o.y); o.z = fmaf(v[k].z, f, o.z); o.w = fmaf(v[k].w, f, o.w);
+                }
+            }
+        }
+        if (side > 1) {
+            __syncthreads();
+            sums[g][sub] = o;
+            if (sub == 0) mls[g] = make_float2(M, L);
+            __syncthreads();
+            if (p_first == 0) {
+                for (int k = 1; k < side; ++k) M = fmaxf(M, mls[g + k].x);
+                const float ref = M == -INFINITY ? 0.f : M;
+                L = 0.f;
+                o = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < side; ++k) {
+                    const float2 x = mls[g + k];
+                    const float f = ex2_approx(x.x - ref);
+                    const float4 v = sums[g + k][sub];
+                    L = fmaf(x.y, f, L);
+                    o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+                }
+            }
+        }
+        if (valid && p_first == 0) {
+            const float f = L != 0.f ? 1.f / L : 0.f;
+            store4(const_cast<X*>(row_of<X>(a.O, rec.b, h, token)) + 4 * sub, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+            if (sub == 0) a.LSE[rec.b * a.lse_sB + h * a.lse_sH + token] = L != 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
+        }
+    }
+}
+
 int check_heads(int64_t B, int nh, int nh_kv, int dtype, float scale) {
     if (dtype < HK_F32 || dtype > HK_F16) return HK_ERR_UNSUPPORTED;
     if (B <= 0 || nh <= 0 || nh_kv <= 0 || nh % nh_kv) return HK_ERR_BAD_SHAPE;
@@ -37,28 +142,29 @@ int check_sizes(const hk_tree_params* p) {
 
 // Slots for what workers leave of blocks that fell to several, if any can: `tiles` are the most that a block meets.
 struct Parts {
-    int workers, rows;
+    int workers, slots, rows;  // slots: of a worker, in pairs
     bool any;
-    size_t bytes() const { return any ? (size_t)workers * (2 * rows * (64 * sizeof(float) + sizeof(float2)) + sizeof(PartRecord)) : 0; }
+    size_t all_rows() const { return (size_t)workers * 2 * slots * rows; }
+    size_t bytes() const { return any ? all_rows() * (64 * sizeof(float) + sizeof(float2)) + workers * sizeof(PartRecord) : 0; }
 };
 Parts parts_of(const hk_prompt_params* p) {
     const RowsPlan plan = rows_plan(p->dtype);
-    return {sm_count(), plan.rows, (p->N + plan.keys - 1) / plan.keys >= 2 * plan.least};
+    return {sm_count(), 1, plan.rows, (p->N + plan.keys - 1) / plan.keys >= 2 * plan.least};
 }
 bool few_rows(const hk_tree_params* p) { return p->T * (p->nh / p->nh_kv) <= 16; }
 Parts parts_of(const hk_tree_params* p) {
     const int64_t keys = (int64_t)p->pool.width * p->pool.page;
     if (few_rows(p)) {
         const TreeFewPlan plan = tree_few_plan(p->dtype, (int)(p->T * (p->nh / p->nh_kv)));
-        return {plan.workers, plan.rows, keys / plan.keys + cdiv(p->T, plan.keys) >= 2 * plan.least};
+        return {plan.workers, plan.slots, plan.rows, keys / plan.keys + cdiv(p->T, plan.keys) >= 2 * plan.least};
     }
     const RowsPlan plan = rows_plan(p->dtype);
-    return {sm_count(), plan.rows, (keys + plan.keys - 1) / plan.keys + 1 >= 2 * plan.least};
+    return {sm_count(), 1, plan.rows, (keys + plan.keys - 1) / plan.keys + 1 >= 2 * plan.least};
 }
 int set_parts(ServingArgs& a, const Parts& parts, void* workspace, size_t bytes) {
     if (!parts.any) return HK_OK;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || bytes < parts.bytes()) return HK_ERR_WORKSPACE;
-    const size_t rows = (size_t)parts.workers * 2 * parts.rows;
+    const size_t rows = parts.all_rows();
     a.part = static_cast<float*>(workspace);
     a.ml = reinterpret_cast<float2*>(a.part + rows * 64);
     a.parts = reinterpret_cast<PartRecord*>(a.ml + rows);
@@ -81,6 +187,16 @@ void set_line(ServingArgs& a, bool tree, int keys) {
     const double blocks = (tree ? (double)a.B * cdiv(a.rows ? a.rows : a.T, a.block_tokens) : (double)a.N / a.block_tokens + a.B) * a.Hk * a.chunks;
     double all = blocks * ((tree ? (double)a.pool.width * a.pool.page + a.new_tiles * keys : a.N + a.block_tokens) + 4.0 * keys);
     for (a.unit_shift = 0; all >= 2e9; all /= 2) ++a.unit_shift;
+}
+
+int launch_combine(const ServingArgs& a, int dtype, int workers, cudaStream_t stream) {
+    typedef void (*Kernel)(ServingArgs, int);
+    static const Kernel kernels[] = {combine_kernel<float>, combine_kernel<__nv_bfloat16>, combine_kernel<__half>};
+    LaunchConfig lc(workers, GROUPS * 16, 0, stream, 1, true);
+    lc.cfg.gridDim.y = cdiv(a.slot_rows, GROUPS);
+    if (cudaLaunchKernelEx(&lc.cfg, kernels[dtype], a, workers) != cudaSuccess) return check_launch();
+    count_launch();
+    return HK_OK;
 }
 
 }  // namespace hk

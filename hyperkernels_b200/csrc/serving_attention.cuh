@@ -40,7 +40,8 @@ struct ServingArgs {
     int stream_tokens, q_bytes;  // many rows: tokens of a stream, bytes of its queries
     int box;            // rows of a page that are loaded at once
     // slots of the workspace, and who has what in them; no parts: blocks are not cut
-    float2* ml;         // [slots][rows]
+    int slot_rows;
+    float2* ml;         // [slots][slot_rows]
     float* part;        // the same, [64]
     PartRecord* parts;
     DeviceStatus* status;
@@ -93,6 +94,12 @@ struct Run {
     int b, kvh, chunk, i, from, to, n;
     __device__ __forceinline__ int slot(int worker) const { return from > 0 ? 2 * worker : to < n ? 2 * worker + 1 : -1; }  // -1: the result
 };
+// Where N stretches of the line begin, found by a whole CTA.
+template <int N>
+struct LineSearch {
+    int sums[32], blocks[32];  // of the warps' requests
+    int b[N], left[N];         // a stretch's first request, and how far behind its beginning
+};
 // A worker's stretch of the line: it begins in block i of request b under key head kvh (blocks of the first chunk of heads, of the second,
 // ..), `done` units behind the block's beginning, and goes on for `units`.
 template <class W>
@@ -100,65 +107,65 @@ struct Line {
     Request r;
     int b, kvh, chunk, i, done, units;
 
-    // By one warp.
-    __device__ __forceinline__ void find(const W& work, int lane, int me, int workers) {
+    // The stretches of worker `me` of at most `workers`, cut in N (of a CTA's warps, say), by all threads.  Stretch k is made for the threads
+    // that ask for it; those of a warp have to ask for the same.
+    template <int N>
+    __device__ __forceinline__ void find(const W& work, LineSearch<N>& sh, int me, int workers, int k) {
         const ServingArgs& a = work.a;
-        constexpr int EACH = 2;  // requests of a lane
-        int each[EACH], sum = 0, all = 0, blocks = 0;
-        auto take = [&](int b0) {
-            sum = 0;
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, each = (a.B + (int)blockDim.x - 1) / (int)blockDim.x;
+        int sum = 0, n = 0;
+        for (int x = 0; x < each; ++x) {
+            if (tid * each + x >= a.B) break;
+            const Request one = work.request(tid * each + x);
+            sum += one.units;
+            n += min(one.blocks * a.chunks, 1 << 20);
+        }
+        int upto = sum;
 #pragma unroll
-            for (int k = 0; k < EACH; ++k) {
-                const int b = b0 + lane * EACH + k;
-                each[k] = 0;
-                if (b < a.B) {
-                    const Request x = work.request(b);
-                    each[k] = x.units;
-                    blocks += x.blocks * a.chunks;
-                }
-                sum += each[k];
-            }
-            int upto = sum;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, upto, off);
-                if (lane >= off) upto += y;
-            }
-            return upto;
-        };
-        units = 0;
-        int upto = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
-            upto = take(b0);
-            all += __shfl_sync(0xffffffffu, upto, 31);
+        for (int off = 1; off < 32; off <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, off);
+            if (lane >= off) upto += y;
+        }
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane == 31) {
+            sh.sums[warp] = upto;
+            sh.blocks[warp] = n;
+        }
+        if (tid < N) sh.b[tid] = -1;
+        __syncthreads();
+        int all = 0, from = upto - sum;
+        n = 0;
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) from += sh.sums[w];
+            all += sh.sums[w];
+            n = min(n + sh.blocks[w], 1 << 20);
         }
         all *= a.Hk;
-        // a worker to a block, more if the blocks are long, as many as there are
-        const int n_blocks = (int)min((int64_t)workers, (int64_t)__reduce_add_sync(0xffffffffu, min(blocks, 1 << 20)) * a.Hk);
-        workers = min(workers, max(n_blocks, all / max(1, W::SHARE * W::KEYS >> a.unit_shift)));
-        if (me >= workers) return;
-        const int share = (unsigned)all / (unsigned)workers, more = all - share * workers;
-        int left = me * share + min(me, more);
-        units = share + (me < more);
-        b = -1;
-        for (int b0 = 0; b0 < a.B; b0 += 32 * EACH) {
-            if (a.B > 32 * EACH) upto = take(b0);  // otherwise they are here still
-            const unsigned here = __ballot_sync(0xffffffffu, left < upto * a.Hk);
-            if (!here) {
-                left -= __shfl_sync(0xffffffffu, upto, 31) * a.Hk;
-                continue;
-            }
-            const int l = __ffs(here) - 1;
-            left -= (upto - sum) * a.Hk;
-            int k = 0;
+        // a worker to N blocks, more if the blocks are long, as many as there are
+        workers = min(workers, max((int)min((int64_t)workers, ((int64_t)n * a.Hk + N - 1) / N), all / max(1, N * W::SHARE * W::KEYS >> a.unit_shift)));
+        const bool mine = me < workers;
+        const int share = mine ? (unsigned)all / (unsigned)workers : 0, more = all - share * workers, begin = me * share + min(me, more), length = mine ? share + (me < more) : 0;
+        auto border = [&](int k) { return k == N ? begin + length : begin + length / N * k; };
 #pragma unroll
-            for (int m = 0; m < EACH - 1; ++m)
-                if (k == m && left >= each[m] * a.Hk) left -= each[m] * a.Hk, ++k;
-            left = __shfl_sync(0xffffffffu, left, l);
-            b = b0 + l * EACH + __shfl_sync(0xffffffffu, k, l);
-            break;
+        for (int x = 0; x < N; ++x) {
+            int left = border(x) - from * a.Hk;
+            if (!mine || left < 0 || left >= sum * a.Hk) continue;
+            for (int y = 0; y < each; ++y) {
+                const int one = work.request(tid * each + y).units * a.Hk;
+                if (left < one) {
+                    sh.b[x] = tid * each + y;
+                    sh.left[x] = left;
+                    break;
+                }
+                left -= one;
+            }
         }
-        r = b >= 0 ? work.request(b) : Request{};
+        __syncthreads();
+        b = sh.b[k];
+        units = mine && b >= 0 ? border(k + 1) - border(k) : 0;
+        if (units <= 0) return;
+        int left = sh.left[k];
+        r = work.request(b);
         kvh = r.units > 0 ? (unsigned)left / (unsigned)r.units : a.Hk;
         if (kvh >= a.Hk) {  // starts that do not ascend can come to more than 32 bits: such a call gives nothing of use, but stays inside
             units = 0;
@@ -211,17 +218,9 @@ struct Line {
         return false;
     }
 };
-// The worker that has the last part of the block that this one has begun, by whole warps.
-__device__ __forceinline__ int last_part(const ServingArgs& a, int worker, int workers) {
-    const int lane = threadIdx.x & 31;
-    for (int w0 = worker + 1;; w0 += 32) {
-        const int w = min(w0 + lane, workers - 1), head = a.parts[w].head;
-        const unsigned stops = __ballot_sync(0xffffffffu, w == workers - 1 || (head != PART_GOES_ON && head != PART_EMPTY));
-        if (stops) return min(w0 + __ffs(stops) - 1, workers - 1);
-    }
-}
-// Host: the constants of the line
+// Host: the constants of the line; the sum of the parts of blocks that fell to several of `workers`
 void set_line(ServingArgs& a, bool tree, int keys);
+int launch_combine(const ServingArgs& a, int dtype, int workers, cudaStream_t stream);
 
 struct RowsPlan {
     int rows;   // of a block
@@ -230,9 +229,9 @@ struct RowsPlan {
 };
 RowsPlan rows_plan(int dtype);
 struct TreeFewPlan {
-    int rows;     // of a slot
+    int rows;  // of a slot
     int keys, least;
-    int workers;
+    int workers, slots;  // CTAs; slots of each, in pairs
 };
 TreeFewPlan tree_few_plan(int dtype, int rows);
 int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream);

@@ -1,9 +1,9 @@
 // serving_few.cu -- attention of few new tokens against a cache of pages (decoding, small trees): bound by reading keys and values.
 //
-// Every warp is a worker of its own: it has an equal stretch of all requests' keys (serving_attention.cuh), which TMA brings into a ring
-// of its own in batches of 8 (fp32) or 16 keys, two or three ahead, over the borders of requests.  A batch lies in one page.  Lengths and tables
-// are read where the batches are asked for, 32 entries of a table at a time, so no product waits for them.  A request whose keys fall to
-// several warps leaves its parts in slots; a second kernel adds them up in their order, with as many lanes to a row as its rows leave.
+// A CTA has an equal stretch of all requests' keys (serving_attention.cuh), each of its four warps a quarter of it, which TMA brings into a
+// ring of its own in batches of 8 (fp32) or 16 keys, two or three ahead, over the borders of requests.  A batch lies in one page.  Lengths
+// and tables are read where the batches are asked for, 32 entries of a table at a time, so no product waits for them.  What a block of rows has in
+// several warps goes to slots; a CTA adds up what its own warps left, and what is left of blocks that fell to several CTAs a second kernel.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -14,10 +14,10 @@
 namespace hk {
 namespace {
 
-constexpr int WARPS = 4, ROWS_MOST = 16;
+constexpr int WARPS = 4;
 
 template <int KEYS>
-using FewWork = Work<KEYS, 128 / KEYS, 128 / KEYS, 2 * KEYS, true>;
+using FewWork = Work<KEYS, 2, 4, 3 * KEYS, true>;
 
 struct Segment {  // a run as the products need it
     int b, kvh, row0, rows, from, to, old, len, slot;
@@ -27,7 +27,8 @@ struct FewShared {
     uint8_t ring[WARPS][Rows::STAGES][4096];  // a batch's keys and values
     Segment segments[WARPS][8];               // as many as can be on their way, and more
     uint64_t full[WARPS][Rows::STAGES];
-    PartRecord record[WARPS];
+    LineSearch<WARPS> search;
+    PartRecord records[WARPS];
     Abort abort;
 };
 static_assert(sizeof(Segment) == 36, "");
@@ -85,6 +86,94 @@ __device__ __forceinline__ void join(RowsOfOne<N>& w) {
     }
 }
 
+// The parts that the CTA's warps left of blocks that go from one to the next, added up in that order, 16 lanes to a row: blocks that end
+// here are results, what one has of a block that goes on in another CTA, at either end, goes to the CTA's slots.
+template <class X, int ROWS>
+__device__ __forceinline__ void join_warps(const ServingArgs& a, const PartRecord (&records)[WARPS]) {
+    constexpr int EACH = (ROWS + 7) / 8;  // rows of a thread
+    const int sub = threadIdx.x & 15, r0 = threadIdx.x >> 4, first = blockIdx.x * WARPS;
+    float4 o[EACH];
+    float2 ml[EACH];
+    PartRecord mine{PART_EMPTY, 0, 0, 0, 0, 0}, open{PART_EMPTY, 0, 0, 0, 0, 0};  // the CTA's; of the block that is being added up
+    bool is_open = false, begun_here = false;
+    auto slot_of = [&](int slot, int r) { return (int64_t)slot * a.slot_rows + r; };
+    auto put = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int r = r0 + 8 * i;
+            if (r >= a.slot_rows) continue;
+            *reinterpret_cast<float4*>(a.part + slot_of(slot, r) * 64 + 4 * sub) = o[i];
+            if (sub == 0) a.ml[slot_of(slot, r)] = ml[i];
+        }
+    };
+    const int done = 2 * WARPS * gridDim.x;  // the CTAs' slots lie behind the warps'
+#pragma unroll 1
+    for (int w = 0; w < WARPS; ++w) {
+        const PartRecord rec = records[w];
+        if (rec.head == PART_EMPTY) continue;
+        if (rec.head != PART_NONE) {  // goes on with what is open, or with what the CTA in front has
+            const int slot = 2 * (first + w);
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int r = r0 + 8 * i;
+                if (r >= a.slot_rows) continue;
+                const float4 v = *reinterpret_cast<const float4*>(a.part + slot_of(slot, r) * 64 + 4 * sub);
+                const float2 x = a.ml[slot_of(slot, r)];
+                if (!is_open) {
+                    o[i] = v;
+                    ml[i] = x;
+                    continue;
+                }
+                const float m = fmaxf(ml[i].x, x.x), ref = m == -INFINITY ? 0.f : m, f = ex2_approx(ml[i].x - ref), g = x.y != 0.f ? ex2_approx(x.x - ref) : 0.f;
+                ml[i] = make_float2(m, ml[i].y * f + x.y * g);
+                o[i] = make_float4(o[i].x * f + v.x * g, o[i].y * f + v.y * g, o[i].z * f + v.z * g, o[i].w * f + v.w * g);
+            }
+            if (!is_open) begun_here = false;
+            is_open = true;
+            if (rec.head == PART_LAST) {
+                if (!begun_here) {
+                    put(done + 2 * blockIdx.x);
+                    mine.head = PART_LAST;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < EACH; ++i) {
+                        const int r = r0 + 8 * i;
+                        if (r >= open.tokens) continue;
+                        const float f = ml[i].y != 0.f ? 1.f / ml[i].y : 0.f;
+                        const int row = open.token0 + r, token = (int)(((uint64_t)(uint32_t)row * a.group_mul) >> a.group_shift), h = open.head0 * a.group + row - token * a.group;
+                        store4(const_cast<X*>(row_of<X>(a.O, open.b, h, token)) + 4 * sub, make_float4(o[i].x * f, o[i].y * f, o[i].z * f, o[i].w * f));
+                        if (sub == 0) a.LSE[open.b * a.lse_sB + h * a.lse_sH + token] = ml[i].y != 0.f ? (ml[i].x + log2f(ml[i].y)) * LN2 : -INFINITY;
+                    }
+                }
+                is_open = false;
+            }
+        }
+        if (mine.head == PART_EMPTY) mine.head = PART_NONE;
+        if (rec.tokens > 0) {
+            const int slot = 2 * (first + w) + 1;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int r = r0 + 8 * i;
+                if (r >= a.slot_rows) continue;
+                o[i] = *reinterpret_cast<const float4*>(a.part + slot_of(slot, r) * 64 + 4 * sub);
+                ml[i] = a.ml[slot_of(slot, r)];
+            }
+            open = rec;
+            is_open = begun_here = true;
+        }
+    }
+    if (is_open) {
+        if (begun_here) {
+            mine.b = open.b; mine.head0 = open.head0; mine.token0 = open.token0; mine.tokens = open.tokens;
+            put(done + 2 * blockIdx.x + 1);
+        } else {
+            mine.head = PART_GOES_ON;
+            put(done + 2 * blockIdx.x);
+        }
+    }
+    if (threadIdx.x == 0) a.parts[blockIdx.x] = mine;
+}
+
 template <class Rows>
 __global__ void __launch_bounds__(WARPS * 32, Rows::CTAS)
 tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
@@ -94,19 +183,18 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     constexpr int KEYS = Rows::KEYS, STAGES = Rows::STAGES, MINE = Rows::ROWS < 16 ? Rows::ROWS : 2;  // rows that a lane works on
     extern __shared__ __align__(1024) uint8_t few_smem[];
     FewShared<Rows>& sh = *reinterpret_cast<FewShared<Rows>*>(few_smem);
-    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, workers = gridDim.x * WARPS, me = warp * gridDim.x + blockIdx.x;
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, me = blockIdx.x * WARPS + warp;
     if (lane < (warp == 0 ? 4 : 0)) tma_prefetch_desc(lane == 0 ? &map_kp : lane == 1 ? &map_vp : lane == 2 ? &map_k : &map_v);
     if (lane == 0) {
         for (int s = 0; s < STAGES; ++s) mbar_init(&sh.full[warp][s], 1);
         if (warp == 0) sh.abort.id = 0;
         fence_mbar_init();
     }
-    __syncthreads();  // the record of waits that gave up
     pdl_wait();
     pdl_trigger();
     const W work{a};
     Line<W> line;
-    line.find(work, lane, me, workers);
+    line.find(work, sh.search, blockIdx.x, gridDim.x, warp);
     WaitNote wc{&sh.abort};
     PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
 
@@ -165,7 +253,6 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     int get_slot = 0, get_segment = 0, j = 0;
     uint32_t phase = 0;
     Segment get = {};
-    bool ok = true;
     Rows w;
     uint64_t bits[MINE];
     int token_of[MINE], head_of[MINE];
@@ -192,7 +279,6 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
         if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.full[warp][get_slot], phase, W_FEW, i))) {
             for (const unsigned long long t0 = globaltimer_ns(); globaltimer_ns() - t0 < 100000ull;) {}  // copies in flight land
-            ok = false;
             break;
         }
         {
@@ -206,7 +292,7 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             join(w);
             float f[2] = {1.f, 1.f};
             if (get.slot >= 0) {
-                const int64_t at = (int64_t)get.slot * ROWS_MOST;
+                const int64_t at = (int64_t)get.slot * a.slot_rows;
                 store_rows(w, lane, get.rows, 1.f, 1.f, [&](int k) { return a.part + (at + Rows::row(k, lane)) * 64; });
 #pragma unroll
                 for (int k = 0; k < MINE; ++k)
@@ -222,96 +308,15 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             }
         }
     }
-    (void)ok;
-    if (a.parts && lane == 0) a.parts[me] = record;
+    if (!a.parts) {
+        __syncthreads();
+        if (threadIdx.x == 0) report_abort(sh.abort, a.status);
+        return;
+    }
+    if (lane == 0) sh.records[warp] = record;
     __syncthreads();
     if (threadIdx.x == 0) report_abort(sh.abort, a.status);
-}
-
-// The parts of each block that fell to several warps, added up in an order of their own: 16 lanes to a part of a row, and as many parts
-// at once as there are lanes left.
-constexpr int GROUPS = 8;
-template <class X>
-__global__ void __launch_bounds__(GROUPS * 16) few_combine_kernel(const __grid_constant__ ServingArgs a, const int workers) {
-    __shared__ float4 sums[GROUPS][16];
-    __shared__ float2 mls[GROUPS];
-    pdl_wait();
-    pdl_trigger();
-    const int first = blockIdx.x;
-    const PartRecord rec = a.parts[first];
-    if (rec.tokens == 0) return;
-    const int last = last_part(a, first, workers), n = last - first + 1;
-    const int sub = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const uint32_t together = threadIdx.x & 16 ? 0xffff0000u : 0xffffu;
-    int side = 1;  // groups to a row
-    while (side * 2 * rec.tokens <= GROUPS && side < n) side *= 2;
-    const int rows_at_once = GROUPS / side;
-    for (int r0 = 0; r0 < rec.tokens; r0 += rows_at_once) {
-        const int r = r0 + g / side, p_first = g % side;
-        float M = -INFINITY, L = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < rec.tokens) {
-            for (int p0 = p_first; p0 < n; p0 += 16 * side) {
-                // a lane looks up one part
-                const int p = p0 + sub * side, worker = first + p;
-                int head = PART_EMPTY;
-                if (p < n) head = p == 0 ? PART_GOES_ON : a.parts[worker].head;
-                const bool there = head == PART_GOES_ON || head == PART_LAST;
-                const int slot = 2 * worker + (p == 0);
-                const float2 x = there ? a.ml[(int64_t)slot * ROWS_MOST + r] : make_float2(-INFINITY, 0.f);
-                float mx = x.x;
-#pragma unroll
-                for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(together, mx, off));
-                mx = fmaxf(mx, M);
-                const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(M - ref), w = there && x.y != 0.f ? ex2_approx(x.x - ref) : 0.f;
-                M = mx;
-                float sum = x.y * w;
-#pragma unroll
-                for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(together, sum, off);
-                L = L * old + sum;
-                o.x *= old; o.y *= old; o.z *= old; o.w *= old;
-                const int parts = min(16, (n - p0 + side - 1) / side);
-                for (int i = 0; i < parts; i += 4) {
-                    float4 v[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int from = __shfl_sync(together, slot, i + k, 16), is = __shfl_sync(together, (int)there, i + k, 16);
-                        v[k] = is ? *reinterpret_cast<const float4*>(a.part + ((int64_t)from * ROWS_MOST + r) * 64 + 4 * sub) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float f = __shfl_sync(together, w, i + k, 16);
-                        o.x = fmaf(v[k].x, f, o.x); o.y = fmaf(v[k].y, f, o.y); o.z = fmaf(v[k].z, f, o.z); o.w = fmaf(v[k].w, f, o.w);
-                    }
-                }
-            }
-        }
-        if (side > 1) {
-            __syncthreads();
-            sums[g][sub] = o;
-            if (sub == 0) mls[g] = make_float2(M, L);
-            __syncthreads();
-            if (p_first == 0) {
-                for (int k = 1; k < side; ++k) M = fmaxf(M, mls[g + k].x);
-                const float ref = M == -INFINITY ? 0.f : M;
-                L = 0.f;
-                o = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int k = 0; k < side; ++k) {
-                    const float2 x = mls[g + k];
-                    const float f = ex2_approx(x.x - ref);
-                    const float4 v = sums[g + k][sub];
-                    L = fmaf(x.y, f, L);
-                    o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
-                }
-            }
-        }
-        if (r < rec.tokens && p_first == 0) {
-            const float f = L != 0.f ? 1.f / L : 0.f;
-            const int row = rec.token0 + r, token = (int)(((uint64_t)(uint32_t)row * a.group_mul) >> a.group_shift), h = rec.head0 * a.group + row - token * a.group;
-            store4(const_cast<X*>(row_of<X>(a.O, rec.b, h, token)) + 4 * sub, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-            if (sub == 0) a.LSE[rec.b * a.lse_sB + h * a.lse_sH + token] = L != 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
-        }
-    }
+    join_warps<X, Rows::ROWS>(a, sh.records);
 }
 
 typedef void (*Kernel)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, ServingArgs);
@@ -339,7 +344,7 @@ void divide_by(int d, uint32_t& mul, int& shift) {
 
 TreeFewPlan tree_few_plan(int dtype, int rows) {
     const Entry e = pick(dtype, rows);
-    return {ROWS_MOST, e.keys, 128 / e.keys, sm_count() * e.per_sm * WARPS};
+    return {std::min(rows, e.rows), e.keys, 2, sm_count() * e.per_sm, WARPS + 1};
 }
 
 int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
@@ -362,6 +367,7 @@ int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
     }
     a.block_tokens = std::min(a.rows, e.rows);
     a.chunks = 1;
+    a.slot_rows = a.block_tokens;
     a.new_tiles = cdiv(a.T, e.keys);
     set_line(a, true, e.keys);
     divide_by(a.group, a.group_mul, a.group_shift);
@@ -377,12 +383,9 @@ int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
     if (cudaLaunchKernelEx(&lc.cfg, e.kernel, k, v, kp, vp, a) != cudaSuccess) return check_launch();
     count_launch();
     if (!a.parts) return HK_OK;
-    typedef void (*Combine)(ServingArgs, int);
-    static const Combine combine[] = {few_combine_kernel<float>, few_combine_kernel<__nv_bfloat16>, few_combine_kernel<__half>};
-    LaunchConfig sum(ctas * WARPS, GROUPS * 16, 0, stream, 1, true);
-    if (cudaLaunchKernelEx(&sum.cfg, combine[dtype], a, ctas * WARPS) != cudaSuccess) return check_launch();
-    count_launch();
-    return HK_OK;
+    a.part += (size_t)2 * WARPS * ctas * a.slot_rows * 64;  // the CTAs' slots
+    a.ml += (size_t)2 * WARPS * ctas * a.slot_rows;
+    return launch_combine(a, dtype, ctas, stream);
 }
 
 }  // namespace hk

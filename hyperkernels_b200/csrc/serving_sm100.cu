@@ -63,6 +63,7 @@ struct __align__(16) RowsShared {
     uint64_t item_full[C::ITEMS], item_empty[C::ITEMS];
     uint64_t kv_ready[C::SLOTS];  // tended: low parts are there, what is behind a last key is cleared
     Item items[C::ITEMS];
+    LineSearch<1> search;
     int keep[C::SLOTS];  // rows of the tile that are values, LAST: none follows
     uint32_t tmem_base;
     Abort abort;
@@ -183,9 +184,8 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
     pdl_wait();
     pdl_trigger();
-    Line<RowsWork<X, TREE>> line = {};
-    if (warp == 0) line.find(RowsWork<X, TREE>{a}, lane, blockIdx.x, gridDim.x);
-    __syncthreads();
+    Line<RowsWork<X, TREE>> line;
+    line.find(RowsWork<X, TREE>{a}, sh.search, blockIdx.x, gridDim.x, 0);
     tc_fence_after_sync();
     constexpr uint32_t tmem = 0;  // all columns are this CTA's
     if (sh.tmem_base != tmem) sh.abort.id = 598;
@@ -876,64 +876,6 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
 }
 
-// ---------------------------------------------------------------------------
-// The parts of each block that fell to several CTAs, added up in their order: 16 lanes a row, four elements a lane.  The block begins in the
-// second slot of one CTA and goes on in the first ones of those behind it.
-// ---------------------------------------------------------------------------
-template <class X, int BLOCK>
-__global__ void __launch_bounds__(256) serving_combine_kernel(const __grid_constant__ ServingArgs a, const int ctas) {
-    pdl_wait();
-    pdl_trigger();
-    const PartRecord rec = a.parts[blockIdx.x];
-    const int sub = threadIdx.x & 15, r0 = blockIdx.y * 64;
-    if (rec.tokens == 0) return;
-    const int last = last_part(a, blockIdx.x, ctas);
-    const int n = last - (int)blockIdx.x + 1;
-    const uint32_t together = threadIdx.x & 16 ? 0xffff0000u : 0xffffu;
-    for (int r = r0 + (int)threadIdx.x / 16; r < r0 + 64; r += 16) {
-        const int t = r / TILE, box_heads = min(a.group, TILE), in_stream = r - t * TILE, token_in = in_stream / box_heads, head = in_stream - token_in * box_heads;
-        const int token = t * a.stream_tokens + token_in;
-        if (token_in >= a.stream_tokens || token >= rec.tokens || head >= rec.heads) continue;
-        float M = -INFINITY, L = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p0 = 0; p0 < n; p0 += 16) {
-            // a lane looks up one part
-            const int cta = blockIdx.x + p0 + sub;
-            const bool there = p0 + sub < n && (p0 + sub == 0 || a.parts[cta].head == PART_GOES_ON || a.parts[cta].head == PART_LAST);
-            const int slot = 2 * cta + (p0 + sub == 0);
-            const float2 x = there ? a.ml[(int64_t)slot * BLOCK + r] : make_float2(-INFINITY, 0.f);
-            float mx = x.x;
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(together, mx, off));
-            mx = fmaxf(mx, M);
-            const float ref = mx == -INFINITY ? 0.f : mx, old = ex2_approx(M - ref), w = there && x.y != 0.f ? ex2_approx(x.x - ref) : 0.f;
-            M = mx;
-            float sum = x.y * w;
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(together, sum, off);
-            L = L * old + sum;
-            o.x *= old; o.y *= old; o.z *= old; o.w *= old;
-            for (int i = 0; i < min(16, n - p0); i += 4) {
-                float4 v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int from = __shfl_sync(together, slot, i + k, 16), is = __shfl_sync(together, (int)there, i + k, 16);
-                    v[k] = is ? *reinterpret_cast<const float4*>(a.part + ((int64_t)from * BLOCK + r) * 64 + 4 * sub) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float f = __shfl_sync(together, w, i + k, 16);
-                    o.x = fmaf(v[k].x, f, o.x); o.y = fmaf(v[k].y, f, o.y); o.z = fmaf(v[k].z, f, o.z); o.w = fmaf(v[k].w, f, o.w);
-                }
-            }
-        }
-        const float f = L != 0.f ? 1.f / L : 0.f;
-        const int h = rec.head0 + head, row = rec.token0 + token;
-        store4(const_cast<X*>(row_of<X>(a.O, rec.b, h, row)) + 4 * sub, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-        if (sub == 0) a.LSE[rec.b * a.lse_sB + h * a.lse_sH + row] = L != 0.f ? (M + log2f(L)) * LN2 : -INFINITY;
-    }
-}
-
 // Boxes of `rows` rows of a page, 128 bytes of each
 int page_map(CUtensorMap* map, const hk_view& v, int dtype, int n_pages, int H, int page, int rows, bool mn_major) {
     EncodeTiledFn enc = get_encode_tiled();
@@ -977,6 +919,7 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     a.block_tokens = C::STREAMS * a.stream_tokens;
     a.chunks = cdiv(a.group, TILE);
     a.new_tiles = 1;
+    a.slot_rows = C::BLOCK;
     set_line(a, TREE, C::KEYS);
     CUtensorMap k, v, kp, vp;
     const int B = TREE ? a.B : 1;
@@ -998,12 +941,7 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     LaunchConfig lc(ctas, C::THREADS, RowsSpace<X>::SMEM, stream, 1, true);
     if (cudaLaunchKernelEx(&lc.cfg, serving_rows_kernel<X, TREE>, q, k, v, kp, vp, a) != cudaSuccess) return check_launch();
     count_launch();
-    if (!a.parts) return HK_OK;
-    LaunchConfig sum(ctas, 256, 0, stream, 1, true);
-    sum.cfg.gridDim.y = C::BLOCK / 64;
-    if (cudaLaunchKernelEx(&sum.cfg, serving_combine_kernel<X, C::BLOCK>, a, ctas) != cudaSuccess) return check_launch();
-    count_launch();
-    return HK_OK;
+    return a.parts ? launch_combine(a, dtype, ctas, stream) : HK_OK;
 }
 template <bool TREE>
 int launch(const ServingArgs& a, int dtype, cudaStream_t stream) {
