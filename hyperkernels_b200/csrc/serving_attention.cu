@@ -151,7 +151,7 @@ Parts parts_of(const hk_prompt_params* p) {
     const RowsPlan plan = rows_plan(p->dtype);
     return {sm_count(), 1, plan.rows, (p->N + plan.keys - 1) / plan.keys >= 2 * plan.least};
 }
-bool few_rows(const hk_tree_params* p) { return p->T * (p->nh / p->nh_kv) <= 16; }
+bool few_rows(const hk_tree_params* p) { return p->T * (p->nh / p->nh_kv) <= (p->dtype == HK_F32 ? 8 : 16); }
 Parts parts_of(const hk_tree_params* p) {
     const int64_t keys = (int64_t)p->pool.width * p->pool.page;
     if (few_rows(p)) {
@@ -180,9 +180,7 @@ int set_scale(ServingArgs& a, int dtype, float scale) {
 }  // namespace
 
 void set_line(ServingArgs& a, bool tree, int keys) {
-    a.block_shift = 31;
-    while ((1LL << (a.block_shift - 31)) < a.block_tokens) ++a.block_shift;
-    a.block_mul = (uint32_t)(((1ULL << a.block_shift) + a.block_tokens - 1) / a.block_tokens);
+    divide_by(a.block_tokens, a.block_mul, a.block_shift);
     // what all requests can come to, in keys: blocks, and what each counts at most
     const double blocks = (tree ? (double)a.B * cdiv(a.rows ? a.rows : a.T, a.block_tokens) : (double)a.N / a.block_tokens + a.B) * a.Hk * a.chunks;
     double all = blocks * ((tree ? (double)a.pool.width * a.pool.page + a.new_tiles * keys : a.N + a.block_tokens) + 4.0 * keys);

@@ -35,7 +35,7 @@ struct ServingArgs {
     int block_tokens, chunks, new_tiles;
     uint32_t block_mul;
     int block_shift, unit_shift;
-    uint32_t group_mul, page_mul;  // few rows: x / group, x / page likewise
+    uint32_t group_mul, page_mul;  // x / group (few rows) and x / page likewise
     int group_shift, page_shift;
     int stream_tokens, q_bytes;  // many rows: tokens of a stream, bytes of its queries
     int box;            // rows of a page that are loaded at once
@@ -218,6 +218,11 @@ struct Line {
         return false;
     }
 };
+// Host: x / d is x * mul >> shift for x below 2^31.
+inline void divide_by(int d, uint32_t& mul, int& shift) {
+    for (shift = 31; (1LL << (shift - 31)) < d;) ++shift;
+    mul = (uint32_t)(((1ULL << shift) + d - 1) / d);
+}
 // Host: the constants of the line; the sum of the parts of blocks that fell to several of `workers`
 void set_line(ServingArgs& a, bool tree, int keys);
 int launch_combine(const ServingArgs& a, int dtype, int workers, cudaStream_t stream);

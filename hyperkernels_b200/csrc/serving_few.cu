@@ -35,15 +35,15 @@ static_assert(sizeof(Segment) == 36, "");
 constexpr int W_FEW = 601;
 
 // The weighted sum of a row's values from registers to memory, scaled: fp32 in slots, or the result.
-template <class T, class P>
-__device__ __forceinline__ void store_rows(const RowsOf16<T>& w, int lane, int rows, float f0, float f1, P&& place) {
+template <class T, int M, class P>
+__device__ __forceinline__ void store_rows(const RowsOf16<T>& w, int lane, int rows, const float (&f_of)[M], P&& place) {
     typedef typename RowsOf16<T>::Math Math;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int r = RowsOf16<T>::row(i, lane);
         if (r >= rows) continue;
         auto* const to = place(i);
-        const float f = i ? f1 : f0;
+        const float f = f_of[i];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int j = (k >> 1) * 4, e = 2 * i + (k & 1);
@@ -52,12 +52,12 @@ __device__ __forceinline__ void store_rows(const RowsOf16<T>& w, int lane, int r
     }
 }
 template <int N, class P>
-__device__ __forceinline__ void store_rows(const RowsOfOne<N>& w, int lane, int rows, float f0, float f1, P&& place) {
+__device__ __forceinline__ void store_rows(const RowsOfOne<N>& w, int lane, int rows, const float (&f_of)[N], P&& place) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         if (i >= rows || lane >= 16) continue;
         auto* const to = place(i);
-        const float f = i ? f1 : f0;
+        const float f = f_of[i];
         store4(to + 4 * lane, make_float4(w.o[i].x * f, w.o[i].y * f, w.o[i].z * f, w.o[i].w * f));
     }
 }
@@ -290,17 +290,17 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         if (++get_slot == STAGES) get_slot = 0, phase ^= 1u;
         if (++j == get.to) {
             join(w);
-            float f[2] = {1.f, 1.f};
+            float f[MINE];
+#pragma unroll
+            for (int k = 0; k < MINE; ++k) f[k] = get.slot >= 0 ? 1.f : w.l[k] != 0.f ? 1.f / w.l[k] : 0.f;
             if (get.slot >= 0) {
                 const int64_t at = (int64_t)get.slot * a.slot_rows;
-                store_rows(w, lane, get.rows, 1.f, 1.f, [&](int k) { return a.part + (at + Rows::row(k, lane)) * 64; });
+                store_rows(w, lane, get.rows, f, [&](int k) { return a.part + (at + Rows::row(k, lane)) * 64; });
 #pragma unroll
                 for (int k = 0; k < MINE; ++k)
                     if (Rows::row(k, lane) < get.rows && (Rows::ROWS < 16 ? lane == 0 : (lane & 3) == 0)) a.ml[at + Rows::row(k, lane)] = make_float2(w.m[k], w.l[k]);
             } else {
-#pragma unroll
-                for (int k = 0; k < MINE; ++k) f[k] = w.l[k] != 0.f ? 1.f / w.l[k] : 0.f;
-                store_rows(w, lane, get.rows, f[0], f[1], [&](int k) { return const_cast<X*>(row_of<X>(a.O, get.b, head_of[k], token_of[k])); });
+                store_rows(w, lane, get.rows, f, [&](int k) { return const_cast<X*>(row_of<X>(a.O, get.b, head_of[k], token_of[k])); });
 #pragma unroll
                 for (int k = 0; k < MINE; ++k)
                     if (Rows::row(k, lane) < get.rows && (Rows::ROWS < 16 ? lane == 0 : (lane & 3) == 0))
@@ -332,12 +332,7 @@ Entry entry() {
 Entry pick(int dtype, int rows) {
     if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>>();
     if (dtype == HK_F16) return entry<RowsOf16<__half>>();
-    return rows == 1 ? entry<RowsOfOne<1>>() : rows == 2 ? entry<RowsOfOne<2>>() : entry<RowsOf16<float>>();
-}
-void divide_by(int d, uint32_t& mul, int& shift) {
-    shift = 31;
-    while ((1LL << (shift - 31)) < d) ++shift;
-    mul = (uint32_t)(((1ULL << shift) + d - 1) / d);
+    return rows == 1 ? entry<RowsOfOne<1>>() : rows == 2 ? entry<RowsOfOne<2>>() : rows <= 4 ? entry<RowsOfOne<4>>() : entry<RowsOfOne<8>>();
 }
 
 }  // namespace

@@ -8,7 +8,7 @@
 // several CTAs leaves its parts (maximum, sum, weighted values) in slots of the workspace, a pair to a CTA, and a second kernel adds
 // them up in their order.
 //   Warp 0 cuts the stretch into items (a block of rows, a run of its tiles), makes them known to the other warps in a ring and loads
-// their tiles by TMA, warp 1 issues the products S = Q K^T and, two products behind, O += P V (tcgen05, operands in shared and tensor memory),
+// their queries and tiles of keys by TMA, another the tiles of values, warp 1 issues the products S = Q K^T and, two products behind, O += P V (tcgen05, operands in shared and tensor memory),
 // four warps to a stream take S through the softmax, a row to a thread.  All of them go from one item to the next without a barrier: the
 // queries and the first tiles of the next are there, and its first scores under way, when the last weights of this one are worked out.
 // Scores are three deep in tensor memory; P takes the place of its S.
@@ -31,7 +31,7 @@ struct Rows {
     static constexpr int STREAMS = LOW ? 1 : 2;  // blocks of 128 rows
     static constexpr int BLOCK = STREAMS * TILE;
     static constexpr int KEYS = LOW ? 64 : 128;  // of a tile
-    static constexpr int SLOTS = LOW ? 6 : 8;    // of the ring of tiles; even: each of two pairs of warps has every other one
+    static constexpr int SLOTS = LOW ? 3 : 4;    // of the rings of tiles of keys and of values
     static constexpr int THREADS = 384;
     static constexpr int SOFTMAX_WARPS = LOW ? 4 : 8;
     static constexpr int LEAST = LOW ? 4 : 2;    // tiles of a part of a block
@@ -58,13 +58,14 @@ struct __align__(16) Item {
 template <class X>
 struct __align__(16) RowsShared {
     typedef Rows<X> C;
-    uint64_t q_full[C::Q_BUFFERS], q_empty[C::Q_BUFFERS], q_ready, kv_full[C::SLOTS], kv_empty[C::SLOTS], p_full[3];
+    uint64_t q_full[C::Q_BUFFERS], q_empty[C::Q_BUFFERS], q_ready, p_full[3];
     uint64_t s_full[C::STREAMS][3], o_full[C::STREAMS][3];  // of a stream's own products: it does not see the other's
     uint64_t item_full[C::ITEMS], item_empty[C::ITEMS];
-    uint64_t kv_ready[C::SLOTS];  // tended: low parts are there, what is behind a last key is cleared
+    uint64_t full[2][C::SLOTS], empty[2][C::SLOTS];  // keys, values
+    uint64_t ready[2][C::SLOTS];                     // tended: low parts are there, what is behind a last key is cleared
     Item items[C::ITEMS];
     LineSearch<1> search;
-    int keep[C::SLOTS];  // rows of the tile that are values, LAST: none follows
+    int keep[2][C::SLOTS];  // rows of the tile that are values, LAST: none follows
     uint32_t tmem_base;
     Abort abort;
 };
@@ -73,7 +74,7 @@ constexpr int LAST = -1;
 template <class X>
 struct RowsSpace {
     typedef Rows<X> C;
-    static constexpr int OFF_Q = C::SLOTS * C::KV_BYTES, OFF_O = OFF_Q + C::STREAMS * C::Q_BUFFERS * C::Q_BYTES, OFF_SH = OFF_O + (C::LOW ? 0 : C::SOFTMAX_WARPS * 4096), SMEM = OFF_SH + (int)sizeof(RowsShared<X>);
+    static constexpr int OFF_Q = 2 * C::SLOTS * C::KV_BYTES, OFF_O = OFF_Q + C::STREAMS * C::Q_BUFFERS * C::Q_BYTES, OFF_SH = OFF_O + (C::LOW ? 0 : C::SOFTMAX_WARPS * 4096), SMEM = OFF_SH + (int)sizeof(RowsShared<X>);
     static_assert(SMEM <= 232448, "exceeds the 227 KiB a CTA may opt in to");
 };
 // Tensor memory.  16-bit types: three buffers of 128 columns for scores and weights, O of two streams.  fp32: three buffers of
@@ -155,9 +156,11 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         mbar_init(&sh.q_ready, 4);
         for (int s = 0; s < SLOTS; ++s) {
-            mbar_init(&sh.kv_full[s], 1);
-            mbar_init(&sh.kv_empty[s], LOW ? 1 : 2);
-            mbar_init(&sh.kv_ready[s], LOW ? 2 : 1);
+            for (int v = 0; v < 2; ++v) {
+                mbar_init(&sh.full[v][s], 1);
+                mbar_init(&sh.empty[v][s], LOW || v == 0 ? 1 : 2);
+                mbar_init(&sh.ready[v][s], LOW ? 2 : 1);
+            }
         }
         for (int b = 0; b < 3; ++b) {
             mbar_init(&sh.p_full[b], 4);
@@ -168,7 +171,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         for (int i = 0; i < ITEMS; ++i) {
             mbar_init(&sh.item_full[i], 1);
-            mbar_init(&sh.item_empty[i], 1 + C::SOFTMAX_WARPS);
+            mbar_init(&sh.item_empty[i], 2 + C::SOFTMAX_WARPS);
         }
         sh.abort.id = 0;
         fence_mbar_init();
@@ -192,305 +195,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     WaitNote wc{&sh.abort};
 
     // three groups of warps, 168 registers a thread at the launch
-    if (warp < 4) {
-        if constexpr (LOW) asm volatile("setmaxnreg.dec.sync.aligned.u32 120;\n");
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
-        if (warp == 0) {
-            // ------------------------------ items, tiles of keys and values ------------------------------
-            const RowsWork<X, TREE> work{a};
-            bool ok = true;
-            PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
-            // The next item into the ring; one without tokens at the end of the stretch
-            auto publish = [&](Item& it) {
-                Run run;
-                it.tokens = 0;
-                if (!line.next(work, run)) return;
-                const int count = run.to - run.from;
-                it.b = run.b; it.kvh = run.kvh; it.chunk = run.chunk;
-                it.token0 = run.i * a.block_tokens;
-                it.tokens = min(a.block_tokens, run.r.tokens - it.token0);
-                it.begin = run.r.begin; it.len = run.r.len; it.key0 = run.from * KEYS;
-                it.new_tile = TREE ? run.n - 1 - run.from : -1;
-                it.n0 = count;
-                it.n1 = 0;
-                if (!LOW && it.tokens > a.stream_tokens) {
-                    it.n1 = count;
-                    if (!TREE && a.causal) it.n0 = max(0, min((it.token0 + a.stream_tokens + KEYS - 1) / KEYS - run.from, count));
-                }
-                it.slot = run.slot(blockIdx.x);
-                if (run.from > 0) {
-                    record.head = run.to < run.n ? PART_GOES_ON : PART_LAST;
-                } else {
-                    if (record.head == PART_EMPTY) record.head = PART_NONE;
-                    if (run.to < run.n) {
-                        record.b = TREE ? it.b : 0; record.head0 = it.kvh * a.group + it.chunk * TILE; record.heads = min(TILE, a.group - it.chunk * TILE);
-                        record.token0 = it.begin + it.token0; record.tokens = it.tokens;
-                    }
-                }
-            };
-            Turn put{0, 0u};
-            int made = 0, s_at = 0, o_at = 0;  // items; the places of those of S and of O
-            bool on = true;
-            Cursor s, o;
-            auto emit = [&]() -> bool {  // false: gave up
-                Item it;
-                publish(it);
-                on = it.tokens > 0;
-                if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.item_empty[put.at], put.phase ^ 1u, W_ITEM_EMPTY, made))) return false;
-                if (lane == 0) {
-                    sh.items[put.at] = it;
-                    mbar_arrive(&sh.item_full[put.at]);
-                }
-                if (it.tokens > 0) {  // its queries, in the place of those of the item before, or before that
-                    const int buf = made & (C::Q_BUFFERS - 1), use = made / C::Q_BUFFERS;
-                    if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(wc, &sh.q_empty[buf], (use - 1) & 1, W_Q_EMPTY, made))) return false;
-                    if (lane == 0) {
-                        const int streams = it.n1 > 0 ? 2 : 1, head = it.kvh * a.group + it.chunk * TILE;
-                        mbar_arrive_expect_tx(&sh.q_full[buf], streams * a.q_bytes);
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {  // streams, or halves of the rows
-                            if (LOW || x < streams)
-                                tma_load_queries(sQ + (buf * 2 + x) * (TILE * 128), &map_q, &sh.q_full[buf], head, it.begin + it.token0 + (LOW ? 0 : x * a.stream_tokens), LOW ? x : 0, TREE ? it.b : 0);
-                        }
-                    }
-                }
-                if (on) s.start(it.n0, it.n1);
-                s_at = put.at;
-                put.next(ITEMS);
-                ++made;
-                return true;
-            };
-            Turn ring{0, 0u};
-            int filled = 0;
-            auto load = [&](const Item& it, int j, bool v) -> bool {
-                if (filled >= SLOTS && !__all_sync(0xffffffffu, mbar_wait(wc, &sh.kv_empty[ring.at], ring.phase ^ 1u, W_EMPTY, filled))) return false;
-                const int key = it.key0 + j * KEYS, s = ring.at;
-                const bool fresh = TREE && j == it.new_tile;
-                uint8_t* to = sKV + s * C::KV_BYTES;
-                if (lane == 0) {
-                    sh.keep[s] = v && !fresh ? min(KEYS, it.len - key) : KEYS;
-                    mbar_arrive_expect_tx(&sh.kv_full[s], C::KV_RAW);
-                    if (!TREE) tma_load_tile(to, v ? &map_v : &map_k, &sh.kv_full[s], it.begin + key, it.kvh, 0);
-                    else if (fresh) tma_load_tile(to, v ? &map_v : &map_k, &sh.kv_full[s], 0, it.kvh, it.b);
-                }
-                if constexpr (TREE) {
-                    if (!fresh) {
-                        __syncwarp();
-                        // a box of a page to a lane; pages that are none, and those behind the last, read as zeros
-                        const int boxes = KEYS / a.box;
-                        if (lane < boxes) {
-                            const int k = key + lane * a.box, at_page = k / a.pool.page;
-                            const int page = k < it.len ? a.pool.pages[it.b * a.pool.pages_stride + at_page] : -1;
-                            const CUtensorMap* map = v ? &map_vp : &map_kp;
-#pragma unroll
-                            for (int half = 0; half < (LOW ? 2 : 1); ++half)
-                                tma_load_box(to + half * C::KV_BOX + lane * a.box * 128, map, &sh.kv_full[s], k - at_page * a.pool.page, half, it.kvh, page);
-                        }
-                    }
-                }
-                ring.next(SLOTS);
-                ++filled;
-                return true;
-            };
-            // In step with the products: S, then O so many products behind it.  (One place of each call: this code has to stay small, see the top.)
-            int ahead = 0, between = -1;  // products and items that S is in front of O
-            bool s_new = true, o_new = true;
-            while (true) {
-                if (s_new) {
-                    if (!(ok = emit())) break;
-                    s_new = false;
-                    ++between;
-                }
-                if (!on && ahead == 0) break;
-                const bool go = on && may_go<LOW>(between);
-                if (o_new) {
-                    __syncwarp();
-                    o.start(sh.items[o_at].n0, sh.items[o_at].n1);
-                    o_new = false;
-                }
-#pragma unroll 1
-                for (int v = 0; v < 2 && ok; ++v) {
-                    if (v ? ahead <= BEHIND && go : !go) continue;
-                    if (v ? o.first() : s.first()) ok = load(sh.items[v ? o_at : s_at], v ? o.j : s.j, v);
-                    if (v) {
-                        --ahead;
-                        if (!o.next()) {
-                            o_new = true;
-                            o_at = o_at == ITEMS - 1 ? 0 : o_at + 1;
-                            --between;
-                        }
-                    } else {
-                        ++ahead;
-                        s_new = !s.next();
-                    }
-                }
-                if (!ok) break;
-            }
-            for (int k = 0; ok && k < (LOW ? 2 : 1); ++k) {  // to those who tend the tiles: no more
-                if (filled >= SLOTS && !(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.kv_empty[ring.at], ring.phase ^ 1u, W_EMPTY, filled)))) break;
-                if (lane == 0) {
-                    sh.keep[ring.at] = LAST;
-                    mbar_arrive(&sh.kv_full[ring.at]);
-                }
-                ring.next(SLOTS);
-                ++filled;
-            }
-            if (a.parts && lane == 0) a.parts[blockIdx.x] = record;
-            // a CTA that gave up may have copies in flight: they get time to land
-            if (!ok)
-                for (const unsigned long long t0 = globaltimer_ns(); globaltimer_ns() - t0 < 100000ull;) {}
-        } else if (warp == 1) {
-            // ------------------------------ products ------------------------------
-            const uint32_t leader = elect_one_sync();
-            struct Barrier {
-                uint64_t* bar;
-                uint32_t parity;
-            };
-            // each barrier is looked at while the products before it are still being issued, and waited for if that look came too early
-            auto seen = [&](const Barrier& x) { return mbar_test_wait(x.bar, x.parity); };
-            auto wait = [&](bool was_seen, const Barrier& x, int id, int aux) {
-                return __all_sync(0xffffffffu, was_seen) || (bool)__all_sync(0xffffffffu, mbar_wait(wc, x.bar, x.parity, id, aux));
-            };
-            const uint32_t kv_addr = smem_u32(sKV);
-            const Desc q_desc = make_smem_desc(smem_u32(sQ), 16, 1024, DESC_SW128), k_desc = make_smem_desc(kv_addr, 16, 1024, DESC_SW128),
-                       v_desc = LOW ? mnmajor_desc(kv_addr, 0, C::KV_BOX) : make_smem_desc(kv_addr, 16, 1024, DESC_SW128);
-            const uint32_t negate = a.flip ? IDESC_NEGATE_A : 0u;
-            Turn tile{0, 0u}, p{0, 0u}, s_item{0, 0u}, o_item{0, 0u};
-            Cursor s, o;
-            int ahead = 0, k_slot = 0, v_slot = 0, s_buf = 0, items = 0, low_buf = 0;
-            int s_own[2] = {0, 0}, o_own[2] = {0, 0};  // the next barriers of a stream's own
-            auto after = [&](int (&own)[2], int t) {
-                const int x = t ? own[1] : own[0], y = x == 2 ? 0 : x + 1;
-                if (t) own[1] = y;
-                else own[0] = y;
-                return t * 3 + x;
-            };
-            bool ok = true, s_on = false, new_queries = false;
-            auto look_at = [&](const Turn& x, bool v) -> Barrier { return LOW || v ? Barrier{&sh.kv_ready[x.at], x.phase} : Barrier{&sh.kv_full[x.at], x.phase}; };
-            auto next_item = [&](Turn& turn, Cursor& c) -> bool {  // false: the end, or gave up
-                if (!(ok = wait(false, {&sh.item_full[turn.at], turn.phase}, W_ITEM, items))) return false;
-                const Item& it = sh.items[turn.at];
-                if ((int)uniform(it.tokens) == 0) return false;
-                c.start((int)uniform(it.n0), (int)uniform(it.n1));
-                return true;
-            };
-            bool s_new = true, o_new = true, seen_k = false, seen_v = false, seen_p = false;
-            int between = -1;
-#pragma unroll 1
-            while (ok) {
-                const bool fresh = s_new;
-                if (s_new) {
-                    s_on = next_item(s_item, s);
-                    if (!ok) break;
-                    s_new = false;
-                    ++between;
-                }
-                if (!s_on && ahead == 0) break;
-                if (o_new) {
-                    if (!next_item(o_item, o)) break;
-                    o_new = false;
-                }
-                const bool go = s_on && may_go<LOW>(between);
-                new_queries |= fresh;
-                if (go) {
-                    if (new_queries) {
-                        if (!(ok = wait(false, LOW ? Barrier{&sh.q_ready, (uint32_t)items & 1u} : Barrier{&sh.q_full[items & 1 & (C::Q_BUFFERS - 1)], (uint32_t)(items >> 1) & 1u}, W_Q, items))) break;
-                        new_queries = false;
-                    }
-                    if (s.first()) {
-                        if (!(ok = wait(seen_k, look_at(tile, false), W_READY, items))) break;
-                        k_slot = tile.at;
-                        tile.next(SLOTS);
-                    }
-                    seen_k = false;
-                    tc_fence_after_sync();
-                    const Desc kd = k_desc + k_slot * C::KV_BYTES;
-                    const bool both = ahead >= BEHIND;  // O follows
-                    auto look = [&] {
-                        seen_v = o.first() && seen(look_at(tile, true));
-                        seen_p = seen({&sh.p_full[p.at], p.phase});
-                    };
-                    if constexpr (LOW) {
-                        constexpr uint32_t IDESC = make_idesc_tf32(TILE, KEYS, false, false);
-                        const uint32_t d = tmem + s_buf * 64;
-                        auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
-                            umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x, kd + y, IDESC, acc);
-                            umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x + 32, kd + (y + C::KV_BOX), IDESC, 1u);
-                        };
-                        eight(64, 0, 0u);
-                        eight(0, C::KV_RAW, 1u);
-                        if (both) look();
-                        eight(0, 0, 1u);
-                    } else {
-                        const uint32_t IDESC = make_idesc_16(TILE, KEYS, BF16, false) | negate;
-                        const uint32_t d = tmem + s_buf * 128;
-                        const Desc qd = q_desc + ((items & 1) * C::STREAMS + s.t) * C::Q_BYTES;
-                        umma_ss_16(leader, d, qd.d, kd.d, IDESC, 0u);
-                        umma_ss_16(leader, d, qd.d + 2, kd.d + 2, IDESC, 1u);
-                        if (both) look();
-                        umma_ss_16(leader, d, qd.d + 4, kd.d + 4, IDESC, 1u);
-                        umma_ss_16(leader, d, qd.d + 6, kd.d + 6, IDESC, 1u);
-                    }
-                    umma_commit_lead(leader, &sh.s_full[0][0] + after(s_own, s.t));
-                    if (s.last()) umma_commit_lead(leader, &sh.kv_empty[k_slot]);
-                    s_buf = s_buf == 2 ? 0 : s_buf + 1;
-                    ++ahead;
-                    if (!s.next()) {
-                        if (!LOW) umma_commit_lead(leader, &sh.q_empty[items & (C::Q_BUFFERS - 1)]);
-                        ++items;
-                        s_item.next(ITEMS);
-                        s_new = true;
-                    }
-                }
-                if (ahead > BEHIND || !go) {  // O
-                    if (o.first()) {
-                        if (!(ok = wait(seen_v, look_at(tile, true), W_READY, items))) break;
-                        v_slot = tile.at;
-                        tile.next(SLOTS);
-                    }
-                    if (!(ok = wait(seen_p, {&sh.p_full[p.at], p.phase}, W_P, items))) break;
-                    tc_fence_after_sync();
-                    seen_v = seen_p = false;
-                    const Desc vd = v_desc + v_slot * C::KV_BYTES;
-                    const uint32_t acc = o.j > 0;
-                    const bool look_k = s_on && !s_new && s.first() && o.last();
-                    if constexpr (LOW) {
-                        constexpr uint32_t IDESC = make_idesc_tf32(TILE, HEAD_DIM, false, true);
-                        const uint32_t high = tmem + p.at * 64, low = tmem + LOW_COL_LOW + low_buf * 64, d = tmem + LOW_COL_O;
-                        auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
-                            umma_ts4<MNMAJOR_STEP>(leader, d, x, vd + y, IDESC, acc);
-                            umma_ts4<MNMAJOR_STEP>(leader, d, x + 32, vd + (y + 4096), IDESC, 1u);
-                        };
-                        eight(low, 0, 0u);
-                        eight(high, C::KV_RAW, 1u);
-                        seen_k = look_k && seen(look_at(tile, false));
-                        eight(high, 0, 1u);
-                        low_buf ^= 1;
-                    } else {
-                        constexpr uint32_t IDESC = make_idesc_16(TILE, HEAD_DIM, BF16, true);
-                        const uint32_t w = tmem + p.at * 128, d = tmem + COL_O + o.t * 64;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            if (k == 4) seen_k = look_k && seen(look_at(tile, false));
-                            umma_ts_16(leader, d, w + 8 * k, vd.d + (2048 >> 4) * k, IDESC, k > 0 ? 1u : acc);
-                        }
-                    }
-                    umma_commit_lead(leader, &sh.o_full[0][0] + after(o_own, o.t));
-                    if (o.last()) umma_commit_lead(leader, &sh.kv_empty[v_slot]);
-                    p.next(3);
-                    --ahead;
-                    if (!o.next()) {
-                        if (lane == 0) mbar_arrive(&sh.item_empty[o_item.at]);
-                        o_item.next(ITEMS);
-                        --between;
-                        o_new = true;
-                    }
-                }
-            }
-        }
-    } else if (LOW && warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;\n");
-    } else {
+    if (warp >= 4 && (!LOW || warp < 8)) {
         // ------------------------------ softmax ------------------------------
         if constexpr (LOW) asm volatile("setmaxnreg.inc.sync.aligned.u32 240;\n");
         else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
@@ -831,40 +536,308 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             mbar_arrive_warp(&sh.item_empty[get.at], lane);
             get.next(ITEMS);
         }
-    }
-    // What the tiles need beside the loads, entry by entry of the ring.  Rows behind the request's last key may hold anything, and 0 times
-    // a NaN is one: they are cleared among the values.  fp32: the tiles' low parts, by two pairs of warps, each of which has every other
-    // slot of the ring for its own: a barrier is waited for by the parity of its phase, and is to be looked at in every one.
-    if (LOW ? warp == 2 || warp == 3 || warp == 8 || warp == 9 : warp == 2) {
-        const int me = LOW ? threadIdx.x & 63 : lane, first = LOW && warp >= 8;
-        constexpr int EVERY = LOW ? 2 : 1;
-        Turn at{first, 0u};
-        while (true) {
-            if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.kv_full[at.at], at.phase, W_KV, at.at))) break;
-            const int keep = sh.keep[at.at];
-            if (keep == LAST) break;
-            uint4* raw = reinterpret_cast<uint4*>(sKV + at.at * C::KV_BYTES);
-            if constexpr (LOW) {
-                constexpr int EACH = C::KV_RAW / 16 / 64;
-                uint4 *from = raw + me, *low = from + C::KV_RAW / 16, x[EACH];
-#pragma unroll
-                for (int k = 0; k < EACH; ++k) x[k] = from[k * 64];
-                if (keep < KEYS) {
-#pragma unroll
-                    for (int k = 0; k < EACH; ++k)
-                        if (((k * 64 + me) & (C::KV_BOX / 16 - 1)) / 8 >= keep) from[k * 64] = x[k] = make_uint4(0, 0, 0, 0);  // row of the box
+    } else {
+        if constexpr (LOW) asm volatile("setmaxnreg.dec.sync.aligned.u32 120;\n");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        if (warp == 0 || warp == (LOW ? 10 : 3)) {
+            // ------------------------------ items, tiles of keys; tiles of values ------------------------------
+            const RowsWork<X, TREE> work{a};
+            bool ok = true;
+            const bool v = warp != 0;
+            PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
+            // The next item into the ring; one without tokens at the end of the stretch
+            auto publish = [&](Item& it) {
+                Run run;
+                it.tokens = 0;
+                if (!line.next(work, run)) return;
+                const int count = run.to - run.from;
+                it.b = run.b; it.kvh = run.kvh; it.chunk = run.chunk;
+                it.token0 = run.i * a.block_tokens;
+                it.tokens = min(a.block_tokens, run.r.tokens - it.token0);
+                it.begin = run.r.begin; it.len = run.r.len; it.key0 = run.from * KEYS;
+                it.new_tile = TREE ? run.n - 1 - run.from : -1;
+                it.n0 = count;
+                it.n1 = 0;
+                if (!LOW && it.tokens > a.stream_tokens) {
+                    it.n1 = count;
+                    if (!TREE && a.causal) it.n0 = max(0, min((it.token0 + a.stream_tokens + KEYS - 1) / KEYS - run.from, count));
                 }
+                it.slot = run.slot(blockIdx.x);
+                if (run.from > 0) {
+                    record.head = run.to < run.n ? PART_GOES_ON : PART_LAST;
+                } else {
+                    if (record.head == PART_EMPTY) record.head = PART_NONE;
+                    if (run.to < run.n) {
+                        record.b = TREE ? it.b : 0; record.head0 = it.kvh * a.group + it.chunk * TILE; record.heads = min(TILE, a.group - it.chunk * TILE);
+                        record.token0 = it.begin + it.token0; record.tokens = it.tokens;
+                    }
+                }
+            };
+            Turn get{0, 0u}, at{0, 0u};  // of the items, of the ring
+            int made = 0;
+            bool filled = false;         // each place of the ring once
+            int ids_b = -1, ids_from = 0, ids = 0;  // entry ids_from + lane of request ids_b's row of the table
+            uint8_t* const ring = sKV + (v ? SLOTS * C::KV_BYTES : 0);
+            while (true) {
+                Item it;
+                if (v) {
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.item_full[get.at], get.phase, W_ITEM, made)))) break;
+                    it = sh.items[get.at];
+                    mbar_arrive_warp(&sh.item_empty[get.at], lane);
+                } else {
+                    publish(it);
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.item_empty[get.at], get.phase ^ 1u, W_ITEM_EMPTY, made)))) break;
+                    if (lane == 0) {
+                        sh.items[get.at] = it;
+                        mbar_arrive(&sh.item_full[get.at]);
+                    }
+                }
+                get.next(ITEMS);
+                if (it.tokens == 0) break;
+                if (!v) {  // its queries, in the place of those of the item before, or before that
+                    const int buf = made & (C::Q_BUFFERS - 1), use = made / C::Q_BUFFERS;
+                    if (use > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.q_empty[buf], (use - 1) & 1, W_Q_EMPTY, made)))) break;
+                    if (lane == 0) {
+                        const int streams = it.n1 > 0 ? 2 : 1, head = it.kvh * a.group + it.chunk * TILE;
+                        mbar_arrive_expect_tx(&sh.q_full[buf], streams * a.q_bytes);
 #pragma unroll
-                for (int k = 0; k < EACH; ++k) low[k * 64] = make_uint4(tf32_rest(x[k].x), tf32_rest(x[k].y), tf32_rest(x[k].z), tf32_rest(x[k].w));
-                fence_proxy_async_smem();
-                mbar_arrive_warp(&sh.kv_ready[at.at], lane);
-            } else {
-                for (int k = keep * 8 + me; k < C::KV_RAW / 16; k += 32) raw[k] = make_uint4(0, 0, 0, 0);
-                fence_proxy_async_smem();
-                mbar_arrive_warp(&sh.kv_ready[at.at], lane);
-                if (lane == 0) mbar_arrive(&sh.kv_empty[at.at]);  // a slot is filled again when this warp has seen what it held
+                        for (int x = 0; x < 2; ++x) {  // streams, or halves of the rows
+                            if (LOW || x < streams)
+                                tma_load_queries(sQ + (buf * 2 + x) * (TILE * 128), &map_q, &sh.q_full[buf], head, it.begin + it.token0 + (LOW ? 0 : x * a.stream_tokens), LOW ? x : 0, TREE ? it.b : 0);
+                        }
+                    }
+                }
+                ++made;
+                const int n = max(it.n0, it.n1);
+                int key = it.key0;
+                for (int j = 0; j < n; ++j, key += KEYS) {
+                    if (filled && !(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.empty[v][at.at], at.phase ^ 1u, W_EMPTY, j)))) break;
+                    uint64_t* const full = &sh.full[v][at.at];
+                    uint8_t* const to = ring + at.at * C::KV_BYTES;
+                    const bool fresh = TREE && j == it.new_tile;
+                    if (lane == 0) {
+                        sh.keep[v][at.at] = v && !fresh ? min(KEYS, it.len - key) : KEYS;
+                        mbar_arrive_expect_tx(full, C::KV_RAW);
+                        if (!TREE || fresh) tma_load_tile(to, v ? &map_v : &map_k, full, TREE ? 0 : it.begin + key, it.kvh, TREE ? it.b : 0);
+                    }
+                    if constexpr (TREE) {
+                        if (!fresh) {
+                            // A box of a page to a lane; pages that are none, and those behind the last, read as zeros.  The table is looked up 32
+                            // entries at a time: a look for every tile took longer than the tile.
+                            const int k = key + lane * a.box, page = (int)(((uint64_t)(uint32_t)k * a.page_mul) >> a.page_shift);
+                            const int first = __shfl_sync(0xffffffffu, page, 0), last = __shfl_sync(0xffffffffu, page, KEYS / a.box - 1);
+                            if (it.b != ids_b || first < ids_from || last >= ids_from + 32) {
+                                ids_b = it.b;
+                                ids_from = first;
+                                ids = first + lane < a.pool.width ? __ldcg(a.pool.pages + it.b * a.pool.pages_stride + first + lane) : -1;
+                            }
+                            const int id = __shfl_sync(0xffffffffu, ids, (page - ids_from) & 31);
+                            if (lane < KEYS / a.box) {
+#pragma unroll
+                                for (int half = 0; half < (LOW ? 2 : 1); ++half)
+                                    tma_load_box(to + half * C::KV_BOX + lane * a.box * 128, v ? &map_vp : &map_kp, full, k - page * a.pool.page, half, it.kvh, k < it.len ? id : -1);
+                            }
+                        }
+                    }
+                    at.next(SLOTS);
+                    filled |= at.at == 0;
+                }
+                if (!ok) break;
             }
-            for (int k = 0; k < EVERY; ++k) at.next(SLOTS);
+            if (ok && (LOW || v)) {  // to those who tend the tiles: no more
+                ok = !filled || __all_sync(0xffffffffu, mbar_wait(wc, &sh.empty[v][at.at], at.phase ^ 1u, W_EMPTY, -1));
+                if (ok && lane == 0) {
+                    sh.keep[v][at.at] = LAST;
+                    mbar_arrive(&sh.full[v][at.at]);
+                }
+            }
+            if (!v && a.parts && lane == 0) a.parts[blockIdx.x] = record;
+            // a CTA that gave up may have copies in flight: they get time to land
+            if (!ok)
+                for (const unsigned long long t0 = globaltimer_ns(); globaltimer_ns() - t0 < 100000ull;) {}
+        } else if (warp == 1) {
+            // ------------------------------ products ------------------------------
+            const uint32_t leader = elect_one_sync();
+            struct Barrier {
+                uint64_t* bar;
+                uint32_t parity;
+            };
+            // each barrier is looked at while the products before it are still being issued, and waited for if that look came too early
+            auto seen = [&](const Barrier& x) { return mbar_test_wait(x.bar, x.parity); };
+            auto wait = [&](bool was_seen, const Barrier& x, int id, int aux) {
+                return __all_sync(0xffffffffu, was_seen) || (bool)__all_sync(0xffffffffu, mbar_wait(wc, x.bar, x.parity, id, aux));
+            };
+            const uint32_t kv_addr = smem_u32(sKV);
+            const Desc q_desc = make_smem_desc(smem_u32(sQ), 16, 1024, DESC_SW128), k_desc = make_smem_desc(kv_addr, 16, 1024, DESC_SW128),
+                       v_desc = LOW ? mnmajor_desc(kv_addr + SLOTS * C::KV_BYTES, 0, C::KV_BOX) : make_smem_desc(kv_addr + SLOTS * C::KV_BYTES, 16, 1024, DESC_SW128);
+            const uint32_t negate = a.flip ? IDESC_NEGATE_A : 0u;
+            Turn k_tile{0, 0u}, v_tile{0, 0u}, p{0, 0u}, s_item{0, 0u}, o_item{0, 0u};
+            Cursor s, o;
+            int ahead = 0, k_slot = 0, v_slot = 0, s_buf = 0, items = 0, low_buf = 0;
+            int s_own[2] = {0, 0}, o_own[2] = {0, 0};  // the next barriers of a stream's own
+            auto after = [&](int (&own)[2], int t) {
+                const int x = t ? own[1] : own[0], y = x == 2 ? 0 : x + 1;
+                if (t) own[1] = y;
+                else own[0] = y;
+                return t * 3 + x;
+            };
+            bool ok = true, s_on = false, new_queries = false;
+            auto key_tile = [&]() -> Barrier { return LOW ? Barrier{&sh.ready[0][k_tile.at], k_tile.phase} : Barrier{&sh.full[0][k_tile.at], k_tile.phase}; };
+            auto value_tile = [&]() -> Barrier { return {&sh.ready[1][v_tile.at], v_tile.phase}; };
+            auto next_item = [&](Turn& turn, Cursor& c) -> bool {  // false: the end, or gave up
+                if (!(ok = wait(false, {&sh.item_full[turn.at], turn.phase}, W_ITEM, items))) return false;
+                const Item& it = sh.items[turn.at];
+                if ((int)uniform(it.tokens) == 0) return false;
+                c.start((int)uniform(it.n0), (int)uniform(it.n1));
+                return true;
+            };
+            bool s_new = true, o_new = true, seen_k = false, seen_v = false, seen_p = false;
+            int between = -1;
+#pragma unroll 1
+            while (ok) {
+                const bool fresh = s_new;
+                if (s_new) {
+                    s_on = next_item(s_item, s);
+                    if (!ok) break;
+                    s_new = false;
+                    ++between;
+                }
+                if (!s_on && ahead == 0) break;
+                if (o_new) {
+                    if (!next_item(o_item, o)) break;
+                    o_new = false;
+                }
+                const bool go = s_on && may_go<LOW>(between);
+                new_queries |= fresh;
+                if (go) {
+                    if (new_queries) {
+                        if (!(ok = wait(false, LOW ? Barrier{&sh.q_ready, (uint32_t)items & 1u} : Barrier{&sh.q_full[items & 1 & (C::Q_BUFFERS - 1)], (uint32_t)(items >> 1) & 1u}, W_Q, items))) break;
+                        new_queries = false;
+                    }
+                    if (s.first()) {
+                        if (!(ok = wait(seen_k, key_tile(), W_READY, items))) break;
+                        k_slot = k_tile.at;
+                        k_tile.next(SLOTS);
+                    }
+                    seen_k = false;
+                    tc_fence_after_sync();
+                    const Desc kd = k_desc + k_slot * C::KV_BYTES;
+                    const bool both = ahead >= BEHIND;  // O follows
+                    auto look = [&] {
+                        seen_v = o.first() && seen(value_tile());
+                        seen_p = seen({&sh.p_full[p.at], p.phase});
+                    };
+                    if constexpr (LOW) {
+                        constexpr uint32_t IDESC = make_idesc_tf32(TILE, KEYS, false, false);
+                        const uint32_t d = tmem + s_buf * 64;
+                        auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
+                            umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x, kd + y, IDESC, acc);
+                            umma_ts4<KMAJOR_STEP>(leader, d, tmem + LOW_COL_Q + x + 32, kd + (y + C::KV_BOX), IDESC, 1u);
+                        };
+                        eight(64, 0, 0u);
+                        eight(0, C::KV_RAW, 1u);
+                        if (both) look();
+                        eight(0, 0, 1u);
+                    } else {
+                        const uint32_t IDESC = make_idesc_16(TILE, KEYS, BF16, false) | negate;
+                        const uint32_t d = tmem + s_buf * 128;
+                        const Desc qd = q_desc + ((items & 1) * C::STREAMS + s.t) * C::Q_BYTES;
+                        umma_ss_16(leader, d, qd.d, kd.d, IDESC, 0u);
+                        umma_ss_16(leader, d, qd.d + 2, kd.d + 2, IDESC, 1u);
+                        if (both) look();
+                        umma_ss_16(leader, d, qd.d + 4, kd.d + 4, IDESC, 1u);
+                        umma_ss_16(leader, d, qd.d + 6, kd.d + 6, IDESC, 1u);
+                    }
+                    umma_commit_lead(leader, &sh.s_full[0][0] + after(s_own, s.t));
+                    if (s.last()) umma_commit_lead(leader, &sh.empty[0][k_slot]);
+                    s_buf = s_buf == 2 ? 0 : s_buf + 1;
+                    ++ahead;
+                    if (!s.next()) {
+                        if (!LOW) umma_commit_lead(leader, &sh.q_empty[items & (C::Q_BUFFERS - 1)]);
+                        ++items;
+                        s_item.next(ITEMS);
+                        s_new = true;
+                    }
+                }
+                if (ahead > BEHIND || !go) {  // O
+                    if (o.first()) {
+                        if (!(ok = wait(seen_v, value_tile(), W_READY, items))) break;
+                        v_slot = v_tile.at;
+                        v_tile.next(SLOTS);
+                    }
+                    if (!(ok = wait(seen_p, {&sh.p_full[p.at], p.phase}, W_P, items))) break;
+                    tc_fence_after_sync();
+                    seen_v = seen_p = false;
+                    const Desc vd = v_desc + v_slot * C::KV_BYTES;
+                    const uint32_t acc = o.j > 0;
+                    const bool look_k = s_on && !s_new && s.first() && o.last();
+                    if constexpr (LOW) {
+                        constexpr uint32_t IDESC = make_idesc_tf32(TILE, HEAD_DIM, false, true);
+                        const uint32_t high = tmem + p.at * 64, low = tmem + LOW_COL_LOW + low_buf * 64, d = tmem + LOW_COL_O;
+                        auto eight = [&](uint32_t x, uint32_t y, uint32_t acc) {
+                            umma_ts4<MNMAJOR_STEP>(leader, d, x, vd + y, IDESC, acc);
+                            umma_ts4<MNMAJOR_STEP>(leader, d, x + 32, vd + (y + 4096), IDESC, 1u);
+                        };
+                        eight(low, 0, 0u);
+                        eight(high, C::KV_RAW, 1u);
+                        seen_k = look_k && seen(key_tile());
+                        eight(high, 0, 1u);
+                        low_buf ^= 1;
+                    } else {
+                        constexpr uint32_t IDESC = make_idesc_16(TILE, HEAD_DIM, BF16, true);
+                        const uint32_t w = tmem + p.at * 128, d = tmem + COL_O + o.t * 64;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            if (k == 4) seen_k = look_k && seen(key_tile());
+                            umma_ts_16(leader, d, w + 8 * k, vd.d + (2048 >> 4) * k, IDESC, k > 0 ? 1u : acc);
+                        }
+                    }
+                    umma_commit_lead(leader, &sh.o_full[0][0] + after(o_own, o.t));
+                    if (o.last()) umma_commit_lead(leader, &sh.empty[1][v_slot]);
+                    p.next(3);
+                    --ahead;
+                    if (!o.next()) {
+                        if (lane == 0) mbar_arrive(&sh.item_empty[o_item.at]);
+                        o_item.next(ITEMS);
+                        --between;
+                        o_new = true;
+                    }
+                }
+            }
+        } else if (warp == 2 || (LOW && (warp == 3 || warp == 8 || warp == 9))) {
+            // What the tiles need beside the loads.  Rows behind the request's last key may hold anything, and 0 times a NaN is one: they are
+            // cleared among the values.  fp32: the tiles' low parts, by a pair of warps each for keys and values.
+            const int me = LOW ? threadIdx.x & 63 : lane, v = !LOW || warp >= 8;
+            Turn at{0, 0u};
+            while (true) {
+                if (!__all_sync(0xffffffffu, mbar_wait(wc, &sh.full[v][at.at], at.phase, W_KV, at.at))) break;
+                const int keep = sh.keep[v][at.at];
+                if (keep == LAST) break;
+                uint4* raw = reinterpret_cast<uint4*>(sKV + (v * SLOTS + at.at) * C::KV_BYTES);
+                if constexpr (LOW) {
+                    constexpr int EACH = C::KV_RAW / 16 / 64;
+                    uint4 *from = raw + me, *low = from + C::KV_RAW / 16, x[EACH];
+#pragma unroll
+                    for (int k = 0; k < EACH; ++k) x[k] = from[k * 64];
+                    if (keep < KEYS) {
+#pragma unroll
+                        for (int k = 0; k < EACH; ++k)
+                            if (((k * 64 + me) & (C::KV_BOX / 16 - 1)) / 8 >= keep) from[k * 64] = x[k] = make_uint4(0, 0, 0, 0);  // row of the box
+                    }
+#pragma unroll
+                    for (int k = 0; k < EACH; ++k) low[k * 64] = make_uint4(tf32_rest(x[k].x), tf32_rest(x[k].y), tf32_rest(x[k].z), tf32_rest(x[k].w));
+                    fence_proxy_async_smem();
+                    mbar_arrive_warp(&sh.ready[v][at.at], lane);
+                } else {
+                    if (keep < KEYS) {
+                        for (int k = keep * 8 + me; k < C::KV_RAW / 16; k += 32) raw[k] = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                    }
+                    mbar_arrive_warp(&sh.ready[v][at.at], lane);
+                    if (lane == 0) mbar_arrive(&sh.empty[v][at.at]);  // a slot is filled again when this warp has seen what it held
+                }
+                at.next(SLOTS);
+            }
         }
     }
     tc_fence_before_sync();
@@ -930,6 +903,7 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     vp = v;
     if (TREE) {
         a.box = std::gcd(a.pool.page, C::KEYS);
+        divide_by(a.pool.page, a.page_mul, a.page_shift);
         if ((s = page_map(&kp, a.pool.K, dtype, a.pool.n_pages, a.Hk, a.pool.page, a.box, false)) ||
             (s = page_map(&vp, a.pool.V, dtype, a.pool.n_pages, a.Hk, a.pool.page, a.box, C::LOW)))
             return s;
