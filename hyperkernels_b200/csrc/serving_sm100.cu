@@ -243,15 +243,82 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 mbar_arrive_warp(&sh.q_empty[0], lane);
             }
         };
+        // The result of an item, or a part of it, from O of its tiles: 32 columns at a time, in loops, for this runs once an item and what bounds it
+        // is how fast its instructions come.  Where it goes is looked up again, not kept in registers all the while.
+        auto finish = [&](int place_of_item, float m, float l, int n, const float* o) {
+            asm volatile("" ::: "memory");
+            const Item& it = sh.items[place_of_item];
+            const bool valid = my_token < it.tokens && my_head < a.group - it.chunk * TILE, live = __any_sync(0xffffffffu, valid);
+            if (!LOW && n > 0 && !wait(sh.o_full[t], own - 1, W_O)) return;
+            const int slot = it.slot;
+            const float f = slot >= 0 ? 1.f : l != 0.f ? rcp_approx(l) : 0.f;
+            const int b = TREE ? it.b : 0, row = it.begin + it.token0 + (valid ? my_token : 0), h = it.kvh * a.group + it.chunk * TILE + my_head;
+            X* const to = const_cast<X*>(row_of<X>(a.O, b, h, row));
+            const int64_t at_slot = (int64_t)slot * C::BLOCK + r;
+            if (LOW || slot >= 0) {
+                uint4* const whole = reinterpret_cast<uint4*>(slot >= 0 ? a.part + at_slot * 64 : reinterpret_cast<float*>(to));
+#pragma unroll(LOW ? 2 : 1)
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t y[32];
+                    if constexpr (LOW) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(o[32 * half + i] * f);
+                    } else if (n > 0) {
+                        tmem_ld32(lanes + COL_O + t * 64 + 32 * half, y);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] = 0u;
+                    }
+                    if (valid) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) whole[8 * half + i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                    }
+                }
+            } else if (live) {
+                if constexpr (!LOW) {
+                    // Through shared memory, so that eight lanes store a row: a row to a lane is 32 lines an instruction.
+                    uint4* const mine = reinterpret_cast<uint4*>(smem + Space::OFF_O + (warp - 4) * 4096);
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t y[32];
+                        tmem_ld32(lanes + COL_O + t * 64 + 32 * half, y);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] = pack<X>(__uint_as_float(y[2 * i]) * f, __uint_as_float(y[2 * i + 1]) * f);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mine[lane * 8 + ((4 * half + i) ^ (lane & 7))] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                    }
+                    __syncwarp();
+                    const uint64_t place = valid ? reinterpret_cast<uint64_t>(to) : 0ull;
+#pragma unroll 4
+                    for (int i = 0; i < 8; ++i) {
+                        const int from = 4 * i + (lane >> 3);
+                        const uint64_t at = __shfl_sync(0xffffffffu, place, from);
+                        const uint4 v = mine[from * 8 + ((lane ^ from) & 7)];
+                        if (at) reinterpret_cast<uint4*>(at)[lane & 7] = v;
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!LOW) tc_fence_before_sync();
+            if (valid) {
+                if (slot >= 0) a.ml[at_slot] = make_float2(m, l);
+                else a.LSE[b * a.lse_sB + h * a.lse_sH + row] = l != 0.f ? (m + __log2f(l)) * LN2 : -INFINITY;
+            }
+            mbar_arrive_warp(&sh.item_empty[place_of_item], lane);
+        };
+        int last_at = -1, last_n = 0;  // 16-bit types: the item before this one, whose O is taken out under the first tile of this
+        float last_m = 0.f, last_l = 0.f;
         Turn get{0, 0u};
         while (ok) {
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(wc, &sh.item_full[get.at], get.phase, W_ITEM, q0)))) break;
             const Item& it = sh.items[get.at];
             const int tokens = it.tokens;
-            if (tokens == 0) break;
+            if (LOW && tokens == 0) break;
             const bool valid = my_token < tokens && my_head < a.group - it.chunk * TILE, live = __any_sync(0xffffffffu, valid);
             const int token = it.token0 + (valid ? my_token : 0);
-            const int new_tile = it.new_tile, n = t == 0 ? it.n0 : it.n1;
+            const int new_tile = it.new_tile, n = tokens == 0 ? 0 : t == 0 ? it.n0 : it.n1;
             const int limit = (!valid ? INT_MAX / 2 : !TREE && a.causal ? token + 1 : it.len) - it.key0;  // keys that the row sees, from the first tile's on
             const uint64_t bits = TREE && valid ? tree_bits(a, it.b, token) : 0ull;
             // the item's product of tile j: the other stream's come in between
@@ -338,10 +405,11 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 constexpr int POLY_OF = 5;  // of so many pairs of weights, one by the polynomial
                 const uint32_t at_o = lanes + COL_O + t * 64;
                 uint32_t x[128];
-                for (int j = 0; j < n && wait(sh.s_full[t], own, W_S); ++j, ++own) {
+                for (int j = 0; j < max(n, 1); ++j) {
+                    if (n > 0 && !wait(sh.s_full[t], own, W_S)) break;
                     const int q = product(j);
                     const uint32_t at_s = lanes + q % 3 * 128;
-                    if (live) {
+                    if (live && n > 0) {
                         const bool fresh = TREE && j == new_tile;
                         const int lim = fresh ? 0 : limit - j * KEYS;  // columns the row sees
                         auto load = [&] {
@@ -466,74 +534,24 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         l = fmaf(l, alpha, add);
                         tmem_wait_st();
                     }
+                    if (j == 0 && last_at >= 0) finish(last_at, last_m, last_l, last_n, nullptr);
+                    if (n == 0 || !ok) break;
                     tc_fence_before_sync();
                     mbar_arrive_warp(&sh.p_full[q % 3], lane);
+                    ++own;
                 }
-                m -= lift<X>();  // what the weights were taken by
-                if (ok && n > 0) wait(sh.o_full[t], own - 1, W_O);
+                if (tokens == 0) break;
             }
             q0 += it.n0 + it.n1;
             if (!ok) break;
-            // Where it goes is looked up again, not kept in registers all the while
-            asm volatile("" ::: "memory");
-            // 32 columns of O at a time, in loops: this runs once an item, and what bounds it is how fast its instructions come.
-            const int slot = it.slot;
-            const float f = slot >= 0 ? 1.f : l != 0.f ? rcp_approx(l) : 0.f;
-            const int b = TREE ? it.b : 0, row = it.begin + it.token0 + (valid ? my_token : 0), h = it.kvh * a.group + it.chunk * TILE + my_head;
-            X* const to = const_cast<X*>(row_of<X>(a.O, b, h, row));
-            const int64_t at_slot = (int64_t)slot * C::BLOCK + r;
-            if (LOW || slot >= 0) {
-                uint4* const whole = reinterpret_cast<uint4*>(slot >= 0 ? a.part + at_slot * 64 : reinterpret_cast<float*>(to));
-#pragma unroll(LOW ? 2 : 1)
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t y[32];
-                    if constexpr (LOW) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(o[32 * half + i] * f);
-                    } else if (n > 0) {
-                        tmem_ld32(lanes + COL_O + t * 64 + 32 * half, y);
-                        tmem_wait_ld();
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] = 0u;
-                    }
-                    if (valid) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) whole[8 * half + i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                    }
-                }
-            } else if (live) {
-                if constexpr (!LOW) {
-                    // Through shared memory, so that eight lanes store a row: a row to a lane is 32 lines an instruction.
-                    uint4* const mine = reinterpret_cast<uint4*>(smem + Space::OFF_O + (warp - 4) * 4096);
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t y[32];
-                        tmem_ld32(lanes + COL_O + t * 64 + 32 * half, y);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) y[i] = pack<X>(__uint_as_float(y[2 * i]) * f, __uint_as_float(y[2 * i + 1]) * f);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) mine[lane * 8 + ((4 * half + i) ^ (lane & 7))] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                    }
-                    __syncwarp();
-                    const uint64_t place = valid ? reinterpret_cast<uint64_t>(to) : 0ull;
-#pragma unroll 4
-                    for (int i = 0; i < 8; ++i) {
-                        const int from = 4 * i + (lane >> 3);
-                        const uint64_t at = __shfl_sync(0xffffffffu, place, from);
-                        const uint4 v = mine[from * 8 + ((lane ^ from) & 7)];
-                        if (at) reinterpret_cast<uint4*>(at)[lane & 7] = v;
-                    }
-                    __syncwarp();
-                }
+            if constexpr (LOW) {
+                finish(get.at, m, l, n, o);
+            } else {
+                last_at = get.at;
+                last_n = n;
+                last_m = m - lift<X>();  // what the weights were taken by
+                last_l = l;
             }
-            if (!LOW) tc_fence_before_sync();
-            if (valid) {
-                if (slot >= 0) a.ml[at_slot] = make_float2(m, l);
-                else a.LSE[b * a.lse_sB + h * a.lse_sH + row] = l != 0.f ? (m + __log2f(l)) * LN2 : -INFINITY;
-            }
-            mbar_arrive_warp(&sh.item_empty[get.at], lane);
             get.next(ITEMS);
         }
     } else {
