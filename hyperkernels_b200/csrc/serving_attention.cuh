@@ -60,9 +60,10 @@ struct Request {
 };
 // A block counts as the keys that it meets and EXTRA for its beginning and end, in units of 2^unit_shift keys, so that all of them fit 32
 // bits: a division of 64-bit numbers takes a warp some 300 cycles.
-template <int KEYS_, int LEAST_, int SHARE_, int EXTRA, bool TREE>
+template <int KEYS_, int LEAST_, int SHARE_, int EXTRA, bool TREE, int DEAL_ = 0>
 struct Work {
-    static constexpr int KEYS = KEYS_, LEAST = LEAST_, SHARE = SHARE_;  // of a tile; tiles that a part of a block has, and a worker, at least
+    // keys of a tile; tiles that a part of a block has, and a worker, at least; blocks for each worker from which on they are dealt out (0: never)
+    static constexpr int KEYS = KEYS_, LEAST = LEAST_, SHARE = SHARE_, DEAL = DEAL_;
     const ServingArgs& a;
     __device__ __forceinline__ int all_tiles(const Request& r) const { return (r.len + KEYS - 1) / KEYS + (TREE ? a.new_tiles : 0); }
     __device__ __forceinline__ int tiles(const Request& r, int i) const {
@@ -98,25 +99,50 @@ struct Run {
 template <int N>
 struct LineSearch {
     int sums[32], blocks[32];  // of the warps' requests
-    int b[N], left[N];         // a stretch's first request, and how far behind its beginning
+    Request r[N];              // a stretch's first request, and how far behind its beginning
+    int b[N], left[N];
 };
 // A worker's stretch of the line: it begins in block i of request b under key head kvh (blocks of the first chunk of heads, of the second,
 // ..), `done` units behind the block's beginning, and goes on for `units`.
+// Where causal prompts make many blocks, these are dealt out whole instead, the longest first, there and back along the workers: no parts, and the
+// workers' shares differ by less than their last blocks.  (16 prompts of 17 to 1 000 tokens, 32 heads on 8, bf16: see serving_sm100.cu.)
 template <class W>
 struct Line {
     Request r;
     int b, kvh, chunk, i, done, units;
+    int me, workers, round, level, before_level;  // dealt: blocks of longer ones, all from `level` on
+    bool dealt;
+    int tall[4];  // dealt: blocks of request 32 k + lane
 
-    // The stretches of worker `me` of at most `workers`, cut in N (of a CTA's warps, say), by all threads.  Stretch k is made for the threads
-    // that ask for it; those of a warp have to ask for the same.
-    template <int N>
-    __device__ __forceinline__ void find(const W& work, LineSearch<N>& sh, int me, int workers, int k) {
+    // Put down for the time until a warp takes it up: held in registers it costs those of the others.
+    struct Saved;
+    __device__ __forceinline__ void save(Saved& to) const {
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) to.line = *this;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to.tall[k][lane] = tall[k];
+        __syncwarp();
+    }
+    __device__ __forceinline__ void load(const Saved& from) {
+        *this = from.line;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tall[k] = from.tall[k][threadIdx.x & 31];
+    }
+
+    static constexpr int DEAL_REQUESTS = 128;
+
+    // The stretches of worker `me` of at most `most`, cut in N (of a CTA's warps, say), by all THREADS threads.  Stretch k is made for the
+    // threads that ask for it; those of a warp have to ask for the same.
+    template <int THREADS, int N>
+    __device__ __forceinline__ void find(const W& work, LineSearch<N>& sh, int worker, int most, int k) {
         const ServingArgs& a = work.a;
-        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, each = (a.B + (int)blockDim.x - 1) / (int)blockDim.x;
+        constexpr int WARPS = THREADS / 32;
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = (a.B + THREADS - 1) / THREADS;
         int sum = 0, n = 0;
+        Request one = {};
         for (int x = 0; x < each; ++x) {
             if (tid * each + x >= a.B) break;
-            const Request one = work.request(tid * each + x);
+            one = work.request(tid * each + x);
             sum += one.units;
             n += min(one.blocks * a.chunks, 1 << 20);
         }
@@ -135,29 +161,49 @@ struct Line {
         __syncthreads();
         int all = 0, from = upto - sum;
         n = 0;
-        for (int w = 0; w < warps; ++w) {
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
             if (w < warp) from += sh.sums[w];
             all += sh.sums[w];
             n = min(n + sh.blocks[w], 1 << 20);
         }
         all *= a.Hk;
+        const int64_t n_blocks = (int64_t)n * a.Hk;
+        dealt = W::DEAL > 0 && a.causal && a.B <= DEAL_REQUESTS && n_blocks >= (int64_t)W::DEAL * most;
+        if (dealt) {
+            me = worker;
+            workers = most;
+            round = before_level = level = 0;
+            units = 1;
+            if (warp == 0) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    tall[x] = 32 * x + lane < a.B ? work.request(32 * x + lane).blocks : 0;
+                    level = max(level, tall[x]);
+                }
+                level = __reduce_max_sync(0xffffffffu, level) - 1;
+            }
+            __syncthreads();
+            return;
+        }
         // a worker to N blocks, more if the blocks are long, as many as there are
-        workers = min(workers, max((int)min((int64_t)workers, ((int64_t)n * a.Hk + N - 1) / N), all / max(1, N * W::SHARE * W::KEYS >> a.unit_shift)));
-        const bool mine = me < workers;
-        const int share = mine ? (unsigned)all / (unsigned)workers : 0, more = all - share * workers, begin = me * share + min(me, more), length = mine ? share + (me < more) : 0;
+        workers = min(most, max((int)min((int64_t)most, (n_blocks + N - 1) / N), all / max(1, N * W::SHARE * W::KEYS >> a.unit_shift)));
+        const bool mine = worker < workers;
+        const int share = mine ? (unsigned)all / (unsigned)workers : 0, more = all - share * workers, begin = worker * share + min(worker, more), length = mine ? share + (worker < more) : 0;
         auto border = [&](int k) { return k == N ? begin + length : begin + length / N * k; };
 #pragma unroll
         for (int x = 0; x < N; ++x) {
             int left = border(x) - from * a.Hk;
             if (!mine || left < 0 || left >= sum * a.Hk) continue;
             for (int y = 0; y < each; ++y) {
-                const int one = work.request(tid * each + y).units * a.Hk;
-                if (left < one) {
+                if (each > 1) one = work.request(tid * each + y);
+                if (left < one.units * a.Hk) {
                     sh.b[x] = tid * each + y;
                     sh.left[x] = left;
+                    sh.r[x] = one;
                     break;
                 }
-                left -= one;
+                left -= one.units * a.Hk;
             }
         }
         __syncthreads();
@@ -165,7 +211,7 @@ struct Line {
         units = mine && b >= 0 ? border(k + 1) - border(k) : 0;
         if (units <= 0) return;
         int left = sh.left[k];
-        r = work.request(b);
+        r = sh.r[k];
         kvh = r.units > 0 ? (unsigned)left / (unsigned)r.units : a.Hk;
         if (kvh >= a.Hk) {  // starts that do not ascend can come to more than 32 bits: such a call gives nothing of use, but stays inside
             units = 0;
@@ -188,6 +234,49 @@ struct Line {
         i = lo;
         done = left - work.before(r, lo);
     }
+    // The next block that is dealt to this worker, by a warp: number x of all in the order of the levels, each of the blocks i = level of all
+    // requests that have so many
+    __device__ __forceinline__ bool next_dealt(const W& work, Run& run) {
+        const int lane = threadIdx.x & 31, x = round * workers + (round & 1 ? workers - 1 - me : me), each = work.a.Hk * work.a.chunks;
+        ++round;
+        while (level >= 0) {
+            unsigned have[4];
+            int n = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                have[k] = __ballot_sync(0xffffffffu, tall[k] > level);
+                n += __popc(have[k]);
+            }
+            if (x >= before_level + n * each) {
+                before_level += n * each;
+                --level;
+                continue;
+            }
+            int rest = x - before_level, q = rest / each;  // the q-th of them
+            rest -= q * each;
+            int request = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = __popc(have[k]);
+                if (q >= 0 && q < c) {
+                    const unsigned it = __ballot_sync(0xffffffffu, (have[k] >> lane & 1) && __popc(have[k] & ((1u << lane) - 1)) == q);
+                    request = 32 * k + __ffs(it) - 1;
+                    q = -1;
+                } else if (q >= 0) {
+                    q -= c;
+                }
+            }
+            run.r = work.request(request);
+            run.b = request;
+            run.kvh = rest / work.a.chunks;
+            run.chunk = rest - run.kvh * work.a.chunks;
+            run.i = level;
+            run.from = 0;
+            run.to = run.n = work.tiles(run.r, level);
+            return true;
+        }
+        return false;
+    }
     // A border inside a block is moved to its beginning or end where a part of less than LEAST tiles would be left.
     __device__ __forceinline__ int border(const W& work, int units, int n) const {
         const int j = (int)min((int64_t)n, ((int64_t)units << work.a.unit_shift) / W::KEYS);
@@ -195,6 +284,7 @@ struct Line {
     }
     // The next run; false: the stretch is over
     __device__ __forceinline__ bool next(const W& work, Run& run) {
+        if (W::DEAL > 0 && dealt) return next_dealt(work, run);
         while (units > 0) {
             if (i >= r.blocks) {
                 i = 0;
@@ -217,6 +307,11 @@ struct Line {
         }
         return false;
     }
+};
+template <class W>
+struct Line<W>::Saved {
+    Line line;
+    int tall[4][32];
 };
 // Host: x / d is x * mul >> shift for x below 2^31.
 inline void divide_by(int d, uint32_t& mul, int& shift) {

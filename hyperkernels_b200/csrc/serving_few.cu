@@ -194,7 +194,7 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     pdl_trigger();
     const W work{a};
     Line<W> line;
-    line.find(work, sh.search, blockIdx.x, gridDim.x, warp);
+    line.template find<WARPS * 32>(work, sh.search, blockIdx.x, gridDim.x, warp);
     WaitNote wc{&sh.abort};
     PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
 
@@ -370,8 +370,8 @@ int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
     CUtensorMap k, v, kp, vp;
     int s;
     if ((s = prefix_tile_map(&k, a.K, dtype, a.B, a.Hk, a.T, e.keys, false)) || (s = prefix_tile_map(&v, a.V, dtype, a.B, a.Hk, a.T, e.keys, false)) ||
-        (s = prefix_tile_map(&kp, a.pool.K, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false)) ||
-        (s = prefix_tile_map(&vp, a.pool.V, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false)))
+        (s = prefix_tile_map(&kp, a.pool.K, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false, a.pool.K.strideM != HEAD_DIM)) ||
+        (s = prefix_tile_map(&vp, a.pool.V, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false, a.pool.V.strideM != HEAD_DIM)))
         return s;
     const int ctas = sm_count() * e.per_sm;
     LaunchConfig lc(ctas, WARPS * 32, e.smem, stream, 1, true);

@@ -41,9 +41,9 @@ struct Rows {
     static constexpr int ITEMS = 8;
 };
 
-// half a tile is masked, and a block's beginning and end take as long as a tile
+// half a tile is masked, and a block's beginning and end take as long as a tile (fp32: 3.7 us, nearly three)
 template <class X, bool TREE>
-using RowsWork = Work<Rows<X>::KEYS, Rows<X>::LEAST, 3 * Rows<X>::LEAST, Rows<X>::KEYS * 3 / 2, TREE>;
+using RowsWork = Work<Rows<X>::KEYS, Rows<X>::LEAST, 3 * Rows<X>::LEAST, Rows<X>::KEYS * (sizeof(X) == 4 ? 6 : 3) / 2, TREE, TREE ? 0 : 5>;
 
 struct __align__(16) Item {
     int b, kvh, chunk;   // request, key head, which 128 of its query heads
@@ -55,7 +55,7 @@ struct __align__(16) Item {
     int new_tile;        // number of the tile that is the new tokens'
 };
 
-template <class X>
+template <class X, bool TREE>
 struct __align__(16) RowsShared {
     typedef Rows<X> C;
     uint64_t q_full[C::Q_BUFFERS], q_empty[C::Q_BUFFERS], q_ready, p_full[3];
@@ -65,6 +65,7 @@ struct __align__(16) RowsShared {
     uint64_t ready[2][C::SLOTS];                     // tended: low parts are there, what is behind a last key is cleared
     Item items[C::ITEMS];
     LineSearch<1> search;
+    typename Line<RowsWork<X, TREE>>::Saved line;
     int keep[2][C::SLOTS];  // rows of the tile that are values, LAST: none follows
     uint32_t tmem_base;
     Abort abort;
@@ -74,7 +75,8 @@ constexpr int LAST = -1;
 template <class X>
 struct RowsSpace {
     typedef Rows<X> C;
-    static constexpr int OFF_Q = 2 * C::SLOTS * C::KV_BYTES, OFF_O = OFF_Q + C::STREAMS * C::Q_BUFFERS * C::Q_BYTES, OFF_SH = OFF_O + (C::LOW ? 0 : C::SOFTMAX_WARPS * 4096), SMEM = OFF_SH + (int)sizeof(RowsShared<X>);
+    static constexpr int OFF_Q = 2 * C::SLOTS * C::KV_BYTES, OFF_O = OFF_Q + C::STREAMS * C::Q_BUFFERS * C::Q_BYTES, OFF_SH = OFF_O + (C::LOW ? 0 : C::SOFTMAX_WARPS * 4096), SMEM = OFF_SH + (int)sizeof(RowsShared<X, false>);
+    static_assert(sizeof(RowsShared<X, false>) == sizeof(RowsShared<X, true>), "");
     static_assert(SMEM <= 232448, "exceeds the 227 KiB a CTA may opt in to");
 };
 // Tensor memory.  16-bit types: three buffers of 128 columns for scores and weights, O of two streams.  fp32: three buffers of
@@ -145,7 +147,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     constexpr int KEYS = C::KEYS, SLOTS = C::SLOTS, ITEMS = C::ITEMS;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *sKV = smem, *sQ = smem + Space::OFF_Q;
-    RowsShared<X>& sh = *reinterpret_cast<RowsShared<X>*>(smem + Space::OFF_SH);
+    RowsShared<X, TREE>& sh = *reinterpret_cast<RowsShared<X, TREE>*>(smem + Space::OFF_SH);
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     if (warp == 2 && lane < (TREE ? 5 : 3)) tma_prefetch_desc(lane == 0 ? &map_q : lane == 1 ? &map_k : lane == 2 ? &map_v : lane == 3 ? &map_kp : &map_vp);
@@ -187,8 +189,11 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
     pdl_wait();
     pdl_trigger();
-    Line<RowsWork<X, TREE>> line;
-    line.find(RowsWork<X, TREE>{a}, sh.search, blockIdx.x, gridDim.x, 0);
+    {
+        Line<RowsWork<X, TREE>> line;
+        line.template find<C::THREADS>(RowsWork<X, TREE>{a}, sh.search, blockIdx.x, gridDim.x, 0);
+        if (warp == 0) line.save(sh.line);
+    }
     tc_fence_after_sync();
     constexpr uint32_t tmem = 0;  // all columns are this CTA's
     if (sh.tmem_base != tmem) sh.abort.id = 598;
@@ -240,7 +245,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 tmem_wait_st();
                 tc_fence_before_sync();
                 mbar_arrive_warp(&sh.q_ready, lane);
-                mbar_arrive_warp(&sh.q_empty[0], lane);
+                if (fetched == 1) mbar_arrive_warp(&sh.q_empty[0], lane);  // later ones' place is needed for O first
             }
         };
         // The result of an item, or a part of it, from O of its tiles: 32 columns at a time, in loops, for this runs once an item and what bounds it
@@ -255,51 +260,61 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const int b = TREE ? it.b : 0, row = it.begin + it.token0 + (valid ? my_token : 0), h = it.kvh * a.group + it.chunk * TILE + my_head;
             X* const to = const_cast<X*>(row_of<X>(a.O, b, h, row));
             const int64_t at_slot = (int64_t)slot * C::BLOCK + r;
-            if (LOW || slot >= 0) {
-                uint4* const whole = reinterpret_cast<uint4*>(slot >= 0 ? a.part + at_slot * 64 : reinterpret_cast<float*>(to));
-#pragma unroll(LOW ? 2 : 1)
+            // Through shared memory, so that 8 lanes store 128 bytes of a row: a row to a lane is 32 lines an instruction.  fp32: in place of the
+            // warp's rows of the queries that have just gone to tensor memory, 16 lanes to a row.  What is left is the way out of the SM for 32 KB.
+            constexpr int LANES = LOW ? 16 : 8;
+            uint8_t* const stage = LOW ? sQ + quarter * 4096 : smem + Space::OFF_O + (warp - 4) * 4096;
+            const uint64_t place = !valid ? 0ull : slot >= 0 ? reinterpret_cast<uint64_t>(a.part + at_slot * 64) : reinterpret_cast<uint64_t>(to);
+            auto store = [&](int offset) {
+                __syncwarp();
+#pragma unroll 4
+                for (int i = 0; i < LANES; ++i) {
+                    const int from = (32 / LANES) * i + lane / LANES, c = lane % LANES;
+                    const uint64_t at = __shfl_sync(0xffffffffu, place, from);
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage + (c >> 3) * (TILE * 128) + from * 128 + (((c & 7) ^ (from & 7)) << 4));
+                    if (at) reinterpret_cast<uint4*>(at + offset)[c] = v;
+                }
+                __syncwarp();
+            };
+            auto put = [&](int c, uint4 v) { *reinterpret_cast<uint4*>(stage + (c >> 3) * (TILE * 128) + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) = v; };
+            if constexpr (LOW) {
+                if (live) {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        put(c, make_uint4(__float_as_uint(o[4 * c] * f), __float_as_uint(o[4 * c + 1] * f), __float_as_uint(o[4 * c + 2] * f), __float_as_uint(o[4 * c + 3] * f)));
+                    store(0);
+                }
+            } else if (live && slot >= 0) {
+#pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     uint32_t y[32];
-                    if constexpr (LOW) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(o[32 * half + i] * f);
-                    } else if (n > 0) {
+                    if (n > 0) {
                         tmem_ld32(lanes + COL_O + t * 64 + 32 * half, y);
                         tmem_wait_ld();
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) y[i] = 0u;
                     }
-                    if (valid) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) whole[8 * half + i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                    }
+                    for (int c = 0; c < 8; ++c) put(c, make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]));
+                    store(128 * half);
                 }
             } else if (live) {
-                if constexpr (!LOW) {
-                    // Through shared memory, so that eight lanes store a row: a row to a lane is 32 lines an instruction.
-                    uint4* const mine = reinterpret_cast<uint4*>(smem + Space::OFF_O + (warp - 4) * 4096);
 #pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t y[32];
-                        tmem_ld32(lanes + COL_O + t * 64 + 32 * half, y);
-                        tmem_wait_ld();
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t y[32];
+                    tmem_ld32(lanes + COL_O + t * 64 + 32 * half, y);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) y[i] = pack<X>(__uint_as_float(y[2 * i]) * f, __uint_as_float(y[2 * i + 1]) * f);
+                    for (int i = 0; i < 16; ++i) y[i] = pack<X>(__uint_as_float(y[2 * i]) * f, __uint_as_float(y[2 * i + 1]) * f);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) mine[lane * 8 + ((4 * half + i) ^ (lane & 7))] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                    }
-                    __syncwarp();
-                    const uint64_t place = valid ? reinterpret_cast<uint64_t>(to) : 0ull;
-#pragma unroll 4
-                    for (int i = 0; i < 8; ++i) {
-                        const int from = 4 * i + (lane >> 3);
-                        const uint64_t at = __shfl_sync(0xffffffffu, place, from);
-                        const uint4 v = mine[from * 8 + ((lane ^ from) & 7)];
-                        if (at) reinterpret_cast<uint4*>(at)[lane & 7] = v;
-                    }
-                    __syncwarp();
+                    for (int c = 0; c < 4; ++c) put(4 * half + c, make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]));
                 }
+                store(0);
+            }
+            if (LOW) {
+                fence_proxy_async_smem();
+                mbar_arrive_warp(&sh.q_empty[0], lane);
             }
             if (!LOW) tc_fence_before_sync();
             if (valid) {
@@ -560,6 +575,8 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (warp == 0 || warp == (LOW ? 10 : 3)) {
             // ------------------------------ items, tiles of keys; tiles of values ------------------------------
             const RowsWork<X, TREE> work{a};
+            Line<RowsWork<X, TREE>> line;
+            line.load(sh.line);
             bool ok = true;
             const bool v = warp != 0;
             PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
@@ -878,7 +895,7 @@ int page_map(CUtensorMap* map, const hk_view& v, int dtype, int n_pages, int H, 
     cuuint32_t box[5] = {(cuuint32_t)inner, (cuuint32_t)rows, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
     const CUtensorMapDataType type = dtype == HK_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == HK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const CUresult r = enc(map, type, 5, v.ptr, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, mn_major ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                           e == 2 && v.strideM != HEAD_DIM ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? HK_OK : HK_ERR_CUDA;
 }
 

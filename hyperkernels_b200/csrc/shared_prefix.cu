@@ -228,7 +228,7 @@ constexpr size_t SLOT_BYTES = 64 * sizeof(float) + sizeof(float2);
 
 }  // namespace
 
-int prefix_tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, int rows, bool mn_major) {
+int prefix_tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, int rows, bool mn_major, bool lines) {
     if (T == 0) {
         memset(map, 0, sizeof(*map));  // no tile of it is loaded
         return HK_OK;
@@ -241,7 +241,8 @@ int prefix_tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, in
     cuuint64_t strides[4] = {(cuuint64_t)sM * 2, 128, (cuuint64_t)sH * 2, (cuuint64_t)sB * 2};
     cuuint32_t box[5] = {HEAD_DIM, (cuuint32_t)rows, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
     const CUresult r = enc(map, dtype == HK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, v.ptr, dims, strides, box, ones,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, lines ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? HK_OK : HK_ERR_CUDA;
 }
 

@@ -70,6 +70,7 @@ __host__ __device__ constexpr float lift() { return std::is_same<X, __half>::val
 
 // Tiles of `rows` rows of a view of keys or values, all heads and batches (tma_load_tile): 128 bytes of each row side by side,
 // swizzled; fp32 rows are two such pieces.  mn_major: the values as an MN-major operand of fp32 products.
-int prefix_tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, int rows, bool mn_major);
+// lines: 128 bytes are brought into the L2, not 256; for rows of 16-bit types whose neighbours are asked for by others, at other times.
+int prefix_tile_map(CUtensorMap* map, const hk_view& v, int dtype, int64_t B, int H, int64_t T, int rows, bool mn_major, bool lines = false);
 
 }  // namespace hk
