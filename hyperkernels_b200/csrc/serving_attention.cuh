@@ -110,26 +110,11 @@ template <class W>
 struct Line {
     Request r;
     int b, kvh, chunk, i, done, units;
-    int me, workers, round, level, before_level;  // dealt: blocks of longer ones, all from `level` on
-    bool dealt;
-    int tall[4];  // dealt: blocks of request 32 k + lane
+    bool dealt;  // to this CTA, in rounds: the next is b, and the level that it comes to i, with `done` blocks in the levels in front
 
+    static constexpr int DEAL_REQUESTS = 128;  // 32 k + lane
     // Put down for the time until a warp takes it up: held in registers it costs those of the others.
     struct Saved;
-    __device__ __forceinline__ void save(Saved& to) const {
-        const int lane = threadIdx.x & 31;
-        if (lane == 0) to.line = *this;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) to.tall[k][lane] = tall[k];
-        __syncwarp();
-    }
-    __device__ __forceinline__ void load(const Saved& from) {
-        *this = from.line;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tall[k] = from.tall[k][threadIdx.x & 31];
-    }
-
-    static constexpr int DEAL_REQUESTS = 128;
 
     // The stretches of worker `me` of at most `most`, cut in N (of a CTA's warps, say), by all THREADS threads.  Stretch k is made for the
     // threads that ask for it; those of a warp have to ask for the same.
@@ -171,23 +156,16 @@ struct Line {
         const int64_t n_blocks = (int64_t)n * a.Hk;
         dealt = W::DEAL > 0 && a.causal && a.B <= DEAL_REQUESTS && n_blocks >= (int64_t)W::DEAL * most;
         if (dealt) {
-            me = worker;
-            workers = most;
-            round = before_level = level = 0;
-            units = 1;
-            if (warp == 0) {
+            i = 0;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    tall[x] = 32 * x + lane < a.B ? work.request(32 * x + lane).blocks : 0;
-                    level = max(level, tall[x]);
-                }
-                level = __reduce_max_sync(0xffffffffu, level) - 1;
-            }
-            __syncthreads();
+            for (int x = 0; x < DEAL_REQUESTS / 32; ++x) i = max(i, 32 * x + lane < a.B ? work.request(32 * x + lane).blocks : 0);
+            i = __reduce_max_sync(0xffffffffu, i) - 1;
+            r = {};
+            b = kvh = chunk = done = units = 0;
             return;
         }
         // a worker to N blocks, more if the blocks are long, as many as there are
-        workers = min(most, max((int)min((int64_t)most, (n_blocks + N - 1) / N), all / max(1, N * W::SHARE * W::KEYS >> a.unit_shift)));
+        const int workers = min(most, max((int)min((int64_t)most, (n_blocks + N - 1) / N), all / max(1, N * W::SHARE * W::KEYS >> a.unit_shift)));
         const bool mine = worker < workers;
         const int share = mine ? (unsigned)all / (unsigned)workers : 0, more = all - share * workers, begin = worker * share + min(worker, more), length = mine ? share + (worker < more) : 0;
         auto border = [&](int k) { return k == N ? begin + length : begin + length / N * k; };
@@ -234,29 +212,29 @@ struct Line {
         i = lo;
         done = left - work.before(r, lo);
     }
-    // The next block that is dealt to this worker, by a warp: number x of all in the order of the levels, each of the blocks i = level of all
-    // requests that have so many
-    __device__ __forceinline__ bool next_dealt(const W& work, Run& run) {
-        const int lane = threadIdx.x & 31, x = round * workers + (round & 1 ? workers - 1 - me : me), each = work.a.Hk * work.a.chunks;
-        ++round;
-        while (level >= 0) {
-            unsigned have[4];
+    // The next block that is dealt to this CTA, by a warp: number x of all in the order of the levels, each of the blocks i of all requests
+    // that have so many (blocks: of every request, in shared memory)
+    __device__ __forceinline__ bool next_dealt(const W& work, Run& run, const int* blocks) {
+        const int lane = threadIdx.x & 31, x = b * gridDim.x + (b & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x), each = work.a.Hk * work.a.chunks;
+        ++b;
+        while (i >= 0) {
+            unsigned have[DEAL_REQUESTS / 32];
             int n = 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                have[k] = __ballot_sync(0xffffffffu, tall[k] > level);
+            for (int k = 0; k < DEAL_REQUESTS / 32; ++k) {
+                have[k] = __ballot_sync(0xffffffffu, blocks[32 * k + lane] > i);
                 n += __popc(have[k]);
             }
-            if (x >= before_level + n * each) {
-                before_level += n * each;
-                --level;
+            if (x >= done + n * each) {
+                done += n * each;
+                --i;
                 continue;
             }
-            int rest = x - before_level, q = rest / each;  // the q-th of them
+            int rest = x - done, q = rest / each;  // the q-th of them
             rest -= q * each;
             int request = 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < DEAL_REQUESTS / 32; ++k) {
                 const int c = __popc(have[k]);
                 if (q >= 0 && q < c) {
                     const unsigned it = __ballot_sync(0xffffffffu, (have[k] >> lane & 1) && __popc(have[k] & ((1u << lane) - 1)) == q);
@@ -270,9 +248,9 @@ struct Line {
             run.b = request;
             run.kvh = rest / work.a.chunks;
             run.chunk = rest - run.kvh * work.a.chunks;
-            run.i = level;
+            run.i = i;
             run.from = 0;
-            run.to = run.n = work.tiles(run.r, level);
+            run.to = run.n = work.tiles(run.r, i);
             return true;
         }
         return false;
@@ -283,8 +261,8 @@ struct Line {
         return j == n ? n : j < W::LEAST ? 0 : n - j < W::LEAST ? n : j;
     }
     // The next run; false: the stretch is over
-    __device__ __forceinline__ bool next(const W& work, Run& run) {
-        if (W::DEAL > 0 && dealt) return next_dealt(work, run);
+    __device__ __forceinline__ bool next(const W& work, Run& run, const int* blocks = nullptr) {
+        if (W::DEAL > 0 && dealt) return next_dealt(work, run, blocks);
         while (units > 0) {
             if (i >= r.blocks) {
                 i = 0;
@@ -311,7 +289,7 @@ struct Line {
 template <class W>
 struct Line<W>::Saved {
     Line line;
-    int tall[4][32];
+    int blocks[DEAL_REQUESTS];  // dealt: of each request
 };
 // Host: x / d is x * mul >> shift for x below 2^31.
 inline void divide_by(int d, uint32_t& mul, int& shift) {

@@ -191,8 +191,11 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     pdl_trigger();
     {
         Line<RowsWork<X, TREE>> line;
-        line.template find<C::THREADS>(RowsWork<X, TREE>{a}, sh.search, blockIdx.x, gridDim.x, 0);
-        if (warp == 0) line.save(sh.line);
+        const RowsWork<X, TREE> work{a};
+        line.template find<C::THREADS>(work, sh.search, blockIdx.x, gridDim.x, 0);
+        if (threadIdx.x == 0) sh.line.line = line;
+        if (line.dealt && threadIdx.x < line.DEAL_REQUESTS) sh.line.blocks[threadIdx.x] = threadIdx.x < a.B ? work.request(threadIdx.x).blocks : 0;
+        __syncthreads();
     }
     tc_fence_after_sync();
     constexpr uint32_t tmem = 0;  // all columns are this CTA's
@@ -261,30 +264,28 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             X* const to = const_cast<X*>(row_of<X>(a.O, b, h, row));
             const int64_t at_slot = (int64_t)slot * C::BLOCK + r;
             // Through shared memory, so that 8 lanes store 128 bytes of a row: a row to a lane is 32 lines an instruction.  fp32: in place of the
-            // warp's rows of the queries that have just gone to tensor memory, 16 lanes to a row.  What is left is the way out of the SM for 32 KB.
-            constexpr int LANES = LOW ? 16 : 8;
-            uint8_t* const stage = LOW ? sQ + quarter * 4096 : smem + Space::OFF_O + (warp - 4) * 4096;
-            const uint64_t place = !valid ? 0ull : slot >= 0 ? reinterpret_cast<uint64_t>(a.part + at_slot * 64) : reinterpret_cast<uint64_t>(to);
-            auto store = [&](int offset) {
-                __syncwarp();
-#pragma unroll 4
-                for (int i = 0; i < LANES; ++i) {
-                    const int from = (32 / LANES) * i + lane / LANES, c = lane % LANES;
-                    const uint64_t at = __shfl_sync(0xffffffffu, place, from);
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage + (c >> 3) * (TILE * 128) + from * 128 + (((c & 7) ^ (from & 7)) << 4));
-                    if (at) reinterpret_cast<uint4*>(at + offset)[c] = v;
-                }
-                __syncwarp();
-            };
-            auto put = [&](int c, uint4 v) { *reinterpret_cast<uint4*>(stage + (c >> 3) * (TILE * 128) + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) = v; };
+            // warp's rows of the queries that have just gone to tensor memory, 16 lanes to a row.
             if constexpr (LOW) {
                 if (live) {
+                    uint8_t* const stage = sQ + quarter * 4096;
 #pragma unroll
                     for (int c = 0; c < 16; ++c)
-                        put(c, make_uint4(__float_as_uint(o[4 * c] * f), __float_as_uint(o[4 * c + 1] * f), __float_as_uint(o[4 * c + 2] * f), __float_as_uint(o[4 * c + 3] * f)));
-                    store(0);
+                        *reinterpret_cast<float4*>(stage + (c >> 3) * (TILE * 128) + lane * 128 + (((c & 7) ^ (lane & 7)) << 4)) =
+                            make_float4(o[4 * c] * f, o[4 * c + 1] * f, o[4 * c + 2] * f, o[4 * c + 3] * f);
+                    __syncwarp();
+                    const uint64_t place = !valid ? 0ull : slot >= 0 ? reinterpret_cast<uint64_t>(a.part + at_slot * 64) : reinterpret_cast<uint64_t>(to);
+#pragma unroll 4
+                    for (int i = 0; i < 16; ++i) {
+                        const int from = 2 * i + (lane >> 4), c = lane & 15;
+                        const uint64_t at = __shfl_sync(0xffffffffu, place, from);
+                        const float4 v = *reinterpret_cast<const float4*>(stage + (c >> 3) * (TILE * 128) + from * 128 + (((c & 7) ^ (from & 7)) << 4));
+                        if (at) reinterpret_cast<float4*>(at)[c] = v;
+                    }
                 }
-            } else if (live && slot >= 0) {
+                fence_proxy_async_smem();
+                mbar_arrive_warp(&sh.q_empty[0], lane);
+            } else if (slot >= 0) {
+                uint4* const whole = reinterpret_cast<uint4*>(a.part + at_slot * 64);
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     uint32_t y[32];
@@ -295,11 +296,13 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                         for (int i = 0; i < 32; ++i) y[i] = 0u;
                     }
+                    if (valid) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) put(c, make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]));
-                    store(128 * half);
+                        for (int i = 0; i < 8; ++i) whole[8 * half + i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                    }
                 }
             } else if (live) {
+                uint4* const mine = reinterpret_cast<uint4*>(smem + Space::OFF_O + (warp - 4) * 4096);
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     uint32_t y[32];
@@ -308,13 +311,18 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                     for (int i = 0; i < 16; ++i) y[i] = pack<X>(__uint_as_float(y[2 * i]) * f, __uint_as_float(y[2 * i + 1]) * f);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) put(4 * half + c, make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]));
+                    for (int i = 0; i < 4; ++i) mine[lane * 8 + ((4 * half + i) ^ (lane & 7))] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
                 }
-                store(0);
-            }
-            if (LOW) {
-                fence_proxy_async_smem();
-                mbar_arrive_warp(&sh.q_empty[0], lane);
+                __syncwarp();
+                const uint64_t place = valid ? reinterpret_cast<uint64_t>(to) : 0ull;
+#pragma unroll 4
+                for (int i = 0; i < 8; ++i) {
+                    const int from = 4 * i + (lane >> 3);
+                    const uint64_t at = __shfl_sync(0xffffffffu, place, from);
+                    const uint4 v = mine[from * 8 + ((lane ^ from) & 7)];
+                    if (at) reinterpret_cast<uint4*>(at)[lane & 7] = v;
+                }
+                __syncwarp();
             }
             if (!LOW) tc_fence_before_sync();
             if (valid) {
@@ -576,7 +584,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             // ------------------------------ items, tiles of keys; tiles of values ------------------------------
             const RowsWork<X, TREE> work{a};
             Line<RowsWork<X, TREE>> line;
-            line.load(sh.line);
+            line = sh.line.line;
             bool ok = true;
             const bool v = warp != 0;
             PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
@@ -584,7 +592,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             auto publish = [&](Item& it) {
                 Run run;
                 it.tokens = 0;
-                if (!line.next(work, run)) return;
+                if (!line.next(work, run, sh.line.blocks)) return;
                 const int count = run.to - run.from;
                 it.b = run.b; it.kvh = run.kvh; it.chunk = run.chunk;
                 it.token0 = run.i * a.block_tokens;
