@@ -78,67 +78,106 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 }
 
 // ---------------------------------------------------------------------------
-// Copies of pages, of the first `rows` rows of every head in every layer, and the table's new entries.
+// Copies of pages, of the first `rows` rows of every head in every layer: a piece of a page's keys or values of a layer to 8 warps, RUN times 16
+// bytes to a thread.
 // ---------------------------------------------------------------------------
 struct Pair {
     int from, to, rows, pad;
 };
-struct CopyArgs {
+struct Copies {
     hk_pool pool;
     int64_t k_strideL, v_strideL;
-    int layers, Hk, esize, parts;
+    int layers, Hk, esize;
+    int parts;     // pieces of a page
+    int of_pair;   // and of all that belongs to it
+    int most;      // pairs, at most
+};
+template <int RUN>
+__device__ __forceinline__ void copy_piece(const Copies& a, const Pair& pair, unsigned piece, int warp, int lane) {
+    if (pair.rows == 0) return;  // there was no page to copy to
+    const unsigned part = piece % a.parts, rest = piece / a.parts;
+    const int kv = rest & 1, layer = rest >> 1, shift = a.esize == 4 ? 4 : 3, inside = lane & ((1 << shift) - 1), rows = 32 >> shift;
+    const hk_view& v = kv ? a.pool.V : a.pool.K;
+    // rows of the page in the order they lie in
+    const bool by_token = v.strideH < v.strideM;
+    const int inner = by_token ? a.Hk : pair.rows, all = a.Hk * pair.rows;
+    const int64_t s_in = by_token ? v.strideH : v.strideM, s_out = by_token ? v.strideM : v.strideH, e = a.esize;
+    const char* base = static_cast<const char*>(v.ptr) + layer * (kv ? a.v_strideL : a.k_strideL) * e + inside * 16;
+    const char* from = base + pair.from * v.strideB * e;
+    char* to = const_cast<char*>(base) + pair.to * v.strideB * e;
+    const int first = ((int)part * 8 + warp) * rows * RUN + (lane >> shift);
+    uint4 x[RUN];
+    int64_t at[RUN];
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) {
+        const int r = first + i * rows, outer = r / inner;
+        at[i] = (outer * s_out + (r - outer * inner) * s_in) * e;
+        if (r < all) x[i] = *reinterpret_cast<const uint4*>(from + at[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < RUN; ++i)
+        if (first + i * rows < all) *reinterpret_cast<uint4*>(to + at[i]) = x[i];
+}
+
+// By a kernel of their own, and the table's new entries
+constexpr int OWN_RUN = 8;
+struct CopyArgs {
+    Copies copies;
     const Pair* pairs;
     const int* n_pairs;
     const int32_t* where;  // compaction: the pages' new places
     int32_t* pages_out;
     int B;
 };
-
-template <int PIECES>
 __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
-    constexpr int ROWS = 32 / PIECES, RUN = 8;  // rows that a warp copies at once, and how often
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const hk_pool& pool = a.copies.pool;
     pdl_wait();
     pdl_trigger();
     if (a.where) {
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)a.B * a.pool.width; i += (int64_t)gridDim.x * 256) {
-            const int64_t b = i / a.pool.width;
-            const int e = a.pool.pages[b * a.pool.pages_stride + (i - b * a.pool.width)];
-            a.pages_out[i] = is_page(e, a.pool.n_pages) ? a.where[e] : -1;
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)a.B * pool.width; i += (int64_t)gridDim.x * 256) {
+            const int64_t b = i / pool.width;
+            const int e = pool.pages[b * pool.pages_stride + (i - b * pool.width)];
+            a.pages_out[i] = is_page(e, pool.n_pages) ? a.where[e] : -1;
         }
     }
-    const int64_t items = (int64_t)*a.n_pairs * a.layers * 2 * a.parts, e = a.esize;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int part = (int)(item % a.parts), kv = (int)(item / a.parts & 1), layer = (int)(item / a.parts / 2 % a.layers);
-        const Pair pair = a.pairs[item / a.parts / 2 / a.layers];
-        const hk_view& v = kv ? a.pool.V : a.pool.K;
-        // rows of the page in the order they lie in
-        const bool by_token = v.strideH < v.strideM;
-        const int inner = by_token ? a.Hk : pair.rows, all = a.Hk * pair.rows;
-        const int64_t s_in = by_token ? v.strideH : v.strideM, s_out = by_token ? v.strideM : v.strideH;
-        const char* base = static_cast<const char*>(v.ptr) + layer * (kv ? a.v_strideL : a.k_strideL) * e + lane % PIECES * 16;
-        const char* from = base + pair.from * v.strideB * e;
-        char* to = const_cast<char*>(base) + pair.to * v.strideB * e;
-        const int first = (part * 8 + warp) * ROWS * RUN + lane / PIECES;
-        uint4 x[RUN];
-        int64_t at[RUN];
-#pragma unroll
-        for (int i = 0; i < RUN; ++i) {
-            const int r = first + i * ROWS, outer = r / inner;
-            at[i] = (outer * s_out + (r - outer * inner) * s_in) * e;
-            if (r < all) x[i] = *reinterpret_cast<const uint4*>(from + at[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < RUN; ++i)
-            if (first + i * ROWS < all) *reinterpret_cast<uint4*>(to + at[i]) = x[i];
-    }
+    const unsigned of_pair = a.copies.of_pair, items = *a.n_pairs * of_pair;
+    for (unsigned item = blockIdx.x; item < items; item += gridDim.x)
+        copy_piece<OWN_RUN>(a.copies, a.pairs[item / of_pair], item % of_pair, threadIdx.x >> 5, threadIdx.x & 31);
 }
-int parts_of(int Hk, int page, int esize) { return cdiv((int64_t)Hk * page, 8 * (esize == 4 ? 2 : 4) * 8); }
 
 // ---------------------------------------------------------------------------
-// Tables: one CTA, since every step needs all of the one before.
+// Tables.  Every step needs all of the one before, so one CTA takes them, with what the steps hand on in shared memory where it fits: a
+// step then waits for the entries it reads, not for what the last one wrote.  Where few pages can have to be copied, every CTA of a grid works the
+// tables out and copies its share: no second kernel, and nobody waits for another (64 requests of 64 pages, a call: 7.1 us, 9.5 with
+// two kernels; 512 of 256: 58 us, most of it in the steps over the entries).
 // ---------------------------------------------------------------------------
 constexpr int THREADS = 1024;
+constexpr size_t ROOM = 220 << 10;  // of the 227 KiB that a CTA may have
+constexpr int RUN = 4;              // 64 registers to a thread
+
+// pairs(k) of n, by all CTAs
+template <class F>
+__device__ __forceinline__ void copy_all(const Copies& a, int n, F pairs) {
+    const unsigned of_pair = a.of_pair, items = n * of_pair;
+    for (unsigned item = blockIdx.x + gridDim.x * (threadIdx.x >> 8); item < items; item += gridDim.x * (THREADS / 256))
+        copy_piece<RUN>(a, pairs(item / of_pair), item % of_pair, threadIdx.x >> 5 & 7, threadIdx.x & 31);
+}
+
+// A thread's share of n, in a row: an odd number, so that the threads of a warp meet different banks of shared memory
+__device__ __forceinline__ int share(int n) { return (n + THREADS - 1) / THREADS | 1; }
+// f(x, at(x)) for x < n by all threads, four of each thread's at a time, so that their loads are under way together
+template <class At, class F>
+__device__ __forceinline__ void for_all(int n, At at, F f) {
+    for (int x0 = threadIdx.x; x0 < n; x0 += 4 * THREADS) {
+        int e[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (x0 + u * THREADS < n) e[u] = at(x0 + u * THREADS);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (x0 + u * THREADS < n) f(x0 + u * THREADS, e[u]);
+    }
+}
 
 // Sum of x over the threads in front of this one, and of all
 struct Sums {
@@ -167,155 +206,245 @@ __device__ __forceinline__ int block_scan(Sums& sh, int x, int& total) {
 
 struct Request {  // of the new batch
     int source;   // row of the old table, -1: none
+    int len;
     int kept;     // pages it has
     int need;     // pages up to where it has room
     int first;    // number of its first new page
+    int copy;     // number of its copy, -1: none
 };
 struct ForkArgs {
-    hk_pool pool;
+    Copies copies;
     const int32_t *lengths, *users, *source, *room;
     int32_t *pages_out, *lengths_out, *users_out, *missing;
     int B, B_out;
     int64_t room_all;
+    uint32_t width_mul;  // x / width is x * width_mul >> width_shift for x below 2^31
+    int width_shift;
     int* owner;    // [B]: the first of the new batch that goes on with a request
     Request* request;  // [B_out]
     int* free;     // [n_pages]
     Pair* pairs;   // [B_out]
     int* n_pairs;
+    int copies_too;  // this kernel makes them
+    static size_t shared_bytes(int64_t P, int64_t B, int64_t B_out) { return B_out * (sizeof(Pair) + sizeof(Request)) + (2 * P + B) * sizeof(int); }
 };
 
+template <bool SHARED>
 __global__ void __launch_bounds__(THREADS) fork_kernel(const __grid_constant__ ForkArgs a) {
     __shared__ Sums sums;
-    __shared__ int lacking, n_pairs;
-    const int tid = threadIdx.x, M = a.pool.width, P = a.pool.n_pages;
+    __shared__ int lacking;
+    extern __shared__ Pair room[];
+    const hk_pool& pool = a.copies.pool;
+    const int tid = threadIdx.x, M = pool.width, P = pool.n_pages;
+    Request* const request = SHARED ? reinterpret_cast<Request*>(room + a.B_out) : a.request;
+    int* const users = SHARED ? reinterpret_cast<int*>(request + a.B_out) : a.users_out;
+    int *const free = SHARED ? users + P : a.free, *const owner = SHARED ? users + 2 * P : a.owner;
+    const bool writes = blockIdx.x == 0;
+    auto row = [&](int x) { return (int)(((uint64_t)(uint32_t)x * a.width_mul) >> a.width_shift); };
+    auto nobody = [&] {
+        for (int b = tid; b < a.B; b += THREADS) owner[b] = INT_MAX;
+    };
+    if (tid == 0) lacking = 0;
+    if (SHARED) nobody();
     pdl_wait();
     pdl_trigger();
-    if (tid == 0) lacking = n_pairs = 0;
-    for (int p = tid; p < P; p += THREADS) a.users_out[p] = a.users[p];
-    for (int b = tid; b < a.B; b += THREADS) a.owner[b] = INT_MAX;
-    __syncthreads();
-    // what the old table held is nobody's, and who goes on with a request first
-    for (int64_t i = tid; i < (int64_t)a.B * M; i += THREADS) {
-        const int64_t b = i / M;
-        const int e = a.pool.pages[b * a.pool.pages_stride + (i - b * M)];
-        if (is_page(e, P)) atomicSub(a.users_out + e, 1);
-    }
-    for (int i = tid; i < a.B_out; i += THREADS)
-        if ((unsigned)a.source[i] < (unsigned)a.B) atomicMin(a.owner + a.source[i], i);
-    __syncthreads();
-    int given = 0;
-    for (int i0 = 0; i0 < a.B_out; i0 += THREADS) {
-        const int i = i0 + tid;
-        Request r = {-1, 0, 0, 0};
-        int len = 0;
+    if (!SHARED) nobody();  // the call before may still have used the workspace
+    // a thread's first request is on its way while the tables are read
+    struct Wish {
+        int source, len;
+        int64_t room;
+    };
+    auto wish = [&](int i) {
+        Wish w = {-1, 0, 0};
         if (i < a.B_out) {
             const int s = a.source[i];
+            w.room = a.room ? (int64_t)max(a.room[i], 0) : a.room_all;
             if ((unsigned)s < (unsigned)a.B) {
-                r.source = s;
-                len = (int)min((int64_t)max(a.lengths[s], 0), (int64_t)M * a.pool.page);
-                r.kept = len / a.pool.page + (len % a.pool.page && a.owner[s] == i);
+                w.source = s;
+                w.len = (int)min((int64_t)max(a.lengths[s], 0), (int64_t)M * pool.page);
             }
-            const int64_t need = (len + (a.room ? (int64_t)max(a.room[i], 0) : a.room_all) + a.pool.page - 1) / a.pool.page;
+        }
+        return w;
+    };
+    const Wish first = wish(tid);
+    for_all(P, [&](int p) { return a.users[p]; }, [&](int p, int n) { users[p] = n; });
+    __syncthreads();
+    // what the old table held is nobody's, and who goes on with a request first
+    for_all(a.B * M, [&](int x) { const int b = row(x); return pool.pages[b * pool.pages_stride + (x - b * M)]; },
+            [&](int, int e) { if (is_page(e, P)) atomicSub(users + e, 1); });
+    for (int i = tid; i < a.B_out; i += THREADS) {
+        const int s = i == tid ? first.source : a.source[i];
+        if ((unsigned)s < (unsigned)a.B) atomicMin(owner + s, i);
+    }
+    __syncthreads();
+    int given = 0, n_pairs = 0;
+    for (int i0 = 0; i0 < a.B_out; i0 += THREADS) {
+        const int i = i0 + tid;
+        const Wish w = i0 == 0 ? first : wish(i);
+        Request r = {w.source, w.len, 0, 0, 0, -1};
+        bool copy = false;
+        if (i < a.B_out) {
+            const bool begun = w.len % pool.page != 0;
+            if (w.source >= 0) {
+                const bool owns = owner[w.source] == i;
+                r.kept = w.len / pool.page + (begun && owns);
+                // of a begun page of which another has the original
+                copy = begun && !owns && is_page(pool.pages[w.source * pool.pages_stride + w.len / pool.page], P);
+            }
+            const int64_t need = (w.len + w.room + pool.page - 1) / pool.page;
             r.need = (int)max((int64_t)r.kept, min(need, (int64_t)M));
             if (need > M) atomicAdd(&lacking, (int)min(need - M, (int64_t)1 << 20));
         }
-        int total;
+        int total, copies;
         r.first = given + block_scan(sums, r.need - r.kept, total);
         given += total;
+        const int number = n_pairs + block_scan(sums, copy, copies);
+        n_pairs += copies;
+        if (copy) r.copy = number;
         if (i < a.B_out) {
-            a.lengths_out[i] = len;
-            a.request[i] = r;
+            if (writes) a.lengths_out[i] = w.len;
+            request[i] = r;
         }
     }
     __syncthreads();
     // pages that are kept
-    for (int64_t k = tid; k < (int64_t)a.B_out * M; k += THREADS) {
-        const int i = (int)(k / M), j = (int)(k - (int64_t)i * M);
-        const Request r = a.request[i];
-        int e = -1;
-        if (j < r.kept) {
-            e = a.pool.pages[r.source * a.pool.pages_stride + j];
-            if (is_page(e, P)) atomicAdd(a.users_out + e, 1);
-            else e = -1;
-        }
-        a.pages_out[k] = e;
-    }
+    for_all(a.B_out * M,
+            [&](int x) {
+                const int i = row(x), j = x - i * M;
+                const Request r = request[i];
+                return j < r.kept ? pool.pages[r.source * pool.pages_stride + j] : -1;
+            },
+            [&](int x, int e) {
+                if (is_page(e, P)) atomicAdd(users + e, 1);
+                else e = -1;
+                if (writes) a.pages_out[x] = e;
+            });
     __syncthreads();
     // the free ones in their order
-    const int each = (P + THREADS - 1) / THREADS, p0 = min(P, tid * each), p1 = min(P, p0 + each);
+    const int each = share(P), p0 = min(P, tid * each), p1 = min(P, p0 + each);
     int n = 0, n_free;
-    for (int p = p0; p < p1; ++p) n += a.users_out[p] == 0;
+    for (int p = p0; p < p1; ++p) n += users[p] == 0;
     n = block_scan(sums, n, n_free);
     for (int p = p0; p < p1; ++p)
-        if (a.users_out[p] == 0) a.free[n++] = p;
+        if (users[p] == 0) free[n++] = p;
     __syncthreads();
-    for (int64_t k = tid; k < (int64_t)a.B_out * M; k += THREADS) {
-        const int i = (int)(k / M), j = (int)(k - (int64_t)i * M);
-        const Request r = a.request[i];
-        if (j < r.kept || j >= r.need) continue;
-        const int f = r.first + j - r.kept, page = f < n_free ? a.free[f] : -1;
-        a.pages_out[k] = page;
-        if (page >= 0) a.users_out[page] = 1;
-        const int len = a.lengths_out[i], rows = len % a.pool.page;
-        if (page >= 0 && j == len / a.pool.page && rows) {  // a begun page of which another has the original
-            const int from = a.pool.pages[r.source * a.pool.pages_stride + j];
-            if (is_page(from, P)) a.pairs[atomicAdd(&n_pairs, 1)] = {from, page, rows, 0};
+    Pair* const pairs = SHARED && a.copies_too ? room : a.pairs;
+    for (int i = tid / 32; i < a.B_out; i += THREADS / 32) {  // a warp to a request
+        const Request r = request[i];
+        const int begun = r.copy >= 0 ? r.len / pool.page : -1;
+        for (int j = r.kept + tid % 32; j < r.need; j += 32) {
+            const int f = r.first + j - r.kept, page = f < n_free ? free[f] : -1;
+            if (page >= 0) users[page] = 1;
+            if (writes) a.pages_out[(int64_t)i * M + j] = page;
+            if (j == begun) pairs[r.copy] = {pool.pages[r.source * pool.pages_stride + j], page, page >= 0 ? r.len % pool.page : 0, 0};
         }
     }
     __syncthreads();
-    if (tid == 0) {
-        *a.missing = lacking + max(0, given - n_free);
-        *a.n_pairs = n_pairs;
+    if (writes) {
+        if (SHARED)
+            for (int p = tid; p < P; p += THREADS) a.users_out[p] = users[p];
+        if (tid == 0) {
+            *a.missing = lacking + max(0, given - n_free);
+            *a.n_pairs = n_pairs;
+        }
     }
+    if (SHARED && a.copies_too) copy_all(a.copies, n_pairs, [&](int k) { return room[k]; });
 }
 
 struct CompactArgs {
+    Copies copies;
     const int32_t* users;
-    int32_t *users_out, *where;
-    int P, page;
+    int32_t *pages_out, *users_out, *where;
+    int B;
     int* hole;    // [n_pages]
     Pair* pairs;  // [n_pages / 2 + 1]
     int* n_pairs;
+    int copies_too;  // this kernel makes them, and the table
+    static size_t shared_bytes(int64_t P) { return 4 * P * sizeof(int); }
 };
+template <bool SHARED>
 __global__ void __launch_bounds__(THREADS) compact_kernel(const __grid_constant__ CompactArgs a) {
     __shared__ Sums sums;
-    const int tid = threadIdx.x, P = a.P, each = (P + THREADS - 1) / THREADS, p0 = min(P, tid * each), p1 = min(P, p0 + each);
+    extern __shared__ Pair room[];
+    const hk_pool& pool = a.copies.pool;
+    const int tid = threadIdx.x, P = pool.n_pages, each = share(P), p0 = min(P, tid * each), p1 = min(P, p0 + each);
+    int *const mine = reinterpret_cast<int*>(room), *const hole = SHARED ? mine + P : a.hole, *const from = mine + 2 * P, *const where = SHARED ? mine + 3 * P : a.where;
+    const int* const users = SHARED ? mine : a.users;
+    const bool writes = blockIdx.x == 0;
     pdl_wait();
     pdl_trigger();
+    if (SHARED) {
+        for_all(P, [&](int p) { return a.users[p]; }, [&](int p, int n) { mine[p] = n; });
+        __syncthreads();
+    }
     int used = 0, n, holes = 0, moves = 0, n_holes, n_moves;
-    for (int p = p0; p < p1; ++p) used += a.users[p] > 0;
+    for (int p = p0; p < p1; ++p) used += users[p] > 0;
     block_scan(sums, used, n);
     for (int p = p0; p < p1; ++p) {
-        const bool u = a.users[p] > 0;
+        const bool u = users[p] > 0;
         holes += !u && p < n;
         moves += u && p >= n;
     }
     holes = block_scan(sums, holes, n_holes);
     moves = block_scan(sums, moves, n_moves);  // as many
     for (int p = p0; p < p1; ++p) {
-        const int u = a.users[p];
-        if (p < n && u <= 0) a.hole[holes++] = p;
-        if (p >= n && u > 0) a.pairs[moves++].from = p;
-        if (p >= n) a.users_out[p] = 0;
-        else if (u > 0) a.users_out[p] = u;
-        a.where[p] = u > 0 && p < n ? p : -1;
+        const int u = users[p];
+        if (p < n && u <= 0) hole[holes++] = p;
+        if (p >= n && u > 0) {
+            if (SHARED) from[moves++] = p;
+            else a.pairs[moves++].from = p;
+        }
+        if (writes && p >= n) a.users_out[p] = 0;
+        else if (writes && u > 0) a.users_out[p] = u;
+        if (p < n || u <= 0) where[p] = u > 0 ? p : -1;
     }
     __syncthreads();
     for (int k = tid; k < n_moves; k += THREADS) {
-        const int from = a.pairs[k].from, to = a.hole[k];
-        a.pairs[k] = {from, to, a.page, 0};
-        a.where[from] = to;
-        a.users_out[to] = a.users[from];
+        const int x = SHARED ? from[k] : a.pairs[k].from, to = hole[k];
+        if (!SHARED || !a.copies_too) a.pairs[k] = {x, to, pool.page, 0};
+        where[x] = to;
+        if (writes) a.users_out[to] = users[x];
     }
-    if (tid == 0) *a.n_pairs = n_moves;
+    if (writes && tid == 0) *a.n_pairs = n_moves;
+    if (!SHARED) return;
+    __syncthreads();
+    if (writes)
+        for (int p = tid; p < P; p += THREADS) a.where[p] = where[p];
+    if (!a.copies_too) return;
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + tid; i < (int64_t)a.B * pool.width; i += (int64_t)gridDim.x * THREADS) {
+        const int64_t b = i / pool.width;
+        const int e = pool.pages[b * pool.pages_stride + (i - b * pool.width)];
+        a.pages_out[i] = is_page(e, P) ? where[e] : -1;
+    }
+    copy_all(a.copies, n_moves, [&](int k) { return Pair{from[k], hole[k], pool.page, 0}; });
 }
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
-int launch_copy(const CopyArgs& a, int64_t most_pairs, cudaStream_t stream) {
-    const int64_t items = std::max<int64_t>(1, most_pairs * a.layers * 2 * a.parts);
+template <class Args>
+int launch_tables(void (*kernel)(Args), const Args& a, int ctas, size_t bytes, cudaStream_t stream) {
+    if (bytes > (40 << 10) && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ROOM) != cudaSuccess) return check_launch();
+    LaunchConfig lc((unsigned)ctas, THREADS, bytes, stream, 1, true);
+    if (cudaLaunchKernelEx(&lc.cfg, kernel, a) != cudaSuccess) return check_launch();
+    count_launch();
+    return HK_OK;
+}
+int pieces(int Hk, int page, int esize, int run) { return cdiv((int64_t)Hk * page, 8 * (esize == 4 ? 2 : 4) * run); }
+template <class Params>
+Copies copies_of(const Params* p, int most, int run) {
+    const int e = esize(p->dtype), parts = pieces(p->nh_kv, p->pool.page, e, run);
+    return {p->pool, p->k_strideL, p->v_strideL, p->layers, p->nh_kv, e, parts, p->layers * 2 * parts, most};
+}
+// CTAs of a kernel that makes the copies too; 0: a kernel of their own does, which keeps more loads under way (5.9 TB/s, not 5.5) but costs 2 us
+int copiers(const Copies& a) {
+    const int64_t rounds = cdiv((int64_t)a.most * a.of_pair, THREADS / 256), sms = sm_count();
+    return rounds > 16 * sms ? 0 : (int)std::min(rounds, sms);
+}
+
+int launch_copy(const CopyArgs& a, cudaStream_t stream) {
+    const int64_t items = (int64_t)a.copies.most * a.copies.of_pair;
     LaunchConfig lc((unsigned)std::min<int64_t>(items, (int64_t)sm_count() * 8), 256, 0, stream, 1, true);
-    if (cudaLaunchKernelEx(&lc.cfg, a.esize == 4 ? copy_pages_kernel<16> : copy_pages_kernel<8>, a) != cudaSuccess) return check_launch();
+    if (cudaLaunchKernelEx(&lc.cfg, copy_pages_kernel, a) != cudaSuccess) return check_launch();
     count_launch();
     return HK_OK;
 }
@@ -331,10 +460,17 @@ int check_layers(const hk_pool& pool, int64_t kL, int64_t vL, int layers, int nh
     }
     return HK_OK;
 }
+// pages that can be copied at once, and their pieces, which are counted in 32 bits: no memory holds as many
+int fork_pairs(const hk_fork_params* p) { return std::min(p->B_out, p->pool.n_pages); }
+int compact_pairs(const hk_compact_params* p) { return std::max(1, p->pool.n_pages / 2); }
+int check_pieces(int64_t pairs, int64_t layers, int nh_kv, int page, int dtype) {
+    return (double)pairs * layers * 2 * pieces(nh_kv, page, esize(dtype), RUN) < (double)INT_MAX ? HK_OK : HK_ERR_BAD_SHAPE;
+}
 int check_fork_sizes(const hk_fork_params* p) {
     if (!p) return HK_ERR_NULL_POINTER;
     if (p->B <= 0 || p->B_out <= 0 || p->layers <= 0 || p->layers > (1 << 20) || p->room_all < 0 || p->room_all > (1 << 30)) return HK_ERR_BAD_SHAPE;
-    return check_pool_sizes(p->pool, std::max(p->B, p->B_out), p->nh_kv, p->dtype);
+    const int rc = check_pool_sizes(p->pool, std::max(p->B, p->B_out), p->nh_kv, p->dtype);
+    return rc == HK_OK ? check_pieces(fork_pairs(p), p->layers, p->nh_kv, p->pool.page, p->dtype) : rc;
 }
 struct ForkSpace {
     size_t owner, request, free, pairs, n_pairs, bytes;
@@ -350,7 +486,8 @@ struct ForkSpace {
 int check_compact_sizes(const hk_compact_params* p) {
     if (!p) return HK_ERR_NULL_POINTER;
     if (p->B <= 0 || p->layers <= 0 || p->layers > (1 << 20)) return HK_ERR_BAD_SHAPE;
-    return check_pool_sizes(p->pool, p->B, p->nh_kv, p->dtype);
+    const int rc = check_pool_sizes(p->pool, p->B, p->nh_kv, p->dtype);
+    return rc == HK_OK ? check_pieces(compact_pairs(p), p->layers, p->nh_kv, p->pool.page, p->dtype) : rc;
 }
 struct CompactSpace {
     size_t hole, pairs, n_pairs, bytes;
@@ -421,14 +558,15 @@ int hk_cache_fork(const hk_fork_params* p, void* stream_) {
     if (!workspace_fits(p->workspace, p->workspace_bytes, at.bytes)) return HK_ERR_WORKSPACE;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     char* ws = static_cast<char*>(p->workspace);
-    const ForkArgs a{p->pool, p->lengths, p->users, p->source, p->room, p->pages_out, p->lengths_out, p->users_out, p->missing, p->B, p->B_out, p->room_all,
-                     reinterpret_cast<int*>(ws + at.owner), reinterpret_cast<Request*>(ws + at.request), reinterpret_cast<int*>(ws + at.free),
-                     reinterpret_cast<Pair*>(ws + at.pairs), reinterpret_cast<int*>(ws + at.n_pairs)};
-    LaunchConfig lc(1, THREADS, 0, stream, 1, true);
-    if (cudaLaunchKernelEx(&lc.cfg, fork_kernel, a) != cudaSuccess) return check_launch();
-    count_launch();
-    const int e = esize(p->dtype);
-    return launch_copy(CopyArgs{p->pool, p->k_strideL, p->v_strideL, p->layers, p->nh_kv, e, parts_of(p->nh_kv, p->pool.page, e), a.pairs, a.n_pairs, nullptr, nullptr, 0}, p->B_out, stream);
+    ForkArgs a{copies_of(p, fork_pairs(p), RUN), p->lengths, p->users, p->source, p->room, p->pages_out, p->lengths_out, p->users_out, p->missing, p->B, p->B_out, p->room_all, 0, 0,
+               reinterpret_cast<int*>(ws + at.owner), reinterpret_cast<Request*>(ws + at.request), reinterpret_cast<int*>(ws + at.free),
+               reinterpret_cast<Pair*>(ws + at.pairs), reinterpret_cast<int*>(ws + at.n_pairs), 0};
+    divide_by(p->pool.width, a.width_mul, a.width_shift);
+    const size_t shared = ForkArgs::shared_bytes(p->pool.n_pages, p->B, p->B_out);
+    const int ctas = shared <= ROOM ? copiers(a.copies) : 0;
+    a.copies_too = ctas > 0;
+    rc = shared <= ROOM ? launch_tables(fork_kernel<true>, a, std::max(1, ctas), shared, stream) : launch_tables(fork_kernel<false>, a, 1, 0, stream);
+    return rc != HK_OK || ctas ? rc : launch_copy(CopyArgs{copies_of(p, fork_pairs(p), OWN_RUN), a.pairs, a.n_pairs, nullptr, nullptr, 0}, stream);
 }
 
 size_t hk_cache_compact_workspace_bytes(const hk_compact_params* p) { return check_compact_sizes(p) == HK_OK ? CompactSpace(p).bytes : 0; }
@@ -443,14 +581,13 @@ int hk_cache_compact(const hk_compact_params* p, void* stream_) {
     if (!workspace_fits(p->workspace, p->workspace_bytes, at.bytes)) return HK_ERR_WORKSPACE;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     char* ws = static_cast<char*>(p->workspace);
-    const CompactArgs a{p->users, p->users_out, p->where, p->pool.n_pages, p->pool.page, reinterpret_cast<int*>(ws + at.hole), reinterpret_cast<Pair*>(ws + at.pairs),
-                        reinterpret_cast<int*>(ws + at.n_pairs)};
-    LaunchConfig lc(1, THREADS, 0, stream, 1, true);
-    if (cudaLaunchKernelEx(&lc.cfg, compact_kernel, a) != cudaSuccess) return check_launch();
-    count_launch();
-    const int e = esize(p->dtype);
-    return launch_copy(CopyArgs{p->pool, p->k_strideL, p->v_strideL, p->layers, p->nh_kv, e, parts_of(p->nh_kv, p->pool.page, e), a.pairs, a.n_pairs, p->where, p->pages_out, p->B},
-                       p->pool.n_pages / 2, stream);
+    CompactArgs a{copies_of(p, compact_pairs(p), RUN), p->users, p->pages_out, p->users_out, p->where, p->B, reinterpret_cast<int*>(ws + at.hole),
+                  reinterpret_cast<Pair*>(ws + at.pairs), reinterpret_cast<int*>(ws + at.n_pairs), 0};
+    const size_t shared = CompactArgs::shared_bytes(p->pool.n_pages);
+    const int ctas = shared <= ROOM ? copiers(a.copies) : 0;
+    a.copies_too = ctas > 0;
+    rc = shared <= ROOM ? launch_tables(compact_kernel<true>, a, std::max(1, ctas), shared, stream) : launch_tables(compact_kernel<false>, a, 1, 0, stream);
+    return rc != HK_OK || ctas ? rc : launch_copy(CopyArgs{copies_of(p, compact_pairs(p), OWN_RUN), a.pairs, a.n_pairs, p->where, p->pages_out, p->B}, stream);
 }
 
 }  // extern "C"

@@ -1,4 +1,4 @@
-// cache_pages.cuh -- what the operators over a cache of pages (cache_pages.cu, tree_attention.cu) share.
+// cache_pages.cuh -- what the operators over a cache of pages (cache_pages.cu) and the attention against it (serving_attention.cuh) share.
 #pragma once
 
 #include "operators.cuh"
@@ -17,6 +17,12 @@ __device__ __forceinline__ int sequence_of(const int32_t* starts, int B, int n, 
         lo += skip;
     }
     return lo;
+}
+
+// Host: x / d is x * mul >> shift for x below 2^31.
+inline void divide_by(int d, uint32_t& mul, int& shift) {
+    for (shift = 31; (1LL << (shift - 31)) < d;) ++shift;
+    mul = (uint32_t)(((1ULL << shift) + d - 1) / d);
 }
 
 int check_pool_sizes(const hk_pool& pool, int64_t B, int nh_kv, int dtype);

@@ -291,11 +291,6 @@ struct Line<W>::Saved {
     Line line;
     int blocks[DEAL_REQUESTS];  // dealt: of each request
 };
-// Host: x / d is x * mul >> shift for x below 2^31.
-inline void divide_by(int d, uint32_t& mul, int& shift) {
-    for (shift = 31; (1LL << (shift - 31)) < d;) ++shift;
-    mul = (uint32_t)(((1ULL << shift) + d - 1) / d);
-}
 // Host: the constants of the line; the sum of the parts of blocks that fell to several of `workers`
 void set_line(ServingArgs& a, bool tree, int keys);
 int launch_combine(const ServingArgs& a, int dtype, int workers, cudaStream_t stream);

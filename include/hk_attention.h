@@ -461,8 +461,8 @@ int hk_cache_append(const hk_append_params* p, void* stream);
  * get a page of their own with its rows copied, in every layer.  Then each request gets pages until it has room for room[i] tokens more,
  * out of those that nobody holds any longer: the lowest first, to the requests in their order.  What does not fit, because the pool is
  * empty or a row of the table at its end, is -1 in the table and counted in `missing`.
- * Pages of requests that do not go on are free at once, and may be the ones that are given.  The old table and the new one, the old
- * users and the new ones may not overlap. */
+ * Pages of requests that do not go on are free at once, and may be the ones that are given.  The tables that are written may not overlap
+ * those that are read. */
 typedef struct hk_fork_params {
     hk_pool pool;             /* of the first layer, with the old table; rows of pages are written */
     int64_t k_strideL, v_strideL; /* from layer to layer */

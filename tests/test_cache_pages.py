@@ -224,10 +224,11 @@ def test_the_next_batch(seed):
 
 
 @pytest.mark.gpu
-def test_large_tables():
-    """More requests and pages than the CTA has threads"""
+@pytest.mark.parametrize("B,P", [(2500, 30000), (1300, 20000), (700, 9000)])
+def test_large_tables(B, P):
+    """More requests and pages than the CTA has threads, and room for"""
     rng, g = random.Random(1), torch.Generator(device="cuda").manual_seed(1)
-    B, page, width, P = 2500, 16, 9, 30000
+    page, width = 16, 9
     lens = [rng.randint(0, width * page) for _ in range(B)]
     pages = table(rng, P, [cdiv(n, page) for n in lens], width)
     users = [0] * P

@@ -132,6 +132,53 @@ def test_long_prompts_and_many(lens, H, Hk, dtype, causal):
     assert hk.last_device_status() == 0
 
 
+DEALT = [  # so many blocks that they are dealt out whole (up to 128 prompts), and some just below
+    ([1] * 92, 8, 8), ([1] * 93, 8, 8), ([0, 1, 400, 65, 0, 130, 7, 33] * 16, 32, 8), ([0, 1, 400, 65, 0, 130, 7, 33] * 16 + [90], 32, 8),
+    ([300, 0, 2, 129] * 8, 64, 64), ([6000], 32, 32), ([0] * 127 + [4000], 24, 12), ([4000] + [0] * 127, 24, 12), ([700, 300], 260, 2), ([5, 900, 40] * 5, 300, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,H,Hk", DEALT, ids=lambda x: f"{len(x)}x{max(x)}" if isinstance(x, list) else None)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_blocks(lens, H, Hk, dtype, causal):
+    x = make_prompts(len(lens), lens, H, Hk, dtype)
+    got = hk.prompt_attention(*x, SCALE, causal)
+    check_prompts(got, prompts(*x, causal), dtype, slice(None))
+    again = hk.prompt_attention(*x, SCALE, causal)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_graph_for_few_blocks_and_many(dtype):
+    """Where the work is cut changes with what `starts` holds when the graph runs."""
+    N, H, Hk = 3000, 32, 8
+    q, k, v, _ = make_prompts(7, [N], H, Hk, dtype)
+    starts = ints([0] * 65)
+    out, lse = torch.empty(N, H, 64, device="cuda", dtype=TYPES[dtype]), torch.empty(H, N, device="cuda")
+    workspace = torch.empty(hk.prompt_workspace_bytes(q, k, starts), dtype=torch.uint8, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        hk.prompt_attention(q, k, v, starts, SCALE, workspace=workspace, out=out, lse=lse)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        hk.prompt_attention(q, k, v, starts, SCALE, workspace=workspace, out=out, lse=lse)
+    for lens in ([N] + [0] * 63, [40] * 64, [0] * 63 + [64], [2] * 64, [0] * 64, [N - 640] + [0, 20] * 31 + [20]):
+        edges = [0]
+        for n in lens:
+            edges.append(edges[-1] + n)
+        starts.copy_(ints(edges))
+        out.fill_(5.0), lse.fill_(5.0)
+        graph.replay()
+        n = edges[-1]
+        check_prompts((out, lse), prompts(q, k, v, starts, True), dtype, slice(0, n))
+        assert bool((out[n:] == 5.0).all()) and bool((lse[:, n:] == 5.0).all())
+    assert hk.last_device_status() == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lens", [[3, 0, 200, 17], [300, 129, 1], [0, 0]])
@@ -529,6 +576,38 @@ def test_given_tensors_and_streams(dtype):
         got = (hk.prompt_attention(*x, SCALE, stream=stream), hk.tree_attention(*y, stream=stream))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_two_threads_on_streams_of_their_own(dtype):
+    from threading import Thread
+
+    lens = [900, 3, 0, 260, 77]
+    p = make_prompts(1, lens, 8, 2, dtype)
+    t = {T: make_tree(T, [700, 0, 65, 128], T, 8, 2, 16, dtype) for T in (1, 12)}
+    call = [lambda: hk.prompt_attention(*p, SCALE)] + [lambda T=T: hk.tree_attention(*t[T]) for T in t]
+    want = [f() for f in call]
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(order):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got = [(i, call[i]()) for _ in range(20) for i in order]
+                torch.cuda.current_stream().synchronize()
+            for i, g in got:
+                assert all(torch.equal(a, b) for a, b in zip(g, want[i])), i
+        except BaseException as e:  # said by the test, not lost with the thread
+            failed.append(e)
+
+    threads = [Thread(target=run, args=(o,)) for o in ((0, 1, 2), (2, 0, 1))]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert not failed, failed
+    assert hk.last_device_status() == 0
 
 
 @pytest.mark.gpu
