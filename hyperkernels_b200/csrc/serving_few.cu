@@ -22,12 +22,12 @@ using FewWork = Work<KEYS, 2, 4, 3 * KEYS, true>;
 struct Segment {  // a run as the products need it
     int b, kvh, row0, rows, from, to, old, len, slot;
 };
-template <class Rows>
+template <class Rows, int SIDE>
 struct FewShared {
     uint8_t ring[WARPS][Rows::STAGES][4096];  // a batch's keys and values
     Segment segments[WARPS][8];               // as many as can be on their way, and more
     uint64_t full[WARPS][Rows::STAGES];
-    LineSearch<WARPS> search;
+    LineSearch<WARPS / SIDE> search;
     PartRecord records[WARPS];
     Abort abort;
 };
@@ -174,7 +174,9 @@ __device__ __forceinline__ void join_warps(const ServingArgs& a, const PartRecor
     if (threadIdx.x == 0) a.parts[blockIdx.x] = mine;
 }
 
-template <class Rows>
+// SIDE key heads side by side: 1, the warps have a stretch each, or 4, a head each of the CTA's stretch (a.Hk and a.group are then of four
+// heads taken for one).
+template <class Rows, int SIDE>
 __global__ void __launch_bounds__(WARPS * 32, Rows::CTAS)
 tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
                 const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ ServingArgs a) {
@@ -182,8 +184,8 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     typedef FewWork<Rows::KEYS> W;
     constexpr int KEYS = Rows::KEYS, STAGES = Rows::STAGES, MINE = Rows::ROWS < 16 ? Rows::ROWS : 2;  // rows that a lane works on
     extern __shared__ __align__(1024) uint8_t few_smem[];
-    FewShared<Rows>& sh = *reinterpret_cast<FewShared<Rows>*>(few_smem);
-    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, me = blockIdx.x * WARPS + warp;
+    FewShared<Rows, SIDE>& sh = *reinterpret_cast<FewShared<Rows, SIDE>*>(few_smem);
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, me = SIDE == 1 ? blockIdx.x * WARPS + warp : blockIdx.x, group = a.group / SIDE;
     if (lane < (warp == 0 ? 4 : 0)) tma_prefetch_desc(lane == 0 ? &map_kp : lane == 1 ? &map_vp : lane == 2 ? &map_k : &map_v);
     if (lane == 0) {
         for (int s = 0; s < STAGES; ++s) mbar_init(&sh.full[warp][s], 1);
@@ -194,7 +196,7 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     pdl_trigger();
     const W work{a};
     Line<W> line;
-    line.template find<WARPS * 32>(work, sh.search, blockIdx.x, gridDim.x, warp);
+    line.template find<WARPS * 32>(work, sh.search, blockIdx.x, gridDim.x, SIDE == 1 ? warp : 0);
     WaitNote wc{&sh.abort};
     PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
 
@@ -209,14 +211,15 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             Run run;
             more = line.next(work, run);
             if (more) {
-                put = {run.b, run.kvh, run.i * a.block_tokens, min(a.block_tokens, run.r.tokens - run.i * a.block_tokens), run.from, run.to, run.n - a.new_tiles, run.r.len, run.slot(me)};
+                const int rows = min(a.block_tokens, run.r.tokens - run.i * a.block_tokens);
+                put = {run.b, SIDE == 1 ? run.kvh : run.kvh * SIDE + warp, run.i * a.block_tokens, rows / SIDE, run.from, run.to, run.n - a.new_tiles, run.r.len, run.slot(me)};
                 put_j = run.from;
                 ids_at = INT_MAX;
                 if (run.from > 0) {
                     record.head = run.to < run.n ? PART_GOES_ON : PART_LAST;
                 } else {
                     if (record.head == PART_EMPTY) record.head = PART_NONE;
-                    if (run.to < run.n) record.b = put.b, record.head0 = put.kvh, record.token0 = put.row0, record.tokens = put.rows;
+                    if (run.to < run.n) record.b = put.b, record.head0 = run.kvh, record.token0 = put.row0, record.tokens = rows;
                 }
             } else {
                 put.rows = 0;
@@ -270,7 +273,7 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             for (int k = 0; k < MINE; ++k) {
                 const int r = Rows::row(k, lane), row = get.row0 + r;
                 token_of[k] = (int)(((uint64_t)(uint32_t)row * a.group_mul) >> a.group_shift);
-                head_of[k] = get.kvh * a.group + row - token_of[k] * a.group;
+                head_of[k] = get.kvh * group + row - token_of[k] * group;
                 const bool there = r < get.rows;
                 query.load(k, there ? row_of<X>(a.Q, get.b, head_of[k], token_of[k]) : nullptr, lane, true);
                 bits[k] = there && get.to > get.old ? tree_bits(a, get.b, token_of[k]) : 0ull;
@@ -295,10 +298,11 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             for (int k = 0; k < MINE; ++k) f[k] = get.slot >= 0 ? 1.f : w.l[k] != 0.f ? 1.f / w.l[k] : 0.f;
             if (get.slot >= 0) {
                 const int64_t at = (int64_t)get.slot * a.slot_rows;
-                store_rows(w, lane, get.rows, f, [&](int k) { return a.part + (at + Rows::row(k, lane)) * 64; });
+                auto place = [&](int k) { return at + Rows::row(k, lane) + (SIDE == 1 ? 0 : token_of[k] * (a.group - group) + warp * group); };
+                store_rows(w, lane, get.rows, f, [&](int k) { return a.part + place(k) * 64; });
 #pragma unroll
                 for (int k = 0; k < MINE; ++k)
-                    if (Rows::row(k, lane) < get.rows && (Rows::ROWS < 16 ? lane == 0 : (lane & 3) == 0)) a.ml[at + Rows::row(k, lane)] = make_float2(w.m[k], w.l[k]);
+                    if (Rows::row(k, lane) < get.rows && (Rows::ROWS < 16 ? lane == 0 : (lane & 3) == 0)) a.ml[place(k)] = make_float2(w.m[k], w.l[k]);
             } else {
                 store_rows(w, lane, get.rows, f, [&](int k) { return const_cast<X*>(row_of<X>(a.O, get.b, head_of[k], token_of[k])); });
 #pragma unroll
@@ -316,7 +320,8 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     if (lane == 0) sh.records[warp] = record;
     __syncthreads();
     if (threadIdx.x == 0) report_abort(sh.abort, a.status);
-    join_warps<X, Rows::ROWS>(a, sh.records);
+    if constexpr (SIDE == 1) join_warps<X, Rows::ROWS>(a, sh.records);
+    else if (threadIdx.x == 0) a.parts[blockIdx.x] = record;
 }
 
 typedef void (*Kernel)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, ServingArgs);
@@ -325,14 +330,19 @@ struct Entry {
     size_t smem;
     int per_sm, keys, rows;
 };
-template <class Rows>
+template <class Rows, int SIDE = 1>
 Entry entry() {
-    return {tree_few_kernel<Rows>, sizeof(FewShared<Rows>), Rows::CTAS, Rows::KEYS, Rows::ROWS};
+    return {tree_few_kernel<Rows, SIDE>, sizeof(FewShared<Rows, SIDE>), Rows::CTAS, Rows::KEYS, Rows::ROWS};
 }
-Entry pick(int dtype, int rows) {
-    if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>>();
-    if (dtype == HK_F16) return entry<RowsOf16<__half>>();
+Entry pick(int dtype, int rows, int side = 1) {
+    if (dtype == HK_BF16) return side == 1 ? entry<RowsOf16<__nv_bfloat16>>() : entry<RowsOf16<__nv_bfloat16>, WARPS>();
+    if (dtype == HK_F16) return side == 1 ? entry<RowsOf16<__half>>() : entry<RowsOf16<__half>, WARPS>();
     return rows == 1 ? entry<RowsOfOne<1>>() : rows == 2 ? entry<RowsOfOne<2>>() : rows <= 4 ? entry<RowsOfOne<4>>() : entry<RowsOfOne<8>>();
+}
+// Key heads that a CTA takes side by side.  Pools that are stored token by token have them next to each other, a line of 128 bytes for each
+// head of 16-bit types, and memory gives neighbouring lines at once for less: SIDEFIG
+int heads_side_by_side(const ServingArgs& a, int dtype) {
+    return dtype != HK_F32 && a.Hk % WARPS == 0 && a.pool.K.strideH < a.pool.K.strideM && a.pool.V.strideH < a.pool.V.strideM ? WARPS : 1;
 }
 
 }  // namespace
@@ -344,7 +354,8 @@ TreeFewPlan tree_few_plan(int dtype, int rows) {
 
 int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
     a.rows = a.T * a.group;
-    const Entry e = pick(dtype, a.rows);
+    const int side = heads_side_by_side(a, dtype);
+    const Entry e = pick(dtype, a.rows, side);
     // once per device and kernel: more than 48 KB of shared memory
     static std::mutex mu;
     static Kernel known[HK_MAX_DEVICES][8];
@@ -362,24 +373,30 @@ int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
     }
     a.block_tokens = std::min(a.rows, e.rows);
     a.chunks = 1;
-    a.slot_rows = a.block_tokens;
-    a.new_tiles = cdiv(a.T, e.keys);
-    set_line(a, true, e.keys);
     divide_by(a.group, a.group_mul, a.group_shift);
-    divide_by(a.pool.page, a.page_mul, a.page_shift);
     CUtensorMap k, v, kp, vp;
     int s;
     if ((s = prefix_tile_map(&k, a.K, dtype, a.B, a.Hk, a.T, e.keys, false)) || (s = prefix_tile_map(&v, a.V, dtype, a.B, a.Hk, a.T, e.keys, false)) ||
         (s = prefix_tile_map(&kp, a.pool.K, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false, a.pool.K.strideM != HEAD_DIM)) ||
         (s = prefix_tile_map(&vp, a.pool.V, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false, a.pool.V.strideM != HEAD_DIM)))
         return s;
+    a.Hk /= side;
+    a.group *= side;
+    a.rows *= side;
+    a.block_tokens *= side;
+    a.slot_rows = a.block_tokens;
+    a.new_tiles = cdiv(a.T, e.keys);
+    set_line(a, true, e.keys);
+    divide_by(a.pool.page, a.page_mul, a.page_shift);
     const int ctas = sm_count() * e.per_sm;
     LaunchConfig lc(ctas, WARPS * 32, e.smem, stream, 1, true);
     if (cudaLaunchKernelEx(&lc.cfg, e.kernel, k, v, kp, vp, a) != cudaSuccess) return check_launch();
     count_launch();
     if (!a.parts) return HK_OK;
-    a.part += (size_t)2 * WARPS * ctas * a.slot_rows * 64;  // the CTAs' slots
-    a.ml += (size_t)2 * WARPS * ctas * a.slot_rows;
+    if (side == 1) {
+        a.part += (size_t)2 * WARPS * ctas * a.slot_rows * 64;  // the CTAs' slots
+        a.ml += (size_t)2 * WARPS * ctas * a.slot_rows;
+    }
     return launch_combine(a, dtype, ctas, stream);
 }
 
