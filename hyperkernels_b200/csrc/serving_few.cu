@@ -334,31 +334,39 @@ template <class Rows, int SIDE = 1>
 Entry entry() {
     return {tree_few_kernel<Rows, SIDE>, sizeof(FewShared<Rows, SIDE>), Rows::CTAS, Rows::KEYS, Rows::ROWS};
 }
-Entry pick(int dtype, int rows, int side = 1) {
-    if (dtype == HK_BF16) return side == 1 ? entry<RowsOf16<__nv_bfloat16>>() : entry<RowsOf16<__nv_bfloat16>, WARPS>();
-    if (dtype == HK_F16) return side == 1 ? entry<RowsOf16<__half>>() : entry<RowsOf16<__half>, WARPS>();
+Entry pick(int dtype, int rows, int side) {
+    if (side > 1) {
+        if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>, WARPS>();
+        if (dtype == HK_F16) return entry<RowsOf16<__half>, WARPS>();
+        return rows == 1 ? entry<RowsOfOne<1>, WARPS>() : rows == 2 ? entry<RowsOfOne<2>, WARPS>() : rows <= 4 ? entry<RowsOfOne<4>, WARPS>() : entry<RowsOfOne<8>, WARPS>();
+    }
+    if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>>();
+    if (dtype == HK_F16) return entry<RowsOf16<__half>>();
     return rows == 1 ? entry<RowsOfOne<1>>() : rows == 2 ? entry<RowsOfOne<2>>() : rows <= 4 ? entry<RowsOfOne<4>>() : entry<RowsOfOne<8>>();
 }
-// Key heads that a CTA takes side by side.  Pools that are stored token by token have them next to each other, a line of 128 bytes for each
-// head of 16-bit types, and memory gives neighbouring lines at once for less: SIDEFIG
-int heads_side_by_side(const ServingArgs& a, int dtype) {
-    return dtype != HK_F32 && a.Hk % WARPS == 0 && a.pool.K.strideH < a.pool.K.strideM && a.pool.V.strideH < a.pool.V.strideM ? WARPS : 1;
+// Key heads that a CTA takes side by side.  Four: its warps have nothing to add up, and where pools are stored token by token, with the heads
+// next to each other, memory is asked for neighbouring lines at once (64 requests of 4 096 tokens, 32 heads on 8, bf16: 97 us, 104 with a head
+// at a time; token by token 100 and 116; fp32, 16 requests of up to 2 047, 12 heads: 19 and 21).  But a block is then cut in four times as many
+// parts, all of which one CTA adds up: at 18 for each block the two are alike (one request of 40 000 tokens: 44 and 24).
+int heads_side_by_side(const ServingArgs& a, const Entry& e) {
+    const int64_t blocks = (int64_t)a.B * a.Hk / WARPS, tiles = (int64_t)a.pool.width * a.pool.page / e.keys;
+    return a.Hk % WARPS == 0 && std::min<int64_t>(sm_count() * e.per_sm / blocks, tiles / FewWork<1>::SHARE) <= 16 ? WARPS : 1;
 }
 
 }  // namespace
 
 TreeFewPlan tree_few_plan(int dtype, int rows) {
-    const Entry e = pick(dtype, rows);
+    const Entry e = pick(dtype, rows, 1);
     return {std::min(rows, e.rows), e.keys, 2, sm_count() * e.per_sm, WARPS + 1};
 }
 
 int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
     a.rows = a.T * a.group;
-    const int side = heads_side_by_side(a, dtype);
+    const int side = heads_side_by_side(a, pick(dtype, a.rows, 1));
     const Entry e = pick(dtype, a.rows, side);
     // once per device and kernel: more than 48 KB of shared memory
     static std::mutex mu;
-    static Kernel known[HK_MAX_DEVICES][8];
+    static Kernel known[HK_MAX_DEVICES][16];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
     {

@@ -405,6 +405,21 @@ def test_long_caches_and_many(lens, T, H, Hk, page, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,H,Hk", [(1, 8, 4), (3, 8, 4), (4, 16, 4), (8, 8, 8), (2, 24, 12), (16, 4, 4), (5, 12, 4), (1, 64, 4)])
+@pytest.mark.parametrize("lens,page", [(list(range(0, 2000, 61)), 16), ([700, 0, 33], 64), ([300] * 50, 48), ([6000, 5], 32)], ids=lambda x: f"{len(x)}x{max(x)}" if isinstance(x, list) else None)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["hpd", "phd"])
+def test_key_heads_in_fours(T, H, Hk, lens, page, dtype, layout):
+    """Where four key heads are taken side by side, and where there are too few of them for that."""
+    x = make_tree(len(lens) + T, lens, T, H, Hk, page, dtype, layout)
+    got = hk.tree_attention(*x)
+    check(got, trees(*x), dtype)
+    again = hk.tree_attention(*x)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T,G", [(1, 1), (1, 4), (3, 1), (9, 2), (40, 4)])
 @pytest.mark.parametrize("junk", [math.nan, math.inf, 60000.0])
