@@ -119,6 +119,22 @@ __device__ __forceinline__ void copy_piece(const Copies& a, const Pair& pair, un
         if (first + i * rows < all) *reinterpret_cast<uint4*>(to + at[i]) = x[i];
 }
 
+// Pieces first, first + step, .. of those of pairs(k), k < n, of which there may be more than 32 bits count
+template <int RUN, class F>
+__device__ __forceinline__ void copy_all(const Copies& a, unsigned first, unsigned step, int n, F pairs) {
+    const unsigned of_pair = a.of_pair, pairs_on = step / of_pair, on = step % of_pair;
+    unsigned k = first / of_pair, piece = first % of_pair;
+    while (k < (unsigned)n) {
+        copy_piece<RUN>(a, pairs(k), piece, threadIdx.x >> 5 & 7, threadIdx.x & 31);
+        k += pairs_on;
+        piece += on;
+        if (piece >= of_pair) {
+            piece -= of_pair;
+            ++k;
+        }
+    }
+}
+
 // By a kernel of their own, and the table's new entries
 constexpr int OWN_RUN = 8;
 struct CopyArgs {
@@ -129,7 +145,7 @@ struct CopyArgs {
     int32_t* pages_out;
     int B;
 };
-__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+__global__ void __launch_bounds__(256, 3) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
     const hk_pool& pool = a.copies.pool;
     pdl_wait();
     pdl_trigger();
@@ -140,9 +156,7 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
             a.pages_out[i] = is_page(e, pool.n_pages) ? a.where[e] : -1;
         }
     }
-    const unsigned of_pair = a.copies.of_pair, items = *a.n_pairs * of_pair;
-    for (unsigned item = blockIdx.x; item < items; item += gridDim.x)
-        copy_piece<OWN_RUN>(a.copies, a.pairs[item / of_pair], item % of_pair, threadIdx.x >> 5, threadIdx.x & 31);
+    copy_all<OWN_RUN>(a.copies, blockIdx.x, gridDim.x, *a.n_pairs, [&](int k) { return a.pairs[k]; });
 }
 
 // ---------------------------------------------------------------------------
@@ -154,14 +168,6 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
 constexpr int THREADS = 1024;
 constexpr size_t ROOM = 220 << 10;  // of the 227 KiB that a CTA may have
 constexpr int RUN = 4;              // 64 registers to a thread
-
-// pairs(k) of n, by all CTAs
-template <class F>
-__device__ __forceinline__ void copy_all(const Copies& a, int n, F pairs) {
-    const unsigned of_pair = a.of_pair, items = n * of_pair;
-    for (unsigned item = blockIdx.x + gridDim.x * (threadIdx.x >> 8); item < items; item += gridDim.x * (THREADS / 256))
-        copy_piece<RUN>(a, pairs(item / of_pair), item % of_pair, threadIdx.x >> 5 & 7, threadIdx.x & 31);
-}
 
 // A thread's share of n, in a row: an odd number, so that the threads of a warp meet different banks of shared memory
 __device__ __forceinline__ int share(int n) { return (n + THREADS - 1) / THREADS | 1; }
@@ -232,7 +238,7 @@ struct ForkArgs {
 template <bool SHARED>
 __global__ void __launch_bounds__(THREADS) fork_kernel(const __grid_constant__ ForkArgs a) {
     __shared__ Sums sums;
-    __shared__ int lacking;
+    __shared__ unsigned long long lacking;
     extern __shared__ Pair room[];
     const hk_pool& pool = a.copies.pool;
     const int tid = threadIdx.x, M = pool.width, P = pool.n_pages;
@@ -293,7 +299,7 @@ __global__ void __launch_bounds__(THREADS) fork_kernel(const __grid_constant__ F
             }
             const int64_t need = (w.len + w.room + pool.page - 1) / pool.page;
             r.need = (int)max((int64_t)r.kept, min(need, (int64_t)M));
-            if (need > M) atomicAdd(&lacking, (int)min(need - M, (int64_t)1 << 20));
+            if (need > M) atomicAdd(&lacking, (unsigned long long)(need - M));
         }
         int total, copies;
         r.first = given + block_scan(sums, r.need - r.kept, total);
@@ -344,11 +350,11 @@ __global__ void __launch_bounds__(THREADS) fork_kernel(const __grid_constant__ F
         if (SHARED)
             for (int p = tid; p < P; p += THREADS) a.users_out[p] = users[p];
         if (tid == 0) {
-            *a.missing = lacking + max(0, given - n_free);
+            *a.missing = (int)min(lacking + max(0, given - n_free), (unsigned long long)INT_MAX);
             *a.n_pairs = n_pairs;
         }
     }
-    if (SHARED && a.copies_too) copy_all(a.copies, n_pairs, [&](int k) { return room[k]; });
+    if (SHARED && a.copies_too) copy_all<RUN>(a.copies, blockIdx.x + gridDim.x * (tid >> 8), gridDim.x * (THREADS / 256), n_pairs, [&](int k) { return room[k]; });
 }
 
 struct CompactArgs {
@@ -416,7 +422,7 @@ __global__ void __launch_bounds__(THREADS) compact_kernel(const __grid_constant_
         const int e = pool.pages[b * pool.pages_stride + (i - b * pool.width)];
         a.pages_out[i] = is_page(e, P) ? where[e] : -1;
     }
-    copy_all(a.copies, n_moves, [&](int k) { return Pair{from[k], hole[k], pool.page, 0}; });
+    copy_all<RUN>(a.copies, blockIdx.x + gridDim.x * (tid >> 8), gridDim.x * (THREADS / 256), n_moves, [&](int k) { return Pair{from[k], hole[k], pool.page, 0}; });
 }
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
@@ -460,17 +466,16 @@ int check_layers(const hk_pool& pool, int64_t kL, int64_t vL, int layers, int nh
     }
     return HK_OK;
 }
-// pages that can be copied at once, and their pieces, which are counted in 32 bits: no memory holds as many
+// pages that can be copied at once
 int fork_pairs(const hk_fork_params* p) { return std::min(p->B_out, p->pool.n_pages); }
 int compact_pairs(const hk_compact_params* p) { return std::max(1, p->pool.n_pages / 2); }
-int check_pieces(int64_t pairs, int64_t layers, int nh_kv, int page, int dtype) {
-    return (double)pairs * layers * 2 * pieces(nh_kv, page, esize(dtype), RUN) < (double)INT_MAX ? HK_OK : HK_ERR_BAD_SHAPE;
-}
+// what belongs to a page is counted in 32 bits: no memory holds as much
+int check_pieces(int64_t layers, int nh_kv, int page, int dtype) { return layers * 2 * pieces(nh_kv, page, esize(dtype), RUN) <= INT_MAX ? HK_OK : HK_ERR_BAD_SHAPE; }
 int check_fork_sizes(const hk_fork_params* p) {
     if (!p) return HK_ERR_NULL_POINTER;
     if (p->B <= 0 || p->B_out <= 0 || p->layers <= 0 || p->layers > (1 << 20) || p->room_all < 0 || p->room_all > (1 << 30)) return HK_ERR_BAD_SHAPE;
     const int rc = check_pool_sizes(p->pool, std::max(p->B, p->B_out), p->nh_kv, p->dtype);
-    return rc == HK_OK ? check_pieces(fork_pairs(p), p->layers, p->nh_kv, p->pool.page, p->dtype) : rc;
+    return rc == HK_OK ? check_pieces(p->layers, p->nh_kv, p->pool.page, p->dtype) : rc;
 }
 struct ForkSpace {
     size_t owner, request, free, pairs, n_pairs, bytes;
@@ -487,7 +492,7 @@ int check_compact_sizes(const hk_compact_params* p) {
     if (!p) return HK_ERR_NULL_POINTER;
     if (p->B <= 0 || p->layers <= 0 || p->layers > (1 << 20)) return HK_ERR_BAD_SHAPE;
     const int rc = check_pool_sizes(p->pool, p->B, p->nh_kv, p->dtype);
-    return rc == HK_OK ? check_pieces(compact_pairs(p), p->layers, p->nh_kv, p->pool.page, p->dtype) : rc;
+    return rc == HK_OK ? check_pieces(p->layers, p->nh_kv, p->pool.page, p->dtype) : rc;
 }
 struct CompactSpace {
     size_t hole, pairs, n_pairs, bytes;

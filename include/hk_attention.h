@@ -398,7 +398,7 @@ typedef struct hk_pool {
  * [0, N] and have to ascend.  Row i sees the keys j of its sequence, with is_causal those with j <= i.  Rows in no sequence are left as
  * they are, in O and LSE.  Heads in groups of nh / nh_kv share a head of keys and values.  NaN, infinities and bits: as in
  * hk_shared_prefix_attention; a key that is_causal alone hides from a row has to have finite values, other sequences' may hold
- * anything. */
+ * anything.  O and LSE may not overlap what is read. */
 typedef struct hk_prompt_params {
     hk_view Q, K, V;  /* [1, nh or nh_kv, N, 64], `dtype`; strideB is not used */
     hk_view O;        /* the same, written */
@@ -418,7 +418,8 @@ size_t hk_prompt_workspace_bytes(const hk_prompt_params* p);
 /* Attention of T <= 64 new tokens of each request.  Token i of request b sees the lengths[b] keys that lie in its pages (taken into [0,
  * width * page]) and of the new tokens those j with bit j of tree[b * tree_stride + i]: its ancestors in a tree of drafts, and itself.
  * Without `tree` it sees j <= i.  T = 1 is plain decoding.  A row that sees nothing gives O = 0, LSE = -inf.  Rows of pages behind a
- * request's last key may hold anything; a new token that the tree hides from a row takes part with weight 0, so its values have to be finite. */
+ * request's last key may hold anything; a new token that the tree hides from a row takes part with weight 0, so its values have to be finite.
+ * O and LSE may not overlap what is read. */
 #define HK_TREE_TOKENS 64
 typedef struct hk_tree_params {
     hk_view Q;        /* [B, nh, T, 64], `dtype` */
@@ -460,7 +461,7 @@ int hk_cache_append(const hk_append_params* p, void* stream);
  * that are full of a request's tokens are shared by all that go on with it.  One that is begun stays with the first of these; the others
  * get a page of their own with its rows copied, in every layer.  Then each request gets pages until it has room for room[i] tokens more,
  * out of those that nobody holds any longer: the lowest first, to the requests in their order.  What does not fit, because the pool is
- * empty or a row of the table at its end, is -1 in the table and counted in `missing`.
+ * empty or a row of the table at its end, is -1 in the table and counted in `missing` (up to 2^31 - 1).
  * Pages of requests that do not go on are free at once, and may be the ones that are given.  The tables that are written may not overlap
  * those that are read. */
 typedef struct hk_fork_params {

@@ -248,6 +248,15 @@ def test_large_tables(B, P):
     assert torch.equal(ka, wk) and torch.equal(va, wv)
 
 
+@pytest.mark.gpu
+def test_more_missing_than_there_are_numbers():
+    g = torch.Generator(device="cuda").manual_seed(0)
+    (_, kp), (_, vp) = pool(g, None, 4, 1, 16, "f32", "hpd"), pool(g, None, 4, 1, 16, "f32", "hpd")
+    for B, room, missing in ((1, 2 ** 31 - 1, 2 ** 27 - 4), (1, 2 ** 30, 2 ** 26 - 4), (3, 2 ** 31 - 1, 3 * 2 ** 27 - 4), (3000, 2 ** 31 - 1, 2 ** 31 - 1), (3000, 0, 0)):
+        got = hk.cache_fork(kp, vp, ints([[-1] * 4] * B), ints([0] * B), ints([0] * 4), ints([-1] * B), ints([room] * B))
+        assert got[3].tolist() == [missing] and got[0].flatten().tolist() == ([0, 1, 2, 3] if missing else []) + [-1] * (4 * B - 4 * (missing > 0))
+
+
 # ---- compacting ------------------------------------------------------------------------------------------------------------------------
 def compact_model(kp, vp, pages, users):
     P = kp.shape[1]
