@@ -1,5 +1,5 @@
 // few_rows.cuh -- a warp's rows against batches of keys in shared memory (shared_prefix_few.cu, serving_few.cu): up to 16 rows by matrix
-// instructions, one or two of fp32 lane by lane.
+// instructions, up to four of fp32 lane by lane.
 #pragma once
 
 #include <type_traits>
@@ -281,7 +281,7 @@ struct RowsOf16 {
 template <int N>
 struct RowsOfOne {
     typedef float X;
-    static constexpr int ROWS = N, KEYS = 8, PARTS = 2, STAGES = N <= 4 ? 3 : 5, CTAS = N <= 4 ? 4 : 2;
+    static constexpr int ROWS = N, KEYS = 8, PARTS = 2, STAGES = 3, CTAS = 4;
     // a lane's piece of key i of its half-warp
     static __device__ __forceinline__ float4 piece(const uint8_t* at, int i, int lane) {
         const int key = 2 * i + (lane >> 4);

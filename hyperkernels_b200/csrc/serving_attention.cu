@@ -151,7 +151,7 @@ Parts parts_of(const hk_prompt_params* p) {
     const RowsPlan plan = rows_plan(p->dtype);
     return {sm_count(), 1, plan.rows, (p->N + plan.keys - 1) / plan.keys >= 2 * plan.least};
 }
-bool few_rows(const hk_tree_params* p) { return p->T * (p->nh / p->nh_kv) <= (p->dtype == HK_F32 ? 8 : 16); }
+bool few_rows(const hk_tree_params* p) { return p->T * (p->nh / p->nh_kv) <= 16; }
 Parts parts_of(const hk_tree_params* p) {
     const int64_t keys = (int64_t)p->pool.width * p->pool.page;
     if (few_rows(p)) {

@@ -5,8 +5,9 @@
 // and tables are read where the batches are asked for, 32 entries of a table at a time, so no product waits for them.  What a block of rows has in
 // several warps goes to slots; a CTA adds up what its own warps left, and what is left of blocks that fell to several CTAs a second kernel.
 // Where key heads come in fours the warps take one each instead, over the whole stretch of the CTA (heads_side_by_side).
-//   What bounds it is memory: 64 requests of 4 096 tokens, 32 heads on 8, bf16, 97 us or 5.6 TB/s, of which some 9 are the launch, the search for
-// the stretches, the first loads and the sum of the parts.  More than 8 rows of fp32 to a key head are bound by the lanes' arithmetic.
+//   What bounds it is memory: 64 requests of 4 096 tokens, 32 heads on 8, bf16, 94 us or 5.7 TB/s, of which some 9 are the launch, the search for
+// the stretches, the first loads and the sum of the parts.  More than two rows of fp32 are bound by arithmetic: 16 requests of up to 2 047 tokens,
+// 12 heads, 1 / 2 / 4 (lane by lane) / 8 / 16 rows (three TF32 products of mma.sync): 18 / 22 / 30 / 33 / 35 us; the kernel of many rows takes 54 to 61.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -22,14 +23,22 @@ constexpr int WARPS = 4;
 template <int KEYS>
 using FewWork = Work<KEYS, 2, 4, 3 * KEYS, true>;
 
+// CTAs that an SM holds, by what their threads need of its registers (16 rows by matrix instructions 160, fp32 233), and batches of a warp's
+// ring, which share its memory.  With four, and registers spilled, 64 requests of up to 4 096 tokens, 32 heads on 8, bf16, took 56 us instead of
+// 53, with two as long or longer; 16 rows of fp32 in three 75 us instead of 56 (16 requests of up to 4 096, 12 heads).
+template <class Rows>
+struct Shape {
+    static constexpr int CTAS = Rows::ROWS == 16 ? (sizeof(typename Rows::X) == 4 ? 2 : 3) : Rows::ROWS > 2 ? 3 : 4, STAGES = 12 / CTAS;
+};
+
 struct Segment {  // a run as the products need it
     int b, kvh, row0, rows, from, to, old, len, slot;
 };
 template <class Rows, int SIDE>
 struct FewShared {
-    uint8_t ring[WARPS][Rows::STAGES][4096];  // a batch's keys and values
+    uint8_t ring[WARPS][Shape<Rows>::STAGES][4096];  // a batch's keys and values
     Segment segments[WARPS][8];               // as many as can be on their way, and more
-    uint64_t full[WARPS][Rows::STAGES];
+    uint64_t full[WARPS][Shape<Rows>::STAGES];
     LineSearch<WARPS / SIDE> search;
     PartRecord records[WARPS];
     Abort abort;
@@ -180,12 +189,12 @@ __device__ __forceinline__ void join_warps(const ServingArgs& a, const PartRecor
 // SIDE key heads side by side: 1, the warps have a stretch each, or 4, a head each of the CTA's stretch (a.Hk and a.group are then of four
 // heads taken for one).
 template <class Rows, int SIDE>
-__global__ void __launch_bounds__(WARPS * 32, Rows::CTAS)
+__global__ void __launch_bounds__(WARPS * 32, Shape<Rows>::CTAS)
 tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
                 const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ ServingArgs a) {
     typedef typename Rows::X X;
     typedef FewWork<Rows::KEYS> W;
-    constexpr int KEYS = Rows::KEYS, STAGES = Rows::STAGES, MINE = Rows::ROWS < 16 ? Rows::ROWS : 2;  // rows that a lane works on
+    constexpr int KEYS = Rows::KEYS, STAGES = Shape<Rows>::STAGES, MINE = Rows::ROWS < 16 ? Rows::ROWS : 2;  // rows that a lane works on
     extern __shared__ __align__(1024) uint8_t few_smem[];
     FewShared<Rows, SIDE>& sh = *reinterpret_cast<FewShared<Rows, SIDE>*>(few_smem);
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, me = SIDE == 1 ? blockIdx.x * WARPS + warp : blockIdx.x, group = a.group / SIDE;
@@ -335,22 +344,22 @@ struct Entry {
 };
 template <class Rows, int SIDE = 1>
 Entry entry() {
-    return {tree_few_kernel<Rows, SIDE>, sizeof(FewShared<Rows, SIDE>), Rows::CTAS, Rows::KEYS, Rows::ROWS};
+    return {tree_few_kernel<Rows, SIDE>, sizeof(FewShared<Rows, SIDE>), Shape<Rows>::CTAS, Rows::KEYS, Rows::ROWS};
 }
 Entry pick(int dtype, int rows, int side) {
     if (side > 1) {
         if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>, WARPS>();
         if (dtype == HK_F16) return entry<RowsOf16<__half>, WARPS>();
-        return rows == 1 ? entry<RowsOfOne<1>, WARPS>() : rows == 2 ? entry<RowsOfOne<2>, WARPS>() : rows <= 4 ? entry<RowsOfOne<4>, WARPS>() : entry<RowsOfOne<8>, WARPS>();
+        return rows == 1 ? entry<RowsOfOne<1>, WARPS>() : rows == 2 ? entry<RowsOfOne<2>, WARPS>() : rows <= 4 ? entry<RowsOfOne<4>, WARPS>() : entry<RowsOf16<float>, WARPS>();
     }
     if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>>();
     if (dtype == HK_F16) return entry<RowsOf16<__half>>();
-    return rows == 1 ? entry<RowsOfOne<1>>() : rows == 2 ? entry<RowsOfOne<2>>() : rows <= 4 ? entry<RowsOfOne<4>>() : entry<RowsOfOne<8>>();
+    return rows == 1 ? entry<RowsOfOne<1>>() : rows == 2 ? entry<RowsOfOne<2>>() : rows <= 4 ? entry<RowsOfOne<4>>() : entry<RowsOf16<float>>();
 }
 // Key heads that a CTA takes side by side.  Four: its warps have nothing to add up, and where pools are stored token by token, with the heads
-// next to each other, memory is asked for neighbouring lines at once (64 requests of 4 096 tokens, 32 heads on 8, bf16: 97 us, 104 with a head
-// at a time; token by token 100 and 116; fp32, 16 requests of up to 2 047, 12 heads: 19 and 21).  But a block is then cut in four times as many
-// parts, all of which one CTA adds up: at 18 for each block the two are alike (one request of 40 000 tokens: 44 and 24).
+// next to each other, memory is asked for neighbouring lines at once (64 requests of 4 096 tokens, 32 heads on 8, bf16: 94 us, 99 with a head
+// at a time; token by token 98 and 110; fp32, 16 requests of up to 2 047, 12 heads: 19 and 22).  But a block is then cut in four times as many
+// parts, all of which one CTA adds up: at 14 to 18 for each block the two are alike (one request of 40 000 tokens: 36 and 22).
 int heads_side_by_side(const ServingArgs& a, const Entry& e) {
     const int64_t blocks = (int64_t)a.B * a.Hk / WARPS, tiles = (int64_t)a.pool.width * a.pool.page / e.keys;
     return a.Hk % WARPS == 0 && std::min<int64_t>(sm_count() * e.per_sm / blocks, tiles / FewWork<1>::SHARE) <= 16 ? WARPS : 1;
