@@ -45,9 +45,10 @@ struct Rows {
     static constexpr int ITEMS = 8;
 };
 
-// half a tile is masked, and a block's beginning and end take as long as a tile (fp32: 3.7 us, nearly three)
-template <class X, bool TREE>
-using RowsWork = Work<Rows<X>::KEYS, Rows<X>::LEAST, 3 * Rows<X>::LEAST, Rows<X>::KEYS * (sizeof(X) == 4 ? 6 : 3) / 2, TREE, TREE ? 0 : 5>;
+// Half a tile is masked, and a block's beginning and end take as long as a tile (fp32: 3.7 us, nearly three; where both streams have the same rows a tile
+// takes half as long: 16 requests of up to 4 096 tokens, 32 drafts, 12 heads, bf16: 34 us, 37 if that is not counted).
+template <class X, bool TREE, bool SPLIT>
+using RowsWork = Work<Rows<X>::KEYS, Rows<X>::LEAST, 3 * Rows<X>::LEAST, Rows<X>::KEYS * (sizeof(X) == 4 ? 6 : SPLIT ? 8 : 3) / 2, TREE, TREE ? 0 : 5>;
 
 struct __align__(16) Item {
     int b, kvh, chunk;   // request, key head, which 128 of its query heads
@@ -59,7 +60,7 @@ struct __align__(16) Item {
     int new_tile;        // number of the tile that is the new tokens'
 };
 
-template <class X, bool TREE>
+template <class X, bool TREE, bool SPLIT>
 struct __align__(16) RowsShared {
     typedef Rows<X> C;
     uint64_t q_full[C::Q_BUFFERS], q_empty[C::Q_BUFFERS], q_ready, p_full[3];
@@ -70,7 +71,7 @@ struct __align__(16) RowsShared {
     Item items[C::ITEMS];
     uint64_t pair_full[2][4], pair_done[2][4];       // what a warp has for that of the other stream's with the same rows; it has read that of it
     LineSearch<1> search;
-    typename Line<RowsWork<X, TREE>>::Saved line;
+    typename Line<RowsWork<X, TREE, SPLIT>>::Saved line;
     int keep[2][C::SLOTS];  // rows of the tile that are values, LAST: none follows
     uint32_t tmem_base;
     Abort abort;
@@ -80,8 +81,8 @@ constexpr int LAST = -1;
 template <class X>
 struct RowsSpace {
     typedef Rows<X> C;
-    static constexpr int OFF_Q = 2 * C::SLOTS * C::KV_BYTES, OFF_O = OFF_Q + C::STREAMS * C::Q_BUFFERS * C::Q_BYTES, OFF_SH = OFF_O + (C::LOW ? 0 : C::SOFTMAX_WARPS * 4096), SMEM = OFF_SH + (int)sizeof(RowsShared<X, false>);
-    static_assert(sizeof(RowsShared<X, false>) == sizeof(RowsShared<X, true>), "");
+    static constexpr int OFF_Q = 2 * C::SLOTS * C::KV_BYTES, OFF_O = OFF_Q + C::STREAMS * C::Q_BUFFERS * C::Q_BYTES, OFF_SH = OFF_O + (C::LOW ? 0 : C::SOFTMAX_WARPS * 4096), SMEM = OFF_SH + (int)sizeof(RowsShared<X, false, false>);
+    static_assert(sizeof(RowsShared<X, false, false>) == sizeof(RowsShared<X, true, false>), "");
     static_assert(SMEM <= 232448, "exceeds the 227 KiB a CTA may opt in to");
 };
 // Tensor memory.  16-bit types: three buffers of 128 columns for scores and weights, O of two streams.  fp32: three buffers of
@@ -154,7 +155,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     constexpr int KEYS = C::KEYS, SLOTS = C::SLOTS, ITEMS = C::ITEMS;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *sKV = smem, *sQ = smem + Space::OFF_Q;
-    RowsShared<X, TREE>& sh = *reinterpret_cast<RowsShared<X, TREE>*>(smem + Space::OFF_SH);
+    RowsShared<X, TREE, SPLIT>& sh = *reinterpret_cast<RowsShared<X, TREE, SPLIT>*>(smem + Space::OFF_SH);
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     if (warp == 2 && lane < (TREE ? 5 : 3)) tma_prefetch_desc(lane == 0 ? &map_q : lane == 1 ? &map_k : lane == 2 ? &map_v : lane == 3 ? &map_kp : &map_vp);
@@ -201,8 +202,8 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     pdl_wait();
     pdl_trigger();
     {
-        Line<RowsWork<X, TREE>> line;
-        const RowsWork<X, TREE> work{a};
+        Line<RowsWork<X, TREE, SPLIT>> line;
+        const RowsWork<X, TREE, SPLIT> work{a};
         line.template find<C::THREADS>(work, sh.search, blockIdx.x, gridDim.x, 0);
         if (threadIdx.x == 0) sh.line.line = line;
         if (line.dealt && threadIdx.x < line.DEAL_REQUESTS) sh.line.blocks[threadIdx.x] = threadIdx.x < a.B ? work.request(threadIdx.x).blocks : 0;
@@ -652,8 +653,8 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         if (warp == 0 || warp == (LOW ? 10 : 3)) {
             // ------------------------------ items, tiles of keys; tiles of values ------------------------------
-            const RowsWork<X, TREE> work{a};
-            Line<RowsWork<X, TREE>> line;
+            const RowsWork<X, TREE, SPLIT> work{a};
+            Line<RowsWork<X, TREE, SPLIT>> line;
             line = sh.line.line;
             bool ok = true;
             const bool v = warp != 0;
