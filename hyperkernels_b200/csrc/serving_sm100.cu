@@ -297,7 +297,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const float f = slot >= 0 ? 1.f : l != 0.f ? rcp_approx(l) : 0.f;
             const int b = TREE ? it.b : 0, row = it.begin + it.token0 + (valid ? my_token : 0), h = it.kvh * a.group + it.chunk * TILE + my_head;
             X* const to = const_cast<X*>(row_of<X>(a.O, b, h, row));
-            const int64_t at_slot = (int64_t)slot * C::BLOCK + r;
+            const int64_t at_slot = (int64_t)slot * (SPLIT ? TILE : C::BLOCK) + r;
             // Through shared memory, so that 8 lanes store 128 bytes of a row: a row to a lane is 32 lines an instruction.  fp32: in place of the
             // warp's rows of the queries that have just gone to tensor memory, 16 lanes to a row.
             if constexpr (LOW) {
@@ -1010,7 +1010,7 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     a.block_tokens = C::STREAMS * a.stream_tokens;
     a.chunks = cdiv(a.group, TILE);
     a.new_tiles = 1;
-    a.slot_rows = C::BLOCK;
+    a.slot_rows = SPLIT ? TILE : C::BLOCK;
     set_line(a, TREE, C::KEYS);
     CUtensorMap k, v, kp, vp;
     const int B = TREE ? a.B : 1;
