@@ -41,6 +41,7 @@ struct ServingArgs {
     int box;            // rows of a page that are loaded at once
     // slots of the workspace, and who has what in them; no parts: blocks are not cut
     int slot_rows;
+    int sum_rows;       // that can be any block's
     float2* ml;         // [slots][slot_rows]
     float* part;        // the same, [64]
     PartRecord* parts;
@@ -294,7 +295,7 @@ struct Line<W>::Saved {
 };
 // Host: the constants of the line; the sum of the parts of blocks that fell to several of `workers`
 void set_line(ServingArgs& a, bool tree, int keys);
-int launch_combine(const ServingArgs& a, int dtype, int workers, cudaStream_t stream);
+int launch_combine(ServingArgs a, int dtype, int workers, cudaStream_t stream);
 
 struct RowsPlan {
     int rows;   // of a block
