@@ -177,14 +177,29 @@ int set_scale(ServingArgs& a, int dtype, float scale) {
     a.status = device_status_ptr();
     return a.status ? HK_OK : HK_ERR_CUDA;
 }
+ServingArgs sizes_of(const hk_prompt_params* p) {
+    ServingArgs a{};
+    a.B = p->B; a.Hk = p->nh_kv; a.group = p->nh / p->nh_kv; a.N = (int)p->N;
+    a.causal = p->is_causal;
+    return a;
+}
+ServingArgs sizes_of(const hk_tree_params* p) {
+    ServingArgs a{};
+    a.pool = p->pool;
+    a.B = p->B; a.Hk = p->nh_kv; a.group = p->nh / p->nh_kv; a.T = (int)p->T;
+    return a;
+}
+void put_line(const LineSum& x, int64_t* out) { out[0] = x.units; out[1] = x.narrowest; out[2] = x.lost; out[3] = x.unit_shift; }
 }  // namespace
 
 void set_line(ServingArgs& a, bool tree, int keys) {
     divide_by(a.block_tokens, a.block_mul, a.block_shift);
-    // what all requests can come to, in keys: blocks, and what each counts at most
-    const double blocks = (tree ? (double)a.B * cdiv(a.rows ? a.rows : a.T, a.block_tokens) : (double)a.N / a.block_tokens + a.B) * a.Hk * a.chunks;
-    double all = blocks * ((tree ? (double)a.pool.width * a.pool.page + a.new_tiles * keys : a.N + a.block_tokens) + 4.0 * keys);
-    for (a.unit_shift = 0; all >= 2e9; all /= 2) ++a.unit_shift;
+    // What all requests can come to: blocks, those of prompts without tokens left out; the keys that they meet, of prompts most where one has all the tokens; of
+    // each block 4 tiles beside them, and up to a unit.
+    const double heads = (double)a.Hk * a.chunks, blocks = heads * (tree ? (double)a.B * cdiv(a.rows ? a.rows : a.T, a.block_tokens) : (double)a.N / a.block_tokens + std::min(a.B, a.N));
+    const double met = tree ? blocks * ((double)a.pool.width * a.pool.page + a.new_tiles * keys) : heads * ((double)a.N * a.N / a.block_tokens + 2.0 * a.N + (double)std::min(a.B, a.N) * a.block_tokens);
+    double all = met + blocks * 4.0 * keys;
+    for (a.unit_shift = 0; all + (a.unit_shift > 0 ? blocks : 0.0) >= 2e9; all /= 2) ++a.unit_shift;
 }
 
 // Sixteen rows to a CTA, 32 of blocks of 256: those that find nothing to add up cost time too (6 prompts of 300 tokens, 32 heads on 8, bf16: 18.5 us,
@@ -217,12 +232,10 @@ int hk_prompt_attention(const hk_prompt_params* p, void* stream) {
     if (!p->LSE || !p->starts) return HK_ERR_NULL_POINTER;
     if (odd(p->LSE, 4) || odd(p->starts, 4)) return HK_ERR_MISALIGNED;
     if (p->nh > 1 && p->lse_strideH < p->N) return HK_ERR_UNSUPPORTED;  // rows on top of each other
-    ServingArgs a{};
+    ServingArgs a = sizes_of(p);
     a.Q = p->Q; a.K = p->K; a.V = p->V; a.O = p->O;
     a.LSE = p->LSE; a.lse_sH = p->lse_strideH;
     a.starts = p->starts;
-    a.B = p->B; a.Hk = p->nh_kv; a.group = p->nh / p->nh_kv; a.N = (int)p->N;
-    a.causal = p->is_causal;
     if ((rc = set_parts(a, parts_of(p), p->workspace, p->workspace_bytes)) || (rc = set_scale(a, p->dtype, p->scale))) return rc;
     return launch_prompt_rows(a, p->dtype, static_cast<cudaStream_t>(stream));
 }
@@ -242,13 +255,24 @@ int hk_tree_attention(const hk_tree_params* p, void* stream) {
     if (p->tree && p->tree_stride < 0) return HK_ERR_BAD_SHAPE;
     Dim lse[] = {{p->B, p->lse_strideB}, {p->nh, p->lse_strideH}};
     if (!lie_apart(lse, p->T)) return HK_ERR_UNSUPPORTED;  // rows on top of each other
-    ServingArgs a{};
-    a.Q = p->Q; a.K = p->K; a.V = p->V; a.O = p->O; a.pool = p->pool;
+    ServingArgs a = sizes_of(p);
+    a.Q = p->Q; a.K = p->K; a.V = p->V; a.O = p->O;
     a.LSE = p->LSE; a.lse_sB = p->lse_strideB; a.lse_sH = p->lse_strideH;
     a.lengths = p->lengths; a.tree = p->tree; a.tree_stride = p->tree_stride;
-    a.B = p->B; a.Hk = p->nh_kv; a.group = p->nh / p->nh_kv; a.T = (int)p->T;
     if ((rc = set_parts(a, parts_of(p), p->workspace, p->workspace_bytes)) || (rc = set_scale(a, p->dtype, p->scale))) return rc;
     return few_rows(p) ? launch_tree_few(a, p->dtype, static_cast<cudaStream_t>(stream)) : launch_tree_rows(a, p->dtype, static_cast<cudaStream_t>(stream));
+}
+
+// For tests: the line (LineSum) of a call of these sizes whose prompts, or requests in their pages, have `lens` keys (host, [B])
+int hk_prompt_line(const hk_prompt_params* p, const int32_t* lens, int64_t* out) {
+    const int rc = check_sizes(p);
+    if (rc == HK_OK) put_line(prompt_rows_line(sizes_of(p), p->dtype, lens), out);
+    return rc;
+}
+int hk_tree_line(const hk_tree_params* p, const int32_t* lens, int64_t* out) {
+    const int rc = check_sizes(p);
+    if (rc == HK_OK) put_line(few_rows(p) ? tree_few_line(sizes_of(p), p->dtype, lens) : tree_rows_line(sizes_of(p), p->dtype, lens), out);
+    return rc;
 }
 
 }  // extern "C"

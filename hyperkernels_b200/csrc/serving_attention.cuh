@@ -1,6 +1,8 @@
 // serving_attention.cuh -- what the kernels of the attention within packed prompts and against a cache of pages have in common.
 #pragma once
 
+#include <climits>
+
 #include "cache_pages.cuh"
 #include "tile_math.cuh"
 
@@ -60,34 +62,42 @@ struct Request {
     int units;                       // of all of its blocks, under one key head
 };
 // A block counts as the keys that it meets and EXTRA for its beginning and end, in units of 2^unit_shift keys, so that all of them fit 32
-// bits: a division of 64-bit numbers takes a warp some 300 cycles.
+// bits: a division of 64-bit numbers takes a warp some 300 cycles.  EXTRA is up to a unit more where a unit is several keys: every block is then at least as
+// wide as what it counts as, so none lies on the line without a width, taken by nobody, and a worker that has all of a block's units has all of its tiles.
 template <int KEYS_, int LEAST_, int SHARE_, int EXTRA, bool TREE, int DEAL_ = 0>
 struct Work {
     // keys of a tile; tiles that a part of a block has, and a worker, at least; blocks for each worker from which on they are dealt out (0: never)
     static constexpr int KEYS = KEYS_, LEAST = LEAST_, SHARE = SHARE_, DEAL = DEAL_;
     const ServingArgs& a;
-    __device__ __forceinline__ int all_tiles(const Request& r) const { return (r.len + KEYS - 1) / KEYS + (TREE ? a.new_tiles : 0); }
-    __device__ __forceinline__ int tiles(const Request& r, int i) const {
-        return TREE || !a.causal ? all_tiles(r) : (min((i + 1) * a.block_tokens, r.len) + KEYS - 1) / KEYS;
+    __host__ __device__ __forceinline__ int all_tiles(const Request& r) const { return (r.len + KEYS - 1) / KEYS + (TREE ? a.new_tiles : 0); }
+    __host__ __device__ __forceinline__ int tiles(const Request& r, int i) const {
+        return TREE || !a.causal ? all_tiles(r) : (((i + 1) * a.block_tokens < r.len ? (i + 1) * a.block_tokens : r.len) + KEYS - 1) / KEYS;
     }
     // units in front of block i, of one chunk of heads
-    __device__ __forceinline__ int before(const Request& r, int i) const {
-        const int64_t keys = TREE || !a.causal ? (int64_t)i * (all_tiles(r) * KEYS + EXTRA) : (int64_t)i * (i + 1) / 2 * a.block_tokens + (int64_t)i * EXTRA;
+    __host__ __device__ __forceinline__ int before(const Request& r, int i) const {
+        const int extra = EXTRA - 1 + (1 << a.unit_shift);
+        const int64_t keys = TREE || !a.causal ? (int64_t)i * (all_tiles(r) * KEYS + extra) : (int64_t)i * (i + 1) / 2 * a.block_tokens + (int64_t)i * extra;
         return (int)(keys >> a.unit_shift);
     }
-    __device__ __forceinline__ Request request(int b) const {
+    // A border inside a block is moved to its beginning or end where a part of less than LEAST tiles would be left.
+    __host__ __device__ __forceinline__ int border(int units, int n) const {
+        const int64_t at = ((int64_t)units << a.unit_shift) / KEYS;
+        const int j = at < n ? (int)at : n;
+        return j == n ? n : j < LEAST ? 0 : n - j < LEAST ? n : j;
+    }
+    __host__ __device__ __forceinline__ Request sized(int begin, int len, int tokens) const {
         Request r;
-        if (TREE) {
-            r.begin = 0;
-            r.len = cache_keys(a, b);
-            r.tokens = a.rows ? a.rows : a.T;
-        } else {
-            r.begin = min(max(a.starts[b], 0), a.N);
-            r.len = r.tokens = max(0, min(max(a.starts[b + 1], 0), a.N) - r.begin);
-        }
+        r.begin = begin;
+        r.len = len;
+        r.tokens = tokens;
         r.blocks = (int)(((uint64_t)(uint32_t)(r.tokens + a.block_tokens - 1) * a.block_mul) >> a.block_shift);
         r.units = before(r, r.blocks) * a.chunks;
         return r;
+    }
+    __device__ __forceinline__ Request request(int b) const {
+        if (TREE) return sized(0, cache_keys(a, b), a.rows ? a.rows : a.T);
+        const int begin = min(max(a.starts[b], 0), a.N), len = max(0, min(max(a.starts[b + 1], 0), a.N) - begin);
+        return sized(begin, len, len);
     }
 };
 // What a worker takes at once: tiles [from, to) of block i's n.
@@ -257,11 +267,6 @@ struct Line {
         }
         return false;
     }
-    // A border inside a block is moved to its beginning or end where a part of less than LEAST tiles would be left.
-    __device__ __forceinline__ int border(const W& work, int units, int n) const {
-        const int j = (int)min((int64_t)n, ((int64_t)units << work.a.unit_shift) / W::KEYS);
-        return j == n ? n : j < W::LEAST ? 0 : n - j < W::LEAST ? n : j;
-    }
     // The next run; false: the stretch is over
     __device__ __forceinline__ bool next(const W& work, Run& run, const int* blocks = nullptr) {
         if (W::DEAL > 0 && dealt) return next_dealt(work, run, blocks);
@@ -278,7 +283,7 @@ struct Line {
                 }
                 continue;
             }
-            const int n = work.tiles(r, i), from = border(work, done, n), to = border(work, done + units, n);
+            const int n = work.tiles(r, i), from = work.border(done, n), to = work.border(done + units, n);
             units -= work.before(r, i + 1) - work.before(r, i) - done;
             done = 0;
             run = {r, b, kvh, chunk, i, from, to, n};
@@ -295,6 +300,26 @@ struct Line<W>::Saved {
 };
 // Host: the constants of the line; the sum of the parts of blocks that fell to several of `workers`
 void set_line(ServingArgs& a, bool tree, int keys);
+// For tests: what the line of requests of these lengths comes to under all key heads, in units; units of its narrowest block; tiles that its blocks
+// would lose at their ends.  2^unit_shift is a unit.
+struct LineSum {
+    int64_t units, narrowest, lost, unit_shift;
+};
+template <class W>
+LineSum line_sum(const ServingArgs& a, const int32_t* lens) {
+    const W work{a};
+    LineSum sum{0, INT_MAX, 0, a.unit_shift};
+    for (int b = 0; b < a.B; ++b) {
+        const Request r = work.sized(0, lens[b], a.T == 0 ? lens[b] : a.rows ? a.rows : a.T);
+        sum.units += (int64_t)r.units * a.Hk;
+        for (int i = 0; i < r.blocks; ++i) {
+            const int width = work.before(r, i + 1) - work.before(r, i), n = work.tiles(r, i);
+            sum.narrowest = std::min<int64_t>(sum.narrowest, width);
+            sum.lost += n - work.border(width, n);
+        }
+    }
+    return sum;
+}
 int launch_combine(ServingArgs a, int dtype, int workers, cudaStream_t stream);
 
 struct RowsPlan {
@@ -312,5 +337,8 @@ TreeFewPlan tree_few_plan(int dtype, int rows);
 int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream);
 int launch_prompt_rows(const ServingArgs& a, int dtype, cudaStream_t stream);
 int launch_tree_rows(const ServingArgs& a, int dtype, cudaStream_t stream);
+LineSum tree_few_line(ServingArgs a, int dtype, const int32_t* lens);
+LineSum prompt_rows_line(const ServingArgs& a, int dtype, const int32_t* lens);
+LineSum tree_rows_line(const ServingArgs& a, int dtype, const int32_t* lens);
 
 }  // namespace hk

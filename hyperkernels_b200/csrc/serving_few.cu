@@ -372,10 +372,35 @@ TreeFewPlan tree_few_plan(int dtype, int rows) {
     return {std::min(rows, e.rows), e.keys, 2, sm_count() * e.per_sm, WARPS + 1};
 }
 
-int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
+namespace {
+// The kernel of the call, and how it cuts the work: `side` key heads are one from there on
+Entry cut(ServingArgs& a, int dtype, int& side) {
     a.rows = a.T * a.group;
-    const int side = heads_side_by_side(a, pick(dtype, a.rows, 1));
+    side = heads_side_by_side(a, pick(dtype, a.rows, 1));
     const Entry e = pick(dtype, a.rows, side);
+    a.block_tokens = std::min(a.rows, e.rows) * side;
+    a.chunks = 1;
+    divide_by(a.group, a.group_mul, a.group_shift);
+    a.Hk /= side;
+    a.group *= side;
+    a.rows *= side;
+    a.slot_rows = a.block_tokens;
+    a.new_tiles = cdiv(a.T, e.keys);
+    set_line(a, true, e.keys);
+    return e;
+}
+}  // namespace
+
+LineSum tree_few_line(ServingArgs a, int dtype, const int32_t* lens) {
+    int side;
+    const Entry e = cut(a, dtype, side);
+    return e.keys == FewMath<float>::KEYS ? line_sum<FewWork<FewMath<float>::KEYS>>(a, lens) : line_sum<FewWork<FewMath<__half>::KEYS>>(a, lens);
+}
+
+int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
+    const int Hk = a.Hk;
+    int side;
+    const Entry e = cut(a, dtype, side);
     // once per device and kernel: more than 48 KB of shared memory
     static std::mutex mu;
     static Kernel known[HK_MAX_DEVICES][16];
@@ -391,22 +416,12 @@ int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
             break;
         }
     }
-    a.block_tokens = std::min(a.rows, e.rows);
-    a.chunks = 1;
-    divide_by(a.group, a.group_mul, a.group_shift);
     CUtensorMap k, v, kp, vp;
     int s;
-    if ((s = prefix_tile_map(&k, a.K, dtype, a.B, a.Hk, a.T, e.keys, false)) || (s = prefix_tile_map(&v, a.V, dtype, a.B, a.Hk, a.T, e.keys, false)) ||
-        (s = prefix_tile_map(&kp, a.pool.K, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false, a.pool.K.strideM != HEAD_DIM)) ||
-        (s = prefix_tile_map(&vp, a.pool.V, dtype, a.pool.n_pages, a.Hk, a.pool.page, e.keys, false, a.pool.V.strideM != HEAD_DIM)))
+    if ((s = prefix_tile_map(&k, a.K, dtype, a.B, Hk, a.T, e.keys, false)) || (s = prefix_tile_map(&v, a.V, dtype, a.B, Hk, a.T, e.keys, false)) ||
+        (s = prefix_tile_map(&kp, a.pool.K, dtype, a.pool.n_pages, Hk, a.pool.page, e.keys, false, a.pool.K.strideM != HEAD_DIM)) ||
+        (s = prefix_tile_map(&vp, a.pool.V, dtype, a.pool.n_pages, Hk, a.pool.page, e.keys, false, a.pool.V.strideM != HEAD_DIM)))
         return s;
-    a.Hk /= side;
-    a.group *= side;
-    a.rows *= side;
-    a.block_tokens *= side;
-    a.slot_rows = a.block_tokens;
-    a.new_tiles = cdiv(a.T, e.keys);
-    set_line(a, true, e.keys);
     divide_by(a.pool.page, a.page_mul, a.page_shift);
     const int ctas = sm_count() * e.per_sm;
     LaunchConfig lc(ctas, WARPS * 32, e.smem, stream, 1, true);

@@ -997,6 +997,18 @@ int query_map(CUtensorMap* map, const hk_view& v, int dtype, int B, int H, int64
     return r == CUDA_SUCCESS ? HK_OK : HK_ERR_CUDA;
 }
 
+// How the work is cut
+template <class X, bool TREE, bool SPLIT>
+void cut(ServingArgs& a) {
+    typedef Rows<X> C;
+    a.stream_tokens = std::max(1, TILE / a.group);
+    a.block_tokens = C::STREAMS * a.stream_tokens;
+    a.chunks = cdiv(a.group, TILE);
+    a.new_tiles = 1;
+    a.slot_rows = SPLIT ? TILE : C::BLOCK;
+    set_line(a, TREE, C::KEYS);
+}
+
 template <class X, bool TREE, bool SPLIT>
 int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     typedef Rows<X> C;
@@ -1006,12 +1018,7 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
     std::call_once(once[dev], [dev] { rc[dev] = cudaFuncSetAttribute(serving_rows_kernel<X, TREE, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSpace<X>::SMEM); });
     if (rc[dev] != cudaSuccess) return HK_ERR_CUDA;
-    a.stream_tokens = std::max(1, TILE / a.group);
-    a.block_tokens = C::STREAMS * a.stream_tokens;
-    a.chunks = cdiv(a.group, TILE);
-    a.new_tiles = 1;
-    a.slot_rows = SPLIT ? TILE : C::BLOCK;
-    set_line(a, TREE, C::KEYS);
+    cut<X, TREE, SPLIT>(a);
     CUtensorMap k, v, kp, vp;
     const int B = TREE ? a.B : 1;
     const int64_t T = TREE ? a.T : a.N;
@@ -1035,6 +1042,15 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     count_launch();
     return a.parts ? launch_combine(a, dtype, ctas, stream) : HK_OK;
 }
+template <class X, bool TREE, bool SPLIT>
+LineSum line(ServingArgs a, const int32_t* lens) {
+    cut<X, TREE, SPLIT>(a);
+    return line_sum<RowsWork<X, TREE, SPLIT>>(a, lens);
+}
+template <bool TREE, bool SPLIT>
+LineSum line(const ServingArgs& a, int dtype, const int32_t* lens) {
+    return dtype == HK_F32 ? line<float, TREE, false>(a, lens) : line<__half, TREE, SPLIT>(a, lens);
+}
 template <bool TREE, bool SPLIT>
 int launch(const ServingArgs& a, int dtype, cudaStream_t stream) {
     return dtype == HK_F32 ? launch<float, TREE, false>(a, dtype, stream) : dtype == HK_BF16 ? launch<__nv_bfloat16, TREE, SPLIT>(a, dtype, stream) : launch<__half, TREE, SPLIT>(a, dtype, stream);
@@ -1046,8 +1062,11 @@ RowsPlan rows_plan(int dtype) { return dtype == HK_F32 ? RowsPlan{Rows<float>::B
 int launch_prompt_rows(const ServingArgs& a, int dtype, cudaStream_t stream) { return launch<false, false>(a, dtype, stream); }
 // Up to 128 rows of a request under a key head: both streams have them, every other tile each (16 requests of up to 4 096 tokens, 16 new ones,
 // 32 heads on 8, bf16: 25 us, 29 where the second stream has nothing to do; 32 new ones of 12 heads 30 and 39).
+static bool one_stream(const ServingArgs& a) { return a.T <= std::max(1, TILE / a.group); }
 int launch_tree_rows(const ServingArgs& a, int dtype, cudaStream_t stream) {
-    return a.T <= std::max(1, TILE / a.group) ? launch<true, true>(a, dtype, stream) : launch<true, false>(a, dtype, stream);
+    return one_stream(a) ? launch<true, true>(a, dtype, stream) : launch<true, false>(a, dtype, stream);
 }
+LineSum prompt_rows_line(const ServingArgs& a, int dtype, const int32_t* lens) { return line<false, false>(a, dtype, lens); }
+LineSum tree_rows_line(const ServingArgs& a, int dtype, const int32_t* lens) { return one_stream(a) ? line<true, true>(a, dtype, lens) : line<true, false>(a, dtype, lens); }
 
 }  // namespace hk

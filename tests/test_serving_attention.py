@@ -302,6 +302,30 @@ def test_many_small_weights_beside_a_large_one(dtype, T):
         assert bool(((lse.double() - LSE).abs() <= d + 245 * U + 4 * U * LSE.abs()).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,times,H,Hk", [([1], 1 << 17, 16, 16), ([1, 16, 2, 40, 5], 1 << 14, 8, 8), ([3, 700, 0, 9], 100, 64, 8)], ids=lambda x: str(len(x)) if isinstance(x, list) else None)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_very_many_prompts(lens, times, H, Hk, dtype, causal):
+    """So many that a short one is little of a unit of the line they make: none may get lost, the first and the last among them."""
+    x = q, k, v, starts = make_prompts(len(lens), lens * times, H, Hk, dtype)
+    N, G = q.shape[0], H // Hk
+    out, lse = torch.full((N, H, 64), math.nan, device="cuda", dtype=TYPES[dtype]), torch.full((H, N), math.nan, device="cuda")
+    got = hk.prompt_attention(*x, SCALE, causal, out=out, lse=lse)
+    again = hk.prompt_attention(*x, SCALE, causal)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    for c, n in enumerate(lens):  # all of one length at once
+        if n == 0:
+            continue
+        i = torch.arange(n, device="cuda")
+        rows = starts[:-1].long()[c::len(lens), None] + i
+        for part in rows.split(max(1, (1 << 18) // (n * H))):
+            qq, kk, vv, oo = (t[part].transpose(1, 2) for t in (q, k.repeat_interleave(G, 1) if G > 1 else k, v.repeat_interleave(G, 1) if G > 1 else v, out))
+            want = attend(qq.reshape(-1, n, 64), kk.reshape(-1, n, 64), vv.reshape(-1, n, 64), (i <= i[:, None]) | (not causal), SCALE)
+            check((oo.reshape(-1, n, 64), lse[:, part].transpose(0, 1).reshape(-1, n)), want, dtype, (n, part[0]))
+    assert hk.last_device_status() == 0
+
+
 # ---- new tokens against the pages -----------------------------------------------------------------------------------------------------
 def make_tree(seed, lens, T, H, Hk, page, dtype, layout="hpd", tree="random", junk=math.nan, sigma=1.0, spare=2):
     """Pages in any order; what is behind a request's last key, and in pages of nobody, is junk"""
@@ -433,6 +457,23 @@ def test_lengths_at_borders_and_outside(dtype, T, G, junk):
         x[p].nan_to_num_(0.5, 0.5, 0.5).clamp_(-5, 5)
     assert x[5].shape[1] == full
     check(hk.tree_attention(*x), trees(*x), dtype)
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,H,Hk", [(1, 1, 1), (3, 8, 4), (2, 16, 2), (20, 2, 1), (64, 12, 2)])
+def test_tables_with_room_for_far_more(dtype, T, H, Hk):
+    """A table that 2^30 keys of each request would fit, which have none or few: a block is little of a unit of the line they make."""
+    x = list(make_tree(T, [0, 1, 40, 0, 300, 2000, 0] * 9 + [0], T, H, Hk, 16384, dtype))
+    x[5] = torch.cat([x[5], x[5].new_full((x[5].shape[0], 65536 - x[5].shape[1]), -1)], 1)
+    out, lse = torch.full(x[0].shape, math.nan, device="cuda", dtype=TYPES[dtype]), torch.full(x[0].shape[:3], math.nan, device="cuda")
+    for lens in (x[6], torch.zeros_like(x[6])):
+        x[6] = lens
+        got = hk.tree_attention(*x, out=out.fill_(math.nan), lse=lse.fill_(math.nan))
+        check(got, trees(*x), dtype)
+        again = hk.tree_attention(*x)
+        assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
     assert hk.last_device_status() == 0
 
 
@@ -869,3 +910,38 @@ def test_blocks_that_are_refused(kind, path, value, status):
     for f in (hk.lib().hk_prompt_attention, hk.lib().hk_tree_attention):
         f.argtypes = [C.c_void_p, C.c_void_p]
         assert f(None, None) == -1
+
+
+# ---- the line of the work --------------------------------------------------------------------------------------------------------------
+def line_of(b, lens):
+    """All units, units of the narrowest block, tiles lost at blocks' ends, 2^x keys to a unit; lens: [n], so often as there are requests"""
+    f = hk.lib().hk_prompt_line if type(b) is Prompt else hk.lib().hk_tree_line
+    f.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+    all_lens = torch.tensor(lens, dtype=torch.int32).repeat(cdiv(b.B, len(lens)))[:b.B].contiguous()
+    out = (C.c_int64 * 4)()
+    assert f(C.byref(b), all_lens.data_ptr(), out) == 0
+    return list(out)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("N,B,H,Hk,lens,shift", [
+    (9, 2, 4, 2, [9, 0], 0), (1 << 17, 1 << 17, 12, 12, [1], 0), (1 << 20, 1 << 20, 8, 8, [1], 5), (1 << 20, 1000, 64, 8, [5, 2000], None), (1 << 20, 1 << 15, 64, 8, [32], None), (1 << 17, 1 << 17, 64, 64, [1], None),
+    (1 << 24, 1 << 20, 64, 1, [16], None), (1 << 24, 3, 1, 1, [100, 0, (1 << 24) - 100], None), (1 << 30, 1 << 20, 1, 1, [1024], None), (1 << 30, 2, 1, 1, [1, (1 << 30) - 1], None), (1 << 21, 7, 300, 1, [300000], None)])
+def test_every_block_of_prompts_is_on_the_line(N, B, H, Hk, lens, shift, dtype, causal):
+    b = block(Prompt)
+    b.N, b.B, b.nh, b.nh_kv, b.dtype, b.is_causal = N, B, H, Hk, dtype, causal
+    units, narrowest, lost, unit_shift = line_of(b, lens)
+    assert 0 < units < 2 ** 31 and narrowest >= 1 and lost == 0, (units, narrowest, lost, unit_shift)
+    assert shift is None or unit_shift == shift or unit_shift == shift + 1
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("B,T,H,Hk,width,page,lens", [
+    (2, 1, 4, 4, 64, 16, [9, 0]), (64, 1, 1, 1, 16384, 65536, [0]), (64, 1, 1, 1, 16384, 65536, [0, 1, 70, 5000]), (1 << 16, 1, 32, 8, 16384, 64, [0, 1 << 20, 17]), (1 << 16, 16, 32, 32, 16384, 64, [3, 1 << 20]),
+    (1 << 16, 64, 256, 1, 1024, 1024, [1 << 20]), (1 << 24, 64, 1, 1, 64, 16, [0, 1]), (1 << 12, 64, 300, 2, 1 << 18, 4096, [1 << 30, 0])])
+def test_every_block_of_a_tree_is_on_the_line(B, T, H, Hk, width, page, lens, dtype):
+    b = block(Tree)
+    b.B, b.T, b.nh, b.nh_kv, b.dtype, b.pool.width, b.pool.page = B, T, H, Hk, dtype, width, page
+    units, narrowest, lost, unit_shift = line_of(b, lens)
+    assert 0 < units < 2 ** 31 and narrowest >= 1 and lost == 0, (units, narrowest, lost, unit_shift)
