@@ -195,10 +195,10 @@ void put_line(const LineSum& x, int64_t* out) { out[0] = x.units; out[1] = x.nar
 void set_line(ServingArgs& a, bool tree, int keys) {
     divide_by(a.block_tokens, a.block_mul, a.block_shift);
     // What all requests can come to: blocks, those of prompts without tokens left out; the keys that they meet, of prompts most where one has all the tokens; of
-    // each block 4 tiles beside them, and up to a unit.
+    // each block 5 tiles beside them (its beginning and end count up to 4, and its last tile as a whole), and up to a unit.
     const double heads = (double)a.Hk * a.chunks, blocks = heads * (tree ? (double)a.B * cdiv(a.rows ? a.rows : a.T, a.block_tokens) : (double)a.N / a.block_tokens + std::min(a.B, a.N));
     const double met = tree ? blocks * ((double)a.pool.width * a.pool.page + a.new_tiles * keys) : heads * ((double)a.N * a.N / a.block_tokens + 2.0 * a.N + (double)std::min(a.B, a.N) * a.block_tokens);
-    double all = met + blocks * 4.0 * keys;
+    double all = met + blocks * 5.0 * keys;
     for (a.unit_shift = 0; all + (a.unit_shift > 0 ? blocks : 0.0) >= 2e9; all /= 2) ++a.unit_shift;
 }
 

@@ -939,7 +939,8 @@ def test_every_block_of_prompts_is_on_the_line(N, B, H, Hk, lens, shift, dtype, 
 @pytest.mark.parametrize("dtype", [0, 1])
 @pytest.mark.parametrize("B,T,H,Hk,width,page,lens", [
     (2, 1, 4, 4, 64, 16, [9, 0]), (64, 1, 1, 1, 16384, 65536, [0]), (64, 1, 1, 1, 16384, 65536, [0, 1, 70, 5000]), (1 << 16, 1, 32, 8, 16384, 64, [0, 1 << 20, 17]), (1 << 16, 16, 32, 32, 16384, 64, [3, 1 << 20]),
-    (1 << 16, 64, 256, 1, 1024, 1024, [1 << 20]), (1 << 24, 64, 1, 1, 64, 16, [0, 1]), (1 << 12, 64, 300, 2, 1 << 18, 4096, [1 << 30, 0])])
+    (1 << 16, 64, 256, 1, 1024, 1024, [1 << 20]), (1 << 24, 64, 1, 1, 64, 16, [0, 1]), (1 << 12, 64, 300, 2, 1 << 18, 4096, [1 << 30, 0]),
+    (2900000, 17, 1, 1, 1, 16, [16]), (2900000, 17, 1, 1, 1, 16, [1]), (2900000, 40, 4, 1, 1, 16, [16])])
 def test_every_block_of_a_tree_is_on_the_line(B, T, H, Hk, width, page, lens, dtype):
     b = block(Tree)
     b.B, b.T, b.nh, b.nh_kv, b.dtype, b.pool.width, b.pool.page = B, T, H, Hk, dtype, width, page
