@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 6) append_kernel(const __gr
         row = (int)item;
         b = sequence_of(a.starts, a.B, row, lane);
         if (b >= a.B || a.starts[b] > row) return;
-        pos = (int64_t)row - a.starts[b];
+        pos = row - max(a.starts[b], 0);
         from_b = 0;
     } else {
         if (item >= (int64_t)a.B * a.T) return;

@@ -441,8 +441,8 @@ int hk_tree_attention(const hk_tree_params* p, void* stream);
 size_t hk_tree_workspace_bytes(const hk_tree_params* p);
 
 /* Brings keys and values of new tokens into the pages, behind the lengths[b] that are there: new token k of request b becomes token
- * lengths[b] + k.  Which rows these are: with `starts` rows starts[b] <= i < starts[b + 1] of a packed [1, nh_kv, T, 64] (k = i -
- * starts[b]); otherwise of [B, nh_kv, T, 64] the rows picks[b * T + k] (NULL: k), k < counts[b] (NULL: T).  A pick outside [0, T) is
+ * lengths[b] + k.  Which rows these are: with `starts`, taken into [0, T] and ascending, rows starts[b] <= i < starts[b + 1] of a packed
+ * [1, nh_kv, T, 64] (k = i - starts[b]); otherwise of [B, nh_kv, T, 64] the rows picks[b * T + k] (NULL: k), k < counts[b] (NULL: T).  A pick outside [0, T) is
  * left out, and so is a token that has no page.  No two tokens may come to the same place. */
 typedef struct hk_append_params {
     hk_view K, V;

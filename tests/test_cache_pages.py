@@ -128,6 +128,31 @@ def test_starts_that_are_no_starts():
     assert torch.equal(ka[0], before[0]) and torch.equal(ka[5:], before[5:])
 
 
+@pytest.mark.gpu
+def test_starts_are_taken_into_the_tensor():
+    """As the attention takes them: a first prompt that begins in front of the tensor begins with its first row."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn((250, 2, 64), generator=g, device="cuda")
+    rows, lens = [list(range(6)), list(range(6, 24))], [3, 20]
+    want = None
+    for starts in ([0, 50, 250], [-7, 50, 100000], [-2 ** 31, 50, 2 ** 31 - 1]):
+        _, kp = pool(torch.Generator(device="cuda").manual_seed(3), None, 24, 2, 16, "f32", "hpd")
+        _, vp = pool(torch.Generator(device="cuda").manual_seed(4), None, 24, 2, 16, "f32", "phd")
+        if want is None:
+            want = kp.clone(), vp.clone()
+            parts = [(x[a:b].transpose(0, 1), -x[a:b].transpose(0, 1), range(b - a)) for a, b in ((0, 50), (50, 250))]
+            append_model(None, None, *want, rows, lens, parts)
+        table_ = ints([r + [-1] * (18 - len(r)) for r in rows])
+        hk.cache_append(x, -x, kp, vp, table_, ints(lens), starts=ints(starts))
+        assert torch.equal(kp, want[0]) and torch.equal(vp, want[1]), starts
+    _, kp = pool(torch.Generator(device="cuda").manual_seed(3), None, 24, 2, 16, "f32", "hpd")
+    hk.cache_append(x, x, kp, kp.clone(), table_, ints(lens), starts=ints([-9, -4, 250]))  # the first is empty
+    first = [(x[:0].transpose(0, 1), None, range(0)), (x.transpose(0, 1), x.transpose(0, 1), range(250))]
+    _, wk = pool(torch.Generator(device="cuda").manual_seed(3), None, 24, 2, 16, "f32", "hpd")
+    append_model(None, None, wk, wk.clone(), rows, lens, first)
+    assert torch.equal(kp, wk)
+
+
 # ---- forking ------------------------------------------------------------------------------------------------------------------------
 def fork_model(kp, vp, pages, lens, users, source, room):
     """Tables, and copies made in kp, vp: [layers, P, Hk, page, 64]"""
