@@ -282,6 +282,40 @@ def test_more_missing_than_there_are_numbers():
         assert got[3].tolist() == [missing] and got[0].flatten().tolist() == ([0, 1, 2, 3] if missing else []) + [-1] * (4 * B - 4 * (missing > 0))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,layout", [("f32", "hpd"), ("bf16", "phd"), ("f16", "wide")])
+def test_beams_of_many_layers(dtype, layout):
+    """More to copy than the kernel over the tables copies, tables that fit its shared memory: the copies are a kernel of their own."""
+    rng, g = random.Random(3), torch.Generator(device="cuda").manual_seed(3)
+    B, beams, layers, Hk, page, width = 16, 4, 28, 12, 64, 5
+    lens = [rng.randint(0, (width - 1) * page) for _ in range(B)]
+    lens[0], lens[1], lens[2] = 0, page, page + 1
+    P = sum(cdiv(n, page) for n in lens) + 2 * B * beams - 100  # too few for all
+    pages = table(rng, P, [cdiv(n, page) for n in lens], width)
+    users = [0] * P
+    for p in sum(pages, []):
+        if p >= 0:
+            users[p] += 1
+    source, room = [b for b in range(B) for _ in range(beams)], [1 + 70 * (i % 3) for i in range(B * beams)]
+    rng.shuffle(source)
+    (ka, kp), (va, vp) = pool(g, layers, P, Hk, page, dtype, layout), pool(g, layers, P, Hk, page, dtype, layout)
+    want_k, want_v = ka.clone(), va.clone()
+    wk, wv = (torch.as_strided(w, p.shape, p.stride(), p.storage_offset()) for w, p in ((want_k, kp), (want_v, vp)))
+    want = fork_model(wk, wv, pages, lens, users, source, room)
+    before = hk.launch_count()
+    got = hk.cache_fork(kp, vp, ints(pages), ints(lens), ints(users), ints(source), ints(room))
+    assert hk.launch_count() - before == 2 and want[3] > 0
+    assert [x.tolist() for x in got] == [want[0], want[1], want[2], [want[3]]]
+    assert torch.equal(ka, want_k) and torch.equal(va, want_v)
+    # and the pages to the front by the same
+    rows, users, where = compact_model(wk, wv, [r[:2] for r in want[0]], [u if p % 3 else 0 for p, u in enumerate(want[2])])
+    before = hk.launch_count()
+    moved = hk.cache_compact(kp, vp, got[0][:, :2], got[2] * ints([1 if p % 3 else 0 for p in range(P)]))
+    assert hk.launch_count() - before == 2
+    assert [x.tolist() for x in moved] == [rows, users, where]
+    assert torch.equal(ka, want_k) and torch.equal(va, want_v)
+
+
 # ---- compacting ------------------------------------------------------------------------------------------------------------------------
 def compact_model(kp, vp, pages, users):
     P = kp.shape[1]
