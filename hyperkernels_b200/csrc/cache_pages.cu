@@ -212,14 +212,30 @@ __device__ __forceinline__ int block_scan(Sums& sh, int x, int& total) {
     return s - x + (warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0);
 }
 
+// The first rows of a page to zeros, in every layer, by a warp
+__device__ __forceinline__ void clear_rows(const Copies& a, int page, int rows, int lane) {
+    const int64_t e = a.esize;
+    const int each = 4 * a.esize;  // 16-byte parts of a row
+    for (int kv = 0; kv < 2; ++kv) {
+        const hk_view& v = kv ? a.pool.V : a.pool.K;
+        for (int layer = 0; layer < a.layers; ++layer) {
+            for (int h = 0; h < a.Hk; ++h) {
+                char* const to = static_cast<char*>(v.ptr) + (layer * (kv ? a.v_strideL : a.k_strideL) + page * v.strideB + h * v.strideH) * e;
+                for (int i = lane; i < rows * each; i += 32) reinterpret_cast<uint4*>(to + i / each * v.strideM * e)[i % each] = make_uint4(0, 0, 0, 0);
+            }
+        }
+    }
+}
+
 struct Request {  // of the new batch
     int source;   // row of the old table, -1: none
     int len;
     int kept;     // pages it has
     int need;     // pages up to where it has room
     int first;    // number of its first new page
-    int copy;     // number of its copy, -1: none
+    int copy;     // number of its copy, -1: none, CLEARED: its begun page is none, it gets one whose rows are zeros
 };
+constexpr int CLEARED = -2;
 struct ForkArgs {
     Copies copies;
     const int32_t *lengths, *users, *source, *room;
@@ -238,7 +254,7 @@ struct ForkArgs {
 };
 
 template <bool SHARED>
-__global__ void __launch_bounds__(THREADS) fork_kernel(const __grid_constant__ ForkArgs a) {
+__global__ void __launch_bounds__(THREADS, 1) fork_kernel(const __grid_constant__ ForkArgs a) {
     __shared__ Sums sums;
     __shared__ unsigned long long lacking;
     extern __shared__ Pair room[];
@@ -259,17 +275,19 @@ __global__ void __launch_bounds__(THREADS) fork_kernel(const __grid_constant__ F
     if (!SHARED) nobody();  // the call before may still have used the workspace
     // a thread's first request is on its way while the tables are read
     struct Wish {
-        int source, len;
+        int source, len, begun;  // begun: the page that is, -1: none
         int64_t room;
     };
     auto wish = [&](int i) {
-        Wish w = {-1, 0, 0};
+        Wish w = {-1, 0, -1, 0};
         if (i < a.B_out) {
             const int s = a.source[i];
             w.room = a.room ? (int64_t)max(a.room[i], 0) : a.room_all;
             if ((unsigned)s < (unsigned)a.B) {
                 w.source = s;
                 w.len = (int)min((int64_t)max(a.lengths[s], 0), (int64_t)M * pool.page);
+                const int full = w.len / pool.page;
+                if (w.len - full * pool.page) w.begun = pool.pages[s * pool.pages_stride + full];
             }
         }
         return w;
@@ -290,14 +308,14 @@ __global__ void __launch_bounds__(THREADS) fork_kernel(const __grid_constant__ F
         const int i = i0 + tid;
         const Wish w = i0 == 0 ? first : wish(i);
         Request r = {w.source, w.len, 0, 0, 0, -1};
-        bool copy = false;
+        bool copy = false, cleared = false;
         if (i < a.B_out) {
             const bool begun = w.len % pool.page != 0;
             if (w.source >= 0) {
-                const bool owns = owner[w.source] == i;
-                r.kept = w.len / pool.page + (begun && owns);
-                // of a begun page of which another has the original
-                copy = begun && !owns && is_page(pool.pages[w.source * pool.pages_stride + w.len / pool.page], P);
+                const bool there = begun && is_page(w.begun, P), owns = there && owner[w.source] == i;
+                r.kept = w.len / pool.page + owns;
+                copy = there && !owns;  // another has the original
+                cleared = begun && !there;
             }
             const int64_t need = (w.len + w.room + pool.page - 1) / pool.page;
             r.need = (int)max((int64_t)r.kept, min(need, (int64_t)M));
@@ -309,6 +327,7 @@ __global__ void __launch_bounds__(THREADS) fork_kernel(const __grid_constant__ F
         const int number = n_pairs + block_scan(sums, copy, copies);
         n_pairs += copies;
         if (copy) r.copy = number;
+        if (cleared) r.copy = CLEARED;
         if (i < a.B_out) {
             if (writes) a.lengths_out[i] = w.len;
             request[i] = r;
@@ -346,6 +365,8 @@ __global__ void __launch_bounds__(THREADS) fork_kernel(const __grid_constant__ F
             if (writes) a.pages_out[(int64_t)i * M + j] = page;
             if (j == begun) pairs[r.copy] = {pool.pages[r.source * pool.pages_stride + j], page, page >= 0 ? r.len % pool.page : 0, 0};
         }
+        // here, not among the copies: there a choice of what to store costs 2 to 4 % of their rate
+        if (writes && r.copy == CLEARED && r.first < n_free) clear_rows(a.copies, free[r.first], r.len % pool.page, tid % 32);
     }
     __syncthreads();
     if (writes) {

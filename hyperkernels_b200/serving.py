@@ -85,7 +85,9 @@ def cache_fork(K_pages, V_pages, pages, lengths, users, source, room=1, *, strea
     more tokens each of them gets pages for, [B'] of int32 on the device, or one number for all.  ``users``:
     [pages] of int32, how many hold each page: the entries of the table, and whoever else (a kept prefix, say) counts on.  Full pages are
     shared by all that go on with them.  One that is begun stays with the first of these; the others get one of their own and its rows
-    copied.  Pages nobody holds any longer are given out at once, lowest first.
+    copied.  Where a request's begun page is none (an earlier call had none to give), all that go on with it get one whose rows are zeros, which is what
+    they counted for.  Who keeps a begun page beside the table keeps the rows that there are; behind them a request goes on, so let one row of the
+    table at a time hold it.  Pages nobody holds any longer are given out at once, lowest first.
     Returns the next batch's ``pages`` [B', width], ``lengths`` [B'], ``users`` [pages], and ``missing`` [1]: how many pages could not be
     given because the pool is empty or the table is full (their entries are -1, rows that were to be copied there are lost)."""
     return _result(_native().fork(K_pages, V_pages, pages, lengths, users, source, room, _handle(stream)), "hk_cache_fork")

@@ -457,9 +457,11 @@ typedef struct hk_append_params {
 int hk_cache_append(const hk_append_params* p, void* stream);
 
 /* The next batch of B_out requests out of one of B: request i of it goes on where source[i] is (an entry outside [0, B): it starts
- * anew, with a length of 0).  users[p] counts who holds page p: the entries of the tables, and whoever else keeps pages (it counts on).  Pages
+ * anew, with a length of 0).  users[p] counts who holds page p: the entries of the tables, and whoever else keeps pages (it counts on; of
+ * a begun page the rows that there are stay, and one request goes on behind them).  Pages
  * that are full of a request's tokens are shared by all that go on with it.  One that is begun stays with the first of these; the others
- * get a page of their own with its rows copied, in every layer.  Then each request gets pages until it has room for room[i] tokens more,
+ * get a page of their own with its rows copied, in every layer; if it is no page, all of them get one, whose rows are zeros, as they counted.
+ * Then each request gets pages until it has room for room[i] tokens more,
  * out of those that nobody holds any longer: the lowest first, to the requests in their order.  What does not fit, because the pool is
  * empty or a row of the table at its end, is -1 in the table and counted in `missing` (up to 2^31 - 1).
  * Pages of requests that do not go on are free at once, and may be the ones that are given.  The tables that are written may not overlap

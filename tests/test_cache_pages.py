@@ -283,6 +283,43 @@ def test_more_missing_than_there_are_numbers():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["hpd", "phd"])
+@pytest.mark.parametrize("beams", [1, 3])
+def test_begun_pages_that_are_none(dtype, layout, beams):
+    """What an earlier call had no page for counts as rows of zeros: whoever goes on there gets a page that begins with such, as
+    soon as there is one.  Full pages that are none are shared as such."""
+    g = torch.Generator(device="cuda").manual_seed(beams)
+    (ka, kp), (va, vp) = (pool(g, 2, 12, 3, 16, dtype, layout) for _ in range(2))
+    ka.fill_(float("nan")), va.fill_(float("nan"))
+    rows, lens, users = [[3, -1, 12], [-1, 5, 40], [-7, -1, -1], [9, -1, -1]], [20, 32, 1, 16], [0] * 12
+    for p in (3, 5, 9):
+        users[p] = 1
+    source = [b for b in range(4) for _ in range(beams)]
+    want_rows, want_users, free = [], list(users), iter(p for p in range(12) if users[p] == 0)
+    begun = []  # new pages that begin with zeros, and how many rows of them
+    for b in source:
+        new = next(free, -1) if b in (0, 2, 3) else None
+        if b in (0, 2) and new >= 0:
+            begun.append((new, lens[b] % 16))
+        want_rows.append({0: [3, new, -1], 1: [-1, 5, -1], 2: [new, -1, -1], 3: [9, new, -1]}[b])
+    for p in range(12):
+        want_users[p] = sum(row.count(p) for row in want_rows)
+    room = [0 if b != 3 else 1 for b in source]
+    got = hk.cache_fork(kp, vp, ints(rows), ints(lens), ints(users), ints(source), ints(room))
+    assert [x.tolist() for x in got] == [want_rows, [lens[b] for b in source], want_users, [0]]
+    for x in (kp, vp):
+        for p in range(12):
+            n = dict(begun).get(p, 0)
+            assert bool((x[:, p, :, :n] == 0).all()) and bool(x[:, p, :, n:].isnan().all()), p
+    # an empty pool: still none, and said so
+    full = [max(u, 1) for u in users]
+    got = hk.cache_fork(kp, vp, ints(rows), ints(lens), ints(full), ints(source), ints(room))
+    assert got[0].tolist() == [[p if p != new else -1 for p, new in zip(r, [{0: r[1], 2: r[0], 3: r[1]}.get(b)] * 3)] for r, b in zip(want_rows, source)]
+    assert got[3].tolist() == [3 * beams]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,layout", [("f32", "hpd"), ("bf16", "phd"), ("f16", "wide")])
 def test_beams_of_many_layers(dtype, layout):
     """More to copy than the kernel over the tables copies, tables that fit its shared memory: the copies are a kernel of their own."""
