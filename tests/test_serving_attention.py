@@ -326,6 +326,19 @@ def test_very_many_prompts(lens, times, H, Hk, dtype, causal):
     assert hk.last_device_status() == 0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,H", [(700, 2), (3000, 40), (9000, 1)])
+def test_the_division_and_the_logarithm_of_fp32(N, H):
+    """Keys that all weigh the same, values that are whole numbers: every sum is exact, and what is left are a division, rounded, times the sum (2 u), and
+    log2 of the sum (an ulp, 2 u of it) times ln 2 (rounded, and its product: 2 u), whether a block was cut in parts or not."""
+    q, k, v = (torch.zeros((N, H, 64), device="cuda") for _ in range(3))
+    v[:] = torch.arange(1, 65, device="cuda")
+    n = torch.arange(1, N + 1, device="cuda", dtype=torch.float64)
+    o, lse = hk.prompt_attention(q, k, v, ints([0, N]), SCALE)
+    assert bool(((o.double() / v.double() - 1).abs() <= 2.001 * U).all())
+    assert bool(((lse.double() - n.log()).abs() <= 4.001 * U * n.log()).all())
+
+
 # ---- new tokens against the pages -----------------------------------------------------------------------------------------------------
 def make_tree(seed, lens, T, H, Hk, page, dtype, layout="hpd", tree="random", junk=math.nan, sigma=1.0, spare=2):
     """Pages in any order; what is behind a request's last key, and in pages of nobody, is junk"""
