@@ -171,7 +171,6 @@ int set_parts(ServingArgs& a, const Parts& parts, void* workspace, size_t bytes)
     return HK_OK;
 }
 int set_scale(ServingArgs& a, int dtype, float scale) {
-    a.scale = scale;
     a.scale_log2e = std::fabs(scale) * LOG2E;
     a.flip = scale > 0.f ? 0u : dtype == HK_F32 ? 0x80000000u : 0x80008000u;
     a.status = device_status_ptr();

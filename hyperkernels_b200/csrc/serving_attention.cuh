@@ -29,8 +29,7 @@ struct ServingArgs {
     int64_t tree_stride;
     int rows;                // few rows: of a request under a key head; many: 0
     int B, Hk, group, T, N;  // sequences, key heads, query heads of each, new tokens of each, tokens of all prompts
-    float scale;
-    float scale_log2e;  // its size; a negative scale turns the queries' signs (flip)
+    float scale_log2e;  // the scale's size; a negative one turns the queries' signs (flip)
     uint32_t flip;
     int causal;
     // a block's tokens (few rows: its rows) and 128s of query heads, tiles of new tokens; x / block_tokens is x * block_mul >> block_shift for x below 2^31
