@@ -116,7 +116,8 @@ struct LineSearch {
 // ..), `done` units behind the block's beginning, and goes on for `units`.
 // Where causal prompts make many blocks, these are dealt out whole instead, the longest first, there and back along the workers: no parts, and the
 // workers' shares differ by less than their last blocks (16 prompts of 17 to 1 000 tokens, 32 heads on 8, bf16: 56 us, 66 in equal stretches;
-// 16 of 1 024: 116 and 129).  With fewer than five blocks to a worker the stretches are the more even.
+// 16 of 1 024: 116 and 129).  With fewer than five blocks to a worker the stretches are the more even; more than 128 prompts, which is what four ballots
+// tell apart, go in stretches whatever their blocks.
 template <class W>
 struct Line {
     Request r;

@@ -5,9 +5,10 @@
 // and tables are read where the batches are asked for, 32 entries of a table at a time, so no product waits for them.  What a block of rows has in
 // several warps goes to slots; a CTA adds up what its own warps left, and what is left of blocks that fell to several CTAs a second kernel.
 // Where key heads come in fours the warps take one each instead, over the whole stretch of the CTA (heads_side_by_side).
-//   What bounds it is memory: 64 requests of 4 096 tokens, 32 heads on 8, bf16, 94 us or 5.7 TB/s, of which some 9 are the launch, the search for
+//   What bounds it is memory: 64 requests of 4 096 tokens, 32 heads on 8, bf16, 96 us or 5.6 TB/s, of which some 9 are the launch, the search for
 // the stretches, the first loads and the sum of the parts.  More than two rows of fp32 are bound by arithmetic: 16 requests of up to 2 047 tokens,
-// 12 heads, 1 / 2 / 4 (lane by lane) / 8 / 16 rows (three TF32 products of mma.sync): 18 / 22 / 30 / 33 / 35 us; the kernel of many rows takes 54 to 61.
+// 12 heads, 1 / 2 / 4 (lane by lane) / 8 / 16 rows (three TF32 products of mma.sync): 24 / 26 / 32 / 34 / 36 us with the keys in memory, 18 / 22 / 31 / 33 / 35 with
+// them in the L2; the kernel of many rows takes 53.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -357,8 +358,8 @@ Entry pick(int dtype, int rows, int side) {
     return rows == 1 ? entry<RowsOfOne<1>>() : rows == 2 ? entry<RowsOfOne<2>>() : rows <= 4 ? entry<RowsOfOne<4>>() : entry<RowsOf16<float>>();
 }
 // Key heads that a CTA takes side by side.  Four: its warps have nothing to add up, and where pools are stored token by token, with the heads
-// next to each other, memory is asked for neighbouring lines at once (64 requests of 4 096 tokens, 32 heads on 8, bf16: 94 us, 99 with a head
-// at a time; token by token 98 and 110; fp32, 16 requests of up to 2 047, 12 heads: 19 and 22).  But a block is then cut in four times as many
+// next to each other, memory is asked for neighbouring lines at once (64 requests of 4 096 tokens, 32 heads on 8, bf16: 96 us, 100 with a head
+// at a time; token by token 98 and 111; fp32, 16 requests of up to 2 047, 12 heads: 24 and 26).  But a block is then cut in four times as many
 // parts, all of which one CTA adds up: at 14 to 18 for each block the two are alike (one request of 40 000 tokens: 36 and 22).
 int heads_side_by_side(const ServingArgs& a, const Entry& e) {
     const int64_t blocks = (int64_t)a.B * a.Hk / WARPS, tiles = (int64_t)a.pool.width * a.pool.page / e.keys;

@@ -15,10 +15,11 @@
 //   fp32: x = h + l with h the upper 11 bits of the significand, which is what the tensor core reads of an fp32 word.  Q lies in tensor memory
 // with its l parts, four warps write those of each tile beside it; a product is l h' + h l' + h h', in this order: what is left out is 2^-22 of it.  P V of
 // a tile comes back into registers and is added there in fp32: the tensor core's additions cut off instead of rounding.
-//   What bounds it: with 16-bit types the softmax warps, whose exponentials (four fifths on the special function units, 64 % of what these can do)
-// take longer than the products (40 % of the tensor pipe): a tile of 256 rows by 128 keys takes 1.38 us, 0.85 the exponentials alone.  fp32:
-// the tensor pipe (49 %) and, with it, the port of shared memory; a tile of 128 by 64 takes 1.3 us.  Beginning and end of a block are 1.6 us (fp32 3.7), of
-// a CTA 6.  4 prompts of 4 096 tokens, 32 heads on 8, bf16: 335 us, 820 TFLOP/s.  How fast instructions come counts too: the loops are some 70 KB of code.
+//   What bounds it: with 16-bit types the softmax warps, whose exponentials (four fifths on the special function units, 62 % of what these can do)
+// take longer than the products (38 % of the tensor pipe): a tile of 256 rows by 128 keys takes 1.38 us, 0.85 the exponentials alone.  fp32:
+// the tensor pipe (43 %) and, with it, the port of shared memory; a tile of 128 by 64 takes 1.3 us.  Beginning and end of a block are 1.6 us (fp32 3.7), of
+// a CTA 6.  4 prompts of 4 096 tokens, 32 heads on 8, bf16: 363 us, 760 TFLOP/s, call after call with other inputs.
+// How fast instructions come counts too: the loops are some 70 KB of code.  With fp32 trees the softmax warps are 80 bytes a thread short of registers.
 #include <climits>
 #include <cmath>
 #include <mutex>

@@ -8,7 +8,7 @@ entry outside the pool stands for no page: nothing is written there, and attenti
 bfloat16 or float16, one for all of a call; arithmetic is fp32 (16-bit types: but for the weights that multiply values, which are rounded to
 the type).  Tables, lengths and starts are read by the kernels, so a captured call follows them.  A call runs on the tensors' device, on
 that device's current stream or the one given; results and workspaces that were not given are allocated for that stream.  All are for
-serving: there is no backward pass.
+serving: there is no backward pass, and tensors that require a gradient are taken as they are: the results are part of no graph.
 """
 from __future__ import annotations
 
@@ -70,7 +70,7 @@ def cache_append(K, V, K_pages, V_pages, pages, lengths, *, starts=None, picks=N
 
     With ``starts``, as of ``prompt_attention``: ``K``, ``V`` are [N, Hkv, 64], the tokens of packed prompts.  Otherwise they are [B, Hkv, T,
     64], and request b gets the rows ``picks[b, k]`` for ``k < counts[b]``: the drafts that were accepted, in their order (``picks``: [B, T]
-    of int32, None: 0, 1, ..; ``counts``: [B] of int32, None: T).  A pick outside [0, T) is left out, and so is a token that has no page.
+    of int32, None: 0, 1, ..; ``counts``: [B] of int32, None: T).  ``starts`` are taken into the tensor, as there.  A pick outside [0, T) is left out, and so is a token that has no page.
     Requests may not share the pages that are written."""
     r = _native().append(K, V, K_pages, V_pages, pages, lengths, starts, picks, counts, _handle(stream))
     if r != 0:
