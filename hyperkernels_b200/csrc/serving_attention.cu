@@ -142,14 +142,15 @@ int check_sizes(const hk_tree_params* p) {
 
 // Slots for what workers leave of blocks that fell to several, if any can: `tiles` are the most that a block meets.
 struct Parts {
-    int workers, slots, rows;  // slots: of a worker, in pairs
+    int workers, slots, rows;  // slots: of a worker
     bool any;
-    size_t all_rows() const { return (size_t)workers * 2 * slots * rows; }
+    size_t all_rows() const { return (size_t)workers * slots * rows; }
     size_t bytes() const { return any ? all_rows() * (64 * sizeof(float) + sizeof(float2)) + workers * sizeof(PartRecord) : 0; }
 };
 Parts parts_of(const hk_prompt_params* p) {
     const RowsPlan plan = rows_plan(p->dtype);
-    return {sm_count(), 1, plan.rows, (p->N + plan.keys - 1) / plan.keys >= 2 * plan.least};
+    const int64_t tiles = (p->N + plan.keys - 1) / plan.keys;
+    return {sm_count(), plan.slots(tiles), plan.rows, tiles >= 2 * plan.least};
 }
 bool few_rows(const hk_tree_params* p) { return p->T * (p->nh / p->nh_kv) <= 16; }
 Parts parts_of(const hk_tree_params* p) {
@@ -159,7 +160,8 @@ Parts parts_of(const hk_tree_params* p) {
         return {plan.workers, plan.slots, plan.rows, keys / plan.keys + cdiv(p->T, plan.keys) >= 2 * plan.least};
     }
     const RowsPlan plan = rows_plan(p->dtype);
-    return {sm_count(), 1, plan.rows, (keys + plan.keys - 1) / plan.keys + 1 >= 2 * plan.least};
+    const int64_t tiles = (keys + plan.keys - 1) / plan.keys + 1;
+    return {sm_count(), plan.slots(tiles), plan.rows, tiles >= 2 * plan.least};
 }
 int set_parts(ServingArgs& a, const Parts& parts, void* workspace, size_t bytes) {
     if (!parts.any) return HK_OK;

@@ -11,7 +11,7 @@ namespace hk {
 // How the work is cut.  The tiles of keys that the rows meet, block of rows by block, key head by key head, request by request, make one
 // line, of which every worker (a CTA, a warp) takes an equal stretch.  A block whose tiles fall to several workers leaves its parts
 // in slots of the workspace, two to a worker: what it has of a block that it has not begun itself, and of one that it has begun
-// and not ended.
+// and not ended.  What a worker has of a block in several pieces (16-bit types) is added up in a third, behind those of all workers.
 enum PartHead { PART_NONE, PART_LAST, PART_GOES_ON, PART_EMPTY /* nothing of any block */ };
 struct PartRecord {
     int head;                             // what the first slot holds: the last part of its block, one in between, or nothing
@@ -326,12 +326,14 @@ struct RowsPlan {
     int rows;   // of a block
     int keys;   // of a tile
     int least;  // tiles of a part of a block
+    int piece;  // tiles that are taken at once of a longer run, 0: all
+    int slots(int64_t tiles) const { return piece > 0 && tiles >= piece + least ? 3 : 2; }  // of a worker, for blocks of up to so many tiles
 };
 RowsPlan rows_plan(int dtype);
 struct TreeFewPlan {
     int rows;  // of a slot
     int keys, least;
-    int workers, slots;  // CTAs; slots of each, in pairs
+    int workers, slots;  // CTAs; slots of each
 };
 TreeFewPlan tree_few_plan(int dtype, int rows);
 int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream);

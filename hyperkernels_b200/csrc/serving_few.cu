@@ -370,7 +370,7 @@ int heads_side_by_side(const ServingArgs& a, const Entry& e) {
 
 TreeFewPlan tree_few_plan(int dtype, int rows) {
     const Entry e = pick(dtype, rows, 1);
-    return {std::min(rows, e.rows), e.keys, 2, sm_count() * e.per_sm, WARPS + 1};
+    return {std::min(rows, e.rows), e.keys, 2, sm_count() * e.per_sm, 2 * (WARPS + 1)};
 }
 
 namespace {

@@ -44,6 +44,9 @@ struct Rows {
     static constexpr int KV_BOX = KEYS * 128;    // 128 bytes of each row
     static constexpr int Q_BYTES = TILE * 64 * (int)sizeof(X), Q_BUFFERS = LOW ? 1 : 2;  // of a stream: K-major operands two items deep; fp32: on their way to tensor memory
     static constexpr int ITEMS = 8;
+    // Tiles that one sum of O in tensor memory has at most.  Its additions cut off, 8e-8 of the sum for every 16 keys (6.4e-3 for 2^20): with so many less than
+    // half a step of the type, 1.6e-4 of fp16 and 1.3e-3 of bf16.
+    static constexpr int PIECE = LOW ? 0 : std::is_same<X, __half>::value ? 256 : 2048;
 };
 
 // Half a tile is masked, and a block's beginning and end take as long as a tile (fp32: 3.7 us, nearly three; where both streams have the same rows a tile
@@ -59,7 +62,9 @@ struct __align__(16) Item {
     int n0, n1;          // tiles of each stream
     int slot;            // of the workspace, -1: the result
     int new_tile;        // number of the tile that is the new tokens'
+    int piece;           // of a longer run: GOES_ON with what the third slot has, NOT_LAST: what there is then comes there
 };
+enum { GOES_ON = 1, NOT_LAST = 2 };
 
 template <class X, bool TREE, bool SPLIT>
 struct __align__(16) RowsShared {
@@ -153,8 +158,41 @@ __device__ __forceinline__ void tma_load_queries(void* to, const CUtensorMap* ma
         : "memory");
 }
 
+// What the pieces of a run before this one came to (maximum and sum in `ml`, weighted values in `part`) added to O of a row in tensor memory; x: its maximum
+// and sum, before and after.  Not inlined: in place it costs the blocks that have no pieces another 1 to 3 %.
+__device__ __noinline__ float2 add_pieces(uint32_t at_o, const float* part, const float2* ml, bool valid, float2 x) {
+    float f_old = 0.f, f_new = 1.f;
+    if (valid) {
+        const float2 before = *ml;
+        const float mn = fmaxf(x.x, before.x), ref = mn == -INFINITY ? 0.f : mn;
+        f_new = x.y != 0.f ? ex2_approx(x.x - ref) : 0.f;
+        f_old = before.y != 0.f ? ex2_approx(before.x - ref) : 0.f;
+        x = make_float2(mn, x.y * f_new + before.y * f_old);
+    }
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 16) {
+        uint32_t y[16];
+        tmem_ld16(at_o + c, y);
+        tmem_wait_ld();
+        const float4* const old = reinterpret_cast<const float4*>(part + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 v = valid ? old[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+            y[4 * i] = __float_as_uint(fmaf(v.x, f_old, __uint_as_float(y[4 * i]) * f_new));
+            y[4 * i + 1] = __float_as_uint(fmaf(v.y, f_old, __uint_as_float(y[4 * i + 1]) * f_new));
+            y[4 * i + 2] = __float_as_uint(fmaf(v.z, f_old, __uint_as_float(y[4 * i + 2]) * f_new));
+            y[4 * i + 3] = __float_as_uint(fmaf(v.w, f_old, __uint_as_float(y[4 * i + 3]) * f_new));
+        }
+        tmem_st16(at_o + c, y);
+    }
+    tmem_wait_st();
+    return x;
+}
 // SPLIT: the rows of a block are a stream's at most, and both streams have them, every other tile each.
-template <class X, bool TREE, bool SPLIT>
+// LONG: 16-bit types, where a block can have more than PIECE tiles.  A run of more is taken in pieces of PIECE, items of their own, which are added up in fp32 with the
+// worker's third slot on their way out; each row by the thread that has it in all of them.  A kernel of its own, for where there can be such runs: what may have to be added up costs
+// the ends of all blocks 0.2 us (512 prompts of 128 tokens, 32 heads on 8, bf16: 178 us and 168).
+template <class X, bool TREE, bool SPLIT, bool LONG>
 __global__ void __launch_bounds__(Rows<X>::THREADS, 1)
 serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
                     const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ ServingArgs a) {
@@ -281,9 +319,17 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const bool valid = my_token < it.tokens && my_head < a.group - it.chunk * TILE && !(SPLIT && t && it.n1 == 0), live = __any_sync(0xffffffffu, valid);
             if (!LOW && n > 0 && !wait(sh.o_full[t], own - 1, W_O)) return;
             const int slot = it.slot;
+            // A piece of a longer run, each stream's for itself
+            const bool not_last = LONG && (it.piece & NOT_LAST);
+            const int64_t at_sum = (2 * gridDim.x + blockIdx.x) * (int64_t)C::BLOCK + t * TILE + in_stream;
+            if (LONG && (it.piece & GOES_ON)) {
+                const float2 x = add_pieces(lanes + COL_O + t * 64, a.part + at_sum * 64, a.ml + at_sum, valid, make_float2(m, l));
+                m = x.x;
+                l = x.y;
+            }
             // Both streams' rows: each warp adds half of the columns up.  O is in tensor memory for both to read, their maxima and sums go
             // through the place that rows of O leave by.
-            const bool both = SPLIT && it.n1 > 0;
+            const bool both = SPLIT && it.n1 > 0 && !not_last;
             float f0 = 1.f, f1 = 0.f;
             auto pair = [&](uint64_t (&bar)[2][4], int id) {
                 tc_fence_before_sync();
@@ -303,10 +349,11 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 l = l * f0 + other.y * f1;
                 m = mn;
             }
-            const float f = slot >= 0 ? 1.f : l != 0.f ? rcp_of<X>(l) : 0.f;
+            const bool kept = slot >= 0 || not_last;  // as a part
+            const float f = kept ? 1.f : l != 0.f ? rcp_of<X>(l) : 0.f;
             const int b = TREE ? it.b : 0, row = it.begin + it.token0 + (valid ? my_token : 0), h = it.kvh * a.group + it.chunk * TILE + my_head;
             X* const to = const_cast<X*>(row_of<X>(a.O, b, h, row));
-            const int64_t at_slot = (int64_t)slot * (SPLIT ? TILE : C::BLOCK) + r;
+            const int64_t at_slot = not_last ? at_sum : (int64_t)slot * (SPLIT ? TILE : C::BLOCK) + r;
             // Through shared memory, so that 8 lanes store 128 bytes of a row: a row to a lane is 32 lines an instruction.  fp32: in place of the
             // warp's rows of the queries that have just gone to tensor memory, 16 lanes to a row.
             if constexpr (LOW) {
@@ -363,7 +410,7 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     __syncwarp();
                 }
-            } else if (slot >= 0) {
+            } else if (kept) {
                 uint4* const whole = reinterpret_cast<uint4*>(a.part + at_slot * 64);
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
@@ -404,8 +451,8 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 __syncwarp();
             }
             if (!LOW) tc_fence_before_sync();
-            if (valid && !(SPLIT && t)) {
-                if (slot >= 0) a.ml[at_slot] = make_float2(m, l);
+            if (valid && (!(SPLIT && t) || not_last)) {
+                if (kept) a.ml[at_slot] = make_float2(m, l);
                 else a.LSE[b * a.lse_sB + h * a.lse_sH + row] = l != 0.f ? (m + log2_of<X>(l)) * LN2 : -INFINITY;
             }
             mbar_arrive_warp(&sh.item_empty[place_of_item], lane);
@@ -668,27 +715,50 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             bool ok = true;
             const bool v = warp != 0;
             PartRecord record{PART_EMPTY, 0, 0, 0, 0, 0};
-            // The next item into the ring; one without tokens at the end of the stretch
-            auto publish = [&](Item& it) {
-                Run run;
-                it.tokens = 0;
-                if (!line.next(work, run, sh.line.blocks)) return;
-                const int count = run.to - run.from;
-                it.b = run.b; it.kvh = run.kvh; it.chunk = run.chunk;
-                it.token0 = run.i * a.block_tokens;
-                it.tokens = min(a.block_tokens, run.r.tokens - it.token0);
-                it.begin = run.r.begin; it.len = run.r.len; it.key0 = run.from * KEYS;
-                it.new_tile = TREE ? run.n - 1 - run.from : -1;
+            Turn get{0, 0u}, at{0, 0u};  // of the items, of the ring
+            int left = 0;  // LONG: tiles of the run behind the piece before
+            // An item's tiles for each stream, of the next `count`
+            auto share_out = [&](Item& it, int count) {
+                if constexpr (LONG) {
+                    left = count;
+                    if (count >= C::PIECE + C::LEAST) {
+                        count = C::PIECE;
+                        it.piece |= NOT_LAST;
+                    }
+                    left -= count;
+                }
                 it.n0 = count;
                 it.n1 = 0;
                 if (!LOW && it.tokens > a.stream_tokens) {
                     it.n1 = count;
-                    if (!TREE && a.causal) it.n0 = max(0, min((it.token0 + a.stream_tokens + KEYS - 1) / KEYS - run.from, count));
+                    if (!TREE && a.causal) it.n0 = max(0, min((it.token0 + a.stream_tokens + KEYS - 1 - it.key0) / KEYS, count));
                 }
                 if (SPLIT) {
                     it.n0 = (count + 1) / 2;
                     it.n1 = count / 2;
                 }
+            };
+            // The next item into the ring; one without tokens at the end of the stretch
+            auto publish = [&](Item& it) {
+                if (LONG && left > 0) {  // the next piece of what the item before began
+                    __syncwarp();
+                    it = sh.items[get.at == 0 ? ITEMS - 1 : get.at - 1];
+                    it.key0 += C::PIECE * KEYS;
+                    it.new_tile -= C::PIECE;
+                    it.piece = GOES_ON;
+                    share_out(it, left);
+                    return;
+                }
+                Run run;
+                it.tokens = 0;
+                it.piece = 0;
+                if (!line.next(work, run, sh.line.blocks)) return;
+                it.b = run.b; it.kvh = run.kvh; it.chunk = run.chunk;
+                it.token0 = run.i * a.block_tokens;
+                it.tokens = min(a.block_tokens, run.r.tokens - it.token0);
+                it.begin = run.r.begin; it.len = run.r.len; it.key0 = run.from * KEYS;
+                it.new_tile = TREE ? run.n - 1 - run.from : -1;
+                share_out(it, run.to - run.from);
                 it.slot = run.slot(blockIdx.x);
                 if (run.from > 0) {
                     record.head = run.to < run.n ? PART_GOES_ON : PART_LAST;
@@ -700,7 +770,6 @@ serving_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                 }
             };
-            Turn get{0, 0u}, at{0, 0u};  // of the items, of the ring
             int made = 0;
             bool filled = false;         // each place of the ring once
             int ids_b = -1, ids_from = 0, ids = 0;  // entry ids_from + lane of request ids_b's row of the table
@@ -1018,14 +1087,14 @@ void cut(ServingArgs& a) {
     set_line(a, TREE, C::KEYS);
 }
 
-template <class X, bool TREE, bool SPLIT>
+template <class X, bool TREE, bool SPLIT, bool LONG>
 int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     typedef Rows<X> C;
     static std::once_flag once[HK_MAX_DEVICES];
     static cudaError_t rc[HK_MAX_DEVICES];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
-    std::call_once(once[dev], [dev] { rc[dev] = cudaFuncSetAttribute(serving_rows_kernel<X, TREE, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSpace<X>::SMEM); });
+    std::call_once(once[dev], [dev] { rc[dev] = cudaFuncSetAttribute(serving_rows_kernel<X, TREE, SPLIT, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSpace<X>::SMEM); });
     if (rc[dev] != cudaSuccess) return HK_ERR_CUDA;
     cut<X, TREE, SPLIT>(a);
     CUtensorMap k, v, kp, vp;
@@ -1047,7 +1116,7 @@ int launch(ServingArgs a, int dtype, cudaStream_t stream) {
     a.q_bytes = std::min(a.group, TILE) * a.stream_tokens * 64 * (int)sizeof(X);
     const int ctas = sm_count();
     LaunchConfig lc(ctas, C::THREADS, RowsSpace<X>::SMEM, stream, 1, true);
-    if (cudaLaunchKernelEx(&lc.cfg, serving_rows_kernel<X, TREE, SPLIT>, q, k, v, kp, vp, a) != cudaSuccess) return check_launch();
+    if (cudaLaunchKernelEx(&lc.cfg, serving_rows_kernel<X, TREE, SPLIT, LONG>, q, k, v, kp, vp, a) != cudaSuccess) return check_launch();
     count_launch();
     return a.parts ? launch_combine(a, dtype, ctas, stream) : HK_OK;
 }
@@ -1060,14 +1129,23 @@ template <bool TREE, bool SPLIT>
 LineSum line(const ServingArgs& a, int dtype, const int32_t* lens) {
     return dtype == HK_F32 ? line<float, TREE, false>(a, lens) : line<__half, TREE, SPLIT>(a, lens);
 }
+template <bool TREE, bool SPLIT, bool LONG>
+int launch_16(const ServingArgs& a, int dtype, cudaStream_t stream) {
+    return dtype == HK_BF16 ? launch<__nv_bfloat16, TREE, SPLIT, LONG>(a, dtype, stream) : launch<__half, TREE, SPLIT, LONG>(a, dtype, stream);
+}
 template <bool TREE, bool SPLIT>
 int launch(const ServingArgs& a, int dtype, cudaStream_t stream) {
-    return dtype == HK_F32 ? launch<float, TREE, false>(a, dtype, stream) : dtype == HK_BF16 ? launch<__nv_bfloat16, TREE, SPLIT>(a, dtype, stream) : launch<__half, TREE, SPLIT>(a, dtype, stream);
+    if (dtype == HK_F32) return launch<float, TREE, false, false>(a, dtype, stream);
+    const RowsPlan plan = rows_plan(dtype);
+    const int64_t tiles = TREE ? cdiv((int64_t)a.pool.width * a.pool.page, plan.keys) + 1 : cdiv(a.N, plan.keys);  // that a block can have
+    return plan.slots(tiles) > 2 ? launch_16<TREE, SPLIT, true>(a, dtype, stream) : launch_16<TREE, SPLIT, false>(a, dtype, stream);
 }
 
 }  // namespace
 
-RowsPlan rows_plan(int dtype) { return dtype == HK_F32 ? RowsPlan{Rows<float>::BLOCK, Rows<float>::KEYS, Rows<float>::LEAST} : RowsPlan{Rows<__half>::BLOCK, Rows<__half>::KEYS, Rows<__half>::LEAST}; }
+template <class C>
+static RowsPlan plan_of() { return {C::BLOCK, C::KEYS, C::LEAST, C::PIECE}; }
+RowsPlan rows_plan(int dtype) { return dtype == HK_F32 ? plan_of<Rows<float>>() : dtype == HK_BF16 ? plan_of<Rows<__nv_bfloat16>>() : plan_of<Rows<__half>>(); }
 int launch_prompt_rows(const ServingArgs& a, int dtype, cudaStream_t stream) { return launch<false, false>(a, dtype, stream); }
 // Up to 128 rows of a request under a key head: both streams have them, every other tile each (16 requests of up to 4 096 tokens, 16 new ones,
 // 32 heads on 8, bf16: 25 us, 29 where the second stream has nothing to do; 32 new ones of 12 heads 30 and 39).

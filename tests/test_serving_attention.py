@@ -56,6 +56,28 @@ def check(got, want, dtype, what=""):
         assert float((o.double() - O).norm()) <= 1e-5 * float(O.norm()), what
 
 
+PIECE = {"f16": 1 << 15, "bf16": 1 << 18}  # keys whose values are summed up at once
+
+
+def check_long(got, want, dtype, n, what=""):
+    """check(), for rows of n keys, whose sums are longer: n / 64 roundings (fp32) of u each in the sum of the weights and in O, which is added up tile by tile.
+    16-bit types sum O up in the tensor core, which cuts off less than the last place, 2 u, of the sum there is for every 16 keys, in pieces of PIECE keys (and up to a
+    tile), and the weights' sum rounds as above.  Pieces and parts that are added up round by 4 u each."""
+    (o, lse), (O, LSE, mean, size) = got, want
+    step = torch.finfo(TYPES[dtype]).eps / 2 if dtype != "f32" else 0.0
+    poly = 45 * U if dtype != "f32" else 0.0
+    d = (80 * size + 3 * (size - 40).clamp(min=0) + 70) * U
+    P = min(n, PIECE.get(dtype, n) + 128)
+    weights = (P / 64 + 4 * (n // P + 1) + 200) * U
+    values = weights if dtype == "f32" else weights + P / 16 * 2 * U
+    bound = (2 * d[..., None] + weights + values + 2 * poly + step) * mean + step * O.abs() + (2.0 ** -25 if dtype == "f16" else 1e-30)
+    off = (o.double() - O).abs()
+    assert bool((off <= bound).all()), (what, float((off / bound).max()), float(off.max()))
+    seen = LSE > -math.inf
+    assert torch.equal(lse > -math.inf, seen) and bool((o[~seen] == 0).all()), what
+    assert bool(((lse.double() - LSE).abs()[seen] <= (d + weights + poly + 4 * U * LSE.abs())[seen]).all()), what
+
+
 # ---- packed prompts -------------------------------------------------------------------------------------------------------------------
 def make_prompts(seed, lens, H, Hk, dtype, layout="packed", before=0, after=0, sigma=1.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -732,6 +754,97 @@ def test_offsets_past_32_bits(dtype):
         y.copy_(torch.randn(y.shape, generator=g, device="cuda"))
     x = (q, k, v, ints([0, 7, 200]))
     check_prompts(hk.prompt_attention(*x, SCALE), prompts(*x, True), dtype, slice(None))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,N,H,Hk,causal", [("bf16", 1 << 20, 2, 1, False), ("f16", (1 << 20) + 77, 1, 1, True), ("bf16", (1 << 20) - 9, 1, 1, True), ("f16", 1 << 17, 12, 4, True), ("f32", 1 << 18, 2, 2, False)])
+def test_very_long_prompts(dtype, N, H, Hk, causal):
+    """Values that do not cancel: a sum that is cut off at every step is too low by more with every key.  Some rows are compared."""
+    x = q, k, v, starts = make_prompts(1, [3, N - 8, 5], H, Hk, dtype)
+    v += 1
+    o, lse = hk.prompt_attention(*x, SCALE, causal)
+    rows = torch.tensor([3, 4, 130, 131, 16390, N // 3, N // 2 - 1, N // 2, N - 137, N - 7, N - 6], device="cuda")
+    check_long((o[rows].transpose(0, 1), lse[:, rows]), attend_rows(q[rows], k[3:N - 5], v[3:N - 5], rows - 3, causal), dtype, N)
+    for a, b in ((0, 3), (N - 5, N)):
+        check_prompts((o[a:b], lse[:, a:b]), prompts(q[a:b], k[a:b], v[a:b], ints([0, b - a]), causal), dtype, slice(None))
+    again = hk.prompt_attention(*x, SCALE, causal)
+    assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
+    assert hk.last_device_status() == 0
+
+
+def attend_rows(q, k, v, rows, causal):
+    """attend() for some rows [R, H, 64] of a prompt's k, v [n, Hk, 64]: the query heads of a key head as rows of one"""
+    (R, H, _), (n, Hk, _) = q.shape, k.shape
+    seen = ((torch.arange(n, device="cuda") <= rows[:, None]) | (not causal)).repeat(H // Hk, 1)
+    out = attend(q.transpose(0, 1).reshape(Hk, H // Hk * R, 64), k.transpose(0, 1), v.transpose(0, 1), seen, SCALE)
+    return tuple(t.reshape(H, R, *t.shape[2:]) for t in out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,H,Hk", [([(1, 0)], 4, 2), ([(1, 1), (0, 40)], 3, 3), ([(1, 128), (0, 0), (0, 1)], 6, 2), ([(1, 129)], 1, 1), ([(1, 256), (0, 70)], 2, 1), ([(2, 300), (1, 257), (0, 7)], 10, 1),
+                                       ([(1, 400)], 130, 1), ([(0, 50), (1, 600), (0, 300), (0, 128)], 24, 24)], ids=lambda x: "-".join(f"{a}p{b}" for a, b in x) if isinstance(x, list) else None)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts_in_pieces(lens, H, Hk, dtype, causal):
+    """Around the length where a block's keys are taken in several pieces, in calls that deal blocks out whole and that cut them; the last rows of each prompt, and some in between."""
+    P = PIECE[dtype]
+    lens = [a * P + b for a, b in lens]
+    x = q, k, v, starts = make_prompts(len(lens), lens, H, Hk, dtype, before=3, after=2)
+    v += 1
+    out, lse = torch.full(q.shape, 7.0, device="cuda", dtype=TYPES[dtype]), torch.full((H, q.shape[0]), 7.0, device="cuda")
+    hk.prompt_attention(*x, SCALE, causal, out=out, lse=lse)
+    edges = starts.tolist()
+    for a, b in zip(edges, edges[1:]):
+        n = b - a
+        rows = {0, 1, 128, n // 2, *(P + i for i in (-1, 0, 1, 127, 128, 129, 255, 256)), 2 * P, 2 * P + 255, *(n - i for i in (300, 257, 256, 129, 128, 65, 2, 1))}
+        rows = torch.tensor(sorted(i for i in rows if 0 <= i < n), device="cuda", dtype=torch.long)
+        if n:
+            check_long((out[a + rows].transpose(0, 1), lse[:, a + rows]), attend_rows(q[a + rows], k[a:b], v[a:b], rows, causal), dtype, n, (a, b))
+    assert bool((out[:3] == 7.0).all()) and bool((out[-2:] == 7.0).all())
+    assert not bool((lse[:, 3:-2] == 7.0).any())
+    again = hk.prompt_attention(*x, SCALE, causal)
+    assert torch.equal(out[3:-2], again[0][3:-2]) and torch.equal(lse[:, 3:-2], again[1][:, 3:-2])
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,H", [(1, 1), (2, 2), (30, 1), (64, 3)])
+def test_very_long_caches(dtype, T, H):
+    x = make_tree(T, [1000001, 3, 0, 250000], T, H, 1, 64, dtype)
+    x[2].add_(1), x[4].add_(1)
+    got, want = hk.tree_attention(*x), trees(*x)
+    for b, n in enumerate(x[6].tolist()):
+        check_long(tuple(t[b] for t in got), tuple(t[b] for t in want), dtype, n + T, b)
+    assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,H", [(17, 1), (40, 2), (64, 4), (5, 130)])
+@pytest.mark.parametrize("tree", ["random", None])
+def test_trees_in_pieces(dtype, T, H, tree):
+    """So many requests that a block is hardly cut, over pages that they share, with caches around the length where a block's keys are taken in several pieces."""
+    rng, P, B, page = random.Random(T), PIECE[dtype], 150, 256
+    lens = [P + rng.choice([-1, 0, 1, 127, 128, 129, 256, 300, 1000, P + 5]) if b % 5 else rng.choice([0, 1, 300]) for b in range(B)]
+    x = list(make_tree(T, [2 * P + 2 * page], T, H, 1, page, dtype, "phd" if T == 40 else "hpd", spare=0))
+    pages = x[5][0, :-1]
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x[0], x[1], x[2] = (torch.randn((B, n, T, 64), generator=g, device="cuda").to(TYPES[dtype]) for n in (H, 1, 1))
+    x[5] = torch.stack([pages.roll(b) for b in range(B)]).contiguous()
+    x[6] = ints(lens)
+    if tree:
+        x[8] = torch.tensor([[rng.getrandbits(i) | 1 << i if i < 63 else -1 for i in range(T)] for _ in range(B)], device="cuda")
+    else:
+        x[8] = None
+    x[2].add_(1), x[4].add_(1)
+    got = hk.tree_attention(*x)
+    for b in list(range(0, B, 11)) + [B - 2, B - 1]:
+        one = trees(*(t[b:b + 1] if i in (0, 1, 2, 5, 6, 8) and t is not None else t for i, t in enumerate(x)))
+        check_long(tuple(t[b:b + 1] for t in got), one, dtype, lens[b] + T, b)
+    again = hk.tree_attention(*x)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    assert hk.last_device_status() == 0
 
 
 # ---- a run of them together --------------------------------------------------------------------------------------------------------------
