@@ -144,30 +144,32 @@ int check_sizes(const hk_tree_params* p) {
 struct Parts {
     int workers, slots, rows;  // slots: of a worker
     bool any;
+    int sums;                  // of a worker, rows of 64 floats
     size_t all_rows() const { return (size_t)workers * slots * rows; }
-    size_t bytes() const { return any ? all_rows() * (64 * sizeof(float) + sizeof(float2)) + workers * sizeof(PartRecord) : 0; }
+    size_t bytes() const { return any ? all_rows() * (64 * sizeof(float) + sizeof(float2)) + (size_t)workers * (sums * 64 * sizeof(float) + sizeof(PartRecord)) : 0; }
 };
 Parts parts_of(const hk_prompt_params* p) {
     const RowsPlan plan = rows_plan(p->dtype);
     const int64_t tiles = (p->N + plan.keys - 1) / plan.keys;
-    return {sm_count(), plan.slots(tiles), plan.rows, tiles >= 2 * plan.least};
+    return {sm_count(), plan.slots(tiles), plan.rows, tiles >= 2 * plan.least, 0};
 }
 bool few_rows(const hk_tree_params* p) { return p->T * (p->nh / p->nh_kv) <= 16; }
 Parts parts_of(const hk_tree_params* p) {
     const int64_t keys = (int64_t)p->pool.width * p->pool.page;
     if (few_rows(p)) {
-        const TreeFewPlan plan = tree_few_plan(p->dtype, (int)(p->T * (p->nh / p->nh_kv)));
-        return {plan.workers, plan.slots, plan.rows, keys / plan.keys + cdiv(p->T, plan.keys) >= 2 * plan.least};
+        const TreeFewPlan plan = tree_few_plan(p->dtype, (int)(p->T * (p->nh / p->nh_kv)), keys);
+        return {plan.workers, plan.slots, plan.rows, keys / plan.keys + cdiv(p->T, plan.keys) >= 2 * plan.least, plan.sums};
     }
     const RowsPlan plan = rows_plan(p->dtype);
     const int64_t tiles = (keys + plan.keys - 1) / plan.keys + 1;
-    return {sm_count(), plan.slots(tiles), plan.rows, tiles >= 2 * plan.least};
+    return {sm_count(), plan.slots(tiles), plan.rows, tiles >= 2 * plan.least, 0};
 }
 int set_parts(ServingArgs& a, const Parts& parts, void* workspace, size_t bytes) {
     if (!parts.any) return HK_OK;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || bytes < parts.bytes()) return HK_ERR_WORKSPACE;
     const size_t rows = parts.all_rows();
-    a.part = static_cast<float*>(workspace);
+    a.sums = parts.sums > 0 ? static_cast<float4*>(workspace) : nullptr;
+    a.part = static_cast<float*>(workspace) + (size_t)parts.workers * parts.sums * 64;
     a.ml = reinterpret_cast<float2*>(a.part + rows * 64);
     a.parts = reinterpret_cast<PartRecord*>(a.ml + rows);
     return HK_OK;

@@ -46,6 +46,7 @@ struct ServingArgs {
     float2* ml;         // [slots][slot_rows]
     float* part;        // the same, [64]
     PartRecord* parts;
+    float4* sums;       // few rows: of what a warp has of a block in several pieces, [16][64] of each
     DeviceStatus* status;
 };
 
@@ -334,8 +335,9 @@ struct TreeFewPlan {
     int rows;  // of a slot
     int keys, least;
     int workers, slots;  // CTAs; slots of each
+    int sums;  // rows of 64 floats of each for sums of blocks' pieces, 0: no block can have several
 };
-TreeFewPlan tree_few_plan(int dtype, int rows);
+TreeFewPlan tree_few_plan(int dtype, int rows, int64_t keys);  // keys: that a request can have
 int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream);
 int launch_prompt_rows(const ServingArgs& a, int dtype, cudaStream_t stream);
 int launch_tree_rows(const ServingArgs& a, int dtype, cudaStream_t stream);

@@ -4,7 +4,9 @@
 // ring of its own in batches of 8 (fp32) or 16 keys, two or three ahead, over the borders of requests.  A batch lies in one page.  Lengths
 // and tables are read where the batches are asked for, 32 entries of a table at a time, so no product waits for them.  What a block of rows has in
 // several warps goes to slots; a CTA adds up what its own warps left, and what is left of blocks that fell to several CTAs a second kernel.
-// Where key heads come in fours the warps take one each instead, over the whole stretch of the CTA (heads_side_by_side).
+// The products of 16-bit types are summed up in the instructions' accumulators, whose additions cut off: with every piece of Pieces batches of a block the sum so far goes to the
+// warp's place in the workspace, where the next is added to it in fp32, and back at the block's end.
+//   Where key heads come in fours the warps take one each instead, over the whole stretch of the CTA (heads_side_by_side).
 //   What bounds it is memory: 64 requests of 4 096 tokens, 32 heads on 8, bf16, 96 us or 5.6 TB/s, of which some 9 are the launch, the search for
 // the stretches, the first loads and the sum of the parts.  More than two rows of fp32 are bound by arithmetic: 16 requests of up to 2 047 tokens,
 // 12 heads, 1 / 2 / 4 (lane by lane) / 8 / 16 rows (three TF32 products of mma.sync): 24 / 26 / 32 / 34 / 36 us with the keys in memory, 18 / 22 / 31 / 33 / 35 with
@@ -30,6 +32,13 @@ using FewWork = Work<KEYS, 2, 4, 3 * KEYS, true>;
 template <class Rows>
 struct Shape {
     static constexpr int CTAS = Rows::ROWS == 16 ? (sizeof(typename Rows::X) == 4 ? 2 : 3) : Rows::ROWS > 2 ? 3 : 4, STAGES = 12 / CTAS;
+};
+
+// Batches of 16 keys that one sum of weighted values has at most: a cut-off of 8e-8 of it for each comes to less than half a step of the type, 1.6e-4 of fp16 and 1.3e-3
+// of bf16.  fp32 adds every batch up by itself, rounded.
+template <class X>
+struct Pieces {
+    static constexpr int BATCHES = std::is_same<X, __half>::value ? 2048 : std::is_same<X, __nv_bfloat16>::value ? 16384 : 0;
 };
 
 struct Segment {  // a run as the products need it
@@ -72,6 +81,30 @@ __device__ __forceinline__ void store_rows(const RowsOfOne<N>& w, int lane, int 
         auto* const to = place(i);
         const float f = f_of[i];
         store4(to + 4 * lane, make_float4(w.o[i].x * f, w.o[i].y * f, w.o[i].z * f, w.o[i].w * f));
+    }
+}
+// A warp's sums of weighted values that were cut into pieces, in `sum`, and the maxima that they were taken by: with those of the piece that is over,
+// which begins anew, or (back) all of them to where they were.
+template <class T>
+__device__ __forceinline__ void sum_pieces(RowsOf16<T>& w, float4* sum, float (&m_sum)[2], int lane, bool first, bool back) {
+    float f[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        f[i] = first ? 0.f : ex2_approx(m_sum[i] - (w.m[i] == -INFINITY ? 0.f : w.m[i]));
+        m_sum[i] = w.m[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float4 x = make_float4(w.o[j][0], w.o[j][1], w.o[j][2], w.o[j][3]);
+        if (!first) {
+            const float4 y = sum[j * 32 + lane];
+            x = make_float4(fmaf(y.x, f[0], x.x), fmaf(y.y, f[0], x.y), fmaf(y.z, f[1], x.z), fmaf(y.w, f[1], x.w));
+        }
+        if (!back) {
+            sum[j * 32 + lane] = x;
+            x = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        w.o[j][0] = x.x; w.o[j][1] = x.y; w.o[j][2] = x.z; w.o[j][3] = x.w;
     }
 }
 // Sums of the lanes that share a row; then every lane of a row has its maximum and sum.
@@ -188,8 +221,9 @@ __device__ __forceinline__ void join_warps(const ServingArgs& a, const PartRecor
 }
 
 // SIDE key heads side by side: 1, the warps have a stretch each, or 4, a head each of the CTA's stretch (a.Hk and a.group are then of four
-// heads taken for one).
-template <class Rows, int SIDE>
+// heads taken for one).  LONG: 16-bit types, where a block can have more batches than a piece; a kernel of its own, for
+// it takes 1 % longer (64 requests of 4 096 tokens, 32 heads on 8, fp16: 98.0 us and 97.2; 16 of up to 2 047, 12 heads: 18.2 and 17.9).
+template <class Rows, int SIDE, bool LONG>
 __global__ void __launch_bounds__(WARPS * 32, Shape<Rows>::CTAS)
 tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_kp,
                 const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ ServingArgs a) {
@@ -272,6 +306,9 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     Rows w;
     uint64_t bits[MINE];
     int token_of[MINE], head_of[MINE];
+    float m_sum[2] = {0.f, 0.f};
+    float4* const sum = LONG ? a.sums + (blockIdx.x * WARPS + warp) * 256 : nullptr;
+    constexpr int PIECE = LONG ? Pieces<X>::BATCHES : 1;
     for (int i = 1 - STAGES;; ++i) {
         copy_next();
         if (i < 0) continue;
@@ -304,7 +341,12 @@ tree_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     [] {});
         }
         if (++get_slot == STAGES) get_slot = 0, phase ^= 1u;
-        if (++j == get.to) {
+        ++j;
+        if constexpr (LONG) {
+            const int done = j - get.from;
+            if (j == get.to ? done > PIECE : done % PIECE == 0) sum_pieces(w, sum, m_sum, lane, done == PIECE, j == get.to);
+        }
+        if (j == get.to) {
             join(w);
             float f[MINE];
 #pragma unroll
@@ -343,18 +385,22 @@ struct Entry {
     size_t smem;
     int per_sm, keys, rows;
 };
-template <class Rows, int SIDE = 1>
+template <class Rows, int SIDE = 1, bool LONG = false>
 Entry entry() {
-    return {tree_few_kernel<Rows, SIDE>, sizeof(FewShared<Rows, SIDE>), Shape<Rows>::CTAS, Rows::KEYS, Rows::ROWS};
+    return {tree_few_kernel<Rows, SIDE, LONG>, sizeof(FewShared<Rows, SIDE>), Shape<Rows>::CTAS, Rows::KEYS, Rows::ROWS};
 }
-Entry pick(int dtype, int rows, int side) {
+template <class X, int SIDE>
+Entry entry_16(bool pieces) {
+    return pieces ? entry<RowsOf16<X>, SIDE, true>() : entry<RowsOf16<X>, SIDE>();
+}
+Entry pick(int dtype, int rows, int side, bool pieces = false) {
     if (side > 1) {
-        if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>, WARPS>();
-        if (dtype == HK_F16) return entry<RowsOf16<__half>, WARPS>();
+        if (dtype == HK_BF16) return entry_16<__nv_bfloat16, WARPS>(pieces);
+        if (dtype == HK_F16) return entry_16<__half, WARPS>(pieces);
         return rows == 1 ? entry<RowsOfOne<1>, WARPS>() : rows == 2 ? entry<RowsOfOne<2>, WARPS>() : rows <= 4 ? entry<RowsOfOne<4>, WARPS>() : entry<RowsOf16<float>, WARPS>();
     }
-    if (dtype == HK_BF16) return entry<RowsOf16<__nv_bfloat16>>();
-    if (dtype == HK_F16) return entry<RowsOf16<__half>>();
+    if (dtype == HK_BF16) return entry_16<__nv_bfloat16, 1>(pieces);
+    if (dtype == HK_F16) return entry_16<__half, 1>(pieces);
     return rows == 1 ? entry<RowsOfOne<1>>() : rows == 2 ? entry<RowsOfOne<2>>() : rows <= 4 ? entry<RowsOfOne<4>>() : entry<RowsOf16<float>>();
 }
 // Key heads that a CTA takes side by side.  Four: its warps have nothing to add up, and where pools are stored token by token, with the heads
@@ -368,9 +414,10 @@ int heads_side_by_side(const ServingArgs& a, const Entry& e) {
 
 }  // namespace
 
-TreeFewPlan tree_few_plan(int dtype, int rows) {
+TreeFewPlan tree_few_plan(int dtype, int rows, int64_t keys) {
     const Entry e = pick(dtype, rows, 1);
-    return {std::min(rows, e.rows), e.keys, 2, sm_count() * e.per_sm, 2 * (WARPS + 1)};
+    const int piece = dtype == HK_F32 ? 0 : dtype == HK_BF16 ? Pieces<__nv_bfloat16>::BATCHES : Pieces<__half>::BATCHES;
+    return {std::min(rows, e.rows), e.keys, 2, sm_count() * e.per_sm, 2 * (WARPS + 1), piece > 0 && keys / e.keys + cdiv(16, e.keys) > piece ? WARPS * 16 : 0};
 }
 
 namespace {
@@ -378,7 +425,7 @@ namespace {
 Entry cut(ServingArgs& a, int dtype, int& side) {
     a.rows = a.T * a.group;
     side = heads_side_by_side(a, pick(dtype, a.rows, 1));
-    const Entry e = pick(dtype, a.rows, side);
+    const Entry e = pick(dtype, a.rows, side, a.sums != nullptr);
     a.block_tokens = std::min(a.rows, e.rows) * side;
     a.chunks = 1;
     divide_by(a.group, a.group_mul, a.group_shift);
@@ -404,7 +451,7 @@ int launch_tree_few(ServingArgs a, int dtype, cudaStream_t stream) {
     const Entry e = cut(a, dtype, side);
     // once per device and kernel: more than 48 KB of shared memory
     static std::mutex mu;
-    static Kernel known[HK_MAX_DEVICES][16];
+    static Kernel known[HK_MAX_DEVICES][32];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= HK_MAX_DEVICES) return HK_ERR_CUDA;
     {

@@ -819,32 +819,55 @@ def test_very_long_caches(dtype, T, H):
     assert hk.last_device_status() == 0
 
 
-@pytest.mark.gpu
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
-@pytest.mark.parametrize("T,H", [(17, 1), (40, 2), (64, 4), (5, 130)])
-@pytest.mark.parametrize("tree", ["random", None])
-def test_trees_in_pieces(dtype, T, H, tree):
-    """So many requests that a block is hardly cut, over pages that they share, with caches around the length where a block's keys are taken in several pieces."""
-    rng, P, B, page = random.Random(T), PIECE[dtype], 150, 256
-    lens = [P + rng.choice([-1, 0, 1, 127, 128, 129, 256, 300, 1000, P + 5]) if b % 5 else rng.choice([0, 1, 300]) for b in range(B)]
-    x = list(make_tree(T, [2 * P + 2 * page], T, H, 1, page, dtype, "phd" if T == 40 else "hpd", spare=0))
+def shared_pages(seed, lens, T, H, Hk, dtype, layout, tree):
+    """Requests over the same pages, each in an order of its own; values that do not cancel"""
+    B, page = len(lens), 256
+    x = list(make_tree(seed, [cdiv(max(lens), page) * page], T, H, Hk, page, dtype, layout, spare=0))
     pages = x[5][0, :-1]
-    g = torch.Generator(device="cuda").manual_seed(T)
-    x[0], x[1], x[2] = (torch.randn((B, n, T, 64), generator=g, device="cuda").to(TYPES[dtype]) for n in (H, 1, 1))
+    g, rng = torch.Generator(device="cuda").manual_seed(seed), random.Random(seed)
+    x[0], x[1], x[2] = (torch.randn((B, n, T, 64), generator=g, device="cuda").to(TYPES[dtype]) for n in (H, Hk, Hk))
     x[5] = torch.stack([pages.roll(b) for b in range(B)]).contiguous()
     x[6] = ints(lens)
-    if tree:
-        x[8] = torch.tensor([[rng.getrandbits(i) | 1 << i if i < 63 else -1 for i in range(T)] for _ in range(B)], device="cuda")
-    else:
-        x[8] = None
+    x[8] = torch.tensor([[rng.getrandbits(i) | 1 << i if i < 63 else -1 for i in range(T)] for _ in range(B)], device="cuda") if tree else None
     x[2].add_(1), x[4].add_(1)
+    return x
+
+
+def check_shared_pages(x, lens, T, dtype, every):
     got = hk.tree_attention(*x)
-    for b in list(range(0, B, 11)) + [B - 2, B - 1]:
+    for b in [*range(0, len(lens), every), len(lens) - 2, len(lens) - 1]:
         one = trees(*(t[b:b + 1] if i in (0, 1, 2, 5, 6, 8) and t is not None else t for i, t in enumerate(x)))
         check_long(tuple(t[b:b + 1] for t in got), one, dtype, lens[b] + T, b)
     again = hk.tree_attention(*x)
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
     assert hk.last_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,H", [(17, 1), (40, 2), (64, 4), (5, 130)])
+@pytest.mark.parametrize("tree", ["random", None])
+def test_trees_in_pieces(dtype, T, H, tree):
+    """So many requests that a block is hardly cut, with caches around the length where a block's keys are taken in several pieces."""
+    rng, P = random.Random(T), PIECE[dtype]
+    lens = [P + rng.choice([-1, 0, 1, 127, 128, 129, 256, 300, 1000, P + 5]) if b % 5 else rng.choice([0, 1, 300]) for b in range(150)]
+    check_shared_pages(shared_pages(T, lens, T, H, 1, dtype, "phd" if T == 40 else "hpd", tree), lens, T, dtype, 11)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,H,Hk,B", [(1, 7, 7, 260), (1, 8, 8, 230), (4, 16, 4, 460), (16, 2, 2, 900)])
+def test_few_rows_in_pieces(dtype, T, H, Hk, B):
+    """The same, for as many requests as there are warps (key heads side by side: CTAs)."""
+    rng, P = random.Random(T), PIECE[dtype]
+    lens = [P + rng.choice([-16, -1, 0, 1, 15, 16, 17, 32, 1000, P + 5]) if b % 7 else rng.choice([0, 1, 300]) for b in range(B)]
+    check_shared_pages(shared_pages(T, lens, T, H, Hk, dtype, "phd" if T == 1 else "hpd", "random" if T == 4 else None), lens, T, dtype, 43)
+
+
+@pytest.mark.gpu
+def test_many_requests_with_a_very_long_cache():
+    lens = [1 << 20] * 600 + [5]
+    check_shared_pages(shared_pages(3, lens, 1, 4, 4, "f16", "hpd", None), lens, 1, "f16", 150)
 
 
 # ---- a run of them together --------------------------------------------------------------------------------------------------------------
